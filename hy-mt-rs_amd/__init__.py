@@ -119,6 +119,17 @@ SIGNATURES = {
     "hyq_gguf_read_f32": (I, [P, P, ctypes.c_char_p, P, SZ]),
     "hyq_sha256": (I, [P, SZ, P]),
     "hyq_dense_from_gguf": (I, [P, P, SZ, ctypes.POINTER(P)]),
+    "hyq_kv_pool_bytes": (SZ, [P]),
+    "hyq_paged_rope_norm_append_d": (I, [P, P, P, I, P, P, P, SZ, SZ, P, P, P, P, P, P,
+                                         ctypes.c_float, I, P]),
+    "hyq_paged_attention_scratch_bytes": (SZ, [P, SZ, SZ, SZ]),
+    "hyq_paged_attention_d": (I, [P, P, P, I, P, P, P, SZ, SZ, SZ, P, P, SZ, P]),
+    "hyq_pages_fork_d": (I, [P, P, P, P, P, P, P, P, P]),
+    "hyq_pages_scratch_bytes": (SZ, [P]),
+    "hyq_pages_extend_d": (I, [P, P, P, P, P, P, P, P, P, P, P, P, SZ]),
+    "hyq_pages_compact_d": (I, [P, P, P, P, P, P, P, P, P, SZ]),
+    "hyq_sample_scratch_bytes": (SZ, [SZ, SZ]),
+    "hyq_sample_d": (I, [P, P, SZ, SZ, P, P, P, P, P, P, SZ, P, P]),
 }
 
 PROFILE_AUTO, PROFILE_STANDARD, PROFILE_TENCENT_Q2_0C, PROFILE_TENCENT_STQ1 = 0, 1, 2, 3
@@ -138,6 +149,13 @@ class DenseConfig(ctypes.Structure):
     _fields_ = [("layers", I), ("hidden", I), ("heads", I), ("kv_heads", I),
                 ("head_dim", I), ("ffn", I), ("vocab", I), ("rope_base", ctypes.c_float),
                 ("rms_eps", ctypes.c_float)]
+
+
+class KvLayout(ctypes.Structure):
+    """hyq_kv_layout: a paged KV cache's pool [layers][pages][2][kv_heads]
+    [page_tokens][head_dim] and page table [seqs][stride]."""
+    _fields_ = [("dtype", I), ("layers", I), ("kv_heads", I), ("head_dim", I),
+                ("page_tokens", I), ("pages", I), ("seqs", I), ("stride", I)]
 
 _lib = None
 
@@ -679,6 +697,114 @@ class DenseDecoder:
         out = np.empty(steps, np.int32)
         check(lib().hyq_dense_generate(self.handle, token, steps, int(use_graph), _ptr(out)))
         return out
+
+
+class PagedCache:
+    """A paged KV cache of many sequence slots and its device state: the pool,
+    the page table, the slots' lengths and the pages' reference counts
+    (include/hyq.h, hyq_kv_layout). A new cache holds no tokens and no pages.
+
+    A serving step: ``fork`` (beams, ended requests), ``extend`` (room for the
+    new tokens), then for every layer ``append_d`` and ``attention_d`` of the
+    packed rows. The calls are asynchronous on the context's stream; those that
+    return numpy arrays wait."""
+
+    def __init__(self, ctx: Context, layers: int, kv_heads: int, pages: int, seqs: int,
+                 context: int, page_tokens: int = 64, dtype: int = F16, head_dim: int = 128):
+        self.ctx = ctx
+        self.layout = KvLayout(dtype, layers, kv_heads, head_dim, page_tokens, pages, seqs,
+                               -(-context // page_tokens) if page_tokens > 0 else 0)
+        self._kl = ctypes.byref(self.layout)
+        size = lib().hyq_kv_pool_bytes(self._kl)
+        if not size:
+            raise ValueError("invalid paged cache layout")
+        self.pool = ctx.empty(size, np.uint8)
+        self.table = ctx.array(np.full((seqs, self.layout.stride), -1, np.int32))
+        self.len = ctx.array(np.zeros(seqs, np.int32))
+        self.refs = ctx.array(np.zeros(pages, np.int32))
+        self._other = (ctx.empty((seqs, self.layout.stride), np.int32),
+                       ctx.empty(seqs, np.int32))
+        self._ints = [ctx.empty(seqs, np.int32) for _ in range(3)]
+        self._live = ctx.empty(1, np.int32)
+        self._scratch = ctx.empty(lib().hyq_pages_scratch_bytes(self._kl), np.uint8)
+        self._attention = None
+
+    def _slots(self, values, into: DeviceArray) -> int:
+        a = np.ascontiguousarray(values, np.int32)
+        if a.shape != (self.layout.seqs,):
+            raise ValueError("one value per slot")
+        into.copy_from(a)
+        return into.ptr
+
+    def fork(self, parent, keep=None) -> None:
+        """hyq_pages_fork_d: slot s becomes (the first keep[s] positions of)
+        slot parent[s]; -1 frees it."""
+        table, length = self._other
+        check(lib().hyq_pages_fork_d(
+            self.ctx.handle, self._kl, self._slots(parent, self._ints[0]),
+            None if keep is None else self._slots(keep, self._ints[1]), self.table.ptr,
+            self.len.ptr, table.ptr, length.ptr, self.refs.ptr))
+        self._other = (self.table, self.len)
+        self.table, self.len = table, length
+
+    def extend(self, add) -> np.ndarray:
+        """hyq_pages_extend_d: room for add[s] more tokens; the slots' status
+        (0 done, 1 no pages left, 2 too long for the slot)."""
+        check(lib().hyq_pages_extend_d(
+            self.ctx.handle, self._kl, self.pool.ptr, self._slots(add, self._ints[0]),
+            self.table.ptr, self.len.ptr, self.refs.ptr, self.table.ptr, self.len.ptr,
+            self.refs.ptr, self._ints[2].ptr, self._scratch.ptr, self._scratch.nbytes))
+        return self._ints[2].numpy()
+
+    def compact(self) -> int:
+        """hyq_pages_compact_d: the pages in use become 0 .. live-1; live."""
+        check(lib().hyq_pages_compact_d(
+            self.ctx.handle, self._kl, self.pool.ptr, self.table.ptr, self.refs.ptr,
+            self.table.ptr, self.refs.ptr, self._live.ptr, self._scratch.ptr,
+            self._scratch.nbytes))
+        return int(self._live.numpy()[0])
+
+    def lengths(self) -> np.ndarray:
+        return self.len.numpy()
+
+    def append_d(self, layer: int, start_d: int, rows: int, heads: int, q_d: int, k_d: int,
+                 v_d: int, q_norm_d: int, k_norm_d: int, freq_d: int, eps: float, q_out_d: int,
+                 norm_first: bool = False) -> None:
+        """hyq_paged_rope_norm_append_d on device buffers."""
+        check(lib().hyq_paged_rope_norm_append_d(
+            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr, self.len.ptr,
+            start_d, rows, heads, q_d, k_d, v_d, q_norm_d, k_norm_d, freq_d, eps,
+            int(norm_first), q_out_d))
+
+    def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,
+                    q_d: int, out_d: int) -> None:
+        """hyq_paged_attention_d on device buffers, with a scratch that grows
+        with the largest call."""
+        need = lib().hyq_paged_attention_scratch_bytes(self._kl, rows, max_rows, heads)
+        if self._attention is None or self._attention.nbytes < need:
+            self.ctx.sync()  # calls before this one may still use the old scratch
+            self._attention = self.ctx.empty(max(need, 16), np.uint8)
+        check(lib().hyq_paged_attention_d(
+            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr, self.len.ptr,
+            start_d, rows, max_rows, heads, q_d, self._attention.ptr, self._attention.nbytes,
+            out_d))
+
+
+def sample(ctx: "Context", logits: np.ndarray, random, temperature=1.0, top_k=0, top_p=1.0,
+           min_p=0.0):
+    """hyq_sample_d of logits [rows][vocab]; settings are values for all rows
+    or arrays of one per row. Returns (tokens int32, probabilities f32)."""
+    logits = np.ascontiguousarray(logits, np.float32)
+    rows, vocab = logits.shape
+    each = lambda v, t: ctx.array(np.ascontiguousarray(np.broadcast_to(np.asarray(v, t), (rows,))))
+    ld, td, kd = ctx.array(logits), each(temperature, np.float32), each(top_k, np.int32)
+    pd, md, ud = each(top_p, np.float32), each(min_p, np.float32), each(random, np.float32)
+    need = lib().hyq_sample_scratch_bytes(rows, vocab)
+    scratch = ctx.empty(max(need, 16), np.uint8)
+    token, prob = ctx.empty(rows, np.int32), ctx.empty(rows, np.float32)
+    check(lib().hyq_sample_d(ctx.handle, ld.ptr, rows, vocab, td.ptr, kd.ptr, pd.ptr, md.ptr,
+                             ud.ptr, scratch.ptr, need, token.ptr, prob.ptr))
+    return token.numpy(), prob.numpy()
 
 
 class Gguf:

@@ -1,0 +1,394 @@
+// Bookkeeping of a paged KV cache on the device: forking, trimming and freeing
+// slots, giving slots the pages of their next tokens, and moving the live
+// pages to the front of the pool. Tables, lengths and counts stay in device
+// memory and every result is exact and independent of the order in which
+// threads run (integer counts; the lowest free page first; slots in order),
+// so a whole serving step can be enqueued, or captured in a graph, without
+// the host.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "hyq_paged.hpp"
+
+namespace hyq {
+
+namespace {
+
+__device__ __forceinline__ int held_pages(int len, int shift, int stride)
+{
+    return min((int)(((long long)max(len, 0) + (1 << shift) - 1) >> shift), stride);
+}
+
+// ---- fork ----
+// table_out[s] = the entries that hold the first min(len[p], keep[s])
+// positions of slot p = parent[s] (none for a p outside the table).
+// Grid: one workgroup per slot, then workgroups that clear the counts.
+__global__ __launch_bounds__(256) void pages_fork_kernel(PagesArgs a, const int *__restrict__ parent,
+                                                         const int *__restrict__ keep,
+                                                         const int *__restrict__ table,
+                                                         const int *__restrict__ len,
+                                                         int *__restrict__ table_out,
+                                                         int *__restrict__ len_out,
+                                                         int *__restrict__ refs_out)
+{
+    const int t = threadIdx.x;
+    if ((int)blockIdx.x >= a.seqs) {
+        const int n = (gridDim.x - a.seqs) * 256;
+        for (int i = (blockIdx.x - a.seqs) * 256 + t; i < a.npages; i += n) refs_out[i] = 0;
+        return;
+    }
+    const int s = blockIdx.x, p = parent[s];
+    int got = 0;
+    if ((unsigned)p < (unsigned)a.seqs) {
+        got = (int)min((long long)max(len[p], 0), (long long)a.stride << a.shift);
+        if (keep) got = min(got, max(keep[s], 0));
+    }
+    const int n = held_pages(got, a.shift, a.stride);
+    const int *src = table + (size_t)(n ? p : 0) * a.stride;
+    int *dst = table_out + (size_t)s * a.stride;
+    for (int i = t; i < a.stride; i += 256) dst[i] = i < n ? src[i] : -1;
+    if (t == 0) len_out[s] = got;
+}
+
+// refs[p] = the entries that name page p, over the entries in use.
+__global__ __launch_bounds__(256) void pages_count_kernel(PagesArgs a, const int *__restrict__ table,
+                                                          const int *__restrict__ len,
+                                                          int *__restrict__ refs)
+{
+    const int s = blockIdx.x;
+    const int n = held_pages(len[s], a.shift, a.stride);
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int p = table[(size_t)s * a.stride + i];
+        if ((unsigned)p < (unsigned)a.npages) atomicAdd(refs + p, 1);
+    }
+}
+
+// ---- extend ----
+// Scratch of the plans, in ints.
+struct PagesScratch {
+    int *count;  // [16]: copies / moves, live pages
+    int *top;    // [npages]
+    int *asks;   // [npages]
+    int *free;   // [npages]
+    int *need;   // [seqs]: 2 * pages a slot wants + whether it copies
+    int *list;   // [3 max(npages, seqs)]
+};
+__device__ inline PagesScratch pages_layout(void *scratch, int npages, int seqs)
+{
+    PagesScratch p;
+    p.count = (int *)scratch;
+    p.top = p.count + 16;
+    p.asks = p.top + npages;
+    p.free = p.asks + npages;
+    p.need = p.free + npages;
+    p.list = p.need + seqs;
+    return p;
+}
+
+__device__ __forceinline__ int fresh(const int *p) // past this workgroup's own cached line
+{
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Exclusive scan over 1024 threads; returns the total.
+__device__ __forceinline__ int scan1024(int mine, int &before, int *wsum)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int v = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) wsum[wave] = v;
+    __syncthreads();
+    int base = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        if (w < wave) base += wsum[w];
+        all += wsum[w];
+    }
+    before = base + v - mine;
+    return all;
+}
+
+struct Ask {
+    int held, wants, fill, last;
+    bool asks, is_long, partial;
+};
+__device__ __forceinline__ Ask ask_of(const PagesArgs &a, const int *add, const int *table,
+                                      const int *len, int s)
+{
+    Ask k;
+    const int n = max(len[s], 0), more = add[s];
+    const long long cap = (long long)a.stride << a.shift;
+    k.is_long = more > 0 && (long long)n + more > cap;
+    k.asks = more > 0 && !k.is_long;
+    k.held = held_pages(n, a.shift, a.stride);
+    k.wants = k.asks ? held_pages(n + more, a.shift, a.stride) : k.held;
+    k.fill = n & ((1 << a.shift) - 1);
+    k.last = k.held > 0 ? table[(size_t)s * a.stride + k.held - 1] : -1;
+    k.partial = k.asks && k.fill > 0 && (unsigned)k.last < (unsigned)a.npages;
+    return k;
+}
+
+// One workgroup of 1024 threads. A slot's partly filled last page that others
+// name too is copied for it, unless all who name the page extend it in this
+// call and the slot holds most of it (the first of those): that one goes on
+// writing behind what any other has. Slots are served in order while free
+// pages last.
+__global__ __launch_bounds__(1024) void pages_extend_kernel(
+    PagesArgs a, const int *__restrict__ add, const int *table, const int *len, const int *refs,
+    int *table_out, int *len_out, int *refs_out, int *__restrict__ status, void *scratch)
+{
+    __shared__ int wsum[16];
+    const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
+    const int t = threadIdx.x;
+    for (int s = t; s < a.seqs; s += 1024) {
+        const Ask k = ask_of(a, add, table, len, s);
+        if (k.partial && refs[k.last] > 1) {
+            w.top[k.last] = 0;
+            w.asks[k.last] = 0;
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    for (int s = t; s < a.seqs; s += 1024) {
+        const Ask k = ask_of(a, add, table, len, s);
+        if (k.partial && refs[k.last] > 1) {
+            atomicAdd(w.asks + k.last, 1);
+            atomicMax((unsigned *)w.top + k.last, (unsigned)k.fill << 16 | (65535u - s));
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    auto copies_of = [&](const Ask &k, int s) {
+        if (!k.partial || refs[k.last] <= 1) return false;
+        const bool keeps = fresh(w.asks + k.last) == refs[k.last] &&
+                           (unsigned)fresh(w.top + k.last) ==
+                               ((unsigned)k.fill << 16 | (65535u - s));
+        return !keeps;
+    };
+    // how many pages all slots want, and as many free ones, lowest first
+    int total = 0;
+    for (int b = 0; b < a.seqs; b += 1024) {
+        int need = 0, before;
+        if (b + t < a.seqs) {
+            const Ask k = ask_of(a, add, table, len, b + t);
+            const bool copies = copies_of(k, b + t);
+            if (k.asks) need = k.wants - k.held + copies;
+            w.need[b + t] = 2 * need + copies;
+        }
+        total += scan1024(need, before, wsum);
+        total = min(total, a.npages + 1); // (no more than that matters)
+    }
+    int found = 0;
+    for (int b = 0; b < a.npages && found < total; b += 1024) {
+        const int p = b + t;
+        const int is = p < a.npages && refs[p] == 0;
+        int before;
+        const int all = scan1024(is, before, wsum);
+        if (is && found + before < total) w.free[found + before] = p;
+        found += all;
+    }
+    __threadfence();
+    __syncthreads();
+    if (table_out != table)
+        for (size_t i = t; i < (size_t)a.seqs * a.stride; i += 1024) table_out[i] = table[i];
+    // (the counts in `refs` are not read again: where refs_out is refs they change now)
+    if (refs_out != refs)
+        for (int i = t; i < a.npages; i += 1024) refs_out[i] = refs[i];
+    __threadfence();
+    __syncthreads();
+    int carry = 0, ncopies = 0;
+    for (int b = 0; b < a.seqs; b += 1024) {
+        const int s = b + t;
+        Ask k{};
+        bool copies = false;
+        int need = 0, before, cbefore;
+        if (s < a.seqs) {
+            k = ask_of(a, add, table, len, s);
+            copies = w.need[s] & 1;
+            need = w.need[s] >> 1;
+        }
+        const int all = scan1024(need, before, wsum);
+        const long long upto = (long long)carry + before + need;
+        const bool served = k.asks && (need == 0 || upto <= found);
+        const int call = scan1024(served && copies, cbefore, wsum);
+        if (s < a.seqs) {
+            int n = max(len[s], 0);
+            if (served) {
+                int at = carry + before;
+                int *row = table_out + (size_t)s * a.stride;
+                if (copies) {
+                    const int p = w.free[at++];
+                    row[k.held - 1] = p;
+                    __hip_atomic_store(refs_out + p, 1, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+                    atomicSub(refs_out + k.last, 1);
+                    int *c = w.list + 3 * (ncopies + cbefore);
+                    c[0] = k.last;
+                    c[1] = p;
+                    c[2] = k.fill;
+                }
+                for (int i = k.held; i < k.wants; ++i) {
+                    const int p = w.free[at++];
+                    row[i] = p;
+                    __hip_atomic_store(refs_out + p, 1, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+                }
+                n += add[s];
+            }
+            len_out[s] = n;
+            status[s] = k.is_long ? 2 : k.asks && !served ? 1 : 0;
+        }
+        carry = min(carry + all, a.npages + 1);
+        ncopies += call;
+        __syncthreads();
+    }
+    if (t == 0) w.count[0] = ncopies;
+}
+
+// Copies the filled rows of the pages on the list: one wave per (page, layer,
+// keys or values, head), rows of contiguous 16-byte words.
+__global__ __launch_bounds__(256) void pages_fill_kernel(PagesArgs a, char *pool, void *scratch)
+{
+    const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
+    const int n = w.count[0], per = a.layers * 2 * a.kvh;
+    const int lane = threadIdx.x & 63;
+    const size_t row = (size_t)KV_D * (a.f16 ? 2 : 4);
+    const size_t head = row << a.shift, page = head * 2 * a.kvh;
+    const long long items = (long long)n * per, step = (long long)gridDim.x * 4;
+    for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += step) {
+        const int c = (int)(i / per), r = (int)(i % per);
+        const int *e = w.list + 3 * c;
+        const size_t at = (size_t)(r / (2 * a.kvh)) * a.npages * page + (size_t)(r % (2 * a.kvh)) * head;
+        const uint4 *src = reinterpret_cast<const uint4 *>(pool + at + e[0] * page);
+        uint4 *dst = reinterpret_cast<uint4 *>(pool + at + e[1] * page);
+        const int words = (int)(e[2] * row / 16);
+        for (int x = lane; x < words; x += 64) dst[x] = src[x];
+    }
+}
+
+// ---- compact ----
+// One workgroup of 1024 threads: the live pages behind the live count, in
+// order, go to the free ids below it, in order; `top` maps an id to its new
+// one.
+__global__ __launch_bounds__(1024) void pages_compact_kernel(PagesArgs a, const int *refs,
+                                                             int *refs_out, int *live,
+                                                             void *scratch)
+{
+    __shared__ int wsum[16];
+    const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
+    const int t = threadIdx.x;
+    int count = 0;
+    for (int b = 0; b < a.npages; b += 1024) {
+        int before;
+        count += scan1024(b + t < a.npages && refs[b + t] > 0, before, wsum);
+    }
+    int moves = 0, holes = 0;
+    for (int b = 0; b < a.npages; b += 1024) {
+        const int p = b + t;
+        const bool in = p < a.npages, is = in && refs[p] > 0;
+        int mb, hb;
+        const int m = scan1024(is && p >= count, mb, wsum);
+        const int h = scan1024(in && !is && p < count, hb, wsum);
+        if (is && p >= count) w.list[moves + mb] = p;
+        if (in && !is && p < count) w.free[holes + hb] = p;
+        if (in) w.top[p] = p;
+        moves += m;
+        holes += h;
+    }
+    __threadfence();
+    __syncthreads();
+    if (refs_out != refs)
+        for (int i = t; i < a.npages; i += 1024) refs_out[i] = max(refs[i], 0);
+    __syncthreads();
+    for (int i = t; i < moves; i += 1024) { // (holes == moves)
+        const int src = fresh(w.list + i), dst = fresh(w.free + i);
+        w.top[src] = dst;
+        refs_out[dst] = refs[src];
+        refs_out[src] = 0;
+    }
+    if (t == 0) {
+        w.count[0] = moves;
+        *live = count;
+    }
+}
+
+// Moves the pages (in pieces of COMPACT_BYTES, a workgroup each) and renames
+// the table's entries.
+constexpr int COMPACT_BYTES = 16384;
+__global__ __launch_bounds__(256) void pages_move_kernel(PagesArgs a, char *pool, const int *table,
+                                                         int *table_out, void *scratch)
+{
+    const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
+    const int t = threadIdx.x;
+    const size_t page = ((size_t)KV_D * (a.f16 ? 2 : 4) << a.shift) * 2 * a.kvh;
+    const int cuts = (int)((page + COMPACT_BYTES - 1) / COMPACT_BYTES);
+    const long long per = (long long)a.layers * cuts, items = w.count[0] * per;
+    for (long long i = blockIdx.x; i < items; i += gridDim.x) {
+        const int m = (int)(i / per), r = (int)(i % per), cut = r % cuts;
+        const size_t layer = (size_t)(r / cuts) * a.npages * page + (size_t)cut * COMPACT_BYTES;
+        const uint4 *src = reinterpret_cast<const uint4 *>(pool + layer + w.list[m] * page);
+        uint4 *dst = reinterpret_cast<uint4 *>(pool + layer + w.free[m] * page);
+        const int words = (int)min((size_t)COMPACT_BYTES, page - (size_t)cut * COMPACT_BYTES) / 16;
+        uint4 v[COMPACT_BYTES / 4096];
+#pragma unroll
+        for (int k = 0; k < COMPACT_BYTES / 4096; ++k)
+            if (t + 256 * k < words) v[k] = src[t + 256 * k];
+#pragma unroll
+        for (int k = 0; k < COMPACT_BYTES / 4096; ++k)
+            if (t + 256 * k < words) dst[t + 256 * k] = v[k];
+    }
+    const size_t n = (size_t)a.seqs * a.stride;
+    for (size_t i = (size_t)blockIdx.x * 256 + t; i < n; i += (size_t)gridDim.x * 256) {
+        const int p = table[i];
+        table_out[i] = (unsigned)p < (unsigned)a.npages ? w.top[p] : p;
+    }
+}
+
+} // namespace
+
+size_t pages_scratch(int npages, int seqs)
+{
+    return (16 + 3 * (size_t)npages + seqs + 3 * (size_t)std::max(npages, seqs)) * 4;
+}
+
+int launch_pages_fork(const PagesArgs &a, const int *parent, const int *keep, const int *table,
+                      const int *len, int *table_out, int *len_out, int *refs_out, void *stream)
+{
+    hipStream_t st = (hipStream_t)stream;
+    const int clears = std::min(64, (a.npages + 255) / 256);
+    hipLaunchKernelGGL(pages_fork_kernel, dim3(a.seqs + clears), dim3(256), 0, st, a, parent, keep,
+                       table, len, table_out, len_out, refs_out);
+    hipLaunchKernelGGL(pages_count_kernel, dim3(a.seqs), dim3(256), 0, st, a, table_out, len_out,
+                       refs_out);
+    return (int)hipGetLastError();
+}
+
+int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const int *table,
+                        const int *len, const int *refs, int *table_out, int *len_out,
+                        int *refs_out, int *status, void *scratch, void *stream)
+{
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len, refs,
+                       table_out, len_out, refs_out, status, scratch);
+    hipLaunchKernelGGL(pages_fill_kernel, dim3(1024), dim3(256), 0, st, a, (char *)pool, scratch);
+    return (int)hipGetLastError();
+}
+
+int launch_pages_compact(const PagesArgs &a, void *pool, const int *table, const int *refs,
+                         int *table_out, int *refs_out, int *live, void *scratch, void *stream)
+{
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(1024), 0, st, a, refs, refs_out, live,
+                       scratch);
+    hipLaunchKernelGGL(pages_move_kernel, dim3(2048), dim3(256), 0, st, a, (char *)pool, table,
+                       table_out, scratch);
+    return (int)hipGetLastError();
+}
+
+} // namespace hyq

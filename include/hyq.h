@@ -347,6 +347,125 @@ int hyq_attention_rows_d(hyq_ctx *ctx, const float *q_d, const float *kcache_d,
  * scratch_d holds 128 floats. */
 int hyq_argmax_d(hyq_ctx *ctx, const float *x_d, size_t n, float *scratch_d, int32_t *token_d);
 
+/* ---- serving many sequences: a paged KV cache (device pointers,
+ * asynchronous) ----
+ * The reference keeps one contiguous cache per session (KvCache,
+ * src/model.rs:650-669); here the keys and values of many sequences lie in
+ * pages of one pool, and every call takes the new tokens of all of them.
+ *
+ *   pool   [layers][pages][2][kv_heads][page_tokens][head_dim] F32 or F16:
+ *          a page's keys, then its values, in every layer under one id
+ *   table  [seqs][stride] int32: the page ids of a slot's positions, in order
+ *          (-1: none; an id outside [0, pages) holds nothing: nothing is
+ *          written there and its positions are not attended)
+ *   len    [seqs] int32: positions a slot holds, its new tokens' included
+ *   start  [seqs + 1] int32, ascending from 0: slot s's new tokens are rows
+ *          start[s] .. start[s+1]-1 of the packed rows, at its last positions
+ *          len[s] - n .. len[s] - 1. Rows from start[seqs] on belong to no
+ *          slot: no call reads or writes them.
+ *
+ * These arrays are device memory that the library cannot check on the host;
+ * the kernels check every id and bound, so a wrong one makes wrong or missing
+ * results but no access outside the buffers given. Pools, rows and scratch
+ * must be 16-byte aligned. Calls that overlap in time (two contexts, two
+ * captured graphs replayed at once) need scratch of their own. Every call can
+ * be captured in a HIP graph: none allocates, copies to the host or waits. */
+typedef struct {
+    int dtype;       /* HYQ_F32 or HYQ_F16: element type of the pool */
+    int layers;
+    int kv_heads;    /* 1..256 */
+    int head_dim;    /* 128 */
+    int page_tokens; /* 16, 32, 64, 128 or 256 */
+    int pages;       /* ids 0 .. pages-1 */
+    int seqs;        /* slots, 1..4096 */
+    int stride;      /* table entries of a slot; stride * page_tokens <= 2^24 */
+} hyq_kv_layout;
+/* Bytes of the pool, 0 when the layout is not one of the above. */
+size_t hyq_kv_pool_bytes(const hyq_kv_layout *kl);
+/* hyq_rope_norm_append_d for the packed rows of many slots: RoPE and the
+ * per-head rms_norm of q [rows][heads*128] and k [rows][kv_heads*128]
+ * (norm_first: the hy_v3 order, src/model.rs:425-446), q to q_out_d (which may
+ * be q_d), k and v to the pages of `layer`. An F16 pool holds the values
+ * rounded once, to nearest. The angle position * freq_d[j] is taken in 64
+ * bits, where hyq_rope_norm_append_d rounds the product to 32 (the reference's
+ * table, src/model.rs:919-925): the two differ by up to position * 2^-24
+ * radians times the frequency, and agree where the product is exact. */
+int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, int layer,
+                                 const int32_t *table_d, const int32_t *len_d,
+                                 const int32_t *start_d, size_t rows, size_t heads,
+                                 const float *q_d, const float *k_d, const float *v_d,
+                                 const float *q_norm_d, const float *k_norm_d,
+                                 const float *freq_d, float eps, int norm_first,
+                                 float *q_out_d);
+/* attention (src/model.rs:949-1037) of the packed rows over their slots'
+ * pages: the row at position p sees the slot's positions 0..p. Any mix of
+ * prompts, decode steps and drafted tokens. max_rows bounds the new rows of
+ * one slot (a slot of more is not computed); heads / kv_heads is at most 16.
+ * Rows that see nothing give zeros. The values of an F32 pool must lie within
+ * the f16 range where a slot has more than 16 * kv_heads / heads new rows
+ * (those products split them into two f16 parts: 22 bits of values from 2^-3
+ * up, 2^-25 absolutely below). scratch_d: hyq_paged_attention_scratch_bytes
+ * bytes (0 for arguments that the call refuses). */
+size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
+                                         size_t heads);
+int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, int layer,
+                          const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
+                          size_t rows, size_t max_rows, size_t heads, const float *q_d,
+                          void *scratch_d, size_t scratch_bytes, float *out_d);
+/* ---- the pages' bookkeeping, on the device ----
+ * refs [pages] int32 counts the table entries that name a page; 0: free. The
+ * results are exact and the same on every run: free pages are taken lowest id
+ * first, slots served in order. */
+/* Forks, trims and frees slots: slot s becomes the first
+ * min(len[p], keep[s]) positions of slot p = parent[s] (as it was before the
+ * call; every position when keep_d is null), empty when parent[s] is outside
+ * [0, seqs). No page is copied: children share their parent's. Entries not in
+ * use are -1; refs_out is counted anew. table_out/len_out must not be
+ * table/len. */
+int hyq_pages_fork_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *parent_d,
+                     const int32_t *keep_d, const int32_t *table_d, const int32_t *len_d,
+                     int32_t *table_out_d, int32_t *len_out_d, int32_t *refs_out_d);
+/* Makes room for add[s] more tokens in every slot (add[s] <= 0: none) and
+ * adds them to its length. A partly filled last page that other slots share
+ * is copied first, in every layer, for the slots that extend it - but for one,
+ * when all slots that name it do: the one that holds most of it, the first of
+ * those. status[s]: 0, or 1 when the pool has too few free pages for slot s
+ * and those before it, or 2 when the slot's table row is too short; such a
+ * slot stays as it is. Each *_out may be its input. */
+size_t hyq_pages_scratch_bytes(const hyq_kv_layout *kl);
+int hyq_pages_extend_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, const int32_t *add_d,
+                       const int32_t *table_d, const int32_t *len_d, const int32_t *refs_d,
+                       int32_t *table_out_d, int32_t *len_out_d, int32_t *refs_out_d,
+                       int32_t *status_d, void *scratch_d, size_t scratch_bytes);
+/* Moves the pages in use to the ids 0 .. live-1, so that a smaller pool can
+ * take their place: those with ids from `live` on go to the free ids below, in
+ * order, in every layer. *live_d = their number. Each *_out may be its
+ * input. */
+int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
+                        const int32_t *table_d, const int32_t *refs_d, int32_t *table_out_d,
+                        int32_t *refs_out_d, int32_t *live_d, void *scratch_d,
+                        size_t scratch_bytes);
+
+/* Sampling (Sampler, src/generation.rs:229-334, from given random numbers):
+ * one token for each row of logits [rows][vocab], with settings of its own in
+ * device arrays of `rows` values. With w_i = exp((l_i - max l) / temperature)
+ * and the order of larger logits first, equal ones by index: the first top_k
+ * of the order (<= 0: all); of those the shortest prefix whose weight reaches
+ * top_p of theirs (>= 1: all); of those the ones with w_i >= min_p (the
+ * largest always); token = in index order the first of them at which the
+ * running weight exceeds random * their weight, random in [0, 1) (values
+ * outside are cut to 0 and 1). temperature <= 0: the first maximum. A NaN or
+ * minus infinity is never taken; a row of nothing else gives token -1. Weights
+ * are summed exactly to 2^-46 of the largest (2^-62 times the vocabulary,
+ * rounded up to a power of two, where that is more): smaller ones count as
+ * zero. prob_d (may be null): the token's weight over the kept ones' (1 at
+ * temperature <= 0, 0 beside -1). */
+size_t hyq_sample_scratch_bytes(size_t rows, size_t vocab);
+int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
+                 const float *temperature_d, const int32_t *top_k_d, const float *top_p_d,
+                 const float *min_p_d, const float *random_d, void *scratch_d,
+                 size_t scratch_bytes, int32_t *token_d, float *prob_d);
+
 /* ---- dense decoder: Model::forward_into at batch 1 (src/model.rs:374-546)
  * for the hunyuan-dense graph, device-resident, KV cache in HBM ---- */
 typedef struct {
