@@ -40,8 +40,8 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int FEW_TILE = 16;
 constexpr int FEW_WAVES = 4;
 
 // before[s], in LDS: the tiles of the slots before s over all KV heads, with
@@ -52,24 +52,24 @@ struct FewPlan {
 };
 
 // (new rows over no positions still have their zeros to be written: one tile)
-__device__ __forceinline__ int slot_tiles(const SlotRows &r)
+__device__ __forceinline__ int slot_tiles(const SlotRows &r, int tile)
 {
-    return max(1, (r.len + FEW_TILE - 1) / FEW_TILE);
+    return max(1, (r.len + tile - 1) / tile);
 }
-__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows)
+__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows, int tile)
 {
     const SlotRows r = slot_rows(kv, s);
-    return r.n > 0 && r.n <= few_rows ? slot_tiles(r) : 0;
+    return r.n > 0 && r.n <= few_rows ? slot_tiles(r, tile) : 0;
 }
 
-__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int max_workers,
+__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int tile, int max_workers,
                                             long long *before, long long *wsum)
 {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     long long carry = 0;
     for (int b = 0; b < kv.seqs; b += 256) {
         const int s = b + t;
-        const long long mine = s < kv.seqs ? (long long)few_tiles(kv, s, few_rows) * kv.kvh : 0;
+        const long long mine = s < kv.seqs ? (long long)few_tiles(kv, s, few_rows, tile) * kv.kvh : 0;
         long long v = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -91,8 +91,8 @@ __device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int
     __syncthreads();
     FewPlan p;
     p.total = carry;
-    // two tiles at least for a worker: fewer would only add partial rows
-    p.workers = (int)min((long long)max_workers, (carry + 1) / 2);
+    // 32 positions at least for a worker: fewer would only add partial rows
+    p.workers = (int)min((long long)max_workers, (carry * tile + 31) / 32);
     return p;
 }
 
@@ -109,10 +109,19 @@ __device__ __forceinline__ f32x4 mfma_f16(const half8 &a, const half8 &b, const 
 // acc[x][e] (see pv): f32 64 (x / 4) + 16 g + 4 e + x % 4, f16 32 g + 8 e + x.
 template <class T> struct Ops;
 
+// A vector at a uniform base and an unsigned 32-bit element offset (a scalar
+// base with a vector offset in the load: no 64-bit address per lane).
+template <class V, class T> __device__ __forceinline__ V at(const T *base, unsigned off)
+{
+    return *reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
+                                        (unsigned)(off * sizeof(T)));
+}
+
 template <> struct Ops<float> {
+    static constexpr int TILE = 16; // positions of a step
     float4 q[8]; // row lane % 16, dims 16 j + 4 g ..
-    float4 k[8]; // position lane % 16, the same dims
-    float4 v[8]; // position 4 g + x / 2, dims 64 (x % 2) + 4 (lane % 16) ..
+    float4 k[1][8]; // position lane % 16, the same dims
+    float4 v[1][8]; // position 4 g + x / 2, dims 64 (x % 2) + 4 (lane % 16) ..
     float qscale;
     __device__ __forceinline__ void load_q(const float *row, bool ok, int g)
     {
@@ -123,54 +132,58 @@ template <> struct Ops<float> {
         }
         qscale = 1.f;
     }
-    __device__ __forceinline__ void load_k(const float *head, int kpos, int g)
+    __device__ __forceinline__ void load_k(int u, const float *head, int kpos, int g)
     {
-        const float *p = head + (size_t)kpos * KV_D + 4 * g;
+        const unsigned o = kpos * KV_D + 4 * g;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const float4 *>(p + 16 * j);
+        for (int j = 0; j < 8; ++j) k[u][j] = at<float4>(head, o + 16 * j);
     }
-    __device__ __forceinline__ void load_v(const float *head, const int (&vpos)[4], int c)
+    __device__ __forceinline__ void load_v(int u, const float *head, const int (&vpos)[4], int c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float *p = head + (size_t)vpos[e] * KV_D + 4 * c;
-            v[2 * e] = *reinterpret_cast<const float4 *>(p);
-            v[2 * e + 1] = *reinterpret_cast<const float4 *>(p + 64);
+            const unsigned o = vpos[e] * KV_D + 4 * c;
+            v[u][2 * e] = at<float4>(head, o);
+            v[u][2 * e + 1] = at<float4>(head, o + 64);
         }
     }
-    __device__ __forceinline__ f32x4 scores() const
+    __device__ __forceinline__ f32x4 scores(int u) const
     {
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            a = mfma_f32(k[j].x, q[j].x, a);
-            b = mfma_f32(k[j].y, q[j].y, b);
-            a = mfma_f32(k[j].z, q[j].z, a);
-            b = mfma_f32(k[j].w, q[j].w, b);
+            a = mfma_f32(k[u][j].x, q[j].x, a);
+            b = mfma_f32(k[u][j].y, q[j].y, b);
+            a = mfma_f32(k[u][j].z, q[j].z, a);
+            b = mfma_f32(k[u][j].w, q[j].w, b);
         }
         return a + b;
     }
-    __device__ __forceinline__ void pv(const f32x4 &p, f32x4 (&acc)[8]) const
+    __device__ __forceinline__ void pv(int u, const f32x4 &p, f32x4 (&acc)[8]) const
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float4 x = v[2 * e + c];
+                const float4 x = v[u][2 * e + c];
                 acc[4 * c] = mfma_f32(x.x, p[e], acc[4 * c]);
                 acc[4 * c + 1] = mfma_f32(x.y, p[e], acc[4 * c + 1]);
                 acc[4 * c + 2] = mfma_f32(x.z, p[e], acc[4 * c + 2]);
                 acc[4 * c + 3] = mfma_f32(x.w, p[e], acc[4 * c + 3]);
             }
     }
-    // 0 where every value of the tile is finite, NaN where one is not
-    __device__ __forceinline__ float odd() const
+    // values that are not finite become zero; whether there were any
+    __device__ __forceinline__ bool clean()
     {
-        float z = 0.f;
+        bool odd = false;
+        auto one = [&](float &x) {
+            const bool fine = fabsf(x) < INFINITY;
+            odd |= !fine;
+            x = fine ? x : 0.f;
+        };
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-            z = fmaf(v[x].x, 0.f, fmaf(v[x].y, 0.f, fmaf(v[x].z, 0.f, fmaf(v[x].w, 0.f, z))));
-        return z;
+        for (int x = 0; x < 8; ++x) one(v[0][x].x), one(v[0][x].y), one(v[0][x].z), one(v[0][x].w);
+        return odd;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g)
     {
@@ -190,9 +203,10 @@ template <> struct Ops<float> {
 };
 
 template <> struct Ops<_Float16> {
+    static constexpr int TILE = 32;
     half8 qh[4], ql[4]; // row lane % 16, dims 32 j + 8 g ..
-    half8 k[4];         // position lane % 16, the same dims
-    half8 v[4];         // position 4 g + e, dims 8 (lane % 16) ..
+    half8 k[2][4];      // position 16 u + lane % 16, the same dims
+    half8 v[2][4];      // position 16 u + 4 g + e, dims 8 (lane % 16) ..
     float qscale;
     // q = 2^e (high + low): the row's power of two brings its largest value
     // to [1, 2), inside f16's range whatever the queries' size, and the low
@@ -228,43 +242,56 @@ template <> struct Ops<_Float16> {
                 ql[j][i] = fabsf(y) < INFINITY ? (_Float16)(y - (float)h) : (_Float16)0.f;
             }
     }
-    __device__ __forceinline__ void load_k(const _Float16 *head, int kpos, int g)
+    __device__ __forceinline__ void load_k(int u, const _Float16 *head, int kpos, int g)
     {
-        const _Float16 *p = head + (size_t)kpos * KV_D + 8 * g;
+        const unsigned o = kpos * KV_D + 8 * g;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const half8 *>(p + 32 * j);
+        for (int j = 0; j < 4; ++j) k[u][j] = at<half8>(head, o + 32 * j);
     }
-    __device__ __forceinline__ void load_v(const _Float16 *head, const int (&vpos)[4], int c)
+    __device__ __forceinline__ void load_v(int u, const _Float16 *head, const int (&vpos)[4], int c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            v[e] = *reinterpret_cast<const half8 *>(head + (size_t)vpos[e] * KV_D + 8 * c);
+            v[u][e] = at<half8>(head, vpos[e] * KV_D + 8 * c);
     }
-    __device__ __forceinline__ f32x4 scores() const
+    __device__ __forceinline__ f32x4 scores(int u) const
     {
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            a = mfma_f16(k[j], qh[j], a);
-            b = mfma_f16(k[j], ql[j], b);
+            a = mfma_f16(k[u][j], qh[j], a);
+            b = mfma_f16(k[u][j], ql[j], b);
         }
         return (a + b) * qscale;
     }
-    __device__ __forceinline__ void pv(const f32x4 &p, f32x4 (&acc)[8]) const
+    __device__ __forceinline__ void pv(int u, const f32x4 &p, f32x4 (&acc)[8]) const
     {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) acc[x] = mfma_f32((float)v[e][x], p[e], acc[x]);
+            for (int x = 0; x < 8; ++x) acc[x] = mfma_f32((float)v[u][e][x], p[e], acc[x]);
+            // (keeps the widened values of later positions out of registers)
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    __device__ __forceinline__ float odd() const
+    __device__ __forceinline__ bool clean()
     {
-        float z = 0.f;
+        bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int x = 0; x < 8; ++x) z = fmaf((float)v[e][x], 0.f, z);
-        return z;
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) { // (two f16 of exponent all ones or not)
+                    u32x4 w = __builtin_bit_cast(u32x4, v[u][e]);
+                    const bool a = (w[x] & 0x7c00u) == 0x7c00u;
+                    const bool b = (w[x] & 0x7c000000u) == 0x7c000000u;
+                    w[x] = a ? w[x] & 0xffff0000u : w[x];
+                    w[x] = b ? w[x] & 0x0000ffffu : w[x];
+                    odd |= a | b;
+                    v[u][e] = __builtin_bit_cast(half8, w);
+                }
+        return odd;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g) { return 32 * g + 8 * e + x; }
     static __device__ __forceinline__ void put(float *o, const f32x4 (&acc)[8], int g, float s)
@@ -280,13 +307,14 @@ template <> struct Ops<_Float16> {
 };
 
 template <class T>
-__global__ __launch_bounds__(64 * FEW_WAVES) void paged_few_kernel(
+__global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     PagedKv kv, int few_rows, int max_workers, const float *__restrict__ q, int part_rows,
     float *__restrict__ part, float *__restrict__ out)
 {
+    constexpr int TILE = Ops<T>::TILE, SUB = TILE / 16;
     extern __shared__ long long before[]; // [seqs + 1]
     __shared__ long long wsum[4];
-    const FewPlan plan = few_plan(kv, few_rows, max_workers, before, wsum);
+    const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be)
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * FEW_WAVES + (threadIdx.x >> 6));
@@ -310,11 +338,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_few_kernel(
     }
     while (at < stop) {
         while (before[s + 1] <= at) ++s; // slots without tiles
+        s = __builtin_amdgcn_readfirstlane(s); // (what comes from LDS, known to be uniform)
         const SlotRows sr = slot_rows(kv, s);
-        const int tiles = slot_tiles(sr);
-        const int in = (int)(at - before[s]);
+        const int tiles = slot_tiles(sr, TILE);
+        const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
         const int kh = in / tiles, t0 = in % tiles;
-        const int t1 = (int)min((long long)tiles, t0 + (stop - at));
+        const int t1 = __builtin_amdgcn_readfirstlane(
+            (int)min((long long)tiles, t0 + (stop - at)));
         at += t1 - t0;
 
         // this lane's row: token c / rep of the slot's new rows
@@ -332,52 +362,63 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_few_kernel(
         float m = -INFINITY, l = 0.f;
 
         const int *entries = kv.table + (size_t)s * kv.stride;
-        const int per = kv.shift - 4; // log2 of a page's tiles
-        int have = -64, pages = -1;   // lane i: the slot's page have + i
-        auto page_of = [&](int t) {
-            const int p = t >> per;
+        int have = -64, pages = -1; // lane i: the slot's page have + i
+        // the page of 16 positions, -1 where the slot has none
+        auto page_of = [&](int p0) {
+            const int p = p0 >> kv.shift;
             if (p - have >= 64 || p < have) {
                 have = p;
                 pages = have + lane < kv.stride ? entries[have + lane] : -1;
             }
-            return __builtin_amdgcn_readlane(pages, p - have);
+            const int id = __builtin_amdgcn_readlane(pages, p - have);
+            return p0 < sr.len && (unsigned)id < (unsigned)kv.npages ? id : -1;
         };
-        auto base_of = [&](int page) {
-            return (const T *)kv.pages + (size_t)page * psize + (size_t)kh * hsize;
+        // A step's loads are unconditional: positions past the length are taken
+        // from the last one, and where there is no page from the pool's first
+        // (their weights are zero, and values that are not finite are cleared).
+        auto head_of = [&](int page) {
+            return (const T *)kv.pages + (size_t)max(page, 0) * psize + (size_t)kh * hsize;
         };
-        // positions of a tile, those past the slot's length taken from its
-        // last one (a valid row, whose weight is zero)
-        auto load = [&](int t, int page, bool keys, bool values) {
-            const int p0 = t * FEW_TILE, lim = sr.len - 1 - p0, in_page = p0 & pmask;
-            const T *b = base_of(page);
-            if (keys) ops.load_k(b, in_page + min(c, lim), g);
-            if (values) {
+        auto load_k = [&](int p0, const int (&page)[SUB]) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                const int p = p0 + 16 * u;
+                ops.load_k(u, head_of(page[u]), (p & pmask) + max(min(c, sr.len - 1 - p), 0), g);
+            }
+        };
+        auto load_v = [&](int p0, const int (&page)[SUB]) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                const int p = p0 + 16 * u, lim = sr.len - 1 - p;
                 int vp[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) vp[e] = in_page + min(4 * g + e, lim);
-                ops.load_v(b + hsize * kv.kvh, vp, c);
+                for (int e = 0; e < 4; ++e) vp[e] = (p & pmask) + max(min(4 * g + e, lim), 0);
+                ops.load_v(u, head_of(page[u]) + hsize * kv.kvh, vp, c);
             }
         };
-        // tiles whose page the table does not name are not seen
-        auto valid = [&](int page) { return sr.len > 0 && (unsigned)page < (unsigned)kv.npages; };
-        int page = page_of(t0);
-        if (valid(page)) load(t0, page, true, true);
+        int page[SUB], next[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) page[u] = page_of(t0 * TILE + 16 * u);
+        load_k(t0 * TILE, page);
+        load_v(t0 * TILE, page);
+        bool odd = false;
         for (int t = t0; t < t1; ++t) {
-            const int next = t + 1 < t1 ? page_of(t + 1) : -1;
-            if (!valid(page)) {
-                page = next;
-                if (valid(page)) load(t + 1, page, true, true);
-                continue;
-            }
-            f32x4 sv = ops.scores();
-            if (valid(next)) load(t + 1, next, true, false);
-            const int p0 = t * FEW_TILE + 4 * g;
+            const int p0 = t * TILE, pn = min(t + 1, t1 - 1) * TILE;
+            f32x4 sv[SUB];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) sv[u] = ops.scores(u);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) next[u] = page_of(pn + 16 * u);
+            load_k(pn, next);
             float mx = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sv[e] = p0 + e <= sees ? sv[e] * sc : -INFINITY;
-                mx = fmaxf(mx, sv[e]);
-            }
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool see = p0 + 16 * u + 4 * g + e <= sees && page[u] >= 0;
+                    sv[u][e] = see ? sv[u][e] * sc : -INFINITY;
+                    mx = fmaxf(mx, sv[u][e]);
+                }
             mx = wave::max_halves(wave::max_rows2(mx));
             const float mn = fmaxf(m, mx);
             // a row that has seen nothing yet keeps zero weights
@@ -385,10 +426,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_few_kernel(
             const float corr = __builtin_amdgcn_exp2f(m - base);
             float rs = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sv[e] = __builtin_amdgcn_exp2f(sv[e] - base);
-                rs += sv[e];
-            }
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sv[u][e] = __builtin_amdgcn_exp2f(sv[u][e] - base);
+                    rs += sv[u][e];
+                }
             if (__any(mn != m)) {
 #pragma unroll
                 for (int x = 0; x < 8; ++x) acc[x] *= corr;
@@ -396,27 +439,35 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_few_kernel(
             }
             l += rs;
             m = mn;
-            // a tile that some row sees in part: a value there that is not finite
-            // must not reach the rows that do not see it (0 * inf)
-            if (t * FEW_TILE + FEW_TILE - 1 > first && __any(ops.odd() != 0.f)) {
-                const T *vb = base_of(page) + hsize * kv.kvh;
-                for (int i = 0; i < FEW_TILE; ++i) {
-                    const int src = (i >> 2) * 16 + c;
-                    const float p = i & 2 ? (i & 1 ? __shfl(sv[3], src, 64) : __shfl(sv[2], src, 64))
-                                          : (i & 1 ? __shfl(sv[1], src, 64) : __shfl(sv[0], src, 64));
-                    if (t * FEW_TILE + i > sees) continue;
-                    const T *vr = vb + (size_t)((t * FEW_TILE + i) & pmask) * KV_D;
+            // a step that some row does not see whole: a value that is not finite
+            // must not reach the rows that do not see it (0 * inf), see below
+            bool whole = p0 + TILE - 1 <= first;
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
+            for (int u = 0; u < SUB; ++u) whole = whole && page[u] >= 0;
+            if (!whole) odd |= __any(ops.clean());
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[x][e] = fmaf(p, (float)vr[Ops<T>::dim(x, e, g)], acc[x][e]);
-                }
-            } else {
-                ops.pv(sv, acc);
+            for (int u = 0; u < SUB; ++u) ops.pv(u, sv[u], acc);
+            load_v(pn, next);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) page[u] = next[u];
+        }
+        if (odd) {
+            // the values left out of the steps above, for the rows that see
+            // them: whatever its weight, such a value makes the sum not finite
+            for (int p = t0 * TILE; p < min(t1 * TILE, sr.len); ++p) {
+                const int id = page_of(p & ~15), pt = p / TILE * TILE;
+                bool whole = pt + TILE - 1 <= first;
+                for (int u = 0; u < SUB; ++u) whole = whole && page_of(pt + 16 * u) >= 0;
+                if (whole || id < 0 || p > sees) continue;
+                const T *vr = head_of(id) + hsize * kv.kvh + (p & pmask) * KV_D;
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = (float)vr[Ops<T>::dim(x, e, g)];
+                        acc[x][e] += fabsf(y) < INFINITY ? 0.f : y;
+                    }
             }
-            if (valid(next)) load(t + 1, next, false, true);
-            page = next;
         }
         l = wave::sum_halves(wave::sum_rows2(l));
         if (t0 == 0 && t1 == tiles) {
@@ -434,8 +485,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_few_kernel(
     }
 }
 
-// Joins the parts of the units that several workers shared, in worker order.
-// Grid (kv heads, seqs), 256 threads: two rows at a time, a dim per thread.
+// Joins the parts of the units that several workers shared. Grid (kv heads,
+// seqs, rows), 256 threads: wave g takes the parts g, g + 4, ..., lane d dims
+// 2 d and 2 d + 1, with eight parts' loads in flight; the waves' sums are
+// added in a fixed order.
+template <int TILE>
 __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedKv kv, int few_rows,
                                                               int max_workers, int part_rows,
                                                               const float *__restrict__ part,
@@ -443,39 +497,60 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedKv kv, int fe
 {
     extern __shared__ long long before[];
     __shared__ long long wsum[4];
-    const FewPlan plan = few_plan(kv, few_rows, max_workers, before, wsum);
-    const int s = blockIdx.y, kh = blockIdx.x;
+    __shared__ float red[4][KV_D + 2];
+    const int s = blockIdx.y, kh = blockIdx.x, c = blockIdx.z;
+    const int rep = kv.heads / kv.kvh;
     const SlotRows sr = slot_rows(kv, s);
-    const int tiles = few_tiles(kv, s, few_rows);
-    if (tiles == 0) return;
+    const int tiles = few_tiles(kv, s, few_rows, TILE);
+    if (tiles == 0 || c >= sr.n * rep) return;
+    const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
     const long long first = before[s] + (long long)kh * tiles, last = first + tiles - 1;
     // the worker of tile x: the largest w with total * w / workers <= x
     auto worker = [&](long long x) {
         return (int)(((x + 1) * plan.workers - 1) / plan.total);
     };
-    const int w0 = worker(first), w1 = worker(last);
-    if (w0 == w1) return; // written whole
-    const int rep = kv.heads / kv.kvh;
-    const long long slot0 = (long long)w0 + (long long)s * kv.kvh + kh;
-    const int d = threadIdx.x & 127;
-    for (int c = threadIdx.x >> 7; c < sr.n * rep; c += 2) {
-        const float *p = part + ((size_t)slot0 * part_rows + c) * PAGED_PART;
-        const size_t step = (size_t)part_rows * PAGED_PART;
-        float M = -INFINITY;
-        for (int i = 0; i <= w1 - w0; ++i) M = fmaxf(M, p[i * step]);
-        const float base = M == -INFINITY ? 0.f : M;
-        float num = 0.f, den = 0.f;
-        for (int i = 0; i <= w1 - w0; ++i) {
-            const float x = __builtin_amdgcn_exp2f(p[i * step] - base);
-            den = fmaf(x, p[i * step + 1], den);
-            num = fmaf(x, p[i * step + 4 + d], num);
+    const int w0 = worker(first), n = worker(last) - w0 + 1;
+    if (n == 1) return; // written whole
+    const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const size_t step = (size_t)part_rows * PAGED_PART;
+    const float *p = part +
+                     ((size_t)((long long)w0 + (long long)s * kv.kvh + kh) * part_rows + c) *
+                         PAGED_PART;
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 64) M = fmaxf(M, p[i * step]);
+    M = wave::max64(M);
+    const float base = M == -INFINITY ? 0.f : M;
+    float den = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int b = g; b < n; b += 32) {
+        float2 ml[8], v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float *o = p + (size_t)min(b + 4 * k, n - 1) * step;
+            ml[k] = *reinterpret_cast<const float2 *>(o);
+            v[k] = *reinterpret_cast<const float2 *>(o + 4 + 2 * lane);
         }
-        const size_t row = (size_t)(sr.begin + c / rep) * kv.heads + kh * rep + c % rep;
-        out[row * KV_D + d] = den > 0.f || den != den ? num / den : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (b + 4 * k >= n) continue;
+            const float w = __builtin_amdgcn_exp2f(ml[k].x - base);
+            den = fmaf(w, ml[k].y, den);
+            x0 = fmaf(w, v[k].x, x0);
+            x1 = fmaf(w, v[k].y, x1);
+        }
     }
+    red[g][2 * lane] = x0;
+    red[g][2 * lane + 1] = x1;
+    if (lane == 0) red[g][KV_D] = den;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= KV_D) return;
+    den = (red[0][KV_D] + red[1][KV_D]) + (red[2][KV_D] + red[3][KV_D]);
+    const float num = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
+    const size_t row = (size_t)(sr.begin + c / rep) * kv.heads + kh * rep + c % rep;
+    out[row * KV_D + d] = den > 0.f || den != den ? num / den : 0.f;
 }
 
-constexpr int FEW_MAX_WORKERS = 2048; // eight waves on each of 256 CUs
+constexpr int FEW_MAX_WORKERS = 2048; // twelve waves on each of 256 CUs
 
 } // namespace
 
@@ -494,14 +569,18 @@ int launch_paged_few(const PagedKv &kv, int few, const float *q, float *part, fl
     const int part_rows = few * (kv.heads / kv.kvh);
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
     const dim3 grid(FEW_MAX_WORKERS / FEW_WAVES), block(64 * FEW_WAVES);
-    if (kv.f16)
+    const dim3 mgrid(kv.kvh, kv.seqs, part_rows);
+    if (kv.f16) {
         hipLaunchKernelGGL(paged_few_kernel<_Float16>, grid, block, lds, st, kv, few,
                            FEW_MAX_WORKERS, q, part_rows, part, out);
-    else
+        hipLaunchKernelGGL(paged_few_merge_kernel<Ops<_Float16>::TILE>, mgrid, dim3(256), lds, st,
+                           kv, few, FEW_MAX_WORKERS, part_rows, part, out);
+    } else {
         hipLaunchKernelGGL(paged_few_kernel<float>, grid, block, lds, st, kv, few,
                            FEW_MAX_WORKERS, q, part_rows, part, out);
-    hipLaunchKernelGGL(paged_few_merge_kernel, dim3(kv.kvh, kv.seqs), dim3(256), lds, st, kv,
-                       few, FEW_MAX_WORKERS, part_rows, part, out);
+        hipLaunchKernelGGL(paged_few_merge_kernel<Ops<float>::TILE>, mgrid, dim3(256), lds, st,
+                           kv, few, FEW_MAX_WORKERS, part_rows, part, out);
+    }
     return (int)hipGetLastError();
 }
 
