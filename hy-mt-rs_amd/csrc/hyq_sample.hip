@@ -15,19 +15,19 @@
 // e^-32 of the largest are zero and never drawn (shift is 62 minus log2 of the
 // vocabulary, at most 46; e^-32 = 2^-46.2).
 //
-// A row is cut into splits of a workgroup each, over three launches that each
-// read the row once, and a last one with a workgroup per row:
+// A row is cut into splits of a workgroup each, a split into a run per wave:
 //   max     the largest value and its first index, by split
 //   bins    a histogram, by split, of (max - l) / T in 2048 bins of 1/64:
 //           counts where top-k is set, weights where top-p needs them
-//   sums    every workgroup adds the splits' histograms and finds the bins that
-//           the cuts fall into; their members go to a list, and the weights of
-//           all smaller bins are summed by split
-//   draw    sorts the list, cuts it exactly, adds the kept members to the
-//           splits' sums, finds the split that holds u W and in it the token
+//   find    (a workgroup per row) adds the splits' histograms and finds the bins
+//           that the cuts fall into
+//   sums    lists those bins' members, and sums the weights of the smaller bins
+//           by run
+//   draw    (a workgroup per row) cuts the list exactly, adds the kept members
+//           to the runs' sums, finds the run that holds u W and in it the token
 // Where a cut's bin has more members than the list holds (equal logits by the
-// thousand) the last launch does the row by itself, refining its cut bit by
-// bit over the row.
+// thousand) the last launch does the row by itself, refining its cut bit by bit
+// over the row.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -69,36 +69,55 @@ __device__ __forceinline__ int bin_of(float l, const RowSettings &s)
     const float d = (s.max - l) * s.per_bin; // (NaN and infinite: no bin)
     return d < (float)SAMPLE_BINS ? (int)d : SAMPLE_BINS;
 }
-// exp(x) for x in [-33, 0]: x = n ln 2 + r with |r| <= 0.347, the series of
-// exp(r) to r^12 (the next term is below 2e-16), times 2^n.
-__device__ __forceinline__ double exp_neg(double x)
+// 2^(i / 64), rounded to 64 bits.
+__constant__ const double EXP2_64[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+// A workgroup's copy of the table (ends with a barrier).
+__device__ __forceinline__ void load_table(double *table)
 {
-    const double n = rint(x * 1.4426950408889634);
-    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));
-    double e = 1.0 / 479001600;
-    e = fma(e, r, 1.0 / 39916800);
-    e = fma(e, r, 1.0 / 3628800);
-    e = fma(e, r, 1.0 / 362880);
-    e = fma(e, r, 1.0 / 40320);
-    e = fma(e, r, 1.0 / 5040);
-    e = fma(e, r, 1.0 / 720);
-    e = fma(e, r, 1.0 / 120);
-    e = fma(e, r, 1.0 / 24);
+    if (threadIdx.x < 64) table[threadIdx.x] = EXP2_64[threadIdx.x];
+    __syncthreads();
+}
+// The weight of a value that has a bin: exp(x), x = (l - max) / T in [-33, 0],
+// is 2^(n / 64) exp(r) with |r| <= ln 2 / 128, the series of exp(r) to r^5
+// (the next term is below 4e-17) times the table's value, times 2^(n >> 6) by
+// its exponent. A third of the 64-bit operations of a series for the whole
+// argument, and those are what bounds a pass that weighs every value.
+__device__ __forceinline__ double weight(float l, const RowSettings &s, const double *table)
+{
+    if (l == s.max) return 1.0;
+    const double x = ((double)l - (double)s.max) * s.inv_t;
+    const double n = rint(x * 92.33248261689366);
+    const double r = fma(n, -3.623510646634843e-19, fma(n, -0.010830424696249145, x));
+    const int k = (int)n;
+    double e = fma(r, 1.0 / 120, 1.0 / 24);
     e = fma(e, r, 1.0 / 6);
     e = fma(e, r, 0.5);
     e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    return ldexp(e, (int)n);
+    e = fma(e, r, 1.0) * table[k & 63];
+    const u64 bits = __builtin_bit_cast(u64, e) + ((u64)(unsigned)(k >> 6) << 52);
+    return __builtin_bit_cast(double, bits); // (e >= 0.99, k >> 6 >= -48: no underflow)
 }
-// The weight of a value that has a bin.
-__device__ __forceinline__ double weight(float l, const RowSettings &s)
-{
-    if (l == s.max) return 1.0;
-    return exp_neg(((double)l - (double)s.max) * s.inv_t);
-}
+// w 2^shift as an integer, to nearest: the sum with 2^52 holds it in its low
+// bits (w 2^shift <= 2^46).
 __device__ __forceinline__ u64 fixed(double w, const RowSettings &s)
 {
-    return (u64)(w * s.scale + 0.5);
+    return __builtin_bit_cast(u64, fma(w, s.scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
 }
 
 __device__ __forceinline__ u64 wave_sum(u64 v)
@@ -142,7 +161,7 @@ struct Cut {
 
 struct SampleArgs {
     const float *logits;
-    int vocab, shift, splits, per; // per: values of a split
+    int vocab, shift, splits, run; // run: values of each of a split's 16 runs
     const float *temperature;
     const int *top_k;
     const float *top_p, *min_p, *random;
@@ -153,7 +172,7 @@ struct SampleArgs {
     int *sidx;       // [rows][splits]: the split's first maximum
     unsigned *count; // [rows][splits][SAMPLE_BINS]
     u64 *wsum;       // [rows][splits][SAMPLE_BINS]
-    u64 *sums;       // [rows][splits]: weights of the bins before the listed ones
+    u64 *sums;       // [rows][splits][16]: a run's weight in the bins before the listed ones
     struct Found *found; // [rows]
     unsigned *have;  // [rows][2]: members listed
     u64 *list;       // [rows][2][SAMPLE_LIST]: order key << 32 | ~index
@@ -225,6 +244,26 @@ __device__ __forceinline__ u64 draw_target(float random, u64 total)
     return min((u64)(u * (double)total) + 1, total);
 }
 
+// f(value, index) for a thread's values of [begin, end): eight loads in flight,
+// then one call at a time from one place in the code. (A launch starts with a
+// cold instruction cache: f's 64-bit exponential is not fetched eight times over.)
+template <class F>
+__device__ __forceinline__ void each_value(const float *x, int begin, int end, int first, int step,
+                                           F f)
+{
+    for (int i = begin + first; i < end; i += 8 * step) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = x[min(i + u * step, end - 1)];
+#pragma unroll 1
+        for (int j = i; j < min(end, i + 8 * step); j += step) {
+            f(v[0], j);
+#pragma unroll
+            for (int u = 0; u < 7; ++u) v[u] = v[u + 1];
+        }
+    }
+}
+
 // ---- max ----
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_max_kernel(SampleArgs a)
 {
@@ -232,20 +271,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_max_kernel(SampleArgs a
     __shared__ int si[SAMPLE_WAVES];
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     const float *x = a.logits + (size_t)row * a.vocab;
-    const int end = min(a.vocab, (s + 1) * a.per);
+    const int per = SAMPLE_WAVES * a.run, end = min(a.vocab, (s + 1) * per);
     float mx = -INFINITY;
     int mi = 0x7fffffff;
-    for (int i = s * a.per + t; i < end; i += 4 * SAMPLE_THREADS) {
-        float v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = x[min(i + u * SAMPLE_THREADS, end - 1)];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i + u * SAMPLE_THREADS < end && v[u] > mx) {
-                mx = v[u];
-                mi = i + u * SAMPLE_THREADS;
-            }
-    }
+    each_value(x, s * per, end, t, SAMPLE_THREADS, [&](float v, int i) {
+        if (v > mx) {
+            mx = v;
+            mi = i;
+        }
+    });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const float v = __shfl_xor(mx, o, 64);
@@ -277,28 +311,24 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_bins_kernel(SampleArgs 
 {
     __shared__ u64 hw[SAMPLE_BINS];
     __shared__ unsigned hc[SAMPLE_BINS];
+    __shared__ double table[64];
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     const RowPlan r = plan_row(a, row);
     if (!r.counts && !r.sums) return;
+    if (r.sums) load_table(table);
     const float *x = a.logits + (size_t)row * a.vocab;
-    const int end = min(a.vocab, (s + 1) * a.per);
+    const int per = SAMPLE_WAVES * a.run, end = min(a.vocab, (s + 1) * per);
     for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
         hw[b] = 0;
         hc[b] = 0;
     }
     __syncthreads();
-    for (int i = s * a.per + t; i < end; i += 4 * SAMPLE_THREADS) {
-        float v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = x[min(i + u * SAMPLE_THREADS, end - 1)];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int b = bin_of(v[u], r.st);
-            if (i + u * SAMPLE_THREADS >= end || b >= SAMPLE_BINS) continue;
-            if (r.counts) atomicAdd(hc + b, 1u);
-            if (r.sums) atomicAdd(hw + b, fixed(weight(v[u], r.st), r.st));
-        }
-    }
+    each_value(x, s * per, end, t, SAMPLE_THREADS, [&](float v, int) {
+        const int b = bin_of(v, r.st);
+        if (b >= SAMPLE_BINS) return;
+        if (r.counts) atomicAdd(hc + b, 1u);
+        if (r.sums) atomicAdd(hw + b, fixed(weight(v, r.st, table), r.st));
+    });
     __syncthreads();
     const size_t at = ((size_t)row * a.splits + s) * SAMPLE_BINS;
     for (int b = t; b < SAMPLE_BINS; b += SAMPLE_THREADS) {
@@ -307,33 +337,31 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_bins_kernel(SampleArgs 
     }
 }
 
-// ---- sums ----
-__global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs a)
+// ---- find ----
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_find_kernel(SampleArgs a)
 {
     __shared__ u64 wsum[SAMPLE_WAVES];
     __shared__ Found f;
-    __shared__ unsigned listed[2], base[2];
-    __shared__ u64 list[2][SAMPLE_LIST];
-    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int row = blockIdx.x, t = threadIdx.x;
     const RowPlan r = plan_row(a, row);
     if (r.greedy) return;
-    if (t == 0) {
-        f = Found{SAMPLE_BINS, SAMPLE_BINS, -1, 0, 0, 0, 0, 0, 0}; // nothing cut: all bins summed
-        listed[0] = listed[1] = 0;
-    }
+    if (t == 0) f = Found{SAMPLE_BINS, SAMPLE_BINS, -1, 0, 0, 0, 0, 0, 0}; // nothing cut: all bins summed
     if (r.counts || r.sums) {
         // this thread's two bins over all splits, and their running totals
         u64 c0 = 0, c1 = 0, w0 = 0, w1 = 0, ctotal = 0, wtotal = 0;
         const size_t at = (size_t)row * a.splits * SAMPLE_BINS + 2 * t;
+        if (r.counts) {
 #pragma unroll 8
-        for (int i = 0; i < a.splits; ++i) {
-            if (r.counts) {
+            for (int i = 0; i < a.splits; ++i) {
                 const uint2 c =
                     *reinterpret_cast<const uint2 *>(a.count + at + (size_t)i * SAMPLE_BINS);
                 c0 += c.x;
                 c1 += c.y;
             }
-            if (r.sums) {
+        }
+        if (r.sums) {
+#pragma unroll 8
+            for (int i = 0; i < a.splits; ++i) {
                 const ulonglong2 w =
                     *reinterpret_cast<const ulonglong2 *>(a.wsum + at + (size_t)i * SAMPLE_BINS);
                 w0 += w.x;
@@ -397,42 +425,44 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
         }
     }
     __syncthreads();
-    const Found g = f;
-    if (s == 0 && t == 0) a.found[row] = g;
+    if (t == 0) a.found[row] = f;
+}
 
+// ---- sums ----
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs a)
+{
+    __shared__ unsigned listed[2], base[2];
+    __shared__ u64 list[2][SAMPLE_LIST];
+    __shared__ double table[64];
+    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const RowPlan r = plan_row(a, row);
+    if (r.greedy) return;
+    const Found g = a.found[row];
+    if (t < 2) listed[t] = 0;
+    load_table(table);
     const float *x = a.logits + (size_t)row * a.vocab;
-    const int end = min(a.vocab, (s + 1) * a.per);
+    const int begin = min(a.vocab, (s * SAMPLE_WAVES + wave) * a.run);
+    const int end = min(a.vocab, begin + a.run);
     u64 sum = 0;
-    for (int i = s * a.per + t; i < end; i += 4 * SAMPLE_THREADS) {
-        float v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = x[min(i + u * SAMPLE_THREADS, end - 1)];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = i + u * SAMPLE_THREADS, b = bin_of(v[u], r.st);
-            if (j >= end || b >= SAMPLE_BINS) continue;
-            if (b < g.lo) {
-                const double w = weight(v[u], r.st);
-                if (w >= r.st.min_p) sum += fixed(w, r.st);
-            }
-            const int which = b >= g.lo && b <= g.hi ? 0 : b == g.kbin ? 1 : -1;
-            if (which >= 0) {
-                const unsigned n = atomicAdd(listed + which, 1u);
-                if (n < SAMPLE_LIST)
-                    list[which][n] = (u64)order_key(v[u]) << 32 | (unsigned)~j;
-            }
+    each_value(x, begin, end, lane, 64, [&](float v, int j) {
+        const int b = bin_of(v, r.st);
+        if (b >= SAMPLE_BINS) return;
+        if (b < g.lo) {
+            const double w = weight(v, r.st, table);
+            if (w >= r.st.min_p) sum += fixed(w, r.st);
         }
-    }
+        const int which = b >= g.lo && b <= g.hi ? 0 : b == g.kbin ? 1 : -1;
+        if (which >= 0) {
+            const unsigned n = atomicAdd(listed + which, 1u);
+            if (n < SAMPLE_LIST) list[which][n] = (u64)order_key(v) << 32 | (unsigned)~j;
+        }
+    });
     sum = wave_sum(sum);
+    if (lane == 0) a.sums[((size_t)row * a.splits + s) * SAMPLE_WAVES + wave] = sum;
     __syncthreads();
-    if (lane == 0) wsum[wave] = sum;
     if (t < 2) base[t] = listed[t] ? atomicAdd(a.have + 2 * row + t, listed[t]) : 0;
     __syncthreads();
-    if (t == 0) {
-        u64 all = 0;
-        for (int w = 0; w < SAMPLE_WAVES; ++w) all += wsum[w];
-        a.sums[row * a.splits + s] = all;
-    }
+#pragma unroll 1
     for (int which = 0; which < 2; ++which)
         for (unsigned n = t; n < min(listed[which], (unsigned)SAMPLE_LIST); n += SAMPLE_THREADS)
             if (base[which] + n < SAMPLE_LIST)
@@ -440,27 +470,6 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
 }
 
 // ---- draw ----
-// Sorts n <= SAMPLE_LIST keys in LDS, largest first.
-__device__ __forceinline__ void sort_desc(u64 *key, int n)
-{
-    int size = 64;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) key[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int e = threadIdx.x; e < size / 2; e += SAMPLE_THREADS) {
-                const int lo = 2 * e - (e & (j - 1)), hi = lo + j;
-                const u64 x = key[lo], y = key[hi];
-                if ((x < y) == ((lo & k) == 0)) {
-                    key[lo] = y;
-                    key[hi] = x;
-                }
-            }
-            __syncthreads();
-        }
-}
-
 __device__ __forceinline__ float value_of(u64 key) // the float of an order key
 {
     const unsigned k = (unsigned)(key >> 32);
@@ -468,8 +477,9 @@ __device__ __forceinline__ float value_of(u64 key) // the float of an order key
 }
 
 // The whole row by one workgroup (see the head of the file).
-__device__ __noinline__ void row_alone(const SampleArgs &a, const RowPlan &plan, int row,
-                                       u64 *hw, unsigned *hc, u64 *wsum, u64 *pick)
+__device__ __forceinline__ void row_alone(const SampleArgs &a, const RowPlan &plan, int row,
+                                          const double *table, u64 *hw, unsigned *hc, u64 *wsum,
+                                          u64 *pick)
 {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, vocab = a.vocab, k = plan.k;
     const float *x = a.logits + (size_t)row * vocab;
@@ -485,7 +495,7 @@ __device__ __noinline__ void row_alone(const SampleArgs &a, const RowPlan &plan,
         const int b = bin_of(v, st);
         if (b < SAMPLE_BINS) {
             atomicAdd(hc + b, 1u);
-            atomicAdd(hw + b, fixed(weight(v, st), st));
+            atomicAdd(hw + b, fixed(weight(v, st, table), st));
         }
     }
     __syncthreads();
@@ -516,7 +526,7 @@ __device__ __noinline__ void row_alone(const SampleArgs &a, const RowPlan &plan,
                 if (level && (key >> (sh + 8)) != prefix) continue;
                 if (bin_of(v, st) != b) continue;
                 atomicAdd(hc + ((key >> sh) & 255), 1u);
-                atomicAdd(hw + ((key >> sh) & 255), fixed(weight(v, st), st));
+                atomicAdd(hw + ((key >> sh) & 255), fixed(weight(v, st, table), st));
             }
             __syncthreads();
             if (t == 0) {
@@ -594,7 +604,7 @@ __device__ __noinline__ void row_alone(const SampleArgs &a, const RowPlan &plan,
         const unsigned key = order_key(v);
         if (key < cut.key || (key == cut.key && i > cut.last)) return 0;
         if (bin_of(v, st) >= SAMPLE_BINS) return 0;
-        const double w = weight(v, st);
+        const double w = weight(v, st, table);
         return w >= st.min_p ? fixed(w, st) : 0;
     };
     int lo = 0, hi = vocab;
@@ -629,7 +639,7 @@ __device__ __noinline__ void row_alone(const SampleArgs &a, const RowPlan &plan,
                     a.token[row] = b + lane;
                     if (a.prob)
                         a.prob[row] =
-                            (float)(weight(x[b + lane], st) * st.scale / (double)whole);
+                            (float)(weight(x[b + lane], st, table) * st.scale / (double)whole);
                 }
                 break;
             }
@@ -639,15 +649,139 @@ __device__ __noinline__ void row_alone(const SampleArgs &a, const RowPlan &plan,
 }
 
 
+// Cuts a list in LDS, by a workgroup: finds the smallest key of the order's
+// shortest prefix that has `count` members or the weight `target` (the other
+// one is unbounded); at most all n members. *weight_of: that prefix's weight.
+// Digits of 8 bits, largest first: a histogram of the members that share the
+// digits so far, of which one wave finds the digit where the prefix ends, until
+// one member is left.
+struct ListScratch {
+    u64 hw[256];
+    unsigned hc[256];
+    u64 out[4]; // digit, members before it, weight before it, members in it
+};
+__device__ __forceinline__ u64 cut_list(const u64 *key, const u64 *w, int n, u64 count, u64 target,
+                                        ListScratch &l, u64 *weight_of)
+{
+    const int t = threadIdx.x, lane = t & 63;
+    // keys relative to the smallest, from the highest bit in which they differ
+    // (members of few bins share theirs: a first digit of one value would be a
+    // histogram of one bin)
+    u64 kmin = ~(u64)0, kmax = 0;
+    for (int i = t; i < n; i += SAMPLE_THREADS) {
+        kmin = min(kmin, key[i]);
+        kmax = max(kmax, key[i]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        kmin = min(kmin, (u64)__shfl_xor(kmin, o, 64));
+        kmax = max(kmax, (u64)__shfl_xor(kmax, o, 64));
+    }
+    __syncthreads();
+    if (t == 0) {
+        l.out[0] = ~(u64)0;
+        l.out[1] = 0;
+    }
+    __syncthreads();
+    if (lane == 0 && t < n) {
+        atomicMin(l.out, kmin);
+        atomicMax(l.out + 1, kmax);
+    }
+    __syncthreads();
+    kmin = l.out[0];
+    kmax = l.out[1] - kmin;
+    const int top = max(0, (kmax ? 63 - __clzll((long long)kmax) : 0) - 7);
+    u64 prefix = 0, before = 0, wbefore = 0;
+    int last = top + 8; // the bits from here on are `prefix`
+    for (int sh = top;; sh = max(0, sh - 8)) {
+        __syncthreads();
+        if (t < 256) {
+            l.hw[t] = 0;
+            l.hc[t] = 0;
+        }
+        __syncthreads();
+        for (int i = t; i < n; i += SAMPLE_THREADS)
+            if (const u64 k = key[i] - kmin; sh == top || k >> last == prefix) {
+                const int d = (int)((k >> sh) & ((1u << (last - sh)) - 1));
+                atomicAdd(l.hc + d, 1u);
+                atomicAdd(l.hw + d, w[i]);
+            }
+        __syncthreads();
+        if (t < 64) { // lane: digits 255 - 4 lane .. 252 - 4 lane
+            u64 c[4], v[4], cs = 0, vs = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                cs += c[i] = l.hc[255 - 4 * lane - i];
+                vs += v[i] = l.hw[255 - 4 * lane - i];
+            }
+            u64 cb = before + wave_scan(cs, lane) - cs, vb = wbefore + wave_scan(vs, lane) - vs;
+            // the digit that reaches the cut, else the last that has members
+            int at = -1;
+            u64 ac = 0, av = 0, am = 0;
+            bool ends = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!ends && c[i]) {
+                    at = 255 - 4 * lane - i;
+                    ac = cb;
+                    av = vb;
+                    am = c[i];
+                    ends = cb + c[i] >= count || vb + v[i] >= target;
+                }
+                cb += c[i];
+                vb += v[i];
+            }
+            const u64 end = __ballot(ends), any = __ballot(at >= 0);
+            const int pick = end ? __ffsll((long long)end) - 1 : 63 - __clzll((long long)any);
+            if (lane == pick) {
+                l.out[0] = at;
+                l.out[1] = ac;
+                l.out[2] = av;
+                l.out[3] = am;
+            }
+        }
+        __syncthreads();
+        prefix = prefix << (last - sh) | l.out[0];
+        before = l.out[1];
+        wbefore = l.out[2];
+        last = sh;
+        if (l.out[3] == 1 || sh == 0) { // one member left (keys differ): it is the cut
+            for (int i = t; i < n; i += SAMPLE_THREADS)
+                if ((key[i] - kmin) >> sh == prefix) {
+                    l.hw[0] = key[i];
+                    l.hw[1] = w[i];
+                }
+            __syncthreads();
+            prefix = l.hw[0];
+            *weight_of = wbefore + l.hw[1];
+            __syncthreads();
+            return prefix;
+        }
+    }
+}
+
+// A list of at most 64 members by one wave, a member per lane: the members
+// with larger keys are counted and weighed by readlane.
+__device__ __forceinline__ u64 lane64(u64 v, int l)
+{
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)v, l);
+}
+
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_draw_kernel(SampleArgs a)
 {
-    __shared__ u64 hw[SAMPLE_BINS];
-    __shared__ unsigned hc[SAMPLE_BINS];
-    __shared__ u64 wsum[SAMPLE_WAVES];
-    __shared__ u64 pick[4];
-    __shared__ u64 split_sum[SAMPLE_SPLITS];
-    __shared__ u64 key[SAMPLE_LIST];
+    __shared__ u64 key[SAMPLE_LIST], lw[SAMPLE_LIST]; // a list's keys and weights
+    __shared__ ListScratch ls;
+    __shared__ u64 wsum[SAMPLE_WAVES], pick[4];
+    __shared__ u64 run_sum[SAMPLE_SPLITS * SAMPLE_WAVES];
+    __shared__ double table[64];
+    static_assert(SAMPLE_SPLITS * SAMPLE_WAVES <= SAMPLE_THREADS, "a run per thread");
     const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const Found f = a.found[row];
+    const unsigned n0 = a.have[2 * row], n1 = a.have[2 * row + 1];
+    const u64 *lists = a.list + (size_t)row * 2 * SAMPLE_LIST;
+    const u64 first_key = lists[lane]; // (of list 0: a small list's members)
+    const float random = a.random[row];
     const RowPlan r = plan_row(a, row);
     if (r.greedy) { // the first maximum, or nothing to take
         if (t == 0) {
@@ -658,114 +792,115 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_draw_kernel(SampleArgs 
         return;
     }
     const RowSettings &st = r.st;
-    const Found f = a.found[row];
-    const unsigned n0 = a.have[2 * row], n1 = a.have[2 * row + 1];
+    load_table(table);
     if (n0 > SAMPLE_LIST || n1 > SAMPLE_LIST) {
-        row_alone(a, r, row, hw, hc, wsum, pick);
+        static_assert(SAMPLE_LIST >= SAMPLE_BINS, "its histograms' place");
+        row_alone(a, r, row, table, key, (unsigned *)lw, wsum, pick);
         return;
     }
-    const u64 *lists = a.list + (size_t)row * 2 * SAMPLE_LIST;
-    // a thread's members 2 t and 2 t + 1 of a sorted list, and the running
-    // weight before them
-    auto load = [&](int which, int n) {
-        for (int i = t; i < n; i += SAMPLE_THREADS) key[i] = lists[which * SAMPLE_LIST + i];
-        __syncthreads();
-        sort_desc(key, n);
-    };
-    auto weight_at = [&](int i, int n) -> u64 {
-        return i < n ? fixed(weight(value_of(key[i]), st), st) : 0;
-    };
-    // the weight that top-p is of
-    u64 of = f.total;
-    if (f.kbin >= 0) {
-        load(1, n1);
-        const int n = min((int)n1, r.k - (int)f.kbefore);
-        u64 all;
-        block_scan(weight_at(2 * t, n) + weight_at(2 * t + 1, n), wsum, &all);
-        of = f.kwbefore + all;
-        __syncthreads();
-    }
-    // the members kept by top-k and top-p: the first `kept`
-    int kept = (int)n0;
-    u64 w0 = 0, w1 = 0;
-    if (n0) {
-        load(0, n0);
-        if (f.k_in_list) kept = min(kept, r.k - (int)f.before);
-        w0 = weight_at(2 * t, kept);
-        w1 = weight_at(2 * t + 1, kept);
-        if (r.by_p) {
-            u64 all;
-            const u64 up = block_scan(w0 + w1, wsum, &all);
-            if (f.k_in_list) of = f.wbefore + all;
-            const u64 target = top_p_target(r.p, max(of, (u64)1));
-            const u64 b = f.wbefore + up - w0 - w1;
-            if (t == 0) pick[0] = kept;
-            __syncthreads();
-            if (b < target && b + w0 + w1 >= target) pick[0] = 2 * t + (b + w0 < target ? 2 : 1);
-            __syncthreads();
-            kept = (int)pick[0];
+    if (f.lo == 0 && f.kbin < 0 && n0 <= 64) { // every kept value is in a list of a wave
+        if (wave) return;
+        const int n = n0;
+        const bool in = lane < n;
+        const u64 k = in ? first_key : 0;
+        const double wd = in ? weight(value_of(k), st, table) : 0.0;
+        u64 w = fixed(wd, st);
+        int rank = 0;
+        u64 before = 0;
+        for (int j = 0; j < n; ++j) {
+            const bool larger = lane64(k, j) > k;
+            rank += larger;
+            before += larger ? lane64(w, j) : 0;
         }
-    }
-    // the kept members' weights to their splits
-    if (t < a.splits) split_sum[t] = a.sums[row * a.splits + t];
-    __syncthreads();
+        bool keep = in && (!f.k_in_list || rank < r.k);
+        const u64 of = f.k_in_list ? wave_sum(keep ? w : 0) : f.total;
+        if (r.by_p) keep = keep && before < top_p_target(r.p, of);
+        keep = keep && wd >= st.min_p;
+        w = keep ? w : 0;
+        const u64 whole = wave_sum(w), target = draw_target(random, whole);
+        u64 upto = 0; // the kept weights up to this index
+        for (int j = 0; j < n; ++j)
+            upto += (unsigned)lane64(k, j) >= (unsigned)k ? lane64(w, j) : 0;
+        int token = keep && upto >= target ? (int)~(unsigned)k : 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int j = 2 * t + i;
-        if (j >= kept || (int)n0 <= j) continue;
-        if (weight(value_of(key[j]), st) >= st.min_p)
-            atomicAdd(split_sum + (int)(~(unsigned)key[j]) / a.per, i ? w1 : w0);
+        for (int o = 32; o > 0; o >>= 1) token = min(token, __shfl_xor(token, o, 64));
+        if (in && (int)~(unsigned)k == token) {
+            a.token[row] = token;
+            if (a.prob) a.prob[row] = (float)(wd * st.scale / (double)whole);
+        }
+        return;
+    }
+    // First the weight that top-p is of, where the top-k's cut lies behind the
+    // list that top-p cuts; then the top-k's cut in that list, then top-p's.
+    // kept: the keys from `last` on. (One place in the code for the three cuts.)
+    u64 of = f.total, last = 0;
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+        const int n = step ? n0 : n1;
+        if (step < 2 && (step || f.kbin >= 0)) { // (a list and its weights)
+            __syncthreads();
+            for (int i = t; i < n; i += SAMPLE_THREADS) {
+                key[i] = lists[(step ? 0 : 1) * SAMPLE_LIST + i];
+                lw[i] = fixed(weight(value_of(key[i]), st, table), st);
+            }
+            __syncthreads();
+        }
+        if (n == 0 || !(step == 0 ? f.kbin >= 0 : step == 1 ? f.k_in_list : r.by_p)) continue;
+        constexpr u64 ALL = ~(u64)0;
+        u64 in;
+        const u64 cut = cut_list(key, lw, n,
+                                 step == 0 ? r.k - f.kbefore : step == 1 ? r.k - f.before : ALL,
+                                 step < 2 ? ALL : top_p_target(r.p, max(of, (u64)1)) - f.wbefore, ls,
+                                 &in);
+        if (step < 2) of = (step ? f.wbefore : f.kwbefore) + in;
+        if (step) last = max(last, cut);
+    }
+    // the kept members' weights to their runs
+    const int runs = a.splits * SAMPLE_WAVES;
+    if (t < runs) run_sum[t] = a.sums[(size_t)row * runs + t];
+    __syncthreads();
+    for (int i = t; i < (int)n0; i += SAMPLE_THREADS)
+        if (key[i] >= last && weight(value_of(key[i]), st, table) >= st.min_p)
+            atomicAdd(run_sum + (int)(~(unsigned)key[i]) / a.run, lw[i]);
+    __syncthreads();
+    // the run that holds the target, and the token in it
+    u64 whole;
+    const u64 mine = t < runs ? run_sum[t] : 0, upto = block_scan(mine, wsum, &whole);
+    const u64 target = draw_target(random, whole);
+    if (upto >= target && upto - mine < target) {
+        pick[0] = t;
+        pick[1] = upto - mine;
     }
     __syncthreads();
-    // the split that holds the target, and the token in it
-    const u64 mine_s = lane < a.splits ? split_sum[lane] : 0, upto_s = wave_scan(mine_s, lane);
-    const u64 whole = __shfl(upto_s, 63, 64);
-    const u64 target = draw_target(a.random[row], whole);
-    const int s = min(__ffsll((long long)__ballot(upto_s >= target)) - 1, a.splits - 1);
-    u64 before = __shfl(upto_s - mine_s, s, 64);
-    const u64 last = n0 && kept ? key[kept - 1] : 0; // kept: this key and larger ones
     const float *x = a.logits + (size_t)row * a.vocab;
-    auto kept_weight = [&](int i) -> u64 {
-        const float v = x[i];
-        const int b = bin_of(v, st);
-        if (b >= SAMPLE_BINS || b > f.hi) return 0;
-        if (b >= f.lo && (kept == 0 || ((u64)order_key(v) << 32 | (unsigned)~i) < last)) return 0;
-        const double w = weight(v, st);
-        return w >= st.min_p ? fixed(w, st) : 0;
-    };
-    const int begin = s * a.per, end = min(a.vocab, begin + a.per);
-    // by runs of a wave: 64 consecutive values a step
-    const int run = ((end - begin + SAMPLE_WAVES - 1) / SAMPLE_WAVES + 63) / 64 * 64;
-    const int i0 = begin + wave * run, i1 = min(end, i0 + run);
-    u64 mine = 0;
-    for (int i = i0 + lane; i < i1; i += 64) mine += kept_weight(i);
-    mine = wave_sum(mine);
-    if (lane == 0) wsum[wave] = mine;
-    __syncthreads();
-    const u64 mine_w = lane < SAMPLE_WAVES ? wsum[lane] : 0;
-    const u64 upto_w = before + wave_scan(mine_w, lane);
-    const int w = __ffsll((long long)__ballot(upto_w >= target)) - 1;
-    if (wave != w) return;
-    before = __shfl(upto_w - mine_w, w, 64);
-    for (int b = i0; b < i1; b += 64) {
-        const u64 v = b + lane < i1 ? kept_weight(b + lane) : 0;
-        const u64 upto = before + wave_scan(v, lane);
-        const u64 hit = __ballot(upto >= target);
-        if (hit) {
-            const int at = __ffsll((long long)hit) - 1;
-            if (lane == at) {
-                a.token[row] = b + lane;
-                if (a.prob)
-                    a.prob[row] = (float)(weight(x[b + lane], st) * st.scale / (double)whole);
+    const int begin = (int)pick[0] * a.run, end = min(a.vocab, begin + a.run);
+    u64 before = pick[1];
+#pragma unroll 1
+    for (int b = begin; b < end; b += SAMPLE_THREADS) {
+        const int i = b + t;
+        u64 w = 0, all;
+        double wd = 0.0;
+        if (i < end) {
+            const float v = x[i];
+            const int bin = bin_of(v, st);
+            if (bin < SAMPLE_BINS && bin <= f.hi &&
+                (bin < f.lo || ((u64)order_key(v) << 32 | (unsigned)~i) >= last)) {
+                wd = weight(v, st, table);
+                if (wd >= st.min_p) w = fixed(wd, st);
             }
-            break;
         }
-        before = __shfl(upto, 63, 64);
+        const u64 up = before + block_scan(w, wsum, &all);
+        if (up >= target && up - w < target) {
+            a.token[row] = i;
+            if (a.prob) a.prob[row] = (float)(wd * st.scale / (double)whole);
+        }
+        before += all;
+        if (before >= target) break;
     }
 }
 
 struct SampleLayout {
-    int splits, per;
+    int splits, run;
     size_t sidx, count, wsum, sums, found, have, list, bytes;
 };
 // Splits: as many workgroups as fill the GPU twice, but at most 32 (each
@@ -776,14 +911,15 @@ SampleLayout sample_layout(int rows, int vocab)
     SampleLayout l;
     const int most = (vocab + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
     l.splits = std::max(1, std::min({512 / rows, SAMPLE_SPLITS, most}));
-    l.per = (vocab + l.splits - 1) / l.splits;
+    const int runs = l.splits * SAMPLE_WAVES;
+    l.run = ((vocab + runs - 1) / runs + 63) / 64 * 64;
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     const size_t n = (size_t)rows * l.splits;
     l.sidx = up(n * 4);
     l.count = l.sidx + up(n * 4);
     l.wsum = l.count + n * SAMPLE_BINS * 4;
     l.sums = l.wsum + n * SAMPLE_BINS * 8;
-    l.found = l.sums + up(n * 8);
+    l.found = l.sums + up(n * SAMPLE_WAVES * 8);
     l.have = l.found + up(rows * sizeof(Found));
     l.list = l.have + up((size_t)rows * 8);
     l.bytes = l.list + (size_t)rows * 2 * SAMPLE_LIST * 8;
@@ -808,7 +944,7 @@ int launch_sample(const float *logits, int rows, int vocab, const float *tempera
     a.vocab = vocab;
     a.shift = std::min(46, 62 - bits);
     a.splits = l.splits;
-    a.per = l.per;
+    a.run = l.run;
     a.temperature = temperature;
     a.top_k = top_k;
     a.top_p = top_p;
@@ -828,6 +964,7 @@ int launch_sample(const float *logits, int rows, int vocab, const float *tempera
     const dim3 grid(l.splits, rows), block(SAMPLE_THREADS);
     hipLaunchKernelGGL(sample_max_kernel, grid, block, 0, st, a);
     hipLaunchKernelGGL(sample_bins_kernel, grid, block, 0, st, a);
+    hipLaunchKernelGGL(sample_find_kernel, dim3(rows), block, 0, st, a);
     hipLaunchKernelGGL(sample_sums_kernel, grid, block, 0, st, a);
     hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), block, 0, st, a);
     return (int)hipGetLastError();
