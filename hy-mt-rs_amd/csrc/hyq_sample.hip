@@ -169,7 +169,6 @@ struct SampleArgs {
     float *prob;
     // scratch
     float *smax;     // [rows][splits]
-    int *sidx;       // [rows][splits]: the split's first maximum
     unsigned *count; // [rows][splits][SAMPLE_BINS]
     u64 *wsum;       // [rows][splits][SAMPLE_BINS]
     u64 *sums;       // [rows][splits][16]: a run's weight in the bins before the listed ones
@@ -194,7 +193,7 @@ struct RowPlan {
     bool by_k, by_p;    // which filters cut
     bool counts, sums;  // which histograms they need
     float max;
-    int first;          // index of the first maximum
+    int split;          // the first split that holds the maximum
     int k;
     double p;
     RowSettings st;
@@ -207,10 +206,8 @@ __device__ __forceinline__ RowPlan plan_row(const SampleArgs &a, int row)
     RowPlan r;
     const int lane = threadIdx.x & 63, at = row * a.splits + min(lane, a.splits - 1);
     const float m = a.smax[at];
-    const int idx = a.sidx[at];
     r.max = wave::max64(m);
-    // (splits ascend: the first lane of the maximum has its first index)
-    r.first = __builtin_amdgcn_readlane(idx, __ffsll((long long)__ballot(m == r.max)) - 1);
+    r.split = __ffsll((long long)__ballot(m == r.max)) - 1;
     const float temp = a.temperature[row];
     r.greedy = !(r.max > -INFINITY) || !(temp > 0.f);
     r.k = a.top_k[row];
@@ -247,62 +244,64 @@ __device__ __forceinline__ u64 draw_target(float random, u64 total)
 // f(value, index) for a thread's values of [begin, end): eight loads in flight,
 // then one call at a time from one place in the code. (A launch starts with a
 // cold instruction cache: f's 64-bit exponential is not fetched eight times over.)
+// Values below `floor`, and NaNs, are left out: where a wave's are all so, as
+// most are when few can be kept, a step is its loads and a comparison each.
 template <class F>
 __device__ __forceinline__ void each_value(const float *x, int begin, int end, int first, int step,
-                                           F f)
+                                           float floor, F f)
 {
     for (int i = begin + first; i < end; i += 8 * step) {
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = x[min(i + u * step, end - 1)];
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) any |= v[u] >= floor;
+        if (!any) continue;
 #pragma unroll 1
         for (int j = i; j < min(end, i + 8 * step); j += step) {
-            f(v[0], j);
+            if (v[0] >= floor) f(v[0], j);
 #pragma unroll
             for (int u = 0; u < 7; ++u) v[u] = v[u + 1];
         }
     }
 }
 
+// A value below which bins are larger than `hi`: the border of hi + 1, less
+// what the rounding of bin_of's difference and product can move it by.
+__device__ __forceinline__ float bin_floor(int hi, const RowSettings &s)
+{
+    if (s.max == INFINITY) return s.max;
+    const float d = (float)(hi + 1) / s.per_bin;
+    const float f = s.max - d;
+    return f - (fabsf(s.max) + d) * 1e-6f;
+}
+
 // ---- max ----
+// (v_max ignores a NaN)
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_max_kernel(SampleArgs a)
 {
     __shared__ float sm[SAMPLE_WAVES];
-    __shared__ int si[SAMPLE_WAVES];
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     const float *x = a.logits + (size_t)row * a.vocab;
     const int per = SAMPLE_WAVES * a.run, end = min(a.vocab, (s + 1) * per);
     float mx = -INFINITY;
-    int mi = 0x7fffffff;
-    each_value(x, s * per, end, t, SAMPLE_THREADS, [&](float v, int i) {
-        if (v > mx) {
-            mx = v;
-            mi = i;
-        }
-    });
+    for (int i = s * per + t; i < end; i += 8 * SAMPLE_THREADS) {
+        float v[8];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float v = __shfl_xor(mx, o, 64);
-        const int i = __shfl_xor(mi, o, 64);
-        if (v > mx || (v == mx && i < mi)) {
-            mx = v;
-            mi = i;
-        }
+        for (int u = 0; u < 8; ++u) v[u] = x[min(i + u * SAMPLE_THREADS, end - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mx = fmaxf(mx, v[u]);
     }
-    if ((t & 63) == 0) {
-        sm[t >> 6] = mx;
-        si[t >> 6] = mi;
-    }
+    mx = wave::max64(mx);
+    if ((t & 63) == 0) sm[t >> 6] = mx;
     __syncthreads();
-    if (t == 0) {
-        for (int w = 1; w < SAMPLE_WAVES; ++w)
-            if (sm[w] > mx || (sm[w] == mx && si[w] < mi)) {
-                mx = sm[w];
-                mi = si[w];
-            }
-        a.smax[row * a.splits + s] = mx;
-        a.sidx[row * a.splits + s] = mi;
-        if (s == 0) a.have[2 * row] = a.have[2 * row + 1] = 0;
+    if (t < 64) {
+        mx = wave::max64(sm[t & (SAMPLE_WAVES - 1)]);
+        if (t == 0) {
+            a.smax[row * a.splits + s] = mx;
+            if (s == 0) a.have[2 * row] = a.have[2 * row + 1] = 0;
+        }
     }
 }
 
@@ -323,7 +322,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_bins_kernel(SampleArgs 
         hc[b] = 0;
     }
     __syncthreads();
-    each_value(x, s * per, end, t, SAMPLE_THREADS, [&](float v, int) {
+    each_value(x, s * per, end, t, SAMPLE_THREADS, bin_floor(SAMPLE_BINS - 1, r.st), [&](float v, int) {
         const int b = bin_of(v, r.st);
         if (b >= SAMPLE_BINS) return;
         if (r.counts) atomicAdd(hc + b, 1u);
@@ -444,7 +443,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
     const int begin = min(a.vocab, (s * SAMPLE_WAVES + wave) * a.run);
     const int end = min(a.vocab, begin + a.run);
     u64 sum = 0;
-    each_value(x, begin, end, lane, 64, [&](float v, int j) {
+    each_value(x, begin, end, lane, 64, bin_floor(min(max(g.hi, g.kbin), SAMPLE_BINS - 1), r.st), [&](float v, int j) {
         const int b = bin_of(v, r.st);
         if (b >= SAMPLE_BINS) return;
         if (b < g.lo) {
@@ -784,9 +783,27 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_draw_kernel(SampleArgs 
     const float random = a.random[row];
     const RowPlan r = plan_row(a, row);
     if (r.greedy) { // the first maximum, or nothing to take
+        const bool any = r.max > -INFINITY;
+        if (t == 0) pick[0] = 0x7fffffff;
+        __syncthreads();
+        if (any) {
+            const int per = SAMPLE_WAVES * a.run, end = min(a.vocab, (r.split + 1) * per);
+            int first = 0x7fffffff;
+            for (int i = r.split * per + t; i < end; i += 8 * SAMPLE_THREADS) {
+                float v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    v[u] = a.logits[(size_t)row * a.vocab + min(i + u * SAMPLE_THREADS, end - 1)];
+#pragma unroll
+                for (int u = 7; u >= 0; --u) // (past the end: the last value again)
+                    if (v[u] == r.max)
+                        first = min(first, min(i + u * SAMPLE_THREADS, end - 1));
+            }
+            if (first != 0x7fffffff) atomicMin(pick, (u64)first);
+        }
+        __syncthreads();
         if (t == 0) {
-            const bool any = r.max > -INFINITY;
-            a.token[row] = any ? r.first : -1;
+            a.token[row] = any ? (int)pick[0] : -1;
             if (a.prob) a.prob[row] = any ? 1.f : 0.f;
         }
         return;
@@ -901,7 +918,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_draw_kernel(SampleArgs 
 
 struct SampleLayout {
     int splits, run;
-    size_t sidx, count, wsum, sums, found, have, list, bytes;
+    size_t count, wsum, sums, found, have, list, bytes;
 };
 // Splits: as many workgroups as fill the GPU twice, but at most 32 (each
 // workgroup of the third launch adds up all of a row's histograms) and none of
@@ -915,8 +932,7 @@ SampleLayout sample_layout(int rows, int vocab)
     l.run = ((vocab + runs - 1) / runs + 63) / 64 * 64;
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     const size_t n = (size_t)rows * l.splits;
-    l.sidx = up(n * 4);
-    l.count = l.sidx + up(n * 4);
+    l.count = up(n * 4);
     l.wsum = l.count + n * SAMPLE_BINS * 4;
     l.sums = l.wsum + n * SAMPLE_BINS * 8;
     l.found = l.sums + up(n * SAMPLE_WAVES * 8);
@@ -953,7 +969,6 @@ int launch_sample(const float *logits, int rows, int vocab, const float *tempera
     a.token = token;
     a.prob = prob;
     a.smax = (float *)base;
-    a.sidx = (int *)(base + l.sidx);
     a.count = (unsigned *)(base + l.count);
     a.wsum = (u64 *)(base + l.wsum);
     a.sums = (u64 *)(base + l.sums);
