@@ -3,20 +3,28 @@
 //
 // A workgroup takes the query rows of one KV head for a block of a slot's new
 // tokens - 128 rows, row r = token r / rep of the block, query head r % rep of
-// the group - and a range of 32-position tiles. Each of its four waves owns 32
-// rows and forms transposed products with v_mfma_f32_32x32x16_f16, so that a
-// lane holds one query row (lane % 32) and 16 of its positions or dims:
-//   S^T [32 pos x 32 rows]   = K_tile . Q^T
-//   O^T [128 dims x 32 rows] += V_tile^T . P^T
+// the group - and a range of 64-position steps. Wave w owns rows 32 (w % 4) ..
+// and of every step the 32 positions of its half w / 4; it forms transposed
+// products with v_mfma_f32_32x32x16_f16, so that a lane holds one query row
+// (lane % 32) and 16 of its positions or dims:
+//   S^T [32 pos x 32 rows]   = K . Q^T, lane (c, h): positions 8a + 4h + b
+//   O^T [128 dims x 32 rows] += V^T . P^T
 // with the softmax's running maximum and sum per lane (one exchange between
-// the row's two lanes). An f32 operand x is split into f16 parts hi = f16(x),
-// lo = f16(x - hi) and products sum hi.hi + lo.hi + hi.lo in f32, which keeps
-// the scores and sums near f32 accuracy; f16 pages are exact as they are and
-// need no low parts of keys and values. f32 pages hold values below 65504.
+// the row's two lanes). The second product takes its positions in the order in
+// which the lane holds them, so no weight moves between lanes. An f32 operand x
+// is split into f16 parts hi = f16(x), lo = f16(x - hi) and products sum
+// hi.hi + lo.hi + hi.lo in f32, which keeps the scores and sums near f32
+// accuracy; f16 pages are exact as they are and need no low parts of keys and
+// values. f32 pages hold values below 65504.
 //
-// Blocks of different slots and places see very different numbers of tiles, so
-// a plan cuts them: one workgroup counts every block's tiles and makes pieces
-// of about equal length, enough to fill the GPU, and the pieces of a block
+// Keys and values go through LDS, two steps of them, rows as they are (values
+// are transposed by ds_read_b64_tr_b16 on their way to the matrix operand).
+// The next step is converted and stored between the products of the present
+// one, and the step after it loaded, with one barrier a step.
+//
+// Blocks of different slots and places see very different numbers of steps, so
+// a plan cuts them: one workgroup counts every block's steps and makes pieces
+// of about equal length, enough to fill the GPU once, and the pieces of a block
 // that was cut leave partial rows, which a merge joins in order.
 #include <hip/hip_runtime.h>
 
@@ -33,13 +41,18 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 
 constexpr int PR_ROWS = 128;        // query rows per workgroup
-constexpr int PR_TILE = 32;         // positions per tile
-constexpr int PR_KP = KV_D + 8;     // K tile row pitch (halves)
-constexpr int PR_VP = PR_TILE + 8;  // V^T tile row pitch (halves)
-constexpr int PR_FILL = 512;        // workgroups that fill the GPU: two per CU
-constexpr int PR_MIN_TILES = 4;     // the shortest piece worth its partial rows
+constexpr int PR_TILE = 64;         // positions per step
+constexpr int PR_THREADS = 512;     // two waves on each SIMD
+// Row pitches in halves, chosen for the banks: keys are read 16 bytes a lane
+// from 16 rows (4 banks apart), values by the transposing read 8 bytes a lane
+// from 4 rows (16 banks apart).
+constexpr int PR_KP = KV_D + 8;
+constexpr int PR_VP = KV_D + 32;
+constexpr int PR_FILL = 256;        // workgroups that fill the GPU: one per CU
+constexpr int PR_MIN_TILES = 2;     // the shortest piece worth its partial rows
 
 // The plan in scratch: counts, the blocks, then the pieces.
 struct Block {
@@ -53,10 +66,12 @@ struct Plan {
 };
 
 int max_blocks(int seqs, int rows, int tq) { return rows / tq + std::min(seqs, rows); }
-// sum of ceil(n / each) with each >= kvh tiles / PR_FILL; a block that is cut
+// Pieces that fill the GPU with kvh workgroups each (at least one).
+__host__ __device__ inline int fill_pieces(int kvh) { return PR_FILL > kvh ? PR_FILL / kvh : 1; }
+// sum of ceil(n / each) with each >= 2 tiles / fill_pieces; a block that is cut
 // (n > each) has fewer than 2 n / each pieces
-int max_pieces(int blocks, int kvh) { return blocks + PR_FILL / kvh + 1; }
-int max_parts(int kvh) { return 2 * (PR_FILL / kvh + 1); }
+int max_pieces(int blocks, int kvh) { return blocks + fill_pieces(kvh); }
+int max_parts(int kvh) { return 2 * fill_pieces(kvh); }
 
 __device__ __forceinline__ int block_tiles(const SlotRows &r, int b, int tq)
 {
@@ -130,7 +145,13 @@ __global__ __launch_bounds__(1024) void paged_rows_plan_kernel(PagedKv kv, int f
         }
         tiles += scan1024(mine, before, wsum);
     }
-    const int each = max((long long)PR_MIN_TILES, (tiles * kv.kvh + PR_FILL - 1) / PR_FILL);
+    // Pieces of `each` tiles number fewer than count + tiles / each: no more than
+    // fill the GPU once, where the blocks alone are few (a second round of a
+    // few pieces would take as long as the first: 66 against 40 us for 544
+    // pieces on 512 places); where they are many, only blocks of twice their
+    // share are cut.
+    const int fill = fill_pieces(kv.kvh), room = max(fill - count, (fill + 1) / 2);
+    const int each = (int)max((long long)PR_MIN_TILES, (tiles + room - 1) / room);
     int npieces = 0, nparts = 0;
     for (int b = 0; b < count; b += 1024) {
         int s = 0, n = 0, k = 0, before, pbefore;
@@ -158,175 +179,233 @@ __device__ __forceinline__ f32x16 mfma(const half8 &a, const half8 &b, const f32
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ void split_f16(float x, _Float16 &hi, _Float16 &lo)
+// Two values' high and low f16 parts, both rounded to nearest: hi, and
+// x - hi (exact in f32) by one mixed-precision fma each.
+__device__ __forceinline__ void split2(float x, float y, half2 &hi, half2 &lo)
 {
-    hi = (_Float16)x;
-    lo = (_Float16)(x - (float)hi);
+    hi = __builtin_convertvector((float2v{x, y}), half2);
+    float a, b;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(b)
+        : "v"(hi), "v"(y));
+    lo = __builtin_convertvector((float2v{a, b}), half2);
 }
-__device__ __forceinline__ int fbits(float v) { return __builtin_bit_cast(int, v); }
-__device__ __forceinline__ float bitsf(int v) { return __builtin_bit_cast(float, v); }
+// Positions p .. p + 3 of 16 dims: lane i of 16 takes dim i of them all, its
+// address being that of row (i / 4), dims 4 (i % 4) ..
+__device__ __forceinline__ half4 read_transposed(const _Float16 *p)
+{
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(
+        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (__attribute__((address_space(3))) short4v *)const_cast<_Float16 *>(p)));
+}
 
-template <class T> struct Four;
-template <> struct Four<float> {
-    typedef float4 type;
-    static __device__ __forceinline__ void get(const float4 &v, float (&x)[4])
+// A vector at a uniform base and an unsigned 32-bit element offset (a scalar
+// base with a vector offset in the load: no 64-bit address per lane).
+template <class V, class T> __device__ __forceinline__ V at(const T *base, unsigned off)
+{
+    return *reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
+                                        (unsigned)(off * sizeof(T)));
+}
+
+// A step's keys and values on their way from memory to LDS: 512 threads, rows
+// of 16 bytes a lane.
+template <class T> struct Raw;
+template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
+    static constexpr int N = 4;
+    typedef float4 Vec;
+    Vec k[N], v[N];
+    static __device__ __forceinline__ int row(int t, int i) { return (t >> 5) + 16 * i; }
+    static __device__ __forceinline__ int group(int, int i) { return i; } // its 16 rows
+    static __device__ __forceinline__ int dim(int t) { return 4 * (t & 31); }
+    // whether a value is not finite; such values become zero
+    __device__ __forceinline__ bool clean()
     {
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        bool odd = false;
+        auto one = [&](float &x) {
+            const bool fine = fabsf(x) < INFINITY;
+            odd |= !fine;
+            x = fine ? x : 0.f;
+        };
+#pragma unroll
+        for (int i = 0; i < N; ++i) one(v[i].x), one(v[i].y), one(v[i].z), one(v[i].w);
+        return odd;
+    }
+    static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *lo, const float4 &x)
+    {
+        half2 a, b, c, d;
+        split2(x.x, x.y, a, b);
+        split2(x.z, x.w, c, d);
+        *reinterpret_cast<half4 *>(hi) = half4{a[0], a[1], c[0], c[1]};
+        *reinterpret_cast<half4 *>(lo) = half4{b[0], b[1], d[0], d[1]};
     }
 };
-template <> struct Four<_Float16> {
-    typedef half4 type;
-    static __device__ __forceinline__ void get(const half4 &v, float (&x)[4])
+template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
+    static constexpr int N = 2;
+    typedef half8 Vec;
+    Vec k[N], v[N];
+    static __device__ __forceinline__ int row(int t, int i) { return (t >> 4) + 32 * i; }
+    static __device__ __forceinline__ int group(int wave, int i) { return 2 * i + (wave >> 2); }
+    static __device__ __forceinline__ int dim(int t) { return 8 * (t & 15); }
+    __device__ __forceinline__ bool clean()
     {
+        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool fine = fabsf((float)v[i][e]) < INFINITY;
+                odd |= !fine;
+                v[i][e] = fine ? v[i][e] : (_Float16)0.f;
+            }
+        return odd;
     }
+    static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *, const half8 &x)
+    {
+        *reinterpret_cast<half8 *>(hi) = x;
+    }
+};
+
+template <bool LO> struct RowsLds { // one step
+    _Float16 khi[PR_TILE][PR_KP], klo[LO ? PR_TILE : 1][PR_KP];
+    _Float16 vhi[PR_TILE][PR_VP], vlo[LO ? PR_TILE : 1][PR_VP];
 };
 
 template <class T>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(
+__global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     PagedKv kv, int tq, const Plan *__restrict__ plan, const Block *__restrict__ blocks,
     const Piece *__restrict__ pieces, const float *__restrict__ q, float *__restrict__ part,
     float *__restrict__ out)
 {
     constexpr bool LO = sizeof(T) == 4; // low parts of keys and values
-    typedef typename Four<T>::type Vec;
-    __shared__ __align__(16) _Float16 Khi[PR_TILE][PR_KP];
-    __shared__ __align__(16) _Float16 Klo[LO ? PR_TILE : 1][PR_KP];
-    __shared__ __align__(16) _Float16 Vhi[KV_D][PR_VP];
-    __shared__ __align__(16) _Float16 Vlo[LO ? KV_D : 1][PR_VP];
+    typedef Raw<T> R;
+    constexpr int JOIN = 66; // a lane's words in the join of the two halves
+    __shared__ __align__(16) union {
+        RowsLds<LO> step[2];
+        float join[4][JOIN][64];
+    } lds;
     if ((int)blockIdx.y >= plan->pieces) return;
     const Piece piece = pieces[blockIdx.y];
     const Block blk = blocks[piece.block];
     const int kh = blockIdx.x, s = blk.slot;
     const SlotRows sr = slot_rows(kv, s);
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), part_of = wave >> 2, rows = wave & 3;
     const int rep = kv.heads / kv.kvh;
     const size_t hsize = (size_t)KV_D << kv.shift, psize = 2 * hsize * kv.kvh;
     const int pmask = (1 << kv.shift) - 1;
-    const float sc = 1.4426950408889634f * 0.08838834764831845f;
+    const float sc = 1.4426950408889634f * 0.08838834764831845f; // log2(e) / sqrt(128)
 
     const int tok0 = blk.index * tq;
-    const int first = sr.len - sr.n;            // position of the slot's first new row
+    const int first = sr.len - sr.n; // position of the slot's first new row
     const int toks = min(tq, sr.n - tok0);
     const int p_end = min(piece.t1 * PR_TILE, first + tok0 + toks);
+    const int p_begin = piece.t0 * PR_TILE;
+    const int all_see = first + tok0; // the last position that every row sees
+
+    // The pages of a step's four 16-position groups, -1 where none. Page ids
+    // come 64 at a time, one per lane. Rows past the end are loaded too, from
+    // the same page or, where there is none, from the pool's first: their
+    // weights are zero, and values that are not finite are cleared.
+    const int *entries = kv.table + (size_t)s * kv.stride;
+    int have = -64, ids = -1; // lane i: the slot's page have + i
+    struct Four {
+        int e[4];
+    };
+    auto pages_of = [&](int p0) {
+        Four f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = max(p0 + 16 * i, 0) >> kv.shift;
+            if (p - have >= 64 || p < have) {
+                have = p;
+                ids = entries[min(have + lane, kv.stride - 1)];
+            }
+            const int e = __builtin_amdgcn_readlane(ids, p - have);
+            f.e[i] = p0 + 16 * i < p_end && (unsigned)e < (unsigned)kv.npages ? e : -1;
+        }
+        return f;
+    };
+    R raw;
+    auto load = [&](int p0, const Four &pg) {
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) {
+            const int g = R::group(wave, i), e = g == 0 ? pg.e[0] : g == 1 ? pg.e[1]
+                                                : g == 2   ? pg.e[2]
+                                                           : pg.e[3];
+            // (a uniform base, and an offset that never changes)
+            const T *b = (const T *)kv.pages + (size_t)max(e, 0) * psize + (size_t)kh * hsize +
+                         (size_t)((p0 + 16 * g) & pmask) * KV_D;
+            const unsigned o = (R::row(t, i) & 15) * KV_D + R::dim(t);
+            raw.k[i] = at<typename R::Vec>(b, o);
+            raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
+        }
+    };
+    // one of the 2 N rows of `raw`, converted, to a buffer
+    auto store = [&](int buf, int n) {
+        RowsLds<LO> &l = lds.step[buf];
+        const int d = R::dim(t), r = R::row(t, n >> 1);
+        if (n & 1)
+            R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
+        else
+            R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
+    };
+    // whether some row sees a step in part
+    auto partial = [&](int p0, const Four &pg) {
+        return p0 + PR_TILE - 1 > all_see || (pg.e[0] | pg.e[1] | pg.e[2] | pg.e[3]) < 0;
+    };
+
+    Four cur = pages_of(p_begin), next = pages_of(p_begin + PR_TILE);
+    load(p_begin, cur);
 
     // this lane's query row
-    const int r = 32 * wave + (lane & 31);
-    const int tl = r / rep;
+    const int r = 32 * rows + c, tl = r / rep;
     const bool ok = tl < toks;
     const int head = kh * rep + r % rep;
     const int sees = ok ? first + tok0 + tl : -1; // its last visible position
-    // the wave's last visible position, and the block's first row's
-    const int wave_last = first + tok0 + min(toks - 1, (32 * wave + 31) / rep);
-    const int all_see = first + tok0;
+    // the last position the wave's last row sees, and its first row
+    const int wave_last = first + tok0 + min(toks - 1, (32 * rows + 31) / rep);
+    const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
     const size_t row = (size_t)(sr.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
 
     // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range
     half8 qhi[KV_D / 16], qlo[KV_D / 16];
     float qscale;
     {
+        // (loaded whatever the row, so that all loads are in flight at once)
         const float *qr = q + row * KV_D + 8 * h;
-        float mx = 0.f;
-        for (int kk = 0; kk < KV_D / 16; ++kk)
+        float4 x[KV_D / 8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(qr[16 * kk + i]));
+        for (int kk = 0; kk < KV_D / 16; ++kk) {
+            x[2 * kk] = *reinterpret_cast<const float4 *>(qr + 16 * kk);
+            x[2 * kk + 1] = *reinterpret_cast<const float4 *>(qr + 16 * kk + 4);
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < KV_D / 8; ++k)
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)),
+                                 fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
         mx = wave::max_halves(mx);
         const int e = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
         qscale = ldexpf(sc, e);
-        const float inv = ldexpf(1.f, -e);
+        const float inv = ok ? ldexpf(1.f, -e) : 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KV_D / 16; ++kk)
+        for (int kk = 0; kk < KV_D / 16; ++kk) {
+            const float4 a = x[2 * kk], b = x[2 * kk + 1];
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = ok ? qr[16 * kk + i] * inv : 0.f;
-                _Float16 hi, lo;
-                split_f16(y, hi, lo);
-                qhi[kk][i] = hi;
-                qlo[kk][i] = fabsf(y) < INFINITY ? lo : (_Float16)0.f;
-            }
-    }
-
-    // tile loads: thread t fetches four dims (d4) of rows {2pp, 2pp+1, 2pp+16, 2pp+17}
-    const int d4 = t & 31, pp = t >> 5;
-    const int *entries = kv.table + (size_t)s * kv.stride;
-    // the pages of a tile's two 16-position halves, -1 where none
-    auto entry = [&](int p) {
-        if (p >= p_end) return -1;
-        const int e = entries[p >> kv.shift];
-        return (unsigned)e < (unsigned)kv.npages ? e : -1;
-    };
-    Vec kr[4], vr[4];
-    auto load_tile = [&](int p0, const int (&pg)[2]) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int p = p0 + 2 * pp + (j & 1) + 16 * (j >> 1);
-            const int e = pg[j >> 1];
-            Vec z{};
-            kr[j] = z;
-            vr[j] = z;
-            if (e >= 0 && p < p_end) {
-                const T *b = (const T *)kv.pages + (size_t)e * psize + (size_t)kh * hsize +
-                             (size_t)(p & pmask) * KV_D + 4 * d4;
-                kr[j] = *reinterpret_cast<const Vec *>(b);
-                vr[j] = *reinterpret_cast<const Vec *>(b + hsize * kv.kvh);
-            }
-        }
-    };
-    // (clean: values that are not finite stay out of the products)
-    auto store_tile = [&](bool clean) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int rr = 2 * pp + (j & 1) + 16 * (j >> 1);
-            float x[4];
-            Four<T>::get(kr[j], x);
-            half4 hi, lo;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                _Float16 a, b;
-                split_f16(x[i], a, b);
-                hi[i] = a;
-                lo[i] = b;
-            }
-            *reinterpret_cast<half4 *>(&Khi[rr][4 * d4]) = hi;
-            if constexpr (LO) *reinterpret_cast<half4 *>(&Klo[rr][4 * d4]) = lo;
-        }
-#pragma unroll
-        for (int jp = 0; jp < 2; ++jp) {
-            const int rr = 2 * pp + 16 * jp;
-            float x[4], y[4];
-            Four<T>::get(vr[2 * jp], x);
-            Four<T>::get(vr[2 * jp + 1], y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (clean) {
-                    x[i] = fabsf(x[i]) < INFINITY ? x[i] : 0.f;
-                    y[i] = fabsf(y[i]) < INFINITY ? y[i] : 0.f;
-                }
+            for (int i = 0; i < 8; i += 2) {
                 half2 hi, lo;
-                _Float16 a, b;
-                split_f16(x[i], a, b);
-                hi[0] = a;
-                lo[0] = b;
-                split_f16(y[i], a, b);
-                hi[1] = a;
-                lo[1] = b;
-                *reinterpret_cast<half2 *>(&Vhi[4 * d4 + i][rr]) = hi;
-                if constexpr (LO) *reinterpret_cast<half2 *>(&Vlo[4 * d4 + i][rr]) = lo;
+                split2(v[i] * inv, v[i + 1] * inv, hi, lo);
+                qhi[kk][i] = hi[0];
+                qhi[kk][i + 1] = hi[1];
+                // (an infinite query: its difference with itself is a NaN)
+                qlo[kk][i] = lo[0] == lo[0] ? lo[0] : (_Float16)0.f;
+                qlo[kk][i + 1] = lo[1] == lo[1] ? lo[1] : (_Float16)0.f;
             }
         }
-    };
-    auto odd = [&]() { // whether this thread's values are not all finite
-        float z = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float x[4];
-            Four<T>::get(vr[j], x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z = fmaf(x[i], 0.f, z);
-        }
-        return z != 0.f;
-    };
+    }
 
     f32x16 acc[KV_D / 32];
 #pragma unroll
@@ -335,140 +414,185 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(
         for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    const int p_begin = piece.t0 * PR_TILE;
-    int pg[2] = {entry(p_begin), entry(p_begin + 16)};
-    int nx[2] = {entry(p_begin + PR_TILE), entry(p_begin + PR_TILE + 16)};
-    load_tile(p_begin, pg);
+    // A step that some row sees in part: values of it that are not finite must
+    // not reach the rows that do not see them (0 * inf), see below.
+    bool odd = partial(p_begin, cur) && raw.clean();
+#pragma unroll
+    for (int n = 0; n < 2 * R::N; ++n) store(0, n);
+    load(p_begin + PR_TILE, next);
+    __syncthreads();
+    int buf = 0;
+    const int o = 32 * part_of; // this wave's 32 positions of a step
     for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
-        // a tile that some row sees in part: a value there that is not finite
-        // must not reach the rows that do not see it (0 * inf). The barrier:
-        // the previous tile's readers are done.
-        bool careful = false;
-        if (p0 + PR_TILE - 1 > all_see) careful = __syncthreads_or(odd());
-        else __syncthreads();
-        store_tile(careful);
-        const int cur[2] = {pg[0], pg[1]};
-        pg[0] = nx[0], pg[1] = nx[1];
-        if (p0 + PR_TILE < p_end) {
-            load_tile(p0 + PR_TILE, pg);
-            nx[0] = entry(p0 + 2 * PR_TILE);
-            nx[1] = entry(p0 + 2 * PR_TILE + 16);
-        }
-        __syncthreads();
-        if (p0 > wave_last) continue; // every row of this wave is before the tile
-
+        const Four after = pages_of(p0 + 2 * PR_TILE);
+        const RowsLds<LO> &l = lds.step[buf];
+        const int p = p0 + o, pa = part_of ? cur.e[2] : cur.e[0], pb = part_of ? cur.e[3] : cur.e[1];
+        if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
         f32x16 sv;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sv[e] = 0.f;
+        // Scores, with the next step's rows converted between their products (the
+        // matrix unit takes 32 cycles for each). Operands are read one product
+        // ahead, and no further: the barriers to the compiler's scheduling keep
+        // the kernel inside its registers.
+        half8 ahi[2], alo[2];
+        auto keys = [&](int kk) {
+            ahi[kk & 1] = *reinterpret_cast<const half8 *>(&l.khi[o + c][16 * kk + 8 * h]);
+            if constexpr (LO)
+                alo[kk & 1] = *reinterpret_cast<const half8 *>(&l.klo[o + c][16 * kk + 8 * h]);
+        };
+        keys(0);
 #pragma unroll
         for (int kk = 0; kk < KV_D / 16; ++kk) {
-            const half8 ahi = *reinterpret_cast<const half8 *>(&Khi[lane & 31][16 * kk + 8 * h]);
-            sv = mfma(ahi, qhi[kk], sv);
-            sv = mfma(ahi, qlo[kk], sv);
-            if constexpr (LO) {
-                const half8 alo =
-                    *reinterpret_cast<const half8 *>(&Klo[lane & 31][16 * kk + 8 * h]);
-                sv = mfma(alo, qhi[kk], sv);
+            if (kk + 1 < KV_D / 16) keys(kk + 1);
+            sv = mfma(ahi[kk & 1], qhi[kk], sv);
+            sv = mfma(ahi[kk & 1], qlo[kk], sv);
+            if constexpr (LO) sv = mfma(alo[kk & 1], qhi[kk], sv);
+            if (kk < 2 * R::N) store(buf ^ 1, kk);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load(p0 + 2 * PR_TILE, after);
+        if (p + 31 > wave_all || (pa | pb) < 0) { // mask
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int pos = p + 8 * (e >> 2) + 4 * h + (e & 3);
+                sv[e] = pos <= sees && (e < 8 ? pa : pb) >= 0 ? sv[e] : -INFINITY;
             }
         }
-        // scale, mask, softmax (one row per lane pair)
-        float tmax = -INFINITY;
+        float tmax = sv[0];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int p = p0 + 8 * (e >> 2) + 4 * h + (e & 3);
-            sv[e] = p <= sees && cur[e >> 3] >= 0 ? sv[e] * qscale : -INFINITY;
-            tmax = fmaxf(tmax, sv[e]);
-        }
-        const float m_new = fmaxf(m_run, wave::max_halves(tmax));
-        const float base = m_new == -INFINITY ? 0.f : m_new; // (nothing seen yet: zero weights)
-        const float corr = __builtin_amdgcn_exp2f(m_run - base);
-        float rs = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            sv[e] = __builtin_amdgcn_exp2f(sv[e] - base);
-            rs += sv[e];
-        }
-        if (__any(m_new != m_run)) {
+        for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, sv[e]);
+        // The running maximum follows only when a score passes it by 2^8 or
+        // more: until then weights are at most 2^8, and the 64 products that
+        // bring the sums to a new one are rare (in 32 rows of equal chances
+        // some row has a new maximum in most steps).
+        const float m_new = wave::max_halves(tmax) * qscale;
+        if (__any(m_new > m_run + 8.f)) {
+            const float m = fmaxf(m_run, m_new);
+            const float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
 #pragma unroll
             for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
             l_run *= corr;
+            m_run = m;
         }
-        l_run += rs;
-        m_run = m_new;
-
-        // P^T operands: positions 16kk + 8h + (0..7) of this lane's row,
-        // half from the partner lane (lane ^ 32)
+        const float base = m_run == -INFINITY ? 0.f : m_run; // (nothing seen yet: zero weights)
+        float rs[2] = {0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < PR_TILE / 16; ++kk) {
-            half8 phi, plo;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const auto sw = __builtin_amdgcn_permlane32_swap(fbits(sv[8 * kk + i]),
-                                                                 fbits(sv[8 * kk + 4 + i]),
-                                                                 false, false);
-                _Float16 a, b;
-                split_f16(bitsf(sw[0]), a, b);
-                phi[i] = a;
-                plo[i] = b;
-                split_f16(bitsf(sw[1]), a, b);
-                phi[4 + i] = a;
-                plo[4 + i] = b;
+        for (int e = 0; e < 16; ++e) {
+            sv[e] = __builtin_amdgcn_exp2f(fmaf(sv[e], qscale, -base));
+            rs[e & 1] += sv[e];
+        }
+        l_run += rs[0] + rs[1];
+        // operand element 4 x + i of product (kk, j): position 16 kk + 8 x + 4 h + i,
+        // which is the lane's weight 8 kk + 4 x + i
+        half8 vhi[2], vlo[2];
+        auto values = [&](int n) {
+            const int kk = n >> 2, j = n & 3;
+            const int vr = o + 16 * kk + 4 * h + ((lane & 15) >> 2);
+            const int vd = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const half4 x = read_transposed(&l.vhi[vr][vd]),
+                        y = read_transposed(&l.vhi[vr + 8][vd]);
+            vhi[n & 1] = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            if constexpr (LO) {
+                const half4 z = read_transposed(&l.vlo[vr][vd]),
+                            w = read_transposed(&l.vlo[vr + 8][vd]);
+                vlo[n & 1] = half8{z[0], z[1], z[2], z[3], w[0], w[1], w[2], w[3]};
             }
+        };
+        half8 phi, plo;
+        values(0);
 #pragma unroll
-            for (int j = 0; j < KV_D / 32; ++j) {
-                const int d = 32 * j + (lane & 31);
-                const half8 vhi = *reinterpret_cast<const half8 *>(&Vhi[d][16 * kk + 8 * h]);
-                acc[j] = mfma(vhi, phi, acc[j]);
-                acc[j] = mfma(vhi, plo, acc[j]);
-                if constexpr (LO) {
-                    const half8 vlo = *reinterpret_cast<const half8 *>(&Vlo[d][16 * kk + 8 * h]);
-                    acc[j] = mfma(vlo, phi, acc[j]);
+        for (int n = 0; n < 8; ++n) {
+            if ((n & 3) == 0) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    half2 hi, lo;
+                    split2(sv[2 * n + i], sv[2 * n + i + 1], hi, lo);
+                    phi[i] = hi[0];
+                    phi[i + 1] = hi[1];
+                    plo[i] = lo[0];
+                    plo[i + 1] = lo[1];
                 }
             }
+            if (n + 1 < 8) values(n + 1);
+            f32x16 &d = acc[n & 3];
+            d = mfma(vhi[n & 1], phi, d);
+            d = mfma(vhi[n & 1], plo, d);
+            if constexpr (LO) d = mfma(vlo[n & 1], phi, d);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (careful) { // the values left out, for the rows that see them
-            for (int i = 0; i < PR_TILE; ++i) {
-                const int src = (lane & 31) + 32 * ((i >> 2) & 1);
-                float w = 0.f;
+        __syncthreads();
+        cur = next;
+        next = after;
+        buf ^= 1;
+    }
+    if (__syncthreads_or(odd)) {
+        // the values left out, for the rows that see them: whatever its weight,
+        // such a value makes the sum not finite
+        for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
+            const Four pg = pages_of(p0);
+            if (!partial(p0, pg)) continue;
+            for (int i = 0; i < 32; ++i) {
+                const int pos = p0 + 32 * part_of + i;
+                const int e = i < 16 ? (part_of ? pg.e[2] : pg.e[0]) : part_of ? pg.e[3] : pg.e[1];
+                if (pos > sees || e < 0) continue;
+                const T *vb = (const T *)kv.pages + (size_t)e * psize +
+                              (size_t)(kv.kvh + kh) * hsize + (size_t)(pos & pmask) * KV_D;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = __shfl(sv[e], src, 64);
-                    if (e == 4 * (i >> 3) + (i & 3)) w = x;
-                }
-                const int p = p0 + i, pe = cur[i >> 4];
-                if (p > sees || pe < 0) continue;
-                const T *vb = (const T *)kv.pages + (size_t)pe * psize +
-                              (size_t)(kv.kvh + kh) * hsize + (size_t)(p & pmask) * KV_D;
+                for (int j = 0; j < KV_D / 32; ++j) {
 #pragma unroll
-                for (int j = 0; j < KV_D / 32; ++j)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float v = (float)vb[32 * j + 8 * (e >> 2) + 4 * h + (e & 3)];
-                        if (!(fabsf(v) < INFINITY)) acc[j][e] = fmaf(w, v, acc[j][e]);
+                    for (int x = 0; x < 16; ++x) {
+                        const float v = (float)vb[32 * j + 8 * (x >> 2) + 4 * h + (x & 3)];
+                        acc[j][x] += fabsf(v) < INFINITY ? 0.f : v;
                     }
+                    asm volatile("" ::: "memory"); // (few loads at once: a rare path)
+                }
             }
         }
     }
-    if (!ok) return;
+
+    // the two halves' rows joined, in the first half's waves
     l_run = wave::sum_halves(l_run);
-    float *o = out + row * KV_D;
+    if (part_of) {
+        float(*o)[64] = lds.join[rows];
+        o[0][lane] = m_run;
+        o[1][lane] = l_run;
+#pragma unroll
+        for (int j = 0; j < KV_D / 32; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[2 + 16 * j + e][lane] = acc[j][e];
+    }
+    __syncthreads();
+    if (part_of || !ok) return;
+    {
+        const float(*o)[64] = lds.join[rows];
+        const float m2 = o[0][lane], m = fmaxf(m_run, m2), base = m == -INFINITY ? 0.f : m;
+        const float a = __builtin_amdgcn_exp2f(m_run - base), b = __builtin_amdgcn_exp2f(m2 - base);
+        l_run = l_run * a + o[1][lane] * b;
+        m_run = m;
+#pragma unroll
+        for (int j = 0; j < KV_D / 32; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * a + o[2 + 16 * j + e][lane] * b;
+    }
+    float *dst = out + row * KV_D;
     float f = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f; // (saw nothing: zeros)
     if (piece.part >= 0) {
-        o = part + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
+        dst = part + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
         if (h == 0) {
-            o[0] = m_run;
-            o[1] = l_run;
+            dst[0] = m_run;
+            dst[1] = l_run;
         }
-        o += 4;
+        dst += 4;
         f = 1.f;
     }
 #pragma unroll
     for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4 *>(o + 32 * j + 8 * g + 4 * h) =
+            *reinterpret_cast<float4 *>(dst + 32 * j + 8 * g + 4 * h) =
                 make_float4(acc[j][4 * g] * f, acc[j][4 * g + 1] * f, acc[j][4 * g + 2] * f,
                             acc[j][4 * g + 3] * f);
 }
@@ -489,20 +613,33 @@ __global__ __launch_bounds__(256) void paged_rows_merge_kernel(
     if (tl >= min(tq, sr.n - blk.index * tq)) return;
     const size_t step = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
     const float *p = part + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
+    const int lane = threadIdx.x & 31;
     float M = -INFINITY;
-    for (int i = 0; i < blk.pieces; ++i) M = fmaxf(M, p[i * step]);
+    for (int i = lane; i < blk.pieces; i += 32) M = fmaxf(M, p[i * step]);
+    M = fmaxf(M, __shfl_xor(M, 16, 32));
+    M = wave::max16(M);
     const float base = M == -INFINITY ? 0.f : M;
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
     float den = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < blk.pieces; ++i) {
-        const float x = __builtin_amdgcn_exp2f(p[i * step] - base);
-        const float4 v = *reinterpret_cast<const float4 *>(p + i * step + 4 + d);
-        den = fmaf(x, p[i * step + 1], den);
-        num.x = fmaf(x, v.x, num.x);
-        num.y = fmaf(x, v.y, num.y);
-        num.z = fmaf(x, v.z, num.z);
-        num.w = fmaf(x, v.w, num.w);
+    for (int b = 0; b < blk.pieces; b += 8) { // eight parts' loads in flight
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float *o = p + (size_t)min(b + k, blk.pieces - 1) * step;
+            ml[k] = *reinterpret_cast<const float2 *>(o);
+            v[k] = *reinterpret_cast<const float4 *>(o + 4 + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (b + k >= blk.pieces) continue;
+            const float x = __builtin_amdgcn_exp2f(ml[k].x - base);
+            den = fmaf(x, ml[k].y, den);
+            num.x = fmaf(x, v[k].x, num.x);
+            num.y = fmaf(x, v[k].y, num.y);
+            num.z = fmaf(x, v[k].z, num.z);
+            num.w = fmaf(x, v[k].w, num.w);
+        }
     }
     const float f = den > 0.f || den != den ? 1.f / den : 0.f;
     const size_t row = (size_t)(sr.begin + blk.index * tq + tl) * kv.heads + kh * rep + r % rep;
@@ -547,11 +684,11 @@ int launch_paged_rows(const PagedKv &kv, const float *q, void *scratch, float *o
                        kv, paged_few_rows(rep), tq, nb, plan, blocks, pieces);
     const dim3 grid(kv.kvh, max_pieces(nb, kv.kvh));
     if (kv.f16)
-        hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(256), 0, st, kv, tq, plan,
-                           blocks, pieces, q, part, out);
+        hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(PR_THREADS), 0, st, kv, tq,
+                           plan, blocks, pieces, q, part, out);
     else
-        hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(256), 0, st, kv, tq, plan, blocks,
-                           pieces, q, part, out);
+        hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(PR_THREADS), 0, st, kv, tq, plan,
+                           blocks, pieces, q, part, out);
     hipLaunchKernelGGL(paged_rows_merge_kernel, dim3(kv.kvh, nb, PR_ROWS / 8), dim3(256), 0, st,
                        kv, tq, plan, blocks, part, out);
     return (int)hipGetLastError();
