@@ -6,6 +6,7 @@
 
 #include "hyq_abi.hpp"
 #include "hyq_paged.hpp"
+#include "hyq_paged_attn.hpp"
 
 using namespace hyq;
 
@@ -92,6 +93,14 @@ PagesArgs pages_args(const hyq_kv_layout *kl)
 // bits, the counts themselves are ints
 constexpr size_t MAX_ROWS = 1 << 20;
 
+// Whether the attention's launches of these rows fit a grid (2^32 threads).
+bool grid_ok(const hyq_kv_layout *kl, size_t rows, size_t heads)
+{
+    const int rep = (int)heads / kl->kv_heads;
+    const int cap = max_blocks(kl->seqs, (int)rows, PR_ROWS / rep);
+    return merge_groups(kl->seqs, kl->kv_heads, paged_few_rows(rep) * rep, cap) < (1 << 24);
+}
+
 } // namespace
 
 extern "C" {
@@ -132,7 +141,8 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
                                          size_t heads)
 {
-    if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0)
+    if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0 ||
+        !grid_ok(kl, rows, heads))
         return 0;
     return paged_attention_scratch(kl->seqs, kl->kv_heads, (int)heads, (int)rows,
                                    (int)std::min(rows, max_rows));
@@ -149,7 +159,8 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
         return fail(HYQ_EINVAL, "paged_attention: null argument");
     if (layer < 0 || layer >= kl->layers)
         return fail(HYQ_EINVAL, "paged_attention: layer %d of %d", layer, kl->layers);
-    if (!heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0)
+    if (!heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0 ||
+        !grid_ok(kl, rows, heads))
         return fail(HYQ_EINVAL, "paged_attention: %zu rows (at most %zu of a slot), heads %zu/%d",
                     rows, max_rows, heads, kl->kv_heads);
     if (!aligned(pool_d) || !aligned(q_d) || !aligned(scratch_d) || !aligned(out_d))
@@ -265,15 +276,15 @@ int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
 // ---------------------------------------------------------------------------
 // the attention's two forms
 // ---------------------------------------------------------------------------
-#include "hyq_paged_attn.hpp"
 
 namespace hyq {
 
+// Scratch: the few-row form's parts, then the tile form's plan and parts.
 size_t paged_attention_scratch(int seqs, int kvh, int heads, int rows, int max_rows)
 {
     const int few = std::min(paged_few_rows(heads / kvh), max_rows);
     size_t n = paged_few_scratch(seqs, kvh, heads, few);
-    if (max_rows > few) n = std::max(n, paged_rows_scratch(seqs, kvh, heads, rows));
+    if (max_rows > few) n += rows_layout(seqs, kvh, heads, rows).bytes;
     return n;
 }
 
@@ -281,8 +292,21 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
                            float *out, void *stream)
 {
     const int few = std::min(paged_few_rows(kv.heads / kv.kvh), max_rows);
-    int rc = launch_paged_few(kv, few, q, (float *)scratch, out, stream);
-    if (rc == 0 && max_rows > few) rc = launch_paged_rows(kv, q, scratch, out, stream);
+    float *part = (float *)scratch;
+    RowsScratch rs{};
+    if (max_rows > few) {
+        const RowsLayout l = rows_layout(kv.seqs, kv.kvh, kv.heads, kv.rows);
+        char *base = (char *)scratch + paged_few_scratch(kv.seqs, kv.kvh, kv.heads, few);
+        rs.plan = (Plan *)base;
+        rs.blocks = (Block *)(base + l.blocks);
+        rs.pieces = (Piece *)(base + l.pieces);
+        rs.parts = (float *)(base + l.parts);
+        rs.tq = PR_ROWS / (kv.heads / kv.kvh);
+        rs.cap = max_blocks(kv.seqs, kv.rows, rs.tq);
+    }
+    int rc = launch_paged_few(kv, few, rs, q, part, out, stream);
+    if (rc == 0 && rs.cap) rc = launch_paged_rows(kv, rs, q, out, stream);
+    if (rc == 0) rc = launch_paged_merge(kv, few, rs, part, out, stream);
     return rc;
 }
 

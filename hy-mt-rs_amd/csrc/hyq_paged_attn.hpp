@@ -1,9 +1,14 @@
-// What the two forms of the paged attention share.
+// What the two forms of the paged attention share: the slots' rows, the plan of
+// the tile form (made by a workgroup of the few-row form's launch) and the
+// layout of its scratch.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "hyq_paged.hpp"
+#include "hyq_wave.hpp"
 
 namespace hyq {
 
@@ -26,14 +31,215 @@ __device__ __forceinline__ SlotRows slot_rows(const PagedKv &kv, int s)
     return r;
 }
 
+// A vector at a uniform base and an unsigned 32-bit element offset (a scalar
+// base with a vector offset in the load: no 64-bit address per lane).
+template <class V, class T> __device__ __forceinline__ V at(const T *base, unsigned off)
+{
+    return *reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
+                                        (unsigned)(off * sizeof(T)));
+}
+
+// ---- the tile form's plan ----
+constexpr int PR_ROWS = 128;        // query rows per workgroup
+constexpr int PR_TILE = 64;         // positions per step
+constexpr int PR_FILL = 256;        // workgroups that fill the GPU: one per CU
+constexpr int PR_MIN_TILES = 2;     // the shortest piece worth its partial rows
+
+// A block of a slot's new tokens, and what its pieces left.
+struct Block {
+    int slot, index, part, pieces; // first partial block and pieces of the block
+};
+// A range of steps of a block, with what its workgroup needs to begin.
+struct Piece {
+    int slot, index, t0, t1;
+    int part;            // the partial block it writes, -1 for the output
+    int begin, n, first; // the slot's rows, and the first one's position
+};
+struct Plan {
+    int blocks, pieces, parts, unused;
+};
+
+// Pieces that fill the GPU with kvh workgroups each (at least one).
+__host__ __device__ inline int fill_pieces(int kvh) { return PR_FILL > kvh ? PR_FILL / kvh : 1; }
+inline int max_blocks(int seqs, int rows, int tq) { return rows / tq + std::min(seqs, rows); }
+// At most fill_pieces, or the sum of ceil(n / each) with each >= tiles / room and
+// room <= fill_pieces, where a block that is cut (n > each) has fewer than
+// 2 n / each pieces.
+inline int max_pieces(int blocks, int kvh) { return blocks + fill_pieces(kvh); }
+inline int max_parts(int kvh) { return 2 * fill_pieces(kvh); }
+// Workgroups of the merge: for every KV head a row of a slot each, and eight
+// rows of a block each.
+inline long long merge_groups(int seqs, int kvh, int part_rows, int cap)
+{
+    return ((long long)seqs * part_rows + (long long)cap * (PR_ROWS / 8)) * kvh;
+}
+
+// Where in the scratch the plan's parts lie.
+struct RowsScratch {
+    Plan *plan;
+    Block *blocks;
+    Piece *pieces;
+    float *parts;
+    int tq, cap; // tokens of a block, blocks there is room for (0: no tile form)
+};
+struct RowsLayout {
+    size_t blocks, pieces, parts, bytes;
+};
+inline RowsLayout rows_layout(int seqs, int kvh, int heads, int rows)
+{
+    const int nb = max_blocks(seqs, rows, PR_ROWS / (heads / kvh));
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    RowsLayout r;
+    r.blocks = up(sizeof(Plan));
+    r.pieces = r.blocks + up(nb * sizeof(Block));
+    r.parts = r.pieces + up(max_pieces(nb, kvh) * sizeof(Piece));
+    r.bytes = r.parts + up((size_t)max_parts(kvh) * kvh * PR_ROWS * PAGED_PART * 4);
+    return r;
+}
+
+__device__ __forceinline__ int block_tiles(const SlotRows &r, int b, int tq)
+{
+    const int last = r.len - r.n + min(r.n, (b + 1) * tq); // one past the last position seen
+    return max(1, (last + PR_TILE - 1) / PR_TILE);
+}
+
+// Exclusive scan of one value per thread over 256 threads; returns the total.
+__device__ __forceinline__ int scan256(int mine, int &before, int *wsum)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int v = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) wsum[wave] = v;
+    __syncthreads();
+    int base = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) base += wsum[w];
+        all += wsum[w];
+    }
+    before = base + v - mine;
+    return all;
+}
+
+// The plan, by one workgroup of 256 threads. first: LDS of seqs ints.
+__device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const RowsScratch &rs,
+                                          int *first)
+{
+    constexpr int TRIES = 16;
+    __shared__ int wsum[4];
+    __shared__ int sums[4][TRIES];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tq = rs.tq;
+    int count = 0;
+    for (int b = 0; b < kv.seqs; b += 256) {
+        int nb = 0, before;
+        if (b + t < kv.seqs) {
+            const SlotRows r = slot_rows(kv, b + t);
+            nb = r.n > few_rows ? (r.n + tq - 1) / tq : 0;
+        }
+        const int all = scan256(nb, before, wsum);
+        if (b + t < kv.seqs) first[b + t] = count + before;
+        count += all;
+    }
+    // (starts that do not ascend could claim rows twice: what the scratch has
+    // no room for is left out)
+    count = min(count, rs.cap);
+    __syncthreads();
+    auto slot_of = [&](int u) {
+        int s = 0, hi = kv.seqs; // the last slot with first[s] <= u
+        while (hi - s > 1) {
+            const int mid = (s + hi) >> 1;
+            if (first[mid] <= u) s = mid;
+            else hi = mid;
+        }
+        return s;
+    };
+    // all tiles of one KV head (a block has at most 2^24 / 64, so that 256 of
+    // them fit an int)
+    long long tiles = 0;
+    for (int b = 0; b < count; b += 256) {
+        int mine = 0, before;
+        if (b + t < count) {
+            const int s = slot_of(b + t);
+            mine = block_tiles(slot_rows(kv, s), b + t - first[s], tq);
+        }
+        tiles += scan256(mine, before, wsum);
+    }
+    // The least length of a piece, of sixteen, with which the pieces number no
+    // more than fill the GPU once: a second round of a few would take as long
+    // as the first. `most` does so where the blocks alone are few; where they
+    // are many, it is twice their share, and only blocks longer than that are
+    // cut.
+    const int fill = fill_pieces(kv.kvh), room = max(fill - count, (fill + 1) / 2);
+    const int least = (int)max((long long)PR_MIN_TILES, (tiles + fill - 1) / fill);
+    const int most = (int)max((long long)PR_MIN_TILES, (tiles + room - 1) / room);
+    auto length = [&](int i) { return least + (int)((long long)(most - least) * i / (TRIES - 1)); };
+    int each = most;
+    if (most > least) {
+        int n[TRIES];
+#pragma unroll
+        for (int i = 0; i < TRIES; ++i) n[i] = 0;
+        for (int b = t; b < count; b += 256) {
+            const int s = slot_of(b), x = block_tiles(slot_rows(kv, s), b - first[s], tq);
+#pragma unroll
+            for (int i = 0; i < TRIES; ++i) n[i] += (x + length(i) - 1) / length(i);
+        }
+#pragma unroll
+        for (int i = 0; i < TRIES; ++i) {
+            n[i] = wave::sum64(n[i]);
+            if (lane == 0) sums[wave][i] = n[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = TRIES - 1; i >= 0; --i)
+            if (sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i] <= fill) each = length(i);
+    }
+    int npieces = 0, nparts = 0;
+    for (int b = 0; b < count; b += 256) {
+        int s = 0, n = 0, k = 0, before, pbefore;
+        SlotRows r{};
+        if (b + t < count) {
+            s = slot_of(b + t);
+            r = slot_rows(kv, s);
+            n = block_tiles(r, b + t - first[s], tq);
+            k = (n + each - 1) / each;
+        }
+        const int all = scan256(k, before, wsum);
+        const int pall = scan256(k > 1 ? k : 0, pbefore, wsum);
+        if (b + t < count) {
+            const int index = b + t - first[s];
+            rs.blocks[b + t] = Block{s, index, nparts + pbefore, k};
+            for (int i = 0; i < k; ++i)
+                rs.pieces[npieces + before + i] =
+                    Piece{s,
+                          index,
+                          (int)((long long)n * i / k),
+                          (int)((long long)n * (i + 1) / k),
+                          k > 1 ? nparts + pbefore + i : -1,
+                          r.begin,
+                          r.n,
+                          r.len - r.n};
+        }
+        npieces += all;
+        nparts += pall;
+    }
+    if (t == 0) *rs.plan = Plan{count, npieces, nparts, 0};
+}
+
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)
-// new rows.
+// new rows, with the plan where there is a tile form; and the merge of both.
 int paged_few_rows(int rep);
 size_t paged_few_scratch(int seqs, int kvh, int heads, int few);
-int launch_paged_few(const PagedKv &kv, int few, const float *q, float *part, float *out,
-                     void *stream);
+int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
+                     float *out, void *stream);
+int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
+                       float *out, void *stream);
 // hyq_paged_rows.hip: the slots of more.
-size_t paged_rows_scratch(int seqs, int kvh, int heads, int rows);
-int launch_paged_rows(const PagedKv &kv, const float *q, void *scratch, float *out, void *stream);
+int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, float *out,
+                      void *stream);
 
 } // namespace hyq

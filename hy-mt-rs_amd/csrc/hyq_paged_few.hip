@@ -109,14 +109,6 @@ __device__ __forceinline__ f32x4 mfma_f16(const half8 &a, const half8 &b, const 
 // acc[x][e] (see pv): f32 64 (x / 4) + 16 g + 4 e + x % 4, f16 32 g + 8 e + x.
 template <class T> struct Ops;
 
-// A vector at a uniform base and an unsigned 32-bit element offset (a scalar
-// base with a vector offset in the load: no 64-bit address per lane).
-template <class V, class T> __device__ __forceinline__ V at(const T *base, unsigned off)
-{
-    return *reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
-                                        (unsigned)(off * sizeof(T)));
-}
-
 template <> struct Ops<float> {
     static constexpr int TILE = 16; // positions of a step
     float4 q[8]; // row lane % 16, dims 16 j + 4 g ..
@@ -308,12 +300,16 @@ template <> struct Ops<_Float16> {
 
 template <class T>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
-    PagedKv kv, int few_rows, int max_workers, const float *__restrict__ q, int part_rows,
-    float *__restrict__ part, float *__restrict__ out)
+    PagedKv kv, int few_rows, int max_workers, RowsScratch rs, const float *__restrict__ q,
+    int part_rows, float *__restrict__ part, float *__restrict__ out)
 {
     constexpr int TILE = Ops<T>::TILE, SUB = TILE / 16;
     extern __shared__ long long before[]; // [seqs + 1]
     __shared__ long long wsum[4];
+    if (blockIdx.x * FEW_WAVES >= max_workers) { // one more workgroup: the tile form's plan
+        rows_plan(kv, few_rows, rs, (int *)before);
+        return;
+    }
     const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be)
@@ -485,20 +481,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     }
 }
 
-// Joins the parts of the units that several workers shared. Grid (kv heads,
-// seqs, rows), 256 threads: wave g takes the parts g, g + 4, ..., lane d dims
-// 2 d and 2 d + 1, with eight parts' loads in flight; the waves' sums are
-// added in a fixed order.
+// Joins the parts of one row of a unit that several workers shared, by 256
+// threads: wave g takes the parts g, g + 4, ..., lane d dims 2 d and 2 d + 1,
+// with eight parts' loads in flight; the waves' sums are added in a fixed order.
 template <int TILE>
-__global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedKv kv, int few_rows,
-                                                              int max_workers, int part_rows,
-                                                              const float *__restrict__ part,
-                                                              float *__restrict__ out)
+__device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int max_workers,
+                                          int part_rows, const float *__restrict__ part,
+                                          float *__restrict__ out, int kh, int s, int c,
+                                          long long *before)
 {
-    extern __shared__ long long before[];
     __shared__ long long wsum[4];
     __shared__ float red[4][KV_D + 2];
-    const int s = blockIdx.y, kh = blockIdx.x, c = blockIdx.z;
     const int rep = kv.heads / kv.kvh;
     const SlotRows sr = slot_rows(kv, s);
     const int tiles = few_tiles(kv, s, few_rows, TILE);
@@ -550,6 +543,71 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(PagedKv kv, int fe
     out[row * KV_D + d] = den > 0.f || den != den ? num / den : 0.f;
 }
 
+// Joins the pieces of a block that was cut, in order, by 256 threads: 8 rows, a
+// 32-lane half wave each.
+__device__ __forceinline__ void merge_rows(const PagedKv &kv, const RowsScratch &rs,
+                                           float *__restrict__ out, int kh, int b, int row8)
+{
+    if (b >= rs.plan->blocks) return;
+    const Block blk = rs.blocks[b];
+    if (blk.pieces < 2) return;
+    const SlotRows sr = slot_rows(kv, blk.slot);
+    const int rep = kv.heads / kv.kvh;
+    const int r = row8 * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+    const int tl = r / rep;
+    if (tl >= min(rs.tq, sr.n - blk.index * rs.tq)) return;
+    const size_t step = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
+    const float *p = rs.parts + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
+    const int lane = threadIdx.x & 31;
+    float M = -INFINITY;
+    for (int i = lane; i < blk.pieces; i += 32) M = fmaxf(M, p[i * step]);
+    M = fmaxf(M, __shfl_xor(M, 16, 32));
+    M = wave::max16(M);
+    const float base = M == -INFINITY ? 0.f : M;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+    for (int b = 0; b < blk.pieces; b += 8) { // eight parts' loads in flight
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float *o = p + (size_t)min(b + k, blk.pieces - 1) * step;
+            ml[k] = *reinterpret_cast<const float2 *>(o);
+            v[k] = *reinterpret_cast<const float4 *>(o + 4 + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (b + k >= blk.pieces) continue;
+            const float x = __builtin_amdgcn_exp2f(ml[k].x - base);
+            den = fmaf(x, ml[k].y, den);
+            num.x = fmaf(x, v[k].x, num.x);
+            num.y = fmaf(x, v[k].y, num.y);
+            num.z = fmaf(x, v[k].z, num.z);
+            num.w = fmaf(x, v[k].w, num.w);
+        }
+    }
+    const float f = den > 0.f || den != den ? 1.f / den : 0.f;
+    const size_t row = (size_t)(sr.begin + blk.index * rs.tq + tl) * kv.heads + kh * rep + r % rep;
+    *reinterpret_cast<float4 *>(out + row * KV_D + d) =
+        make_float4(num.x * f, num.y * f, num.z * f, num.w * f);
+}
+
+// Grid: merge_groups workgroups, the KV heads of a row or block in sequence.
+template <int TILE>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_rows, int max_workers,
+                                                          int part_rows, RowsScratch rs,
+                                                          const float *__restrict__ part,
+                                                          float *__restrict__ out)
+{
+    extern __shared__ long long before[];
+    const int kh = blockIdx.x % kv.kvh, i = blockIdx.x / kv.kvh, n = kv.seqs * part_rows;
+    if (i < n)
+        merge_few<TILE>(kv, few_rows, max_workers, part_rows, part, out, kh, i / part_rows, i % part_rows,
+                        before);
+    else
+        merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / 8), (i - n) % (PR_ROWS / 8));
+}
+
 constexpr int FEW_MAX_WORKERS = 2048; // twelve waves on each of 256 CUs
 
 } // namespace
@@ -562,25 +620,35 @@ size_t paged_few_scratch(int seqs, int kvh, int heads, int few)
     return ((size_t)FEW_MAX_WORKERS + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
 }
 
-int launch_paged_few(const PagedKv &kv, int few, const float *q, float *part, float *out,
-                     void *stream)
+int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
+                     float *out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
-    const dim3 grid(FEW_MAX_WORKERS / FEW_WAVES), block(64 * FEW_WAVES);
-    const dim3 mgrid(kv.kvh, kv.seqs, part_rows);
-    if (kv.f16) {
+    const dim3 grid(FEW_MAX_WORKERS / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
+    if (kv.f16)
         hipLaunchKernelGGL(paged_few_kernel<_Float16>, grid, block, lds, st, kv, few,
-                           FEW_MAX_WORKERS, q, part_rows, part, out);
-        hipLaunchKernelGGL(paged_few_merge_kernel<Ops<_Float16>::TILE>, mgrid, dim3(256), lds, st,
-                           kv, few, FEW_MAX_WORKERS, part_rows, part, out);
-    } else {
+                           FEW_MAX_WORKERS, rs, q, part_rows, part, out);
+    else
         hipLaunchKernelGGL(paged_few_kernel<float>, grid, block, lds, st, kv, few,
-                           FEW_MAX_WORKERS, q, part_rows, part, out);
-        hipLaunchKernelGGL(paged_few_merge_kernel<Ops<float>::TILE>, mgrid, dim3(256), lds, st,
-                           kv, few, FEW_MAX_WORKERS, part_rows, part, out);
-    }
+                           FEW_MAX_WORKERS, rs, q, part_rows, part, out);
+    return (int)hipGetLastError();
+}
+
+int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
+                       float *out, void *stream)
+{
+    hipStream_t st = (hipStream_t)stream;
+    const int part_rows = few * (kv.heads / kv.kvh);
+    const size_t lds = ((size_t)kv.seqs + 1) * 8;
+    const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, part_rows, rs.cap));
+    if (kv.f16)
+        hipLaunchKernelGGL(paged_merge_kernel<Ops<_Float16>::TILE>, grid, dim3(256), lds, st, kv,
+                           few, FEW_MAX_WORKERS, part_rows, rs, part, out);
+    else
+        hipLaunchKernelGGL(paged_merge_kernel<Ops<float>::TILE>, grid, dim3(256), lds, st, kv, few,
+                           FEW_MAX_WORKERS, part_rows, rs, part, out);
     return (int)hipGetLastError();
 }
 

@@ -23,9 +23,10 @@
 // one, and the step after it loaded, with one barrier a step.
 //
 // Blocks of different slots and places see very different numbers of steps, so
-// a plan cuts them: one workgroup counts every block's steps and makes pieces
-// of about equal length, enough to fill the GPU once, and the pieces of a block
-// that was cut leave partial rows, which a merge joins in order.
+// a plan cuts them (rows_plan): one workgroup counts every block's steps and
+// makes pieces of about equal length, enough to fill the GPU once, and the
+// pieces of a block that was cut leave partial rows, which a merge joins in
+// order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -43,137 +44,12 @@ typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 
-constexpr int PR_ROWS = 128;        // query rows per workgroup
-constexpr int PR_TILE = 64;         // positions per step
 constexpr int PR_THREADS = 512;     // two waves on each SIMD
 // Row pitches in halves, chosen for the banks: keys are read 16 bytes a lane
 // from 16 rows (4 banks apart), values by the transposing read 8 bytes a lane
 // from 4 rows (16 banks apart).
 constexpr int PR_KP = KV_D + 8;
 constexpr int PR_VP = KV_D + 32;
-constexpr int PR_FILL = 256;        // workgroups that fill the GPU: one per CU
-constexpr int PR_MIN_TILES = 2;     // the shortest piece worth its partial rows
-
-// The plan in scratch: counts, the blocks, then the pieces.
-struct Block {
-    int slot, index, part, pieces; // first partial block and pieces of the block
-};
-struct Piece {
-    int block, t0, t1, part; // part: the partial block it writes, -1 for the output
-};
-struct Plan {
-    int blocks, pieces, parts, unused;
-};
-
-int max_blocks(int seqs, int rows, int tq) { return rows / tq + std::min(seqs, rows); }
-// Pieces that fill the GPU with kvh workgroups each (at least one).
-__host__ __device__ inline int fill_pieces(int kvh) { return PR_FILL > kvh ? PR_FILL / kvh : 1; }
-// sum of ceil(n / each) with each >= 2 tiles / fill_pieces; a block that is cut
-// (n > each) has fewer than 2 n / each pieces
-int max_pieces(int blocks, int kvh) { return blocks + fill_pieces(kvh); }
-int max_parts(int kvh) { return 2 * fill_pieces(kvh); }
-
-__device__ __forceinline__ int block_tiles(const SlotRows &r, int b, int tq)
-{
-    const int last = r.len - r.n + min(r.n, (b + 1) * tq); // one past the last position seen
-    return max(1, (last + PR_TILE - 1) / PR_TILE);
-}
-
-// Exclusive scan of one value per thread over 1024 threads; returns the total.
-__device__ __forceinline__ int scan1024(int mine, int &before, int *wsum)
-{
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    int v = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    __syncthreads();
-    if (lane == 63) wsum[wave] = v;
-    __syncthreads();
-    int base = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        if (w < wave) base += wsum[w];
-        all += wsum[w];
-    }
-    before = base + v - mine;
-    return all;
-}
-
-// One workgroup of 1024 threads. Dynamic LDS: seqs ints.
-__global__ __launch_bounds__(1024) void paged_rows_plan_kernel(PagedKv kv, int few_rows, int tq,
-                                                               int cap, Plan *plan,
-                                                               Block *blocks, Piece *pieces)
-{
-    extern __shared__ int first[]; // a slot's first block
-    __shared__ int wsum[16];
-    const int t = threadIdx.x;
-    int count = 0;
-    for (int b = 0; b < kv.seqs; b += 1024) {
-        int nb = 0, before;
-        if (b + t < kv.seqs) {
-            const SlotRows r = slot_rows(kv, b + t);
-            nb = r.n > few_rows ? (r.n + tq - 1) / tq : 0;
-        }
-        const int all = scan1024(nb, before, wsum);
-        if (b + t < kv.seqs) first[b + t] = count + before;
-        count += all;
-    }
-    // (starts that do not ascend could claim rows twice: what the scratch has
-    // no room for is left out)
-    count = min(count, cap);
-    __syncthreads();
-    auto slot_of = [&](int u) {
-        int s = 0, hi = kv.seqs; // the last slot with first[s] <= u
-        while (hi - s > 1) {
-            const int mid = (s + hi) >> 1;
-            if (first[mid] <= u) s = mid;
-            else hi = mid;
-        }
-        return s;
-    };
-    // all tiles of one KV head (a block has at most 2^24 / 32, so that 1024 of
-    // them fit an int)
-    long long tiles = 0;
-    for (int b = 0; b < count; b += 1024) {
-        int mine = 0, before;
-        if (b + t < count) {
-            const int s = slot_of(b + t);
-            mine = block_tiles(slot_rows(kv, s), b + t - first[s], tq);
-        }
-        tiles += scan1024(mine, before, wsum);
-    }
-    // Pieces of `each` tiles number fewer than count + tiles / each: no more than
-    // fill the GPU once, where the blocks alone are few (a second round of a
-    // few pieces would take as long as the first: 66 against 40 us for 544
-    // pieces on 512 places); where they are many, only blocks of twice their
-    // share are cut.
-    const int fill = fill_pieces(kv.kvh), room = max(fill - count, (fill + 1) / 2);
-    const int each = (int)max((long long)PR_MIN_TILES, (tiles + room - 1) / room);
-    int npieces = 0, nparts = 0;
-    for (int b = 0; b < count; b += 1024) {
-        int s = 0, n = 0, k = 0, before, pbefore;
-        if (b + t < count) {
-            s = slot_of(b + t);
-            n = block_tiles(slot_rows(kv, s), b + t - first[s], tq);
-            k = (n + each - 1) / each;
-        }
-        const int all = scan1024(k, before, wsum);
-        const int pall = scan1024(k > 1 ? k : 0, pbefore, wsum);
-        if (b + t < count) {
-            blocks[b + t] = Block{s, b + t - first[s], nparts + pbefore, k};
-            for (int i = 0; i < k; ++i)
-                pieces[npieces + before + i] =
-                    Piece{b + t, (int)((long long)n * i / k), (int)((long long)n * (i + 1) / k),
-                          k > 1 ? nparts + pbefore + i : -1};
-        }
-        npieces += all;
-        nparts += pall;
-    }
-    if (t == 0) *plan = Plan{count, npieces, nparts, 0};
-}
 
 __device__ __forceinline__ f32x16 mfma(const half8 &a, const half8 &b, const f32x16 &c)
 {
@@ -199,14 +75,6 @@ __device__ __forceinline__ half4 read_transposed(const _Float16 *p)
     return __builtin_bit_cast(
         half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                    (__attribute__((address_space(3))) short4v *)const_cast<_Float16 *>(p)));
-}
-
-// A vector at a uniform base and an unsigned 32-bit element offset (a scalar
-// base with a vector offset in the load: no 64-bit address per lane).
-template <class V, class T> __device__ __forceinline__ V at(const T *base, unsigned off)
-{
-    return *reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
-                                        (unsigned)(off * sizeof(T)));
 }
 
 // A step's keys and values on their way from memory to LDS: 512 threads, rows
@@ -274,9 +142,7 @@ template <bool LO> struct RowsLds { // one step
 
 template <class T>
 __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
-    PagedKv kv, int tq, const Plan *__restrict__ plan, const Block *__restrict__ blocks,
-    const Piece *__restrict__ pieces, const float *__restrict__ q, float *__restrict__ part,
-    float *__restrict__ out)
+    PagedKv kv, RowsScratch rs, const float *__restrict__ q, float *__restrict__ out)
 {
     constexpr bool LO = sizeof(T) == 4; // low parts of keys and values
     typedef Raw<T> R;
@@ -285,11 +151,12 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         RowsLds<LO> step[2];
         float join[4][JOIN][64];
     } lds;
-    if ((int)blockIdx.y >= plan->pieces) return;
-    const Piece piece = pieces[blockIdx.y];
-    const Block blk = blocks[piece.block];
-    const int kh = blockIdx.x, s = blk.slot;
-    const SlotRows sr = slot_rows(kv, s);
+    // (a piece's KV heads in sequence, so that an XCD, which takes every eighth
+    // workgroup, reads few heads' keys and values into its L2)
+    const int kh = blockIdx.x % kv.kvh, at_piece = blockIdx.x / kv.kvh;
+    const Piece piece = rs.pieces[at_piece]; // (in the scratch, whatever their number)
+    if (at_piece >= rs.plan->pieces) return;
+    const int s = piece.slot, tq = rs.tq;
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), part_of = wave >> 2, rows = wave & 3;
     const int rep = kv.heads / kv.kvh;
@@ -297,9 +164,9 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     const int pmask = (1 << kv.shift) - 1;
     const float sc = 1.4426950408889634f * 0.08838834764831845f; // log2(e) / sqrt(128)
 
-    const int tok0 = blk.index * tq;
-    const int first = sr.len - sr.n; // position of the slot's first new row
-    const int toks = min(tq, sr.n - tok0);
+    const int tok0 = piece.index * tq;
+    const int first = piece.first; // position of the slot's first new row
+    const int toks = min(tq, piece.n - tok0);
     const int p_end = min(piece.t1 * PR_TILE, first + tok0 + toks);
     const int p_begin = piece.t0 * PR_TILE;
     const int all_see = first + tok0; // the last position that every row sees
@@ -367,7 +234,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     // the last position the wave's last row sees, and its first row
     const int wave_last = first + tok0 + min(toks - 1, (32 * rows + 31) / rep);
     const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
-    const size_t row = (size_t)(sr.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
+    const size_t row = (size_t)(piece.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
 
     // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range
     half8 qhi[KV_D / 16], qlo[KV_D / 16];
@@ -423,14 +290,20 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     __syncthreads();
     int buf = 0;
     const int o = 32 * part_of; // this wave's 32 positions of a step
+    // The two waves of a SIMD would go through their products together and then
+    // through the softmax together; with the first half's waves issuing first
+    // they take turns at the matrix unit.
+    if (part_of) __builtin_amdgcn_s_setprio(0);
+    else __builtin_amdgcn_s_setprio(3);
     for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
         const Four after = pages_of(p0 + 2 * PR_TILE);
         const RowsLds<LO> &l = lds.step[buf];
         const int p = p0 + o, pa = part_of ? cur.e[2] : cur.e[0], pb = part_of ? cur.e[3] : cur.e[1];
         if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
-        f32x16 sv;
+        // (two chains of sums: a product waits for the one it adds to)
+        f32x16 sv, sx;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sv[e] = 0.f;
+        for (int e = 0; e < 16; ++e) sv[e] = sx[e] = 0.f;
         // Scores, with the next step's rows converted between their products (the
         // matrix unit takes 32 cycles for each). Operands are read one product
         // ahead, and no further: the barriers to the compiler's scheduling keep
@@ -446,12 +319,16 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         for (int kk = 0; kk < KV_D / 16; ++kk) {
             if (kk + 1 < KV_D / 16) keys(kk + 1);
             sv = mfma(ahi[kk & 1], qhi[kk], sv);
-            sv = mfma(ahi[kk & 1], qlo[kk], sv);
-            if constexpr (LO) sv = mfma(alo[kk & 1], qhi[kk], sv);
+            sx = mfma(ahi[kk & 1], qlo[kk], sx);
+            if constexpr (LO) {
+                if (kk & 1) sv = mfma(alo[kk & 1], qhi[kk], sv);
+                else sx = mfma(alo[kk & 1], qhi[kk], sx);
+            }
             if (kk < 2 * R::N) store(buf ^ 1, kk);
             __builtin_amdgcn_sched_barrier(0);
         }
         load(p0 + 2 * PR_TILE, after);
+        sv += sx;
         if (p + 31 > wave_all || (pa | pb) < 0) { // mask
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -487,24 +364,25 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         l_run += rs[0] + rs[1];
         // operand element 4 x + i of product (kk, j): position 16 kk + 8 x + 4 h + i,
         // which is the lane's weight 8 kk + 4 x + i
-        half8 vhi[2], vlo[2];
+        half8 vhi[4], vlo[4];
         auto values = [&](int n) {
             const int kk = n >> 2, j = n & 3;
             const int vr = o + 16 * kk + 4 * h + ((lane & 15) >> 2);
             const int vd = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
             const half4 x = read_transposed(&l.vhi[vr][vd]),
                         y = read_transposed(&l.vhi[vr + 8][vd]);
-            vhi[n & 1] = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            vhi[n & 3] = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             if constexpr (LO) {
                 const half4 z = read_transposed(&l.vlo[vr][vd]),
                             w = read_transposed(&l.vlo[vr + 8][vd]);
-                vlo[n & 1] = half8{z[0], z[1], z[2], z[3], w[0], w[1], w[2], w[3]};
+                vlo[n & 3] = half8{z[0], z[1], z[2], z[3], w[0], w[1], w[2], w[3]};
             }
         };
         half8 phi, plo;
         values(0);
+        values(1);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        for (int n = 0; n < 8; n += 2) { // two products' sums in turn
             if ((n & 3) == 0) {
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
@@ -516,11 +394,19 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     plo[i + 1] = lo[1];
                 }
             }
-            if (n + 1 < 8) values(n + 1);
-            f32x16 &d = acc[n & 3];
-            d = mfma(vhi[n & 1], phi, d);
-            d = mfma(vhi[n & 1], plo, d);
-            if constexpr (LO) d = mfma(vlo[n & 1], phi, d);
+            if (n + 2 < 8) {
+                values(n + 2);
+                values(n + 3);
+            }
+            f32x16 &d = acc[n & 3], &e = acc[(n + 1) & 3];
+            d = mfma(vhi[n & 3], phi, d);
+            e = mfma(vhi[(n + 1) & 3], phi, e);
+            d = mfma(vhi[n & 3], plo, d);
+            e = mfma(vhi[(n + 1) & 3], plo, e);
+            if constexpr (LO) {
+                d = mfma(vlo[n & 3], phi, d);
+                e = mfma(vlo[(n + 1) & 3], phi, e);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
@@ -580,7 +466,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     float *dst = out + row * KV_D;
     float f = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f; // (saw nothing: zeros)
     if (piece.part >= 0) {
-        dst = part + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
+        dst = rs.parts + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
         if (h == 0) {
             dst[0] = m_run;
             dst[1] = l_run;
@@ -597,100 +483,18 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                             acc[j][4 * g + 3] * f);
 }
 
-// Joins the pieces of a block that was cut, in order. Grid (kv heads, blocks,
-// PR_ROWS / 8): 8 rows, a 32-lane half wave each.
-__global__ __launch_bounds__(256) void paged_rows_merge_kernel(
-    PagedKv kv, int tq, const Plan *__restrict__ plan, const Block *__restrict__ blocks,
-    const float *__restrict__ part, float *__restrict__ out)
-{
-    if ((int)blockIdx.y >= plan->blocks) return;
-    const Block blk = blocks[blockIdx.y];
-    if (blk.pieces < 2) return;
-    const SlotRows sr = slot_rows(kv, blk.slot);
-    const int rep = kv.heads / kv.kvh, kh = blockIdx.x;
-    const int r = blockIdx.z * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
-    const int tl = r / rep;
-    if (tl >= min(tq, sr.n - blk.index * tq)) return;
-    const size_t step = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
-    const float *p = part + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
-    const int lane = threadIdx.x & 31;
-    float M = -INFINITY;
-    for (int i = lane; i < blk.pieces; i += 32) M = fmaxf(M, p[i * step]);
-    M = fmaxf(M, __shfl_xor(M, 16, 32));
-    M = wave::max16(M);
-    const float base = M == -INFINITY ? 0.f : M;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-    for (int b = 0; b < blk.pieces; b += 8) { // eight parts' loads in flight
-        float2 ml[8];
-        float4 v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float *o = p + (size_t)min(b + k, blk.pieces - 1) * step;
-            ml[k] = *reinterpret_cast<const float2 *>(o);
-            v[k] = *reinterpret_cast<const float4 *>(o + 4 + d);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (b + k >= blk.pieces) continue;
-            const float x = __builtin_amdgcn_exp2f(ml[k].x - base);
-            den = fmaf(x, ml[k].y, den);
-            num.x = fmaf(x, v[k].x, num.x);
-            num.y = fmaf(x, v[k].y, num.y);
-            num.z = fmaf(x, v[k].z, num.z);
-            num.w = fmaf(x, v[k].w, num.w);
-        }
-    }
-    const float f = den > 0.f || den != den ? 1.f / den : 0.f;
-    const size_t row = (size_t)(sr.begin + blk.index * tq + tl) * kv.heads + kh * rep + r % rep;
-    *reinterpret_cast<float4 *>(out + row * KV_D + d) =
-        make_float4(num.x * f, num.y * f, num.z * f, num.w * f);
-}
-
-struct RowsScratch {
-    size_t blocks, pieces, parts, bytes;
-};
-RowsScratch rows_layout(int seqs, int kvh, int heads, int rows)
-{
-    const int nb = max_blocks(seqs, rows, PR_ROWS / (heads / kvh));
-    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    RowsScratch r;
-    r.blocks = up(sizeof(Plan));
-    r.pieces = r.blocks + up(nb * sizeof(Block));
-    r.parts = r.pieces + up(max_pieces(nb, kvh) * sizeof(Piece));
-    r.bytes = r.parts + up((size_t)max_parts(kvh) * kvh * PR_ROWS * PAGED_PART * 4);
-    return r;
-}
-
 } // namespace
 
-size_t paged_rows_scratch(int seqs, int kvh, int heads, int rows)
-{
-    return rows_layout(seqs, kvh, heads, rows).bytes;
-}
-
-int launch_paged_rows(const PagedKv &kv, const float *q, void *scratch, float *out, void *stream)
+int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, float *out,
+                      void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
-    const int rep = kv.heads / kv.kvh, tq = PR_ROWS / rep;
-    const int nb = max_blocks(kv.seqs, kv.rows, tq);
-    const RowsScratch l = rows_layout(kv.seqs, kv.kvh, kv.heads, kv.rows);
-    char *base = (char *)scratch;
-    Plan *plan = (Plan *)base;
-    Block *blocks = (Block *)(base + l.blocks);
-    Piece *pieces = (Piece *)(base + l.pieces);
-    float *part = (float *)(base + l.parts);
-    hipLaunchKernelGGL(paged_rows_plan_kernel, dim3(1), dim3(1024), (size_t)kv.seqs * 4, st,
-                       kv, paged_few_rows(rep), tq, nb, plan, blocks, pieces);
-    const dim3 grid(kv.kvh, max_pieces(nb, kv.kvh));
+    const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh);
     if (kv.f16)
-        hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(PR_THREADS), 0, st, kv, tq,
-                           plan, blocks, pieces, q, part, out);
+        hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(PR_THREADS), 0, st, kv, rs, q,
+                           out);
     else
-        hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(PR_THREADS), 0, st, kv, tq, plan,
-                           blocks, pieces, q, part, out);
-    hipLaunchKernelGGL(paged_rows_merge_kernel, dim3(kv.kvh, nb, PR_ROWS / 8), dim3(256), 0, st,
-                       kv, tq, plan, blocks, part, out);
+        hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(PR_THREADS), 0, st, kv, rs, q, out);
     return (int)hipGetLastError();
 }
 
