@@ -267,9 +267,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                 split2(v[i] * inv, v[i + 1] * inv, hi, lo);
                 qhi[kk][i] = hi[0];
                 qhi[kk][i + 1] = hi[1];
-                // (an infinite query: its difference with itself is a NaN)
-                qlo[kk][i] = lo[0] == lo[0] ? lo[0] : (_Float16)0.f;
-                qlo[kk][i + 1] = lo[1] == lo[1] ? lo[1] : (_Float16)0.f;
+                qlo[kk][i] = lo[0];
+                qlo[kk][i + 1] = lo[1];
             }
         }
     }

@@ -15,6 +15,8 @@ namespace hyq {
 
 namespace {
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ int held_pages(int len, int shift, int stride)
 {
     return min((int)(((long long)max(len, 0) + (1 << shift) - 1) >> shift), stride);
@@ -62,6 +64,44 @@ __global__ __launch_bounds__(256) void pages_count_kernel(PagesArgs a, const int
         const int p = table[(size_t)s * a.stride + i];
         if ((unsigned)p < (unsigned)a.npages) atomicAdd(refs + p, 1);
     }
+}
+
+// Both by one workgroup, the counts in LDS, where table and pool are small: one
+// launch instead of two.
+constexpr int SMALL_PAGES = 4096, SMALL_SLOTS = 1024, SMALL_ENTRIES = 16384;
+__global__ __launch_bounds__(1024) void pages_fork_small_kernel(
+    PagesArgs a, const int *__restrict__ parent, const int *__restrict__ keep,
+    const int *__restrict__ table, const int *__restrict__ len, int *__restrict__ table_out,
+    int *__restrict__ len_out, int *__restrict__ refs_out)
+{
+    extern __shared__ int count[]; // [npages]
+    __shared__ int from[SMALL_SLOTS], used[SMALL_SLOTS];
+    const int t = threadIdx.x;
+    for (int i = t; i < a.npages; i += 1024) count[i] = 0;
+    if (t < a.seqs) {
+        const int p = parent[t];
+        int got = 0;
+        if ((unsigned)p < (unsigned)a.seqs) {
+            got = (int)min((long long)max(len[p], 0), (long long)a.stride << a.shift);
+            if (keep) got = min(got, max(keep[t], 0));
+        }
+        len_out[t] = got;
+        from[t] = p;
+        used[t] = held_pages(got, a.shift, a.stride);
+    }
+    __syncthreads();
+    const int n = a.seqs * a.stride;
+    for (int i = t; i < n; i += 1024) {
+        const int s = i / a.stride, e = i - s * a.stride;
+        int p = -1;
+        if (e < used[s]) {
+            p = table[from[s] * a.stride + e];
+            if ((unsigned)p < (unsigned)a.npages) atomicAdd(count + p, 1);
+        }
+        table_out[i] = p;
+    }
+    __syncthreads();
+    for (int i = t; i < a.npages; i += 1024) refs_out[i] = count[i];
 }
 
 // ---- extend ----
@@ -251,6 +291,89 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(
     if (t == 0) w.count[0] = ncopies;
 }
 
+// The same for at most SMALL_SLOTS slots and SMALL_PAGES pages, a slot and four
+// pages per thread, with the counts in LDS: what the larger form does in rounds
+// of global memory takes a load, a dependent load and a few barriers (21 -> 8 us
+// for 8 slots and 260 pages).
+__global__ __launch_bounds__(1024) void pages_extend_small_kernel(
+    PagesArgs a, const int *__restrict__ add, const int *table, const int *len, const int *refs,
+    int *table_out, int *len_out, int *refs_out, int *__restrict__ status, void *scratch)
+{
+    extern __shared__ int lds[];
+    __shared__ int wsum[16];
+    const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
+    int *const lrefs = lds, *const asks = lrefs + a.npages;
+    unsigned *const top = (unsigned *)(asks + a.npages);
+    int *const free = asks; // (once the asks are counted)
+    const int t = threadIdx.x, s = t;
+    constexpr int EACH = SMALL_PAGES / 1024;
+    int r[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) r[i] = refs[min(EACH * t + i, a.npages - 1)];
+    Ask k{};
+    int n = 0;
+    if (s < a.seqs) {
+        k = ask_of(a, add, table, len, s);
+        n = max(len[s], 0);
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (EACH * t + i < a.npages) {
+            lrefs[EACH * t + i] = r[i];
+            asks[EACH * t + i] = 0;
+            top[EACH * t + i] = 0;
+        }
+    if (table_out != table)
+        for (int i = t; i < a.seqs * a.stride; i += 1024) table_out[i] = table[i];
+    __syncthreads();
+    const bool shared = k.partial && lrefs[k.last] > 1;
+    const unsigned key = (unsigned)k.fill << 16 | (65535u - s);
+    if (shared) {
+        atomicAdd(asks + k.last, 1);
+        atomicMax(top + k.last, key);
+    }
+    __syncthreads();
+    const bool copies = shared && !(asks[k.last] == lrefs[k.last] && top[k.last] == key);
+    const int need = k.asks ? k.wants - k.held + copies : 0;
+    int before, fbefore, cbefore, is = 0;
+    const int total = scan1024(need, before, wsum);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) is += EACH * t + i < a.npages && r[i] == 0;
+    const int found = scan1024(is, fbefore, wsum);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (EACH * t + i < a.npages && r[i] == 0 && fbefore < total) free[fbefore++] = EACH * t + i;
+    const bool served = k.asks && (need == 0 || before + need <= found);
+    const int ncopies = scan1024(served && copies, cbefore, wsum); // (and the list is whole)
+    if (s < a.seqs) {
+        if (served) {
+            int at = before;
+            int *row = table_out + (size_t)s * a.stride;
+            if (copies) {
+                const int p = free[at++];
+                row[k.held - 1] = p;
+                lrefs[p] = 1;
+                atomicSub(lrefs + k.last, 1);
+                int *c = w.list + 3 * cbefore;
+                c[0] = k.last;
+                c[1] = p;
+                c[2] = k.fill;
+            }
+            for (int i = k.held; i < k.wants; ++i) {
+                const int p = free[at++];
+                row[i] = p;
+                lrefs[p] = 1;
+            }
+            n += add[s];
+        }
+        len_out[s] = n;
+        status[s] = k.is_long ? 2 : k.asks && !served ? 1 : 0;
+    }
+    if (t == 0) w.count[0] = ncopies;
+    __syncthreads();
+    for (int i = t; i < a.npages; i += 1024) refs_out[i] = lrefs[i];
+}
+
 // Copies the filled rows of the pages on the list: one wave per (page, layer,
 // keys or values, head), rows of contiguous 16-byte words.
 __global__ __launch_bounds__(256) void pages_fill_kernel(PagesArgs a, char *pool, void *scratch)
@@ -265,10 +388,18 @@ __global__ __launch_bounds__(256) void pages_fill_kernel(PagesArgs a, char *pool
         const int c = (int)(i / per), r = (int)(i % per);
         const int *e = w.list + 3 * c;
         const size_t at = (size_t)(r / (2 * a.kvh)) * a.npages * page + (size_t)(r % (2 * a.kvh)) * head;
-        const uint4 *src = reinterpret_cast<const uint4 *>(pool + at + e[0] * page);
-        uint4 *dst = reinterpret_cast<uint4 *>(pool + at + e[1] * page);
+        const u32x4 *src = reinterpret_cast<const u32x4 *>(pool + at + e[0] * page);
+        u32x4 *dst = reinterpret_cast<u32x4 *>(pool + at + e[1] * page);
         const int words = (int)(e[2] * row / 16);
-        for (int x = lane; x < words; x += 64) dst[x] = src[x];
+        // (eight loads in flight, those past the end of the last word again)
+        for (int x = lane; x < words; x += 512) {
+            u32x4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = src[min(x + 64 * k, words - 1)];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (x + 64 * k < words) dst[x + 64 * k] = v[k];
+        }
     }
 }
 
@@ -332,16 +463,16 @@ __global__ __launch_bounds__(256) void pages_move_kernel(PagesArgs a, char *pool
     for (long long i = blockIdx.x; i < items; i += gridDim.x) {
         const int m = (int)(i / per), r = (int)(i % per), cut = r % cuts;
         const size_t layer = (size_t)(r / cuts) * a.npages * page + (size_t)cut * COMPACT_BYTES;
-        const uint4 *src = reinterpret_cast<const uint4 *>(pool + layer + w.list[m] * page);
-        uint4 *dst = reinterpret_cast<uint4 *>(pool + layer + w.free[m] * page);
+        const u32x4 *src = reinterpret_cast<const u32x4 *>(pool + layer + w.list[m] * page);
+        u32x4 *dst = reinterpret_cast<u32x4 *>(pool + layer + w.free[m] * page);
         const int words = (int)min((size_t)COMPACT_BYTES, page - (size_t)cut * COMPACT_BYTES) / 16;
-        uint4 v[COMPACT_BYTES / 4096];
+        u32x4 v[COMPACT_BYTES / 4096];
 #pragma unroll
         for (int k = 0; k < COMPACT_BYTES / 4096; ++k)
-            if (t + 256 * k < words) v[k] = src[t + 256 * k];
+            v[k] = __builtin_nontemporal_load(src + min(t + 256 * k, words - 1));
 #pragma unroll
         for (int k = 0; k < COMPACT_BYTES / 4096; ++k)
-            if (t + 256 * k < words) dst[t + 256 * k] = v[k];
+            if (t + 256 * k < words) __builtin_nontemporal_store(v[k], dst + t + 256 * k);
     }
     const size_t n = (size_t)a.seqs * a.stride;
     for (size_t i = (size_t)blockIdx.x * 256 + t; i < n; i += (size_t)gridDim.x * 256) {
@@ -361,6 +492,11 @@ int launch_pages_fork(const PagesArgs &a, const int *parent, const int *keep, co
                       const int *len, int *table_out, int *len_out, int *refs_out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
+    if (a.npages <= SMALL_PAGES && a.seqs <= SMALL_SLOTS && a.seqs * a.stride <= SMALL_ENTRIES) {
+        hipLaunchKernelGGL(pages_fork_small_kernel, dim3(1), dim3(1024), (size_t)a.npages * 4, st,
+                           a, parent, keep, table, len, table_out, len_out, refs_out);
+        return (int)hipGetLastError();
+    }
     const int clears = std::min(64, (a.npages + 255) / 256);
     hipLaunchKernelGGL(pages_fork_kernel, dim3(a.seqs + clears), dim3(256), 0, st, a, parent, keep,
                        table, len, table_out, len_out, refs_out);
@@ -374,8 +510,14 @@ int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const in
                         int *refs_out, int *status, void *scratch, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len, refs,
-                       table_out, len_out, refs_out, status, scratch);
+    // (a table that is copied as well: by one workgroup while it is small)
+    if (a.npages <= SMALL_PAGES && a.seqs <= SMALL_SLOTS)
+        hipLaunchKernelGGL(pages_extend_small_kernel, dim3(1), dim3(1024), (size_t)a.npages * 12,
+                           st, a, add, table, len, refs, table_out, len_out, refs_out, status,
+                           scratch);
+    else
+        hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len,
+                           refs, table_out, len_out, refs_out, status, scratch);
     hipLaunchKernelGGL(pages_fill_kernel, dim3(1024), dim3(256), 0, st, a, (char *)pool, scratch);
     return (int)hipGetLastError();
 }
