@@ -518,7 +518,7 @@ int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const in
     else
         hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len,
                            refs, table_out, len_out, refs_out, status, scratch);
-    hipLaunchKernelGGL(pages_fill_kernel, dim3(1024), dim3(256), 0, st, a, (char *)pool, scratch);
+    hipLaunchKernelGGL(pages_fill_kernel, dim3(2048), dim3(256), 0, st, a, (char *)pool, scratch);
     return (int)hipGetLastError();
 }
 
