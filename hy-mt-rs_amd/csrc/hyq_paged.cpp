@@ -300,6 +300,7 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
         rs.plan = (Plan *)base;
         rs.blocks = (Block *)(base + l.blocks);
         rs.pieces = (Piece *)(base + l.pieces);
+        rs.groups = (int *)(base + l.groups);
         rs.parts = (float *)(base + l.parts);
         rs.tq = PR_ROWS / (kv.heads / kv.kvh);
         rs.cap = max_blocks(kv.seqs, kv.rows, rs.tq);

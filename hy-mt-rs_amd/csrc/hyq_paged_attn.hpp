@@ -47,7 +47,8 @@ constexpr int PR_MIN_TILES = 2;     // the shortest piece worth its partial rows
 
 // A block of a slot's new tokens, and what its pieces left.
 struct Block {
-    int slot, index, part, pieces; // first partial block and pieces of the block
+    int row, toks;    // its first packed row and its tokens
+    int part, pieces; // its first partial block and its pieces
 };
 // A range of steps of a block, with what its workgroup needs to begin.
 struct Piece {
@@ -56,22 +57,21 @@ struct Piece {
     int begin, n, first; // the slot's rows, and the first one's position
 };
 struct Plan {
-    int blocks, pieces, parts, unused;
+    int blocks, groups, unused[2];
 };
 
 // Pieces that fill the GPU with kvh workgroups each (at least one).
 __host__ __device__ inline int fill_pieces(int kvh) { return PR_FILL > kvh ? PR_FILL / kvh : 1; }
 inline int max_blocks(int seqs, int rows, int tq) { return rows / tq + std::min(seqs, rows); }
-// At most fill_pieces, or the sum of ceil(n / each) with each >= tiles / room and
-// room <= fill_pieces, where a block that is cut (n > each) has fewer than
-// 2 n / each pieces.
+// Pieces: at most fill_pieces cuts. A block that is cut c times leaves c + 1 <=
+// 2 c parts. Groups: a piece each, or fill_pieces.
 inline int max_pieces(int blocks, int kvh) { return blocks + fill_pieces(kvh); }
 inline int max_parts(int kvh) { return 2 * fill_pieces(kvh); }
-// Workgroups of the merge: for every KV head a row of a slot each, and eight
-// rows of a block each.
-inline long long merge_groups(int seqs, int kvh, int part_rows, int cap)
+// Workgroups of the merge: `each` of a slot and one per eight rows of a block,
+// for every KV head.
+inline long long merge_groups(int seqs, int kvh, int each, int cap)
 {
-    return ((long long)seqs * part_rows + (long long)cap * (PR_ROWS / 8)) * kvh;
+    return ((long long)seqs * each + (long long)cap * (PR_ROWS / 8)) * kvh;
 }
 
 // Where in the scratch the plan's parts lie.
@@ -79,11 +79,12 @@ struct RowsScratch {
     Plan *plan;
     Block *blocks;
     Piece *pieces;
+    int *groups; // a workgroup's first piece; one more entry than groups
     float *parts;
     int tq, cap; // tokens of a block, blocks there is room for (0: no tile form)
 };
 struct RowsLayout {
-    size_t blocks, pieces, parts, bytes;
+    size_t blocks, pieces, groups, parts, bytes;
 };
 inline RowsLayout rows_layout(int seqs, int kvh, int heads, int rows)
 {
@@ -92,7 +93,8 @@ inline RowsLayout rows_layout(int seqs, int kvh, int heads, int rows)
     RowsLayout r;
     r.blocks = up(sizeof(Plan));
     r.pieces = r.blocks + up(nb * sizeof(Block));
-    r.parts = r.pieces + up(max_pieces(nb, kvh) * sizeof(Piece));
+    r.groups = r.pieces + up(max_pieces(nb, kvh) * sizeof(Piece));
+    r.parts = r.groups + up((max_pieces(nb, kvh) + 1) * sizeof(int));
     r.bytes = r.parts + up((size_t)max_parts(kvh) * kvh * PR_ROWS * PAGED_PART * 4);
     return r;
 }
@@ -169,65 +171,97 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
         }
         tiles += scan256(mine, before, wsum);
     }
-    // The least length of a piece, of sixteen, with which the pieces number no
-    // more than fill the GPU once: a second round of a few would take as long
-    // as the first. `most` does so where the blocks alone are few; where they
-    // are many, it is twice their share, and only blocks longer than that are
-    // cut.
+    // Two ways to cut. A workgroup per piece, every block in equal pieces of at
+    // most `each` steps: the least length, of sixteen, with which the pieces
+    // number no more than fill the GPU once (a second round of a few would take
+    // as long as the first), or `most`, of which that is sure unless the blocks
+    // alone are many. Or, where that leaves the longest piece more than
+    // GROUP_COST steps above the mean, the blocks' steps in sequence in equal
+    // shares, a workgroup going through the pieces of its share (it begins and
+    // ends each, which takes about as long as GROUP_COST steps).
+    constexpr int GROUP_COST = 4;
     const int fill = fill_pieces(kv.kvh), room = max(fill - count, (fill + 1) / 2);
     const int least = (int)max((long long)PR_MIN_TILES, (tiles + fill - 1) / fill);
     const int most = (int)max((long long)PR_MIN_TILES, (tiles + room - 1) / room);
     auto length = [&](int i) { return least + (int)((long long)(most - least) * i / (TRIES - 1)); };
-    int each = most;
-    if (most > least) {
-        int n[TRIES];
+    int n[TRIES], longest = 0;
 #pragma unroll
-        for (int i = 0; i < TRIES; ++i) n[i] = 0;
-        for (int b = t; b < count; b += 256) {
-            const int s = slot_of(b), x = block_tiles(slot_rows(kv, s), b - first[s], tq);
+    for (int i = 0; i < TRIES; ++i) n[i] = 0;
+    for (int b = t; b < count; b += 256) {
+        const int s = slot_of(b), x = block_tiles(slot_rows(kv, s), b - first[s], tq);
+        longest = max(longest, x);
 #pragma unroll
-            for (int i = 0; i < TRIES; ++i) n[i] += (x + length(i) - 1) / length(i);
-        }
-#pragma unroll
-        for (int i = 0; i < TRIES; ++i) {
-            n[i] = wave::sum64(n[i]);
-            if (lane == 0) sums[wave][i] = n[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = TRIES - 1; i >= 0; --i)
-            if (sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i] <= fill) each = length(i);
+        for (int i = 0; i < TRIES; ++i) n[i] += (x + length(i) - 1) / length(i);
     }
+#pragma unroll
+    for (int i = 0; i < TRIES; ++i) {
+        n[i] = wave::sum64(n[i]);
+        if (lane == 0) sums[wave][i] = n[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+    __syncthreads(); // (wsum's readers in the scan above)
+    if (lane == 0) wsum[wave] = longest;
+    __syncthreads();
+    longest = max(max(wsum[0], wsum[1]), max(wsum[2], wsum[3]));
+    int each = most;
+    bool once = false;
+#pragma unroll
+    for (int i = TRIES - 1; i >= 0; --i)
+        if (sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i] <= fill) {
+            each = length(i);
+            once = true;
+        }
+    const bool shares = !once || min(each, longest) > least + GROUP_COST;
     int npieces = 0, nparts = 0;
+    long long done = 0; // steps before this round's blocks
     for (int b = 0; b < count; b += 256) {
-        int s = 0, n = 0, k = 0, before, pbefore;
+        int s = 0, x = 0, k = 0, before, pbefore, xbefore;
         SlotRows r{};
         if (b + t < count) {
             s = slot_of(b + t);
             r = slot_rows(kv, s);
-            n = block_tiles(r, b + t - first[s], tq);
-            k = (n + each - 1) / each;
+            x = block_tiles(r, b + t - first[s], tq);
         }
+        const int xall = scan256(x, xbefore, wsum);
+        const long long at = done + xbefore; // the block's first step in the sequence
+        const int share = (int)(at / least);
+        if (x) k = shares ? (int)((at + x - 1) / least) - share + 1 : (x + each - 1) / each;
         const int all = scan256(k, before, wsum);
         const int pall = scan256(k > 1 ? k : 0, pbefore, wsum);
-        if (b + t < count) {
+        if (x) {
             const int index = b + t - first[s];
-            rs.blocks[b + t] = Block{s, index, nparts + pbefore, k};
-            for (int i = 0; i < k; ++i)
-                rs.pieces[npieces + before + i] =
-                    Piece{s,
-                          index,
-                          (int)((long long)n * i / k),
-                          (int)((long long)n * (i + 1) / k),
-                          k > 1 ? nparts + pbefore + i : -1,
-                          r.begin,
-                          r.n,
-                          r.len - r.n};
+            rs.blocks[b + t] = Block{r.begin + index * tq, min(tq, r.n - index * tq),
+                                     nparts + pbefore, k};
+            for (int i = 0; i < k; ++i) {
+                const int piece = npieces + before + i;
+                long long t0 = (long long)x * i / k, t1 = (long long)x * (i + 1) / k;
+                if (shares) {
+                    t0 = max(0ll, (long long)(share + i) * least - at);
+                    t1 = min((long long)x, (long long)(share + i + 1) * least - at);
+                    if ((at + t0) % least == 0) rs.groups[share + i] = piece;
+                } else {
+                    rs.groups[piece] = piece;
+                }
+                rs.pieces[piece] = Piece{s,
+                                         index,
+                                         (int)t0,
+                                         (int)t1,
+                                         k > 1 ? nparts + pbefore + i : -1,
+                                         r.begin,
+                                         r.n,
+                                         r.len - r.n};
+            }
         }
         npieces += all;
         nparts += pall;
+        done += xall;
     }
-    if (t == 0) *rs.plan = Plan{count, npieces, nparts, 0};
+    if (t == 0) {
+        const int groups = shares ? (int)((tiles + least - 1) / least) : npieces;
+        rs.groups[groups] = npieces;
+        *rs.plan = Plan{count, groups, {0, 0}};
+    }
 }
 
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)

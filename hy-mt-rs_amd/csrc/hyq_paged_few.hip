@@ -40,6 +40,7 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int FEW_WAVES = 4;
@@ -481,13 +482,50 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     }
 }
 
-// Joins the parts of one row of a unit that several workers shared, by 256
-// threads: wave g takes the parts g, g + 4, ..., lane d dims 2 d and 2 d + 1,
-// with eight parts' loads in flight; the waves' sums are added in a fixed order.
+// One row's parts p, p + step, ..., n of them, eight in flight: the running
+// maximum m, exp-sum l and a lane's sums x.
+template <class V> struct Joined {
+    float m = -INFINITY, l = 0.f;
+    V x{};
+    __device__ __forceinline__ void add(const float *p, size_t step, int n, int d)
+    {
+        for (int b = 0; b < n; b += 8) {
+            float2v ml[8];
+            V v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float *o = p + (size_t)min(b + k, n - 1) * step;
+                ml[k] = *reinterpret_cast<const float2v *>(o);
+                v[k] = *reinterpret_cast<const V *>(o + 4 + d);
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k][0]);
+            const float base = top == -INFINITY ? 0.f : top;
+            const float c = __builtin_amdgcn_exp2f(m - base);
+            l *= c;
+            x *= c;
+            m = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float w = b + k < n ? __builtin_amdgcn_exp2f(ml[k][0] - base) : 0.f;
+                l = fmaf(w, ml[k][1], l);
+                x += w * v[k];
+            }
+        }
+    }
+    // what the row's sums are to be multiplied with (a row that saw nothing: 0)
+    __device__ __forceinline__ float scale() const { return l > 0.f || l != l ? 1.f / l : 0.f; }
+};
+
+// Joins the parts of a slot's rows over a KV head, where several workers shared
+// them, by 256 threads, lane d dims 2 d and 2 d + 1. wide: row c by all four
+// waves, a quarter of the parts each, joined in wave order; otherwise rows c ..
+// c + 3, one per wave.
 template <int TILE>
 __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int max_workers,
                                           int part_rows, const float *__restrict__ part,
-                                          float *__restrict__ out, int kh, int s, int c,
+                                          float *__restrict__ out, int kh, int s, int c, bool wide,
                                           long long *before)
 {
     __shared__ long long wsum[4];
@@ -505,105 +543,71 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int m
     const int w0 = worker(first), n = worker(last) - w0 + 1;
     if (n == 1) return; // written whole
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int r = wide ? c : c + g;
+    if (!wide && r >= sr.n * rep) return;
     const size_t step = (size_t)part_rows * PAGED_PART;
-    const float *p = part +
-                     ((size_t)((long long)w0 + (long long)s * kv.kvh + kh) * part_rows + c) *
-                         PAGED_PART;
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 64) M = fmaxf(M, p[i * step]);
-    M = wave::max64(M);
-    const float base = M == -INFINITY ? 0.f : M;
-    float den = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int b = g; b < n; b += 32) {
-        float2 ml[8], v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float *o = p + (size_t)min(b + 4 * k, n - 1) * step;
-            ml[k] = *reinterpret_cast<const float2 *>(o);
-            v[k] = *reinterpret_cast<const float2 *>(o + 4 + 2 * lane);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (b + 4 * k >= n) continue;
-            const float w = __builtin_amdgcn_exp2f(ml[k].x - base);
-            den = fmaf(w, ml[k].y, den);
-            x0 = fmaf(w, v[k].x, x0);
-            x1 = fmaf(w, v[k].y, x1);
-        }
+    const float *p = part + ((size_t)((long long)w0 + (long long)s * kv.kvh + kh) * part_rows + r) *
+                                PAGED_PART;
+    const int a = wide ? n * g / 4 : 0, b = wide ? n * (g + 1) / 4 : n;
+    Joined<float2v> j;
+    j.add(p + (size_t)a * step, step, b - a, 2 * lane);
+    float *o = out + ((size_t)(sr.begin + r / rep) * kv.heads + kh * rep + r % rep) * KV_D;
+    if (!wide) {
+        *reinterpret_cast<float2v *>(o + 2 * lane) = j.x * j.scale();
+        return;
     }
-    red[g][2 * lane] = x0;
-    red[g][2 * lane + 1] = x1;
-    if (lane == 0) red[g][KV_D] = den;
+    red[g][2 * lane] = j.x[0];
+    red[g][2 * lane + 1] = j.x[1];
+    if (lane == 0) {
+        red[g][KV_D] = j.m;
+        red[g][KV_D + 1] = j.l;
+    }
     __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= KV_D) return;
-    den = (red[0][KV_D] + red[1][KV_D]) + (red[2][KV_D] + red[3][KV_D]);
-    const float num = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
-    const size_t row = (size_t)(sr.begin + c / rep) * kv.heads + kh * rep + c % rep;
-    out[row * KV_D + d] = den > 0.f || den != den ? num / den : 0.f;
+    if (g) return;
+    const float M = fmaxf(fmaxf(red[0][KV_D], red[1][KV_D]), fmaxf(red[2][KV_D], red[3][KV_D]));
+    const float base = M == -INFINITY ? 0.f : M;
+    j.l = 0.f;
+    j.x = float2v{0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(red[w][KV_D] - base);
+        j.l = fmaf(f, red[w][KV_D + 1], j.l);
+        j.x += f * float2v{red[w][2 * lane], red[w][2 * lane + 1]};
+    }
+    *reinterpret_cast<float2v *>(o + 2 * lane) = j.x * j.scale();
 }
 
-// Joins the pieces of a block that was cut, in order, by 256 threads: 8 rows, a
-// 32-lane half wave each.
+// Joins the pieces of a block that was cut, by 256 threads: 8 rows, a 32-lane
+// half wave each, lane d dims 4 d ..
 __device__ __forceinline__ void merge_rows(const PagedKv &kv, const RowsScratch &rs,
                                            float *__restrict__ out, int kh, int b, int row8)
 {
-    if (b >= rs.plan->blocks) return;
     const Block blk = rs.blocks[b];
-    if (blk.pieces < 2) return;
-    const SlotRows sr = slot_rows(kv, blk.slot);
+    if (b >= rs.plan->blocks || blk.pieces < 2) return;
     const int rep = kv.heads / kv.kvh;
-    const int r = row8 * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
-    const int tl = r / rep;
-    if (tl >= min(rs.tq, sr.n - blk.index * rs.tq)) return;
-    const size_t step = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
-    const float *p = rs.parts + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
-    const int lane = threadIdx.x & 31;
-    float M = -INFINITY;
-    for (int i = lane; i < blk.pieces; i += 32) M = fmaxf(M, p[i * step]);
-    M = fmaxf(M, __shfl_xor(M, 16, 32));
-    M = wave::max16(M);
-    const float base = M == -INFINITY ? 0.f : M;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-    for (int b = 0; b < blk.pieces; b += 8) { // eight parts' loads in flight
-        float2 ml[8];
-        float4 v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float *o = p + (size_t)min(b + k, blk.pieces - 1) * step;
-            ml[k] = *reinterpret_cast<const float2 *>(o);
-            v[k] = *reinterpret_cast<const float4 *>(o + 4 + d);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (b + k >= blk.pieces) continue;
-            const float x = __builtin_amdgcn_exp2f(ml[k].x - base);
-            den = fmaf(x, ml[k].y, den);
-            num.x = fmaf(x, v[k].x, num.x);
-            num.y = fmaf(x, v[k].y, num.y);
-            num.z = fmaf(x, v[k].z, num.z);
-            num.w = fmaf(x, v[k].w, num.w);
-        }
-    }
-    const float f = den > 0.f || den != den ? 1.f / den : 0.f;
-    const size_t row = (size_t)(sr.begin + blk.index * rs.tq + tl) * kv.heads + kh * rep + r % rep;
-    *reinterpret_cast<float4 *>(out + row * KV_D + d) =
-        make_float4(num.x * f, num.y * f, num.z * f, num.w * f);
+    const int r = row8 * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31), tl = r / rep;
+    if (tl >= blk.toks) return;
+    Joined<f32x4> j;
+    j.add(rs.parts + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART,
+          (size_t)kv.kvh * PR_ROWS * PAGED_PART, blk.pieces, d);
+    *reinterpret_cast<f32x4 *>(out + ((size_t)(blk.row + tl) * kv.heads + kh * rep + r % rep) * KV_D +
+                               d) = j.x * j.scale();
 }
 
-// Grid: merge_groups workgroups, the KV heads of a row or block in sequence.
+// Grid: the slots' rows, one or four a workgroup, then the blocks', eight a
+// workgroup; the KV heads of a row in sequence.
 template <int TILE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_rows, int max_workers,
-                                                          int part_rows, RowsScratch rs,
+                                                          int part_rows, int wide, RowsScratch rs,
                                                           const float *__restrict__ part,
                                                           float *__restrict__ out)
 {
     extern __shared__ long long before[];
-    const int kh = blockIdx.x % kv.kvh, i = blockIdx.x / kv.kvh, n = kv.seqs * part_rows;
+    const int each = wide ? part_rows : (part_rows + 3) / 4; // workgroups of a slot and KV head
+    const int kh = blockIdx.x % kv.kvh, i = blockIdx.x / kv.kvh, n = kv.seqs * each;
     if (i < n)
-        merge_few<TILE>(kv, few_rows, max_workers, part_rows, part, out, kh, i / part_rows, i % part_rows,
-                        before);
+        merge_few<TILE>(kv, few_rows, max_workers, part_rows, part, out, kh, i / each,
+                        (i % each) * (wide ? 1 : 4), wide != 0, before);
     else
         merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / 8), (i - n) % (PR_ROWS / 8));
 }
@@ -642,13 +646,17 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
-    const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, part_rows, rs.cap));
+    // Few rows have many parts each (2048 workers over four slots: 128), which
+    // all of a workgroup's waves read; many rows have few.
+    const int wide = kv.seqs * kv.kvh * part_rows <= 1024;
+    const int each = wide ? part_rows : (part_rows + 3) / 4;
+    const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, each, rs.cap));
     if (kv.f16)
         hipLaunchKernelGGL(paged_merge_kernel<Ops<_Float16>::TILE>, grid, dim3(256), lds, st, kv,
-                           few, FEW_MAX_WORKERS, part_rows, rs, part, out);
+                           few, FEW_MAX_WORKERS, part_rows, wide, rs, part, out);
     else
         hipLaunchKernelGGL(paged_merge_kernel<Ops<float>::TILE>, grid, dim3(256), lds, st, kv, few,
-                           FEW_MAX_WORKERS, part_rows, rs, part, out);
+                           FEW_MAX_WORKERS, part_rows, wide, rs, part, out);
     return (int)hipGetLastError();
 }
 

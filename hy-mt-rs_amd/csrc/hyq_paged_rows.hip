@@ -151,11 +151,15 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         RowsLds<LO> step[2];
         float join[4][JOIN][64];
     } lds;
-    // (a piece's KV heads in sequence, so that an XCD, which takes every eighth
+    // (a group's KV heads in sequence, so that an XCD, which takes every eighth
     // workgroup, reads few heads' keys and values into its L2)
-    const int kh = blockIdx.x % kv.kvh, at_piece = blockIdx.x / kv.kvh;
-    const Piece piece = rs.pieces[at_piece]; // (in the scratch, whatever their number)
-    if (at_piece >= rs.plan->pieces) return;
+    const int kh = blockIdx.x % kv.kvh, group = blockIdx.x / kv.kvh;
+    const int from = rs.groups[group], to = rs.groups[group + 1]; // (read whatever their number)
+    if (group >= rs.plan->groups) return;
+#pragma unroll 1
+    for (int at_piece = from; at_piece < to; ++at_piece) {
+    if (at_piece > from) __syncthreads(); // the last piece's readers of LDS are done
+    const Piece piece = rs.pieces[at_piece];
     const int s = piece.slot, tq = rs.tq;
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), part_of = wave >> 2, rows = wave & 3;
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             for (int e = 0; e < 16; ++e) o[2 + 16 * j + e][lane] = acc[j][e];
     }
     __syncthreads();
-    if (part_of || !ok) return;
+    if (part_of || !ok) continue;
     {
         const float(*o)[64] = lds.join[rows];
         const float m2 = o[0][lane], m = fmaxf(m_run, m2), base = m == -INFINITY ? 0.f : m;
@@ -480,6 +484,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             *reinterpret_cast<float4 *>(dst + 32 * j + 8 * g + 4 * h) =
                 make_float4(acc[j][4 * g] * f, acc[j][4 * g + 1] * f, acc[j][4 * g + 2] * f,
                             acc[j][4 * g + 3] * f);
+    }
 }
 
 } // namespace
@@ -488,7 +493,7 @@ int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, 
                       void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh);
+    const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh); // (more groups there are not)
     if (kv.f16)
         hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(PR_THREADS), 0, st, kv, rs, q,
                            out);
