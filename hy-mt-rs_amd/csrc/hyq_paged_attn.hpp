@@ -128,14 +128,23 @@ __device__ __forceinline__ int scan256(int mine, int &before, int *wsum)
     return all;
 }
 
-// The plan, by one workgroup of 256 threads. first: LDS of seqs ints.
+// x / y for 0 <= x, 1 <= y: 32-bit division where it serves.
+__device__ __forceinline__ int divide(long long x, int y)
+{
+    return x >> 31 ? (int)(x / y) : (int)((unsigned)x / (unsigned)y);
+}
+
+// The plan, by one workgroup of 256 threads. first: LDS of seqs ints. (The tile
+// form's launch waits for it: a round of up to 256 blocks is read and counted
+// once, and its scans are few.)
 __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const RowsScratch &rs,
                                           int *first)
 {
     constexpr int TRIES = 16;
     __shared__ int wsum[4];
-    __shared__ int sums[4][TRIES];
+    __shared__ int sums[TRIES], steps[256];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tq = rs.tq;
+    if (t < TRIES) sums[t] = 0;
     int count = 0;
     for (int b = 0; b < kv.seqs; b += 256) {
         int nb = 0, before;
@@ -151,25 +160,35 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
     // no room for is left out)
     count = min(count, rs.cap);
     __syncthreads();
-    auto slot_of = [&](int u) {
-        int s = 0, hi = kv.seqs; // the last slot with first[s] <= u
-        while (hi - s > 1) {
-            const int mid = (s + hi) >> 1;
-            if (first[mid] <= u) s = mid;
+    // block b, where there is one: its slot, rows and steps (0: none)
+    struct At {
+        int s, x;
+        SlotRows r;
+    };
+    auto block_at = [&](int b) {
+        At a{};
+        if (b >= count) return a;
+        int hi = kv.seqs; // the last slot with first[s] <= b
+        while (hi - a.s > 1) {
+            const int mid = (a.s + hi) >> 1;
+            if (first[mid] <= b) a.s = mid;
             else hi = mid;
         }
-        return s;
+        a.r = slot_rows(kv, a.s);
+        a.x = block_tiles(a.r, b - first[a.s], tq);
+        return a;
     };
-    // all tiles of one KV head (a block has at most 2^24 / 64, so that 256 of
-    // them fit an int)
+    const At a0 = block_at(t);
+    // all steps of one KV head, and the longest block's (a block has at most
+    // 2^24 / 64 steps, so that 256 of them fit an int)
     long long tiles = 0;
+    int before0 = 0, longest = a0.x;
     for (int b = 0; b < count; b += 256) {
-        int mine = 0, before;
-        if (b + t < count) {
-            const int s = slot_of(b + t);
-            mine = block_tiles(slot_rows(kv, s), b + t - first[s], tq);
-        }
-        tiles += scan256(mine, before, wsum);
+        const int x = b ? block_at(b + t).x : a0.x;
+        int before;
+        tiles += scan256(x, before, wsum);
+        if (b == 0) before0 = before;
+        longest = max(longest, x);
     }
     // Two ways to cut. A workgroup per piece, every block in equal pieces of at
     // most `each` steps: the least length, of sixteen, with which the pieces
@@ -181,84 +200,70 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
     // ends each, which takes about as long as GROUP_COST steps).
     constexpr int GROUP_COST = 4;
     const int fill = fill_pieces(kv.kvh), room = max(fill - count, (fill + 1) / 2);
-    const int least = (int)max((long long)PR_MIN_TILES, (tiles + fill - 1) / fill);
-    const int most = (int)max((long long)PR_MIN_TILES, (tiles + room - 1) / room);
-    auto length = [&](int i) { return least + (int)((long long)(most - least) * i / (TRIES - 1)); };
-    int n[TRIES], longest = 0;
-#pragma unroll
-    for (int i = 0; i < TRIES; ++i) n[i] = 0;
-    for (int b = t; b < count; b += 256) {
-        const int s = slot_of(b), x = block_tiles(slot_rows(kv, s), b - first[s], tq);
-        longest = max(longest, x);
-#pragma unroll
-        for (int i = 0; i < TRIES; ++i) n[i] += (x + length(i) - 1) / length(i);
-    }
-#pragma unroll
-    for (int i = 0; i < TRIES; ++i) {
-        n[i] = wave::sum64(n[i]);
-        if (lane == 0) sums[wave][i] = n[i];
-    }
+    const int least = max(PR_MIN_TILES, divide(tiles + fill - 1, fill));
+    const int most = max(PR_MIN_TILES, divide(tiles + room - 1, room));
+    auto length = [&](int i) { return least + divide((long long)(most - least) * i, TRIES - 1); };
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
-    __syncthreads(); // (wsum's readers in the scan above)
+    // a length for each of 16 threads, a sixteenth of a round's blocks for each
+    // 16 threads
+    const int mine = length(t & (TRIES - 1));
+    int tried = 0;
+    for (int b = 0; b < count; b += 256) {
+        __syncthreads(); // (the last round's readers, and wsum's)
+        steps[t] = b ? block_at(b + t).x : a0.x;
+        __syncthreads();
+        for (int i = t / TRIES; i < min(count - b, 256); i += 256 / TRIES)
+            tried += (unsigned)(steps[i] + mine - 1) / (unsigned)mine;
+    }
+    atomicAdd(sums + (t & (TRIES - 1)), tried);
     if (lane == 0) wsum[wave] = longest;
     __syncthreads();
     longest = max(max(wsum[0], wsum[1]), max(wsum[2], wsum[3]));
-    int each = most;
-    bool once = false;
-#pragma unroll
-    for (int i = TRIES - 1; i >= 0; --i)
-        if (sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i] <= fill) {
-            each = length(i);
-            once = true;
-        }
-    const bool shares = !once || min(each, longest) > least + GROUP_COST;
+    tried = sums[lane & (TRIES - 1)];
+    const unsigned fits = (unsigned)__ballot(tried <= fill) & 0xffffu;
+    const int each = fits ? length(__ffs((int)fits) - 1) : most;
+    const bool shares = !fits || min(each, longest) > least + GROUP_COST;
     int npieces = 0, nparts = 0;
     long long done = 0; // steps before this round's blocks
     for (int b = 0; b < count; b += 256) {
-        int s = 0, x = 0, k = 0, before, pbefore, xbefore;
-        SlotRows r{};
-        if (b + t < count) {
-            s = slot_of(b + t);
-            r = slot_rows(kv, s);
-            x = block_tiles(r, b + t - first[s], tq);
-        }
-        const int xall = scan256(x, xbefore, wsum);
+        const At a = b ? block_at(b + t) : a0;
+        int xbefore = before0, before, k = 0, share = 0;
+        const int xall = b || count > 256 ? scan256(a.x, xbefore, wsum) : 0;
         const long long at = done + xbefore; // the block's first step in the sequence
-        const int share = (int)(at / least);
-        if (x) k = shares ? (int)((at + x - 1) / least) - share + 1 : (x + each - 1) / each;
-        const int all = scan256(k, before, wsum);
-        const int pall = scan256(k > 1 ? k : 0, pbefore, wsum);
-        if (x) {
-            const int index = b + t - first[s];
-            rs.blocks[b + t] = Block{r.begin + index * tq, min(tq, r.n - index * tq),
-                                     nparts + pbefore, k};
+        done += xall;
+        if (a.x) {
+            share = divide(at, least);
+            k = shares ? divide(at + a.x - 1, least) - share + 1
+                       : (int)((unsigned)(a.x + each - 1) / (unsigned)each);
+        }
+        // pieces and parts by one scan: both below 2^15 in a round
+        const int all = scan256(k | (k > 1 ? k : 0) << 16, before, wsum);
+        if (a.x) {
+            const int index = b + t - first[a.s], part = nparts + (before >> 16);
+            rs.blocks[b + t] = Block{a.r.begin + index * tq, min(tq, a.r.n - index * tq), part, k};
             for (int i = 0; i < k; ++i) {
-                const int piece = npieces + before + i;
-                long long t0 = (long long)x * i / k, t1 = (long long)x * (i + 1) / k;
+                const int piece = npieces + (before & 0xffff) + i;
+                int t0, t1;
                 if (shares) {
-                    t0 = max(0ll, (long long)(share + i) * least - at);
-                    t1 = min((long long)x, (long long)(share + i + 1) * least - at);
-                    if ((at + t0) % least == 0) rs.groups[share + i] = piece;
+                    const long long from = (long long)(share + i) * least;
+                    t0 = (int)max(0ll, from - at);
+                    t1 = (int)min((long long)a.x, from + least - at);
+                    if (at + t0 == from) rs.groups[share + i] = piece;
                 } else {
+                    t0 = divide((long long)a.x * i, k);
+                    t1 = divide((long long)a.x * (i + 1), k);
                     rs.groups[piece] = piece;
                 }
-                rs.pieces[piece] = Piece{s,
-                                         index,
-                                         (int)t0,
-                                         (int)t1,
-                                         k > 1 ? nparts + pbefore + i : -1,
-                                         r.begin,
-                                         r.n,
-                                         r.len - r.n};
+                rs.pieces[piece] = Piece{a.s,       index,   t0,    t1, k > 1 ? part + i : -1,
+                                         a.r.begin, a.r.n, a.r.len - a.r.n};
             }
         }
-        npieces += all;
-        nparts += pall;
-        done += xall;
+        npieces += all & 0xffff;
+        nparts += all >> 16;
     }
     if (t == 0) {
-        const int groups = shares ? (int)((tiles + least - 1) / least) : npieces;
+        const int groups = shares ? divide(tiles + least - 1, least) : npieces;
         rs.groups[groups] = npieces;
         *rs.plan = Plan{count, groups, {0, 0}};
     }
