@@ -59,15 +59,31 @@ __device__ __forceinline__ unsigned order_key(float x)
 
 struct RowSettings {
     float max, per_bin; // 64 / T
+    float floor;        // no value below it, and no NaN, has a bin
     double inv_t, scale, min_p;
 };
-// The bin of a value, SAMPLE_BINS where its weight is zero. (Rounding is
-// monotone, so larger values never have larger bins.)
+// The bin of a value from the row's floor on, SAMPLE_BINS where its weight is zero.
+// (Rounding is monotone, so larger values never have larger bins. Where the
+// maximum is infinite its difference with itself is a NaN, whose maximum with
+// zero is zero, and every other value's is infinite.)
 __device__ __forceinline__ int bin_of(float l, const RowSettings &s)
 {
-    if (l == s.max) return 0;
-    const float d = (s.max - l) * s.per_bin; // (NaN and infinite: no bin)
-    return d < (float)SAMPLE_BINS ? (int)d : SAMPLE_BINS;
+    return (int)fminf(fmaxf((s.max - l) * s.per_bin, 0.f), (float)SAMPLE_BINS);
+}
+// A value below which bins are larger than `hi`: the border of hi + 1, less
+// what the rounding of bin_of's difference and product can move it by.
+__device__ __forceinline__ float bin_floor(int hi, const RowSettings &s)
+{
+    if (s.max == INFINITY) return s.max;
+    const float d = (float)(hi + 1) / s.per_bin;
+    const float f = s.max - d;
+    return fmaxf(f - (fabsf(s.max) + d) * 1e-6f, -3.402823466e38f); // (minus infinity has none)
+}
+
+// The bin of any value.
+__device__ __forceinline__ int bin_at(float l, const RowSettings &s)
+{
+    return l >= s.floor ? bin_of(l, s) : SAMPLE_BINS;
 }
 // 2^(i / 64), rounded to 64 bits.
 __constant__ const double EXP2_64[64] = {
@@ -100,8 +116,7 @@ __device__ __forceinline__ void load_table(double *table)
 // argument, and those are what bounds a pass that weighs every value.
 __device__ __forceinline__ double weight(float l, const RowSettings &s, const double *table)
 {
-    if (l == s.max) return 1.0;
-    const double x = ((double)l - (double)s.max) * s.inv_t;
+    const double x = fmin(((double)l - (double)s.max) * s.inv_t, 0.0); // (inf - inf: 0)
     const double n = rint(x * 92.33248261689366);
     const double r = fma(n, -3.623510646634843e-19, fma(n, -0.010830424696249145, x));
     const int k = (int)n;
@@ -221,6 +236,7 @@ __device__ __forceinline__ RowPlan plan_row(const SampleArgs &a, int row)
     r.st.inv_t = 1.0 / (double)temp;
     r.st.per_bin = (float)(64.0 * r.st.inv_t);
     r.st.scale = ldexp(1.0, a.shift);
+    r.st.floor = bin_floor(SAMPLE_BINS - 1, r.st);
     const float least = a.min_p[row];
     r.st.min_p = least > 0.f ? fmin((double)least, 1.0) : 0.0;
     return r;
@@ -241,11 +257,12 @@ __device__ __forceinline__ u64 draw_target(float random, u64 total)
     return min((u64)(u * (double)total) + 1, total);
 }
 
-// f(value, index) for a thread's values of [begin, end): eight loads in flight,
-// then one call at a time from one place in the code. (A launch starts with a
-// cold instruction cache: f's 64-bit exponential is not fetched eight times over.)
-// Values below `floor`, and NaNs, are left out: where a wave's are all so, as
-// most are when few can be kept, a step is its loads and a comparison each.
+// f(value, index, whether it counts) for a thread's values of [begin, end): eight
+// loads in flight, then four calls at a time from one place in the code. (A
+// launch starts with a cold instruction cache: f's 64-bit exponential is not
+// fetched eight times over.) Values below `floor`, and NaNs, do not count: where
+// a wave's are all so, as most are when few can be kept, a step is its loads
+// and a comparison each.
 template <class F>
 __device__ __forceinline__ void each_value(const float *x, int begin, int end, int first, int step,
                                            float floor, F f)
@@ -257,24 +274,18 @@ __device__ __forceinline__ void each_value(const float *x, int begin, int end, i
         bool any = false;
 #pragma unroll
         for (int u = 0; u < 8; ++u) any |= v[u] >= floor;
-        if (!any) continue;
+        if (!__any(any)) continue;
 #pragma unroll 1
-        for (int j = i; j < min(end, i + 8 * step); j += step) {
-            if (v[0] >= floor) f(v[0], j);
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int u = 0; u < 7; ++u) v[u] = v[u + 1];
+            for (int u = 0; u < 4; ++u) {
+                const int j = i + (4 * h + u) * step;
+                f(v[u], j, j < end && v[u] >= floor);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = v[u + 4];
         }
     }
-}
-
-// A value below which bins are larger than `hi`: the border of hi + 1, less
-// what the rounding of bin_of's difference and product can move it by.
-__device__ __forceinline__ float bin_floor(int hi, const RowSettings &s)
-{
-    if (s.max == INFINITY) return s.max;
-    const float d = (float)(hi + 1) / s.per_bin;
-    const float f = s.max - d;
-    return f - (fabsf(s.max) + d) * 1e-6f;
 }
 
 // ---- max ----
@@ -322,9 +333,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_bins_kernel(SampleArgs 
         hc[b] = 0;
     }
     __syncthreads();
-    each_value(x, s * per, end, t, SAMPLE_THREADS, bin_floor(SAMPLE_BINS - 1, r.st), [&](float v, int) {
+    each_value(x, s * per, end, t, SAMPLE_THREADS, r.st.floor, [&](float v, int, bool counts) {
         const int b = bin_of(v, r.st);
-        if (b >= SAMPLE_BINS) return;
+        if (!counts || b >= SAMPLE_BINS) return;
         if (r.counts) atomicAdd(hc + b, 1u);
         if (r.sums) atomicAdd(hw + b, fixed(weight(v, r.st, table), r.st));
     });
@@ -443,15 +454,17 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
     const int begin = min(a.vocab, (s * SAMPLE_WAVES + wave) * a.run);
     const int end = min(a.vocab, begin + a.run);
     u64 sum = 0;
-    each_value(x, begin, end, lane, 64, bin_floor(min(max(g.hi, g.kbin), SAMPLE_BINS - 1), r.st), [&](float v, int j) {
+    each_value(x, begin, end, lane, 64, bin_floor(min(max(g.hi, g.kbin), SAMPLE_BINS - 1), r.st), [&](float v, int j, bool counts) {
         const int b = bin_of(v, r.st);
-        if (b >= SAMPLE_BINS) return;
-        if (b < g.lo) {
+        counts = counts && b < SAMPLE_BINS;
+        if (g.lo > 0) { // (no branch by value: a wave's values are mixed)
             const double w = weight(v, r.st, table);
-            if (w >= r.st.min_p) sum += fixed(w, r.st);
+            const u64 x = fixed(w, r.st);
+            sum += counts && b < g.lo && w >= r.st.min_p ? x : 0;
         }
-        const int which = b >= g.lo && b <= g.hi ? 0 : b == g.kbin ? 1 : -1;
-        if (which >= 0) {
+        const bool in0 = counts && b >= g.lo && b <= g.hi, in1 = counts && b == g.kbin;
+        if (in0 || in1) {
+            const int which = in0 ? 0 : 1;
             const unsigned n = atomicAdd(listed + which, 1u);
             if (n < SAMPLE_LIST) list[which][n] = (u64)order_key(v) << 32 | (unsigned)~j;
         }
@@ -491,7 +504,7 @@ __device__ __forceinline__ void row_alone(const SampleArgs &a, const RowPlan &pl
     __syncthreads();
     for (int i = t; i < vocab; i += SAMPLE_THREADS) {
         const float v = x[i];
-        const int b = bin_of(v, st);
+        const int b = bin_at(v, st);
         if (b < SAMPLE_BINS) {
             atomicAdd(hc + b, 1u);
             atomicAdd(hw + b, fixed(weight(v, st, table), st));
@@ -523,7 +536,7 @@ __device__ __forceinline__ void row_alone(const SampleArgs &a, const RowPlan &pl
                 const float v = x[i];
                 const unsigned key = order_key(v);
                 if (level && (key >> (sh + 8)) != prefix) continue;
-                if (bin_of(v, st) != b) continue;
+                if (bin_at(v, st) != b) continue;
                 atomicAdd(hc + ((key >> sh) & 255), 1u);
                 atomicAdd(hw + ((key >> sh) & 255), fixed(weight(v, st, table), st));
             }
@@ -602,7 +615,7 @@ __device__ __forceinline__ void row_alone(const SampleArgs &a, const RowPlan &pl
         const float v = x[i];
         const unsigned key = order_key(v);
         if (key < cut.key || (key == cut.key && i > cut.last)) return 0;
-        if (bin_of(v, st) >= SAMPLE_BINS) return 0;
+        if (bin_at(v, st) >= SAMPLE_BINS) return 0;
         const double w = weight(v, st, table);
         return w >= st.min_p ? fixed(w, st) : 0;
     };
@@ -899,7 +912,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_draw_kernel(SampleArgs 
         double wd = 0.0;
         if (i < end) {
             const float v = x[i];
-            const int bin = bin_of(v, st);
+            const int bin = bin_at(v, st);
             if (bin < SAMPLE_BINS && bin <= f.hi &&
                 (bin < f.lo || ((u64)order_key(v) << 32 | (unsigned)~i) >= last)) {
                 wd = weight(v, st, table);
