@@ -165,18 +165,19 @@ template <> struct Ops<float> {
                 acc[4 * c + 3] = mfma_f32(x.w, p[e], acc[4 * c + 3]);
             }
     }
-    // values that are not finite become zero; whether there were any
+    // values that are not finite become zero; whether the wave had any
     __device__ __forceinline__ bool clean()
     {
-        bool odd = false;
-        auto one = [&](float &x) {
-            const bool fine = fabsf(x) < INFINITY;
-            odd |= !fine;
-            x = fine ? x : 0.f;
-        };
+        float z = 0.f; // (a sum of v * 0: not zero if one is not finite)
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            z = fmaf(v[0][x].x, 0.f,
+                     fmaf(v[0][x].y, 0.f, fmaf(v[0][x].z, 0.f, fmaf(v[0][x].w, 0.f, z))));
+        if (!__any(z != 0.f)) return false;
+        auto one = [&](float &x) { x = fabsf(x) < INFINITY ? x : 0.f; };
 #pragma unroll
         for (int x = 0; x < 8; ++x) one(v[0][x].x), one(v[0][x].y), one(v[0][x].z), one(v[0][x].w);
-        return odd;
+        return true;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g)
     {
@@ -269,7 +270,13 @@ template <> struct Ops<_Float16> {
     }
     __device__ __forceinline__ bool clean()
     {
-        bool odd = false;
+        half8 z = {}; // (a sum of v * 0)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z += v[u][e] * (_Float16)0.f;
+        const u32x4 w = __builtin_bit_cast(u32x4, z); // (a NaN, or zeros of any sign)
+        if (!__any(((w[0] | w[1] | w[2] | w[3]) & 0x7fff7fffu) != 0)) return false;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -277,14 +284,11 @@ template <> struct Ops<_Float16> {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) { // (two f16 of exponent all ones or not)
                     u32x4 w = __builtin_bit_cast(u32x4, v[u][e]);
-                    const bool a = (w[x] & 0x7c00u) == 0x7c00u;
-                    const bool b = (w[x] & 0x7c000000u) == 0x7c000000u;
-                    w[x] = a ? w[x] & 0xffff0000u : w[x];
-                    w[x] = b ? w[x] & 0x0000ffffu : w[x];
-                    odd |= a | b;
+                    w[x] = (w[x] & 0x7c00u) == 0x7c00u ? w[x] & 0xffff0000u : w[x];
+                    w[x] = (w[x] & 0x7c000000u) == 0x7c000000u ? w[x] & 0x0000ffffu : w[x];
                     v[u][e] = __builtin_bit_cast(half8, w);
                 }
-        return odd;
+        return true;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g) { return 32 * g + 8 * e + x; }
     static __device__ __forceinline__ void put(float *o, const f32x4 (&acc)[8], int g, float s)
@@ -441,7 +445,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
             bool whole = p0 + TILE - 1 <= first;
 #pragma unroll
             for (int u = 0; u < SUB; ++u) whole = whole && page[u] >= 0;
-            if (!whole) odd |= __any(ops.clean());
+            if (!whole) odd |= ops.clean();
 #pragma unroll
             for (int u = 0; u < SUB; ++u) ops.pv(u, sv[u], acc);
             load_v(pn, next);

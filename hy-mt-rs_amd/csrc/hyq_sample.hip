@@ -46,7 +46,7 @@ constexpr int SAMPLE_WAVES = SAMPLE_THREADS / 64;
 constexpr int SAMPLE_BINS = 2048;  // 1/64 wide: 32 in all
 constexpr int SAMPLE_LIST = 2048;  // members of a cut's bins
 constexpr int SAMPLE_SMALL = 1024; // the largest top-k whose members are listed whole
-constexpr int SAMPLE_SPLITS = 32;
+constexpr int SAMPLE_SPLITS = 16;
 
 // An integer that orders floats (a NaN as minus infinity).
 __device__ __forceinline__ unsigned order_key(float x)
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_find_kernel(SampleArgs 
             }
         }
         const u64 cup = block_scan(c0 + c1, wsum, &ctotal);
-        const u64 wup = block_scan(w0 + w1, wsum, &wtotal);
+        const u64 wup = r.sums ? block_scan(w0 + w1, wsum, &wtotal) : 0;
         const u64 cb = cup - c0 - c1, wb = wup - w0 - w1;
         // which of this thread's bins a running value reaches a target in: -1, 0, 1
         auto reaches = [](u64 before, u64 x0, u64 x1, u64 target) {
@@ -933,7 +933,7 @@ struct SampleLayout {
     int splits, run;
     size_t count, wsum, sums, found, have, list, bytes;
 };
-// Splits: as many workgroups as fill the GPU twice, but at most 32 (each
+// Splits: as many workgroups as fill the GPU twice, but at most 16 (each
 // workgroup of the third launch adds up all of a row's histograms) and none of
 // fewer than 1024 values.
 SampleLayout sample_layout(int rows, int vocab)
