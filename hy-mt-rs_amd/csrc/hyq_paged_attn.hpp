@@ -39,6 +39,12 @@ template <class V, class T> __device__ __forceinline__ V at(const T *base, unsig
                                         (unsigned)(off * sizeof(T)));
 }
 
+// x / y for 0 <= x, 1 <= y: 32-bit division where it serves.
+__device__ __forceinline__ int divide(long long x, int y)
+{
+    return x >> 31 ? (int)(x / y) : (int)((unsigned)x / (unsigned)y);
+}
+
 // ---- the tile form's plan ----
 constexpr int PR_ROWS = 128;        // query rows per workgroup
 constexpr int PR_TILE = 64;         // positions per step
@@ -126,12 +132,6 @@ __device__ __forceinline__ int scan256(int mine, int &before, int *wsum)
     }
     before = base + v - mine;
     return all;
-}
-
-// x / y for 0 <= x, 1 <= y: 32-bit division where it serves.
-__device__ __forceinline__ int divide(long long x, int y)
-{
-    return x >> 31 ? (int)(x / y) : (int)((unsigned)x / (unsigned)y);
 }
 
 // The plan, by one workgroup of 256 threads. first: LDS of seqs ints. (The tile

@@ -22,8 +22,8 @@
 // parts (22 bits of each q, keys exact), and their values are widened.
 //
 // Work is cut evenly whatever the lengths: the tiles of all (slot, KV head)
-// units are numbered in order and worker w of W takes tiles
-// [w T / W, (w + 1) T / W). A range that covers a unit whole writes the output,
+// units are numbered in order and each of W workers takes the next T / W of
+// them. A range that covers a unit whole writes the output,
 // a part of one its maximum, sum and unnormalised row to slot w + u (workers
 // and units both ascend, so w + u names each pair once), which the merge
 // joins in worker order.
@@ -47,9 +47,20 @@ constexpr int FEW_WAVES = 4;
 
 // before[s], in LDS: the tiles of the slots before s over all KV heads, with
 // the total at before[seqs]. 256 threads.
+// Worker w of `workers` takes `base` tiles, the first `more` workers one more.
 struct FewPlan {
     long long total;
-    int workers;
+    int workers, base, more;
+    __device__ __forceinline__ long long begin(int w) const
+    {
+        return (long long)w * base + min(w, more);
+    }
+    // the worker that takes tile x
+    __device__ __forceinline__ int worker(long long x) const
+    {
+        const long long longer = (long long)more * (base + 1);
+        return x < longer ? divide(x, base + 1) : more + divide(x - longer, base);
+    }
 };
 
 // (new rows over no positions still have their zeros to be written: one tile)
@@ -94,6 +105,8 @@ __device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int
     p.total = carry;
     // 32 positions at least for a worker: fewer would only add partial rows
     p.workers = (int)min((long long)max_workers, (carry * tile + 31) / 32);
+    p.base = divide(carry, max(p.workers, 1));
+    p.more = (int)(carry - (long long)p.base * p.workers);
     return p;
 }
 
@@ -320,8 +333,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     // (uniform over the wave, and known to be)
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * FEW_WAVES + (threadIdx.x >> 6));
     if (w >= plan.workers) return;
-    long long at = plan.total * w / plan.workers;
-    const long long stop = plan.total * (w + 1) / plan.workers;
+    long long at = plan.begin(w);
+    const long long stop = plan.begin(w + 1);
     const int rep = kv.heads / kv.kvh;
     const size_t hsize = (size_t)KV_D << kv.shift, psize = 2 * hsize * kv.kvh;
     const int pmask = (1 << kv.shift) - 1;
@@ -540,11 +553,7 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int m
     if (tiles == 0 || c >= sr.n * rep) return;
     const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
     const long long first = before[s] + (long long)kh * tiles, last = first + tiles - 1;
-    // the worker of tile x: the largest w with total * w / workers <= x
-    auto worker = [&](long long x) {
-        return (int)(((x + 1) * plan.workers - 1) / plan.total);
-    };
-    const int w0 = worker(first), n = worker(last) - w0 + 1;
+    const int w0 = plan.worker(first), n = plan.worker(last) - w0 + 1;
     if (n == 1) return; // written whole
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int r = wide ? c : c + g;
