@@ -15,7 +15,8 @@
 // is split into f16 parts hi = f16(x), lo = f16(x - hi) and products sum
 // hi.hi + lo.hi + hi.lo in f32, which keeps the scores and sums near f32
 // accuracy; f16 pages are exact as they are and need no low parts of keys and
-// values. f32 pages hold values below 65504.
+// values. f32 pages hold values below 65504, of which those from 2^-14 up keep
+// 22 bits.
 //
 // Keys and values go through LDS, two steps of them, rows as they are (values
 // are transposed by ds_read_b64_tr_b16 on their way to the matrix operand).
@@ -67,6 +68,22 @@ __device__ __forceinline__ void split2(float x, float y, half2 &hi, half2 &lo)
         : "v"(hi), "v"(y));
     lo = __builtin_convertvector((float2v{a, b}), half2);
 }
+// The same with the low parts 2^11 times as large: a value keeps 22 bits as long
+// as its high part is a normal number (from 2^-14 up), where low parts in place
+// would be subnormal below 2^-3. The product takes the factor off the weights.
+constexpr float LO_SCALE = 2048.f;
+__device__ __forceinline__ void split2_scaled(float x, float y, half2 &hi, half2 &lo)
+{
+    hi = __builtin_convertvector((float2v{x, y}), half2);
+    float a, b;
+    asm("v_fma_mix_f32 %0, -%1, %3, %2 op_sel_hi:[1,0,0]"
+        : "=v"(a)
+        : "v"(hi), "v"(x * LO_SCALE), "s"(LO_SCALE));
+    asm("v_fma_mix_f32 %0, -%1, %3, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(b)
+        : "v"(hi), "v"(y * LO_SCALE), "s"(LO_SCALE));
+    lo = __builtin_convertvector((float2v{a, b}), half2);
+}
 // Positions p .. p + 3 of 16 dims: lane i of 16 takes dim i of them all, its
 // address being that of row (i / 4), dims 4 (i % 4) ..
 __device__ __forceinline__ half4 read_transposed(const _Float16 *p)
@@ -100,11 +117,17 @@ template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
         for (int i = 0; i < N; ++i) one(v[i].x), one(v[i].y), one(v[i].z), one(v[i].w);
         return odd;
     }
+    template <bool VALUE>
     static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *lo, const float4 &x)
     {
         half2 a, b, c, d;
-        split2(x.x, x.y, a, b);
-        split2(x.z, x.w, c, d);
+        if constexpr (VALUE) {
+            split2_scaled(x.x, x.y, a, b);
+            split2_scaled(x.z, x.w, c, d);
+        } else {
+            split2(x.x, x.y, a, b);
+            split2(x.z, x.w, c, d);
+        }
         *reinterpret_cast<half4 *>(hi) = half4{a[0], a[1], c[0], c[1]};
         *reinterpret_cast<half4 *>(lo) = half4{b[0], b[1], d[0], d[1]};
     }
@@ -129,6 +152,7 @@ template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
             }
         return odd;
     }
+    template <bool VALUE>
     static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *, const half8 &x)
     {
         *reinterpret_cast<half8 *>(hi) = x;
@@ -218,9 +242,9 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         RowsLds<LO> &l = lds.step[buf];
         const int d = R::dim(t), r = R::row(t, n >> 1);
         if (n & 1)
-            R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
+            R::template put<true>(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
         else
-            R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
+            R::template put<false>(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
     };
     // whether some row sees a step in part
     auto partial = [&](int p0, const Four &pg) {
@@ -381,7 +405,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                 vlo[n & 3] = half8{z[0], z[1], z[2], z[3], w[0], w[1], w[2], w[3]};
             }
         };
-        half8 phi, plo;
+        half8 phi, plo, pls; // (pls: the weights of the values' low parts)
         values(0);
         values(1);
 #pragma unroll
@@ -396,6 +420,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     plo[i] = lo[0];
                     plo[i + 1] = lo[1];
                 }
+                if constexpr (LO) pls = phi * (_Float16)(1.f / LO_SCALE);
             }
             if (n + 2 < 8) {
                 values(n + 2);
@@ -407,8 +432,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             d = mfma(vhi[n & 3], plo, d);
             e = mfma(vhi[(n + 1) & 3], plo, e);
             if constexpr (LO) {
-                d = mfma(vlo[n & 3], phi, d);
-                e = mfma(vlo[(n + 1) & 3], phi, e);
+                d = mfma(vlo[n & 3], pls, d);
+                e = mfma(vlo[(n + 1) & 3], pls, e);
             }
             __builtin_amdgcn_sched_barrier(0);
         }

@@ -403,8 +403,8 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
  * one slot (a slot of more is not computed); heads / kv_heads is at most 16.
  * Rows that see nothing give zeros. The values of an F32 pool must lie within
  * the f16 range where a slot has more than 16 * kv_heads / heads new rows
- * (those products split them into two f16 parts: 22 bits of values from 2^-3
- * up, 2^-25 absolutely below). scratch_d: hyq_paged_attention_scratch_bytes
+ * (those products split them into two f16 parts: 22 bits of values from 2^-14
+ * up, 2^-36 absolutely below). scratch_d: hyq_paged_attention_scratch_bytes
  * bytes (0 for arguments that the call refuses). */
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
                                          size_t heads);

@@ -178,6 +178,16 @@ def test_queries_of_any_size(gpu_ctx, hyq, f16):
             assert np.all(np.abs(got - want).max(-1) <= tol)
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -10, 2.0 ** -13, 2.0 ** 10])
+@pytest.mark.parametrize("news", [2, 40])
+def test_values_of_any_size(gpu_ctx, hyq, news, scale):
+    """Small and large cached values keep their relative accuracy in an f32
+    pool, in both forms (tolerance() is relative to the largest value)."""
+    b = R.Batch([300, 90], [news, news], 8, 2, 32, False, seed=17)
+    b.pool[:, 1] *= np.float32(scale)
+    check(b, attention(hyq, gpu_ctx, b))
+
+
 def test_offsets_past_32_bits(gpu_ctx, hyq):
     """Pages whose byte offsets pass 2^32 (and element offsets 2^31 in f16)."""
     small = R.Batch([600, 530], [1, 40], 8, 8, 256, True, seed=15, spare=1)
