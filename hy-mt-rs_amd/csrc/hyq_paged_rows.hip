@@ -367,10 +367,13 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
         for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, sv[e]);
         // The running maximum follows only when a score passes it by 2^8 or
-        // more: until then weights are at most 2^8, and the 64 products that
-        // bring the sums to a new one are rare (in 32 rows of equal chances
-        // some row has a new maximum in most steps).
-        const float m_new = wave::max_halves(tmax) * qscale;
+        // more: until then weights are at most 2^8 times the first, and the 64
+        // products that bring the sums to a new one are rare (in 32 rows of
+        // equal chances some row has a new maximum in most steps). m_run lies 7
+        // below the maximum, so that weights go up to 2^15: their f16 parts
+        // resolve 2^-25, which is 2^-32 of the first weight. (Many equal small
+        // weights are rounded the same way, and their errors add up.)
+        const float m_new = fmaf(wave::max_halves(tmax), qscale, -7.f);
         if (__any(m_new > m_run + 8.f)) {
             const float m = fmaxf(m_run, m_new);
             const float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);

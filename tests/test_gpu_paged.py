@@ -188,6 +188,33 @@ def test_values_of_any_size(gpu_ctx, hyq, news, scale):
     check(b, attention(hyq, gpu_ctx, b))
 
 
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("news", [2, 40])
+def test_many_small_weights(gpu_ctx, hyq, news, f16):
+    """Thousands of positions of one small weight, 194.5 * 2^-24 of the largest,
+    whose values alone make the output: they are rounded alike, so that a
+    weight's error does not average out. Keys are zero but for one in every 32
+    positions, whose values are zero. Relative bound: the score's (tolerance()'s
+    d, twice), the sums' 2 (n + 8) U, and the weight's resolution where its f16
+    parts hold 2^-25 of 2^7: 2^-32 of it, 2^-15.6 of the small ones."""
+    n = 2000
+    b = R.Batch([n], [news], 4, 2, 64, f16, seed=18, spare=0)
+    b.pool[:] = 0
+    for s in range(0, n, 32):
+        b.pool[b.table[0, s // 64], 0, :, s % 64, 0] = 2.0
+    for i in range(n):
+        if i % 32:
+            b.pool[b.table[0, i // 64], 1, :, i % 64] = 1.0
+    b.q[:] = 0
+    b.q[..., 0] = -np.log2(194.5 * 2.0 ** -24) * np.log(2) * np.sqrt(128) / 2.0
+    out = attention(hyq, gpu_ctx, b)
+    want, _ = b.attention()
+    score = 11.4
+    d = (128 * R.U + 3 * 2.0 ** -22) * (score + 1) + 9 * R.U * score + 2 * R.U
+    bound = 2 * d + 2 * (n + 8) * R.U + 2.0 ** -15.6
+    assert np.all(np.abs(out / want - 1) <= bound), np.abs(out / want - 1).max()
+
+
 def test_offsets_past_32_bits(gpu_ctx, hyq):
     """Pages whose byte offsets pass 2^32 (and element offsets 2^31 in f16)."""
     small = R.Batch([600, 530], [1, 40], 8, 8, 256, True, seed=15, spare=1)
