@@ -15,8 +15,8 @@
 // is split into f16 parts hi = f16(x), lo = f16(x - hi) and products sum
 // hi.hi + lo.hi + hi.lo in f32, which keeps the scores and sums near f32
 // accuracy; f16 pages are exact as they are and need no low parts of keys and
-// values. f32 pages hold values below 65504, of which those from 2^-14 up keep
-// 22 bits.
+// values. f32 pages hold keys and values below 65504, of which those from 2^-14
+// up keep 22 bits.
 //
 // Keys and values go through LDS, two steps of them, rows as they are (values
 // are transposed by ds_read_b64_tr_b16 on their way to the matrix operand).
@@ -68,9 +68,11 @@ __device__ __forceinline__ void split2(float x, float y, half2 &hi, half2 &lo)
         : "v"(hi), "v"(y));
     lo = __builtin_convertvector((float2v{a, b}), half2);
 }
-// The same with the low parts 2^11 times as large: a value keeps 22 bits as long
-// as its high part is a normal number (from 2^-14 up), where low parts in place
-// would be subnormal below 2^-3. The product takes the factor off the weights.
+// The same with the low parts 2^11 times as large: an operand keeps 22 bits as
+// long as its high part is a normal number (from 2^-14 up), where low parts in
+// place would be subnormal below 2^-3. The factor is taken off the scores' sum
+// of such products, and off the weights that values' low parts are multiplied
+// with.
 constexpr float LO_SCALE = 2048.f;
 __device__ __forceinline__ void split2_scaled(float x, float y, half2 &hi, half2 &lo)
 {
@@ -117,17 +119,11 @@ template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
         for (int i = 0; i < N; ++i) one(v[i].x), one(v[i].y), one(v[i].z), one(v[i].w);
         return odd;
     }
-    template <bool VALUE>
     static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *lo, const float4 &x)
     {
         half2 a, b, c, d;
-        if constexpr (VALUE) {
-            split2_scaled(x.x, x.y, a, b);
-            split2_scaled(x.z, x.w, c, d);
-        } else {
-            split2(x.x, x.y, a, b);
-            split2(x.z, x.w, c, d);
-        }
+        split2_scaled(x.x, x.y, a, b);
+        split2_scaled(x.z, x.w, c, d);
         *reinterpret_cast<half4 *>(hi) = half4{a[0], a[1], c[0], c[1]};
         *reinterpret_cast<half4 *>(lo) = half4{b[0], b[1], d[0], d[1]};
     }
@@ -152,7 +148,6 @@ template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
             }
         return odd;
     }
-    template <bool VALUE>
     static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *, const half8 &x)
     {
         *reinterpret_cast<half8 *>(hi) = x;
@@ -242,9 +237,9 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         RowsLds<LO> &l = lds.step[buf];
         const int d = R::dim(t), r = R::row(t, n >> 1);
         if (n & 1)
-            R::template put<true>(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
+            R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
         else
-            R::template put<false>(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
+            R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
     };
     // whether some row sees a step in part
     auto partial = [&](int p0, const Four &pg) {
@@ -292,7 +287,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 half2 hi, lo;
-                split2(v[i] * inv, v[i + 1] * inv, hi, lo);
+                split2_scaled(v[i] * inv, v[i + 1] * inv, hi, lo);
                 qhi[kk][i] = hi[0];
                 qhi[kk][i + 1] = hi[1];
                 qlo[kk][i] = lo[0];
@@ -345,17 +340,14 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
         for (int kk = 0; kk < KV_D / 16; ++kk) {
             if (kk + 1 < KV_D / 16) keys(kk + 1);
-            sv = mfma(ahi[kk & 1], qhi[kk], sv);
             sx = mfma(ahi[kk & 1], qlo[kk], sx);
-            if constexpr (LO) {
-                if (kk & 1) sv = mfma(alo[kk & 1], qhi[kk], sv);
-                else sx = mfma(alo[kk & 1], qhi[kk], sx);
-            }
+            sv = mfma(ahi[kk & 1], qhi[kk], sv);
+            if constexpr (LO) sx = mfma(alo[kk & 1], qhi[kk], sx);
             if (kk < 2 * R::N) store(buf ^ 1, kk);
             __builtin_amdgcn_sched_barrier(0);
         }
         load(p0 + 2 * PR_TILE, after);
-        sv += sx;
+        sv += sx * (1.f / LO_SCALE);
         if (p + 31 > wave_all || (pa | pb) < 0) { // mask
 #pragma unroll
             for (int e = 0; e < 16; ++e) {

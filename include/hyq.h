@@ -401,9 +401,9 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
  * pages: the row at position p sees the slot's positions 0..p. Any mix of
  * prompts, decode steps and drafted tokens. max_rows bounds the new rows of
  * one slot (a slot of more is not computed); heads / kv_heads is at most 16.
- * Rows that see nothing give zeros. The values of an F32 pool must lie within
- * the f16 range where a slot has more than 16 * kv_heads / heads new rows
- * (those products split them into two f16 parts: 22 bits of values from 2^-14
+ * Rows that see nothing give zeros. The keys and values of an F32 pool must lie
+ * within the f16 range where a slot has more than 16 * kv_heads / heads new rows
+ * (those products split them into two f16 parts: 22 bits of numbers from 2^-14
  * up, 2^-36 absolutely below). scratch_d: hyq_paged_attention_scratch_bytes
  * bytes (0 for arguments that the call refuses). */
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
@@ -447,19 +447,20 @@ int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
                         size_t scratch_bytes);
 
 /* Sampling (Sampler, src/generation.rs:229-334, from given random numbers):
- * one token for each row of logits [rows][vocab], with settings of its own in
- * device arrays of `rows` values. With w_i = exp((l_i - max l) / temperature)
- * and the order of larger logits first, equal ones by index: the first top_k
- * of the order (<= 0: all); of those the shortest prefix whose weight reaches
- * top_p of theirs (>= 1: all); of those the ones with w_i >= min_p (the
- * largest always); token = in index order the first of them at which the
- * running weight exceeds random * their weight, random in [0, 1) (values
- * outside are cut to 0 and 1). temperature <= 0: the first maximum. A NaN or
- * minus infinity is never taken; a row of nothing else gives token -1. Weights
- * are summed exactly to 2^-46 of the largest (2^-62 times the vocabulary,
- * rounded up to a power of two, where that is more): smaller ones count as
- * zero. prob_d (may be null): the token's weight over the kept ones' (1 at
- * temperature <= 0, 0 beside -1). */
+ * one token for each row of logits [rows][vocab] (at most 65535 rows of 2^24),
+ * with settings of its own in device arrays of `rows` values. With
+ * w_i = exp((l_i - max l) / temperature) and the order of larger logits first,
+ * equal ones by index: the first top_k of the order (<= 0: all); of those the
+ * shortest prefix whose weight reaches top_p of theirs (>= 1: all); of those
+ * the ones with w_i >= min_p (the largest always); token = in index order the
+ * first of them at which the running weight exceeds random * their weight,
+ * random in [0, 1) (values outside are cut to 0 and 1). temperature <= 0 or
+ * NaN: the first maximum; one below 2^-100 counts as 2^-100. A NaN or minus
+ * infinity is never taken (a row of nothing else gives token -1), and beside a
+ * plus infinity nothing finite is. Weights are summed exactly to 2^-46 of the
+ * largest (2^-62 times the vocabulary, rounded up to a power of two, where
+ * that is more): smaller ones count as zero. prob_d (may be null): the token's
+ * weight over the kept ones' (1 at temperature <= 0, 0 beside -1). */
 size_t hyq_sample_scratch_bytes(size_t rows, size_t vocab);
 int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
                  const float *temperature_d, const int32_t *top_k_d, const float *top_p_d,

@@ -188,6 +188,17 @@ def test_values_of_any_size(gpu_ctx, hyq, news, scale):
     check(b, attention(hyq, gpu_ctx, b))
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -10, 2.0 ** 10])
+@pytest.mark.parametrize("news", [2, 40])
+def test_keys_of_any_size(gpu_ctx, hyq, news, scale):
+    """The same of keys, with queries that bring the scores back to size: what
+    tolerance() allows them is relative to the products' magnitude."""
+    b = R.Batch([300, 90], [news, news], 8, 2, 32, False, seed=19)
+    b.pool[:, 0] *= np.float32(scale)
+    b.q *= np.float32(1 / scale)
+    check(b, attention(hyq, gpu_ctx, b))
+
+
 @pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
 @pytest.mark.parametrize("news", [2, 40])
 def test_many_small_weights(gpu_ctx, hyq, news, f16):
