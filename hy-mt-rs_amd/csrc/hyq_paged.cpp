@@ -245,7 +245,7 @@ int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
 
 size_t hyq_sample_scratch_bytes(size_t rows, size_t vocab)
 {
-    if (rows == 0 || rows > 65536 || vocab == 0 || vocab > (1 << 24)) return 0;
+    if (rows == 0 || rows > 65535 || vocab == 0 || vocab > (1 << 24)) return 0;
     return sample_scratch((int)rows, (int)vocab);
 }
 
@@ -258,7 +258,7 @@ int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
     if (!logits_d || !temperature_d || !top_k_d || !top_p_d || !min_p_d || !random_d ||
         !scratch_d || !token_d)
         return fail(HYQ_EINVAL, "sample: null argument");
-    if (rows == 0 || rows > 65536 || vocab == 0 || vocab > (1 << 24))
+    if (rows == 0 || rows > 65535 || vocab == 0 || vocab > (1 << 24))
         return fail(HYQ_EINVAL, "sample: %zu rows of %zu logits", rows, vocab);
     if (!aligned(scratch_d)) return fail(HYQ_EINVAL, "sample: scratch is not 16-byte aligned");
     if (scratch_bytes < hyq_sample_scratch_bytes(rows, vocab))

@@ -58,20 +58,19 @@ __device__ __forceinline__ void angle(int p, float freq, float &sn, float &cs)
     sincosf((float)r, &sn, &cs);
 }
 
-// Grid (rows, ceil(groups / (4 * groups_per_wave))), four waves: a wave takes
-// groups_per_wave groups of four heads, in the order query heads, key heads,
-// value heads. (q_out may be q: a thread reads what it writes first.)
+// Grid (rows, ceil(groups / 4)), four waves: a wave takes a group of four heads,
+// in the order query heads, key heads, value heads. (q_out may be q: a thread
+// reads what it writes first.)
 template <class T>
 __global__ __launch_bounds__(256) void paged_append_kernel(
     PagedKv kv, const float *q, const float *__restrict__ k,
     const float *__restrict__ v, const float *__restrict__ qn, const float *__restrict__ kn,
-    const float *__restrict__ freq, float eps, int norm_first, int groups_per_wave,
-    float *q_out)
+    const float *__restrict__ freq, float eps, int norm_first, float *q_out)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.x, j = lane & 15;
     const int total = kv.heads + 2 * kv.kvh;
-    const int first = (blockIdx.y * 4 + wave) * groups_per_wave * 4;
+    const int first = (blockIdx.y * 4 + wave) * 4;
     if (first >= total) return;
     const int slot = slot_of_row(kv.start, kv.seqs, row, lane);
     if (slot < 0) return; // a row behind the last slot's
@@ -94,8 +93,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
         angle(pos, f.z, sn[2], cs[2]);
         angle(pos, f.w, sn[3], cs[3]);
     }
-    const int last = min(first + groups_per_wave * 4, total);
-    for (int h = first + (lane >> 4); h < last; h += 4) {
+    const int h = first + (lane >> 4);
+    if (h < total) {
         const bool is_q = h < kv.heads, is_v = h >= kv.heads + kv.kvh;
         const int kh = h - kv.heads - (is_v ? kv.kvh : 0);
         const float *src = is_q ? q + ((size_t)row * kv.heads + h) * KV_D
@@ -155,15 +154,14 @@ int launch_paged_append(const PagedKv &kv, const float *q, const float *k, const
 {
     if (kv.rows <= 0) return 0;
     const int groups = (kv.heads + 2 * kv.kvh + 3) / 4;
-    const int per = 1;
-    const dim3 grid(kv.rows, (groups + 4 * per - 1) / (4 * per));
+    const dim3 grid(kv.rows, (groups + 3) / 4);
     hipStream_t st = (hipStream_t)stream;
     if (kv.f16)
         hipLaunchKernelGGL(paged_append_kernel<_Float16>, grid, dim3(256), 0, st, kv, q, k, v, qn,
-                           kn, freq, eps, (int)norm_first, per, q_out);
+                           kn, freq, eps, (int)norm_first, q_out);
     else
         hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(256), 0, st, kv, q, k, v, qn,
-                           kn, freq, eps, (int)norm_first, per, q_out);
+                           kn, freq, eps, (int)norm_first, q_out);
     return (int)hipGetLastError();
 }
 

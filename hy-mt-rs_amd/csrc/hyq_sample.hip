@@ -47,6 +47,7 @@ constexpr int SAMPLE_BINS = 2048;  // 1/64 wide: 32 in all
 constexpr int SAMPLE_LIST = 2048;  // members of a cut's bins
 constexpr int SAMPLE_SMALL = 1024; // the largest top-k whose members are listed whole
 constexpr int SAMPLE_SPLITS = 16;
+constexpr float LEAST_TEMPERATURE = 0x1p-100f;
 
 // An integer that orders floats (a NaN as minus infinity).
 __device__ __forceinline__ unsigned order_key(float x)
@@ -58,26 +59,27 @@ __device__ __forceinline__ unsigned order_key(float x)
 }
 
 struct RowSettings {
-    float max, per_bin; // 64 / T
+    float max, half_max, per_bin; // (128 / T, see bin_of)
     float floor;        // no value below it, and no NaN, has a bin
     double inv_t, scale, min_p;
 };
 // The bin of a value from the row's floor on, SAMPLE_BINS where its weight is zero.
-// (Rounding is monotone, so larger values never have larger bins. Where the
-// maximum is infinite its difference with itself is a NaN, whose maximum with
-// zero is zero, and every other value's is infinite.)
+// (Rounding is monotone, so larger values never have larger bins. Half the
+// difference, which no two values' overflows. Where the maximum is infinite its
+// difference with itself is a NaN, whose maximum with zero is zero, and every
+// other value's is infinite.)
 __device__ __forceinline__ int bin_of(float l, const RowSettings &s)
 {
-    return (int)fminf(fmaxf((s.max - l) * s.per_bin, 0.f), (float)SAMPLE_BINS);
+    return (int)fminf(fmaxf(fmaf(-0.5f, l, s.half_max) * s.per_bin, 0.f), (float)SAMPLE_BINS);
 }
 // A value below which bins are larger than `hi`: the border of hi + 1, less
 // what the rounding of bin_of's difference and product can move it by.
 __device__ __forceinline__ float bin_floor(int hi, const RowSettings &s)
 {
     if (s.max == INFINITY) return s.max;
-    const float d = (float)(hi + 1) / s.per_bin;
-    const float f = s.max - d;
-    return fmaxf(f - (fabsf(s.max) + d) * 1e-6f, -3.402823466e38f); // (minus infinity has none)
+    const float d = (float)(hi + 1) / s.per_bin; // (half, as in bin_of)
+    const float f = s.half_max - d - (fabsf(s.half_max) + d) * 1e-6f;
+    return fmaxf(2.f * f, -3.402823466e38f); // (minus infinity has no bin)
 }
 
 // The bin of any value.
@@ -233,8 +235,10 @@ __device__ __forceinline__ RowPlan plan_row(const SampleArgs &a, int row)
     r.counts = !r.greedy && r.by_k;
     r.sums = !r.greedy && r.by_p && !(r.by_k && r.k <= SAMPLE_SMALL);
     r.st.max = r.max;
-    r.st.inv_t = 1.0 / (double)temp;
-    r.st.per_bin = (float)(64.0 * r.st.inv_t);
+    r.st.half_max = 0.5f * r.max;
+    // (so that bins of 1/64 are numbers; equal maxima share what there is)
+    r.st.inv_t = 1.0 / (double)fmaxf(temp, LEAST_TEMPERATURE);
+    r.st.per_bin = (float)(128.0 * r.st.inv_t);
     r.st.scale = ldexp(1.0, a.shift);
     r.st.floor = bin_floor(SAMPLE_BINS - 1, r.st);
     const float least = a.min_p[row];

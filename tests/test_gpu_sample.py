@@ -108,6 +108,46 @@ def test_infinities_and_nans(gpu_ctx, hyq):
     assert token.tolist() == [7, 7]
 
 
+def test_extreme_sizes(gpu_ctx, hyq):
+    """Logits whose differences pass f32's range, and temperatures at its ends
+    (below 2^-100 only equal maxima are left)."""
+    r = np.random.default_rng(8)
+    n, vocab = 8, 900
+    x = (r.uniform(-1, 1, (n, vocab)) * 3.3e38).astype(np.float32)
+    u = r.random(n)
+    check(hyq, gpu_ctx, x, u, [(1e38, 0, 1.0, 0.0), (3e38, 50, 0.7, 0.0), (2e37, 0, 0.9, 0.0),
+                               (3e38, 0, 1.0, 0.3), (1e38, 300, 0.99, 0.0), (1.0, 0, 1.0, 0.0),
+                               (np.inf, 0, 1.0, 0.0), (np.inf, 0, 0.5, 0.0)])
+    x = r.normal(0, 2, (n, vocab)).astype(np.float32)
+    x[:, [5, 300, 301, 888]] = 20.0
+    tiny = [(t, k, p, 0.0) for t, k, p in ((1e-38, 0, 1.0), (1e-45, 3, 1.0), (1e-31, 0, 0.6),
+                                           (1e-30, 0, 1.0), (2e-29, 2, 0.9), (1e-38, 2000, 0.5),
+                                           (1e-12, 0, 0.9), (1e-38, 1, 1.0))]
+    check(hyq, gpu_ctx, x, u, tiny)
+
+
+def test_more_rows_than_splits_serve(gpu_ctx, hyq):
+    """Rows by a workgroup each (more than half of 512), and by two."""
+    r = np.random.default_rng(9)
+    for rows, vocab in ((600, 1500), (257, 4100), (256, 4100)):
+        x = r.normal(0, 2.5, (rows, vocab)).astype(np.float32)
+        check(hyq, gpu_ctx, x, r.random(rows), [SETTINGS[i % len(SETTINGS)] for i in range(rows)])
+
+
+@pytest.mark.parametrize("vocab", [2049, 128167])
+def test_where_lists_end(gpu_ctx, hyq, vocab):
+    """A top-k around the largest whose members are listed whole, and cuts by
+    top-k far behind the one by top-p."""
+    r = np.random.default_rng(10)
+    settings = [(1.0, k, p, 0.0) for k in (63, 64, 65, 1023, 1024, 1025, 2047, 2048, 30000)
+                for p in (1.0, 0.3, 0.97)]
+    n = len(settings)
+    x = r.normal(0, 2.5, (n, vocab)).astype(np.float32)
+    check(hyq, gpu_ctx, x, r.random(n), settings)
+    flat = r.uniform(0, 0.02, (n, vocab)).astype(np.float32)  # (all in two bins)
+    check(hyq, gpu_ctx, flat, r.random(n), settings)
+
+
 def test_without_probabilities_and_the_argmax(gpu_ctx, hyq):
     """prob may be null; temperature 0 is hyq_argmax_d's token."""
     r = np.random.default_rng(5)

@@ -132,6 +132,13 @@ def test_sample_refusals(hyq, L, ctx):
     assert L.hyq_sample_scratch_bytes(0, 5) == 0 and L.hyq_sample_scratch_bytes(5, 0) == 0
 
 
+def test_sample_rows_of_a_grid(hyq, L, ctx):
+    """A row is a workgroup's second grid index: at most 65535."""
+    p = 4096
+    assert L.hyq_sample_scratch_bytes(65535, 7) > 0 and L.hyq_sample_scratch_bytes(65536, 7) == 0
+    assert L.hyq_sample_d(ctx, p, 65536, 7, p, p, p, p, p, p, 1 << 40, p, p) == hyq.EINVAL
+
+
 def test_cache_checks_its_layout(hyq):
     with pytest.raises(ValueError, match="layout"):
         hyq.PagedCache(None, 1, 4, 10, 2, 100, page_tokens=24)
