@@ -707,7 +707,9 @@ class PagedCache:
     A serving step: ``fork`` (beams, ended requests), ``extend`` (room for the
     new tokens), then for every layer ``append_d`` and ``attention_d`` of the
     packed rows. The calls are asynchronous on the context's stream; those that
-    return numpy arrays wait."""
+    return numpy arrays wait. ``table`` and ``len`` alternate between two buffers
+    with every ``fork``, and a captured graph keeps those of its capture: capture
+    an even number of forks, or none and replay after an even number."""
 
     def __init__(self, ctx: Context, layers: int, kv_heads: int, pages: int, seqs: int,
                  context: int, page_tokens: int = 64, dtype: int = F16, head_dim: int = 128):
@@ -727,7 +729,7 @@ class PagedCache:
         self._ints = [ctx.empty(seqs, np.int32) for _ in range(3)]
         self._live = ctx.empty(1, np.int32)
         self._scratch = ctx.empty(lib().hyq_pages_scratch_bytes(self._kl), np.uint8)
-        self._attention = None
+        self._attention = []
 
     def _slots(self, values, into: DeviceArray) -> int:
         a = np.ascontiguousarray(values, np.int32)
@@ -778,16 +780,18 @@ class PagedCache:
 
     def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,
                     q_d: int, out_d: int) -> None:
-        """hyq_paged_attention_d on device buffers, with a scratch that grows
-        with the largest call."""
+        """hyq_paged_attention_d on device buffers. The scratch grows with the
+        largest call, at least twofold; the smaller ones live as long as the
+        cache, since a captured graph may hold them. (A capture allocates
+        nothing: run the largest call once before it.)"""
         need = lib().hyq_paged_attention_scratch_bytes(self._kl, rows, max_rows, heads)
-        if self._attention is None or self._attention.nbytes < need:
-            self.ctx.sync()  # calls before this one may still use the old scratch
-            self._attention = self.ctx.empty(max(need, 16), np.uint8)
+        have = self._attention[-1].nbytes if self._attention else 0
+        if need > have or not have:  # (0: a call that is refused)
+            self._attention.append(self.ctx.empty(max(need, 2 * have, 16), np.uint8))
+        scratch = self._attention[-1]
         check(lib().hyq_paged_attention_d(
             self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr, self.len.ptr,
-            start_d, rows, max_rows, heads, q_d, self._attention.ptr, self._attention.nbytes,
-            out_d))
+            start_d, rows, max_rows, heads, q_d, scratch.ptr, scratch.nbytes, out_d))
 
 
 def sample(ctx: "Context", logits: np.ndarray, random, temperature=1.0, top_k=0, top_p=1.0,

@@ -87,6 +87,26 @@ def test_long_and_short(gpu_ctx, hyq, f16):
 
 
 @pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+def test_uneven_prompts(gpu_ctx, hyq, f16):
+    """Two long prompts beside many short ones, too many blocks for the long
+    ones to be cut finely by themselves: workgroups take several blocks' steps."""
+    b = R.Batch([30] * 15 + [2500] + [30] * 13 + [2437], [30] * 15 + [64] + [30] * 13 + [64], 16, 8,
+                64, f16, seed=20, tail=1)
+    check(b, attention(hyq, gpu_ctx, b))
+
+
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+def test_more_blocks_than_the_plan_takes_at_once(gpu_ctx, hyq, f16):
+    """Some 390 blocks of prompts, with decode steps and empty slots between."""
+    news = np.array([5, 1, 0] * 300)
+    lens = news + np.arange(900) % 97
+    news[[100, 700]] = 350, 353
+    lens[[100, 700]] = 900, 353
+    b = R.Batch(lens, news, 16, 1, 16, f16, seed=21)
+    check(b, attention(hyq, gpu_ctx, b))
+
+
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
 def test_many_slots(gpu_ctx, hyq, f16):
     """More slots than a workgroup has threads, most of them empty."""
     r = np.random.default_rng(3)

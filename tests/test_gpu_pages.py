@@ -194,6 +194,28 @@ def test_large_tables(gpu_ctx, hyq, in_place):
         d.check(m)
 
 
+@pytest.mark.parametrize("pages,seqs,width", [(4096, 1024, 16), (4096, 1024, 17), (4097, 1024, 16),
+                                              (4096, 1025, 15), (4095, 1023, 5)])
+def test_where_the_small_forms_end(gpu_ctx, hyq, pages, seqs, width):
+    """Pools and tables on both sides of what one workgroup's counts hold."""
+    pt = 16
+    m = model(pages, seqs, width, pt, seed=6)
+    d = Device(hyq, gpu_ctx, pages, seqs, width, pt, layers=1, kvh=1, dtype=1)
+    r = np.random.default_rng(7)
+    d.put(m)
+    for step in range(2):
+        add = r.integers(0, 40, seqs)
+        assert np.array_equal(d.extend(add, True), m.extend(add))
+        parent = np.where(r.random(seqs) < 0.6, r.integers(-1, seqs, seqs), np.arange(seqs))
+        keep = None if step else r.integers(0, width * pt, seqs)
+        m.fork(parent, keep)
+        d.fork(parent, keep)
+        d.check(m, pool=False)
+        add = r.integers(0, 3, seqs)
+        assert np.array_equal(d.extend(add, False), m.extend(add))
+        d.check(m)
+
+
 def test_wrong_entries_and_counts(gpu_ctx, hyq):
     """Ids outside the pool, negative lengths and counts that fit no table make
     no access outside the arrays, and slots beside them stay right."""
@@ -230,3 +252,20 @@ def test_cache_class(gpu_ctx, hyq):
     assert c.table.numpy().tolist() == [[-1] * 4, [0, 1, -1, -1], [2, -1, -1, -1]]
     with pytest.raises(ValueError):
         c.extend([1, 2])
+
+
+def test_cache_class_keeps_its_scratch(gpu_ctx, hyq):
+    """A larger attention call takes a larger scratch and leaves the first one,
+    which a captured graph may hold, allocated; a refused call says why."""
+    c = hyq.PagedCache(gpu_ctx, layers=1, kv_heads=1, pages=4, seqs=1, context=64, page_tokens=16)
+    c.extend([50])
+    c.pool.copy_from(np.zeros(c.pool.nbytes, np.uint8))
+    q = gpu_ctx.array(np.ones((50, 2, 128), np.float32))
+    out = gpu_ctx.array(np.ones((50, 2, 128), np.float32))
+    for n in (1, 50, 20):
+        start = gpu_ctx.array(np.array([0, n], np.int32))
+        c.attention_d(0, start.ptr, n, n, 2, q.ptr, out.ptr)
+        assert np.all(out.numpy()[:n] == 0)
+    assert len(c._attention) == 2 and all(x.ptr for x in c._attention)
+    with pytest.raises(ValueError, match="0 rows"):
+        c.attention_d(0, start.ptr, 0, 1, 2, q.ptr, out.ptr)

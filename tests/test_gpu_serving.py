@@ -197,6 +197,56 @@ def test_a_captured_step(gpu_ctx, hyq, f16):
     ok(hip("hipGraphDestroy")(graph))
 
 
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+def test_a_captured_ragged_batch(gpu_ctx, hyq, f16):
+    """Append and attention of prompts, drafts and single tokens in one graph,
+    replayed for other splits of the same number of rows, shorter ones among
+    them: every replay gives the eager call's bits and leaves the rows behind."""
+    ctx, L = gpu_ctx, hyq.lib()
+    rows, most, context = 300, 200, 512
+    r = np.random.default_rng(6)
+    kl = hyq.KvLayout(hyq.F16 if f16 else hyq.F32, 1, KVH, D, PT, 5 * context // PT, 5,
+                      context // PT)
+    ref = ctypes.byref(kl)
+    f = lambda *s: ctx.array(r.normal(0, 1, s).astype(np.float32))
+    q, k, v, w, freq = f(rows, HEADS, D), f(rows, KVH, D), f(rows, KVH, D), f(D), f(64)
+    pool0 = r.normal(0, 1, (kl.pages, 2, KVH, PT, D)).astype(np.float16 if f16 else np.float32)
+    table = ctx.array(r.permutation(kl.pages).reshape(5, -1).astype(np.int32))
+    lens, start = ctx.empty(5, np.int32), ctx.empty(6, np.int32)
+    pool, qo, out = ctx.array(pool0), ctx.empty((rows, HEADS, D), np.float32), f(rows, HEADS, D)
+    need = L.hyq_paged_attention_scratch_bytes(ref, rows, most, HEADS)
+    scratch = ctx.empty(need, np.uint8)
+
+    def work():
+        hyq.check(L.hyq_paged_rope_norm_append_d(
+            ctx.handle, ref, pool.ptr, 0, table.ptr, lens.ptr, start.ptr, rows, HEADS, q.ptr,
+            k.ptr, v.ptr, w.ptr, w.ptr, freq.ptr, ctypes.c_float(1e-5), 0, qo.ptr))
+        hyq.check(L.hyq_paged_attention_d(
+            ctx.handle, ref, pool.ptr, 0, table.ptr, lens.ptr, start.ptr, rows, most, HEADS,
+            qo.ptr, scratch.ptr, need, out.ptr))
+
+    graph, run = captured(ctx, work)
+    for news, held in (([1, 1, 1, 1, 1], [40, 0, 511, 3, 64]), ([200, 50, 8, 9, 33], [0, 20, 1, 0, 9]),
+                       ([0, 200, 0, 100, 0], [5, 312, 0, 0, 0]), ([0, 0, 0, 0, 0], [9, 9, 9, 9, 9]),
+                       ([1, 1, 1, 1, 1], [40, 0, 511, 3, 64]), ([60, 60, 60, 60, 60], [100] * 5)):
+        got = []
+        start.copy_from(np.cumsum([0] + news).astype(np.int32))
+        lens.copy_from(np.add(news, held).astype(np.int32))
+        for call in (work, lambda: ok(hip("hipGraphLaunch")(run, ctypes.c_void_p(ctx.stream)))):
+            pool.copy_from(pool0)
+            qo.copy_from(np.full((rows, HEADS, D), 5, np.float32))
+            out.copy_from(np.full((rows, HEADS, D), -7, np.float32))
+            scratch.copy_from(np.full(need, 0xFF, np.uint8))
+            call()
+            got.append([a.numpy() for a in (pool, qo, out)])
+        n = sum(news)
+        for a, b in zip(*got):
+            assert np.array_equal(a, b), news
+        assert np.all(got[0][2][n:] == -7) and not np.any(got[0][2][:n] == -7)
+    ok(hip("hipGraphExecDestroy")(run))
+    ok(hip("hipGraphDestroy")(graph))
+
+
 def test_two_contexts_at_once(gpu_ctx, hyq):
     """Steps enqueued on two contexts (streams) in turn, each with buffers of
     its own, give what one alone gives."""
