@@ -48,6 +48,7 @@ constexpr int SAMPLE_LIST = 2048;  // members of a cut's bins
 constexpr int SAMPLE_SMALL = 1024; // the largest top-k whose members are listed whole
 constexpr int SAMPLE_SPLITS = 16;
 constexpr float LEAST_TEMPERATURE = 0x1p-100f;
+constexpr float FLT_MAX = 3.402823466e38f;
 
 // An integer that orders floats (a NaN as minus infinity).
 __device__ __forceinline__ unsigned order_key(float x)
@@ -61,7 +62,7 @@ __device__ __forceinline__ unsigned order_key(float x)
 struct RowSettings {
     float max, half_max, per_bin; // (128 / T, see bin_of)
     float floor;        // no value below it, and no NaN, has a bin
-    double inv_t, scale, min_p;
+    double weigh_max, weigh, scale, min_p; // weigh: 1024 / (T ln 2)
 };
 // The bin of a value from the row's floor on, SAMPLE_BINS where its weight is zero.
 // (Rounding is monotone, so larger values never have larger bins. Half the
@@ -79,7 +80,7 @@ __device__ __forceinline__ float bin_floor(int hi, const RowSettings &s)
     if (s.max == INFINITY) return s.max;
     const float d = (float)(hi + 1) / s.per_bin; // (half, as in bin_of)
     const float f = s.half_max - d - (fabsf(s.half_max) + d) * 1e-6f;
-    return fmaxf(2.f * f, -3.402823466e38f); // (minus infinity has no bin)
+    return fmaxf(2.f * f, -FLT_MAX); // (minus infinity has no bin)
 }
 
 // The bin of any value.
@@ -105,30 +106,40 @@ __constant__ const double EXP2_64[64] = {
     1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
-// A workgroup's copy of the table (ends with a barrier).
+// 2^(i / 1024).
+__constant__ const double EXP2_1024[16] = {
+    1.0, 1.0006771306930664, 1.0013547198921082, 1.002032767907594,
+    1.0027112750502025, 1.0033902416308227, 1.004069667960554, 1.0047495543507072,
+    1.0054299011128027, 1.006110708558573, 1.0067919769999607, 1.0074737067491204,
+    1.0081558981184175, 1.0088385514204294, 1.0095216669679448, 1.0102052450739643};
+// The table 2^(i / 1024) in LDS (ends with a barrier).
+constexpr int SAMPLE_TABLE = 1024;
 __device__ __forceinline__ void load_table(double *table)
 {
-    if (threadIdx.x < 64) table[threadIdx.x] = EXP2_64[threadIdx.x];
+    static_assert(SAMPLE_TABLE == SAMPLE_THREADS, "an entry per thread");
+    table[threadIdx.x] = EXP2_64[threadIdx.x >> 4] * EXP2_1024[threadIdx.x & 15];
     __syncthreads();
 }
-// The weight of a value that has a bin: exp(x), x = (l - max) / T in [-33, 0],
-// is 2^(n / 64) exp(r) with |r| <= ln 2 / 128, the series of exp(r) to r^5
-// (the next term is below 4e-17) times the table's value, times 2^(n >> 6) by
-// its exponent. A third of the 64-bit operations of a series for the whole
-// argument, and those are what bounds a pass that weighs every value.
+// The weight of a value that has a bin: exp((l - max) / T) = 2^(y / 1024) with
+// y = (l - max) 1024 / (T ln 2) in [-48800, 0], y = n + f with n whole and
+// |f| <= 1/2: 2^(n >> 10), by the exponent, times the table's 2^((n & 1023) /
+// 1024) times 2^(f / 1024), whose series to f^3 is off by less than 6e-16 (the
+// first term left out, (ln 2 / 2048)^4 / 24) where a unit of the sums is 2^-46 =
+// 1.4e-14. n comes of adding 1.5 2^52, whose low bits then hold it. Ten 64-bit
+// operations a value, and those are what bounds a pass that weighs every value:
+// 18 of them (a table of 64, a series to r^5, n by rounding and conversion)
+// made the sums' pass over 64 rows of 128167 17.2 us instead of 16.4.
 __device__ __forceinline__ double weight(float l, const RowSettings &s, const double *table)
 {
-    const double x = fmin(((double)l - (double)s.max) * s.inv_t, 0.0); // (inf - inf: 0)
-    const double n = rint(x * 92.33248261689366);
-    const double r = fma(n, -3.623510646634843e-19, fma(n, -0.010830424696249145, x));
-    const int k = (int)n;
-    double e = fma(r, 1.0 / 120, 1.0 / 24);
-    e = fma(e, r, 1.0 / 6);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0) * table[k & 63];
-    const u64 bits = __builtin_bit_cast(u64, e) + ((u64)(unsigned)(k >> 6) << 52);
-    return __builtin_bit_cast(double, bits); // (e >= 0.99, k >> 6 >= -48: no underflow)
+    constexpr double WHOLE = 6755399441055744.0, LN2 = 0.6931471805599453 / SAMPLE_TABLE;
+    const double d = (double)fminf(l, FLT_MAX) - s.weigh_max; // (inf and inf: 0)
+    const double t = fma(d, s.weigh, WHOLE), f = fma(d, s.weigh, WHOLE - t);
+    const int n = (int)(unsigned)__builtin_bit_cast(u64, t);
+    double e = fma(f, LN2 * LN2 * LN2 / 6, LN2 * LN2 / 2);
+    e = fma(e, f, LN2);
+    e = fma(e, f, 1.0) * table[n & (SAMPLE_TABLE - 1)];
+    const u64 bits = __builtin_bit_cast(u64, e) + ((u64)(unsigned)(n >> 10) << 52);
+    return __builtin_bit_cast(double, bits); // (e >= 0.99, n >> 10 >= -48: no underflow)
 }
 // w 2^shift as an integer, to nearest: the sum with 2^52 holds it in its low
 // bits (w 2^shift <= 2^46).
@@ -237,8 +248,10 @@ __device__ __forceinline__ RowPlan plan_row(const SampleArgs &a, int row)
     r.st.max = r.max;
     r.st.half_max = 0.5f * r.max;
     // (so that bins of 1/64 are numbers; equal maxima share what there is)
-    r.st.inv_t = 1.0 / (double)fmaxf(temp, LEAST_TEMPERATURE);
-    r.st.per_bin = (float)(128.0 * r.st.inv_t);
+    const double inv_t = 1.0 / (double)fmaxf(temp, LEAST_TEMPERATURE);
+    r.st.per_bin = (float)(128.0 * inv_t);
+    r.st.weigh_max = fminf(r.max, FLT_MAX);
+    r.st.weigh = inv_t * (SAMPLE_TABLE * 1.4426950408889634);
     r.st.scale = ldexp(1.0, a.shift);
     r.st.floor = bin_floor(SAMPLE_BINS - 1, r.st);
     const float least = a.min_p[row];
@@ -325,7 +338,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_bins_kernel(SampleArgs 
 {
     __shared__ u64 hw[SAMPLE_BINS];
     __shared__ unsigned hc[SAMPLE_BINS];
-    __shared__ double table[64];
+    __shared__ double table[SAMPLE_TABLE];
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     const RowPlan r = plan_row(a, row);
     if (!r.counts && !r.sums) return;
@@ -447,7 +460,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
 {
     __shared__ unsigned listed[2], base[2];
     __shared__ u64 list[2][SAMPLE_LIST];
-    __shared__ double table[64];
+    __shared__ double table[SAMPLE_TABLE];
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const RowPlan r = plan_row(a, row);
     if (r.greedy) return;
@@ -458,7 +471,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
     const int begin = min(a.vocab, (s * SAMPLE_WAVES + wave) * a.run);
     const int end = min(a.vocab, begin + a.run);
     u64 sum = 0;
-    each_value(x, begin, end, lane, 64, bin_floor(min(max(g.hi, g.kbin), SAMPLE_BINS - 1), r.st), [&](float v, int j, bool counts) {
+    const float least = bin_floor(min(max(g.hi, g.kbin), SAMPLE_BINS - 1), r.st);
+    each_value(x, begin, end, lane, 64, least, [&](float v, int j, bool counts) {
         const int b = bin_of(v, r.st);
         counts = counts && b < SAMPLE_BINS;
         if (g.lo > 0) { // (no branch by value: a wave's values are mixed)
@@ -790,7 +804,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_draw_kernel(SampleArgs 
     __shared__ ListScratch ls;
     __shared__ u64 wsum[SAMPLE_WAVES], pick[4];
     __shared__ u64 run_sum[SAMPLE_SPLITS * SAMPLE_WAVES];
-    __shared__ double table[64];
+    __shared__ double table[SAMPLE_TABLE];
     static_assert(SAMPLE_SPLITS * SAMPLE_WAVES <= SAMPLE_THREADS, "a run per thread");
     const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Found f = a.found[row];
