@@ -144,8 +144,8 @@ size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, s
     if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0 ||
         !grid_ok(kl, rows, heads))
         return 0;
-    return paged_attention_scratch(kl->seqs, kl->kv_heads, (int)heads, (int)rows,
-                                   (int)std::min(rows, max_rows));
+    return paged_attention_scratch(kl->dtype == HYQ_F16, kl->seqs, kl->kv_heads, (int)heads,
+                                   (int)rows, (int)std::min(rows, max_rows));
 }
 
 int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, int layer,
@@ -280,10 +280,10 @@ int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
 namespace hyq {
 
 // Scratch: the few-row form's parts, then the tile form's plan and parts.
-size_t paged_attention_scratch(int seqs, int kvh, int heads, int rows, int max_rows)
+size_t paged_attention_scratch(bool f16, int seqs, int kvh, int heads, int rows, int max_rows)
 {
     const int few = std::min(paged_few_rows(heads / kvh), max_rows);
-    size_t n = paged_few_scratch(seqs, kvh, heads, few);
+    size_t n = paged_few_scratch(f16, seqs, kvh, heads, few);
     if (max_rows > few) n += rows_layout(seqs, kvh, heads, rows).bytes;
     return n;
 }
@@ -296,7 +296,7 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
     RowsScratch rs{};
     if (max_rows > few) {
         const RowsLayout l = rows_layout(kv.seqs, kv.kvh, kv.heads, kv.rows);
-        char *base = (char *)scratch + paged_few_scratch(kv.seqs, kv.kvh, kv.heads, few);
+        char *base = (char *)scratch + paged_few_scratch(kv.f16, kv.seqs, kv.kvh, kv.heads, few);
         rs.plan = (Plan *)base;
         rs.blocks = (Block *)(base + l.blocks);
         rs.pieces = (Piece *)(base + l.pieces);

@@ -30,7 +30,7 @@ int launch_paged_append(const PagedKv &kv, const float *q, const float *k, const
 
 // Attention: the one-wave form for slots of few new rows and the tile form for
 // the others; scratch as paged_attention_scratch says.
-size_t paged_attention_scratch(int seqs, int kvh, int heads, int rows, int max_rows);
+size_t paged_attention_scratch(bool f16, int seqs, int kvh, int heads, int rows, int max_rows);
 int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void *scratch,
                            float *out, void *stream);
 

@@ -272,7 +272,7 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)
 // new rows, with the plan where there is a tile form; and the merge of both.
 int paged_few_rows(int rep);
-size_t paged_few_scratch(int seqs, int kvh, int heads, int few);
+size_t paged_few_scratch(bool f16, int seqs, int kvh, int heads, int few);
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
                      float *out, void *stream);
 int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,

@@ -636,16 +636,20 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_ro
         merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / 8), (i - n) % (PR_ROWS / 8));
 }
 
-constexpr int FEW_MAX_WORKERS = 1024;
+// Workers: a wave on each SIMD for f32 pages, two for f16 pages, whose steps
+// have twice the products for each byte (64 sessions of up to 8192 positions in
+// f16 pages: 162 us with 1024, 149 with 2048; four of up to 60001 in f32 pages:
+// 106 and 113). Numbers between leave SIMDs unequal: 190 and 146 with 1280.
+int few_workers(bool f16) { return f16 ? 2048 : 1024; }
 
 } // namespace
 
 int paged_few_rows(int rep) { return 16 / rep; }
 
-size_t paged_few_scratch(int seqs, int kvh, int heads, int few)
+size_t paged_few_scratch(bool f16, int seqs, int kvh, int heads, int few)
 {
     const int part_rows = few * (heads / kvh);
-    return ((size_t)FEW_MAX_WORKERS + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
+    return ((size_t)few_workers(f16) + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
 }
 
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
@@ -654,13 +658,14 @@ int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const fl
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
-    const dim3 grid(FEW_MAX_WORKERS / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
+    const int workers = few_workers(kv.f16);
+    const dim3 grid(workers / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
     if (kv.f16)
         hipLaunchKernelGGL(paged_few_kernel<_Float16>, grid, block, lds, st, kv, few,
-                           FEW_MAX_WORKERS, rs, q, part_rows, part, out);
+                           workers, rs, q, part_rows, part, out);
     else
         hipLaunchKernelGGL(paged_few_kernel<float>, grid, block, lds, st, kv, few,
-                           FEW_MAX_WORKERS, rs, q, part_rows, part, out);
+                           workers, rs, q, part_rows, part, out);
     return (int)hipGetLastError();
 }
 
@@ -676,11 +681,11 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
     const int each = wide ? part_rows : (part_rows + 3) / 4;
     const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, each, rs.cap));
     if (kv.f16)
-        hipLaunchKernelGGL(paged_merge_kernel<Ops<_Float16>::TILE>, grid, dim3(256), lds, st, kv,
-                           few, FEW_MAX_WORKERS, part_rows, wide, rs, part, out);
+        hipLaunchKernelGGL(paged_merge_kernel<Ops<_Float16>::TILE>, grid, dim3(256), lds, st, kv, few,
+                           few_workers(kv.f16), part_rows, wide, rs, part, out);
     else
         hipLaunchKernelGGL(paged_merge_kernel<Ops<float>::TILE>, grid, dim3(256), lds, st, kv, few,
-                           FEW_MAX_WORKERS, part_rows, wide, rs, part, out);
+                           few_workers(kv.f16), part_rows, wide, rs, part, out);
     return (int)hipGetLastError();
 }
 
