@@ -21,6 +21,7 @@ namespace hyq {
 namespace {
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The slot of packed row `row`: the last one whose first row is <= row among
 // those that hold it (a slot without rows holds none); -1 past the last row.
@@ -99,9 +100,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(
         const int kh = h - kv.heads - (is_v ? kv.kvh : 0);
         const float *src = is_q ? q + ((size_t)row * kv.heads + h) * KV_D
                                 : (is_v ? v : k) + ((size_t)row * kv.kvh + kh) * KV_D;
-        const float4 a4 = *reinterpret_cast<const float4 *>(src + 4 * j);
-        const float4 b4 = *reinterpret_cast<const float4 *>(src + 64 + 4 * j);
-        float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+        // (read once: prompts of 2367 rows 24.2 -> 22.9 us)
+        const f32x4 a4 = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(src + 4 * j));
+        const f32x4 b4 =
+            __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(src + 64 + 4 * j));
+        float a[4] = {a4[0], a4[1], a4[2], a4[3]}, b[4] = {b4[0], b4[1], b4[2], b4[3]};
         if (!is_v) {
             const float *w = is_q ? qn : kn;
             const float4 wa = *reinterpret_cast<const float4 *>(w + 4 * j);

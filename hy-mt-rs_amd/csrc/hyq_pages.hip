@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void pages_fill_kernel(PagesArgs a, char *pool
             for (int k = 0; k < 8; ++k) v[k] = src[min(x + 64 * k, words - 1)];
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (x + 64 * k < words) dst[x + 64 * k] = v[k];
+                if (x + 64 * k < words) __builtin_nontemporal_store(v[k], dst + x + 64 * k);
         }
     }
 }
@@ -518,7 +518,7 @@ int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const in
     else
         hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len,
                            refs, table_out, len_out, refs_out, status, scratch);
-    hipLaunchKernelGGL(pages_fill_kernel, dim3(2048), dim3(256), 0, st, a, (char *)pool, scratch);
+    hipLaunchKernelGGL(pages_fill_kernel, dim3(512), dim3(256), 0, st, a, (char *)pool, scratch);
     return (int)hipGetLastError();
 }
 
@@ -528,7 +528,7 @@ int launch_pages_compact(const PagesArgs &a, void *pool, const int *table, const
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(1024), 0, st, a, refs, refs_out, live,
                        scratch);
-    hipLaunchKernelGGL(pages_move_kernel, dim3(2048), dim3(256), 0, st, a, (char *)pool, table,
+    hipLaunchKernelGGL(pages_move_kernel, dim3(1024), dim3(256), 0, st, a, (char *)pool, table,
                        table_out, scratch);
     return (int)hipGetLastError();
 }
