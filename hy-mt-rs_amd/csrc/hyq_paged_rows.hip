@@ -103,7 +103,8 @@ template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
     static constexpr int N = 4;
     typedef float4 Vec;
     Vec k[N], v[N];
-    static __device__ __forceinline__ int row(int t, int i) { return (t >> 5) + 16 * i; }
+    static constexpr int STEP = 16;
+    static __device__ __forceinline__ int row(int t) { return t >> 5; }
     static __device__ __forceinline__ int group(int, int i) { return i; } // its 16 rows
     static __device__ __forceinline__ int dim(int t) { return 4 * (t & 31); }
     // whether a value is not finite; such values become zero
@@ -132,7 +133,8 @@ template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
     static constexpr int N = 2;
     typedef half8 Vec;
     Vec k[N], v[N];
-    static __device__ __forceinline__ int row(int t, int i) { return (t >> 4) + 32 * i; }
+    static constexpr int STEP = 32;
+    static __device__ __forceinline__ int row(int t) { return t >> 4; }
     static __device__ __forceinline__ int group(int wave, int i) { return 2 * i + (wave >> 2); }
     static __device__ __forceinline__ int dim(int t) { return 8 * (t & 15); }
     __device__ __forceinline__ bool clean()
@@ -159,7 +161,9 @@ template <bool LO> struct RowsLds { // one step
     _Float16 vhi[PR_TILE][PR_VP], vlo[LO ? PR_TILE : 1][PR_VP];
 };
 
-template <class T>
+// WHOLE: a step lies in one page (of 64 tokens or more), so that it takes one
+// look at the table and one base address instead of four of each.
+template <class T, bool WHOLE>
 __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     PagedKv kv, RowsScratch rs, const float *__restrict__ q, float *__restrict__ out)
 {
@@ -194,59 +198,79 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     const int p_begin = piece.t0 * PR_TILE;
     const int all_see = first + tok0; // the last position that every row sees
 
-    // The pages of a step's four 16-position groups, -1 where none. Page ids
-    // come 64 at a time, one per lane. Rows past the end are loaded too, from
-    // the same page or, where there is none, from the pool's first: their
-    // weights are zero, and values that are not finite are cleared.
+    // The pages of a step's four 16-position groups (or the step's one), -1 where
+    // none. Page ids come 64 at a time, one per lane. Rows past the end are
+    // loaded too, from the same page or, where there is none, from the pool's
+    // first: their weights are zero, and values that are not finite are cleared.
     const int *entries = kv.table + (size_t)s * kv.stride;
     int have = -64, ids = -1; // lane i: the slot's page have + i
-    struct Four {
-        int e[4];
+    constexpr int GROUPS = WHOLE ? 1 : 4;
+    struct Pages {
+        int e[GROUPS];
+        __device__ __forceinline__ int of(int group) const { return e[WHOLE ? 0 : group]; }
+        __device__ __forceinline__ bool missing() const
+        {
+            int all = e[0];
+#pragma unroll
+            for (int i = 1; i < GROUPS; ++i) all |= e[i];
+            return all < 0;
+        }
     };
     auto pages_of = [&](int p0) {
-        Four f;
+        Pages f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = max(p0 + 16 * i, 0) >> kv.shift;
+        for (int i = 0; i < GROUPS; ++i) {
+            const int at = p0 + 16 * i, p = at >> kv.shift;
             if (p - have >= 64 || p < have) {
                 have = p;
                 ids = entries[min(have + lane, kv.stride - 1)];
             }
             const int e = __builtin_amdgcn_readlane(ids, p - have);
-            f.e[i] = p0 + 16 * i < p_end && (unsigned)e < (unsigned)kv.npages ? e : -1;
+            f.e[i] = (WHOLE || at < p_end) && (unsigned)e < (unsigned)kv.npages ? e : -1;
         }
         return f;
     };
     R raw;
-    auto load = [&](int p0, const Four &pg) {
+    auto load = [&](int p0, const Pages &pg) {
+        if constexpr (WHOLE) {
+            const T *b = (const T *)kv.pages + (size_t)max(pg.e[0], 0) * psize + (size_t)kh * hsize +
+                         (size_t)(p0 & pmask) * KV_D;
 #pragma unroll
-        for (int i = 0; i < R::N; ++i) {
-            const int g = R::group(wave, i), e = g == 0 ? pg.e[0] : g == 1 ? pg.e[1]
-                                                : g == 2   ? pg.e[2]
-                                                           : pg.e[3];
-            // (a uniform base, and an offset that never changes)
-            const T *b = (const T *)kv.pages + (size_t)max(e, 0) * psize + (size_t)kh * hsize +
-                         (size_t)((p0 + 16 * g) & pmask) * KV_D;
-            const unsigned o = (R::row(t, i) & 15) * KV_D + R::dim(t);
-            raw.k[i] = at<typename R::Vec>(b, o);
-            raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
+            for (int i = 0; i < R::N; ++i) {
+                const unsigned o = (R::row(t) + R::STEP * i) * KV_D + R::dim(t);
+                raw.k[i] = at<typename R::Vec>(b, o);
+                raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < R::N; ++i) {
+                const int g = R::group(wave, i), e = g == 0 ? pg.of(0) : g == 1 ? pg.of(1)
+                                                    : g == 2   ? pg.of(2)
+                                                               : pg.of(3);
+                // (a uniform base, and an offset that never changes)
+                const T *b = (const T *)kv.pages + (size_t)max(e, 0) * psize + (size_t)kh * hsize +
+                             (size_t)((p0 + 16 * g) & pmask) * KV_D;
+                const unsigned o = (R::row(t) & 15) * KV_D + R::dim(t);
+                raw.k[i] = at<typename R::Vec>(b, o);
+                raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
+            }
         }
     };
     // one of the 2 N rows of `raw`, converted, to a buffer
     auto store = [&](int buf, int n) {
         RowsLds<LO> &l = lds.step[buf];
-        const int d = R::dim(t), r = R::row(t, n >> 1);
+        const int d = R::dim(t), r = R::row(t) + R::STEP * (n >> 1);
         if (n & 1)
             R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
         else
             R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
     };
     // whether some row sees a step in part
-    auto partial = [&](int p0, const Four &pg) {
-        return p0 + PR_TILE - 1 > all_see || (pg.e[0] | pg.e[1] | pg.e[2] | pg.e[3]) < 0;
+    auto partial = [&](int p0, const Pages &pg) {
+        return p0 + PR_TILE - 1 > all_see || pg.missing();
     };
 
-    Four cur = pages_of(p_begin), next = pages_of(p_begin + PR_TILE);
+    Pages cur = pages_of(p_begin), next = pages_of(p_begin + PR_TILE);
     load(p_begin, cur);
 
     // this lane's query row
@@ -312,15 +336,11 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     __syncthreads();
     int buf = 0;
     const int o = 32 * part_of; // this wave's 32 positions of a step
-    // The two waves of a SIMD would go through their products together and then
-    // through the softmax together; with the first half's waves issuing first
-    // they take turns at the matrix unit.
-    if (part_of) __builtin_amdgcn_s_setprio(0);
-    else __builtin_amdgcn_s_setprio(3);
     for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
-        const Four after = pages_of(p0 + 2 * PR_TILE);
+        const Pages after = pages_of(p0 + 2 * PR_TILE);
         const RowsLds<LO> &l = lds.step[buf];
-        const int p = p0 + o, pa = part_of ? cur.e[2] : cur.e[0], pb = part_of ? cur.e[3] : cur.e[1];
+        const int p = p0 + o, pa = part_of ? cur.of(2) : cur.of(0),
+                  pb = part_of ? cur.of(3) : cur.of(1);
         if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
         // (two chains of sums: a product waits for the one it adds to)
         f32x16 sv, sx;
@@ -441,11 +461,11 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         // the values left out, for the rows that see them: whatever its weight,
         // such a value makes the sum not finite
         for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
-            const Four pg = pages_of(p0);
+            const Pages pg = pages_of(p0);
             if (!partial(p0, pg)) continue;
             for (int i = 0; i < 32; ++i) {
                 const int pos = p0 + 32 * part_of + i;
-                const int e = i < 16 ? (part_of ? pg.e[2] : pg.e[0]) : part_of ? pg.e[3] : pg.e[1];
+                const int e = i < 16 ? (part_of ? pg.of(2) : pg.of(0)) : part_of ? pg.of(3) : pg.of(1);
                 if (pos > sees || e < 0) continue;
                 const T *vb = (const T *)kv.pages + (size_t)e * psize +
                               (size_t)(kv.kvh + kh) * hsize + (size_t)(pos & pmask) * KV_D;
@@ -514,11 +534,11 @@ int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, 
 {
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh); // (more groups there are not)
-    if (kv.f16)
-        hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(PR_THREADS), 0, st, kv, rs, q,
-                           out);
-    else
-        hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(PR_THREADS), 0, st, kv, rs, q, out);
+    const auto kernel = 1 << kv.shift >= PR_TILE
+                            ? (kv.f16 ? paged_rows_kernel<_Float16, true> : paged_rows_kernel<float, true>)
+                            : (kv.f16 ? paged_rows_kernel<_Float16, false>
+                                      : paged_rows_kernel<float, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(PR_THREADS), 0, st, kv, rs, q, out);
     return (int)hipGetLastError();
 }
 
