@@ -11,6 +11,11 @@
 // A 16-lane row of a wave takes a head: lane j its dims 4j..4j+3 and
 // 64+4j..64+4j+3 as two float4, so the norm's sum is four DPP steps and a wave
 // forms four heads at once from one set of angles.
+//
+// Bound by memory: 2367 rows of 32 + 2 * 8 heads into f32 pages move 116 MB in
+// 22.7 us (5.1 TB/s, what a copy reaches), 48 rows of 16 + 2 * 4 heads into f16
+// pages take 4.2 to 5 us, a launch and four dependent loads (starts, length,
+// page, row).
 #include <hip/hip_runtime.h>
 
 #include "hyq_paged.hpp"
