@@ -292,7 +292,9 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
     const size_t row = (size_t)(piece.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
 
-    // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range
+    // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range: to
+    // below 2^14 where the low parts stay as they are, and to below 2 where they
+    // are scaled like those of the keys that they are added up with.
     half8 qhi[KV_D / 16], qlo[KV_D / 16];
     float qscale;
     {
@@ -310,7 +312,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)),
                                  fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
         mx = wave::max_halves(mx);
-        const int e = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
+        const int e = (mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0) - (LO ? 0 : 13);
         qscale = ldexpf(sc, e);
         const float inv = ok ? ldexpf(1.f, -e) : 0.f;
 #pragma unroll
@@ -320,7 +322,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 half2 hi, lo;
-                split2_scaled(v[i] * inv, v[i + 1] * inv, hi, lo);
+                if constexpr (LO) split2_scaled(v[i] * inv, v[i + 1] * inv, hi, lo);
+                else split2(v[i] * inv, v[i + 1] * inv, hi, lo);
                 qhi[kk][i] = hi[0];
                 qhi[kk][i + 1] = hi[1];
                 qlo[kk][i] = lo[0];
@@ -351,7 +354,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         const int p = p0 + o, pa = part_of ? cur.of(2) : cur.of(0),
                   pb = part_of ? cur.of(3) : cur.of(1);
         if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
-        // (two chains of sums: a product waits for the one it adds to)
+        // (sx: the products with low parts, where those are scaled)
         f32x16 sv, sx;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sv[e] = sx[e] = 0.f;
@@ -369,14 +372,19 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
         for (int kk = 0; kk < KV_D / 16; ++kk) {
             if (kk + 1 < KV_D / 16) keys(kk + 1);
-            sx = mfma(ahi[kk & 1], qlo[kk], sx);
-            sv = mfma(ahi[kk & 1], qhi[kk], sv);
-            if constexpr (LO) sx = mfma(alo[kk & 1], qhi[kk], sx);
+            if constexpr (LO) {
+                sx = mfma(ahi[kk & 1], qlo[kk], sx);
+                sv = mfma(ahi[kk & 1], qhi[kk], sv);
+                sx = mfma(alo[kk & 1], qhi[kk], sx);
+            } else {
+                sv = mfma(ahi[kk & 1], qhi[kk], sv);
+                sv = mfma(ahi[kk & 1], qlo[kk], sv);
+            }
             if (kk < 2 * R::N) store(buf ^ 1, kk);
             __builtin_amdgcn_sched_barrier(0);
         }
         load(p0 + 2 * PR_TILE, after);
-        sv += sx * (1.f / LO_SCALE);
+        if constexpr (LO) sv += sx * (1.f / LO_SCALE);
         if (p + 31 > wave_all || (pa | pb) < 0) { // mask
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
