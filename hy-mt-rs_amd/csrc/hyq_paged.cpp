@@ -14,15 +14,22 @@ namespace {
 
 bool aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+size_t page_bytes(const hyq_kv_layout *kl)
+{
+    return (size_t)2 * kl->kv_heads * kl->page_tokens * KV_D * (kl->dtype == HYQ_F16 ? 2 : 4);
+}
+
 bool layout_ok(const hyq_kv_layout *kl)
 {
     if (!kl || (kl->dtype != HYQ_F32 && kl->dtype != HYQ_F16)) return false;
     const int pt = kl->page_tokens;
     if (pt < 16 || pt > 256 || (pt & (pt - 1))) return false;
-    return kl->layers >= 1 && kl->layers <= 65536 && kl->kv_heads >= 1 && kl->kv_heads <= 256 &&
-           kl->head_dim == KV_D && kl->pages >= 1 && kl->pages <= (1 << 24) && kl->seqs >= 1 &&
-           kl->seqs <= KV_MAX_SEQS && kl->stride >= 1 &&
-           (long long)kl->stride * pt <= (1 << 24);
+    if (kl->layers < 1 || kl->layers > 65536 || kl->kv_heads < 1 || kl->kv_heads > 256 ||
+        kl->head_dim != KV_D || kl->pages < 1 || kl->pages > (1 << 24) || kl->seqs < 1 ||
+        kl->seqs > KV_MAX_SEQS || kl->stride < 1 || (long long)kl->stride * pt > (1 << 24))
+        return false;
+    // (a pool whose bytes would not fit: layers * pages may be 2^40, a page 2^26)
+    return (size_t)kl->layers * kl->pages <= (((size_t)1 << 62) / page_bytes(kl));
 }
 
 int check_layout(hyq_ctx *ctx, const hyq_kv_layout *kl, const char *who)
@@ -45,11 +52,6 @@ int shift_of(const hyq_kv_layout *kl)
     int s = 4;
     while ((1 << s) < kl->page_tokens) ++s;
     return s;
-}
-
-size_t page_bytes(const hyq_kv_layout *kl)
-{
-    return (size_t)2 * kl->kv_heads * kl->page_tokens * KV_D * (kl->dtype == HYQ_F16 ? 2 : 4);
 }
 
 bool heads_ok(const hyq_kv_layout *kl, size_t heads)
@@ -169,6 +171,7 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
     if (scratch_bytes < need)
         return fail(HYQ_EINVAL, "paged_attention: scratch of %zu bytes, %zu needed", scratch_bytes,
                     need);
+    if (out_d == q_d) return fail(HYQ_EINVAL, "paged_attention: the output must not be q");
     DeviceGuard g(ctx->device);
     HYQ_LAUNCH(launch_paged_attention(view(kl, pool_d, layer, table_d, len_d, start_d, rows, heads),
                                       (int)std::min(rows, max_rows), q_d, scratch_d, out_d,

@@ -380,13 +380,15 @@ typedef struct {
     int seqs;        /* slots, 1..4096 */
     int stride;      /* table entries of a slot; stride * page_tokens <= 2^24 */
 } hyq_kv_layout;
-/* Bytes of the pool, 0 when the layout is not one of the above. */
+/* Bytes of the pool, 0 when the layout is not one of the above (or they pass
+ * 2^62). */
 size_t hyq_kv_pool_bytes(const hyq_kv_layout *kl);
 /* hyq_rope_norm_append_d for the packed rows of many slots: RoPE and the
  * per-head rms_norm of q [rows][heads*128] and k [rows][kv_heads*128]
  * (norm_first: the hy_v3 order, src/model.rs:425-446), q to q_out_d (which may
- * be q_d), k and v to the pages of `layer`. An F16 pool holds the values
- * rounded once, to nearest. The angle position * freq_d[j] is taken in 64
+ * be q_d), k and v to the pages of `layer` (of two rows for one place, in a page
+ * that two slots name, either stays: hyq_pages_extend_d gives each its own). An
+ * F16 pool holds the values rounded once, to nearest. The angle position * freq_d[j] is taken in 64
  * bits, where hyq_rope_norm_append_d rounds the product to 32 (the reference's
  * table, src/model.rs:919-925): the two differ by up to position * 2^-24
  * radians times the frequency, and agree where the product is exact. */
@@ -404,7 +406,7 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
  * Rows that see nothing give zeros. The keys and values of an F32 pool must lie
  * within the f16 range where a slot has more than 16 * kv_heads / heads new rows
  * (those products split them into two f16 parts: 22 bits of numbers from 2^-14
- * up, 2^-36 absolutely below). scratch_d: hyq_paged_attention_scratch_bytes
+ * up, 2^-36 absolutely below). out_d must not be q_d. scratch_d: hyq_paged_attention_scratch_bytes
  * bytes (0 for arguments that the call refuses). */
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
                                          size_t heads);

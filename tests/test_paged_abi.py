@@ -33,13 +33,15 @@ def test_pool_bytes(hyq, L):
 BAD = [dict(dtype=8), dict(layers=0), dict(kv_heads=0), dict(kv_heads=257), dict(head_dim=64),
        dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=512), dict(pages=0),
        dict(pages=(1 << 24) + 1), dict(seqs=0), dict(seqs=4097), dict(stride=0),
-       dict(stride=(1 << 18) + 1)]
+       dict(stride=(1 << 18) + 1),
+       # more bytes than a size holds (2^16 * 2^24 pages of 2^26)
+       dict(dtype=0, layers=65536, pages=1 << 24, kv_heads=256, page_tokens=256)]
 
 
 @pytest.mark.parametrize("bad", BAD, ids=str)
 def test_layouts_are_refused(hyq, L, ctx, bad):
     kl = ctypes.byref(layout(hyq, **bad))
-    code = hyq.EDTYPE if "dtype" in bad else hyq.EINVAL
+    code = hyq.EDTYPE if bad.get("dtype", 0) == 8 else hyq.EINVAL
     assert L.hyq_kv_pool_bytes(kl) == 0
     assert L.hyq_pages_scratch_bytes(kl) == 0
     assert L.hyq_paged_attention_scratch_bytes(kl, 1, 1, 4) == 0
@@ -110,6 +112,7 @@ def test_shapes_and_scratch_are_refused(hyq, L, ctx):
     need = L.hyq_paged_attention_scratch_bytes(kl, 5, 2, 16)
     assert need > 0
     refused("attention", b"scratch", _12=need - 1)
+    refused("attention", b"must not be q", _12=need)  # (the output is q here)
     refused("extend", b"scratch", _12=L.hyq_pages_scratch_bytes(kl) - 1)
     refused("compact", b"scratch", _9=L.hyq_pages_scratch_bytes(kl) - 1)
     refused("fork", b"old", _6=4096)
