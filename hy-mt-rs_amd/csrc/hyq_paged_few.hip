@@ -26,13 +26,13 @@
 // them. A range that covers a unit whole writes the output,
 // a part of one its maximum, sum and unnormalised row to slot w + u (workers
 // and units both ascend, so w + u names each pair once), which the merge
-// joins in worker order.
+// joins in worker order. The worker of a unit's first tile notes who shares it.
 //
 // Bound by memory, and for few positions by the loads that wait for each other
 // (starts and lengths, table, keys) and the merge's launch. With the merge: 64
 // slots of up to 8192 positions, 32 heads over 8, f16 pages, 149 us for 848 MB
 // (5.7 TB/s); four of up to 60001, 16 over 4, f32 pages, 106 us for 642 MB (6.1);
-// two of up to 1100, 13.8 us, of which the merge's launch takes 4.7.
+// two of up to 1100, 11.8 us, of which the merge's launch takes 4.0.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -110,8 +110,9 @@ __device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int
     __syncthreads();
     FewPlan p;
     p.total = carry;
-    // 32 positions at least for a worker: fewer would only add partial rows
-    p.workers = (int)min((long long)max_workers, (carry * tile + 31) / 32);
+    // (a tile for a worker, while there are fewer tiles than workers: two slots of
+    // 1100 positions in f32 pages 11.8 us, two tiles a worker 13.0)
+    p.workers = (int)min((long long)max_workers, carry);
     p.base = divide(carry, max(p.workers, 1));
     p.more = (int)(carry - (long long)p.base * p.workers);
     return p;
@@ -336,7 +337,7 @@ template <> struct Ops<_Float16> {
 template <class T>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     PagedKv kv, int few_rows, int max_workers, RowsScratch rs, const float *__restrict__ q,
-    int part_rows, float *__restrict__ part, float *__restrict__ out)
+    int part_rows, float *__restrict__ part, int2 *__restrict__ shared, float *__restrict__ out)
 {
     constexpr int TILE = Ops<T>::TILE, SUB = TILE / 16;
     extern __shared__ long long before[]; // [seqs + 1]
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be; few workers lie on many CUs: two
-    // slots of 1100 positions took 14.9 us with four to a workgroup, now 13.8)
+    // slots of 1100 positions took 1.5 us longer with four to a workgroup)
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x + max_workers / FEW_WAVES *
                                                                   (threadIdx.x >> 6));
     if (w >= plan.workers) return;
@@ -503,6 +504,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
             }
         }
         l = wave::sum_halves(wave::sum_rows2(l));
+        if (t0 == 0 && lane == 0) { // who shares the unit, for the merge
+            const long long last = before[s] + (long long)(kh + 1) * tiles - 1;
+            const int n = t1 == tiles ? 1 : plan.worker(last) - w + 1;
+            shared[(size_t)s * kv.kvh + kh] = make_int2(w, n);
+        }
         if (t0 == 0 && t1 == tiles) {
             // (a row that saw nothing gives zeros)
             if (ok) Ops<T>::put(out + row * KV_D, acc, g, l > 0.f || l != l ? 1.f / l : 0.f);
@@ -558,21 +564,17 @@ template <class V> struct Joined {
 // them, by 256 threads, lane d dims 2 d and 2 d + 1. wide: row c by all four
 // waves, a quarter of the parts each, joined in wave order; otherwise rows c ..
 // c + 3, one per wave.
-template <int TILE>
-__device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int max_workers,
-                                          int part_rows, const float *__restrict__ part,
-                                          float *__restrict__ out, int kh, int s, int c, bool wide,
-                                          long long *before)
+__device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int part_rows,
+                                          const float *__restrict__ part,
+                                          const int2 *__restrict__ shared, float *__restrict__ out,
+                                          int kh, int s, int c, bool wide)
 {
-    __shared__ long long wsum[4];
     __shared__ float red[4][KV_D + 2];
     const int rep = kv.heads / kv.kvh;
+    const int2 by = shared[(size_t)s * kv.kvh + kh]; // (of a slot without rows: anything)
     const SlotRows sr = slot_rows(kv, s);
-    const int tiles = few_tiles(kv, s, few_rows, TILE);
-    if (tiles == 0 || c >= sr.n * rep) return;
-    const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
-    const long long first = before[s] + (long long)kh * tiles, last = first + tiles - 1;
-    const int w0 = plan.worker(first), n = plan.worker(last) - w0 + 1;
+    if (sr.n > few_rows || c >= sr.n * rep) return;
+    const int w0 = by.x, n = by.y;
     if (n == 1) return; // written whole
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int r = wide ? c : c + g;
@@ -628,18 +630,17 @@ __device__ __forceinline__ void merge_rows(const PagedKv &kv, const RowsScratch 
 
 // Grid: the slots' rows, one or four a workgroup, then the blocks', eight a
 // workgroup; the KV heads of a row in sequence.
-template <int TILE>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_rows, int max_workers,
-                                                          int part_rows, int wide, RowsScratch rs,
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_rows, int part_rows,
+                                                          int wide, RowsScratch rs,
                                                           const float *__restrict__ part,
+                                                          const int2 *__restrict__ shared,
                                                           float *__restrict__ out)
 {
-    extern __shared__ long long before[];
     const int each = wide ? part_rows : (part_rows + 3) / 4; // workgroups of a slot and KV head
     const int kh = blockIdx.x % kv.kvh, i = blockIdx.x / kv.kvh, n = kv.seqs * each;
     if (i < n)
-        merge_few<TILE>(kv, few_rows, max_workers, part_rows, part, out, kh, i / each,
-                        (i % each) * (wide ? 1 : 4), wide != 0, before);
+        merge_few(kv, few_rows, part_rows, part, shared, out, kh, i / each,
+                  (i % each) * (wide ? 1 : 4), wide != 0);
     else
         merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / 8), (i - n) % (PR_ROWS / 8));
 }
@@ -657,10 +658,19 @@ int few_workers(bool f16) { return f16 ? 2048 : 1024; }
 // and with five 52 us there; here they would be read twice.)
 int paged_few_rows(int rep) { return 16 / rep; }
 
+namespace {
+
+size_t parts_bytes(bool f16, int seqs, int kvh, int part_rows)
+{
+    return ((size_t)few_workers(f16) + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
+}
+
+} // namespace
+
+// Parts, then the workers of each slot and KV head.
 size_t paged_few_scratch(bool f16, int seqs, int kvh, int heads, int few)
 {
-    const int part_rows = few * (heads / kvh);
-    return ((size_t)few_workers(f16) + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
+    return parts_bytes(f16, seqs, kvh, few * (heads / kvh)) + ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
 }
 
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
@@ -668,15 +678,16 @@ int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const fl
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
+    int2 *shared = (int2 *)((char *)part + parts_bytes(kv.f16, kv.seqs, kv.kvh, part_rows));
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
     const int workers = few_workers(kv.f16);
     const dim3 grid(workers / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
     if (kv.f16)
-        hipLaunchKernelGGL(paged_few_kernel<_Float16>, grid, block, lds, st, kv, few,
-                           workers, rs, q, part_rows, part, out);
+        hipLaunchKernelGGL(paged_few_kernel<_Float16>, grid, block, lds, st, kv, few, workers, rs, q,
+                           part_rows, part, shared, out);
     else
-        hipLaunchKernelGGL(paged_few_kernel<float>, grid, block, lds, st, kv, few,
-                           workers, rs, q, part_rows, part, out);
+        hipLaunchKernelGGL(paged_few_kernel<float>, grid, block, lds, st, kv, few, workers, rs, q,
+                           part_rows, part, shared, out);
     return (int)hipGetLastError();
 }
 
@@ -685,7 +696,8 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
-    const size_t lds = ((size_t)kv.seqs + 1) * 8;
+    const int2 *shared =
+        (const int2 *)((const char *)part + parts_bytes(kv.f16, kv.seqs, kv.kvh, part_rows));
     // Few rows have many parts each (1024 workers over four slots of four KV
     // heads: 64), which all of a workgroup's waves read; many rows have few, and
     // a wave each. Wide and not: four slots of 60001 positions 124 and 134 us,
@@ -693,12 +705,8 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
     const int wide = kv.seqs * kv.kvh * part_rows <= 1024;
     const int each = wide ? part_rows : (part_rows + 3) / 4;
     const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, each, rs.cap));
-    if (kv.f16)
-        hipLaunchKernelGGL(paged_merge_kernel<Ops<_Float16>::TILE>, grid, dim3(256), lds, st, kv, few,
-                           few_workers(kv.f16), part_rows, wide, rs, part, out);
-    else
-        hipLaunchKernelGGL(paged_merge_kernel<Ops<float>::TILE>, grid, dim3(256), lds, st, kv, few,
-                           few_workers(kv.f16), part_rows, wide, rs, part, out);
+    hipLaunchKernelGGL(paged_merge_kernel, grid, dim3(256), 0, st, kv, few, part_rows, wide, rs, part,
+                       shared, out);
     return (int)hipGetLastError();
 }
 
