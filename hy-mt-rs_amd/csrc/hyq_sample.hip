@@ -19,8 +19,8 @@
 //   max     the largest value and its first index, by split
 //   bins    a histogram, by split, of (max - l) / T in 2048 bins of 1/64:
 //           counts where top-k is set, weights where top-p needs them
-//   find    (a workgroup per row) adds the splits' histograms and finds the bins
-//           that the cuts fall into
+//   find    (a workgroup per row; of few rows, every workgroup of the next launch)
+//           adds the splits' histograms and finds the bins that the cuts fall into
 //   sums    lists those bins' members, and sums the weights of the smaller bins
 //           by run
 //   draw    (a workgroup per row) cuts the list exactly, adds the kept members
@@ -29,8 +29,8 @@
 // thousand) the last launch does the row by itself, refining its cut bit by bit
 // over the row.
 //
-// Two rows of 120818 with top-k 20 and top-p are five short launches, 22 us (2.6,
-// 4.4, 5.6, 5.1, 5.6). 64 rows of 128167 with settings of all kinds take 57 us:
+// Two rows of 120818 with top-k 20 and top-p are four short launches, 20.7 us (2.6,
+// 4.4, 9.2, 5.6). 64 rows of 128167 with settings of all kinds take 57 us:
 // max 6 (the logits' stream), bins 13 and sums 16 (instructions, some 55 for each
 // value weighed, of which ten are 64-bit operations), find 8 and draw 15 (a
 // workgroup per row: latency).
@@ -53,6 +53,10 @@ constexpr int SAMPLE_BINS = 2048;  // 1/64 wide: 32 in all
 constexpr int SAMPLE_LIST = 2048;  // members of a cut's bins
 constexpr int SAMPLE_SMALL = 1024; // the largest top-k whose members are listed whole
 constexpr int SAMPLE_SPLITS = 16;
+// Up to this many rows the splits' workgroups find the cuts each for itself: 256
+// of them, one per CU. Together and apart, top-k 20: 2 rows 9.2 and 10.8 us, 16
+// rows 10.1 and 11.6, 24 rows 17.2 and 12.5.
+constexpr int FIND_ROWS = 16;
 constexpr float LEAST_TEMPERATURE = 0x1p-100f;
 constexpr float FLT_MAX = 3.402823466e38f;
 
@@ -371,13 +375,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_bins_kernel(SampleArgs 
 }
 
 // ---- find ----
-__global__ __launch_bounds__(SAMPLE_THREADS) void sample_find_kernel(SampleArgs a)
+// f, in LDS: what the row's histogram says, by a workgroup. (Ends with a barrier.)
+__device__ __forceinline__ void find_cuts(const SampleArgs &a, const RowPlan &r, int row, Found &f,
+                                          u64 *wsum)
 {
-    __shared__ u64 wsum[SAMPLE_WAVES];
-    __shared__ Found f;
-    const int row = blockIdx.x, t = threadIdx.x;
-    const RowPlan r = plan_row(a, row);
-    if (r.greedy) return;
+    const int t = threadIdx.x;
     if (t == 0) f = Found{SAMPLE_BINS, SAMPLE_BINS, -1, 0, 0, 0, 0, 0, 0}; // nothing cut: all bins summed
     if (r.counts || r.sums) {
         // this thread's two bins over all splits, and their running totals
@@ -458,10 +460,22 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_find_kernel(SampleArgs 
         }
     }
     __syncthreads();
-    if (t == 0) a.found[row] = f;
+}
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_find_kernel(SampleArgs a)
+{
+    __shared__ u64 wsum[SAMPLE_WAVES];
+    __shared__ Found f;
+    const int row = blockIdx.x;
+    const RowPlan r = plan_row(a, row);
+    if (r.greedy) return;
+    find_cuts(a, r, row, f, wsum);
+    if (threadIdx.x == 0) a.found[row] = f;
 }
 
 // ---- sums ----
+// FIND: every split finds the cuts for itself, without the launch before (see
+// FIND_ROWS).
+template <bool FIND>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs a)
 {
     __shared__ unsigned listed[2], base[2];
@@ -470,7 +484,16 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const RowPlan r = plan_row(a, row);
     if (r.greedy) return;
-    const Found g = a.found[row];
+    Found g;
+    if (FIND) {
+        __shared__ u64 wsum[SAMPLE_WAVES];
+        __shared__ Found f;
+        find_cuts(a, r, row, f, wsum);
+        g = f;
+        if (s == 0 && t == 0) a.found[row] = f;
+    } else {
+        g = a.found[row];
+    }
     if (t < 2) listed[t] = 0;
     load_table(table);
     const float *x = a.logits + (size_t)row * a.vocab;
@@ -992,7 +1015,8 @@ struct SampleLayout {
 };
 // Splits: as many workgroups as fill the GPU twice (64 rows: 57.4 us; filled once
 // 60.1, four times 61.4), but at most 16 (each workgroup of the third launch adds
-// up all of a row's histograms; two rows: 21.9 us, with 8 23.1, with 32 23.6) and
+// up all of a row's histograms; two rows, as five launches: 21.9 us, with 8 23.1,
+// with 32 23.6) and
 // none of fewer than 1024 values.
 SampleLayout sample_layout(int rows, int vocab)
 {
@@ -1050,8 +1074,12 @@ int launch_sample(const float *logits, int rows, int vocab, const float *tempera
     const dim3 grid(l.splits, rows), block(SAMPLE_THREADS);
     hipLaunchKernelGGL(sample_max_kernel, grid, block, 0, st, a);
     hipLaunchKernelGGL(sample_bins_kernel, grid, block, 0, st, a);
-    hipLaunchKernelGGL(sample_find_kernel, dim3(rows), block, 0, st, a);
-    hipLaunchKernelGGL(sample_sums_kernel, grid, block, 0, st, a);
+    if (rows <= FIND_ROWS) {
+        hipLaunchKernelGGL(sample_sums_kernel<true>, grid, block, 0, st, a);
+    } else {
+        hipLaunchKernelGGL(sample_find_kernel, dim3(rows), block, 0, st, a);
+        hipLaunchKernelGGL(sample_sums_kernel<false>, grid, block, 0, st, a);
+    }
     hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), block, 0, st, a);
     return (int)hipGetLastError();
 }

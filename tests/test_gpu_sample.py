@@ -127,9 +127,10 @@ def test_extreme_sizes(gpu_ctx, hyq):
 
 
 def test_more_rows_than_splits_serve(gpu_ctx, hyq):
-    """Rows by a workgroup each (more than half of 512), and by two."""
+    """Rows by a workgroup each (more than half of 512), by two, and on both sides
+    of those whose splits find their cuts by themselves."""
     r = np.random.default_rng(9)
-    for rows, vocab in ((600, 1500), (257, 4100), (256, 4100)):
+    for rows, vocab in ((600, 1500), (257, 4100), (256, 4100), (17, 9000), (16, 9000)):
         x = r.normal(0, 2.5, (rows, vocab)).astype(np.float32)
         check(hyq, gpu_ctx, x, r.random(rows), [SETTINGS[i % len(SETTINGS)] for i in range(rows)])
 
