@@ -73,11 +73,12 @@ inline int max_blocks(int seqs, int rows, int tq) { return rows / tq + std::min(
 // 2 c parts. Groups: a piece each, or fill_pieces.
 inline int max_pieces(int blocks, int kvh) { return blocks + fill_pieces(kvh); }
 inline int max_parts(int kvh) { return 2 * fill_pieces(kvh); }
-// Workgroups of the merge: `each` of a slot and one per eight rows of a block,
-// for every KV head.
+// Workgroups of the merge: `each` of a slot and one per MERGE_ROWS rows of a
+// block, for every KV head.
+constexpr int MERGE_ROWS = 16;
 inline long long merge_groups(int seqs, int kvh, int each, int cap)
 {
-    return ((long long)seqs * each + (long long)cap * (PR_ROWS / 8)) * kvh;
+    return ((long long)seqs * each + (long long)cap * (PR_ROWS / MERGE_ROWS)) * kvh;
 }
 
 // Where in the scratch the plan's parts lie.

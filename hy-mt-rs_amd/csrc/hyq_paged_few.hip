@@ -524,40 +524,58 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     }
 }
 
-// One row's parts p, p + step, ..., n of them, eight in flight: the running
-// maximum m, exp-sum l and a lane's sums x.
-template <class V> struct Joined {
-    float m = -INFINITY, l = 0.f;
-    V x{};
-    __device__ __forceinline__ void add(const float *p, size_t step, int n, int d)
+// ROWS rows' parts p, p + step, ..., n of each, eight in flight in all: the
+// running maxima m, exp-sums l and a lane's sums x.
+template <class V, int ROWS> struct Joined {
+    float m[ROWS], l[ROWS];
+    V x[ROWS];
+    __device__ __forceinline__ Joined()
     {
-        for (int b = 0; b < n; b += 8) {
-            float2v ml[8];
-            V v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float *o = p + (size_t)min(b + k, n - 1) * step;
-                ml[k] = *reinterpret_cast<const float2v *>(o);
-                v[k] = *reinterpret_cast<const V *>(o + 4 + d);
-            }
-            float top = m;
+        for (int r = 0; r < ROWS; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+            x[r] = V{};
+        }
+    }
+    __device__ __forceinline__ void add(const float *const (&p)[ROWS], size_t step, int n, int d)
+    {
+        constexpr int DEPTH = 8 / ROWS;
+        for (int b = 0; b < n; b += DEPTH) {
+            float2v ml[ROWS][DEPTH];
+            V v[ROWS][DEPTH];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k][0]);
-            const float base = top == -INFINITY ? 0.f : top;
-            const float c = __builtin_amdgcn_exp2f(m - base);
-            l *= c;
-            x *= c;
-            m = top;
+            for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float w = b + k < n ? __builtin_amdgcn_exp2f(ml[k][0] - base) : 0.f;
-                l = fmaf(w, ml[k][1], l);
-                x += w * v[k];
+                for (int k = 0; k < DEPTH; ++k) {
+                    const float *o = p[r] + (size_t)min(b + k, n - 1) * step;
+                    ml[r][k] = *reinterpret_cast<const float2v *>(o);
+                    v[r][k] = *reinterpret_cast<const V *>(o + 4 + d);
+                }
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                float top = m[r];
+#pragma unroll
+                for (int k = 0; k < DEPTH; ++k) top = fmaxf(top, ml[r][k][0]);
+                const float base = top == -INFINITY ? 0.f : top;
+                const float c = __builtin_amdgcn_exp2f(m[r] - base);
+                l[r] *= c;
+                x[r] *= c;
+                m[r] = top;
+#pragma unroll
+                for (int k = 0; k < DEPTH; ++k) {
+                    const float w = b + k < n ? __builtin_amdgcn_exp2f(ml[r][k][0] - base) : 0.f;
+                    l[r] = fmaf(w, ml[r][k][1], l[r]);
+                    x[r] += w * v[r][k];
+                }
             }
         }
     }
-    // what the row's sums are to be multiplied with (a row that saw nothing: 0)
-    __device__ __forceinline__ float scale() const { return l > 0.f || l != l ? 1.f / l : 0.f; }
+    // what a row's sums are to be multiplied with (a row that saw nothing: 0)
+    __device__ __forceinline__ float scale(int r) const
+    {
+        return l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
+    }
 };
 
 // Joins the parts of a slot's rows over a KV head, where several workers shared
@@ -583,52 +601,58 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     const float *p = part + ((size_t)((long long)w0 + (long long)s * kv.kvh + kh) * part_rows + r) *
                                 PAGED_PART;
     const int a = wide ? n * g / 4 : 0, b = wide ? n * (g + 1) / 4 : n;
-    Joined<float2v> j;
-    j.add(p + (size_t)a * step, step, b - a, 2 * lane);
+    Joined<float2v, 1> j;
+    j.add({p + (size_t)a * step}, step, b - a, 2 * lane);
     float *o = out + ((size_t)(sr.begin + r / rep) * kv.heads + kh * rep + r % rep) * KV_D;
     if (!wide) {
-        *reinterpret_cast<float2v *>(o + 2 * lane) = j.x * j.scale();
+        *reinterpret_cast<float2v *>(o + 2 * lane) = j.x[0] * j.scale(0);
         return;
     }
-    red[g][2 * lane] = j.x[0];
-    red[g][2 * lane + 1] = j.x[1];
+    red[g][2 * lane] = j.x[0][0];
+    red[g][2 * lane + 1] = j.x[0][1];
     if (lane == 0) {
-        red[g][KV_D] = j.m;
-        red[g][KV_D + 1] = j.l;
+        red[g][KV_D] = j.m[0];
+        red[g][KV_D + 1] = j.l[0];
     }
     __syncthreads();
     if (g) return;
     const float M = fmaxf(fmaxf(red[0][KV_D], red[1][KV_D]), fmaxf(red[2][KV_D], red[3][KV_D]));
     const float base = M == -INFINITY ? 0.f : M;
-    j.l = 0.f;
-    j.x = float2v{0.f, 0.f};
+    j.l[0] = 0.f;
+    j.x[0] = float2v{0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         const float f = __builtin_amdgcn_exp2f(red[w][KV_D] - base);
-        j.l = fmaf(f, red[w][KV_D + 1], j.l);
-        j.x += f * float2v{red[w][2 * lane], red[w][2 * lane + 1]};
+        j.l[0] = fmaf(f, red[w][KV_D + 1], j.l[0]);
+        j.x[0] += f * float2v{red[w][2 * lane], red[w][2 * lane + 1]};
     }
-    *reinterpret_cast<float2v *>(o + 2 * lane) = j.x * j.scale();
+    *reinterpret_cast<float2v *>(o + 2 * lane) = j.x[0] * j.scale(0);
 }
 
-// Joins the pieces of a block that was cut, by 256 threads: 8 rows, a 32-lane
-// half wave each, lane d dims 4 d ..
+// Joins the pieces of a block that was cut, by 256 threads: MERGE_ROWS rows, two
+// for a 32-lane half wave, lane d dims 4 d ..
 __device__ __forceinline__ void merge_rows(const PagedKv &kv, const RowsScratch &rs,
-                                           float *__restrict__ out, int kh, int b, int row8)
+                                           float *__restrict__ out, int kh, int b, int part)
 {
     const Block blk = rs.blocks[b];
     if (b >= rs.plan->blocks || blk.pieces < 2) return;
     const int rep = kv.heads / kv.kvh;
-    const int r = row8 * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31), tl = r / rep;
-    if (tl >= blk.toks) return;
-    Joined<f32x4> j;
-    j.add(rs.parts + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART,
-          (size_t)kv.kvh * PR_ROWS * PAGED_PART, blk.pieces, d);
-    *reinterpret_cast<f32x4 *>(out + ((size_t)(blk.row + tl) * kv.heads + kh * rep + r % rep) * KV_D +
-                               d) = j.x * j.scale();
+    const int r = part * MERGE_ROWS + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+    if (r / rep >= blk.toks) return;
+    const float *p = rs.parts + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
+    Joined<f32x4, 2> j; // (a row past the block's is not stored)
+    j.add({p, p + 8 * PAGED_PART}, (size_t)kv.kvh * PR_ROWS * PAGED_PART, blk.pieces, d);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int at = r + 8 * i, tl = at / rep;
+        if (tl < blk.toks)
+            *reinterpret_cast<f32x4 *>(
+                out + ((size_t)(blk.row + tl) * kv.heads + kh * rep + at % rep) * KV_D + d) =
+                j.x[i] * j.scale(i);
+    }
 }
 
-// Grid: the slots' rows, one or four a workgroup, then the blocks', eight a
+// Grid: the slots' rows, one or four a workgroup, then the blocks', MERGE_ROWS a
 // workgroup; the KV heads of a row in sequence.
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_rows, int part_rows,
                                                           int wide, RowsScratch rs,
@@ -642,7 +666,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_ro
         merge_few(kv, few_rows, part_rows, part, shared, out, kh, i / each,
                   (i % each) * (wide ? 1 : 4), wide != 0);
     else
-        merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / 8), (i - n) % (PR_ROWS / 8));
+        merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / MERGE_ROWS),
+                   (i - n) % (PR_ROWS / MERGE_ROWS));
 }
 
 // Workers: a wave on each SIMD for f32 pages, two for f16 pages, whose steps
