@@ -74,7 +74,8 @@ inline int max_blocks(int seqs, int rows, int tq) { return rows / tq + std::min(
 inline int max_pieces(int blocks, int kvh) { return blocks + fill_pieces(kvh); }
 inline int max_parts(int kvh) { return 2 * fill_pieces(kvh); }
 // Workgroups of the merge: `each` of a slot and one per MERGE_ROWS rows of a
-// block, for every KV head.
+// block, for every KV head. (Rows: three prompts beside 27 sessions took 155.1 us
+// with 8 and 152.9 with 16 and 32, one prompt 45.3, 44.8 and 45.4.)
 constexpr int MERGE_ROWS = 16;
 inline long long merge_groups(int seqs, int kvh, int each, int cap)
 {
