@@ -36,6 +36,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "hyq_paged_attn.hpp"
 #include "hyq_wave.hpp"
@@ -81,14 +82,15 @@ __device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows,
 // before[s], in LDS: the tiles of the slots before s over all KV heads, with
 // the total at before[seqs]. 256 threads. (Every workgroup forms it for itself:
 // a launch before this one would cost more than the few loads and barriers.)
-__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int tile, int max_workers,
-                                            long long *before, long long *wsum)
+__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int tile,
+                                            int max_workers, long long *before, long long *wsum)
 {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     long long carry = 0;
     for (int b = 0; b < kv.seqs; b += 256) {
         const int s = b + t;
-        const long long mine = s < kv.seqs ? (long long)few_tiles(kv, s, few_rows, tile) * kv.kvh : 0;
+        const long long mine =
+            s < kv.seqs ? (long long)few_tiles(kv, s, few_rows, tile) * kv.kvh : 0;
         long long v = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -127,13 +129,14 @@ __device__ __forceinline__ f32x4 mfma_f16(const half8 &a, const half8 &b, const 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// A vector of the cache: read once by one worker, and not to be kept in the
-// caches, which the rows and parts of this launch and the next ones are for
-// (169 -> 163 us for three prompts beside 27 sessions, 1 % for sessions alone).
-template <class V, class T> __device__ __forceinline__ V once(const T *base, unsigned off)
+// A vector of the cache: ONCE, of pages that one slot reads, not to be kept in the
+// caches, which the rows and parts of this launch and the next ones are for.
+template <class V, bool ONCE, class T>
+__device__ __forceinline__ V cached(const T *base, unsigned off)
 {
-    return __builtin_nontemporal_load(reinterpret_cast<const V *>(
-        reinterpret_cast<const char *>(base) + (unsigned)(off * sizeof(T))));
+    const V *p = reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
+                                             (unsigned)(off * sizeof(T)));
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
 }
 
 // The operands of one tile, by element type. Dims of an output element
@@ -155,19 +158,21 @@ template <> struct Ops<float> {
         }
         qscale = 1.f;
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load_k(int u, const float *head, int kpos, int g)
     {
         const unsigned o = kpos * KV_D + 4 * g;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[u][j] = once<f32x4>(head, o + 16 * j);
+        for (int j = 0; j < 8; ++j) k[u][j] = cached<f32x4, ONCE>(head, o + 16 * j);
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load_v(int u, const float *head, const int (&vpos)[4], int c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const unsigned o = vpos[e] * KV_D + 4 * c;
-            v[u][2 * e] = once<f32x4>(head, o);
-            v[u][2 * e + 1] = once<f32x4>(head, o + 64);
+            v[u][2 * e] = cached<f32x4, ONCE>(head, o);
+            v[u][2 * e + 1] = cached<f32x4, ONCE>(head, o + 64);
         }
     }
     __device__ __forceinline__ f32x4 scores(int u) const
@@ -207,7 +212,8 @@ template <> struct Ops<float> {
 #pragma unroll
         for (int x = 0; x < 8; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[0][x][i] = fabsf(v[0][x][i]) < INFINITY ? v[0][x][i] : 0.f;
+            for (int i = 0; i < 4; ++i)
+                v[0][x][i] = fabsf(v[0][x][i]) < INFINITY ? v[0][x][i] : 0.f;
         return true;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g)
@@ -267,17 +273,19 @@ template <> struct Ops<_Float16> {
                 ql[j][i] = fabsf(y) < INFINITY ? (_Float16)(y - (float)h) : (_Float16)0.f;
             }
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load_k(int u, const _Float16 *head, int kpos, int g)
     {
         const unsigned o = kpos * KV_D + 8 * g;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[u][j] = once<half8>(head, o + 32 * j);
+        for (int j = 0; j < 4; ++j) k[u][j] = cached<half8, ONCE>(head, o + 32 * j);
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load_v(int u, const _Float16 *head, const int (&vpos)[4], int c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            v[u][e] = once<half8>(head, vpos[e] * KV_D + 8 * c);
+            v[u][e] = cached<half8, ONCE>(head, vpos[e] * KV_D + 8 * c);
     }
     __device__ __forceinline__ f32x4 scores(int u) const
     {
@@ -413,78 +421,92 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         auto head_of = [&](int page) {
             return (const T *)kv.pages + (size_t)max(page, 0) * psize + (size_t)kh * hsize;
         };
-        auto load_k = [&](int p0, const int (&page)[SUB]) {
+        auto load_k = [&](auto once, int p0, const int (&page)[SUB]) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const int p = p0 + 16 * u;
-                ops.load_k(u, head_of(page[u]), (p & pmask) + max(min(c, sr.len - 1 - p), 0), g);
+                ops.template load_k<once.value>(
+                    u, head_of(page[u]), (p & pmask) + max(min(c, sr.len - 1 - p), 0), g);
             }
         };
-        auto load_v = [&](int p0, const int (&page)[SUB]) {
+        auto load_v = [&](auto once, int p0, const int (&page)[SUB]) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const int p = p0 + 16 * u, lim = sr.len - 1 - p;
                 int vp[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) vp[e] = (p & pmask) + max(min(4 * g + e, lim), 0);
-                ops.load_v(u, head_of(page[u]) + hsize * kv.kvh, vp, c);
+                ops.template load_v<once.value>(u, head_of(page[u]) + hsize * kv.kvh, vp, c);
             }
         };
+        // Whether the range begins in a page that neither neighbouring slot names
+        // at this place: beams of one prompt share their pages, and find them in
+        // the caches. Read as such and as read once, us for 64 slots of up to 8192
+        // positions: 167 and 147 alone, 131 and 152 in fours that share.
+        const int at0 = min((t0 * TILE) >> kv.shift, kv.stride - 1);
+        const int mine = entries[at0], below = s ? entries[at0 - kv.stride] : -1,
+                  above = s + 1 < kv.seqs ? entries[at0 + kv.stride] : -1;
         int page[SUB], next[SUB];
 #pragma unroll
         for (int u = 0; u < SUB; ++u) page[u] = page_of(t0 * TILE + 16 * u);
-        load_k(t0 * TILE, page);
-        load_v(t0 * TILE, page);
+        const bool alone =
+            __builtin_amdgcn_readfirstlane(mine != below && mine != above) != 0;
         bool odd = false;
-        for (int t = t0; t < t1; ++t) {
-            const int p0 = t * TILE, pn = min(t + 1, t1 - 1) * TILE;
-            f32x4 sv[SUB];
+        auto stream = [&](auto once) {
+            load_k(once, t0 * TILE, page);
+            load_v(once, t0 * TILE, page);
+            for (int t = t0; t < t1; ++t) {
+                const int p0 = t * TILE, pn = min(t + 1, t1 - 1) * TILE;
+                f32x4 sv[SUB];
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) sv[u] = ops.scores(u);
+                for (int u = 0; u < SUB; ++u) sv[u] = ops.scores(u);
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) next[u] = page_of(pn + 16 * u);
-            load_k(pn, next);
-            float mx = -INFINITY;
+                for (int u = 0; u < SUB; ++u) next[u] = page_of(pn + 16 * u);
+                load_k(once, pn, next);
+                float mx = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
+                for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool see = p0 + 16 * u + 4 * g + e <= sees && page[u] >= 0;
-                    sv[u][e] = see ? sv[u][e] * sc : -INFINITY;
-                    mx = fmaxf(mx, sv[u][e]);
+                    for (int e = 0; e < 4; ++e) {
+                        const bool see = p0 + 16 * u + 4 * g + e <= sees && page[u] >= 0;
+                        sv[u][e] = see ? sv[u][e] * sc : -INFINITY;
+                        mx = fmaxf(mx, sv[u][e]);
+                    }
+                mx = wave::max_halves(wave::max_rows2(mx));
+                const float mn = fmaxf(m, mx);
+                // a row that has seen nothing yet keeps zero weights
+                const float base = mn == -INFINITY ? 0.f : mn;
+                const float corr = __builtin_amdgcn_exp2f(m - base);
+                float rs = 0.f;
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sv[u][e] = __builtin_amdgcn_exp2f(sv[u][e] - base);
+                        rs += sv[u][e];
+                    }
+                if (__any(mn != m)) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) acc[x] *= corr;
+                    l *= corr;
                 }
-            mx = wave::max_halves(wave::max_rows2(mx));
-            const float mn = fmaxf(m, mx);
-            // a row that has seen nothing yet keeps zero weights
-            const float base = mn == -INFINITY ? 0.f : mn;
-            const float corr = __builtin_amdgcn_exp2f(m - base);
-            float rs = 0.f;
+                l += rs;
+                m = mn;
+                // a step that some row does not see whole: a value that is not finite
+                // must not reach the rows that do not see it (0 * inf), see below
+                bool whole = p0 + TILE - 1 <= first;
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
+                for (int u = 0; u < SUB; ++u) whole = whole && page[u] >= 0;
+                if (!whole) odd |= ops.clean();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sv[u][e] = __builtin_amdgcn_exp2f(sv[u][e] - base);
-                    rs += sv[u][e];
-                }
-            if (__any(mn != m)) {
+                for (int u = 0; u < SUB; ++u) ops.pv(u, sv[u], acc);
+                load_v(once, pn, next);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) acc[x] *= corr;
-                l *= corr;
+                for (int u = 0; u < SUB; ++u) page[u] = next[u];
             }
-            l += rs;
-            m = mn;
-            // a step that some row does not see whole: a value that is not finite
-            // must not reach the rows that do not see it (0 * inf), see below
-            bool whole = p0 + TILE - 1 <= first;
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) whole = whole && page[u] >= 0;
-            if (!whole) odd |= ops.clean();
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) ops.pv(u, sv[u], acc);
-            load_v(pn, next);
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) page[u] = next[u];
-        }
+        };
+        if (alone) stream(std::true_type{});
+        else stream(std::false_type{});
         if (odd) {
             // the values left out of the steps above, for the rows that see
             // them: whatever its weight, such a value makes the sum not finite
@@ -695,7 +717,8 @@ size_t parts_bytes(bool f16, int seqs, int kvh, int part_rows)
 // Parts, then the workers of each slot and KV head.
 size_t paged_few_scratch(bool f16, int seqs, int kvh, int heads, int few)
 {
-    return parts_bytes(f16, seqs, kvh, few * (heads / kvh)) + ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
+    const size_t shared = ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
+    return parts_bytes(f16, seqs, kvh, few * (heads / kvh)) + shared;
 }
 
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,

@@ -87,6 +87,18 @@ def test_long_and_short(gpu_ctx, hyq, f16):
 
 
 @pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("news", [1, 30])
+def test_slots_that_share_pages(gpu_ctx, hyq, news, f16):
+    """Beams of one prompt: slots that name the same pages at the same places,
+    all of them, the first ones, later ones only, and none."""
+    b = R.Batch([600, 600, 480, 600, 600, 200], [news] * 6, 8, 2, 32, f16, seed=22)
+    b.table[1, :18] = b.table[0, :18]
+    b.table[2, :14] = b.table[0, :14]
+    b.table[4, 7:18] = b.table[3, 7:18]
+    check(b, attention(hyq, gpu_ctx, b))
+
+
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
 def test_uneven_prompts(gpu_ctx, hyq, f16):
     """Two long prompts beside many short ones, too many blocks for the long
     ones to be cut finely by themselves: workgroups take several blocks' steps."""
