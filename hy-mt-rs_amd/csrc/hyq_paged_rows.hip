@@ -190,357 +190,361 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     if (group >= rs.plan->groups) return;
 #pragma unroll 1
     for (int at_piece = from; at_piece < to; ++at_piece) {
-    if (at_piece > from) __syncthreads(); // the last piece's readers of LDS are done
-    const Piece piece = rs.pieces[at_piece];
-    const int s = piece.slot, tq = rs.tq;
-    const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), part_of = wave >> 2, rows = wave & 3;
-    const int rep = kv.heads / kv.kvh;
-    const size_t hsize = (size_t)KV_D << kv.shift, psize = 2 * hsize * kv.kvh;
-    const int pmask = (1 << kv.shift) - 1;
-    const float sc = 1.4426950408889634f * 0.08838834764831845f; // log2(e) / sqrt(128)
+        if (at_piece > from) __syncthreads(); // the last piece's readers of LDS are done
+        const Piece piece = rs.pieces[at_piece];
+        const int s = piece.slot, tq = rs.tq;
+        const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;
+        const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+        const int part_of = wave >> 2, rows = wave & 3;
+        const int rep = kv.heads / kv.kvh;
+        const size_t hsize = (size_t)KV_D << kv.shift, psize = 2 * hsize * kv.kvh;
+        const int pmask = (1 << kv.shift) - 1;
+        const float sc = 1.4426950408889634f * 0.08838834764831845f; // log2(e) / sqrt(128)
 
-    const int tok0 = piece.index * tq;
-    const int first = piece.first; // position of the slot's first new row
-    const int toks = min(tq, piece.n - tok0);
-    const int p_end = min(piece.t1 * PR_TILE, first + tok0 + toks);
-    const int p_begin = piece.t0 * PR_TILE;
-    const int all_see = first + tok0; // the last position that every row sees
+        const int tok0 = piece.index * tq;
+        const int first = piece.first; // position of the slot's first new row
+        const int toks = min(tq, piece.n - tok0);
+        const int p_end = min(piece.t1 * PR_TILE, first + tok0 + toks);
+        const int p_begin = piece.t0 * PR_TILE;
+        const int all_see = first + tok0; // the last position that every row sees
 
-    // The pages of a step's four 16-position groups (or the step's one), -1 where
-    // none. Page ids come 64 at a time, one per lane. Rows past the end are
-    // loaded too, from the same page or, where there is none, from the pool's
-    // first: their weights are zero, and values that are not finite are cleared.
-    const int *entries = kv.table + (size_t)s * kv.stride;
-    int have = -64, ids = -1; // lane i: the slot's page have + i
-    constexpr int GROUPS = WHOLE ? 1 : 4;
-    struct Pages {
-        int e[GROUPS];
-        __device__ __forceinline__ int of(int group) const { return e[WHOLE ? 0 : group]; }
-        __device__ __forceinline__ bool missing() const
-        {
-            int all = e[0];
+        // The pages of a step's four 16-position groups (or the step's one), -1 where
+        // none. Page ids come 64 at a time, one per lane. Rows past the end are
+        // loaded too, from the same page or, where there is none, from the pool's
+        // first: their weights are zero, and values that are not finite are cleared.
+        const int *entries = kv.table + (size_t)s * kv.stride;
+        int have = -64, ids = -1; // lane i: the slot's page have + i
+        constexpr int GROUPS = WHOLE ? 1 : 4;
+        struct Pages {
+            int e[GROUPS];
+            __device__ __forceinline__ int of(int group) const { return e[WHOLE ? 0 : group]; }
+            __device__ __forceinline__ bool missing() const
+            {
+                int all = e[0];
 #pragma unroll
-            for (int i = 1; i < GROUPS; ++i) all |= e[i];
-            return all < 0;
-        }
-    };
-    auto pages_of = [&](int p0) {
-        Pages f;
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            const int at = p0 + 16 * i, p = at >> kv.shift;
-            if (p - have >= 64 || p < have) {
-                have = p;
-                ids = entries[min(have + lane, kv.stride - 1)];
+                for (int i = 1; i < GROUPS; ++i) all |= e[i];
+                return all < 0;
             }
-            const int e = __builtin_amdgcn_readlane(ids, p - have);
-            f.e[i] = (WHOLE || at < p_end) && (unsigned)e < (unsigned)kv.npages ? e : -1;
-        }
-        return f;
-    };
-    R raw;
-    auto load = [&](int p0, const Pages &pg) {
-        if constexpr (WHOLE) {
-            const T *b = (const T *)kv.pages + (size_t)max(pg.e[0], 0) * psize + (size_t)kh * hsize +
-                         (size_t)(p0 & pmask) * KV_D;
-#pragma unroll
-            for (int i = 0; i < R::N; ++i) {
-                const unsigned o = (R::row(t) + R::STEP * i) * KV_D + R::dim(t);
-                raw.k[i] = at<typename R::Vec>(b, o);
-                raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < R::N; ++i) {
-                const int g = R::group(wave, i), e = g == 0 ? pg.of(0) : g == 1 ? pg.of(1)
-                                                    : g == 2   ? pg.of(2)
-                                                               : pg.of(3);
-                // (a uniform base, and an offset that never changes)
-                const T *b = (const T *)kv.pages + (size_t)max(e, 0) * psize + (size_t)kh * hsize +
-                             (size_t)((p0 + 16 * g) & pmask) * KV_D;
-                const unsigned o = (R::row(t) & 15) * KV_D + R::dim(t);
-                raw.k[i] = at<typename R::Vec>(b, o);
-                raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
-            }
-        }
-    };
-    // one of the 2 N rows of `raw`, converted, to a buffer
-    auto store = [&](int buf, int n) {
-        RowsLds<LO> &l = lds.step[buf];
-        const int d = R::dim(t), r = R::row(t) + R::STEP * (n >> 1);
-        if (n & 1)
-            R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
-        else
-            R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
-    };
-    // whether some row sees a step in part
-    auto partial = [&](int p0, const Pages &pg) {
-        return p0 + PR_TILE - 1 > all_see || pg.missing();
-    };
-
-    Pages cur = pages_of(p_begin), next = pages_of(p_begin + PR_TILE);
-    load(p_begin, cur);
-
-    // this lane's query row
-    const int r = 32 * rows + c, tl = r / rep;
-    const bool ok = tl < toks;
-    const int head = kh * rep + r % rep;
-    const int sees = ok ? first + tok0 + tl : -1; // its last visible position
-    // the last position the wave's last row sees, and its first row
-    const int wave_last = first + tok0 + min(toks - 1, (32 * rows + 31) / rep);
-    const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
-    const size_t row = (size_t)(piece.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
-
-    // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range: to
-    // below 2^14 where the low parts stay as they are, and to below 2 where they
-    // are scaled like those of the keys that they are added up with.
-    half8 qhi[KV_D / 16], qlo[KV_D / 16];
-    float qscale;
-    {
-        // (loaded whatever the row, so that all loads are in flight at once)
-        const float *qr = q + row * KV_D + 8 * h;
-        float4 x[KV_D / 8];
-#pragma unroll
-        for (int kk = 0; kk < KV_D / 16; ++kk) {
-            x[2 * kk] = *reinterpret_cast<const float4 *>(qr + 16 * kk);
-            x[2 * kk + 1] = *reinterpret_cast<const float4 *>(qr + 16 * kk + 4);
-        }
-        float mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < KV_D / 8; ++k)
-            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)),
-                                 fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
-        mx = wave::max_halves(mx);
-        const int e = (mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0) - (LO ? 0 : 13);
-        qscale = ldexpf(sc, e);
-        const float inv = ok ? ldexpf(1.f, -e) : 0.f;
-#pragma unroll
-        for (int kk = 0; kk < KV_D / 16; ++kk) {
-            const float4 a = x[2 * kk], b = x[2 * kk + 1];
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                half2 hi, lo;
-                if constexpr (LO) split2_scaled(v[i] * inv, v[i + 1] * inv, hi, lo);
-                else split2(v[i] * inv, v[i + 1] * inv, hi, lo);
-                qhi[kk][i] = hi[0];
-                qhi[kk][i + 1] = hi[1];
-                qlo[kk][i] = lo[0];
-                qlo[kk][i + 1] = lo[1];
-            }
-        }
-    }
-
-    f32x16 acc[KV_D / 32];
-#pragma unroll
-    for (int j = 0; j < KV_D / 32; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-
-    // A step that some row sees in part: values of it that are not finite must
-    // not reach the rows that do not see them (0 * inf), see below.
-    bool odd = partial(p_begin, cur) && raw.clean();
-#pragma unroll
-    for (int n = 0; n < 2 * R::N; ++n) store(0, n);
-    load(p_begin + PR_TILE, next);
-    __syncthreads();
-    int buf = 0;
-    const int o = 32 * part_of; // this wave's 32 positions of a step
-    for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
-        const Pages after = pages_of(p0 + 2 * PR_TILE);
-        const RowsLds<LO> &l = lds.step[buf];
-        const int p = p0 + o, pa = part_of ? cur.of(2) : cur.of(0),
-                  pb = part_of ? cur.of(3) : cur.of(1);
-        if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
-        // (sx: the products with low parts, where those are scaled)
-        f32x16 sv, sx;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sv[e] = sx[e] = 0.f;
-        // Scores, with the next step's rows converted between their products (the
-        // matrix unit takes 32 cycles for each). Operands are read one product
-        // ahead, and no further: the barriers to the compiler's scheduling keep
-        // the kernel inside its registers.
-        half8 ahi[2], alo[2];
-        auto keys = [&](int kk) {
-            ahi[kk & 1] = *reinterpret_cast<const half8 *>(&l.khi[o + c][16 * kk + 8 * h]);
-            if constexpr (LO)
-                alo[kk & 1] = *reinterpret_cast<const half8 *>(&l.klo[o + c][16 * kk + 8 * h]);
         };
-        keys(0);
+        auto pages_of = [&](int p0) {
+            Pages f;
 #pragma unroll
-        for (int kk = 0; kk < KV_D / 16; ++kk) {
-            if (kk + 1 < KV_D / 16) keys(kk + 1);
-            if constexpr (LO) {
-                sx = mfma(ahi[kk & 1], qlo[kk], sx);
-                sv = mfma(ahi[kk & 1], qhi[kk], sv);
-                sx = mfma(alo[kk & 1], qhi[kk], sx);
+            for (int i = 0; i < GROUPS; ++i) {
+                const int at = p0 + 16 * i, p = at >> kv.shift;
+                if (p - have >= 64 || p < have) {
+                    have = p;
+                    ids = entries[min(have + lane, kv.stride - 1)];
+                }
+                const int e = __builtin_amdgcn_readlane(ids, p - have);
+                f.e[i] = (WHOLE || at < p_end) && (unsigned)e < (unsigned)kv.npages ? e : -1;
+            }
+            return f;
+        };
+        R raw;
+        auto load = [&](int p0, const Pages &pg) {
+            if constexpr (WHOLE) {
+                const T *b = (const T *)kv.pages + (size_t)max(pg.e[0], 0) * psize +
+                             (size_t)kh * hsize + (size_t)(p0 & pmask) * KV_D;
+#pragma unroll
+                for (int i = 0; i < R::N; ++i) {
+                    const unsigned o = (R::row(t) + R::STEP * i) * KV_D + R::dim(t);
+                    raw.k[i] = at<typename R::Vec>(b, o);
+                    raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
+                }
             } else {
-                sv = mfma(ahi[kk & 1], qhi[kk], sv);
-                sv = mfma(ahi[kk & 1], qlo[kk], sv);
-            }
-            if (kk < 2 * R::N) store(buf ^ 1, kk);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        load(p0 + 2 * PR_TILE, after);
-        if constexpr (LO) sv += sx * (1.f / LO_SCALE);
-        if (p + 31 > wave_all || (pa | pb) < 0) { // mask
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int pos = p + 8 * (e >> 2) + 4 * h + (e & 3);
-                sv[e] = pos <= sees && (e < 8 ? pa : pb) >= 0 ? sv[e] : -INFINITY;
-            }
-        }
-        float tmax = sv[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, sv[e]);
-        // The running maximum follows only when a score passes it by 2^8 or
-        // more: until then weights are at most 2^8 times the first, and the 64
-        // products that bring the sums to a new one are rare (in 32 rows of
-        // equal chances some row has a new maximum in most steps). m_run lies 7
-        // below the maximum, so that weights go up to 2^15: their f16 parts
-        // resolve 2^-25, which is 2^-32 of the first weight. (Many equal small
-        // weights are rounded the same way, and their errors add up.)
-        const float m_new = fmaf(wave::max_halves(tmax), qscale, -7.f);
-        if (__any(m_new > m_run + 8.f)) {
-            const float m = fmaxf(m_run, m_new);
-            const float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
-#pragma unroll
-            for (int j = 0; j < KV_D / 32; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
-            l_run *= corr;
-            m_run = m;
-        }
-        const float base = m_run == -INFINITY ? 0.f : m_run; // (nothing seen yet: zero weights)
-        float rs[2] = {0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            sv[e] = __builtin_amdgcn_exp2f(fmaf(sv[e], qscale, -base));
-            rs[e & 1] += sv[e];
-        }
-        l_run += rs[0] + rs[1];
-        // operand element 4 x + i of product (kk, j): position 16 kk + 8 x + 4 h + i,
-        // which is the lane's weight 8 kk + 4 x + i
-        half8 vhi[4], vlo[4];
-        auto values = [&](int n) {
-            const int kk = n >> 2, j = n & 3;
-            const int vr = o + 16 * kk + 4 * h + ((lane & 15) >> 2);
-            const int vd = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const half4 x = read_transposed(&l.vhi[vr][vd]),
-                        y = read_transposed(&l.vhi[vr + 8][vd]);
-            vhi[n & 3] = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            if constexpr (LO) {
-                const half4 z = read_transposed(&l.vlo[vr][vd]),
-                            w = read_transposed(&l.vlo[vr + 8][vd]);
-                vlo[n & 3] = half8{z[0], z[1], z[2], z[3], w[0], w[1], w[2], w[3]};
+                for (int i = 0; i < R::N; ++i) {
+                    const int g = R::group(wave, i), e = g == 0 ? pg.of(0) : g == 1 ? pg.of(1)
+                                                        : g == 2   ? pg.of(2)
+                                                                   : pg.of(3);
+                    // (a uniform base, and an offset that never changes)
+                    const T *b = (const T *)kv.pages + (size_t)max(e, 0) * psize +
+                                 (size_t)kh * hsize + (size_t)((p0 + 16 * g) & pmask) * KV_D;
+                    const unsigned o = (R::row(t) & 15) * KV_D + R::dim(t);
+                    raw.k[i] = at<typename R::Vec>(b, o);
+                    raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
+                }
             }
         };
-        half8 phi, plo, pls; // (pls: the weights of the values' low parts)
-        values(0);
-        values(1);
+        // one of the 2 N rows of `raw`, converted, to a buffer
+        auto store = [&](int buf, int n) {
+            RowsLds<LO> &l = lds.step[buf];
+            const int d = R::dim(t), r = R::row(t) + R::STEP * (n >> 1);
+            if (n & 1)
+                R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
+            else
+                R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
+        };
+        // whether some row sees a step in part
+        auto partial = [&](int p0, const Pages &pg) {
+            return p0 + PR_TILE - 1 > all_see || pg.missing();
+        };
+
+        Pages cur = pages_of(p_begin), next = pages_of(p_begin + PR_TILE);
+        load(p_begin, cur);
+
+        // this lane's query row
+        const int r = 32 * rows + c, tl = r / rep;
+        const bool ok = tl < toks;
+        const int head = kh * rep + r % rep;
+        const int sees = ok ? first + tok0 + tl : -1; // its last visible position
+        // the last position the wave's last row sees, and its first row
+        const int wave_last = first + tok0 + min(toks - 1, (32 * rows + 31) / rep);
+        const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
+        const size_t row = (size_t)(piece.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
+
+        // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range: to
+        // below 2^14 where the low parts stay as they are, and to below 2 where they
+        // are scaled like those of the keys that they are added up with.
+        half8 qhi[KV_D / 16], qlo[KV_D / 16];
+        float qscale;
+        {
+            // (loaded whatever the row, so that all loads are in flight at once)
+            const float *qr = q + row * KV_D + 8 * h;
+            float4 x[KV_D / 8];
 #pragma unroll
-        for (int n = 0; n < 8; n += 2) { // two products' sums in turn
-            if ((n & 3) == 0) {
+            for (int kk = 0; kk < KV_D / 16; ++kk) {
+                x[2 * kk] = *reinterpret_cast<const float4 *>(qr + 16 * kk);
+                x[2 * kk + 1] = *reinterpret_cast<const float4 *>(qr + 16 * kk + 4);
+            }
+            float mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < KV_D / 8; ++k)
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)),
+                                     fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
+            mx = wave::max_halves(mx);
+            const int e = (mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0) - (LO ? 0 : 13);
+            qscale = ldexpf(sc, e);
+            const float inv = ok ? ldexpf(1.f, -e) : 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KV_D / 16; ++kk) {
+                const float4 a = x[2 * kk], b = x[2 * kk + 1];
+                const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     half2 hi, lo;
-                    split2(sv[2 * n + i], sv[2 * n + i + 1], hi, lo);
-                    phi[i] = hi[0];
-                    phi[i + 1] = hi[1];
-                    plo[i] = lo[0];
-                    plo[i + 1] = lo[1];
+                    if constexpr (LO) split2_scaled(v[i] * inv, v[i + 1] * inv, hi, lo);
+                    else split2(v[i] * inv, v[i + 1] * inv, hi, lo);
+                    qhi[kk][i] = hi[0];
+                    qhi[kk][i + 1] = hi[1];
+                    qlo[kk][i] = lo[0];
+                    qlo[kk][i + 1] = lo[1];
                 }
-                if constexpr (LO) pls = phi * (_Float16)(1.f / LO_SCALE);
             }
-            if (n + 2 < 8) {
-                values(n + 2);
-                values(n + 3);
+        }
+
+        f32x16 acc[KV_D / 32];
+#pragma unroll
+        for (int j = 0; j < KV_D / 32; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+        float m_run = -INFINITY, l_run = 0.f;
+
+        // A step that some row sees in part: values of it that are not finite must
+        // not reach the rows that do not see them (0 * inf), see below.
+        bool odd = partial(p_begin, cur) && raw.clean();
+#pragma unroll
+        for (int n = 0; n < 2 * R::N; ++n) store(0, n);
+        load(p_begin + PR_TILE, next);
+        __syncthreads();
+        int buf = 0;
+        const int o = 32 * part_of; // this wave's 32 positions of a step
+        for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
+            const Pages after = pages_of(p0 + 2 * PR_TILE);
+            const RowsLds<LO> &l = lds.step[buf];
+            const int p = p0 + o, pa = part_of ? cur.of(2) : cur.of(0),
+                      pb = part_of ? cur.of(3) : cur.of(1);
+            if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
+            // (sx: the products with low parts, where those are scaled)
+            f32x16 sv, sx;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sv[e] = sx[e] = 0.f;
+            // Scores, with the next step's rows converted between their products (the
+            // matrix unit takes 32 cycles for each). Operands are read one product
+            // ahead, and no further: the barriers to the compiler's scheduling keep
+            // the kernel inside its registers.
+            half8 ahi[2], alo[2];
+            auto keys = [&](int kk) {
+                ahi[kk & 1] = *reinterpret_cast<const half8 *>(&l.khi[o + c][16 * kk + 8 * h]);
+                if constexpr (LO)
+                    alo[kk & 1] = *reinterpret_cast<const half8 *>(&l.klo[o + c][16 * kk + 8 * h]);
+            };
+            keys(0);
+#pragma unroll
+            for (int kk = 0; kk < KV_D / 16; ++kk) {
+                if (kk + 1 < KV_D / 16) keys(kk + 1);
+                if constexpr (LO) {
+                    sx = mfma(ahi[kk & 1], qlo[kk], sx);
+                    sv = mfma(ahi[kk & 1], qhi[kk], sv);
+                    sx = mfma(alo[kk & 1], qhi[kk], sx);
+                } else {
+                    sv = mfma(ahi[kk & 1], qhi[kk], sv);
+                    sv = mfma(ahi[kk & 1], qlo[kk], sv);
+                }
+                if (kk < 2 * R::N) store(buf ^ 1, kk);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            f32x16 &d = acc[n & 3], &e = acc[(n + 1) & 3];
-            d = mfma(vhi[n & 3], phi, d);
-            e = mfma(vhi[(n + 1) & 3], phi, e);
-            d = mfma(vhi[n & 3], plo, d);
-            e = mfma(vhi[(n + 1) & 3], plo, e);
-            if constexpr (LO) {
-                d = mfma(vlo[n & 3], pls, d);
-                e = mfma(vlo[(n + 1) & 3], pls, e);
+            load(p0 + 2 * PR_TILE, after);
+            if constexpr (LO) sv += sx * (1.f / LO_SCALE);
+            if (p + 31 > wave_all || (pa | pb) < 0) { // mask
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int pos = p + 8 * (e >> 2) + 4 * h + (e & 3);
+                    sv[e] = pos <= sees && (e < 8 ? pa : pb) >= 0 ? sv[e] : -INFINITY;
+                }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            float tmax = sv[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, sv[e]);
+            // The running maximum follows only when a score passes it by 2^8 or
+            // more: until then weights are at most 2^8 times the first, and the 64
+            // products that bring the sums to a new one are rare (in 32 rows of
+            // equal chances some row has a new maximum in most steps). m_run lies 7
+            // below the maximum, so that weights go up to 2^15: their f16 parts
+            // resolve 2^-25, which is 2^-32 of the first weight. (Many equal small
+            // weights are rounded the same way, and their errors add up.)
+            const float m_new = fmaf(wave::max_halves(tmax), qscale, -7.f);
+            if (__any(m_new > m_run + 8.f)) {
+                const float m = fmaxf(m_run, m_new);
+                const float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+#pragma unroll
+                for (int j = 0; j < KV_D / 32; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
+                l_run *= corr;
+                m_run = m;
+            }
+            const float base = m_run == -INFINITY ? 0.f : m_run; // (nothing seen yet: zero weights)
+            float rs[2] = {0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sv[e] = __builtin_amdgcn_exp2f(fmaf(sv[e], qscale, -base));
+                rs[e & 1] += sv[e];
+            }
+            l_run += rs[0] + rs[1];
+            // operand element 4 x + i of product (kk, j): position 16 kk + 8 x + 4 h + i,
+            // which is the lane's weight 8 kk + 4 x + i
+            half8 vhi[4], vlo[4];
+            auto values = [&](int n) {
+                const int kk = n >> 2, j = n & 3;
+                const int vr = o + 16 * kk + 4 * h + ((lane & 15) >> 2);
+                const int vd = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const half4 x = read_transposed(&l.vhi[vr][vd]),
+                            y = read_transposed(&l.vhi[vr + 8][vd]);
+                vhi[n & 3] = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                if constexpr (LO) {
+                    const half4 z = read_transposed(&l.vlo[vr][vd]),
+                                w = read_transposed(&l.vlo[vr + 8][vd]);
+                    vlo[n & 3] = half8{z[0], z[1], z[2], z[3], w[0], w[1], w[2], w[3]};
+                }
+            };
+            half8 phi, plo, pls; // (pls: the weights of the values' low parts)
+            values(0);
+            values(1);
+#pragma unroll
+            for (int n = 0; n < 8; n += 2) { // two products' sums in turn
+                if ((n & 3) == 0) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        half2 hi, lo;
+                        split2(sv[2 * n + i], sv[2 * n + i + 1], hi, lo);
+                        phi[i] = hi[0];
+                        phi[i + 1] = hi[1];
+                        plo[i] = lo[0];
+                        plo[i + 1] = lo[1];
+                    }
+                    if constexpr (LO) pls = phi * (_Float16)(1.f / LO_SCALE);
+                }
+                if (n + 2 < 8) {
+                    values(n + 2);
+                    values(n + 3);
+                }
+                f32x16 &d = acc[n & 3], &e = acc[(n + 1) & 3];
+                d = mfma(vhi[n & 3], phi, d);
+                e = mfma(vhi[(n + 1) & 3], phi, e);
+                d = mfma(vhi[n & 3], plo, d);
+                e = mfma(vhi[(n + 1) & 3], plo, e);
+                if constexpr (LO) {
+                    d = mfma(vlo[n & 3], pls, d);
+                    e = mfma(vlo[(n + 1) & 3], pls, e);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __syncthreads();
+            cur = next;
+            next = after;
+            buf ^= 1;
+        }
+        if (__syncthreads_or(odd)) {
+            // the values left out, for the rows that see them: whatever its weight,
+            // such a value makes the sum not finite
+            for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
+                const Pages pg = pages_of(p0);
+                if (!partial(p0, pg)) continue;
+                for (int i = 0; i < 32; ++i) {
+                    const int pos = p0 + 32 * part_of + i;
+                    const int e = i < 16 ? (part_of ? pg.of(2) : pg.of(0))
+                                         : (part_of ? pg.of(3) : pg.of(1));
+                    if (pos > sees || e < 0) continue;
+                    const T *vb = (const T *)kv.pages + (size_t)e * psize +
+                                  (size_t)(kv.kvh + kh) * hsize + (size_t)(pos & pmask) * KV_D;
+#pragma unroll
+                    for (int j = 0; j < KV_D / 32; ++j) {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            const float v = (float)vb[32 * j + 8 * (x >> 2) + 4 * h + (x & 3)];
+                            acc[j][x] += fabsf(v) < INFINITY ? 0.f : v;
+                        }
+                        asm volatile("" ::: "memory"); // (few loads at once: a rare path)
+                    }
+                }
+            }
+        }
+
+        // the two halves' rows joined, in the first half's waves
+        l_run = wave::sum_halves(l_run);
+        if (part_of) {
+            float(*o)[64] = lds.join[rows];
+            o[0][lane] = m_run;
+            o[1][lane] = l_run;
+#pragma unroll
+            for (int j = 0; j < KV_D / 32; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[2 + 16 * j + e][lane] = acc[j][e];
         }
         __syncthreads();
-        cur = next;
-        next = after;
-        buf ^= 1;
-    }
-    if (__syncthreads_or(odd)) {
-        // the values left out, for the rows that see them: whatever its weight,
-        // such a value makes the sum not finite
-        for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
-            const Pages pg = pages_of(p0);
-            if (!partial(p0, pg)) continue;
-            for (int i = 0; i < 32; ++i) {
-                const int pos = p0 + 32 * part_of + i;
-                const int e = i < 16 ? (part_of ? pg.of(2) : pg.of(0)) : part_of ? pg.of(3) : pg.of(1);
-                if (pos > sees || e < 0) continue;
-                const T *vb = (const T *)kv.pages + (size_t)e * psize +
-                              (size_t)(kv.kvh + kh) * hsize + (size_t)(pos & pmask) * KV_D;
+        if (part_of || !ok) continue;
+        {
+            const float(*o)[64] = lds.join[rows];
+            const float m2 = o[0][lane], m = fmaxf(m_run, m2), base = m == -INFINITY ? 0.f : m;
+            const float a = __builtin_amdgcn_exp2f(m_run - base),
+                        b = __builtin_amdgcn_exp2f(m2 - base);
+            l_run = l_run * a + o[1][lane] * b;
+            m_run = m;
 #pragma unroll
-                for (int j = 0; j < KV_D / 32; ++j) {
+            for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const float v = (float)vb[32 * j + 8 * (x >> 2) + 4 * h + (x & 3)];
-                        acc[j][x] += fabsf(v) < INFINITY ? 0.f : v;
-                    }
-                    asm volatile("" ::: "memory"); // (few loads at once: a rare path)
-                }
+                for (int e = 0; e < 16; ++e)
+                    acc[j][e] = acc[j][e] * a + o[2 + 16 * j + e][lane] * b;
+        }
+        float *dst = out + row * KV_D;
+        float f = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f; // (saw nothing: zeros)
+        if (piece.part >= 0) {
+            dst = rs.parts + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
+            if (h == 0) {
+                dst[0] = m_run;
+                dst[1] = l_run;
             }
+            dst += 4;
+            f = 1.f;
         }
-    }
-
-    // the two halves' rows joined, in the first half's waves
-    l_run = wave::sum_halves(l_run);
-    if (part_of) {
-        float(*o)[64] = lds.join[rows];
-        o[0][lane] = m_run;
-        o[1][lane] = l_run;
 #pragma unroll
         for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[2 + 16 * j + e][lane] = acc[j][e];
-    }
-    __syncthreads();
-    if (part_of || !ok) continue;
-    {
-        const float(*o)[64] = lds.join[rows];
-        const float m2 = o[0][lane], m = fmaxf(m_run, m2), base = m == -INFINITY ? 0.f : m;
-        const float a = __builtin_amdgcn_exp2f(m_run - base), b = __builtin_amdgcn_exp2f(m2 - base);
-        l_run = l_run * a + o[1][lane] * b;
-        m_run = m;
-#pragma unroll
-        for (int j = 0; j < KV_D / 32; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * a + o[2 + 16 * j + e][lane] * b;
-    }
-    float *dst = out + row * KV_D;
-    float f = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f; // (saw nothing: zeros)
-    if (piece.part >= 0) {
-        dst = rs.parts + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
-        if (h == 0) {
-            dst[0] = m_run;
-            dst[1] = l_run;
-        }
-        dst += 4;
-        f = 1.f;
-    }
-#pragma unroll
-    for (int j = 0; j < KV_D / 32; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4 *>(dst + 32 * j + 8 * g + 4 * h) =
-                make_float4(acc[j][4 * g] * f, acc[j][4 * g + 1] * f, acc[j][4 * g + 2] * f,
-                            acc[j][4 * g + 3] * f);
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4 *>(dst + 32 * j + 8 * g + 4 * h) =
+                    make_float4(acc[j][4 * g] * f, acc[j][4 * g + 1] * f, acc[j][4 * g + 2] * f,
+                                acc[j][4 * g + 3] * f);
     }
 }
 
@@ -551,10 +555,10 @@ int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, 
 {
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh); // (more groups there are not)
-    const auto kernel = 1 << kv.shift >= PR_TILE
-                            ? (kv.f16 ? paged_rows_kernel<_Float16, true> : paged_rows_kernel<float, true>)
-                            : (kv.f16 ? paged_rows_kernel<_Float16, false>
-                                      : paged_rows_kernel<float, false>);
+    const bool whole = 1 << kv.shift >= PR_TILE;
+    auto kernel = whole ? paged_rows_kernel<float, true> : paged_rows_kernel<float, false>;
+    if (kv.f16)
+        kernel = whole ? paged_rows_kernel<_Float16, true> : paged_rows_kernel<_Float16, false>;
     hipLaunchKernelGGL(kernel, grid, dim3(PR_THREADS), 0, st, kv, rs, q, out);
     return (int)hipGetLastError();
 }

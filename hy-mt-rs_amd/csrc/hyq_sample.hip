@@ -380,7 +380,8 @@ __device__ __forceinline__ void find_cuts(const SampleArgs &a, const RowPlan &r,
                                           u64 *wsum)
 {
     const int t = threadIdx.x;
-    if (t == 0) f = Found{SAMPLE_BINS, SAMPLE_BINS, -1, 0, 0, 0, 0, 0, 0}; // nothing cut: all bins summed
+    // (nothing cut: all bins summed)
+    if (t == 0) f = Found{SAMPLE_BINS, SAMPLE_BINS, -1, 0, 0, 0, 0, 0, 0};
     if (r.counts || r.sums) {
         // this thread's two bins over all splits, and their running totals
         u64 c0 = 0, c1 = 0, w0 = 0, w1 = 0, ctotal = 0, wtotal = 0;
@@ -708,14 +709,15 @@ __device__ __forceinline__ void row_alone(const SampleArgs &a, const RowPlan &pl
 }
 
 
-// Cuts a list in LDS, whose keys lie in `range`, by a workgroup: finds the smallest key of the order's
-// shortest prefix that has `count` members or the weight `target` (the other
-// one is unbounded); at most all n members. *weight_of: that prefix's weight.
-// Digits of 8 bits, largest first: a histogram of the members that share the
-// digits so far, of which one wave finds the digit where the prefix ends, until
-// 64 members are left, which are ranked against each other (going on to a single
-// one took up to two more digits: a launch of two cuts of 1000 members 18.5 ->
-// 17.1 us, and 15.1 with the keys' range found while they are loaded).
+// Cuts a list in LDS, whose keys lie in `range`, by a workgroup: finds the
+// smallest key of the order's shortest prefix that has `count` members or the
+// weight `target` (the other one is unbounded); at most all n members.
+// *weight_of: that prefix's weight. Digits of 8 bits, largest first: a histogram
+// of the members that share the digits so far, of which one wave finds the digit
+// where the prefix ends, until 64 members are left, which are ranked against each
+// other (going on to a single one took up to two more digits: a launch of two cuts
+// of 1000 members 18.5 -> 17.1 us, and 15.1 with the keys' range found while they
+// are loaded).
 struct ListScratch {
     u64 hw[256];
     u64 rank[64];           // of the members ranked: the weight before them
