@@ -51,6 +51,7 @@ typedef float float2v __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int FEW_WAVES = 4;
+constexpr int TILE = 16; // positions of a step
 
 // Worker w of `workers` takes `base` tiles, the first `more` workers one more.
 struct FewPlan {
@@ -69,28 +70,27 @@ struct FewPlan {
 };
 
 // (new rows over no positions still have their zeros to be written: one tile)
-__device__ __forceinline__ int slot_tiles(const SlotRows &r, int tile)
+__device__ __forceinline__ int slot_tiles(const SlotRows &r)
 {
-    return max(1, (r.len + tile - 1) / tile);
+    return max(1, (r.len + TILE - 1) / TILE);
 }
-__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows, int tile)
+__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows)
 {
     const SlotRows r = slot_rows(kv, s);
-    return r.n > 0 && r.n <= few_rows ? slot_tiles(r, tile) : 0;
+    return r.n > 0 && r.n <= few_rows ? slot_tiles(r) : 0;
 }
 
 // before[s], in LDS: the tiles of the slots before s over all KV heads, with
 // the total at before[seqs]. 256 threads. (Every workgroup forms it for itself:
 // a launch before this one would cost more than the few loads and barriers.)
-__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int tile,
-                                            int max_workers, long long *before, long long *wsum)
+__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int max_workers,
+                                            long long *before, long long *wsum)
 {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     long long carry = 0;
     for (int b = 0; b < kv.seqs; b += 256) {
         const int s = b + t;
-        const long long mine =
-            s < kv.seqs ? (long long)few_tiles(kv, s, few_rows, tile) * kv.kvh : 0;
+        const long long mine = s < kv.seqs ? (long long)few_tiles(kv, s, few_rows) * kv.kvh : 0;
         long long v = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -144,10 +144,9 @@ __device__ __forceinline__ V cached(const T *base, unsigned off)
 template <class T> struct Ops;
 
 template <> struct Ops<float> {
-    static constexpr int TILE = 16; // positions of a step
     float4 q[8]; // row lane % 16, dims 16 j + 4 g ..
-    f32x4 k[1][8]; // position lane % 16, the same dims
-    f32x4 v[1][8]; // position 4 g + x / 2, dims 64 (x % 2) + 4 (lane % 16) ..
+    f32x4 k[8];  // position lane % 16, the same dims
+    f32x4 v[8];  // position 4 g + x / 2, dims 64 (x % 2) + 4 (lane % 16) ..
     float qscale;
     __device__ __forceinline__ void load_q(const float *row, bool ok, int g)
     {
@@ -159,41 +158,41 @@ template <> struct Ops<float> {
         qscale = 1.f;
     }
     template <bool ONCE>
-    __device__ __forceinline__ void load_k(int u, const float *head, int kpos, int g)
+    __device__ __forceinline__ void load_k(const float *head, int kpos, int g)
     {
         const unsigned o = kpos * KV_D + 4 * g;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[u][j] = cached<f32x4, ONCE>(head, o + 16 * j);
+        for (int j = 0; j < 8; ++j) k[j] = cached<f32x4, ONCE>(head, o + 16 * j);
     }
     template <bool ONCE>
-    __device__ __forceinline__ void load_v(int u, const float *head, const int (&vpos)[4], int c)
+    __device__ __forceinline__ void load_v(const float *head, const int (&vpos)[4], int c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const unsigned o = vpos[e] * KV_D + 4 * c;
-            v[u][2 * e] = cached<f32x4, ONCE>(head, o);
-            v[u][2 * e + 1] = cached<f32x4, ONCE>(head, o + 64);
+            v[2 * e] = cached<f32x4, ONCE>(head, o);
+            v[2 * e + 1] = cached<f32x4, ONCE>(head, o + 64);
         }
     }
-    __device__ __forceinline__ f32x4 scores(int u) const
+    __device__ __forceinline__ f32x4 scores() const
     {
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            a = mfma_f32(k[u][j].x, q[j].x, a);
-            b = mfma_f32(k[u][j].y, q[j].y, b);
-            a = mfma_f32(k[u][j].z, q[j].z, a);
-            b = mfma_f32(k[u][j].w, q[j].w, b);
+            a = mfma_f32(k[j].x, q[j].x, a);
+            b = mfma_f32(k[j].y, q[j].y, b);
+            a = mfma_f32(k[j].z, q[j].z, a);
+            b = mfma_f32(k[j].w, q[j].w, b);
         }
         return a + b;
     }
-    __device__ __forceinline__ void pv(int u, const f32x4 &p, f32x4 (&acc)[8]) const
+    __device__ __forceinline__ void pv(const f32x4 &p, f32x4 (&acc)[8]) const
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const f32x4 x = v[u][2 * e + c];
+                const f32x4 x = v[2 * e + c];
                 acc[4 * c] = mfma_f32(x.x, p[e], acc[4 * c]);
                 acc[4 * c + 1] = mfma_f32(x.y, p[e], acc[4 * c + 1]);
                 acc[4 * c + 2] = mfma_f32(x.z, p[e], acc[4 * c + 2]);
@@ -206,14 +205,14 @@ template <> struct Ops<float> {
         float z = 0.f; // (a sum of v * 0: not zero if one is not finite)
 #pragma unroll
         for (int x = 0; x < 8; ++x)
-            z = fmaf(v[0][x].x, 0.f,
-                     fmaf(v[0][x].y, 0.f, fmaf(v[0][x].z, 0.f, fmaf(v[0][x].w, 0.f, z))));
+            z = fmaf(v[x].x, 0.f,
+                     fmaf(v[x].y, 0.f, fmaf(v[x].z, 0.f, fmaf(v[x].w, 0.f, z))));
         if (!__any(z != 0.f)) return false;
 #pragma unroll
         for (int x = 0; x < 8; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                v[0][x][i] = fabsf(v[0][x][i]) < INFINITY ? v[0][x][i] : 0.f;
+                v[x][i] = fabsf(v[x][i]) < INFINITY ? v[x][i] : 0.f;
         return true;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g)
@@ -234,10 +233,9 @@ template <> struct Ops<float> {
 };
 
 template <> struct Ops<_Float16> {
-    static constexpr int TILE = 32;
     half8 qh[4], ql[4]; // row lane % 16, dims 32 j + 8 g ..
-    half8 k[2][4];      // position 16 u + lane % 16, the same dims
-    half8 v[2][4];      // position 16 u + 4 g + e, dims 8 (lane % 16) ..
+    half8 k[4];         // position lane % 16, the same dims
+    half8 v[4];         // position 4 g + e, dims 8 (lane % 16) ..
     float qscale;
     // q = 2^e (high + low): the row's power of two brings its largest value
     // to [1, 2), inside f16's range whatever the queries' size, and the low
@@ -274,35 +272,35 @@ template <> struct Ops<_Float16> {
             }
     }
     template <bool ONCE>
-    __device__ __forceinline__ void load_k(int u, const _Float16 *head, int kpos, int g)
+    __device__ __forceinline__ void load_k(const _Float16 *head, int kpos, int g)
     {
         const unsigned o = kpos * KV_D + 8 * g;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[u][j] = cached<half8, ONCE>(head, o + 32 * j);
+        for (int j = 0; j < 4; ++j) k[j] = cached<half8, ONCE>(head, o + 32 * j);
     }
     template <bool ONCE>
-    __device__ __forceinline__ void load_v(int u, const _Float16 *head, const int (&vpos)[4], int c)
+    __device__ __forceinline__ void load_v(const _Float16 *head, const int (&vpos)[4], int c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            v[u][e] = cached<half8, ONCE>(head, vpos[e] * KV_D + 8 * c);
+            v[e] = cached<half8, ONCE>(head, vpos[e] * KV_D + 8 * c);
     }
-    __device__ __forceinline__ f32x4 scores(int u) const
+    __device__ __forceinline__ f32x4 scores() const
     {
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            a = mfma_f16(k[u][j], qh[j], a);
-            b = mfma_f16(k[u][j], ql[j], b);
+            a = mfma_f16(k[j], qh[j], a);
+            b = mfma_f16(k[j], ql[j], b);
         }
         return (a + b) * qscale;
     }
-    __device__ __forceinline__ void pv(int u, const f32x4 &p, f32x4 (&acc)[8]) const
+    __device__ __forceinline__ void pv(const f32x4 &p, f32x4 (&acc)[8]) const
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) acc[x] = mfma_f32((float)v[u][e][x], p[e], acc[x]);
+            for (int x = 0; x < 8; ++x) acc[x] = mfma_f32((float)v[e][x], p[e], acc[x]);
             // (keeps the widened values of later positions out of registers)
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -311,22 +309,18 @@ template <> struct Ops<_Float16> {
     {
         half8 z = {}; // (a sum of v * 0)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z += v[u][e] * (_Float16)0.f;
+        for (int e = 0; e < 4; ++e) z += v[e] * (_Float16)0.f;
         const u32x4 w = __builtin_bit_cast(u32x4, z); // (a NaN, or zeros of any sign)
         if (!__any(((w[0] | w[1] | w[2] | w[3]) & 0x7fff7fffu) != 0)) return false;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) { // (two f16 of exponent all ones or not)
-                    u32x4 w = __builtin_bit_cast(u32x4, v[u][e]);
-                    w[x] = (w[x] & 0x7c00u) == 0x7c00u ? w[x] & 0xffff0000u : w[x];
-                    w[x] = (w[x] & 0x7c000000u) == 0x7c000000u ? w[x] & 0x0000ffffu : w[x];
-                    v[u][e] = __builtin_bit_cast(half8, w);
-                }
+            for (int x = 0; x < 4; ++x) { // (two f16 of exponent all ones or not)
+                u32x4 w = __builtin_bit_cast(u32x4, v[e]);
+                w[x] = (w[x] & 0x7c00u) == 0x7c00u ? w[x] & 0xffff0000u : w[x];
+                w[x] = (w[x] & 0x7c000000u) == 0x7c000000u ? w[x] & 0x0000ffffu : w[x];
+                v[e] = __builtin_bit_cast(half8, w);
+            }
         return true;
     }
     static __device__ __forceinline__ int dim(int x, int e, int g) { return 32 * g + 8 * e + x; }
@@ -347,14 +341,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     PagedKv kv, int few_rows, int max_workers, RowsScratch rs, const float *__restrict__ q,
     int part_rows, float *__restrict__ part, int2 *__restrict__ shared, float *__restrict__ out)
 {
-    constexpr int TILE = Ops<T>::TILE, SUB = TILE / 16;
     extern __shared__ long long before[]; // [seqs + 1]
     __shared__ long long wsum[4];
     if (blockIdx.x * FEW_WAVES >= max_workers) { // one more workgroup: the tile form's plan
         rows_plan(kv, few_rows, rs, (int *)before);
         return;
     }
-    const FewPlan plan = few_plan(kv, few_rows, TILE, max_workers, before, wsum);
+    const FewPlan plan = few_plan(kv, few_rows, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be; few workers lie on many CUs: two
     // slots of 1100 positions took 1.5 us longer with four to a workgroup)
@@ -382,7 +375,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         while (before[s + 1] <= at) ++s; // slots without tiles
         s = __builtin_amdgcn_readfirstlane(s); // (what comes from LDS, known to be uniform)
         const SlotRows sr = slot_rows(kv, s);
-        const int tiles = slot_tiles(sr, TILE);
+        const int tiles = slot_tiles(sr);
         const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
         const int kh = in / tiles, t0 = in % tiles;
         const int t1 = __builtin_amdgcn_readfirstlane(
@@ -421,23 +414,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         auto head_of = [&](int page) {
             return (const T *)kv.pages + (size_t)max(page, 0) * psize + (size_t)kh * hsize;
         };
-        auto load_k = [&](auto once, int p0, const int (&page)[SUB]) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                const int p = p0 + 16 * u;
-                ops.template load_k<once.value>(
-                    u, head_of(page[u]), (p & pmask) + max(min(c, sr.len - 1 - p), 0), g);
-            }
+        auto load_k = [&](auto once, int p, int page) {
+            ops.template load_k<once.value>(
+                head_of(page), (p & pmask) + max(min(c, sr.len - 1 - p), 0), g);
         };
-        auto load_v = [&](auto once, int p0, const int (&page)[SUB]) {
+        auto load_v = [&](auto once, int p, int page) {
+            int vp[4];
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                const int p = p0 + 16 * u, lim = sr.len - 1 - p;
-                int vp[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) vp[e] = (p & pmask) + max(min(4 * g + e, lim), 0);
-                ops.template load_v<once.value>(u, head_of(page[u]) + hsize * kv.kvh, vp, c);
-            }
+            for (int e = 0; e < 4; ++e)
+                vp[e] = (p & pmask) + max(min(4 * g + e, sr.len - 1 - p), 0);
+            ops.template load_v<once.value>(head_of(page) + hsize * kv.kvh, vp, c);
         };
         // Whether the range begins in a page that neither neighbouring slot names
         // at this place: beams of one prompt share their pages, and find them in
@@ -446,9 +432,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         const int at0 = min((t0 * TILE) >> kv.shift, kv.stride - 1);
         const int mine = entries[at0], below = s ? entries[at0 - kv.stride] : -1,
                   above = s + 1 < kv.seqs ? entries[at0 + kv.stride] : -1;
-        int page[SUB], next[SUB];
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) page[u] = page_of(t0 * TILE + 16 * u);
+        int page = page_of(t0 * TILE);
         const bool alone =
             __builtin_amdgcn_readfirstlane(mine != below && mine != above) != 0;
         bool odd = false;
@@ -457,21 +441,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
             load_v(once, t0 * TILE, page);
             for (int t = t0; t < t1; ++t) {
                 const int p0 = t * TILE, pn = min(t + 1, t1 - 1) * TILE;
-                f32x4 sv[SUB];
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) sv[u] = ops.scores(u);
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) next[u] = page_of(pn + 16 * u);
+                f32x4 sv = ops.scores();
+                const int next = page_of(pn);
                 load_k(once, pn, next);
                 float mx = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool see = p0 + 16 * u + 4 * g + e <= sees && page[u] >= 0;
-                        sv[u][e] = see ? sv[u][e] * sc : -INFINITY;
-                        mx = fmaxf(mx, sv[u][e]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const bool see = p0 + 4 * g + e <= sees && page >= 0;
+                    sv[e] = see ? sv[e] * sc : -INFINITY;
+                    mx = fmaxf(mx, sv[e]);
+                }
                 mx = wave::max_halves(wave::max_rows2(mx));
                 const float mn = fmaxf(m, mx);
                 // a row that has seen nothing yet keeps zero weights
@@ -479,12 +458,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
                 const float corr = __builtin_amdgcn_exp2f(m - base);
                 float rs = 0.f;
 #pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sv[u][e] = __builtin_amdgcn_exp2f(sv[u][e] - base);
-                        rs += sv[u][e];
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    sv[e] = __builtin_amdgcn_exp2f(sv[e] - base);
+                    rs += sv[e];
+                }
                 if (__any(mn != m)) {
 #pragma unroll
                     for (int x = 0; x < 8; ++x) acc[x] *= corr;
@@ -494,15 +471,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
                 m = mn;
                 // a step that some row does not see whole: a value that is not finite
                 // must not reach the rows that do not see it (0 * inf), see below
-                bool whole = p0 + TILE - 1 <= first;
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) whole = whole && page[u] >= 0;
-                if (!whole) odd |= ops.clean();
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) ops.pv(u, sv[u], acc);
+                if (p0 + TILE - 1 > first || page < 0) odd |= ops.clean();
+                ops.pv(sv, acc);
                 load_v(once, pn, next);
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) page[u] = next[u];
+                page = next;
             }
         };
         if (alone) stream(std::true_type{});
@@ -511,10 +483,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
             // the values left out of the steps above, for the rows that see
             // them: whatever its weight, such a value makes the sum not finite
             for (int p = t0 * TILE; p < min(t1 * TILE, sr.len); ++p) {
-                const int id = page_of(p & ~15), pt = p / TILE * TILE;
-                bool whole = pt + TILE - 1 <= first;
-                for (int u = 0; u < SUB; ++u) whole = whole && page_of(pt + 16 * u) >= 0;
-                if (whole || id < 0 || p > sees) continue;
+                const int id = page_of(p & ~15);
+                if ((p | 15) <= first || id < 0 || p > sees) continue;
                 const T *vr = head_of(id) + hsize * kv.kvh + (p & pmask) * KV_D;
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
