@@ -30,8 +30,8 @@
 //
 // Bound by memory, and for few positions by the loads that wait for each other
 // (starts and lengths, table, keys) and the merge's launch. With the merge: 64
-// slots of up to 8192 positions, 32 heads over 8, f16 pages, 149 us for 848 MB
-// (5.7 TB/s); four of up to 60001, 16 over 4, f32 pages, 105 us for 642 MB (6.1);
+// slots of up to 8192 positions, 32 heads over 8, f16 pages, 143 us for 848 MB
+// (5.9 TB/s; with 32 positions a step 149, with 64 153); four of up to 60001, 16 over 4, f32 pages, 105 us for 642 MB (6.1);
 // two of up to 1100, 11.8 us, of which the merge's launch takes 4.0.
 #include <hip/hip_runtime.h>
 
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         // Whether the range begins in a page that neither neighbouring slot names
         // at this place: beams of one prompt share their pages, and find them in
         // the caches. Read as such and as read once, us for 64 slots of up to 8192
-        // positions: 167 and 147 alone, 131 and 152 in fours that share.
+        // positions: 167 and 147 where none share, 131 and 152 where fours do.
         const int at0 = min((t0 * TILE) >> kv.shift, kv.stride - 1);
         const int mine = entries[at0], below = s ? entries[at0 - kv.stride] : -1,
                   above = s + 1 < kv.seqs ? entries[at0 + kv.stride] : -1;
@@ -664,8 +664,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_ro
 
 // Workers: a wave on each SIMD for f32 pages, two for f16 pages, whose steps
 // have twice the products for each byte (64 sessions of up to 8192 positions in
-// f16 pages: 162 us with 1024, 149 with 2048; four of up to 60001 in f32 pages:
-// 106 and 113). Numbers between leave SIMDs unequal: 190 and 146 with 1280.
+// f16 pages: 184 us with 1024, 143 with 2048, 149 with 3072; four of up to 60001
+// in f32 pages: 105 with 1024, 113 with 2048). Numbers between leave SIMDs
+// unequal: 165 with 1536 in f16 pages, 146 with 1280 in f32 ones.
 int few_workers(bool f16) { return f16 ? 2048 : 1024; }
 
 } // namespace
