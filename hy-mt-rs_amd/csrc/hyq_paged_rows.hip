@@ -103,6 +103,10 @@ __device__ __forceinline__ half4 read_transposed(const _Float16 *p)
                    (__attribute__((address_space(3))) short4v *)const_cast<_Float16 *>(p)));
 }
 
+// Whether f16 parts hold a value: from 65520 on the high one would be infinite.
+// (Any finite f16 does.)
+__device__ __forceinline__ bool has_parts(float x) { return fabsf(x) < 65520.f; }
+
 // A step's keys and values on their way from memory to LDS: 512 threads, rows
 // of 16 bytes a lane.
 template <class T> struct Raw;
@@ -114,17 +118,20 @@ template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
     static __device__ __forceinline__ int row(int t) { return t >> 5; }
     static __device__ __forceinline__ int group(int, int i) { return i; } // its 16 rows
     static __device__ __forceinline__ int dim(int t) { return 4 * (t & 31); }
-    // whether a value is not finite; such values become zero
-    __device__ __forceinline__ bool clean()
+    // values of rows that nobody sees become zero, and those of no f16 parts;
+    // whether there were any of the latter in the other rows
+    __device__ __forceinline__ bool clean(const bool (&unseen)[N])
     {
         bool odd = false;
-        auto one = [&](float &x) {
-            const bool fine = fabsf(x) < INFINITY;
-            odd |= !fine;
-            x = fine ? x : 0.f;
-        };
 #pragma unroll
-        for (int i = 0; i < N; ++i) one(v[i].x), one(v[i].y), one(v[i].z), one(v[i].w);
+        for (int i = 0; i < N; ++i) {
+            auto one = [&](float &x) {
+                const bool fine = has_parts(x);
+                odd |= !fine && !unseen[i];
+                x = fine && !unseen[i] ? x : 0.f;
+            };
+            one(v[i].x), one(v[i].y), one(v[i].z), one(v[i].w);
+        }
         return odd;
     }
     static __device__ __forceinline__ void put(_Float16 *hi, _Float16 *lo, const float4 &x)
@@ -144,16 +151,16 @@ template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
     static __device__ __forceinline__ int row(int t) { return t >> 4; }
     static __device__ __forceinline__ int group(int wave, int i) { return 2 * i + (wave >> 2); }
     static __device__ __forceinline__ int dim(int t) { return 8 * (t & 15); }
-    __device__ __forceinline__ bool clean()
+    __device__ __forceinline__ bool clean(const bool (&unseen)[N])
     {
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const bool fine = fabsf((float)v[i][e]) < INFINITY;
-                odd |= !fine;
-                v[i][e] = fine ? v[i][e] : (_Float16)0.f;
+                const bool fine = has_parts((float)v[i][e]);
+                odd |= !fine && !unseen[i];
+                v[i][e] = fine && !unseen[i] ? v[i][e] : (_Float16)0.f;
             }
         return odd;
     }
@@ -204,20 +211,26 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         const int tok0 = piece.index * tq;
         const int first = piece.first; // position of the slot's first new row
         const int toks = min(tq, piece.n - tok0);
-        const int p_end = min(piece.t1 * PR_TILE, first + tok0 + toks);
+        const int seen_end = first + tok0 + toks; // one past the last position that a row sees
+        const int p_end = min(piece.t1 * PR_TILE, seen_end);
         const int p_begin = piece.t0 * PR_TILE;
         const int all_see = first + tok0; // the last position that every row sees
 
         // The pages of a step's four 16-position groups (or the step's one), -1 where
         // none. Page ids come 64 at a time, one per lane. Rows past the end are
         // loaded too, from the same page or, where there is none, from the pool's
-        // first: their weights are zero, and values that are not finite are cleared.
+        // first: their weights are zero, and their values, whatever lies there,
+        // are cleared.
         const int *entries = kv.table + (size_t)s * kv.stride;
         int have = -64, ids = -1; // lane i: the slot's page have + i
         constexpr int GROUPS = WHOLE ? 1 : 4;
         struct Pages {
             int e[GROUPS];
             __device__ __forceinline__ int of(int group) const { return e[WHOLE ? 0 : group]; }
+            __device__ __forceinline__ int at(int g) const // (no index that is not constant)
+            {
+                return g == 0 ? of(0) : g == 1 ? of(1) : g == 2 ? of(2) : of(3);
+            }
             __device__ __forceinline__ bool missing() const
             {
                 int all = e[0];
@@ -254,9 +267,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             } else {
 #pragma unroll
                 for (int i = 0; i < R::N; ++i) {
-                    const int g = R::group(wave, i), e = g == 0 ? pg.of(0) : g == 1 ? pg.of(1)
-                                                        : g == 2   ? pg.of(2)
-                                                                   : pg.of(3);
+                    const int g = R::group(wave, i), e = pg.at(g);
                     // (a uniform base, and an offset that never changes)
                     const T *b = (const T *)kv.pages + (size_t)max(e, 0) * psize +
                                  (size_t)kh * hsize + (size_t)((p0 + 16 * g) & pmask) * KV_D;
@@ -278,6 +289,15 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         // whether some row sees a step in part
         auto partial = [&](int p0, const Pages &pg) {
             return p0 + PR_TILE - 1 > all_see || pg.missing();
+        };
+        // `raw` of such a step, cleaned: its rows behind the last one that a query
+        // sees, or without a page, may hold anything
+        auto clean = [&](int p0, const Pages &pg) {
+            bool unseen[R::N];
+#pragma unroll
+            for (int i = 0; i < R::N; ++i)
+                unseen[i] = p0 + R::row(t) + R::STEP * i >= seen_end || pg.at(R::group(wave, i)) < 0;
+            return raw.clean(unseen);
         };
 
         Pages cur = pages_of(p_begin), next = pages_of(p_begin + PR_TILE);
@@ -340,9 +360,10 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
         float m_run = -INFINITY, l_run = 0.f;
 
-        // A step that some row sees in part: values of it that are not finite must
-        // not reach the rows that do not see them (0 * inf), see below.
-        bool odd = partial(p_begin, cur) && raw.clean();
+        // A step that some row sees in part: values of it that are not finite, or
+        // would not be as f16 parts, must not reach the rows that do not see them
+        // (0 * inf), see below.
+        bool odd = partial(p_begin, cur) && clean(p_begin, cur);
 #pragma unroll
         for (int n = 0; n < 2 * R::N; ++n) store(0, n);
         load(p_begin + PR_TILE, next);
@@ -354,7 +375,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             const RowsLds<LO> &l = lds.step[buf];
             const int p = p0 + o, pa = part_of ? cur.of(2) : cur.of(0),
                       pb = part_of ? cur.of(3) : cur.of(1);
-            if (partial(p0 + PR_TILE, next)) odd |= raw.clean();
+            if (partial(p0 + PR_TILE, next)) odd |= clean(p0 + PR_TILE, next);
             // (sx: the products with low parts, where those are scaled)
             f32x16 sv, sx;
 #pragma unroll
@@ -477,7 +498,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         }
         if (__syncthreads_or(odd)) {
             // the values left out, for the rows that see them: whatever its weight,
-            // such a value makes the sum not finite
+            // such a value makes the sum not finite (as it does in a step that all
+            // rows see whole)
             for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
                 const Pages pg = pages_of(p0);
                 if (!partial(p0, pg)) continue;
@@ -493,7 +515,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
                         for (int x = 0; x < 16; ++x) {
                             const float v = (float)vb[32 * j + 8 * (x >> 2) + 4 * h + (x & 3)];
-                            acc[j][x] += fabsf(v) < INFINITY ? 0.f : v;
+                            acc[j][x] += has_parts(v) ? 0.f : v * INFINITY;
                         }
                         asm volatile("" ::: "memory"); // (few loads at once: a rare path)
                     }

@@ -168,6 +168,60 @@ def test_pages_that_are_not_there(gpu_ctx, hyq, f16):
     assert np.all(got[b.start[1]:b.start[2]] == 0) and np.all(got[b.start[3]:b.start[4]] == 0)
 
 
+def fill_unused(b, what):
+    """Another content than NaN for every place of the pool that no position
+    uses, page 0 (which is read where a slot has no page) among them."""
+    spare = np.setdiff1d(np.arange(b.pages), b.table)[0]
+    b.table[b.table == 0] = spare
+    b.pool[[0, spare]] = b.pool[[spare, 0]]
+    assert np.isnan(b.pool[0]).all()
+    holes = np.isnan(b.pool)
+    if what == "bits":
+        kind = np.uint16 if b.f16 else np.uint32
+        b.pool[holes] = b.rng.integers(0, np.iinfo(kind).max, holes.sum(), kind, True).view(
+            b.pool.dtype)
+    else:
+        b.pool[holes] = what
+
+
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("what", ["bits", np.inf, -np.inf, 65504.0, 65520.0, -1e5, 3e38], ids=str)
+@pytest.mark.parametrize("pt", [16, 32, 64, 256])
+def test_places_that_nobody_wrote(gpu_ctx, hyq, pt, what, f16):
+    """The rest of a slot's last page and a missing page's places hold anything,
+    finite numbers past f16's range among them: nothing of it reaches a row."""
+    if f16 and what not in ("bits", np.inf, -np.inf, 65504.0):
+        what = np.float16(np.sign(what) * 65504)
+    news = [1, 3, 40, 130, 33, 1]
+    lens = [70, 3, 110, 140, 600, 65]
+    b = R.Batch(lens, news, 8, 2, pt, f16, seed=31 + pt, tail=1)
+    fill_unused(b, what)
+    with np.errstate(invalid="ignore"):  # (bits that are signalling NaNs)
+        check(b, attention(hyq, gpu_ctx, b))
+    if pt < 256:
+        b.table[2, 1], b.table[4, 2], b.table[4, -2], b.table[0, 0] = -1, b.pages, -1, -9
+    b.table[5, 0] = -1
+    with np.errstate(invalid="ignore"):
+        check(b, attention(hyq, gpu_ctx, b))
+
+
+@pytest.mark.parametrize("news", [3, 40])
+@pytest.mark.parametrize("what", [65520.0, -3e38], ids=str)
+def test_values_past_f16_stay_unseen(gpu_ctx, hyq, news, what):
+    """A new token's finite value beyond what f16 parts hold reaches the rows
+    that see it and no other."""
+    b = R.Batch([70 + news], [news], 4, 1, 64, False, seed=32)
+    clean, tol = b.attention()
+    at = 70 + news - 2  # seen by the last two rows alone
+    b.pool[b.table[0, at // 64], 1, 0, at % 64, 5] = what
+    got = attention(hyq, gpu_ctx, b)
+    assert np.all(np.abs(got[:news - 2] - clean[:news - 2]).max(-1) <= tol[:news - 2])
+    seen = got[news - 2:, :, 5]
+    assert np.all((np.abs(seen) > 1) | ~np.isfinite(seen))
+    keep = np.arange(D) != 5
+    assert np.all(np.abs(got - clean)[..., keep].max(-1) <= tol)
+
+
 def test_starts_and_lengths_out_of_range(gpu_ctx, hyq):
     """Wrong starts and lengths make wrong rows but stay inside the buffers;
     slots that they leave right are right."""
