@@ -31,6 +31,15 @@ __device__ __forceinline__ SlotRows slot_rows(const PagedKv &kv, int s)
     return r;
 }
 
+// The power of two that a row of queries whose largest is mx is divided by
+// before it is split into f16 parts. Not below 2^-100, whose inverse, and that of
+// 2^-113, is still a number: scores of such queries and f16 keys stay below 2^-76,
+// which no weight feels.
+__device__ __forceinline__ int query_exponent(float mx)
+{
+    return mx > 0.f && mx < INFINITY ? max(ilogbf(mx), -100) : 0;
+}
+
 // A vector at a uniform base and an unsigned 32-bit element offset (a scalar
 // base with a vector offset in the load: no 64-bit address per lane).
 template <class V, class T> __device__ __forceinline__ V at(const T *base, unsigned off)

@@ -256,8 +256,7 @@ template <> struct Ops<_Float16> {
             }
         }
         mx = wave::max_halves(wave::max_rows2(mx));
-        int e = 0;
-        if (mx > 0.f && mx < INFINITY) e = ilogbf(mx);
+        const int e = query_exponent(mx);
         qscale = ldexpf(1.f, e);
         const float inv = ldexpf(1.f, -e);
 #pragma unroll

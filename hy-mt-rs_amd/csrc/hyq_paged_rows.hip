@@ -333,7 +333,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)),
                                      fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
             mx = wave::max_halves(mx);
-            const int e = (mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0) - (LO ? 0 : 13);
+            const int e = query_exponent(mx) - (LO ? 0 : 13);
             qscale = ldexpf(sc, e);
             const float inv = ok ? ldexpf(1.f, -e) : 0.f;
 #pragma unroll

@@ -264,6 +264,19 @@ def test_queries_of_any_size(gpu_ctx, hyq, f16):
             assert np.all(np.abs(got - want).max(-1) <= tol)
 
 
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("power", [-99, -100, -101, -113, -115, -126, -128, -140, -149])
+def test_tiny_queries(gpu_ctx, hyq, power, f16):
+    """Queries down to the smallest f32, zeros among their dims: every score is
+    zero, the output the mean of the values seen, in both forms."""
+    b = R.Batch([100, 60, 9], [1, 40, 3], 4, 1, 16, f16, seed=33)
+    b.q = np.ldexp(np.clip(np.round(b.q * 2), -4, 4) / 4, power).astype(np.float32)
+    if power == -149:
+        b.q[:] = np.where(b.q > 0, np.float32(2.0 ** -149), 0)
+    assert (b.q != 0).any(-1).all() and (b.q == 0).any(-1).all()
+    check(b, attention(hyq, gpu_ctx, b))
+
+
 @pytest.mark.parametrize("scale", [2.0 ** -10, 2.0 ** -13, 2.0 ** 10])
 @pytest.mark.parametrize("news", [2, 40])
 def test_values_of_any_size(gpu_ctx, hyq, news, scale):
