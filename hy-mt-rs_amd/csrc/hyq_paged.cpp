@@ -307,6 +307,7 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
         rs.parts = (float *)(base + l.parts);
         rs.tq = PR_ROWS / (kv.heads / kv.kvh);
         rs.cap = max_blocks(kv.seqs, kv.rows, rs.tq);
+        rs.most = max_rows;
     }
     int rc = launch_paged_few(kv, few, rs, q, part, out, stream);
     if (rc == 0 && rs.cap) rc = launch_paged_rows(kv, rs, q, out, stream);

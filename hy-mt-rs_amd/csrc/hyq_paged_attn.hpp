@@ -99,6 +99,7 @@ struct RowsScratch {
     int *groups; // a workgroup's first piece; one more entry than groups
     float *parts;
     int tq, cap; // tokens of a block, blocks there is room for (0: no tile form)
+    int most;    // new rows of a slot at most; those of more are not computed
 };
 struct RowsLayout {
     size_t blocks, pieces, groups, parts, bytes;
@@ -161,7 +162,7 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
         int nb = 0, before;
         if (b + t < kv.seqs) {
             const SlotRows r = slot_rows(kv, b + t);
-            nb = r.n > few_rows ? (r.n + tq - 1) / tq : 0;
+            nb = r.n > few_rows && r.n <= rs.most ? (r.n + tq - 1) / tq : 0;
         }
         const int all = scan256(nb, before, wsum);
         if (b + t < kv.seqs) first[b + t] = count + before;

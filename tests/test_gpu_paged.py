@@ -250,6 +250,21 @@ def test_rows_past_the_promise_are_left(gpu_ctx, hyq):
         assert np.all(np.abs(got[r] - want[r]).max(-1) <= tol[r])
 
 
+@pytest.mark.parametrize("most", [20, 33])
+def test_prompts_past_the_promise_are_left(gpu_ctx, hyq, most):
+    """The same where max_rows admits prompts."""
+    b = R.Batch([40, 90, 60, 50], [1, 40, 20, 34], 4, 1, 16, True, seed=34, tail=2)
+    want, tol = b.attention()
+    got = attention(hyq, gpu_ctx, b, max_rows=most)
+    for s in range(4):
+        r = slice(b.start[s], b.start[s + 1])
+        if b.news[s] > most:
+            assert np.all(got[r] == -7)
+        else:
+            assert np.all(np.abs(got[r] - want[r]).max(-1) <= tol[r])
+    assert np.all(got[b.new:] == -7)
+
+
 @pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
 def test_queries_of_any_size(gpu_ctx, hyq, f16):
     """Large and small queries, beyond what f16 holds: scores far apart, and
