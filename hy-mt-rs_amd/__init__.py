@@ -127,6 +127,7 @@ SIGNATURES = {
     "hyq_pages_fork_d": (I, [P, P, P, P, P, P, P, P, P]),
     "hyq_pages_scratch_bytes": (SZ, [P]),
     "hyq_pages_extend_d": (I, [P, P, P, P, P, P, P, P, P, P, P, P, SZ]),
+    "hyq_pages_extend_served_d": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, SZ]),
     "hyq_pages_compact_d": (I, [P, P, P, P, P, P, P, P, P, SZ]),
     "hyq_sample_scratch_bytes": (SZ, [SZ, SZ]),
     "hyq_sample_d": (I, [P, P, SZ, SZ, P, P, P, P, P, P, SZ, P, P]),
@@ -727,6 +728,8 @@ class PagedCache:
         self._other = (ctx.empty((seqs, self.layout.stride), np.int32),
                        ctx.empty(seqs, np.int32))
         self._ints = [ctx.empty(seqs, np.int32) for _ in range(3)]
+        self._served = ctx.empty(seqs, np.int32)
+        self._rows_len = self.len  # the lengths that append and attention go by
         self._live = ctx.empty(1, np.int32)
         self._scratch = ctx.empty(lib().hyq_pages_scratch_bytes(self._kl), np.uint8)
         self._attention = []
@@ -748,14 +751,19 @@ class PagedCache:
             self.len.ptr, table.ptr, length.ptr, self.refs.ptr))
         self._other = (self.table, self.len)
         self.table, self.len = table, length
+        self._rows_len = self.len
 
     def extend(self, add) -> np.ndarray:
-        """hyq_pages_extend_d: room for add[s] more tokens; the slots' status
-        (0 done, 1 no pages left, 2 too long for the slot)."""
-        check(lib().hyq_pages_extend_d(
+        """hyq_pages_extend_served_d: room for add[s] more tokens; the slots'
+        status (0 done, 1 no pages left, 2 too long for the slot). Until the next
+        fork or extend, rows of a slot that was refused write nothing and give
+        zeros."""
+        check(lib().hyq_pages_extend_served_d(
             self.ctx.handle, self._kl, self.pool.ptr, self._slots(add, self._ints[0]),
             self.table.ptr, self.len.ptr, self.refs.ptr, self.table.ptr, self.len.ptr,
-            self.refs.ptr, self._ints[2].ptr, self._scratch.ptr, self._scratch.nbytes))
+            self.refs.ptr, self._ints[2].ptr, self._served.ptr, self._scratch.ptr,
+            self._scratch.nbytes))
+        self._rows_len = self._served
         return self._ints[2].numpy()
 
     def compact(self) -> int:
@@ -774,8 +782,8 @@ class PagedCache:
                  norm_first: bool = False) -> None:
         """hyq_paged_rope_norm_append_d on device buffers."""
         check(lib().hyq_paged_rope_norm_append_d(
-            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr, self.len.ptr,
-            start_d, rows, heads, q_d, k_d, v_d, q_norm_d, k_norm_d, freq_d, eps,
+            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
+            self._rows_len.ptr, start_d, rows, heads, q_d, k_d, v_d, q_norm_d, k_norm_d, freq_d, eps,
             int(norm_first), q_out_d))
 
     def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,
@@ -790,8 +798,8 @@ class PagedCache:
             self._attention.append(self.ctx.empty(max(need, 2 * have, 16), np.uint8))
         scratch = self._attention[-1]
         check(lib().hyq_paged_attention_d(
-            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr, self.len.ptr,
-            start_d, rows, max_rows, heads, q_d, scratch.ptr, scratch.nbytes, out_d))
+            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
+            self._rows_len.ptr, start_d, rows, max_rows, heads, q_d, scratch.ptr, scratch.nbytes, out_d))
 
 
 def sample(ctx: "Context", logits: np.ndarray, random, temperature=1.0, top_k=0, top_p=1.0,

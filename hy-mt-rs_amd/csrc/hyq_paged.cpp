@@ -103,6 +103,36 @@ bool grid_ok(const hyq_kv_layout *kl, size_t rows, size_t heads)
     return merge_groups(kl->seqs, kl->kv_heads, paged_few_rows(rep) * rep, cap) < (1 << 24);
 }
 
+// (served_len_d: null where the caller wants none)
+int extend(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, const int32_t *add_d,
+           const int32_t *table_d, const int32_t *len_d, const int32_t *refs_d,
+           int32_t *table_out_d, int32_t *len_out_d, int32_t *refs_out_d, int32_t *status_d,
+           int32_t *served_len_d, void *scratch_d, size_t scratch_bytes)
+{
+    int rc = check_layout(ctx, kl, "pages_extend");
+    if (rc) return rc;
+    if (!pool_d || !add_d || !table_d || !len_d || !refs_d || !table_out_d || !len_out_d ||
+        !refs_out_d || !status_d || !scratch_d)
+        return fail(HYQ_EINVAL, "pages_extend: null argument");
+    for (const int32_t *other : {add_d, table_d, len_d, refs_d, (const int32_t *)table_out_d,
+                                 (const int32_t *)len_out_d, (const int32_t *)refs_out_d,
+                                 (const int32_t *)status_d})
+        if (other == served_len_d)
+            return fail(HYQ_EINVAL, "pages_extend: the served lengths must be an array of their "
+                                    "own");
+    if (!aligned(pool_d) || !aligned(scratch_d))
+        return fail(HYQ_EINVAL, "pages_extend: a buffer is not 16-byte aligned");
+    if (scratch_bytes < hyq_pages_scratch_bytes(kl))
+        return fail(HYQ_EINVAL, "pages_extend: scratch of %zu bytes, %zu needed", scratch_bytes,
+                    hyq_pages_scratch_bytes(kl));
+    DeviceGuard g(ctx->device);
+    HYQ_LAUNCH(launch_pages_extend(pages_args(kl), pool_d, add_d, table_d, len_d, refs_d,
+                                   table_out_d, len_out_d, refs_out_d, status_d, served_len_d,
+                                   scratch_d, ctx->stream),
+               "pages_extend");
+    return HYQ_OK;
+}
+
 } // namespace
 
 extern "C" {
@@ -207,22 +237,19 @@ int hyq_pages_extend_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, cons
                        int32_t *table_out_d, int32_t *len_out_d, int32_t *refs_out_d,
                        int32_t *status_d, void *scratch_d, size_t scratch_bytes)
 {
-    int rc = check_layout(ctx, kl, "pages_extend");
-    if (rc) return rc;
-    if (!pool_d || !add_d || !table_d || !len_d || !refs_d || !table_out_d || !len_out_d ||
-        !refs_out_d || !status_d || !scratch_d)
-        return fail(HYQ_EINVAL, "pages_extend: null argument");
-    if (!aligned(pool_d) || !aligned(scratch_d))
-        return fail(HYQ_EINVAL, "pages_extend: a buffer is not 16-byte aligned");
-    if (scratch_bytes < hyq_pages_scratch_bytes(kl))
-        return fail(HYQ_EINVAL, "pages_extend: scratch of %zu bytes, %zu needed", scratch_bytes,
-                    hyq_pages_scratch_bytes(kl));
-    DeviceGuard g(ctx->device);
-    HYQ_LAUNCH(launch_pages_extend(pages_args(kl), pool_d, add_d, table_d, len_d, refs_d,
-                                   table_out_d, len_out_d, refs_out_d, status_d, scratch_d,
-                                   ctx->stream),
-               "pages_extend");
-    return HYQ_OK;
+    return extend(ctx, kl, pool_d, add_d, table_d, len_d, refs_d, table_out_d, len_out_d,
+                  refs_out_d, status_d, nullptr, scratch_d, scratch_bytes);
+}
+
+int hyq_pages_extend_served_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
+                              const int32_t *add_d, const int32_t *table_d, const int32_t *len_d,
+                              const int32_t *refs_d, int32_t *table_out_d, int32_t *len_out_d,
+                              int32_t *refs_out_d, int32_t *status_d, int32_t *served_len_d,
+                              void *scratch_d, size_t scratch_bytes)
+{
+    if (!served_len_d) return fail(HYQ_EINVAL, "pages_extend: null argument");
+    return extend(ctx, kl, pool_d, add_d, table_d, len_d, refs_d, table_out_d, len_out_d,
+                  refs_out_d, status_d, served_len_d, scratch_d, scratch_bytes);
 }
 
 int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,

@@ -40,9 +40,10 @@ struct PagesArgs {
 size_t pages_scratch(int npages, int seqs);
 int launch_pages_fork(const PagesArgs &a, const int *parent, const int *keep, const int *table,
                       const int *len, int *table_out, int *len_out, int *refs_out, void *stream);
+// (served: the lengths of the slots that were served, 0 for the others, or null)
 int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const int *table,
                         const int *len, const int *refs, int *table_out, int *len_out,
-                        int *refs_out, int *status, void *scratch, void *stream);
+                        int *refs_out, int *status, int *served, void *scratch, void *stream);
 int launch_pages_compact(const PagesArgs &a, void *pool, const int *table, const int *refs,
                          int *table_out, int *refs_out, int *live, void *scratch, void *stream);
 

@@ -189,7 +189,8 @@ __device__ __forceinline__ Ask ask_of(const PagesArgs &a, const int *add, const 
 // pages last.
 __global__ __launch_bounds__(1024) void pages_extend_kernel(
     PagesArgs a, const int *__restrict__ add, const int *table, const int *len, const int *refs,
-    int *table_out, int *len_out, int *refs_out, int *__restrict__ status, void *scratch)
+    int *table_out, int *len_out, int *refs_out, int *__restrict__ status,
+    int *__restrict__ served_len, void *scratch)
 {
     __shared__ int wsum[16];
     const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
@@ -290,7 +291,9 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(
                 n += add[s];
             }
             len_out[s] = n;
-            status[s] = k.is_long ? 2 : k.asks && !served ? 1 : 0;
+            const int refused = k.is_long ? 2 : k.asks && !served ? 1 : 0;
+            status[s] = refused;
+            if (served_len) served_len[s] = refused ? 0 : n;
         }
         carry = min(carry + all, a.npages + 1);
         ncopies += call;
@@ -305,7 +308,8 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(
 // for 8 slots and 260 pages).
 __global__ __launch_bounds__(1024) void pages_extend_small_kernel(
     PagesArgs a, const int *__restrict__ add, const int *table, const int *len, const int *refs,
-    int *table_out, int *len_out, int *refs_out, int *__restrict__ status, void *scratch)
+    int *table_out, int *len_out, int *refs_out, int *__restrict__ status,
+    int *__restrict__ served_len, void *scratch)
 {
     extern __shared__ int lds[];
     __shared__ int wsum[16];
@@ -375,7 +379,9 @@ __global__ __launch_bounds__(1024) void pages_extend_small_kernel(
             n += add[s];
         }
         len_out[s] = n;
-        status[s] = k.is_long ? 2 : k.asks && !served ? 1 : 0;
+        const int refused = k.is_long ? 2 : k.asks && !served ? 1 : 0;
+        status[s] = refused;
+        if (served_len) served_len[s] = refused ? 0 : n;
     }
     if (t == 0) w.count[0] = ncopies;
     __syncthreads();
@@ -517,17 +523,17 @@ int launch_pages_fork(const PagesArgs &a, const int *parent, const int *keep, co
 
 int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const int *table,
                         const int *len, const int *refs, int *table_out, int *len_out,
-                        int *refs_out, int *status, void *scratch, void *stream)
+                        int *refs_out, int *status, int *served, void *scratch, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
     // (a table that is copied as well: by one workgroup while it is small)
     if (a.npages <= SMALL_PAGES && a.seqs <= SMALL_SLOTS)
         hipLaunchKernelGGL(pages_extend_small_kernel, dim3(1), dim3(1024), (size_t)a.npages * 12,
                            st, a, add, table, len, refs, table_out, len_out, refs_out, status,
-                           scratch);
+                           served, scratch);
     else
         hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len,
-                           refs, table_out, len_out, refs_out, status, scratch);
+                           refs, table_out, len_out, refs_out, status, served, scratch);
     hipLaunchKernelGGL(pages_fill_kernel, dim3(512), dim3(256), 0, st, a, (char *)pool, scratch);
     return (int)hipGetLastError();
 }

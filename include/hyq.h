@@ -437,12 +437,22 @@ int hyq_pages_fork_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *paren
  * when all slots that name it do: the one that holds most of it, the first of
  * those. status[s]: 0, or 1 when the pool has too few free pages for slot s
  * and those before it, or 2 when the slot's table row is too short; such a
- * slot stays as it is. Each *_out may be its input. */
+ * slot stays as it is, and new rows given to it would be written over its last
+ * positions, in a page that others may share. Each *_out may be its input. */
 size_t hyq_pages_scratch_bytes(const hyq_kv_layout *kl);
 int hyq_pages_extend_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, const int32_t *add_d,
                        const int32_t *table_d, const int32_t *len_d, const int32_t *refs_d,
                        int32_t *table_out_d, int32_t *len_out_d, int32_t *refs_out_d,
                        int32_t *status_d, void *scratch_d, size_t scratch_bytes);
+/* The same, and served_len[s] = the new length of a slot of status 0, 0 for the
+ * others: the append and the attention of the step take it for len, so that a
+ * refused slot's rows write nothing and give zeros without the host's looking
+ * at status (in a captured step, say). It must not be one of the other arrays. */
+int hyq_pages_extend_served_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
+                              const int32_t *add_d, const int32_t *table_d, const int32_t *len_d,
+                              const int32_t *refs_d, int32_t *table_out_d, int32_t *len_out_d,
+                              int32_t *refs_out_d, int32_t *status_d, int32_t *served_len_d,
+                              void *scratch_d, size_t scratch_bytes);
 /* Moves the pages in use to the ids 0 .. live-1, so that a smaller pool can
  * take their place: those with ids from `live` on go to the free ids below, in
  * order, in every layer. *live_d = their number. Each *_out may be its

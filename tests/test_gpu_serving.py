@@ -149,6 +149,61 @@ def test_steps_against_the_plain_forms(gpu_ctx, hyq):
             assert got[6][r] == want and abs(got[7][r] - pw) <= 4 * R.U
 
 
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("pages", [3, 4200])
+@pytest.mark.parametrize("chunk", [1, 7])
+def test_refused_slots_write_nothing(gpu_ctx, hyq, chunk, pages, f16):
+    """Beams of one prompt, and a slot at its table's end, in a pool that runs
+    out: the new rows of those that extend refuses (of one of them in a page that
+    a served beam goes on writing) change no cached row and attend nothing; the
+    others' are as if they were alone. (4200 pages: the large form of extend,
+    whose other pages a slot of its own holds.)"""
+    seqs, stride = 6, max(4, pages - 3)
+    c = hyq.PagedCache(gpu_ctx, 1, KVH, pages, seqs, stride * PT, PT,
+                       hyq.F16 if f16 else hyq.F32)
+    r = np.random.default_rng(chunk)
+    f = lambda *n: r.normal(0, 1, n).astype(np.float32)
+    pool0 = f(pages, 2, KVH, PT, D).astype(np.float16 if f16 else np.float32)
+    c.pool.copy_from(np.frombuffer(pool0.tobytes(), np.uint8))
+    hoard = (pages - 3) * PT
+    assert c.extend([5, 0, 0, 0, hoard, 0]).tolist() == [0] * 6
+    c.fork([0, 0, 0, 0, 4, -1])
+    held = c.lengths()
+    add = [chunk] * 4 + [stride * PT + 1 - hoard, 0]
+    news = np.array([chunk] * 5 + [0], np.int32)
+    status = c.extend(add)
+    assert status.tolist() == [0, 0, 0, 1, 2, 0]
+    start = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    rows = int(start[-1])
+    q, k, v = f(rows, HEADS, D), f(rows, KVH, D), f(rows, KVH, D)
+    w, freq = f(D), (10000.0 ** (-np.arange(64) / 64)).astype(np.float32)
+    a = [gpu_ctx.array(x) for x in (start, q, k, v, w, freq)]
+    qo, out = (gpu_ctx.array(np.full((rows, HEADS, D), -7, np.float32)) for _ in range(2))
+    c.append_d(0, a[0].ptr, rows, HEADS, a[1].ptr, a[2].ptr, a[3].ptr, a[4].ptr, a[4].ptr,
+               a[5].ptr, 1e-5, qo.ptr)
+    c.attention_d(0, a[0].ptr, rows, chunk, HEADS, qo.ptr, out.ptr)
+    got = np.frombuffer(c.pool.numpy().tobytes(), pool0.dtype).reshape(pool0.shape)
+    table, lens = c.table.numpy(), c.lengths()
+    assert np.array_equal(lens, held + np.where(status == 0, add, 0))
+    # what is written: the served slots' new positions, nothing else
+    fresh = np.zeros(pool0.shape, bool)
+    for s in range(3):
+        for p in range(lens[s] - chunk, lens[s]):
+            fresh[table[s, p // PT], :, :, p % PT] = True
+    kept = pool0.copy()  # (the beams' shared positions, copied)
+    for s in range(3):
+        kept[table[s, 0], :, :, :5] = pool0[table[3, 0], :, :, :5]
+    assert np.array_equal(got[~fresh], kept[~fresh])
+    b = R.Batch([1] * seqs, [1] * seqs, HEADS, KVH, PT, f16, 0)
+    b.table, b.lens, b.news, b.start = table, np.where(status == 0, lens, 0), news, start
+    b.pool, b.pages, b.width, b.rows = got, pages, stride, rows
+    b.q = qo.numpy()
+    want, tol = b.attention()
+    o = out.numpy()
+    assert np.all(np.abs(o - want).max(-1) <= tol)
+    assert np.all(o[3 * chunk:] == 0)
+
+
 def hip(name):
     """The HIP runtime that libhyq.so uses."""
     lib = ctypes.CDLL("libamdhip64.so")

@@ -122,6 +122,27 @@ def test_shapes_and_scratch_are_refused(hyq, L, ctx):
     assert L.hyq_paged_attention_scratch_bytes(kl, 1, 1, 6) == 0
 
 
+def test_served_lengths_are_refused(hyq, L, ctx):
+    """hyq_pages_extend_served_d: hyq_pages_extend_d's refusals, and served
+    lengths that are null or one of the other arrays."""
+    layout_ = layout(hyq)
+    kl, p = ctypes.byref(layout_), 4096
+    good = [ctx, kl, p, p, p, p, p, p, p, p, p, p + 64, p, 1 << 40]
+    call = L.hyq_pages_extend_served_d
+    for i in range(13):
+        assert call(*[None if j == i else a for j, a in enumerate(good)]) == hyq.EINVAL, i
+        assert b"null" in L.hyq_last_error()
+    for i in range(3, 11):
+        assert call(*[p + 64 if j == i else a for j, a in enumerate(good)]) == hyq.EINVAL, i
+        assert b"own" in L.hyq_last_error()
+    for i in (2, 12):
+        assert call(*[a + 4 if j == i else a for j, a in enumerate(good)]) == hyq.EINVAL, i
+        assert b"aligned" in L.hyq_last_error()
+    assert call(*good[:-1], L.hyq_pages_scratch_bytes(kl) - 1) == hyq.EINVAL
+    bad = layout(hyq, dtype=8)
+    assert call(ctx, ctypes.byref(bad), *good[2:]) == hyq.EDTYPE
+
+
 def test_sample_refusals(hyq, L, ctx):
     p, big = 4096, 1 << 40
     good = [ctx, p, 2, 100, p, p, p, p, p, p, big, p, p]
