@@ -182,6 +182,18 @@ __device__ __forceinline__ Ask ask_of(const PagesArgs &a, const int *add, const 
     return k;
 }
 
+// The tables and counts that the plan writes elsewhere, by many workgroups.
+__global__ __launch_bounds__(256) void pages_copy_kernel(const int *__restrict__ table,
+                                                         int *__restrict__ table_out,
+                                                         size_t entries,
+                                                         const int *__restrict__ refs,
+                                                         int *__restrict__ refs_out, int npages)
+{
+    const size_t first = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256;
+    for (size_t i = first; i < entries; i += step) table_out[i] = table[i];
+    for (size_t i = first; i < (size_t)npages; i += step) refs_out[i] = refs[i];
+}
+
 // One workgroup of 1024 threads. A slot's partly filled last page that others
 // name too is copied for it, unless all who name the page extend it in this
 // call and the slot holds most of it (the first of those): that one goes on
@@ -242,13 +254,8 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(
         if (is && found + before < total) w.free[found + before] = p;
         found += all;
     }
-    __threadfence();
-    __syncthreads();
-    if (table_out != table)
-        for (size_t i = t; i < (size_t)a.seqs * a.stride; i += 1024) table_out[i] = table[i];
-    // (the counts in `refs` are not read again: where refs_out is refs they change now)
-    if (refs_out != refs)
-        for (int i = t; i < a.npages; i += 1024) refs_out[i] = refs[i];
+    // (the counts in `refs` are not read again: where refs_out is refs they change
+    // now, elsewhere the launch before has copied them, and the table)
     __threadfence();
     __syncthreads();
     int carry = 0, ncopies = 0;
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(1024) void pages_extend_kernel(
 __global__ __launch_bounds__(1024) void pages_extend_small_kernel(
     PagesArgs a, const int *__restrict__ add, const int *table, const int *len, const int *refs,
     int *table_out, int *len_out, int *refs_out, int *__restrict__ status,
-    int *__restrict__ served_len, void *scratch)
+    int *__restrict__ served_len, void *scratch, int copy)
 {
     extern __shared__ int lds[];
     __shared__ int wsum[16];
@@ -335,7 +342,7 @@ __global__ __launch_bounds__(1024) void pages_extend_small_kernel(
             asks[EACH * t + i] = 0;
             top[EACH * t + i] = 0;
         }
-    if (table_out != table)
+    if (copy)
         for (int i = t; i < a.seqs * a.stride; i += 1024) table_out[i] = table[i];
     __syncthreads();
     const bool shared = k.partial && lrefs[k.last] > 1;
@@ -526,11 +533,24 @@ int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const in
                         int *refs_out, int *status, int *served, void *scratch, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
-    // (a table that is copied as well: by one workgroup while it is small)
-    if (a.npages <= SMALL_PAGES && a.seqs <= SMALL_SLOTS)
+    // A table that goes elsewhere is copied by the one workgroup while it is small,
+    // by a launch of its own beyond (16384 entries 9.0 and 9.2 us, 32768 11.1 and
+    // 9.8, 2^20 293 and 10.9; 128 slots of 512 entries over 50,000 pages, with their
+    // counts, 36.6 and 19.2).
+    const size_t entries = (size_t)a.seqs * a.stride;
+    const bool small = a.npages <= SMALL_PAGES && a.seqs <= SMALL_SLOTS;
+    const bool copy = small && table_out != table && entries <= SMALL_ENTRIES;
+    const size_t nt = table_out != table && !copy ? entries : 0;
+    const int nr = refs_out != refs && !small ? a.npages : 0;
+    if (nt || nr) {
+        const size_t groups = (std::max(nt, (size_t)nr) + 255) / 256;
+        hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)std::min(groups, (size_t)1024)),
+                           dim3(256), 0, st, table, table_out, nt, refs, refs_out, nr);
+    }
+    if (small)
         hipLaunchKernelGGL(pages_extend_small_kernel, dim3(1), dim3(1024), (size_t)a.npages * 12,
                            st, a, add, table, len, refs, table_out, len_out, refs_out, status,
-                           served, scratch);
+                           served, scratch, (int)copy);
     else
         hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(1024), 0, st, a, add, table, len,
                            refs, table_out, len_out, refs_out, status, served, scratch);
