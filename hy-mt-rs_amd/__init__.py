@@ -707,10 +707,14 @@ class PagedCache:
 
     A serving step: ``fork`` (beams, ended requests), ``extend`` (room for the
     new tokens), then for every layer ``append_d`` and ``attention_d`` of the
-    packed rows. The calls are asynchronous on the context's stream; those that
-    return numpy arrays wait. ``table`` and ``len`` alternate between two buffers
-    with every ``fork``, and a captured graph keeps those of its capture: capture
-    an even number of forks, or none and replay after an even number."""
+    packed rows. ``fork``, ``extend`` and ``compact`` take and return host values
+    and wait for the context's stream. The calls whose names end in _d take device
+    buffers, are only enqueued and can be captured in a graph: ``fork_d``,
+    ``extend_d`` (the statuses stay in ``status``), ``append_d``, ``attention_d``.
+    A fork leaves ``table`` and ``len`` in a second pair of buffers, the extension
+    after it (or a second fork) brings them back, and a captured graph keeps the
+    buffers of its capture: capture every fork with its extension, and replay after
+    an extension, not between it and a fork."""
 
     def __init__(self, ctx: Context, layers: int, kv_heads: int, pages: int, seqs: int,
                  context: int, page_tokens: int = 64, dtype: int = F16, head_dim: int = 128):
@@ -727,7 +731,9 @@ class PagedCache:
         self.refs = ctx.array(np.zeros(pages, np.int32))
         self._other = (ctx.empty((seqs, self.layout.stride), np.int32),
                        ctx.empty(seqs, np.int32))
-        self._ints = [ctx.empty(seqs, np.int32) for _ in range(3)]
+        self._home = (self.table, self.len)
+        self._ints = [ctx.empty(seqs, np.int32) for _ in range(2)]
+        self.status = ctx.array(np.zeros(seqs, np.int32))
         self._served = ctx.empty(seqs, np.int32)
         self._rows_len = self.len  # the lengths that append and attention go by
         self._live = ctx.empty(1, np.int32)
@@ -742,29 +748,38 @@ class PagedCache:
         return into.ptr
 
     def fork(self, parent, keep=None) -> None:
-        """hyq_pages_fork_d: slot s becomes (the first keep[s] positions of)
-        slot parent[s]; -1 frees it."""
+        """Slot s becomes (the first keep[s] positions of) slot parent[s]; -1
+        frees it."""
+        self.fork_d(self._slots(parent, self._ints[0]),
+                    None if keep is None else self._slots(keep, self._ints[1]))
+
+    def fork_d(self, parent_d: int, keep_d: int | None = None) -> None:
+        """hyq_pages_fork_d on device buffers."""
         table, length = self._other
-        check(lib().hyq_pages_fork_d(
-            self.ctx.handle, self._kl, self._slots(parent, self._ints[0]),
-            None if keep is None else self._slots(keep, self._ints[1]), self.table.ptr,
-            self.len.ptr, table.ptr, length.ptr, self.refs.ptr))
+        check(lib().hyq_pages_fork_d(self.ctx.handle, self._kl, parent_d, keep_d, self.table.ptr,
+                                     self.len.ptr, table.ptr, length.ptr, self.refs.ptr))
         self._other = (self.table, self.len)
         self.table, self.len = table, length
         self._rows_len = self.len
 
     def extend(self, add) -> np.ndarray:
-        """hyq_pages_extend_served_d: room for add[s] more tokens; the slots'
-        status (0 done, 1 no pages left, 2 too long for the slot). Until the next
-        fork or extend, rows of a slot that was refused write nothing and give
-        zeros."""
+        """Room for add[s] more tokens; the slots' status (0 done, 1 no pages
+        left, 2 too long for the slot). Until the next fork or extension, rows of
+        a slot that was refused write nothing and give zeros."""
+        self.extend_d(self._slots(add, self._ints[0]))
+        return self.status.numpy()
+
+    def extend_d(self, add_d: int) -> None:
+        """hyq_pages_extend_served_d on a device buffer; see ``status``."""
+        table, length = self._home
         check(lib().hyq_pages_extend_served_d(
-            self.ctx.handle, self._kl, self.pool.ptr, self._slots(add, self._ints[0]),
-            self.table.ptr, self.len.ptr, self.refs.ptr, self.table.ptr, self.len.ptr,
-            self.refs.ptr, self._ints[2].ptr, self._served.ptr, self._scratch.ptr,
-            self._scratch.nbytes))
+            self.ctx.handle, self._kl, self.pool.ptr, add_d, self.table.ptr, self.len.ptr,
+            self.refs.ptr, table.ptr, length.ptr, self.refs.ptr, self.status.ptr,
+            self._served.ptr, self._scratch.ptr, self._scratch.nbytes))
+        if self.table is not table:
+            self._other = (self.table, self.len)
+            self.table, self.len = table, length
         self._rows_len = self._served
-        return self._ints[2].numpy()
 
     def compact(self) -> int:
         """hyq_pages_compact_d: the pages in use become 0 .. live-1; live."""
@@ -805,7 +820,9 @@ class PagedCache:
 def sample(ctx: "Context", logits: np.ndarray, random, temperature=1.0, top_k=0, top_p=1.0,
            min_p=0.0):
     """hyq_sample_d of logits [rows][vocab]; settings are values for all rows
-    or arrays of one per row. Returns (tokens int32, probabilities f32)."""
+    or arrays of one per row. Returns (tokens int32, probabilities f32).
+    (All of it from and to host arrays, with buffers of its own; a serving loop
+    whose logits are on the device calls hyq_sample_d.)"""
     logits = np.ascontiguousarray(logits, np.float32)
     rows, vocab = logits.shape
     each = lambda v, t: ctx.array(np.ascontiguousarray(np.broadcast_to(np.asarray(v, t), (rows,))))

@@ -302,6 +302,65 @@ def test_a_captured_ragged_batch(gpu_ctx, hyq, f16):
     ok(hip("hipGraphDestroy")(graph))
 
 
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "f16"])
+def test_a_captured_step_of_the_cache_class(gpu_ctx, hyq, f16):
+    """PagedCache's step of one fork, extension, append and attention in a graph,
+    replayed for other forks, refused slots among them, with eager calls between:
+    every replay gives the eager step's bits."""
+    ctx = gpu_ctx
+    r = np.random.default_rng(8)
+    f = lambda *n: ctx.array(r.normal(0, 1, n).astype(np.float32))
+    q, k, v, w, freq = f(SEQS, HEADS, D), f(SEQS, KVH, D), f(SEQS, KVH, D), f(D), f(64)
+    start = ctx.array(np.arange(SEQS + 1, dtype=np.int32))
+    parent, add = ctx.empty(SEQS, np.int32), ctx.empty(SEQS, np.int32)
+    qo, out = f(SEQS, HEADS, D), f(SEQS, HEADS, D)
+    pool0 = r.normal(0, 1, (30, 2, KVH, PT, D)).astype(np.float16 if f16 else np.float32)
+
+    def cache():
+        c = hyq.PagedCache(ctx, 1, KVH, 30, SEQS, STRIDE * PT, PT, hyq.F16 if f16 else hyq.F32)
+        c.pool.copy_from(np.frombuffer(pool0.tobytes(), np.uint8))
+        assert not c.extend([17, 32, 1, 0, 47]).any()
+        return c
+
+    def step(c):
+        c.fork_d(parent.ptr)
+        c.extend_d(add.ptr)
+        c.append_d(0, start.ptr, SEQS, HEADS, q.ptr, k.ptr, v.ptr, w.ptr, w.ptr, freq.ptr, 1e-5,
+                   qo.ptr)
+        c.attention_d(0, start.ptr, SEQS, 1, HEADS, qo.ptr, out.ptr)
+
+    eager, graphed = cache(), cache()
+    parent.copy_from(np.arange(SEQS, dtype=np.int32))
+    add.copy_from(np.zeros(SEQS, np.int32))
+    step(graphed)  # (its attention's scratch)
+    step(eager)
+    for c in (eager, graphed):
+        c.pool.copy_from(np.frombuffer(pool0.tobytes(), np.uint8))
+    graph, run = captured(ctx, lambda: step(graphed))
+    seen = set()
+    long = (np.arange(SEQS), [1, STRIDE * PT + 1, 1, 1, 1])  # (no slot has that much room)
+    for i, (p, a) in enumerate([INPUTS[i % len(INPUTS)] for i in range(12)] + [long, long]):
+        got = []
+        for c, call in ((eager, lambda: step(eager)),
+                        (graphed, lambda: ok(hip("hipGraphLaunch")(run, ctypes.c_void_p(ctx.stream))))):
+            if i == 6:  # (a slot freed between, by the calls that wait)
+                c.fork([0, 1, -1, 3, 4])
+                assert not c.extend([0, 0, 3, 0, 0]).any()
+            parent.copy_from(np.array(p, np.int32))
+            add.copy_from(np.array(a, np.int32))
+            out.copy_from(np.full((SEQS, HEADS, D), -7, np.float32))
+            call()
+            got.append([x.numpy() for x in (c.table, c.len, c.refs, c.status, c.pool, qo, out)])
+        for x, y in zip(*got):
+            assert np.array_equal(x, y), i
+        refused = got[0][3] != 0
+        seen |= set(got[0][3].tolist())
+        assert not got[0][6][refused].any() and (got[0][6][~refused] != -7).all()
+    assert seen >= {0, 2}
+    ok(hip("hipGraphExecDestroy")(run))
+    ok(hip("hipGraphDestroy")(graph))
+
+
 def test_two_contexts_at_once(gpu_ctx, hyq):
     """Steps enqueued on two contexts (streams) in turn, each with buffers of
     its own, give what one alone gives."""
