@@ -72,7 +72,7 @@ struct Piece {
     int begin, n, first; // the slot's rows, and the first one's position
 };
 struct Plan {
-    int blocks, groups, unused[2];
+    int blocks, groups;
 };
 
 // Pieces that fill the GPU with kvh workgroups each (at least one).
@@ -279,7 +279,7 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
     if (t == 0) {
         const int groups = shares ? divide(tiles + least - 1, least) : npieces;
         rs.groups[groups] = npieces;
-        *rs.plan = Plan{count, groups, {0, 0}};
+        *rs.plan = Plan{count, groups};
     }
 }
 

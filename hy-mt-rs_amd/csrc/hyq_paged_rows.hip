@@ -177,8 +177,8 @@ template <bool LO> struct RowsLds { // one step
 
 // WHOLE: a step lies in one page (of 64 tokens or more), so that it takes one
 // look at the table and one base address instead of four of each, whose scalar
-// work was a sixth of a wave's time (512 tokens over 32012 positions: 404 -> 380
-// us in f32 pages, 272 -> 245 in f16).
+// work was a sixth of a wave's time (512 tokens over 32012 positions, pages of 16
+// and of 64 tokens: 406 and 394 us in f32 pages, 268 and 250 in f16).
 template <class T, bool WHOLE>
 __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     PagedKv kv, RowsScratch rs, const float *__restrict__ q, float *__restrict__ out)
@@ -308,8 +308,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         const bool ok = tl < toks;
         const int head = kh * rep + r % rep;
         const int sees = ok ? first + tok0 + tl : -1; // its last visible position
-        // the last position the wave's last row sees, and its first row
-        const int wave_last = first + tok0 + min(toks - 1, (32 * rows + 31) / rep);
+        // the last position that the wave's first row sees, and with it all of them
         const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
         const size_t row = (size_t)(piece.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
 
@@ -382,8 +381,9 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             for (int e = 0; e < 16; ++e) sv[e] = sx[e] = 0.f;
             // Scores, with the next step's rows converted between their products (the
             // matrix unit takes 32 cycles for each). Operands are read one product
-            // ahead, and no further: the barriers to the compiler's scheduling keep
-            // the kernel inside its registers.
+            // ahead, and no further, by barriers to the compiler's scheduling: 512
+            // tokens over 32012 positions take 394 us with them and 397 without in f32
+            // pages, 250 either way in f16 ones.
             half8 ahi[2], alo[2];
             auto keys = [&](int kk) {
                 ahi[kk & 1] = *reinterpret_cast<const half8 *>(&l.khi[o + c][16 * kk + 8 * h]);
