@@ -178,7 +178,7 @@ template <bool LO> struct RowsLds { // one step
 // WHOLE: a step lies in one page (of 64 tokens or more), so that it takes one
 // look at the table and one base address instead of four of each, whose scalar
 // work was a sixth of a wave's time (512 tokens over 32012 positions, pages of 16
-// and of 64 tokens: 406 and 394 us in f32 pages, 268 and 250 in f16).
+// and of 64 tokens: 405 and 394 us in f32 pages, 266 and 249 in f16).
 template <class T, bool WHOLE>
 __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     PagedKv kv, RowsScratch rs, const float *__restrict__ q, float *__restrict__ out)
@@ -295,8 +295,10 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         auto clean = [&](int p0, const Pages &pg) {
             bool unseen[R::N];
 #pragma unroll
-            for (int i = 0; i < R::N; ++i)
-                unseen[i] = p0 + R::row(t) + R::STEP * i >= seen_end || pg.at(R::group(wave, i)) < 0;
+            for (int i = 0; i < R::N; ++i) {
+                const int seen = pg.at(R::group(wave, i)) < 0 ? 0 : seen_end - p0 - R::STEP * i;
+                unseen[i] = R::row(t) >= seen;
+            }
             return raw.clean(unseen);
         };
 
