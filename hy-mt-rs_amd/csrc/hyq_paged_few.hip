@@ -32,7 +32,7 @@
 // (starts and lengths, table, keys) and the merge's launch. With the merge: 64
 // slots of up to 8192 positions, 32 heads over 8, f16 pages, 143 us for 848 MB
 // (5.9 TB/s; with 32 positions a step 149, with 64 153); four of up to 60001, 16 over 4, f32 pages, 105 us for 642 MB (6.1);
-// two of up to 1100, 11.8 us, of which the merge's launch takes 4.0.
+// two of up to 1100, 11.8 us, of which the merge's launch takes 4.4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -31,9 +31,9 @@
 //
 // Bound by a step's matrix products (1.8 us at the rate at which all SIMDs
 // sustain them for f32 pages, 1.2 for f16), its LDS traffic (0.6) and its VALU
-// work, which overlap in part: a step takes 2.9 and 1.85 us. 512 new tokens of
+// work, which overlap in part: a step takes 3.0 and 1.8 us. 512 new tokens of
 // one slot over 2012 positions, 16 heads over 4, f32 pages: 45 us in all, the
-// plan 6, this launch 37 (eight steps, and 10 us to begin and end: cold code and
+// plan 6, this launch 37 (eight steps, and 13 us to begin and end: cold code and
 // loads that wait for each other), the merge 5.
 #include <hip/hip_runtime.h>
 

@@ -7,7 +7,9 @@
 // the host.
 //
 // Where nothing is copied these are launches and dependent loads: a fork and an
-// extension of 8 slots take 10 to 12 us. Copies are bound by memory: 128 beams of
+// extension of 8 slots take 10 to 13 us, of 128 slots over 20,000 to 200,000 pages
+// 33 (the larger forms below). A compaction's plan, by one workgroup, grows with
+// the pool: 8 us for 700 pages, 53 for 20,000, 460 for 200,000. Copies are bound by memory: 128 beams of
 // 32 layers, 4 heads, f16, whose last pages are copied 42 us in all (the copies
 // 31, of rows scattered over a pool of 10 GB), a compaction that reads and writes
 // 1.3 GB 253 us (5.2 TB/s, what a copy reaches).
@@ -74,8 +76,8 @@ __global__ __launch_bounds__(256) void pages_count_kernel(PagesArgs a, const int
 
 // Both by one workgroup, the counts in LDS, where table and pool are small: one
 // launch instead of two. (With the small form of the extension, against the two
-// larger ones: 8 slots 12 and 28 us a step, 128 slots, with their copies, 54 and
-// 73.)
+// larger ones in the same small pool: 8 slots 12 and 28 us a step, 128 slots, with
+// copies that took longer then, 54 and 73.)
 constexpr int SMALL_PAGES = 4096, SMALL_SLOTS = 1024, SMALL_ENTRIES = 16384;
 __global__ __launch_bounds__(1024) void pages_fork_small_kernel(
     PagesArgs a, const int *__restrict__ parent, const int *__restrict__ keep,

@@ -27,7 +27,9 @@
 //           to the runs' sums, finds the run that holds u W and in it the token
 // Where a cut's bin has more members than the list holds (equal logits by the
 // thousand) the last launch does the row by itself, refining its cut bit by bit
-// over the row.
+// over the row: a dozen passes by one workgroup where both cuts fall among ties.
+// Rows of 128167 equal logits with top-p take 1.3 ms, with top-k 50000 as well 2.3
+// (64 of them 1.4 and 2.5); rounded to quarters 0.5 and 0.8.
 //
 // Two rows of 120818 with top-k 20 and top-p are four short launches, 20.7 us (2.6,
 // 4.4, 9.2, 5.6). 64 rows of 128167 with settings of all kinds take 57 us:

@@ -407,8 +407,8 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
  * within the f16 range where a slot has more than 16 * kv_heads / heads new rows
  * (those products split them into two f16 parts: 22 bits of numbers from 2^-14
  * up, 2^-36 absolutely below). A value beyond it there, and one that is not
- * finite in any form, makes its dim of the rows that see it not finite, and
- * changes no other row. What places hold that no position uses (a page's rest,
+ * finite in any form, makes its dim of the rows that see it not finite (such a
+ * key the whole of those rows), and changes no other row. What places hold that no position uses (a page's rest,
  * pages never written) is never part of a result. out_d must not be q_d.
  * scratch_d: hyq_paged_attention_scratch_bytes bytes (0 for arguments that the
  * call refuses). */
@@ -476,7 +476,8 @@ int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
  * plus infinity nothing finite is. Weights are summed exactly to 2^-46 of the
  * largest (2^-62 times the vocabulary, rounded up to a power of two, where
  * that is more): smaller ones count as zero. prob_d (may be null): the token's
- * weight over the kept ones' (1 at temperature <= 0, 0 beside -1). */
+ * weight over the kept ones' (1 at temperature <= 0, 0 beside -1). Scratch: up to
+ * 429 KB a row for up to 32 rows, 58 KB a row from 512 on (3.8 GB at 65535). */
 size_t hyq_sample_scratch_bytes(size_t rows, size_t vocab);
 int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
                  const float *temperature_d, const int32_t *top_k_d, const float *top_p_d,
