@@ -408,10 +408,10 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
  * (those products split them into two f16 parts: 22 bits of numbers from 2^-14
  * up, 2^-36 absolutely below). A value beyond it there, and one that is not
  * finite in any form, makes its dim of the rows that see it not finite (such a
- * key the whole of those rows), and changes no other row. What places hold that no position uses (a page's rest,
- * pages never written) is never part of a result. out_d must not be q_d.
- * scratch_d: hyq_paged_attention_scratch_bytes bytes (0 for arguments that the
- * call refuses). */
+ * key the whole of those rows), and changes no other row. What places hold that
+ * no position uses (a page's rest, pages never written) is never part of a
+ * result. out_d must not be q_d. scratch_d: hyq_paged_attention_scratch_bytes
+ * bytes (0 for arguments that the call refuses). */
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
                                          size_t heads);
 int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, int layer,
