@@ -22,6 +22,8 @@ LIB_PATH = os.path.join(HERE, "libhyq.so")
 F32, F16, Q8_0, Q4_K, Q6_K, Q2_0C, STQ1_0 = 0, 1, 8, 12, 14, 40, 42
 DTYPES = {"F32": F32, "F16": F16, "Q8_0": Q8_0, "Q4_K": Q4_K, "Q6_K": Q6_K,
           "Q2_0C": Q2_0C, "STQ1_0": STQ1_0}
+# Of paged caches alone: a byte for each number, a scale for each 128 (hyq_kv_layout).
+KV_Q8 = 1008
 OK, EINVAL, EDTYPE, EDEVICE, ENOMEM = 0, -1, -2, -3, -4
 
 # Every exported symbol of include/hyq.h with its ctypes signature.
@@ -122,6 +124,7 @@ SIGNATURES = {
     "hyq_kv_pool_bytes": (SZ, [P]),
     "hyq_paged_rope_norm_append_d": (I, [P, P, P, I, P, P, P, SZ, SZ, P, P, P, P, P, P,
                                          ctypes.c_float, I, P]),
+    "hyq_paged_read_d": (I, [P, P, P, I, P, P, P, SZ, P, P]),
     "hyq_paged_attention_scratch_bytes": (SZ, [P, SZ, SZ, SZ]),
     "hyq_paged_attention_d": (I, [P, P, P, I, P, P, P, SZ, SZ, SZ, P, P, SZ, P]),
     "hyq_pages_fork_d": (I, [P, P, P, P, P, P, P, P, P]),
@@ -707,7 +710,8 @@ class PagedCache:
 
     A serving step: ``fork`` (beams, ended requests), ``extend`` (room for the
     new tokens), then for every layer ``append_d`` and ``attention_d`` of the
-    packed rows. ``fork``, ``extend`` and ``compact`` take and return host values
+    packed rows. ``dtype`` KV_Q8 holds a byte for each number and a scale for each
+    128; ``read`` gives them back. ``fork``, ``extend`` and ``compact`` take and return host values
     and wait for the context's stream. The calls whose names end in _d take device
     buffers, are only enqueued and can be captured in a graph: ``fork_d``,
     ``extend_d`` (the statuses stay in ``status``), ``append_d``, ``attention_d``.
@@ -800,6 +804,26 @@ class PagedCache:
             self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
             self._rows_len.ptr, start_d, rows, heads, q_d, k_d, v_d, q_norm_d, k_norm_d, freq_d, eps,
             int(norm_first), q_out_d))
+
+    def read_d(self, layer: int, start_d: int, rows: int, k_d: int, v_d: int) -> None:
+        """hyq_paged_read_d on device buffers."""
+        check(lib().hyq_paged_read_d(self.ctx.handle, self._kl, self.pool.ptr, layer,
+                                     self.table.ptr, self._rows_len.ptr, start_d, rows, k_d, v_d))
+
+    def read(self, layer: int) -> list:
+        """Every slot's cached keys and values in one layer, as the cache holds
+        them: (keys, values) [positions][kv_heads*head_dim] f32, which
+        ``DenseDecoder.load_kv`` takes."""
+        start = np.concatenate([[0], np.cumsum(self.lengths(), dtype=np.int64)])
+        rows, width = int(start[-1]), self.layout.kv_heads * self.layout.head_dim
+        if rows >= 1 << 20:
+            raise ValueError("more than 2^20 positions: read them in parts (read_d)")
+        at = self.ctx.array(start.astype(np.int32))
+        k, v = (self.ctx.empty((max(rows, 1), width), np.float32) for _ in range(2))
+        check(lib().hyq_paged_read_d(self.ctx.handle, self._kl, self.pool.ptr, layer,
+                                     self.table.ptr, self.len.ptr, at.ptr, rows, k.ptr, v.ptr))
+        k, v = k.numpy(), v.numpy()
+        return [(k[a:b], v[a:b]) for a, b in zip(start[:-1], start[1:])]
 
     def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,
                     q_d: int, out_d: int) -> None:

@@ -14,14 +14,24 @@ namespace {
 
 bool aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+int type_of(const hyq_kv_layout *kl)
+{
+    return kl->dtype == HYQ_KV_Q8 ? KV_T_Q8 : kl->dtype == HYQ_F16 ? KV_T_F16 : KV_T_F32;
+}
+
+bool dtype_ok(const hyq_kv_layout *kl)
+{
+    return kl->dtype == HYQ_F32 || kl->dtype == HYQ_F16 || kl->dtype == HYQ_KV_Q8;
+}
+
 size_t page_bytes(const hyq_kv_layout *kl)
 {
-    return (size_t)2 * kl->kv_heads * kl->page_tokens * KV_D * (kl->dtype == HYQ_F16 ? 2 : 4);
+    return (size_t)2 * kl->kv_heads * kl->page_tokens * kv_row_bytes(type_of(kl));
 }
 
 bool layout_ok(const hyq_kv_layout *kl)
 {
-    if (!kl || (kl->dtype != HYQ_F32 && kl->dtype != HYQ_F16)) return false;
+    if (!kl || !dtype_ok(kl)) return false;
     const int pt = kl->page_tokens;
     if (pt < 16 || pt > 256 || (pt & (pt - 1))) return false;
     if (kl->layers < 1 || kl->layers > 65536 || kl->kv_heads < 1 || kl->kv_heads > 256 ||
@@ -36,7 +46,7 @@ int check_layout(hyq_ctx *ctx, const hyq_kv_layout *kl, const char *who)
 {
     if (!ctx) return fail(HYQ_EINVAL, "%s: null context", who);
     if (!kl) return fail(HYQ_EINVAL, "%s: null argument", who);
-    if (kl->dtype != HYQ_F32 && kl->dtype != HYQ_F16)
+    if (!dtype_ok(kl))
         return fail(HYQ_EDTYPE, "%s: pages of type %d", who, kl->dtype);
     if (!layout_ok(kl))
         return fail(HYQ_EINVAL,
@@ -67,7 +77,7 @@ PagedKv view(const hyq_kv_layout *kl, const void *pool, int layer, const int32_t
     v.table = table;
     v.len = len;
     v.start = start;
-    v.f16 = kl->dtype == HYQ_F16;
+    v.type = type_of(kl);
     v.seqs = kl->seqs;
     v.stride = kl->stride;
     v.npages = kl->pages;
@@ -81,7 +91,7 @@ PagedKv view(const hyq_kv_layout *kl, const void *pool, int layer, const int32_t
 PagesArgs pages_args(const hyq_kv_layout *kl)
 {
     PagesArgs a{};
-    a.f16 = kl->dtype == HYQ_F16;
+    a.type = type_of(kl);
     a.layers = kl->layers;
     a.kvh = kl->kv_heads;
     a.shift = shift_of(kl);
@@ -170,13 +180,34 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
     return HYQ_OK;
 }
 
+int hyq_paged_read_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, int layer,
+                     const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
+                     size_t rows, float *k_d, float *v_d)
+{
+    int rc = check_layout(ctx, kl, "paged_read");
+    if (rc) return rc;
+    if (!pool_d || !table_d || !len_d || !start_d || !k_d || !v_d)
+        return fail(HYQ_EINVAL, "paged_read: null argument");
+    if (layer < 0 || layer >= kl->layers)
+        return fail(HYQ_EINVAL, "paged_read: layer %d of %d", layer, kl->layers);
+    if (rows > MAX_ROWS) return fail(HYQ_EINVAL, "paged_read: %zu rows", rows);
+    if (!aligned(pool_d) || !aligned(k_d) || !aligned(v_d))
+        return fail(HYQ_EINVAL, "paged_read: a buffer is not 16-byte aligned");
+    if (k_d == v_d) return fail(HYQ_EINVAL, "paged_read: keys and values to one place");
+    DeviceGuard g(ctx->device);
+    HYQ_LAUNCH(launch_paged_read(view(kl, pool_d, layer, table_d, len_d, start_d, rows, 0), k_d,
+                                 v_d, ctx->stream),
+               "paged_read");
+    return HYQ_OK;
+}
+
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
                                          size_t heads)
 {
     if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0 ||
         !grid_ok(kl, rows, heads))
         return 0;
-    return paged_attention_scratch(kl->dtype == HYQ_F16, kl->seqs, kl->kv_heads, (int)heads,
+    return paged_attention_scratch(type_of(kl), kl->seqs, kl->kv_heads, (int)heads,
                                    (int)rows, (int)std::min(rows, max_rows));
 }
 
@@ -310,10 +341,10 @@ int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
 namespace hyq {
 
 // Scratch: the few-row form's parts, then the tile form's plan and parts.
-size_t paged_attention_scratch(bool f16, int seqs, int kvh, int heads, int rows, int max_rows)
+size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows)
 {
     const int few = std::min(paged_few_rows(heads / kvh), max_rows);
-    size_t n = paged_few_scratch(f16, seqs, kvh, heads, few);
+    size_t n = paged_few_scratch(type, seqs, kvh, heads, few);
     if (max_rows > few) n += rows_layout(seqs, kvh, heads, rows).bytes;
     return n;
 }
@@ -326,7 +357,7 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
     RowsScratch rs{};
     if (max_rows > few) {
         const RowsLayout l = rows_layout(kv.seqs, kv.kvh, kv.heads, kv.rows);
-        char *base = (char *)scratch + paged_few_scratch(kv.f16, kv.seqs, kv.kvh, kv.heads, few);
+        char *base = (char *)scratch + paged_few_scratch(kv.type, kv.seqs, kv.kvh, kv.heads, few);
         rs.plan = (Plan *)base;
         rs.blocks = (Block *)(base + l.blocks);
         rs.pieces = (Piece *)(base + l.pieces);

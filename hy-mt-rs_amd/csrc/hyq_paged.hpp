@@ -12,14 +12,27 @@ constexpr int KV_D = 128;           // head dimension
 constexpr int KV_MAX_SEQS = 4096;   // slots of a page table
 constexpr int KV_MAX_REP = 16;      // query heads per KV head
 
+// Element types of a pool. KV_T_Q8: a byte for each number and an f32 scale for
+// the 128 of a position and head, x = scale * code with codes from -127 to 127;
+// a key's code as a signed byte (an operand of the int8 matrix instructions as
+// it is), a value's as code + 128 (which one fma on f16 pairs turns into a code).
+enum { KV_T_F32 = 0, KV_T_F16 = 1, KV_T_Q8 = 2 };
+// Bytes of one position of a head.
+constexpr int kv_row_bytes(int type)
+{
+    return type == KV_T_Q8 ? KV_D + 4 : type == KV_T_F16 ? KV_D * 2 : KV_D * 4;
+}
+
 // One layer's pages as the kernels read them: page p holds keys
-// [kv_heads][page_tokens][128] and then values of the same shape.
+// [kv_heads][page_tokens][128] and then values of the same shape; with KV_T_Q8
+// behind them the scales [2][kv_heads][page_tokens].
 struct PagedKv {
     const void *pages;  // the layer's first page
     const int *table;   // [seqs][stride] page ids, -1 where none
     const int *len;     // [seqs] positions held, the new rows' among them
     const int *start;   // [seqs + 1] first new row of a slot
-    int f16;            // element type: 0 f32, 1 f16
+    const int *skip;    // [seqs] leading positions that another launch attends, or null
+    int type;           // KV_T_*
     int seqs, stride, npages, shift; // page_tokens == 1 << shift
     int kvh, heads, rows;
 };
@@ -27,15 +40,17 @@ struct PagedKv {
 int launch_paged_append(const PagedKv &kv, const float *q, const float *k, const float *v,
                         const float *qn, const float *kn, const float *freq, float eps,
                         bool norm_first, float *q_out, void *stream);
+// The packed rows' keys and values as f32 rows (kv.heads is not read).
+int launch_paged_read(const PagedKv &kv, float *k, float *v, void *stream);
 
 // Attention: the one-wave form for slots of few new rows and the tile form for
 // the others; scratch as paged_attention_scratch says.
-size_t paged_attention_scratch(bool f16, int seqs, int kvh, int heads, int rows, int max_rows);
+size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows);
 int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void *scratch,
                            float *out, void *stream);
 
 struct PagesArgs {
-    int f16, layers, kvh, shift, npages, seqs, stride;
+    int type, layers, kvh, shift, npages, seqs, stride;
 };
 size_t pages_scratch(int npages, int seqs);
 int launch_pages_fork(const PagesArgs &a, const int *parent, const int *keep, const int *table,

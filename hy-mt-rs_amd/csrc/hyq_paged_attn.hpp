@@ -54,6 +54,113 @@ __device__ __forceinline__ int divide(long long x, int y)
     return x >> 31 ? (int)(x / y) : (int)((unsigned)x / (unsigned)y);
 }
 
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+// Two values' high and low f16 parts, both rounded to nearest: hi, and
+// x - hi (exact in f32) by one mixed-precision fma each.
+// (The low part is taken from the high one as it is: written as a difference, the
+// compiler forms the high part twice, once of an unrounded product, and a value
+// near the middle of two f16 loses its low part.)
+__device__ __forceinline__ void split2(float x, float y, half2 &hi, half2 &lo)
+{
+    hi = __builtin_convertvector((float2v{x, y}), half2);
+    float a, b;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(b)
+        : "v"(hi), "v"(y));
+    lo = __builtin_convertvector((float2v{a, b}), half2);
+}
+
+// ---- the few-row form's plan ----
+constexpr int FEW_WAVES = 4;
+
+// Worker w of `workers` takes `base` tiles, the first `more` workers one more.
+struct FewPlan {
+    long long total;
+    int workers, base, more;
+    __device__ __forceinline__ long long begin(int w) const
+    {
+        return (long long)w * base + min(w, more);
+    }
+    // the worker that takes tile x
+    __device__ __forceinline__ int worker(long long x) const
+    {
+        const long long longer = (long long)more * (base + 1);
+        return x < longer ? divide(x, base + 1) : more + divide(x - longer, base);
+    }
+};
+
+// (new rows over no positions still have their zeros to be written: one tile)
+template <int TILE> __device__ __forceinline__ int slot_tiles(int positions)
+{
+    return max(1, (positions + TILE - 1) / TILE);
+}
+// A slot's leading positions that the few-row form leaves out: whole groups of 16
+// before its new rows.
+template <bool SHARED>
+__device__ __forceinline__ int skipped(const PagedKv &kv, int s, const SlotRows &r)
+{
+    return SHARED ? max(0, min(kv.skip[s], r.len - r.n)) & ~15 : 0;
+}
+template <int TILE, bool SHARED>
+__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows)
+{
+    const SlotRows r = slot_rows(kv, s);
+    return r.n > 0 && r.n <= few_rows ? slot_tiles<TILE>(r.len - skipped<SHARED>(kv, s, r)) : 0;
+}
+
+// before[s], in LDS: the tiles of the slots before s over all KV heads, with
+// the total at before[seqs]. 256 threads. (Every workgroup forms it for itself:
+// a launch before this one would cost more than the few loads and barriers.)
+template <int TILE, bool SHARED>
+__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int max_workers,
+                                            long long *before, long long *wsum)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    long long carry = 0;
+    for (int b = 0; b < kv.seqs; b += 256) {
+        const int s = b + t;
+        const long long mine = s < kv.seqs ? (long long)few_tiles<TILE, SHARED>(kv, s, few_rows) * kv.kvh : 0;
+        long long v = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const long long u = __shfl_up(v, o, 64);
+            if (lane >= o) v += u;
+        }
+        if (lane == 63) wsum[wave] = v;
+        __syncthreads();
+        long long base = carry, all = carry;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) base += wsum[w];
+            all += wsum[w];
+        }
+        if (s < kv.seqs) before[s] = base + v - mine;
+        carry = all;
+        __syncthreads();
+    }
+    if (t == 0) before[kv.seqs] = carry;
+    __syncthreads();
+    FewPlan p;
+    p.total = carry;
+    // (a tile for a worker, while there are fewer tiles than workers: two slots of
+    // 1100 positions in f32 pages 11.8 us, two tiles a worker 13.0)
+    p.workers = (int)min((long long)max_workers, carry);
+    p.base = divide(carry, max(p.workers, 1));
+    p.more = (int)(carry - (long long)p.base * p.workers);
+    return p;
+}
+
+// A vector of the cache: ONCE, of pages that one slot reads, not to be kept in the
+// caches, which the rows and parts of this launch and the next ones are for.
+template <class V, bool ONCE, class T>
+__device__ __forceinline__ V cached(const T *base, unsigned off)
+{
+    const V *p = reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
+                                             (unsigned)(off * sizeof(T)));
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
+
 // ---- the tile form's plan ----
 constexpr int PR_ROWS = 128;        // query rows per workgroup
 constexpr int PR_TILE = 64;         // positions per step
@@ -286,11 +393,16 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)
 // new rows, with the plan where there is a tile form; and the merge of both.
 int paged_few_rows(int rep);
-size_t paged_few_scratch(bool f16, int seqs, int kvh, int heads, int few);
+size_t paged_few_scratch(int type, int seqs, int kvh, int heads, int few);
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
                      float *out, void *stream);
 int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
                        float *out, void *stream);
+// hyq_paged_few_q8.hip: the few-row form of 8-bit pages, as launch_paged_few has
+// laid it out.
+int launch_paged_few_q8(const PagedKv &kv, int few, int workers, const RowsScratch &rs,
+                        const float *q, int part_rows, float *part, int2 *shared, float *out,
+                        void *stream);
 // hyq_paged_rows.hip: the slots of more.
 int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, float *out,
                       void *stream);

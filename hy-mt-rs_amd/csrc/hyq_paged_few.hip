@@ -47,78 +47,9 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float float2v __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int FEW_WAVES = 4;
 constexpr int TILE = 16; // positions of a step
-
-// Worker w of `workers` takes `base` tiles, the first `more` workers one more.
-struct FewPlan {
-    long long total;
-    int workers, base, more;
-    __device__ __forceinline__ long long begin(int w) const
-    {
-        return (long long)w * base + min(w, more);
-    }
-    // the worker that takes tile x
-    __device__ __forceinline__ int worker(long long x) const
-    {
-        const long long longer = (long long)more * (base + 1);
-        return x < longer ? divide(x, base + 1) : more + divide(x - longer, base);
-    }
-};
-
-// (new rows over no positions still have their zeros to be written: one tile)
-__device__ __forceinline__ int slot_tiles(const SlotRows &r)
-{
-    return max(1, (r.len + TILE - 1) / TILE);
-}
-__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows)
-{
-    const SlotRows r = slot_rows(kv, s);
-    return r.n > 0 && r.n <= few_rows ? slot_tiles(r) : 0;
-}
-
-// before[s], in LDS: the tiles of the slots before s over all KV heads, with
-// the total at before[seqs]. 256 threads. (Every workgroup forms it for itself:
-// a launch before this one would cost more than the few loads and barriers.)
-__device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int max_workers,
-                                            long long *before, long long *wsum)
-{
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    long long carry = 0;
-    for (int b = 0; b < kv.seqs; b += 256) {
-        const int s = b + t;
-        const long long mine = s < kv.seqs ? (long long)few_tiles(kv, s, few_rows) * kv.kvh : 0;
-        long long v = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const long long u = __shfl_up(v, o, 64);
-            if (lane >= o) v += u;
-        }
-        if (lane == 63) wsum[wave] = v;
-        __syncthreads();
-        long long base = carry, all = carry;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) base += wsum[w];
-            all += wsum[w];
-        }
-        if (s < kv.seqs) before[s] = base + v - mine;
-        carry = all;
-        __syncthreads();
-    }
-    if (t == 0) before[kv.seqs] = carry;
-    __syncthreads();
-    FewPlan p;
-    p.total = carry;
-    // (a tile for a worker, while there are fewer tiles than workers: two slots of
-    // 1100 positions in f32 pages 11.8 us, two tiles a worker 13.0)
-    p.workers = (int)min((long long)max_workers, carry);
-    p.base = divide(carry, max(p.workers, 1));
-    p.more = (int)(carry - (long long)p.base * p.workers);
-    return p;
-}
 
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, const f32x4 &c)
 {
@@ -127,16 +58,6 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, const f32x4 &c)
 __device__ __forceinline__ f32x4 mfma_f16(const half8 &a, const half8 &b, const f32x4 &c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// A vector of the cache: ONCE, of pages that one slot reads, not to be kept in the
-// caches, which the rows and parts of this launch and the next ones are for.
-template <class V, bool ONCE, class T>
-__device__ __forceinline__ V cached(const T *base, unsigned off)
-{
-    const V *p = reinterpret_cast<const V *>(reinterpret_cast<const char *>(base) +
-                                             (unsigned)(off * sizeof(T)));
-    return ONCE ? __builtin_nontemporal_load(p) : *p;
 }
 
 // The operands of one tile, by element type. Dims of an output element
@@ -335,7 +256,7 @@ template <> struct Ops<_Float16> {
     }
 };
 
-template <class T>
+template <class T, bool SHARED>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
     PagedKv kv, int few_rows, int max_workers, RowsScratch rs, const float *__restrict__ q,
     int part_rows, float *__restrict__ part, int2 *__restrict__ shared, float *__restrict__ out)
@@ -346,7 +267,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         rows_plan(kv, few_rows, rs, (int *)before);
         return;
     }
-    const FewPlan plan = few_plan(kv, few_rows, max_workers, before, wsum);
+    const FewPlan plan = few_plan<TILE, SHARED>(kv, few_rows, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be; few workers lie on many CUs: two
     // slots of 1100 positions took 1.5 us longer with four to a workgroup)
@@ -374,7 +295,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         while (before[s + 1] <= at) ++s; // slots without tiles
         s = __builtin_amdgcn_readfirstlane(s); // (what comes from LDS, known to be uniform)
         const SlotRows sr = slot_rows(kv, s);
-        const int tiles = slot_tiles(sr);
+        const int skip = skipped<SHARED>(kv, s, sr);
+        const int tiles = slot_tiles<TILE>(sr.len - skip);
         const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
         const int kh = in / tiles, t0 = in % tiles;
         const int t1 = __builtin_amdgcn_readfirstlane(
@@ -428,18 +350,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         // at this place: beams of one prompt share their pages, and find them in
         // the caches. Read as such and as read once, us for 64 slots of up to 8192
         // positions: 167 and 147 where none share, 131 and 152 where fours do.
-        const int at0 = min((t0 * TILE) >> kv.shift, kv.stride - 1);
+        const int p_begin = skip + t0 * TILE;
+        const int at0 = min(p_begin >> kv.shift, kv.stride - 1);
         const int mine = entries[at0], below = s ? entries[at0 - kv.stride] : -1,
                   above = s + 1 < kv.seqs ? entries[at0 + kv.stride] : -1;
-        int page = page_of(t0 * TILE);
+        int page = page_of(p_begin);
         const bool alone =
             __builtin_amdgcn_readfirstlane(mine != below && mine != above) != 0;
         bool odd = false;
         auto stream = [&](auto once) {
-            load_k(once, t0 * TILE, page);
-            load_v(once, t0 * TILE, page);
+            load_k(once, p_begin, page);
+            load_v(once, p_begin, page);
             for (int t = t0; t < t1; ++t) {
-                const int p0 = t * TILE, pn = min(t + 1, t1 - 1) * TILE;
+                const int p0 = skip + t * TILE, pn = skip + min(t + 1, t1 - 1) * TILE;
                 f32x4 sv = ops.scores();
                 const int next = page_of(pn);
                 load_k(once, pn, next);
@@ -481,7 +404,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         if (odd) {
             // the values left out of the steps above, for the rows that see
             // them: whatever its weight, such a value makes the sum not finite
-            for (int p = t0 * TILE; p < min(t1 * TILE, sr.len); ++p) {
+            for (int p = p_begin; p < min(skip + t1 * TILE, sr.len); ++p) {
                 const int id = page_of(p & ~15);
                 if ((p | 15) <= first || id < 0 || p > sees) continue;
                 const T *vr = head_of(id) + hsize * kv.kvh + (p & pmask) * KV_D;
@@ -500,7 +423,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
             const int n = t1 == tiles ? 1 : plan.worker(last) - w + 1;
             shared[(size_t)s * kv.kvh + kh] = make_int2(w, n);
         }
-        if (t0 == 0 && t1 == tiles) {
+        if (t0 == 0 && t1 == tiles && skip == 0) {
             // (a row that saw nothing gives zeros)
             if (ok) Ops<T>::put(out + row * KV_D, acc, g, l > 0.f || l != l ? 1.f / l : 0.f);
         } else if (ok) {
@@ -666,7 +589,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_ro
 // f16 pages: 184 us with 1024, 143 with 2048, 149 with 3072; four of up to 60001
 // in f32 pages: 105 with 1024, 113 with 2048). Numbers between leave SIMDs
 // unequal: 165 with 1536 in f16 pages, 146 with 1280 in f32 ones.
-int few_workers(bool f16) { return f16 ? 2048 : 1024; }
+int few_workers(int type) { return type == KV_T_F32 ? 1024 : 2048; }
 
 } // namespace
 
@@ -678,18 +601,18 @@ int paged_few_rows(int rep) { return 16 / rep; }
 
 namespace {
 
-size_t parts_bytes(bool f16, int seqs, int kvh, int part_rows)
+size_t parts_bytes(int type, int seqs, int kvh, int part_rows)
 {
-    return ((size_t)few_workers(f16) + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
+    return ((size_t)few_workers(type) + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
 }
 
 } // namespace
 
 // Parts, then the workers of each slot and KV head.
-size_t paged_few_scratch(bool f16, int seqs, int kvh, int heads, int few)
+size_t paged_few_scratch(int type, int seqs, int kvh, int heads, int few)
 {
     const size_t shared = ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
-    return parts_bytes(f16, seqs, kvh, few * (heads / kvh)) + shared;
+    return parts_bytes(type, seqs, kvh, few * (heads / kvh)) + shared;
 }
 
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
@@ -697,16 +620,17 @@ int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const fl
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
-    int2 *shared = (int2 *)((char *)part + parts_bytes(kv.f16, kv.seqs, kv.kvh, part_rows));
+    int2 *shared = (int2 *)((char *)part + parts_bytes(kv.type, kv.seqs, kv.kvh, part_rows));
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
-    const int workers = few_workers(kv.f16);
+    const int workers = few_workers(kv.type);
     const dim3 grid(workers / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
-    if (kv.f16)
-        hipLaunchKernelGGL(paged_few_kernel<_Float16>, grid, block, lds, st, kv, few, workers, rs, q,
-                           part_rows, part, shared, out);
-    else
-        hipLaunchKernelGGL(paged_few_kernel<float>, grid, block, lds, st, kv, few, workers, rs, q,
-                           part_rows, part, shared, out);
+    if (kv.type == KV_T_Q8)
+        return launch_paged_few_q8(kv, few, workers, rs, q, part_rows, part, shared, out, stream);
+    auto kernel = kv.skip ? paged_few_kernel<float, true> : paged_few_kernel<float, false>;
+    if (kv.type == KV_T_F16)
+        kernel = kv.skip ? paged_few_kernel<_Float16, true> : paged_few_kernel<_Float16, false>;
+    hipLaunchKernelGGL(kernel, grid, block, lds, st, kv, few, workers, rs, q, part_rows, part, shared,
+                       out);
     return (int)hipGetLastError();
 }
 
@@ -716,7 +640,7 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
     const int2 *shared =
-        (const int2 *)((const char *)part + parts_bytes(kv.f16, kv.seqs, kv.kvh, part_rows));
+        (const int2 *)((const char *)part + parts_bytes(kv.type, kv.seqs, kv.kvh, part_rows));
     // Few rows have many parts each (1024 workers over four slots of four KV
     // heads: 64), which all of a workgroup's waves read; many rows have few, and
     // a wave each. Wide and not: four slots of 60001 positions 124 and 134 us,

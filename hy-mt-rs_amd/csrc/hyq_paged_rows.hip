@@ -18,6 +18,12 @@
 // values. f32 pages hold keys and values below 65504, of which those from 2^-14
 // up keep 22 bits.
 //
+// 8-bit pages hold a code for each number, which f16 holds too, and a scale for
+// each position of a head: codes go through both products, the scores are
+// multiplied with the keys' scales, and the weights with the values' before they
+// are split. Those are kept below 2^15 by a power of two above all scales that the
+// row has seen, which the sums are a multiple of.
+//
 // Keys and values go through LDS, two steps of them, rows as they are (values
 // are transposed by ds_read_b64_tr_b16 on their way to the matrix operand).
 // The next step is converted and stored between the products of the present
@@ -38,6 +44,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "hyq_paged_attn.hpp"
 #include "hyq_wave.hpp"
@@ -48,9 +55,9 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int PR_THREADS = 512;     // two waves on each SIMD
 // Row pitches in halves, chosen for the banks: keys are read 16 bytes a lane
@@ -63,19 +70,7 @@ __device__ __forceinline__ f32x16 mfma(const half8 &a, const half8 &b, const f32
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-// Two values' high and low f16 parts, both rounded to nearest: hi, and
-// x - hi (exact in f32) by one mixed-precision fma each.
-__device__ __forceinline__ void split2(float x, float y, half2 &hi, half2 &lo)
-{
-    hi = __builtin_convertvector((float2v{x, y}), half2);
-    float a, b;
-    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi), "v"(x));
-    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-        : "=v"(b)
-        : "v"(hi), "v"(y));
-    lo = __builtin_convertvector((float2v{a, b}), half2);
-}
-// The same with the low parts 2^11 times as large: an operand keeps 22 bits as
+// split2 with the low parts 2^11 times as large: an operand keeps 22 bits as
 // long as its high part is a normal number (from 2^-14 up), where low parts in
 // place would be subnormal below 2^-3. The factor is taken off the scores' sum
 // of such products, and off the weights that values' low parts are multiplied
@@ -170,9 +165,46 @@ template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
     }
 };
 
+template <> struct Raw<unsigned char> { // row t / 8, dims 16 (t % 8) ..
+    static constexpr int N = 1;
+    typedef u32x4 Vec;
+    Vec k[N], v[N];
+    float scale; // waves 0 and 1: of the keys and the values of row t % 64
+    static constexpr int STEP = 64;
+    static __device__ __forceinline__ int row(int t) { return t >> 3; }
+    static __device__ __forceinline__ int group(int wave, int) { return wave >> 1; }
+    static __device__ __forceinline__ int dim(int t) { return 16 * (t & 7); }
+    // (codes are numbers wherever they lie; the scales of rows that nobody sees are
+    // put away as zeros)
+    __device__ __forceinline__ bool clean(const bool (&)[N]) { return false; }
+    // u + 1024 is a byte u under the exponent of 1024
+    static __device__ __forceinline__ void put(_Float16 *hi, const u32x4 &x, unsigned sign)
+    {
+        half8 y[2];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const unsigned u = x[w] ^ sign;
+            const half2 a = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)),
+                        b = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+            const half2 from = {(_Float16)1152.f, (_Float16)1152.f};
+            const half2 c = a - from, d = b - from;
+            y[w >> 1][4 * (w & 1)] = c[0];
+            y[w >> 1][4 * (w & 1) + 1] = c[1];
+            y[w >> 1][4 * (w & 1) + 2] = d[0];
+            y[w >> 1][4 * (w & 1) + 3] = d[1];
+        }
+        *reinterpret_cast<half8 *>(hi) = y[0];
+        *reinterpret_cast<half8 *>(hi + 8) = y[1];
+    }
+};
+
 template <bool LO> struct RowsLds { // one step
     _Float16 khi[PR_TILE][PR_KP], klo[LO ? PR_TILE : 1][PR_KP];
     _Float16 vhi[PR_TILE][PR_VP], vlo[LO ? PR_TILE : 1][PR_VP];
+};
+struct CodesLds {
+    _Float16 khi[PR_TILE][PR_KP], vhi[PR_TILE][PR_VP];
+    float scale[2][PR_TILE]; // of keys, of values
 };
 
 // WHOLE: a step lies in one page (of 64 tokens or more), so that it takes one
@@ -184,10 +216,12 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     PagedKv kv, RowsScratch rs, const float *__restrict__ q, float *__restrict__ out)
 {
     constexpr bool LO = sizeof(T) == 4; // low parts of keys and values
+    constexpr bool Q8 = sizeof(T) == 1; // codes and scales
     typedef Raw<T> R;
+    typedef std::conditional_t<Q8, CodesLds, RowsLds<LO>> Lds;
     constexpr int JOIN = 66; // a lane's words in the join of the two halves
     __shared__ __align__(16) union {
-        RowsLds<LO> step[2];
+        Lds step[2];
         float join[4][JOIN][64];
     } lds;
     // (a group's KV heads in sequence, so that an XCD, which takes every eighth
@@ -204,7 +238,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
         const int part_of = wave >> 2, rows = wave & 3;
         const int rep = kv.heads / kv.kvh;
-        const size_t hsize = (size_t)KV_D << kv.shift, psize = 2 * hsize * kv.kvh;
+        const size_t hsize = (size_t)KV_D << kv.shift;
+        const size_t psize = 2 * kv.kvh * (Q8 ? hsize / KV_D * kv_row_bytes(KV_T_Q8) : hsize);
         const int pmask = (1 << kv.shift) - 1;
         const float sc = 1.4426950408889634f * 0.08838834764831845f; // log2(e) / sqrt(128)
 
@@ -264,6 +299,14 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     raw.k[i] = at<typename R::Vec>(b, o);
                     raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
                 }
+                if constexpr (Q8) {
+                    if (wave < 2)
+                        raw.scale = at<float>(
+                            (const float *)((const T *)kv.pages + (size_t)max(pg.e[0], 0) * psize +
+                                            2 * kv.kvh * hsize) +
+                                ((size_t)(wave * kv.kvh + kh) << kv.shift) + (p0 & pmask),
+                            lane);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < R::N; ++i) {
@@ -275,13 +318,37 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     raw.k[i] = at<typename R::Vec>(b, o);
                     raw.v[i] = at<typename R::Vec>(b + hsize * kv.kvh, o);
                 }
+                if constexpr (Q8) {
+                    if (wave < 2) {
+                        const int g = lane >> 4, e = g == 0   ? pg.at(0)
+                                                     : g == 1 ? pg.at(1)
+                                                     : g == 2 ? pg.at(2)
+                                                              : pg.at(3);
+                        const float *b = (const float *)((const T *)kv.pages +
+                                                         (size_t)max(e, 0) * psize +
+                                                         2 * kv.kvh * hsize) +
+                                         ((size_t)(wave * kv.kvh + kh) << kv.shift);
+                        raw.scale = b[((p0 + 16 * g) & pmask) + (lane & 15)];
+                    }
+                }
             }
         };
-        // one of the 2 N rows of `raw`, converted, to a buffer
-        auto store = [&](int buf, int n) {
-            RowsLds<LO> &l = lds.step[buf];
+        // one of the 2 N rows of `raw`, the step from p0 on, converted, to a buffer
+        auto store = [&](int buf, int n, int p0, const Pages &pg) {
+            Lds &l = lds.step[buf];
             const int d = R::dim(t), r = R::row(t) + R::STEP * (n >> 1);
-            if (n & 1)
+            if constexpr (Q8) {
+                if (n) R::put(&l.vhi[r][d], raw.v[0], 0u);
+                else R::put(&l.khi[r][d], raw.k[0], 0x80808080u);
+                if (n == 0 && wave < 2) {
+                    const int g = lane >> 4, e = WHOLE    ? pg.e[0]
+                                                 : g == 0 ? pg.at(0)
+                                                 : g == 1 ? pg.at(1)
+                                                 : g == 2 ? pg.at(2)
+                                                          : pg.at(3);
+                    l.scale[wave][lane] = lane < seen_end - p0 && e >= 0 ? raw.scale : 0.f;
+                }
+            } else if (n & 1)
                 R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
             else
                 R::put(&l.khi[r][d], &l.klo[LO ? r : 0][LO ? d : 0], raw.k[n >> 1]);
@@ -360,20 +427,21 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
         float m_run = -INFINITY, l_run = 0.f;
+        float top = 0x1p-100f; // (codes: above all scales of values seen, see above)
 
         // A step that some row sees in part: values of it that are not finite, or
         // would not be as f16 parts, must not reach the rows that do not see them
         // (0 * inf), see below.
         bool odd = partial(p_begin, cur) && clean(p_begin, cur);
 #pragma unroll
-        for (int n = 0; n < 2 * R::N; ++n) store(0, n);
+        for (int n = 0; n < 2 * R::N; ++n) store(0, n, p_begin, cur);
         load(p_begin + PR_TILE, next);
         __syncthreads();
         int buf = 0;
         const int o = 32 * part_of; // this wave's 32 positions of a step
         for (int p0 = p_begin; p0 < p_end; p0 += PR_TILE) {
             const Pages after = pages_of(p0 + 2 * PR_TILE);
-            const RowsLds<LO> &l = lds.step[buf];
+            const Lds &l = lds.step[buf];
             const int p = p0 + o, pa = part_of ? cur.of(2) : cur.of(0),
                       pb = part_of ? cur.of(3) : cur.of(1);
             if (partial(p0 + PR_TILE, next)) odd |= clean(p0 + PR_TILE, next);
@@ -404,16 +472,32 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     sv = mfma(ahi[kk & 1], qhi[kk], sv);
                     sv = mfma(ahi[kk & 1], qlo[kk], sv);
                 }
-                if (kk < 2 * R::N) store(buf ^ 1, kk);
+                if (kk < 2 * R::N) store(buf ^ 1, kk, p0 + PR_TILE, next);
                 __builtin_amdgcn_sched_barrier(0);
             }
             load(p0 + 2 * PR_TILE, after);
             if constexpr (LO) sv += sx * (1.f / LO_SCALE);
+            // the scales of the lane's positions
+            f32x16 bs;
+            if constexpr (Q8) {
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&l.scale[0][o + 8 * a + 4 * h]);
+                    const f32x4 y = *reinterpret_cast<const f32x4 *>(&l.scale[1][o + 8 * a + 4 * h]);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        sv[4 * a + b] *= x[b];
+                        bs[4 * a + b] = y[b];
+                    }
+                }
+            }
             if (p + 31 > wave_all || (pa | pb) < 0) { // mask
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int pos = p + 8 * (e >> 2) + 4 * h + (e & 3);
-                    sv[e] = pos <= sees && (e < 8 ? pa : pb) >= 0 ? sv[e] : -INFINITY;
+                    const bool see = pos <= sees && (e < 8 ? pa : pb) >= 0;
+                    sv[e] = see ? sv[e] : -INFINITY;
+                    if constexpr (Q8) bs[e] = see ? bs[e] : 0.f;
                 }
             }
             float tmax = sv[0];
@@ -427,14 +511,28 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             // resolve 2^-25, which is 2^-32 of the first weight. (Many equal small
             // weights are rounded the same way, and their errors add up.)
             const float m_new = fmaf(wave::max_halves(tmax), qscale, -7.f);
-            if (__any(m_new > m_run + 8.f)) {
+            float bmax = 0.f;
+            if constexpr (Q8) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) bmax = fmaxf(bmax, bs[e]);
+                bmax = wave::max_halves(bmax);
+            }
+            if (__any(m_new > m_run + 8.f || (Q8 && bmax > top))) {
                 const float m = fmaxf(m_run, m_new);
-                const float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+                float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+                l_run *= corr;
+                if constexpr (Q8) {
+                    if (bmax > top) { // (the power of two above bmax)
+                        const float up = __builtin_bit_cast(
+                            float, (__builtin_bit_cast(unsigned, bmax) & 0x7f800000u) + 0x00800000u);
+                        corr *= top / up;
+                        top = up;
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
-                l_run *= corr;
                 m_run = m;
             }
             const float base = m_run == -INFINITY ? 0.f : m_run; // (nothing seen yet: zero weights)
@@ -445,6 +543,12 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                 rs[e & 1] += sv[e];
             }
             l_run += rs[0] + rs[1];
+            if constexpr (Q8) {
+                const float inv = __builtin_bit_cast(
+                    float, 0x7f000000u - __builtin_bit_cast(unsigned, top)); // 1 / top
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sv[e] *= bs[e] * inv;
+            }
             // operand element 4 x + i of product (kk, j): position 16 kk + 8 x + 4 h + i,
             // which is the lane's weight 8 kk + 4 x + i
             half8 vhi[4], vlo[4];
@@ -497,6 +601,14 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             cur = next;
             next = after;
             buf ^= 1;
+        }
+        if constexpr (Q8) { // the sums themselves, of weights of at most 1
+#pragma unroll
+            for (int j = 0; j < KV_D / 32; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[j][e] *= top * 0x1p-15f;
+            l_run *= 0x1p-15f;
+            m_run += 15.f;
         }
         if (__syncthreads_or(odd)) {
             // the values left out, for the rows that see them: whatever its weight,
@@ -581,7 +693,10 @@ int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, 
     const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh); // (more groups there are not)
     const bool whole = 1 << kv.shift >= PR_TILE;
     auto kernel = whole ? paged_rows_kernel<float, true> : paged_rows_kernel<float, false>;
-    if (kv.f16)
+    if (kv.type == KV_T_Q8)
+        kernel = whole ? paged_rows_kernel<unsigned char, true>
+                       : paged_rows_kernel<unsigned char, false>;
+    if (kv.type == KV_T_F16)
         kernel = whole ? paged_rows_kernel<_Float16, true> : paged_rows_kernel<_Float16, false>;
     hipLaunchKernelGGL(kernel, grid, dim3(PR_THREADS), 0, st, kv, rs, q, out);
     return (int)hipGetLastError();

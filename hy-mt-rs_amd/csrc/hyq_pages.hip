@@ -405,8 +405,8 @@ __global__ __launch_bounds__(256) void pages_fill_kernel(PagesArgs a, char *pool
     const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
     const int n = w.count[0], per = a.layers * 2 * a.kvh;
     const int lane = threadIdx.x & 63;
-    const size_t row = (size_t)KV_D * (a.f16 ? 2 : 4);
-    const size_t head = row << a.shift, page = head * 2 * a.kvh;
+    const size_t scales = a.type == KV_T_Q8 ? 4 : 0, row = kv_row_bytes(a.type) - scales;
+    const size_t head = row << a.shift, page = (head + (scales << a.shift)) * 2 * a.kvh;
     const long long items = (long long)n * per, step = (long long)gridDim.x * 4;
     for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += step) {
         const int c = (int)(i / per), r = (int)(i % per);
@@ -423,6 +423,13 @@ __global__ __launch_bounds__(256) void pages_fill_kernel(PagesArgs a, char *pool
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (x + 64 * k < words) __builtin_nontemporal_store(v[k], dst + x + 64 * k);
+        }
+        if (scales) { // (at most 256 of them, behind all heads' codes; the last words of four whole)
+            const size_t by = (size_t)(r / (2 * a.kvh)) * a.npages * page + head * 2 * a.kvh +
+                              (size_t)(r % (2 * a.kvh)) * (scales << a.shift) + lane * 16;
+            if (lane < (e[2] + 3) / 4)
+                *reinterpret_cast<u32x4 *>(pool + by + e[1] * page) =
+                    *reinterpret_cast<const u32x4 *>(pool + by + e[0] * page);
         }
     }
 }
@@ -482,7 +489,7 @@ __global__ __launch_bounds__(256) void pages_move_kernel(PagesArgs a, char *pool
 {
     const PagesScratch w = pages_layout(scratch, a.npages, a.seqs);
     const int t = threadIdx.x;
-    const size_t page = ((size_t)KV_D * (a.f16 ? 2 : 4) << a.shift) * 2 * a.kvh;
+    const size_t page = ((size_t)kv_row_bytes(a.type) << a.shift) * 2 * a.kvh;
     const int cuts = (int)((page + COMPACT_BYTES - 1) / COMPACT_BYTES);
     const long long per = (long long)a.layers * cuts, items = w.count[0] * per;
     for (long long i = blockIdx.x; i < items; i += gridDim.x) {

@@ -354,7 +354,11 @@ int hyq_argmax_d(hyq_ctx *ctx, const float *x_d, size_t n, float *scratch_d, int
  * pages of one pool, and every call takes the new tokens of all of them.
  *
  *   pool   [layers][pages][2][kv_heads][page_tokens][head_dim] F32 or F16:
- *          a page's keys, then its values, in every layer under one id
+ *          a page's keys, then its values, in every layer under one id. With
+ *          HYQ_KV_Q8 a byte for each number and behind a page's 2 * kv_heads *
+ *          page_tokens * head_dim of them an f32 scale for each position of a
+ *          head, [2][kv_heads][page_tokens]: x = scale * code, codes from -127
+ *          to 127, a key's as a signed byte, a value's as code + 128
  *   table  [seqs][stride] int32: the page ids of a slot's positions, in order
  *          (-1: none; an id outside [0, pages) holds nothing: nothing is
  *          written there and its positions are not attended)
@@ -370,8 +374,9 @@ int hyq_argmax_d(hyq_ctx *ctx, const float *x_d, size_t n, float *scratch_d, int
  * must be 16-byte aligned. Calls that overlap in time (two contexts, two
  * captured graphs replayed at once) need scratch of their own. Every call can
  * be captured in a HIP graph: none allocates, copies to the host or waits. */
+enum { HYQ_KV_Q8 = 1008 }; /* of pools alone: no format of a file or weight */
 typedef struct {
-    int dtype;       /* HYQ_F32 or HYQ_F16: element type of the pool */
+    int dtype;       /* HYQ_F32, HYQ_F16 or HYQ_KV_Q8: element type of the pool */
     int layers;
     int kv_heads;    /* 1..256 */
     int head_dim;    /* 128 */
@@ -388,7 +393,10 @@ size_t hyq_kv_pool_bytes(const hyq_kv_layout *kl);
  * (norm_first: the hy_v3 order, src/model.rs:425-446), q to q_out_d (which may
  * be q_d), k and v to the pages of `layer` (of two rows for one place, in a page
  * that two slots name, either stays: hyq_pages_extend_d gives each its own). An
- * F16 pool holds the values rounded once, to nearest. The angle position * freq_d[j] is taken in 64
+ * F16 pool holds the values rounded once, to nearest. An HYQ_KV_Q8 pool holds the
+ * 128 numbers x of a position and head as scale = max |x| / 127 in f32 and codes
+ * rint(x / scale), off by at most half a scale; one that is not finite makes the
+ * scale, and with it the head, a NaN. Such keys are formed in 64 bits. The angle position * freq_d[j] is taken in 64
  * bits, where hyq_rope_norm_append_d rounds the product to 32 (the reference's
  * table, src/model.rs:919-925): the two differ by up to position * 2^-24
  * radians times the frequency, and agree where the product is exact. */
@@ -399,6 +407,12 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
                                  const float *q_norm_d, const float *k_norm_d,
                                  const float *freq_d, float eps, int norm_first,
                                  float *q_out_d);
+/* The packed rows' keys and values as the pages of `layer` hold them, to k_d and
+ * v_d [rows][kv_heads*128] f32: slot s's last start[s+1] - start[s] positions (all
+ * of them where that is its length). Zeros where no page holds a position. */
+int hyq_paged_read_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, int layer,
+                     const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
+                     size_t rows, float *k_d, float *v_d);
 /* attention (src/model.rs:949-1037) of the packed rows over their slots'
  * pages: the row at position p sees the slot's positions 0..p. Any mix of
  * prompts, decode steps and drafted tokens. max_rows bounds the new rows of
@@ -408,7 +422,9 @@ int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *po
  * (those products split them into two f16 parts: 22 bits of numbers from 2^-14
  * up, 2^-36 absolutely below). A value beyond it there, and one that is not
  * finite in any form, makes its dim of the rows that see it not finite (such a
- * key the whole of those rows), and changes no other row. What places hold that
+ * key the whole of those rows), and changes no other row. An HYQ_KV_Q8 pool has
+ * no such limit: its codes enter the products exactly, queries to 22 bits of the
+ * row's largest, values to 2^-31 of the largest that the row sees (each). What places hold that
  * no position uses (a page's rest, pages never written) is never part of a
  * result. out_d must not be q_d. scratch_d: hyq_paged_attention_scratch_bytes
  * bytes (0 for arguments that the call refuses). */
