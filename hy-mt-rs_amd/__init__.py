@@ -132,6 +132,7 @@ SIGNATURES = {
     "hyq_pages_extend_d": (I, [P, P, P, P, P, P, P, P, P, P, P, P, SZ]),
     "hyq_pages_extend_served_d": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, SZ]),
     "hyq_pages_compact_d": (I, [P, P, P, P, P, P, P, P, P, SZ]),
+    "hyq_logits_adjust_d": (I, [P, P, SZ, SZ, P, P]),
     "hyq_sample_scratch_bytes": (SZ, [SZ, SZ]),
     "hyq_sample_d": (I, [P, P, SZ, SZ, P, P, P, P, P, P, SZ, P, P]),
 }
@@ -153,6 +154,14 @@ class DenseConfig(ctypes.Structure):
     _fields_ = [("layers", I), ("hidden", I), ("heads", I), ("kv_heads", I),
                 ("head_dim", I), ("ffn", I), ("vocab", I), ("rope_base", ctypes.c_float),
                 ("rms_eps", ctypes.c_float)]
+
+
+class LogitRules(ctypes.Structure):
+    """hyq_logit_rules: device arrays of penalties, biases and masks (null: none)."""
+    _fields_ = [("history", P), ("history_len", P), ("prompt_len", P), ("history_stride", SZ),
+                ("repetition", P), ("presence", P), ("frequency", P), ("bias_start", P),
+                ("bias_token", P), ("bias", P), ("biases", SZ), ("mask", P), ("mask_row", P),
+                ("masks", SZ)]
 
 
 class KvLayout(ctypes.Structure):
@@ -839,6 +848,57 @@ class PagedCache:
         check(lib().hyq_paged_attention_d(
             self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
             self._rows_len.ptr, start_d, rows, max_rows, heads, q_d, scratch.ptr, scratch.nbytes, out_d))
+
+
+def adjust_logits(ctx: "Context", logits: np.ndarray, history=None, prompt_len=None,
+                  repetition=1.0, presence=0.0, frequency=0.0, bias=None, masks=None,
+                  mask_row=None) -> np.ndarray:
+    """hyq_logits_adjust_d of logits [rows][vocab]: the logits that ``sample`` is to
+    take. history: the tokens of each row, of which the first prompt_len[row] are its
+    prompt; the penalties are values for all rows or arrays of one per row; bias: the
+    (tokens, values) of each row; masks: truth values [masks][vocab] of the tokens
+    allowed, of which row r goes by mask_row[r] (-1: none). (All of it from and to host
+    arrays; a serving loop whose logits are on the device calls hyq_logits_adjust_d.)"""
+    logits = np.ascontiguousarray(logits, np.float32)
+    rows, vocab = logits.shape
+    rules, keep = LogitRules(), []
+
+    def put(values, dtype):
+        keep.append(ctx.array(np.ascontiguousarray(values, dtype)))
+        return keep[-1].ptr
+
+    each = lambda v, t: put(np.broadcast_to(np.asarray(v, t), (rows,)), t)
+    if history is not None:
+        if len(history) != rows:
+            raise ValueError("one history per row")
+        held = [len(h) for h in history]
+        table = np.zeros((rows, max(held + [1])), np.int32)
+        for r, h in enumerate(history):
+            table[r, :held[r]] = h
+        rules.history, rules.history_stride = put(table, np.int32), table.shape[1]
+        rules.history_len = put(held, np.int32)
+        rules.prompt_len = None if prompt_len is None else each(prompt_len, np.int32)
+        rules.repetition, rules.presence = each(repetition, np.float32), each(presence, np.float32)
+        rules.frequency = each(frequency, np.float32)
+    if bias is not None:
+        if len(bias) != rows or any(len(t) != len(v) for t, v in bias):
+            raise ValueError("tokens and values of each row")
+        rules.biases = sum(len(t) for t, _ in bias)
+        rules.bias_start = put(np.cumsum([0] + [len(t) for t, _ in bias]), np.int32)
+        # (one more of each: a list may be empty, an array may not)
+        rules.bias_token = put(np.concatenate([t for t, _ in bias] + [[0]]), np.int32)
+        rules.bias = put(np.concatenate([v for _, v in bias] + [[0]]), np.float32)
+    if masks is not None:
+        masks = np.asarray(masks, bool)
+        if masks.ndim != 2 or masks.shape[1] != vocab or not masks.shape[0] or mask_row is None:
+            raise ValueError("masks of the vocabulary's width, and the mask of each row")
+        bits = np.zeros((len(masks), -(-vocab // 32) * 32), bool)
+        bits[:, :vocab] = masks
+        rules.mask = put(np.packbits(bits, axis=1, bitorder="little"), np.uint8)
+        rules.mask_row, rules.masks = each(mask_row, np.int32), len(masks)
+    d = ctx.array(logits)
+    check(lib().hyq_logits_adjust_d(ctx.handle, d.ptr, rows, vocab, ctypes.byref(rules), d.ptr))
+    return d.numpy()
 
 
 def sample(ctx: "Context", logits: np.ndarray, random, temperature=1.0, top_k=0, top_p=1.0,

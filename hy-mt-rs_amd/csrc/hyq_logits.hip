@@ -1,0 +1,111 @@
+// Rules on rows of logits before a token is drawn: penalties for tokens that a row
+// has already, biases and grammar masks, in one pass.
+//
+//   l' = l / r or l * r (l > 0 or not) for a token of the row's history,
+//   l' -= presence + frequency n for one that it has made n > 0 times,
+//   l' += bias (of several pairs of one token the last), -inf where the mask's bit is 0.
+//
+// A workgroup takes CHUNK logits of a row. It holds their counts in LDS, which it
+// fills from the row's whole history (a few KB, which the row's other workgroups
+// read too and find in the caches): whole numbers, so that the order of the
+// atomics does not matter, and of a token's biases the greatest place, not a sum.
+// Nothing is sorted, and no launch waits for another.
+//
+// Bound by memory for many rows.
+#include <hip/hip_runtime.h>
+
+#include "hyq_paged.hpp"
+
+namespace hyq {
+
+namespace {
+
+constexpr int PER = 8, CHUNK = 256 * PER;
+constexpr unsigned PROMPT = 0x80000000u; // a count's mark of a token that the prompt has
+
+// KEEP: the output is the input; logits that no rule changes are not read.
+template <bool KEEP>
+__global__ __launch_bounds__(256) void logits_adjust_kernel(const float *logits, int vocab,
+                                                            LogitRulesArgs a, float *out)
+{
+    __shared__ unsigned count[CHUNK];
+    __shared__ int pair[CHUNK]; // 1 + the last of the row's pairs for a token
+    const int t = threadIdx.x, row = blockIdx.y;
+    const int v0 = blockIdx.x * CHUNK, n = min(CHUNK, vocab - v0);
+    const float *src = logits + (size_t)row * vocab + v0;
+    float *dst = out + (size_t)row * vocab + v0;
+    float x[PER];
+    if constexpr (!KEEP) { // (in flight while the history is read)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) x[k] = src[min(t + 256 * k, n - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) count[t + 256 * k] = 0, pair[t + 256 * k] = 0;
+    int held = 0, prompt = 0, from = 0, to = 0;
+    if (a.history) {
+        held = min(max(a.history_len[row], 0), a.history_stride);
+        prompt = a.prompt_len ? a.prompt_len[row] : 0;
+    }
+    if (a.bias_start) {
+        from = min(max(a.bias_start[row], 0), a.biases);
+        to = min(max(a.bias_start[row + 1], from), a.biases);
+    }
+    __syncthreads();
+    const int *history = a.history + (size_t)row * a.history_stride;
+    for (int b = t; b < held; b += 256 * 4) { // (four loads in flight)
+        int tok[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tok[k] = history[min(b + 256 * k, held - 1)] - v0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = b + 256 * k;
+            if (i < held && (unsigned)tok[k] < (unsigned)n) {
+                if (i < prompt) atomicOr(count + tok[k], PROMPT);
+                else atomicAdd(count + tok[k], 1u);
+            }
+        }
+    }
+    for (int i = from + t; i < to; i += 256) {
+        const int v = a.bias_token[i] - v0;
+        if ((unsigned)v < (unsigned)n) atomicMax(pair + v, i + 1);
+    }
+    __syncthreads();
+    float r = a.repetition ? a.repetition[row] : 1.f;
+    r = r > 0.f ? r : 1.f;
+    const float presence = a.presence ? a.presence[row] : 0.f;
+    const float frequency = a.frequency ? a.frequency[row] : 0.f;
+    const int which = a.mask ? a.mask_row[row] : -1;
+    const unsigned *mask = (unsigned)which < (unsigned)a.masks
+                               ? a.mask + (size_t)which * ((vocab + 31) / 32)
+                               : nullptr;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = t + 256 * k;
+        if (i >= n) break;
+        const unsigned c = count[i], made = c & ~PROMPT;
+        const int p = pair[i];
+        const bool allowed = !mask || (mask[(v0 + i) >> 5] >> ((v0 + i) & 31) & 1);
+        if constexpr (KEEP) {
+            if (allowed && !c && !p) continue;
+            x[k] = allowed ? src[i] : 0.f;
+        }
+        float y = x[k];
+        if (c) y = y > 0.f ? y / r : y * r;
+        if (made) y -= presence + frequency * (float)made;
+        if (p) y += a.bias[p - 1];
+        dst[i] = allowed ? y : -INFINITY;
+    }
+}
+
+} // namespace
+
+int launch_logits_adjust(const float *logits, int rows, int vocab, const LogitRulesArgs &a,
+                         float *out, void *stream)
+{
+    const dim3 grid((vocab + CHUNK - 1) / CHUNK, rows);
+    auto kernel = out == logits ? logits_adjust_kernel<true> : logits_adjust_kernel<false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, logits, vocab, a, out);
+    return (int)hipGetLastError();
+}
+
+} // namespace hyq

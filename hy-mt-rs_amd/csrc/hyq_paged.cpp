@@ -304,6 +304,53 @@ int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
     return HYQ_OK;
 }
 
+int hyq_logits_adjust_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
+                        const hyq_logit_rules *r, float *out_d)
+{
+    if (!ctx) return fail(HYQ_EINVAL, "logits_adjust: null context");
+    if (!logits_d || !r || !out_d) return fail(HYQ_EINVAL, "logits_adjust: null argument");
+    if (rows == 0 || rows > 65535 || vocab == 0 || vocab > (1 << 24))
+        return fail(HYQ_EINVAL, "logits_adjust: %zu rows of %zu logits", rows, vocab);
+    if (r->history_d && !r->history_len_d)
+        return fail(HYQ_EINVAL, "logits_adjust: a history without lengths");
+    if (r->history_d && (r->history_stride == 0 || r->history_stride > (1 << 24)))
+        return fail(HYQ_EINVAL, "logits_adjust: a history of %zu tokens a row", r->history_stride);
+    if ((r->bias_start_d || r->bias_token_d || r->bias_d) &&
+        !(r->bias_start_d && r->bias_token_d && r->bias_d))
+        return fail(HYQ_EINVAL, "logits_adjust: biases without starts, tokens or values");
+    if (r->bias_d && r->biases > (1 << 30))
+        return fail(HYQ_EINVAL, "logits_adjust: %zu biases", r->biases);
+    if ((r->mask_d || r->mask_row_d) && !(r->mask_d && r->mask_row_d))
+        return fail(HYQ_EINVAL, "logits_adjust: masks without the rows' choice, or that alone");
+    if (r->mask_d && r->masks > (1 << 24))
+        return fail(HYQ_EINVAL, "logits_adjust: %zu masks", r->masks);
+    const uintptr_t from = reinterpret_cast<uintptr_t>(logits_d),
+                    to = reinterpret_cast<uintptr_t>(out_d), bytes = rows * vocab * 4;
+    if (from != to && from < to + bytes && to < from + bytes)
+        return fail(HYQ_EINVAL, "logits_adjust: the output overlaps the logits in part");
+    LogitRulesArgs a{};
+    if (r->history_d) {
+        a.history = r->history_d;
+        a.history_len = r->history_len_d;
+        a.prompt_len = r->prompt_len_d;
+        a.history_stride = (int)r->history_stride;
+        a.repetition = r->repetition_d;
+        a.presence = r->presence_d;
+        a.frequency = r->frequency_d;
+    }
+    a.bias_start = r->bias_start_d;
+    a.bias_token = r->bias_token_d;
+    a.bias = r->bias_d;
+    a.biases = (int)r->biases;
+    a.mask = r->mask_d;
+    a.mask_row = r->mask_row_d;
+    a.masks = (int)r->masks;
+    DeviceGuard g(ctx->device);
+    HYQ_LAUNCH(launch_logits_adjust(logits_d, (int)rows, (int)vocab, a, out_d, ctx->stream),
+               "logits_adjust");
+    return HYQ_OK;
+}
+
 size_t hyq_sample_scratch_bytes(size_t rows, size_t vocab)
 {
     if (rows == 0 || rows > 65535 || vocab == 0 || vocab > (1 << 24)) return 0;

@@ -1,6 +1,5 @@
 // Launchers of the paged KV cache's operators and of the sampler (kernels in
-// hyq_paged_append.hip, hyq_paged_few.hip, hyq_paged_rows.hip, hyq_pages.hip
-// and hyq_sample.hip).
+// hyq_paged_*.hip, hyq_pages.hip, hyq_logits.hip and hyq_sample.hip).
 #pragma once
 
 #include <stddef.h>
@@ -61,6 +60,19 @@ int launch_pages_extend(const PagesArgs &a, void *pool, const int *add, const in
                         int *refs_out, int *status, int *served, void *scratch, void *stream);
 int launch_pages_compact(const PagesArgs &a, void *pool, const int *table, const int *refs,
                          int *table_out, int *refs_out, int *live, void *scratch, void *stream);
+
+// Rules on rows of logits (hyq_logit_rules, hyq_logits.hip).
+struct LogitRulesArgs {
+    const int *history, *history_len, *prompt_len;
+    const float *repetition, *presence, *frequency;
+    const int *bias_start, *bias_token;
+    const float *bias;
+    const unsigned *mask;
+    const int *mask_row;
+    int history_stride, biases, masks;
+};
+int launch_logits_adjust(const float *logits, int rows, int vocab, const LogitRulesArgs &a,
+                         float *out, void *stream);
 
 size_t sample_scratch(int rows, int vocab);
 int launch_sample(const float *logits, int rows, int vocab, const float *temperature,

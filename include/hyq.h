@@ -478,6 +478,37 @@ int hyq_pages_compact_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d,
                         int32_t *refs_out_d, int32_t *live_d, void *scratch_d,
                         size_t scratch_bytes);
 
+/* Rules on logits before a token is drawn (device arrays, any group of them null):
+ * the repetition penalty of Sampler (src/generation.rs:229-334) and what other
+ * servers' requests ask for. For row r and token v, in this order:
+ *   v among the first history_len[r] tokens of history row r: l = l > 0 ?
+ *     l / repetition[r] : l * repetition[r] (null, or not above 0: 1);
+ *   v n > 0 times among those from prompt_len[r] on (null: all): l -=
+ *     presence[r] + frequency[r] * n (null: 0);
+ *   v in the pairs bias_start[r] .. bias_start[r+1]-1: l += the last such bias;
+ *   0 <= mask_row[r] < masks, and bit v % 32 of word v / 32 of that mask 0:
+ *     l = minus infinity, whatever it was.
+ * Tokens outside the vocabulary are passed over, and lengths, starts and rows cut
+ * to what there is. */
+typedef struct {
+    const int32_t *history_d;     /* [rows][history_stride] */
+    const int32_t *history_len_d; /* [rows] */
+    const int32_t *prompt_len_d;  /* [rows] or null */
+    size_t history_stride;        /* at most 2^24 */
+    const float *repetition_d, *presence_d, *frequency_d; /* [rows] or null */
+    const int32_t *bias_start_d; /* [rows + 1], ascending */
+    const int32_t *bias_token_d; /* [biases] */
+    const float *bias_d;         /* [biases] */
+    size_t biases;               /* at most 2^30 */
+    const uint32_t *mask_d;      /* [masks][(vocab + 31) / 32] */
+    const int32_t *mask_row_d;   /* [rows] */
+    size_t masks;                /* at most 2^24 */
+} hyq_logit_rules;
+/* The rules applied to logits [rows][vocab] (at most 65535 rows of 2^24). out_d may
+ * be logits_d (then only logits that a rule changes are read and written) but not
+ * overlap it otherwise. No scratch. */
+int hyq_logits_adjust_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
+                        const hyq_logit_rules *rules, float *out_d);
 /* Sampling (Sampler, src/generation.rs:229-334, from given random numbers):
  * one token for each row of logits [rows][vocab] (at most 65535 rows of 2^24),
  * with settings of its own in device arrays of `rows` values. With
