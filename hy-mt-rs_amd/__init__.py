@@ -127,6 +127,10 @@ SIGNATURES = {
     "hyq_paged_read_d": (I, [P, P, P, I, P, P, P, SZ, P, P]),
     "hyq_paged_attention_scratch_bytes": (SZ, [P, SZ, SZ, SZ]),
     "hyq_paged_attention_d": (I, [P, P, P, I, P, P, P, SZ, SZ, SZ, P, P, SZ, P]),
+    "hyq_paged_shared_plan_bytes": (SZ, [P, SZ, SZ]),
+    "hyq_paged_shared_plan_d": (I, [P, P, P, P, P, P, SZ, SZ, P, SZ]),
+    "hyq_paged_shared_attention_scratch_bytes": (SZ, [P, SZ, SZ, SZ]),
+    "hyq_paged_shared_attention_d": (I, [P, P, P, I, P, P, P, SZ, SZ, SZ, P, SZ, P, P, SZ, P]),
     "hyq_pages_fork_d": (I, [P, P, P, P, P, P, P, P, P]),
     "hyq_pages_scratch_bytes": (SZ, [P]),
     "hyq_pages_extend_d": (I, [P, P, P, P, P, P, P, P, P, P, P, P, SZ]),
@@ -751,7 +755,7 @@ class PagedCache:
         self._rows_len = self.len  # the lengths that append and attention go by
         self._live = ctx.empty(1, np.int32)
         self._scratch = ctx.empty(lib().hyq_pages_scratch_bytes(self._kl), np.uint8)
-        self._attention = []
+        self._attention, self._plans, self._planned = [], [], None
 
     def _slots(self, values, into: DeviceArray) -> int:
         a = np.ascontiguousarray(values, np.int32)
@@ -773,7 +777,7 @@ class PagedCache:
                                      self.len.ptr, table.ptr, length.ptr, self.refs.ptr))
         self._other = (self.table, self.len)
         self.table, self.len = table, length
-        self._rows_len = self.len
+        self._rows_len, self._planned = self.len, None
 
     def extend(self, add) -> np.ndarray:
         """Room for add[s] more tokens; the slots' status (0 done, 1 no pages
@@ -792,7 +796,7 @@ class PagedCache:
         if self.table is not table:
             self._other = (self.table, self.len)
             self.table, self.len = table, length
-        self._rows_len = self._served
+        self._rows_len, self._planned = self._served, None
 
     def compact(self) -> int:
         """hyq_pages_compact_d: the pages in use become 0 .. live-1; live."""
@@ -800,6 +804,7 @@ class PagedCache:
             self.ctx.handle, self._kl, self.pool.ptr, self.table.ptr, self.refs.ptr,
             self.table.ptr, self.refs.ptr, self._live.ptr, self._scratch.ptr,
             self._scratch.nbytes))
+        self._planned = None
         return int(self._live.numpy()[0])
 
     def lengths(self) -> np.ndarray:
@@ -834,20 +839,43 @@ class PagedCache:
         k, v = k.numpy(), v.numpy()
         return [(k[a:b], v[a:b]) for a, b in zip(start[:-1], start[1:])]
 
+    def _grown(self, buffers: list, need: int) -> DeviceArray:
+        have = buffers[-1].nbytes if buffers else 0
+        if need > have or not have:  # (0: a call that is refused)
+            buffers.append(self.ctx.empty(max(need, 2 * have, 16), np.uint8))
+        return buffers[-1]
+
+    def share_d(self, start_d: int, rows: int, heads: int, group_d: int | None = None) -> None:
+        """hyq_paged_shared_plan_d: finds the prefixes that slots share, for the
+        ``attention_d`` calls with ``shared`` until the next fork, extension or
+        compaction. Its buffer grows as attention_d's."""
+        need = lib().hyq_paged_shared_plan_bytes(self._kl, rows, heads)
+        plan = self._grown(self._plans, need)
+        check(lib().hyq_paged_shared_plan_d(
+            self.ctx.handle, self._kl, group_d, self.table.ptr, self._rows_len.ptr, start_d, rows,
+            heads, plan.ptr, plan.nbytes))
+        self._planned = (start_d, rows, heads)
+
     def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,
-                    q_d: int, out_d: int) -> None:
-        """hyq_paged_attention_d on device buffers. The scratch grows with the
-        largest call, at least twofold; the smaller ones live as long as the
+                    q_d: int, out_d: int, shared: bool = False) -> None:
+        """hyq_paged_attention_d on device buffers, or with ``shared``
+        hyq_paged_shared_attention_d by the plan of ``share_d``. The scratch grows
+        with the largest call, at least twofold; the smaller ones live as long as the
         cache, since a captured graph may hold them. (A capture allocates
         nothing: run the largest call once before it.)"""
-        need = lib().hyq_paged_attention_scratch_bytes(self._kl, rows, max_rows, heads)
-        have = self._attention[-1].nbytes if self._attention else 0
-        if need > have or not have:  # (0: a call that is refused)
-            self._attention.append(self.ctx.empty(max(need, 2 * have, 16), np.uint8))
-        scratch = self._attention[-1]
-        check(lib().hyq_paged_attention_d(
-            self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
-            self._rows_len.ptr, start_d, rows, max_rows, heads, q_d, scratch.ptr, scratch.nbytes, out_d))
+        if shared and self._planned != (start_d, rows, heads):
+            raise ValueError("no plan of these rows: share_d comes first, after a step's pages")
+        size = (lib().hyq_paged_shared_attention_scratch_bytes if shared else
+                lib().hyq_paged_attention_scratch_bytes)
+        scratch = self._grown(self._attention, size(self._kl, rows, max_rows, heads))
+        args = [self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
+                self._rows_len.ptr, start_d, rows, max_rows, heads]
+        if shared:
+            plan = self._plans[-1]
+            check(lib().hyq_paged_shared_attention_d(*args, plan.ptr, plan.nbytes, q_d,
+                                                     scratch.ptr, scratch.nbytes, out_d))
+        else:
+            check(lib().hyq_paged_attention_d(*args, q_d, scratch.ptr, scratch.nbytes, out_d))
 
 
 def adjust_logits(ctx: "Context", logits: np.ndarray, history=None, prompt_len=None,

@@ -235,9 +235,82 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
     if (out_d == q_d) return fail(HYQ_EINVAL, "paged_attention: the output must not be q");
     DeviceGuard g(ctx->device);
     HYQ_LAUNCH(launch_paged_attention(view(kl, pool_d, layer, table_d, len_d, start_d, rows, heads),
-                                      (int)std::min(rows, max_rows), q_d, scratch_d, out_d,
-                                      ctx->stream),
+                                      (int)std::min(rows, max_rows), q_d, scratch_d, nullptr,
+                                      out_d, ctx->stream),
                "paged_attention");
+    return HYQ_OK;
+}
+
+size_t hyq_paged_shared_plan_bytes(const hyq_kv_layout *kl, size_t rows, size_t heads)
+{
+    if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS) return 0;
+    return shared_plan_bytes(kl->seqs, kl->kv_heads, (int)heads, (int)rows);
+}
+
+int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
+                            const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
+                            size_t rows, size_t heads, void *plan_d, size_t plan_bytes)
+{
+    int rc = check_layout(ctx, kl, "paged_shared_plan");
+    if (rc) return rc;
+    if (!table_d || !len_d || !start_d || !plan_d)
+        return fail(HYQ_EINVAL, "paged_shared_plan: null argument");
+    if (!heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS)
+        return fail(HYQ_EINVAL, "paged_shared_plan: %zu rows, heads %zu/%d", rows, heads,
+                    kl->kv_heads);
+    if (!aligned(plan_d)) return fail(HYQ_EINVAL, "paged_shared_plan: the plan is not 16-byte aligned");
+    const size_t need = hyq_paged_shared_plan_bytes(kl, rows, heads);
+    if (plan_bytes < need)
+        return fail(HYQ_EINVAL, "paged_shared_plan: a plan of %zu bytes, %zu needed", plan_bytes,
+                    need);
+    DeviceGuard g(ctx->device);
+    HYQ_LAUNCH(launch_shared_plan(view(kl, nullptr, 0, table_d, len_d, start_d, rows, heads),
+                                  group_d, plan_d, ctx->stream),
+               "paged_shared_plan");
+    return HYQ_OK;
+}
+
+size_t hyq_paged_shared_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows,
+                                                size_t max_rows, size_t heads)
+{
+    if (!hyq_paged_attention_scratch_bytes(kl, rows, max_rows, heads)) return 0;
+    return shared_attention_scratch(type_of(kl), kl->seqs, kl->kv_heads, (int)heads, (int)rows,
+                                    (int)std::min(rows, max_rows));
+}
+
+int hyq_paged_shared_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d,
+                                 int layer, const int32_t *table_d, const int32_t *len_d,
+                                 const int32_t *start_d, size_t rows, size_t max_rows, size_t heads,
+                                 const void *plan_d, size_t plan_bytes, const float *q_d,
+                                 void *scratch_d, size_t scratch_bytes, float *out_d)
+{
+    int rc = check_layout(ctx, kl, "paged_shared_attention");
+    if (rc) return rc;
+    if (!pool_d || !table_d || !len_d || !start_d || !plan_d || !q_d || !scratch_d || !out_d)
+        return fail(HYQ_EINVAL, "paged_shared_attention: null argument");
+    if (layer < 0 || layer >= kl->layers)
+        return fail(HYQ_EINVAL, "paged_shared_attention: layer %d of %d", layer, kl->layers);
+    if (!heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0 ||
+        !grid_ok(kl, rows, heads))
+        return fail(HYQ_EINVAL,
+                    "paged_shared_attention: %zu rows (at most %zu of a slot), heads %zu/%d", rows,
+                    max_rows, heads, kl->kv_heads);
+    if (!aligned(pool_d) || !aligned(plan_d) || !aligned(q_d) || !aligned(scratch_d) ||
+        !aligned(out_d))
+        return fail(HYQ_EINVAL, "paged_shared_attention: a buffer is not 16-byte aligned");
+    if (plan_bytes < hyq_paged_shared_plan_bytes(kl, rows, heads))
+        return fail(HYQ_EINVAL, "paged_shared_attention: a plan of %zu bytes, %zu needed",
+                    plan_bytes, hyq_paged_shared_plan_bytes(kl, rows, heads));
+    const size_t need = hyq_paged_shared_attention_scratch_bytes(kl, rows, max_rows, heads);
+    if (scratch_bytes < need)
+        return fail(HYQ_EINVAL, "paged_shared_attention: scratch of %zu bytes, %zu needed",
+                    scratch_bytes, need);
+    if (out_d == q_d) return fail(HYQ_EINVAL, "paged_shared_attention: the output must not be q");
+    DeviceGuard g(ctx->device);
+    HYQ_LAUNCH(launch_paged_attention(view(kl, pool_d, layer, table_d, len_d, start_d, rows, heads),
+                                      (int)std::min(rows, max_rows), q_d, scratch_d, plan_d, out_d,
+                                      ctx->stream),
+               "paged_shared_attention");
     return HYQ_OK;
 }
 
@@ -396,9 +469,33 @@ size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows,
     return n;
 }
 
-int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void *scratch,
-                           float *out, void *stream)
+// Behind them, in whole 256 bytes, the prefixes' parts.
+size_t shared_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows)
 {
+    const size_t n = paged_attention_scratch(type, seqs, kvh, heads, rows, max_rows);
+    return (n + 255) / 256 * 256 + shared_parts_bytes(seqs, kvh, heads, rows);
+}
+
+size_t shared_plan_bytes(int seqs, int kvh, int heads, int rows)
+{
+    return shared_layout(seqs, kvh, heads, rows).bytes;
+}
+
+int launch_paged_attention(const PagedKv &given, int max_rows, const float *q, void *scratch,
+                           const void *plan, float *out, void *stream)
+{
+    PagedKv kv = given;
+    SharedPlan sp{};
+    float *prefix = nullptr;
+    if (plan) {
+        sp = shared_plan(plan, kv.seqs, kv.kvh, kv.heads, kv.rows);
+        kv.skip = sp.skip;
+        const size_t n =
+            paged_attention_scratch(kv.type, kv.seqs, kv.kvh, kv.heads, kv.rows, max_rows);
+        prefix = (float *)((char *)scratch + (n + 255) / 256 * 256);
+        const int rc = launch_paged_prefix(kv, sp, q, prefix, stream);
+        if (rc) return rc;
+    }
     const int few = std::min(paged_few_rows(kv.heads / kv.kvh), max_rows);
     float *part = (float *)scratch;
     RowsScratch rs{};
@@ -416,7 +513,7 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
     }
     int rc = launch_paged_few(kv, few, rs, q, part, out, stream);
     if (rc == 0 && rs.cap) rc = launch_paged_rows(kv, rs, q, out, stream);
-    if (rc == 0) rc = launch_paged_merge(kv, few, rs, part, out, stream);
+    if (rc == 0) rc = launch_paged_merge(kv, few, rs, part, plan ? &sp : nullptr, prefix, out, stream);
     return rc;
 }
 

@@ -45,8 +45,15 @@ int launch_paged_read(const PagedKv &kv, float *k, float *v, void *stream);
 // Attention: the one-wave form for slots of few new rows and the tile form for
 // the others; scratch as paged_attention_scratch says.
 size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows);
+// plan: of the prefixes that slots share (launch_shared_plan's), or null; their
+// parts lie in the scratch behind what paged_attention_scratch says.
 int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void *scratch,
-                           float *out, void *stream);
+                           const void *plan, float *out, void *stream);
+
+// The plan of a step's shared prefixes. group: the slots' groups, or null.
+size_t shared_plan_bytes(int seqs, int kvh, int heads, int rows);
+size_t shared_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows);
+int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *stream);
 
 struct PagesArgs {
     int type, layers, kvh, shift, npages, seqs, stride;

@@ -207,6 +207,7 @@ struct RowsScratch {
     float *parts;
     int tq, cap; // tokens of a block, blocks there is room for (0: no tile form)
     int most;    // new rows of a slot at most; those of more are not computed
+    const int *list; // prefixes: the blocks' packed rows
 };
 struct RowsLayout {
     size_t blocks, pieces, groups, parts, bytes;
@@ -390,14 +391,77 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
     }
 }
 
+// ---- prefixes that several slots share ----
+// A group's slots have their first `skip` positions in common, on the same pages.
+// The tokens of the group's slots, one after another, stand in blocks of tq in
+// `list` (block b's at places b * tq ..), and their query rows see those positions
+// whole: the tile form attends them from the first slot's table row, a piece a
+// workgroup, and leaves parts that the merge joins with the slots' own.
+struct SharedPlan {
+    Plan *plan;    // blocks, pieces (as groups)
+    int *skip;     // [seqs] positions that the slot's group attends, 0: none
+    int *place;    // [seqs] the first place of its tokens in the list
+    int *leader;   // [seqs] the first slot of its group, -1: it can be in none
+    int *run;      // [seqs] pages that it has in common with that one
+    int *list;     // [cap * tq] packed rows
+    Block *blocks; // [cap]
+    Piece *pieces; // [most]
+    int tq, cap, most;
+};
+struct SharedLayout {
+    size_t ints, list, blocks, pieces, bytes;
+    int cap, most;
+};
+// (rows: of few-row slots, as many as there can be)
+inline SharedLayout shared_layout(int seqs, int kvh, int heads, int rows)
+{
+    const int rep = heads / kvh, tq = PR_ROWS / rep;
+    const long long few = std::min<long long>(rows, (long long)seqs * (16 / rep));
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    SharedLayout l;
+    l.cap = (int)(few / tq) + seqs / 2 + 1; // (a group has two slots or more)
+    l.most = l.cap + fill_pieces(kvh);
+    l.ints = up(sizeof(Plan));
+    l.list = l.ints + up((size_t)seqs * 4) * 4;
+    l.blocks = l.list + up((size_t)l.cap * tq * 4);
+    l.pieces = l.blocks + up((size_t)l.cap * sizeof(Block));
+    l.bytes = l.pieces + up((size_t)l.most * sizeof(Piece));
+    return l;
+}
+inline SharedPlan shared_plan(const void *plan, int seqs, int kvh, int heads, int rows)
+{
+    const SharedLayout l = shared_layout(seqs, kvh, heads, rows);
+    char *base = (char *)const_cast<void *>(plan);
+    const size_t each = ((size_t)seqs * 4 + 255) / 256 * 256;
+    SharedPlan p;
+    p.plan = (Plan *)base;
+    p.skip = (int *)(base + l.ints);
+    p.place = (int *)(base + l.ints + each);
+    p.leader = (int *)(base + l.ints + 2 * each);
+    p.run = (int *)(base + l.ints + 3 * each);
+    p.list = (int *)(base + l.list);
+    p.blocks = (Block *)(base + l.blocks);
+    p.pieces = (Piece *)(base + l.pieces);
+    p.tq = PR_ROWS / (heads / kvh);
+    p.cap = l.cap;
+    p.most = l.most;
+    return p;
+}
+inline size_t shared_parts_bytes(int seqs, int kvh, int heads, int rows)
+{
+    return (size_t)shared_layout(seqs, kvh, heads, rows).most * kvh * PR_ROWS * PAGED_PART * 4;
+}
+
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)
 // new rows, with the plan where there is a tile form; and the merge of both.
 int paged_few_rows(int rep);
 size_t paged_few_scratch(int type, int seqs, int kvh, int heads, int few);
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
                      float *out, void *stream);
+// (shared, with its parts: null where no prefix is attended for several slots)
 int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
-                       float *out, void *stream);
+                       const SharedPlan *shared, const float *shared_parts, float *out,
+                       void *stream);
 // hyq_paged_few_q8.hip: the few-row form of 8-bit pages, as launch_paged_few has
 // laid it out.
 int launch_paged_few_q8(const PagedKv &kv, int few, int workers, const RowsScratch &rs,
@@ -406,5 +470,8 @@ int launch_paged_few_q8(const PagedKv &kv, int few, int workers, const RowsScrat
 // hyq_paged_rows.hip: the slots of more.
 int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, float *out,
                       void *stream);
+// The shared prefixes, to parts.
+int launch_paged_prefix(const PagedKv &kv, const SharedPlan &sp, const float *q, float *parts,
+                        void *stream);
 
 } // namespace hyq

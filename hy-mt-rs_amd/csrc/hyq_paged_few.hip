@@ -496,10 +496,12 @@ template <class V, int ROWS> struct Joined {
 // them, by 256 threads, lane d dims 2 d and 2 d + 1. wide: row c by all four
 // waves, a quarter of the parts each, joined in wave order; otherwise rows c ..
 // c + 3, one per wave.
+template <bool SHARED>
 __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int part_rows,
                                           const float *__restrict__ part,
-                                          const int2 *__restrict__ shared, float *__restrict__ out,
-                                          int kh, int s, int c, bool wide)
+                                          const int2 *__restrict__ shared, const SharedPlan &sp,
+                                          const float *__restrict__ prefix,
+                                          float *__restrict__ out, int kh, int s, int c, bool wide)
 {
     __shared__ float red[4][KV_D + 2];
     const int rep = kv.heads / kv.kvh;
@@ -507,7 +509,8 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     const SlotRows sr = slot_rows(kv, s);
     if (sr.n > few_rows || c >= sr.n * rep) return;
     const int w0 = by.x, n = by.y;
-    if (n == 1) return; // written whole
+    const bool grouped = SHARED && skipped<SHARED>(kv, s, sr) > 0;
+    if (n == 1 && !grouped) return; // written whole
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int r = wide ? c : c + g;
     if (!wide && r >= sr.n * rep) return;
@@ -517,6 +520,20 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     const int a = wide ? n * g / 4 : 0, b = wide ? n * (g + 1) / 4 : n;
     Joined<float2v, 1> j;
     j.add({p + (size_t)a * step}, step, b - a, 2 * lane);
+    if constexpr (SHARED) {
+        if (grouped) { // the prefix's pieces, for this row of its block
+            const int last = sp.cap * sp.tq - 1;
+            const int at = min(min(max(sp.place[s], 0), last) + r / rep, last);
+            const Block blk = sp.blocks[at / sp.tq];
+            const int first = min(max(blk.part, 0), sp.most - 1);
+            const int k = min(max(blk.pieces, 0), sp.most - first);
+            const int c0 = wide ? k * g / 4 : 0, c1 = wide ? k * (g + 1) / 4 : k;
+            const size_t each = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
+            const float *x = prefix + ((size_t)first * kv.kvh + kh) * PR_ROWS * PAGED_PART +
+                             (size_t)(at % sp.tq * rep + r % rep) * PAGED_PART;
+            j.add({x + (size_t)c0 * each}, each, c1 - c0, 2 * lane);
+        }
+    }
     float *o = out + ((size_t)(sr.begin + r / rep) * kv.heads + kh * rep + r % rep) * KV_D;
     if (!wide) {
         *reinterpret_cast<float2v *>(o + 2 * lane) = j.x[0] * j.scale(0);
@@ -568,17 +585,20 @@ __device__ __forceinline__ void merge_rows(const PagedKv &kv, const RowsScratch 
 
 // Grid: the slots' rows, one or four a workgroup, then the blocks', MERGE_ROWS a
 // workgroup; the KV heads of a row in sequence.
+template <bool SHARED>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_rows, int part_rows,
                                                           int wide, RowsScratch rs,
                                                           const float *__restrict__ part,
                                                           const int2 *__restrict__ shared,
+                                                          SharedPlan sp,
+                                                          const float *__restrict__ prefix,
                                                           float *__restrict__ out)
 {
     const int each = wide ? part_rows : (part_rows + 3) / 4; // workgroups of a slot and KV head
     const int kh = blockIdx.x % kv.kvh, i = blockIdx.x / kv.kvh, n = kv.seqs * each;
     if (i < n)
-        merge_few(kv, few_rows, part_rows, part, shared, out, kh, i / each,
-                  (i % each) * (wide ? 1 : 4), wide != 0);
+        merge_few<SHARED>(kv, few_rows, part_rows, part, shared, sp, prefix, out, kh, i / each,
+                          (i % each) * (wide ? 1 : 4), wide != 0);
     else
         merge_rows(kv, rs, out, kh, (i - n) / (PR_ROWS / MERGE_ROWS),
                    (i - n) % (PR_ROWS / MERGE_ROWS));
@@ -635,7 +655,7 @@ int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const fl
 }
 
 int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
-                       float *out, void *stream)
+                       const SharedPlan *plan, const float *prefix, float *out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
@@ -648,8 +668,9 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
     const int wide = kv.seqs * kv.kvh * part_rows <= 1024;
     const int each = wide ? part_rows : (part_rows + 3) / 4;
     const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, each, rs.cap));
-    hipLaunchKernelGGL(paged_merge_kernel, grid, dim3(256), 0, st, kv, few, part_rows, wide, rs, part,
-                       shared, out);
+    auto kernel = plan ? paged_merge_kernel<true> : paged_merge_kernel<false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, kv, few, part_rows, wide, rs, part, shared,
+                       plan ? *plan : SharedPlan{}, prefix, out);
     return (int)hipGetLastError();
 }
 

@@ -211,7 +211,10 @@ struct CodesLds {
 // look at the table and one base address instead of four of each, whose scalar
 // work was a sixth of a wave's time (512 tokens over 32012 positions, pages of 16
 // and of 64 tokens: 405 and 394 us in f32 pages, 266 and 249 in f16).
-template <class T, bool WHOLE>
+// PREFIX: blocks of several slots' tokens over positions that all of them see, a
+// piece a workgroup, always to parts (rs.most of them). What the plan says is cut
+// to what there is: it may be of another batch.
+template <class T, bool WHOLE, bool PREFIX>
 __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     PagedKv kv, RowsScratch rs, const float *__restrict__ q, float *__restrict__ out)
 {
@@ -227,12 +230,20 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     // (a group's KV heads in sequence, so that an XCD, which takes every eighth
     // workgroup, reads few heads' keys and values into its L2)
     const int kh = blockIdx.x % kv.kvh, group = blockIdx.x / kv.kvh;
-    const int from = rs.groups[group], to = rs.groups[group + 1]; // (read whatever their number)
+    // (read whatever their number)
+    const int from = PREFIX ? group : rs.groups[group], to = PREFIX ? group + 1 : rs.groups[group + 1];
     if (group >= rs.plan->groups) return;
 #pragma unroll 1
     for (int at_piece = from; at_piece < to; ++at_piece) {
         if (at_piece > from) __syncthreads(); // the last piece's readers of LDS are done
-        const Piece piece = rs.pieces[at_piece];
+        Piece piece = rs.pieces[at_piece];
+        if constexpr (PREFIX) {
+            piece.slot = min(max(piece.slot, 0), kv.seqs - 1);
+            piece.index = min(max(piece.index, 0), rs.cap - 1);
+            piece.part = min(max(piece.part, 0), rs.most - 1);
+            piece.first = (int)min((long long)max(piece.first, 0), (long long)kv.stride << kv.shift);
+            piece.t0 = min(max(piece.t0, 0), piece.first / PR_TILE);
+        }
         const int s = piece.slot, tq = rs.tq;
         const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;
         const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -243,13 +254,13 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         const int pmask = (1 << kv.shift) - 1;
         const float sc = 1.4426950408889634f * 0.08838834764831845f; // log2(e) / sqrt(128)
 
-        const int tok0 = piece.index * tq;
+        const int tok0 = piece.index * tq; // (PREFIX: in the list)
         const int first = piece.first; // position of the slot's first new row
-        const int toks = min(tq, piece.n - tok0);
-        const int seen_end = first + tok0 + toks; // one past the last position that a row sees
+        const int toks = min(tq, PREFIX ? piece.n : piece.n - tok0);
+        const int seen_end = PREFIX ? first : first + tok0 + toks; // one past the last position that a row sees
         const int p_end = min(piece.t1 * PR_TILE, seen_end);
         const int p_begin = piece.t0 * PR_TILE;
-        const int all_see = first + tok0; // the last position that every row sees
+        const int all_see = PREFIX ? first - 1 : first + tok0; // the last position that every row sees
 
         // The pages of a step's four 16-position groups (or the step's one), -1 where
         // none. Page ids come 64 at a time, one per lane. Rows past the end are
@@ -376,10 +387,12 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         const int r = 32 * rows + c, tl = r / rep;
         const bool ok = tl < toks;
         const int head = kh * rep + r % rep;
-        const int sees = ok ? first + tok0 + tl : -1; // its last visible position
+        const int sees = !ok ? -1 : PREFIX ? first - 1 : first + tok0 + tl; // its last visible position
         // the last position that the wave's first row sees, and with it all of them
-        const int wave_all = first + tok0 + min(toks - 1, (32 * rows) / rep);
-        const size_t row = (size_t)(piece.begin + tok0 + (ok ? tl : 0)) * kv.heads + head;
+        const int wave_all = PREFIX ? first - 1 : first + tok0 + min(toks - 1, (32 * rows) / rep);
+        const int packed = PREFIX ? min(max(rs.list[tok0 + (ok ? tl : 0)], 0), kv.rows - 1)
+                                  : piece.begin + tok0 + (ok ? tl : 0);
+        const size_t row = (size_t)packed * kv.heads + head;
 
         // q = 2^e (hi + lo), the row's power of two bringing it inside f16's range: to
         // below 2^14 where the low parts stay as they are, and to below 2 where they
@@ -665,7 +678,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         }
         float *dst = out + row * KV_D;
         float f = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f; // (saw nothing: zeros)
-        if (piece.part >= 0) {
+        if (PREFIX || piece.part >= 0) {
             dst = rs.parts + (((size_t)piece.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
             if (h == 0) {
                 dst[0] = m_run;
@@ -684,6 +697,17 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
     }
 }
 
+template <bool PREFIX> auto kernel_of(int type, bool whole)
+{
+    if (type == KV_T_Q8)
+        return whole ? paged_rows_kernel<unsigned char, true, PREFIX>
+                     : paged_rows_kernel<unsigned char, false, PREFIX>;
+    if (type == KV_T_F16)
+        return whole ? paged_rows_kernel<_Float16, true, PREFIX>
+                     : paged_rows_kernel<_Float16, false, PREFIX>;
+    return whole ? paged_rows_kernel<float, true, PREFIX> : paged_rows_kernel<float, false, PREFIX>;
+}
+
 } // namespace
 
 int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, float *out,
@@ -692,13 +716,25 @@ int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, 
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid(max_pieces(rs.cap, kv.kvh) * kv.kvh); // (more groups there are not)
     const bool whole = 1 << kv.shift >= PR_TILE;
-    auto kernel = whole ? paged_rows_kernel<float, true> : paged_rows_kernel<float, false>;
-    if (kv.type == KV_T_Q8)
-        kernel = whole ? paged_rows_kernel<unsigned char, true>
-                       : paged_rows_kernel<unsigned char, false>;
-    if (kv.type == KV_T_F16)
-        kernel = whole ? paged_rows_kernel<_Float16, true> : paged_rows_kernel<_Float16, false>;
+    auto kernel = kernel_of<false>(kv.type, whole);
     hipLaunchKernelGGL(kernel, grid, dim3(PR_THREADS), 0, st, kv, rs, q, out);
+    return (int)hipGetLastError();
+}
+
+int launch_paged_prefix(const PagedKv &kv, const SharedPlan &sp, const float *q, float *parts,
+                        void *stream)
+{
+    RowsScratch rs{};
+    rs.plan = sp.plan;
+    rs.pieces = sp.pieces;
+    rs.parts = parts;
+    rs.list = sp.list;
+    rs.tq = sp.tq;
+    rs.cap = sp.cap;
+    rs.most = sp.most;
+    auto kernel = kernel_of<true>(kv.type, 1 << kv.shift >= PR_TILE);
+    hipLaunchKernelGGL(kernel, dim3(sp.most * kv.kvh), dim3(PR_THREADS), 0, (hipStream_t)stream, kv,
+                       rs, q, (float *)nullptr);
     return (int)hipGetLastError();
 }
 

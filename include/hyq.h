@@ -434,6 +434,37 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
                           const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
                           size_t rows, size_t max_rows, size_t heads, const float *q_d,
                           void *scratch_d, size_t scratch_bytes, float *out_d);
+/* ---- prefixes that several slots share ----
+ * Slots that were forked from one another, or that begin with one instruction, name
+ * the same pages for their first positions. hyq_paged_shared_plan_d finds them, once
+ * a step; hyq_paged_shared_attention_d then gives every layer what
+ * hyq_paged_attention_d gives, up to rounding, but reads and multiplies a prefix
+ * once for all slots that share it.
+ *
+ * A group is the slots of one number in group_d ([seqs] int32, negative: in none),
+ * or where that is null those whose first entry is one page; of it, those that have
+ * at most 16 * kv_heads / heads new rows, and at least a page of positions before
+ * them. They are compared with the first of them, and the prefix is as many whole
+ * pages as save the most: pages in common, times the slots but one that have them.
+ * (Ids are compared, not assumed: a wrong group costs time, no result.) The plan
+ * goes by the table, lengths and starts as they are, and holds for attention calls
+ * with the same ones, layout, rows and heads; with others the results are wrong,
+ * without access outside the buffers. plan_d: hyq_paged_shared_plan_bytes bytes (0
+ * for arguments that the call refuses), 16-byte aligned. */
+size_t hyq_paged_shared_plan_bytes(const hyq_kv_layout *kl, size_t rows, size_t heads);
+int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
+                            const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
+                            size_t rows, size_t heads, void *plan_d, size_t plan_bytes);
+/* hyq_paged_attention_d by a plan; its arguments, limits and refusals. The keys and
+ * values of an F32 pool must lie within the f16 range in a shared prefix too.
+ * scratch_d: hyq_paged_shared_attention_scratch_bytes bytes. */
+size_t hyq_paged_shared_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows,
+                                                size_t max_rows, size_t heads);
+int hyq_paged_shared_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d,
+                                 int layer, const int32_t *table_d, const int32_t *len_d,
+                                 const int32_t *start_d, size_t rows, size_t max_rows, size_t heads,
+                                 const void *plan_d, size_t plan_bytes, const float *q_d,
+                                 void *scratch_d, size_t scratch_bytes, float *out_d);
 /* ---- the pages' bookkeeping, on the device ----
  * refs [pages] int32 counts the table entries that name a page; 0: free. The
  * results are exact and the same on every run: free pages are taken lowest id

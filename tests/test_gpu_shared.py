@@ -1,0 +1,389 @@
+"""Attention over prefixes that several slots share, on the GPU: the plan against a
+plain one, the results against the 64-bit forms of tests/paged_ref.py and
+tests/paged_q8_ref.py."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import paged_q8_ref as Q
+import paged_ref as R
+from test_gpu_serving import captured, hip, ok
+
+pytestmark = pytest.mark.gpu
+D = R.D
+KINDS = ["F32", "F16", "Q8"]
+# (heads, kv heads): 1, 2, 3, 4, 8 and 16 query heads per KV head
+HEADS = [(2, 2), (4, 2), (6, 2), (16, 4), (8, 1), (16, 1)]
+
+
+def batch(kind, lens, news, heads, pt, seed, **kw):
+    if kind == "Q8":
+        return Q.BatchQ8(lens, news, *heads, pt, seed=seed, **kw)
+    return R.Batch(lens, news, *heads, pt, kind == "F16", seed=seed, **kw)
+
+
+def layout(hyq, b):
+    kind = hyq.KV_Q8 if hasattr(b, "bytes") else hyq.F16 if b.f16 else hyq.F32
+    return hyq.KvLayout(kind, 1, b.kvh, D, b.pt, b.pages, b.seqs, b.width)
+
+
+class Call:
+    """The plan and the attention of a batch, its buffers filled with NaNs."""
+
+    def __init__(self, hyq, ctx, b, max_rows=None, group=None):
+        self.hyq, self.ctx, self.b, self.L = hyq, ctx, b, hyq.lib()
+        self.most = max_rows or max(1, int(b.news.max()))
+        self.kl = layout(hyq, b)
+        self.k = ctypes.byref(self.kl)
+        self.d = {n: ctx.array(a) for n, a in dict(
+            pool=getattr(b, "bytes", b.pool), table=b.table, len=b.lens, start=b.start,
+            q=b.q).items()}
+        self.group = None if group is None else ctx.array(np.array(group, np.int32))
+        self.np = self.L.hyq_paged_shared_plan_bytes(self.k, b.rows, b.heads)
+        self.ns = self.L.hyq_paged_shared_attention_scratch_bytes(self.k, b.rows, self.most, b.heads)
+        assert self.np and self.ns
+        self.plan = ctx.array(np.full(self.np, 0xFF, np.uint8))
+        self.scratch = ctx.array(np.full(self.ns, 0xFF, np.uint8))
+        self.out = ctx.array(np.full((b.rows, b.heads, D), -7, np.float32))
+
+    def make(self):
+        self.hyq.check(self.L.hyq_paged_shared_plan_d(
+            self.ctx.handle, self.k, self.group.ptr if self.group else None, self.d["table"].ptr,
+            self.d["len"].ptr, self.d["start"].ptr, self.b.rows, self.b.heads, self.plan.ptr,
+            self.np))
+        return self
+
+    def enqueue(self):
+        self.hyq.check(self.L.hyq_paged_shared_attention_d(
+            self.ctx.handle, self.k, self.d["pool"].ptr, 0, self.d["table"].ptr, self.d["len"].ptr,
+            self.d["start"].ptr, self.b.rows, self.most, self.b.heads, self.plan.ptr, self.np,
+            self.d["q"].ptr, self.scratch.ptr, self.ns, self.out.ptr))
+
+    def attend(self):
+        self.enqueue()
+        return self.out.numpy()
+
+    def skips(self):
+        """What the plan leaves to the slots' groups: its [seqs] ints behind the first
+        256 bytes."""
+        return self.plan.numpy()[256:256 + 4 * self.b.seqs].view(np.int32)
+
+
+def plain_skips(b, group=None):
+    few, first = 16 // (b.heads // b.kvh), {}
+    run, lead = np.zeros(b.seqs, int), np.full(b.seqs, -1)
+    own = np.maximum(b.lens - b.news, 0) // b.pt
+    for s in range(b.seqs):
+        page = b.table[s, 0]
+        if not 1 <= b.news[s] <= few or own[s] < 1 or not 0 <= page < b.pages:
+            continue
+        key = page if group is None else group[s]
+        if key < 0:
+            continue
+        lead[s] = first.setdefault(key, s)
+        n = min(own[s], own[lead[s]])
+        same = (b.table[s, :n] == b.table[lead[s], :n]) & (b.table[s, :n] >= 0)
+        same &= b.table[s, :n] < b.pages
+        run[s] = own[s] if lead[s] == s else (n if same.all() else same.argmin())
+    skip = np.zeros(b.seqs, int)
+    for l in set(lead[lead >= 0]):
+        who = np.flatnonzero(lead == l)
+        saves = [(int((run[who] >= run[s]).sum() - 1) * int(run[s]), int(run[s])) for s in who]
+        best = max(saves)
+        if best[0] > 0:
+            skip[who[run[who] >= best[1]]] = best[1] * b.pt
+    return skip
+
+
+def check(b, got, rows=None):
+    want, tol = b.attention()
+    for s in range(b.seqs):
+        for r in range(b.start[s], b.start[s + 1]):
+            err = np.abs(got[r] - want[r]).max(-1)
+            assert np.all(err <= tol[r]), (
+                f"slot {s} (len {b.lens[s]}, {b.news[s]} new) row {r - b.start[s]}: "
+                f"{err.max():.3e} > {tol[r][err.argmax()]:.3e}")
+    assert np.all(got[b.new:] == -7), "rows behind the last slot changed"
+
+
+def share(b, members, pages):
+    """Slots of `members` name the pages of the first of them for their first ones."""
+    for s in members[1:]:
+        b.table[s, :pages] = b.table[members[0], :pages]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("pt", [16, 64, 256])
+def test_a_group(gpu_ctx, hyq, heads, pt, kind):
+    """Slots of one to as many new rows as the form takes behind three common pages,
+    their own parts of one position up to pages, a slot beside them."""
+    few = 16 // (heads[0] // heads[1])
+    news = [1, few, 1, max(1, few // 2), 1, 1]
+    lens = [3 * pt + x + n for x, n in zip([0, 5, pt, 70, 1, 0], news)]
+    lens[5] = 40
+    b = batch(kind, lens, news, heads, pt, seed=pt + heads[0], tail=2)
+    share(b, [0, 1, 2, 3, 4], 3)
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.array_equal(c.skips(), [3 * pt] * 5 + [0])
+    check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pt", [16, 32, 64])
+def test_groups_beside_others(gpu_ctx, hyq, pt, kind):
+    """Several groups mixed among slots without new rows, prompts, slots of one page
+    in common, slots without pages, and prefixes that are no whole steps."""
+    r = np.random.default_rng(pt)
+    news = r.choice([1, 1, 2, 0, 4, 30], 40)
+    lens = news + 5 * pt + r.integers(0, 90, 40)
+    lens[7], lens[8] = news[7], 0
+    news[8] = 0
+    b = batch(kind, lens, news, (8, 2), pt, seed=pt, tail=3)
+    share(b, list(range(0, 40, 4)), 5)
+    share(b, list(range(1, 40, 4)), 3)
+    share(b, list(range(2, 40, 8)), 1)
+    b.table[30, :] = -1
+    c = Call(hyq, gpu_ctx, b).make()
+    want = plain_skips(b)
+    assert (want > 0).sum() > 10 and np.array_equal(c.skips(), want)
+    check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_more_rows_than_a_block(gpu_ctx, hyq, kind):
+    """A group whose rows fill several blocks, a long prefix cut into many pieces, slot
+    borders inside blocks."""
+    news = [3, 1, 2, 5] * 20
+    b = batch(kind, [1300 + n + i for i, n in enumerate(news)], news, (3, 1), 32, seed=4, tail=1)
+    share(b, list(range(80)), 40)
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.all(c.skips() == 40 * 32)
+    check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_the_prefix_that_saves_most(gpu_ctx, hyq, kind):
+    """One instruction of a page before several requests' beams: beams that share more
+    with the first slot are taken, if they save more; and by groups, each request's."""
+    b = batch(kind, [700] * 9, [1] * 9, (4, 2), 64, seed=6)
+    share(b, list(range(9)), 1)
+    share(b, [0, 1, 2], 9)
+    share(b, [3, 4, 5], 8)
+    share(b, [6, 8], 7)
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.array_equal(c.skips(), [576] * 3 + [0] * 6)  # 18 pages against 8
+    check(b, c.attend())
+    group = [5, 5, 5, 70000, 70000, 70000, 2, -1, 2]
+    c = Call(hyq, gpu_ctx, b, group=group).make()
+    assert np.array_equal(c.skips(), [576] * 3 + [512] * 3 + [448, 0, 448])
+    assert np.array_equal(c.skips(), plain_skips(b, group))
+    check(b, c.attend())
+    # a group that has nothing in common, and one of a single slot
+    c = Call(hyq, gpu_ctx, b, group=[-1, -1, 1, 1, 9, 9, -3, 4, 3]).make()
+    assert np.array_equal(c.skips(), plain_skips(b, [-1, -1, 1, 1, 9, 9, -3, 4, 3]))
+    check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_pages_missing_in_a_prefix(gpu_ctx, hyq, kind):
+    """Entries that name no page end what slots have in common."""
+    b = batch(kind, [500] * 4, [2] * 4, (4, 1), 32, seed=7)
+    share(b, [0, 1, 2, 3], 15)
+    b.table[:, 4] = -1
+    b.table[:, 9] = b.pages + 3
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.all(c.skips() == 4 * 32)
+    check(b, c.attend())
+    b.table[:, 0] = -1
+    c = Call(hyq, gpu_ctx, b).make()
+    assert not c.skips().any()
+    check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_far_scores(gpu_ctx, hyq, kind):
+    """All weight in the prefix, and all behind it."""
+    for size in (30.0, -30.0):
+        b = batch(kind, [260] * 3, [1] * 3, (2, 1), 64, seed=8)
+        share(b, [0, 1, 2], 3)
+        b.q[:] = 0
+        b.q[:, :, 0] = size
+        if kind == "Q8":
+            b.codes[..., 0] = 0
+            b.codes[b.table[0, :3], 0, :, :, 0] = 100
+            b.bytes = Q.join(b.codes, b.scales)
+        else:
+            used = ~np.isnan(b.pool[:, 0, :, :, 0])
+            b.pool[:, 0, :, :, 0][used] = 0
+            b.pool[b.table[0, :3], 0, :, :, 0] = 3
+        check(b, Call(hyq, gpu_ctx, b).make().attend())
+
+
+def test_numbers_that_are_not_finite(gpu_ctx, hyq):
+    """A NaN in a common page reaches all its slots, one in a slot's own page that one."""
+    for kind in KINDS:
+        b = batch(kind, [200] * 4, [1] * 4, (4, 2), 32, seed=9)
+        share(b, [0, 1, 2], 5)
+        clean = Call(hyq, gpu_ctx, b).make().attend()
+        for page, at, rows in ((b.table[0, 2], 3, [0, 1, 2]), (b.table[1, 6], 1, [1])):
+            if kind == "Q8":
+                kept = b.scales.copy()
+                b.scales[page, 0, 1, at] = np.nan
+                b.bytes = Q.join(b.codes, b.scales)
+            else:
+                kept = b.pool.copy()
+                b.pool[page, 0, 1, at, 7] = np.nan
+            got = Call(hyq, gpu_ctx, b).make().attend()
+            bad = np.zeros((4, 4), bool)
+            bad[rows, 2:] = True
+            assert not np.isfinite(got[bad]).any(), kind
+            assert np.array_equal(got[~bad], clean[~bad]), kind
+            if kind == "Q8":
+                b.scales = kept
+            else:
+                b.pool = kept
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_fewer_rows_than_the_plan_took(gpu_ctx, hyq, kind):
+    """A slot of more new rows than max_rows is left alone, grouped or not."""
+    b = batch(kind, [200, 203, 201, 300], [1, 4, 2, 60], (4, 1), 32, seed=11)
+    share(b, [0, 1, 2], 5)
+    c = Call(hyq, gpu_ctx, b, max_rows=2).make()
+    assert np.array_equal(c.skips(), [160, 160, 160, 0])
+    got, (want, tol) = c.attend(), b.attention()
+    for r in (0, 5, 6):
+        assert np.all(np.abs(got[r] - want[r]).max(-1) <= tol[r])
+    assert np.all(got[1:5] == -7) and np.all(got[7:] == -7)
+
+
+def test_many_slots(gpu_ctx, hyq):
+    """A table of 4096 slots: 512 groups of seven slots and one of its own."""
+    seqs, pt = 4096, 16
+    b = R.Batch([1] * 2, [1] * 2, 2, 2, pt, True, seed=1)
+    r = np.random.default_rng(12)
+    pages = 512 * 3 + seqs
+    b.seqs, b.pages, b.width = seqs, pages, 5
+    b.pool = r.normal(0, 1, (pages, 2, 2, pt, D)).astype(np.float16)
+    b.lens = np.where(np.arange(seqs) % 8 == 7, 9, 3 * pt + 4).astype(np.int32)
+    b.news = np.ones(seqs, np.int32)
+    b.start = np.arange(seqs + 1, dtype=np.int32)
+    b.new = b.rows = seqs
+    b.q = r.normal(0, 1, (seqs, 2, D)).astype(np.float32)
+    b.table = np.full((seqs, 5), -1, np.int32)
+    order = r.permutation(512).repeat(8)
+    for s in range(seqs):
+        if s % 8 < 7:
+            b.table[s, :3] = 3 * order[s] + np.arange(3)
+            b.table[s, 3] = 512 * 3 + s
+        else:
+            b.table[s, 0] = 512 * 3 + s
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.array_equal(c.skips(), np.where(np.arange(seqs) % 8 == 7, 0, 3 * pt))
+    got = c.attend()
+    for s in list(range(0, 24)) + [2047, 2048, 4088, 4095]:
+        for h in range(2):
+            k, v, _ = b.kv(s, h)
+            sc = k @ b.q[s, h].astype(np.float64) / np.sqrt(D)
+            w = np.exp(sc - sc.max())
+            want = (w[:, None] * v).sum(0) / w.sum()
+            tol = R.tolerance((np.abs(k) @ np.abs(b.q[s, h])).max() / np.sqrt(D), np.abs(sc).max(),
+                              np.abs(v).max(), len(k))
+            assert np.abs(got[s, h] - want).max() <= tol
+
+
+def test_a_plan_of_another_batch(gpu_ctx, hyq):
+    """A plan that is not the batch's, and one of any bytes: no access outside."""
+    b = R.Batch([200] * 6, [2] * 6, 8, 2, 32, True, seed=13, tail=3)
+    share(b, [0, 1, 2, 3, 4, 5], 6)
+    c = Call(hyq, gpu_ctx, b).make()
+    plan = c.plan.numpy()
+    c.d["len"].copy_from(np.array([3, 0, 200, 1, 90, 7], np.int32))
+    c.d["start"].copy_from(np.array([0, 1, 1, 9, 9, 10, 11], np.int32))
+    assert np.all(c.attend()[11:] == -7)
+    r = np.random.default_rng(14)
+    for i in range(6):
+        junk = r.integers(0, 256, plan.size).astype(np.uint8)
+        words = junk.view(np.int32)
+        if i % 2:  # (small numbers, which bounds do not cut away)
+            words[:] = r.integers(-3, 40, words.size)
+        words[:2] = [1, r.integers(1, 12)]  # blocks, pieces
+        c.plan.copy_from(junk)
+        assert np.all(c.attend()[11:] == -7)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_cache(gpu_ctx, hyq, kind):
+    """PagedCache: forked slots attend with and without the plan alike; a plan is
+    asked for after each step's pages."""
+    b = batch(kind, [90], [1], (4, 2), 16, seed=16)
+    c = hyq.PagedCache(gpu_ctx, 1, 2, 64, 5, 200, page_tokens=16,
+                       dtype={"F32": hyq.F32, "F16": hyq.F16, "Q8": hyq.KV_Q8}[kind])
+    r = np.random.default_rng(17)
+    one, freq = (gpu_ctx.array(x) for x in (np.ones(D, np.float32),
+                                            (10000.0 ** (-np.arange(64) / 64)).astype(np.float32)))
+    start = gpu_ctx.array(np.zeros(6, np.int32))
+
+    def step(news):
+        first = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+        start.copy_from(first)
+        rows = int(first[-1])
+        x = [gpu_ctx.array(r.normal(0, 1, (rows, n, D)).astype(np.float32)) for n in (4, 2, 2)]
+        out = [gpu_ctx.array(np.full((rows, 4, D), -7, np.float32)) for _ in range(2)]
+        assert not c.extend(news).any()
+        qo = gpu_ctx.empty((rows, 4, D), np.float32)
+        c.append_d(0, start.ptr, rows, 4, *[a.ptr for a in x], one.ptr, one.ptr, freq.ptr, 1e-5,
+                   qo.ptr)
+        with pytest.raises(ValueError, match="share_d"):
+            c.attention_d(0, start.ptr, rows, max(news), 4, qo.ptr, out[0].ptr, shared=True)
+        c.share_d(start.ptr, rows, 4)
+        c.attention_d(0, start.ptr, rows, max(news), 4, qo.ptr, out[0].ptr, shared=True)
+        c.attention_d(0, start.ptr, rows, max(news), 4, qo.ptr, out[1].ptr)
+        a, b = (o.numpy() for o in out)
+        assert np.abs(a - b).max() < 2e-5 and np.abs(a).max() > 0.01
+        return a, b
+
+    step([70, 0, 0, 0, 0])
+    c.fork([0, 0, 0, 0, -1])
+    step([1, 1, 1, 1, 33])
+    a, b = step([1, 2, 1, 3, 1])
+    assert not np.array_equal(a, b)  # (the prefix was summed apart)
+    c.fork([3, 0, 1, 4, 4])
+    step([1, 1, 1, 1, 1])
+
+
+def test_captured(gpu_ctx, hyq):
+    """A captured plan and attention follow the tables of each replay, with eager work
+    between; two graphs with buffers of their own replayed side by side."""
+    other = hyq.Context(0)
+    try:
+        b = R.Batch([200] * 6, [1] * 6, 8, 2, 32, True, seed=18)
+        calls = [Call(hyq, gpu_ctx, b) for _ in range(2)]
+        graphs = [captured(gpu_ctx, lambda: c.make().enqueue()) for c in calls]
+        tables = [b.table.copy() for _ in range(4)]
+        for s in range(6):
+            tables[1][s, :6] = tables[1][0, :6]
+            tables[2][s, :2 + s // 3] = tables[2][s // 3 * 3, :2 + s // 3]
+        tables[3][1, :5] = tables[3][4, :5]
+        for i in range(6):
+            for j, c in enumerate(calls):
+                c.d["table"].copy_from(tables[(i + j) % 4])
+                c.out.copy_from(np.full(c.out.shape, -7, np.float32))
+            gpu_ctx.sync()
+            for (_, run), ctx in zip(graphs, (gpu_ctx, other)):
+                ok(hip("hipGraphLaunch")(run, ctypes.c_void_p(ctx.stream)))
+            other.sync()
+            gpu_ctx.sync()
+            for j, c in enumerate(calls):
+                b.table = tables[(i + j) % 4]
+                check(b, c.out.numpy())
+                eager = Call(hyq, gpu_ctx, b).make().attend()
+                assert np.array_equal(eager, c.out.numpy())
+                assert np.array_equal(c.skips(), plain_skips(b))
+        for graph, run in graphs:
+            ok(hip("hipGraphExecDestroy")(run))
+            ok(hip("hipGraphDestroy")(graph))
+    finally:
+        other.close()
