@@ -207,7 +207,7 @@ size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, s
     if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS || max_rows == 0 ||
         !grid_ok(kl, rows, heads))
         return 0;
-    return paged_attention_scratch(type_of(kl), kl->seqs, kl->kv_heads, (int)heads,
+    return paged_attention_scratch(type_of(kl), false, kl->seqs, kl->kv_heads, (int)heads,
                                    (int)rows, (int)std::min(rows, max_rows));
 }
 
@@ -244,7 +244,7 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
 size_t hyq_paged_shared_plan_bytes(const hyq_kv_layout *kl, size_t rows, size_t heads)
 {
     if (!layout_ok(kl) || !heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS) return 0;
-    return shared_plan_bytes(kl->seqs, kl->kv_heads, (int)heads, (int)rows);
+    return shared_plan_bytes(kl->seqs, kl->kv_heads, (int)heads);
 }
 
 int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
@@ -461,10 +461,11 @@ int hyq_sample_d(hyq_ctx *ctx, const float *logits_d, size_t rows, size_t vocab,
 namespace hyq {
 
 // Scratch: the few-row form's parts, then the tile form's plan and parts.
-size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows)
+size_t paged_attention_scratch(int type, bool shared, int seqs, int kvh, int heads, int rows,
+                               int max_rows)
 {
     const int few = std::min(paged_few_rows(heads / kvh), max_rows);
-    size_t n = paged_few_scratch(type, seqs, kvh, heads, few);
+    size_t n = paged_few_scratch(type, shared, seqs, kvh, heads, few);
     if (max_rows > few) n += rows_layout(seqs, kvh, heads, rows).bytes;
     return n;
 }
@@ -472,26 +473,24 @@ size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows,
 // Behind them, in whole 256 bytes, the prefixes' parts.
 size_t shared_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows)
 {
-    const size_t n = paged_attention_scratch(type, seqs, kvh, heads, rows, max_rows);
-    return (n + 255) / 256 * 256 + shared_parts_bytes(seqs, kvh, heads, rows);
+    const size_t n = paged_attention_scratch(type, true, seqs, kvh, heads, rows, max_rows);
+    return (n + 255) / 256 * 256 + shared_parts_bytes(seqs, kvh, heads);
 }
 
-size_t shared_plan_bytes(int seqs, int kvh, int heads, int rows)
+size_t shared_plan_bytes(int seqs, int kvh, int heads)
 {
-    return shared_layout(seqs, kvh, heads, rows).bytes;
+    return shared_layout(seqs, kvh, heads).bytes;
 }
 
-int launch_paged_attention(const PagedKv &given, int max_rows, const float *q, void *scratch,
+int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void *scratch,
                            const void *plan, float *out, void *stream)
 {
-    PagedKv kv = given;
     SharedPlan sp{};
     float *prefix = nullptr;
     if (plan) {
-        sp = shared_plan(plan, kv.seqs, kv.kvh, kv.heads, kv.rows);
-        kv.skip = sp.skip;
+        sp = shared_plan(plan, kv.seqs, kv.kvh, kv.heads);
         const size_t n =
-            paged_attention_scratch(kv.type, kv.seqs, kv.kvh, kv.heads, kv.rows, max_rows);
+            paged_attention_scratch(kv.type, true, kv.seqs, kv.kvh, kv.heads, kv.rows, max_rows);
         prefix = (float *)((char *)scratch + (n + 255) / 256 * 256);
         const int rc = launch_paged_prefix(kv, sp, q, prefix, stream);
         if (rc) return rc;
@@ -501,7 +500,7 @@ int launch_paged_attention(const PagedKv &given, int max_rows, const float *q, v
     RowsScratch rs{};
     if (max_rows > few) {
         const RowsLayout l = rows_layout(kv.seqs, kv.kvh, kv.heads, kv.rows);
-        char *base = (char *)scratch + paged_few_scratch(kv.type, kv.seqs, kv.kvh, kv.heads, few);
+        char *base = (char *)scratch + paged_few_scratch(kv.type, plan, kv.seqs, kv.kvh, kv.heads, few);
         rs.plan = (Plan *)base;
         rs.blocks = (Block *)(base + l.blocks);
         rs.pieces = (Piece *)(base + l.pieces);
@@ -511,9 +510,10 @@ int launch_paged_attention(const PagedKv &given, int max_rows, const float *q, v
         rs.cap = max_blocks(kv.seqs, kv.rows, rs.tq);
         rs.most = max_rows;
     }
-    int rc = launch_paged_few(kv, few, rs, q, part, out, stream);
+    int rc = launch_paged_few(kv, few, rs, plan ? &sp : nullptr, q, part, out, stream);
     if (rc == 0 && rs.cap) rc = launch_paged_rows(kv, rs, q, out, stream);
-    if (rc == 0) rc = launch_paged_merge(kv, few, rs, part, plan ? &sp : nullptr, prefix, out, stream);
+    if (rc == 0)
+        rc = launch_paged_merge(kv, few, rs, plan ? &sp : nullptr, part, prefix, out, stream);
     return rc;
 }
 

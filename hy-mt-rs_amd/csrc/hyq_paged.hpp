@@ -30,7 +30,6 @@ struct PagedKv {
     const int *table;   // [seqs][stride] page ids, -1 where none
     const int *len;     // [seqs] positions held, the new rows' among them
     const int *start;   // [seqs + 1] first new row of a slot
-    const int *skip;    // [seqs] leading positions that another launch attends, or null
     int type;           // KV_T_*
     int seqs, stride, npages, shift; // page_tokens == 1 << shift
     int kvh, heads, rows;
@@ -44,14 +43,15 @@ int launch_paged_read(const PagedKv &kv, float *k, float *v, void *stream);
 
 // Attention: the one-wave form for slots of few new rows and the tile form for
 // the others; scratch as paged_attention_scratch says.
-size_t paged_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows);
+size_t paged_attention_scratch(int type, bool shared, int seqs, int kvh, int heads, int rows,
+                               int max_rows);
 // plan: of the prefixes that slots share (launch_shared_plan's), or null; their
 // parts lie in the scratch behind what paged_attention_scratch says.
 int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void *scratch,
                            const void *plan, float *out, void *stream);
 
 // The plan of a step's shared prefixes. group: the slots' groups, or null.
-size_t shared_plan_bytes(int seqs, int kvh, int heads, int rows);
+size_t shared_plan_bytes(int seqs, int kvh, int heads);
 size_t shared_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows);
 int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *stream);
 

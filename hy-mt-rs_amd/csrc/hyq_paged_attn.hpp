@@ -96,24 +96,16 @@ template <int TILE> __device__ __forceinline__ int slot_tiles(int positions)
 {
     return max(1, (positions + TILE - 1) / TILE);
 }
-// A slot's leading positions that the few-row form leaves out: whole groups of 16
-// before its new rows.
-template <bool SHARED>
-__device__ __forceinline__ int skipped(const PagedKv &kv, int s, const SlotRows &r)
-{
-    return SHARED ? max(0, min(kv.skip[s], r.len - r.n)) & ~15 : 0;
-}
-template <int TILE, bool SHARED>
-__device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows)
+template <int TILE> __device__ __forceinline__ int few_tiles(const PagedKv &kv, int s, int few_rows)
 {
     const SlotRows r = slot_rows(kv, s);
-    return r.n > 0 && r.n <= few_rows ? slot_tiles<TILE>(r.len - skipped<SHARED>(kv, s, r)) : 0;
+    return r.n > 0 && r.n <= few_rows ? slot_tiles<TILE>(r.len) : 0;
 }
 
 // before[s], in LDS: the tiles of the slots before s over all KV heads, with
 // the total at before[seqs]. 256 threads. (Every workgroup forms it for itself:
 // a launch before this one would cost more than the few loads and barriers.)
-template <int TILE, bool SHARED>
+template <int TILE>
 __device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int max_workers,
                                             long long *before, long long *wsum)
 {
@@ -121,7 +113,7 @@ __device__ __forceinline__ FewPlan few_plan(const PagedKv &kv, int few_rows, int
     long long carry = 0;
     for (int b = 0; b < kv.seqs; b += 256) {
         const int s = b + t;
-        const long long mine = s < kv.seqs ? (long long)few_tiles<TILE, SHARED>(kv, s, few_rows) * kv.kvh : 0;
+        const long long mine = s < kv.seqs ? (long long)few_tiles<TILE>(kv, s, few_rows) * kv.kvh : 0;
         long long v = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -393,80 +385,118 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 
 // ---- prefixes that several slots share ----
 // A group's slots have their first `skip` positions in common, on the same pages.
-// The tokens of the group's slots, one after another, stand in blocks of tq in
-// `list` (block b's at places b * tq ..), and their query rows see those positions
-// whole: the tile form attends them from the first slot's table row, a piece a
-// workgroup, and leaves parts that the merge joins with the slots' own.
+// The tokens of the group's slots stand in blocks of tq in `list` (block b's at b *
+// tq ..), each slot in as many places as the group's widest, so that none lies in
+// two blocks, and their query rows see those positions whole: the tile form attends
+// them from the first slot's table row, a piece a workgroup, and leaves parts that
+// the merge joins with the slots' own. Those are attended by the few-row form, whose
+// pieces, one of a slot and KV head for a worker, the plan lists too.
+constexpr int FEW_PIECES = 3072; // three waves on each SIMD
+// (a slot and KV head has a piece at least)
+inline int few_most(int seqs, int kvh) { return (FEW_PIECES + seqs * kvh + 3) / 4 * 4; }
+struct SharedPlace {
+    int begin, n;     // the slot's rows (n = 0: not of the few-row form)
+    int part, pieces; // of its block (0 pieces: in no group)
+    int row, block;   // its first row there
+    int first, ways;  // its first worker, and its workers for each KV head
+};
+struct FewPiece {
+    int slot, kh, t0, t1;      // tiles of the slot's positions from skip on
+    int begin, n, len, skip;   // the slot's rows and positions
+    int ways, unused[3];
+};
+struct SharedHead {
+    Plan plan;   // blocks, their pieces (as groups)
+    int workers; // of the few-row form, a piece each
+};
 struct SharedPlan {
-    Plan *plan;    // blocks, pieces (as groups)
-    int *skip;     // [seqs] positions that the slot's group attends, 0: none
-    int *place;    // [seqs] the first place of its tokens in the list
-    int *leader;   // [seqs] the first slot of its group, -1: it can be in none
-    int *run;      // [seqs] pages that it has in common with that one
-    int *list;     // [cap * tq] packed rows
-    Block *blocks; // [cap]
-    Piece *pieces; // [most]
-    int tq, cap, most;
+    SharedHead *head;
+    int *leader; // [seqs] the first slot of its group, -1: it can be in none
+    int *run;    // [seqs] pages that it has in common with that one
+    int *skip;   // [seqs] positions that the slot's group attends, 0: none
+    SharedPlace *place; // [seqs]
+    FewPiece *few;      // [few_most]
+    int *list;          // [cap * tq] packed rows, -1 where none
+    Block *blocks;      // [cap]
+    Piece *pieces;      // [most]
+    int tq, cap, most, few_most;
 };
 struct SharedLayout {
-    size_t ints, list, blocks, pieces, bytes;
+    size_t ints, place, few, list, blocks, pieces, bytes;
     int cap, most;
 };
-// (rows: of few-row slots, as many as there can be)
-inline SharedLayout shared_layout(int seqs, int kvh, int heads, int rows)
+inline SharedLayout shared_layout(int seqs, int kvh, int heads)
 {
-    const int rep = heads / kvh, tq = PR_ROWS / rep;
-    const long long few = std::min<long long>(rows, (long long)seqs * (16 / rep));
+    const int tq = PR_ROWS / (heads / kvh);
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     SharedLayout l;
-    l.cap = (int)(few / tq) + seqs / 2 + 1; // (a group has two slots or more)
+    // (a group has two slots or more, a block eight or more but for its last one)
+    l.cap = seqs / 8 + seqs / 2 + 1;
     l.most = l.cap + fill_pieces(kvh);
-    l.ints = up(sizeof(Plan));
-    l.list = l.ints + up((size_t)seqs * 4) * 4;
+    l.ints = up(sizeof(SharedHead));
+    l.place = l.ints + up((size_t)seqs * 4) * 3;
+    l.few = l.place + up((size_t)seqs * sizeof(SharedPlace));
+    l.list = l.few + up((size_t)few_most(seqs, kvh) * sizeof(FewPiece));
     l.blocks = l.list + up((size_t)l.cap * tq * 4);
     l.pieces = l.blocks + up((size_t)l.cap * sizeof(Block));
     l.bytes = l.pieces + up((size_t)l.most * sizeof(Piece));
     return l;
 }
-inline SharedPlan shared_plan(const void *plan, int seqs, int kvh, int heads, int rows)
+inline SharedPlan shared_plan(const void *plan, int seqs, int kvh, int heads)
 {
-    const SharedLayout l = shared_layout(seqs, kvh, heads, rows);
+    const SharedLayout l = shared_layout(seqs, kvh, heads);
     char *base = (char *)const_cast<void *>(plan);
     const size_t each = ((size_t)seqs * 4 + 255) / 256 * 256;
     SharedPlan p;
-    p.plan = (Plan *)base;
+    p.head = (SharedHead *)base;
     p.skip = (int *)(base + l.ints);
-    p.place = (int *)(base + l.ints + each);
-    p.leader = (int *)(base + l.ints + 2 * each);
-    p.run = (int *)(base + l.ints + 3 * each);
+    p.leader = (int *)(base + l.ints + each);
+    p.run = (int *)(base + l.ints + 2 * each);
+    p.place = (SharedPlace *)(base + l.place);
+    p.few = (FewPiece *)(base + l.few);
     p.list = (int *)(base + l.list);
     p.blocks = (Block *)(base + l.blocks);
     p.pieces = (Piece *)(base + l.pieces);
     p.tq = PR_ROWS / (heads / kvh);
     p.cap = l.cap;
     p.most = l.most;
+    p.few_most = few_most(seqs, kvh);
     return p;
 }
-inline size_t shared_parts_bytes(int seqs, int kvh, int heads, int rows)
+inline size_t shared_parts_bytes(int seqs, int kvh, int heads)
 {
-    return (size_t)shared_layout(seqs, kvh, heads, rows).most * kvh * PR_ROWS * PAGED_PART * 4;
+    return (size_t)shared_layout(seqs, kvh, heads).most * kvh * PR_ROWS * PAGED_PART * 4;
+}
+// A worker's piece, cut to what there is: the plan may be of another batch.
+template <int TILE> __device__ __forceinline__ FewPiece few_piece(const PagedKv &kv, const FewPiece *p)
+{
+    FewPiece f = *p;
+    f.slot = min(max(f.slot, 0), kv.seqs - 1);
+    f.kh = min(max(f.kh, 0), kv.kvh - 1);
+    f.begin = min(max(f.begin, 0), kv.rows);
+    f.n = min(max(f.n, 0), kv.rows - f.begin);
+    f.len = (int)min((long long)max(f.len, 0), (long long)kv.stride << kv.shift);
+    f.skip = min(max(f.skip, 0), f.len) & ~15;
+    const int tiles = (f.len - f.skip + TILE - 1) / TILE;
+    f.t0 = min(max(f.t0, 0), max(tiles - 1, 0));
+    f.t1 = min(max(f.t1, f.t0 + 1), max(tiles, 1));
+    return f;
 }
 
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)
 // new rows, with the plan where there is a tile form; and the merge of both.
 int paged_few_rows(int rep);
-size_t paged_few_scratch(int type, int seqs, int kvh, int heads, int few);
-int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
-                     float *out, void *stream);
-// (shared, with its parts: null where no prefix is attended for several slots)
-int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
-                       const SharedPlan *shared, const float *shared_parts, float *out,
-                       void *stream);
+size_t paged_few_scratch(int type, bool shared, int seqs, int kvh, int heads, int few);
+// (sp, and the prefixes' parts: null where there is no plan of shared prefixes)
+int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const SharedPlan *sp,
+                     const float *q, float *part, float *out, void *stream);
+int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const SharedPlan *sp,
+                       const float *part, const float *prefix, float *out, void *stream);
 // hyq_paged_few_q8.hip: the few-row form of 8-bit pages, as launch_paged_few has
 // laid it out.
 int launch_paged_few_q8(const PagedKv &kv, int few, int workers, const RowsScratch &rs,
-                        const float *q, int part_rows, float *part, int2 *shared, float *out,
-                        void *stream);
+                        const SharedPlan *sp, const float *q, int part_rows, float *part,
+                        int2 *shared, float *out, void *stream);
 // hyq_paged_rows.hip: the slots of more.
 int launch_paged_rows(const PagedKv &kv, const RowsScratch &rs, const float *q, float *out,
                       void *stream);

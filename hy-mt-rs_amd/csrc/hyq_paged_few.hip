@@ -257,9 +257,10 @@ template <> struct Ops<_Float16> {
 };
 
 template <class T, bool SHARED>
-__global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
-    PagedKv kv, int few_rows, int max_workers, RowsScratch rs, const float *__restrict__ q,
-    int part_rows, float *__restrict__ part, int2 *__restrict__ shared, float *__restrict__ out)
+__global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_kernel(
+    PagedKv kv, int few_rows, int max_workers, RowsScratch rs, SharedPlan sp,
+    const float *__restrict__ q, int part_rows, float *__restrict__ part,
+    int2 *__restrict__ shared, float *__restrict__ out)
 {
     extern __shared__ long long before[]; // [seqs + 1]
     __shared__ long long wsum[4];
@@ -267,15 +268,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         rows_plan(kv, few_rows, rs, (int *)before);
         return;
     }
-    const FewPlan plan = few_plan<TILE, SHARED>(kv, few_rows, max_workers, before, wsum);
+    FewPlan plan;
+    if constexpr (!SHARED) plan = few_plan<TILE>(kv, few_rows, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be; few workers lie on many CUs: two
     // slots of 1100 positions took 1.5 us longer with four to a workgroup)
-    const int w = __builtin_amdgcn_readfirstlane(blockIdx.x + max_workers / FEW_WAVES *
-                                                                  (threadIdx.x >> 6));
-    if (w >= plan.workers) return;
-    long long at = plan.begin(w);
-    const long long stop = plan.begin(w + 1);
+    // (SHARED: alike on the SIMDs of a CU, whose workgroups are 256 apart)
+    const int w = __builtin_amdgcn_readfirstlane(
+        blockIdx.x + max_workers / FEW_WAVES *
+                         (((threadIdx.x >> 6) + (SHARED ? blockIdx.x >> 8 : 0)) & 3));
+    if (w >= (SHARED ? sp.head->workers : plan.workers)) return;
+    long long at = SHARED ? 0 : plan.begin(w);
+    const long long stop = SHARED ? 1 : plan.begin(w + 1);
     const int rep = kv.heads / kv.kvh;
     const size_t hsize = (size_t)KV_D << kv.shift, psize = 2 * hsize * kv.kvh;
     const int pmask = (1 << kv.shift) - 1;
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
 
     // the slot that holds tile `at`: the last with before[s] <= at
     int s = 0;
-    {
+    if constexpr (!SHARED) {
         int hi = kv.seqs; // before[hi] > at
         while (hi - s > 1) {
             const int mid = (s + hi) >> 1;
@@ -292,16 +296,27 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
         }
     }
     while (at < stop) {
-        while (before[s + 1] <= at) ++s; // slots without tiles
-        s = __builtin_amdgcn_readfirstlane(s); // (what comes from LDS, known to be uniform)
-        const SlotRows sr = slot_rows(kv, s);
-        const int skip = skipped<SHARED>(kv, s, sr);
-        const int tiles = slot_tiles<TILE>(sr.len - skip);
-        const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
-        const int kh = in / tiles, t0 = in % tiles;
-        const int t1 = __builtin_amdgcn_readfirstlane(
-            (int)min((long long)tiles, t0 + (stop - at)));
-        at += t1 - t0;
+        SlotRows sr;
+        int kh, t0, t1, tiles = 0, skip = 0;
+        bool whole; // no other worker's part, and no prefix's, is to be joined
+        if constexpr (SHARED) {
+            const FewPiece f = few_piece<TILE>(kv, sp.few + w);
+            if (f.n > few_rows) return;
+            s = f.slot, kh = f.kh, t0 = f.t0, t1 = f.t1, skip = f.skip;
+            sr = SlotRows{f.begin, f.n, f.len};
+            whole = f.ways == 1 && skip == 0;
+            at = stop;
+        } else {
+            while (before[s + 1] <= at) ++s; // slots without tiles
+            s = __builtin_amdgcn_readfirstlane(s); // (what comes from LDS, known to be uniform)
+            sr = slot_rows(kv, s);
+            tiles = slot_tiles<TILE>(sr.len);
+            const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
+            kh = in / tiles, t0 = in % tiles;
+            t1 = __builtin_amdgcn_readfirstlane((int)min((long long)tiles, t0 + (stop - at)));
+            whole = t0 == 0 && t1 == tiles;
+            at += t1 - t0;
+        }
 
         // this lane's row: token c / rep of the slot's new rows
         const int tok = c / rep;
@@ -418,16 +433,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(
             }
         }
         l = wave::sum_halves(wave::sum_rows2(l));
-        if (t0 == 0 && lane == 0) { // who shares the unit, for the merge
+        if (!SHARED && t0 == 0 && lane == 0) { // who shares the unit, for the merge
             const long long last = before[s] + (long long)(kh + 1) * tiles - 1;
             const int n = t1 == tiles ? 1 : plan.worker(last) - w + 1;
             shared[(size_t)s * kv.kvh + kh] = make_int2(w, n);
         }
-        if (t0 == 0 && t1 == tiles && skip == 0) {
+        if (whole) {
             // (a row that saw nothing gives zeros)
             if (ok) Ops<T>::put(out + row * KV_D, acc, g, l > 0.f || l != l ? 1.f / l : 0.f);
         } else if (ok) {
-            const long long slot = (long long)w + (long long)s * kv.kvh + kh;
+            const long long slot = SHARED ? w : (long long)w + (long long)s * kv.kvh + kh;
             float *o = part + ((size_t)slot * part_rows + c) * PAGED_PART;
             if (g == 0) {
                 o[0] = m;
@@ -505,34 +520,40 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
 {
     __shared__ float red[4][KV_D + 2];
     const int rep = kv.heads / kv.kvh;
-    const int2 by = shared[(size_t)s * kv.kvh + kh]; // (of a slot without rows: anything)
-    const SlotRows sr = slot_rows(kv, s);
+    SlotRows sr;
+    SharedPlace pl{};
+    int w0, n;
+    if constexpr (SHARED) {
+        pl = sp.place[s];
+        sr.begin = min(max(pl.begin, 0), kv.rows);
+        sr.n = min(max(pl.n, 0), kv.rows - sr.begin);
+        pl.part = min(max(pl.part, 0), sp.most - 1);
+        pl.pieces = min(max(pl.pieces, 0), sp.most - pl.part);
+        n = min(max(pl.ways, 0), sp.few_most);
+        w0 = (int)min((long long)max(pl.first, 0) + (long long)kh * n, (long long)sp.few_most);
+        n = min(n, sp.few_most - w0);
+    } else {
+        const int2 by = shared[(size_t)s * kv.kvh + kh]; // (of a slot without rows: anything)
+        sr = slot_rows(kv, s);
+        w0 = by.x, n = by.y;
+    }
     if (sr.n > few_rows || c >= sr.n * rep) return;
-    const int w0 = by.x, n = by.y;
-    const bool grouped = SHARED && skipped<SHARED>(kv, s, sr) > 0;
-    if (n == 1 && !grouped) return; // written whole
+    if (n == 1 && pl.pieces == 0) return; // written whole
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int r = wide ? c : c + g;
     if (!wide && r >= sr.n * rep) return;
     const size_t step = (size_t)part_rows * PAGED_PART;
-    const float *p = part + ((size_t)((long long)w0 + (long long)s * kv.kvh + kh) * part_rows + r) *
-                                PAGED_PART;
+    const long long slot = SHARED ? w0 : (long long)w0 + (long long)s * kv.kvh + kh;
+    const float *p = part + ((size_t)slot * part_rows + r) * PAGED_PART;
     const int a = wide ? n * g / 4 : 0, b = wide ? n * (g + 1) / 4 : n;
     Joined<float2v, 1> j;
     j.add({p + (size_t)a * step}, step, b - a, 2 * lane);
-    if constexpr (SHARED) {
-        if (grouped) { // the prefix's pieces, for this row of its block
-            const int last = sp.cap * sp.tq - 1;
-            const int at = min(min(max(sp.place[s], 0), last) + r / rep, last);
-            const Block blk = sp.blocks[at / sp.tq];
-            const int first = min(max(blk.part, 0), sp.most - 1);
-            const int k = min(max(blk.pieces, 0), sp.most - first);
-            const int c0 = wide ? k * g / 4 : 0, c1 = wide ? k * (g + 1) / 4 : k;
-            const size_t each = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
-            const float *x = prefix + ((size_t)first * kv.kvh + kh) * PR_ROWS * PAGED_PART +
-                             (size_t)(at % sp.tq * rep + r % rep) * PAGED_PART;
-            j.add({x + (size_t)c0 * each}, each, c1 - c0, 2 * lane);
-        }
+    if constexpr (SHARED) { // the prefix's pieces, for this row of its block
+        const int c0 = wide ? pl.pieces * g / 4 : 0, c1 = wide ? pl.pieces * (g + 1) / 4 : pl.pieces;
+        const size_t each = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
+        const float *x = prefix + ((size_t)pl.part * kv.kvh + kh) * PR_ROWS * PAGED_PART +
+                         (size_t)min(min(max(pl.row, 0), PR_ROWS) + r, PR_ROWS - 1) * PAGED_PART;
+        j.add({x + (size_t)c0 * each}, each, c1 - c0, 2 * lane);
     }
     float *o = out + ((size_t)(sr.begin + r / rep) * kv.heads + kh * rep + r % rep) * KV_D;
     if (!wide) {
@@ -621,46 +642,48 @@ int paged_few_rows(int rep) { return 16 / rep; }
 
 namespace {
 
-size_t parts_bytes(int type, int seqs, int kvh, int part_rows)
+size_t parts_bytes(int type, bool shared, int seqs, int kvh, int part_rows)
 {
-    return ((size_t)few_workers(type) + (size_t)seqs * kvh) * part_rows * PAGED_PART * 4;
+    const size_t n = shared ? (size_t)few_most(seqs, kvh) // (a plan's pieces, one a worker)
+                            : (size_t)few_workers(type) + (size_t)seqs * kvh;
+    return n * part_rows * PAGED_PART * 4;
 }
 
 } // namespace
 
 // Parts, then the workers of each slot and KV head.
-size_t paged_few_scratch(int type, int seqs, int kvh, int heads, int few)
+size_t paged_few_scratch(int type, bool shared, int seqs, int kvh, int heads, int few)
 {
-    const size_t shared = ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
-    return parts_bytes(type, seqs, kvh, few * (heads / kvh)) + shared;
+    const size_t units = ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
+    return parts_bytes(type, shared, seqs, kvh, few * (heads / kvh)) + units;
 }
 
-int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const float *q, float *part,
-                     float *out, void *stream)
+int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const SharedPlan *sp,
+                     const float *q, float *part, float *out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
-    int2 *shared = (int2 *)((char *)part + parts_bytes(kv.type, kv.seqs, kv.kvh, part_rows));
+    int2 *shared = (int2 *)((char *)part + parts_bytes(kv.type, sp, kv.seqs, kv.kvh, part_rows));
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
-    const int workers = few_workers(kv.type);
+    const int workers = sp ? sp->few_most : few_workers(kv.type);
     const dim3 grid(workers / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
     if (kv.type == KV_T_Q8)
-        return launch_paged_few_q8(kv, few, workers, rs, q, part_rows, part, shared, out, stream);
-    auto kernel = kv.skip ? paged_few_kernel<float, true> : paged_few_kernel<float, false>;
+        return launch_paged_few_q8(kv, few, workers, rs, sp, q, part_rows, part, shared, out, stream);
+    auto kernel = sp ? paged_few_kernel<float, true> : paged_few_kernel<float, false>;
     if (kv.type == KV_T_F16)
-        kernel = kv.skip ? paged_few_kernel<_Float16, true> : paged_few_kernel<_Float16, false>;
-    hipLaunchKernelGGL(kernel, grid, block, lds, st, kv, few, workers, rs, q, part_rows, part, shared,
-                       out);
+        kernel = sp ? paged_few_kernel<_Float16, true> : paged_few_kernel<_Float16, false>;
+    hipLaunchKernelGGL(kernel, grid, block, lds, st, kv, few, workers, rs, sp ? *sp : SharedPlan{}, q,
+                       part_rows, part, shared, out);
     return (int)hipGetLastError();
 }
 
-int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const float *part,
-                       const SharedPlan *plan, const float *prefix, float *out, void *stream)
+int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const SharedPlan *sp,
+                       const float *part, const float *prefix, float *out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
     const int part_rows = few * (kv.heads / kv.kvh);
     const int2 *shared =
-        (const int2 *)((const char *)part + parts_bytes(kv.type, kv.seqs, kv.kvh, part_rows));
+        (const int2 *)((const char *)part + parts_bytes(kv.type, sp, kv.seqs, kv.kvh, part_rows));
     // Few rows have many parts each (1024 workers over four slots of four KV
     // heads: 64), which all of a workgroup's waves read; many rows have few, and
     // a wave each. Wide and not: four slots of 60001 positions 124 and 134 us,
@@ -668,9 +691,9 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
     const int wide = kv.seqs * kv.kvh * part_rows <= 1024;
     const int each = wide ? part_rows : (part_rows + 3) / 4;
     const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, each, rs.cap));
-    auto kernel = plan ? paged_merge_kernel<true> : paged_merge_kernel<false>;
+    auto kernel = sp ? paged_merge_kernel<true> : paged_merge_kernel<false>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, kv, few, part_rows, wide, rs, part, shared,
-                       plan ? *plan : SharedPlan{}, prefix, out);
+                       sp ? *sp : SharedPlan{}, prefix, out);
     return (int)hipGetLastError();
 }
 

@@ -44,55 +44,57 @@ constexpr int TILE = 32; // positions of a step, two of 16 (a page may end betwe
 constexpr float LIFT = 14.f; // weights go up to 2^LIFT
 
 // A row's queries as 22-bit whole numbers in three signed bytes, lowest first;
-// lane (c, g): row c, dims 32 g + 16 j + b.
+// lane (c, g): row c, dims 64 j + 16 g + b (so that a load of keys takes 64 bytes of
+// a row from four lanes).
 struct Query {
     i32x4 digit[3][2];
     float scale; // of the numbers, with log2(e) / sqrt(128); NaN for a row that is not finite
-    __device__ __forceinline__ void load(const float *row, bool ok, int g)
+    __device__ __forceinline__ void form(const f32x4 (&v)[8], bool ok)
     {
         float x[32];
-        float mx = 0.f, odd = 0.f; // (a sum of x * 0: NaN if one is not finite)
+        float mx = 0.f; // (a NaN stays one)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 v = *reinterpret_cast<const float4 *>(row + 32 * g + 4 * i);
-            const float w[4] = {v.x, v.y, v.z, v.w};
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const float y = ok ? w[b] : 0.f;
-                x[4 * i + b] = y;
-                mx = fmaxf(mx, fabsf(y));
-                odd = fmaf(y, 0.f, odd);
+                x[4 * i + b] = v[i][b];
+                mx = wave::nmax(mx, fabsf(v[i][b]));
             }
-        }
-        mx = wave::max_halves(wave::max_rows2(mx));
-        odd = wave::sum_halves(wave::sum_rows2(odd));
+        int lo, hi;
+        wave::swap32(__builtin_bit_cast(int, wave::nmax_rows2(mx)), lo, hi);
+        mx = wave::nmax(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
         const int e = query_exponent(mx);
-        scale = ldexpf(1.4426950408889634f * 0.08838834764831845f, e - 21) + odd;
-        const float up = ldexpf(1.f, 21 - e);
+        scale = ldexpf(1.4426950408889634f * 0.08838834764831845f, e - 21);
+        if (!(mx < INFINITY)) scale = __builtin_nanf("");
+        const float up = ok ? ldexpf(1.f, 21 - e) : 0.f;
+        // A number is rounded by adding 1.5 * 2^23, whose last bit is 1, and with 128
+        // added to each of its bytes these are the digits but for their upper bits.
+        constexpr unsigned SIGNS = 0x808080u, ONE = 0x4b400000u; // (1.5 * 2^23)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                unsigned d[3] = {0, 0, 0};
+                unsigned n[4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    int n = (int)rintf(x[16 * j + 4 * w + b] * up); // below 2^22 in magnitude
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        const int low = (int)(signed char)n;
-                        d[i] |= (unsigned)(low & 255) << (8 * b);
-                        n = (n - low) >> 8;
-                    }
+                    const float y = fminf(x[16 * j + 4 * w + b] * up, 4194303.f) + 12582912.f;
+                    n[b] = (__builtin_bit_cast(unsigned, y) + (SIGNS - ONE)) ^ SIGNS;
                 }
-#pragma unroll
-                for (int i = 0; i < 3; ++i) digit[i][j][w] = (int)d[i];
+                // the four numbers' bytes 0 and 1, and 2, by pairs; then by fours
+                const unsigned a = __builtin_amdgcn_perm(n[1], n[0], 0x05010400u),
+                               b = __builtin_amdgcn_perm(n[3], n[2], 0x05010400u),
+                               c = __builtin_amdgcn_perm(n[1], n[0], 0x0c0c0602u),
+                               d = __builtin_amdgcn_perm(n[3], n[2], 0x06020c0cu);
+                digit[0][j][w] = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
+                digit[1][j][w] = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+                digit[2][j][w] = (int)(c | d);
             }
     }
 };
 
 // A step's codes and scales of one KV head.
 struct Step {
-    i32x4 k[2][2]; // position 16 t + lane % 16, dims 32 g + 16 j ..
+    i32x4 k[2][2]; // position 16 t + lane % 16, dims 64 j + 16 g ..
     u32x2 v[8];    // position 16 t + 4 g + e (4 t + e), dims 8 (lane % 16) ..
     f32x4 a[2], b[2]; // the scales of positions 16 t + 4 g ..
 };
@@ -113,9 +115,10 @@ __device__ __forceinline__ half2 values(unsigned first, unsigned second, int x)
 }
 
 template <bool SHARED>
-__global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
-    PagedKv kv, int few_rows, int max_workers, RowsScratch rs, const float *__restrict__ q,
-    int part_rows, float *__restrict__ part, int2 *__restrict__ shared, float *__restrict__ out)
+__global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_kernel(
+    PagedKv kv, int few_rows, int max_workers, RowsScratch rs, SharedPlan sp,
+    const float *__restrict__ q, int part_rows, float *__restrict__ part,
+    int2 *__restrict__ shared, float *__restrict__ out)
 {
     extern __shared__ long long before[]; // [seqs + 1]
     __shared__ long long wsum[4];
@@ -123,20 +126,23 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
         rows_plan(kv, few_rows, rs, (int *)before);
         return;
     }
-    const FewPlan plan = few_plan<TILE, SHARED>(kv, few_rows, max_workers, before, wsum);
+    FewPlan plan;
+    if constexpr (!SHARED) plan = few_plan<TILE>(kv, few_rows, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int w = __builtin_amdgcn_readfirstlane(blockIdx.x + max_workers / FEW_WAVES *
-                                                                  (threadIdx.x >> 6));
-    if (w >= plan.workers) return;
-    long long at = plan.begin(w);
-    const long long stop = plan.begin(w + 1);
+    // (SHARED: alike on the SIMDs of a CU, whose workgroups are 256 apart)
+    const int w = __builtin_amdgcn_readfirstlane(
+        blockIdx.x + max_workers / FEW_WAVES *
+                         (((threadIdx.x >> 6) + (SHARED ? blockIdx.x >> 8 : 0)) & 3));
+    if (w >= (SHARED ? sp.head->workers : plan.workers)) return;
+    long long at = SHARED ? 0 : plan.begin(w);
+    const long long stop = SHARED ? 1 : plan.begin(w + 1);
     const int rep = kv.heads / kv.kvh;
     const size_t hsize = (size_t)KV_D << kv.shift; // a head's codes of a page
     const size_t psize = 2 * kv.kvh * (hsize / KV_D * kv_row_bytes(KV_T_Q8));
     const int pmask = (1 << kv.shift) - 1;
 
     int s = 0; // the slot that holds tile `at`: the last with before[s] <= at
-    {
+    if constexpr (!SHARED) {
         int hi = kv.seqs;
         while (hi - s > 1) {
             const int mid = (s + hi) >> 1;
@@ -145,16 +151,27 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
         }
     }
     while (at < stop) {
-        while (before[s + 1] <= at) ++s; // slots without tiles
-        s = __builtin_amdgcn_readfirstlane(s);
-        const SlotRows sr = slot_rows(kv, s);
-        const int skip = skipped<SHARED>(kv, s, sr);
-        const int tiles = slot_tiles<TILE>(sr.len - skip);
-        const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
-        const int kh = in / tiles, t0 = in % tiles;
-        const int t1 = __builtin_amdgcn_readfirstlane(
-            (int)min((long long)tiles, t0 + (stop - at)));
-        at += t1 - t0;
+        SlotRows sr;
+        int kh, t0, t1, tiles = 0, skip = 0;
+        bool whole; // no other worker's part, and no prefix's, is to be joined
+        if constexpr (SHARED) {
+            const FewPiece f = few_piece<TILE>(kv, sp.few + w);
+            if (f.n > few_rows) return;
+            s = f.slot, kh = f.kh, t0 = f.t0, t1 = f.t1, skip = f.skip;
+            sr = SlotRows{f.begin, f.n, f.len};
+            whole = f.ways == 1 && skip == 0;
+            at = stop;
+        } else {
+            while (before[s + 1] <= at) ++s; // slots without tiles
+            s = __builtin_amdgcn_readfirstlane(s);
+            sr = slot_rows(kv, s);
+            tiles = slot_tiles<TILE>(sr.len);
+            const int in = __builtin_amdgcn_readfirstlane((int)(at - before[s]));
+            kh = in / tiles, t0 = in % tiles;
+            t1 = __builtin_amdgcn_readfirstlane((int)min((long long)tiles, t0 + (stop - at)));
+            whole = t0 == 0 && t1 == tiles;
+            at += t1 - t0;
+        }
 
         // this lane's row: token c / rep of the slot's new rows
         const int tok = c / rep;
@@ -162,8 +179,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
         const int head = kh * rep + c % rep;
         const size_t row = (size_t)(sr.begin + (ok ? tok : 0)) * kv.heads + head;
         const int sees = ok ? sr.len - sr.n + tok : -1; // this row's last visible position
+        f32x4 qrow[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            qrow[i] = *reinterpret_cast<const f32x4 *>(q + row * KV_D + 64 * (i >> 2) + 16 * g +
+                                                       4 * (i & 3));
         Query query;
-        query.load(q + row * KV_D, ok, g);
+        query.form(qrow, ok);
         f32x4 acc[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -206,7 +228,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
                 const unsigned char *kb = b + kh * hsize;
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
-                    st.k[t][j] = cached<i32x4, once.value>(kb, (p + c) * KV_D + 32 * g + 16 * j);
+                    st.k[t][j] = cached<i32x4, once.value>(kb, (p + c) * KV_D + 64 * j + 16 * g);
                 st.a[t] = cached<f32x4, once.value>(
                     (const float *)(b + 2 * kv.kvh * hsize) + ((size_t)kh << kv.shift), p + 4 * g);
             }
@@ -320,18 +342,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
         if (alone) stream(std::true_type{});
         else stream(std::false_type{});
         l = wave::sum_halves(wave::sum_rows2(l));
-        if (t0 == 0 && lane == 0) { // who shares the unit, for the merge
+        if (!SHARED && t0 == 0 && lane == 0) { // who shares the unit, for the merge
             const long long last = before[s] + (long long)(kh + 1) * tiles - 1;
             const int n = t1 == tiles ? 1 : plan.worker(last) - w + 1;
             shared[(size_t)s * kv.kvh + kh] = make_int2(w, n);
         }
         float *o, f;
-        if (t0 == 0 && t1 == tiles && skip == 0) {
+        if (whole) {
             // (a row that saw nothing gives zeros)
             o = out + row * KV_D;
             f = l > 0.f || l != l ? top * (512.f / l) : 0.f;
         } else {
-            const long long slot = (long long)w + (long long)s * kv.kvh + kh;
+            const long long slot = SHARED ? w : (long long)w + (long long)s * kv.kvh + kh;
             o = part + ((size_t)slot * part_rows + c) * PAGED_PART;
             if (ok && g == 0) { // (the maximum itself, and weights of at most 1)
                 o[0] = m + LIFT;
@@ -355,14 +377,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_q8_kernel(
 } // namespace
 
 int launch_paged_few_q8(const PagedKv &kv, int few, int workers, const RowsScratch &rs,
-                        const float *q, int part_rows, float *part, int2 *shared, float *out,
-                        void *stream)
+                        const SharedPlan *sp, const float *q, int part_rows, float *part,
+                        int2 *shared, float *out, void *stream)
 {
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
     const dim3 grid(workers / FEW_WAVES + (rs.cap > 0)), block(64 * FEW_WAVES);
-    auto kernel = kv.skip ? paged_few_q8_kernel<true> : paged_few_q8_kernel<false>;
-    hipLaunchKernelGGL(kernel, grid, block, lds, (hipStream_t)stream, kv, few, workers, rs, q,
-                       part_rows, part, shared, out);
+    auto kernel = sp ? paged_few_q8_kernel<true> : paged_few_q8_kernel<false>;
+    hipLaunchKernelGGL(kernel, grid, block, lds, (hipStream_t)stream, kv, few, workers, rs,
+                       sp ? *sp : SharedPlan{}, q, part_rows, part, shared, out);
     return (int)hipGetLastError();
 }
 

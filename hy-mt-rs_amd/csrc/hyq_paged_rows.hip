@@ -385,12 +385,13 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 
         // this lane's query row
         const int r = 32 * rows + c, tl = r / rep;
-        const bool ok = tl < toks;
+        const int listed = PREFIX ? rs.list[tok0 + min(tl, tq - 1)] : 0;
+        const bool ok = tl < toks && listed >= 0;
         const int head = kh * rep + r % rep;
         const int sees = !ok ? -1 : PREFIX ? first - 1 : first + tok0 + tl; // its last visible position
         // the last position that the wave's first row sees, and with it all of them
         const int wave_all = PREFIX ? first - 1 : first + tok0 + min(toks - 1, (32 * rows) / rep);
-        const int packed = PREFIX ? min(max(rs.list[tok0 + (ok ? tl : 0)], 0), kv.rows - 1)
+        const int packed = PREFIX ? min(max(listed, 0), kv.rows - 1)
                                   : piece.begin + tok0 + (ok ? tl : 0);
         const size_t row = (size_t)packed * kv.heads + head;
 
@@ -725,7 +726,7 @@ int launch_paged_prefix(const PagedKv &kv, const SharedPlan &sp, const float *q,
                         void *stream)
 {
     RowsScratch rs{};
-    rs.plan = sp.plan;
+    rs.plan = &sp.head->plan;
     rs.pieces = sp.pieces;
     rs.parts = parts;
     rs.list = sp.list;

@@ -4,7 +4,7 @@
 // A launch of one workgroup per slot finds the first slot of its group and counts
 // the entries that both tables have in common. One workgroup then takes of every
 // group the prefix that saves most, sum over its slots but one of the prefix's
-// pages, numbers the tokens of the slots that have it, and cuts their blocks'
+// pages, gives the slots that have it their places in blocks, and cuts the blocks'
 // steps into pieces that fill the GPU once. Everything is whole numbers, and every
 // slot's place follows from the slots before it, so the plan does not depend on
 // the order in which threads run.
@@ -101,29 +101,37 @@ __device__ __forceinline__ int scan1024(int mine, int &before, int *wsum)
     return all;
 }
 
-// One workgroup.
+// One workgroup. A wave takes a slot at a time where others are counted for it.
 __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few, SharedPlan sp)
 {
     extern __shared__ unsigned long long best[]; // [seqs] of a group's first slot: saving, pages
-    int *lead = (int *)(best + kv.seqs), *run = lead + kv.seqs, *rows = run + kv.seqs,
-        *base = rows + kv.seqs; // [seqs] each
-    __shared__ int wsum[16];
-    const int t = threadIdx.x, n = kv.seqs;
+    // [seqs] each; base: the group's slots, its first block, then a slot's first worker
+    int *run = (int *)(best + kv.seqs), *base = run + kv.seqs;
+    short *lead = (short *)(base + kv.seqs);
+    unsigned char *rows = (unsigned char *)(lead + kv.seqs), *wide = rows + kv.seqs;
+    unsigned *steps = (unsigned *)(best + 3 * kv.seqs); // [cap]
+    constexpr int TRIES = 16;
+    __shared__ int wsum[16], tried[TRIES];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = kv.seqs;
     for (int s = t; s < n; s += 1024) {
         best[s] = 0;
-        lead[s] = sp.leader[s];
+        lead[s] = (short)sp.leader[s];
         run[s] = sp.run[s];
-        rows[s] = lead[s] < 0 ? 0 : slot_rows(kv, s).n;
+        rows[s] = (unsigned char)(lead[s] < 0 ? 0 : slot_rows(kv, s).n);
         base[s] = 0;
     }
     __syncthreads();
     // the saving of a prefix as long as each slot's run, and the largest of a group
-    for (int s = t; s < n; s += 1024) {
-        if (lead[s] < 0 || run[s] < 1) continue;
+    for (int s = wave; s < n; s += 16) {
+        const int l = lead[s], pages = run[s];
+        if (l < 0 || pages < 1) continue;
         int others = -1;
-        for (int x = lead[s]; x < n; ++x) others += lead[x] == lead[s] && run[x] >= run[s];
-        if (others > 0)
-            atomicMax(best + lead[s], (unsigned long long)others * run[s] << 24 | (unsigned)run[s]);
+        for (int b = l; b < n; b += 64) {
+            const int x = min(b + lane, n - 1);
+            others += __popcll(__ballot(b + lane < n && lead[x] == l && run[x] >= pages));
+        }
+        if (lane == 0 && others > 0)
+            atomicMax(best + l, (unsigned long long)others * pages << 24 | (unsigned)pages);
     }
     __syncthreads();
     // the pages that a slot's group attends for it
@@ -131,81 +139,166 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few, 
         const int pages = lead[s] < 0 ? 0 : (int)(best[lead[s]] & 0xffffff);
         return pages > 0 && run[s] >= pages ? pages : 0;
     };
-    // tokens of every group, at its first slot, and its first block
-    for (int s = t; s < n; s += 1024)
-        if (shares(s)) atomicAdd(base + lead[s], rows[s]);
+    // a slot's place among its group's, the group's slots and its widest one's tokens
+    for (int s = wave; s < n; s += 16) {
+        const int l = lead[s], pages = shares(s);
+        int before = 0, all = 0, most = 0;
+        if (pages)
+            for (int b = l; b < n; b += 64) {
+                const int x = min(b + lane, n - 1);
+                const bool in = b + lane < n && lead[x] == l && run[x] >= pages;
+                before += __popcll(__ballot(in && x < s));
+                all += __popcll(__ballot(in));
+                most = max(most, in ? (int)rows[x] : 0);
+            }
+        if (lane == 0) {
+            sp.skip[s] = pages << kv.shift;
+            sp.place[s].block = before;
+        }
+        if (l != s || !pages) continue;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+        if (lane == 0) {
+            base[s] = all;
+            wide[s] = (unsigned char)most;
+        }
+    }
     __syncthreads();
     int blocks = 0;
     for (int b = 0; b < n; b += 1024) {
-        const int s = b + t;
-        const int tokens = s < n ? base[s] : 0, mine = (tokens + sp.tq - 1) / sp.tq;
+        const int s = b + t, slots = s < n ? base[s] : 0;
+        const int each = slots ? sp.tq / wide[s] : 1, mine = (slots + each - 1) / each;
         int before;
         const int all = scan1024(mine, before, wsum);
         const int first = blocks + before;
-        for (int i = 0; i < mine && first + i < sp.cap; ++i)
-            sp.blocks[first + i] =
-                Block{s, min(sp.tq, tokens - i * sp.tq), 0, shares(s) << kv.shift};
+        for (int i = 0; i < mine && first + i < sp.cap; ++i) {
+            const int pages = shares(s);
+            sp.blocks[first + i] = Block{s, min(each, slots - i * each) * wide[s], 0, 0};
+            steps[first + i] = (((unsigned)pages << kv.shift) + PR_TILE - 1) / PR_TILE;
+        }
         if (s < n) base[s] = first;
         blocks += all;
     }
-    blocks = min(blocks, sp.cap); // (starts that do not ascend could claim rows twice)
+    blocks = min(blocks, sp.cap);
     __syncthreads();
     for (int s = t; s < n; s += 1024) {
-        const int pages = shares(s);
-        int at = 0;
-        if (pages) {
-            at = base[lead[s]] * sp.tq;
-            for (int x = lead[s]; x < s; ++x) at += lead[x] == lead[s] && run[x] >= pages ? rows[x] : 0;
-            const int begin = slot_rows(kv, s).begin;
-            for (int i = 0; i < rows[s]; ++i)
-                if (at + i < sp.cap * sp.tq) sp.list[at + i] = begin + i;
-        }
-        sp.place[s] = at;
-        sp.skip[s] = pages << kv.shift;
+        if (!shares(s)) continue;
+        const int l = lead[s], each = sp.tq / wide[l], rank = sp.place[s].block;
+        const int b = min(base[l] + rank / each, sp.cap - 1), at = rank % each * wide[l];
+        const int begin = slot_rows(kv, s).begin;
+        for (int i = 0; i < wide[l]; ++i)
+            sp.list[b * sp.tq + at + i] = i < rows[s] ? begin + i : -1;
+        sp.place[s].row = at * (kv.heads / kv.kvh);
+        sp.place[s].block = b;
     }
-    __threadfence_block();
+    // Pieces of at most `each` steps: the least, of sixteen lengths, with which they
+    // number no more than fill the GPU once, or the last one, of which that is sure
+    // unless the blocks alone are many.
+    int count = 0;
+    for (int b = t; b < blocks; b += 1024) count += (int)steps[b];
+    int unused;
+    const int total = scan1024(count, unused, wsum);
+    const int fill = fill_pieces(kv.kvh), room = max(fill - blocks, (fill + 1) / 2);
+    const int least = max(PR_MIN_TILES, (total + fill - 1) / fill);
+    const int most = max(least, (total + room - 1) / room);
+    auto length = [&](int i) { return least + (int)((long long)(most - least) * i / (TRIES - 1)); };
+    int pieces = 0;
+    for (int b = lane; b < blocks; b += 64) pieces += ((int)steps[b] - 1) / length(wave) + 1;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) pieces += __shfl_xor(pieces, o, 64);
+    if (lane == 0) tried[wave] = pieces;
     __syncthreads();
-    // Pieces of at most `each` steps, so many that they fill the GPU once beside
-    // the blocks' last ones (rounded up, a piece a block more than that at most).
-    auto steps_of = [&](int b) { return (sp.blocks[b].pieces + PR_TILE - 1) / PR_TILE; };
-    long long steps = 0;
-    for (int b = 0; b < blocks; b += 1024) {
-        int before;
-        steps += scan1024(b + t < blocks ? steps_of(b + t) : 0, before, wsum);
-    }
-    const int fill = fill_pieces(kv.kvh);
-    const int each = max(PR_MIN_TILES, divide(steps + fill - 1, fill));
+    int each = most;
+    for (int i = TRIES - 1; i >= 0; --i)
+        if (tried[i] <= fill) each = length(i);
     int parts = 0;
     for (int b = 0; b < blocks; b += 1024) {
         Block blk{};
         int x = 0, k = 0, before;
         if (b + t < blocks) {
             blk = sp.blocks[b + t];
-            x = steps_of(b + t);
-            k = (x + each - 1) / each;
+            x = (int)steps[b + t];
+            k = (x - 1) / each + 1;
         }
         const int all = scan1024(k, before, wsum);
         for (int i = 0; i < k; ++i)
-            sp.pieces[parts + before + i] =
-                Piece{blk.row, b + t, divide((long long)x * i, k), divide((long long)x * (i + 1), k),
-                      parts + before + i, 0, blk.toks, blk.pieces};
+            sp.pieces[parts + before + i] = Piece{
+                blk.row, b + t, (int)((long long)x * i / k), (int)((long long)x * (i + 1) / k),
+                parts + before + i, 0, blk.toks, shares(blk.row) << kv.shift};
         if (k) sp.blocks[b + t] = Block{blk.row, blk.toks, parts + before, k};
         parts += all;
     }
-    if (t == 0) *sp.plan = Plan{blocks, parts};
+    // The slots' own positions, by the few-row form: pieces of at most `length` tiles,
+    // so long that they number FEW_PIECES at most (or half as many beside a piece for
+    // each slot and head, where those are many).
+    const int tile = kv.type == KV_T_Q8 ? 32 : 16;
+    auto tiles_of = [&](const SlotRows &r, int s) {
+        const int skip = shares(s) << kv.shift;
+        return r.n < 1 || r.n > few ? 0 : max(1, (r.len - skip + tile - 1) / tile);
+    };
+    long long all = 0;
+    int units = 0;
+    for (int b = 0; b < n; b += 1024) {
+        const int own = b + t < n ? tiles_of(slot_rows(kv, b + t), b + t) : 0;
+        int before;
+        all += scan1024(own, before, wsum);
+        units += __syncthreads_count(own > 0);
+    }
+    all *= kv.kvh;
+    units *= kv.kvh;
+    const int spread = max(FEW_PIECES - units, FEW_PIECES / 2);
+    const long long piece = max(1ll, (all + spread - 1) / spread);
+    int workers = 0;
+    for (int b = 0; b < n; b += 1024) {
+        const int s = b + t;
+        const SlotRows r = s < n ? slot_rows(kv, s) : SlotRows{};
+        const int own = s < n ? tiles_of(r, s) : 0;
+        const int ways = (int)((own + piece - 1) / piece);
+        int before;
+        const int in_all = scan1024(ways * kv.kvh, before, wsum);
+        if (s < n) {
+            SharedPlace p{r.begin, own ? r.n : 0, 0, 0, 0, 0, workers + before, ways};
+            if (shares(s)) {
+                const SharedPlace at = sp.place[s];
+                const Block blk = sp.blocks[at.block];
+                p.part = blk.part, p.pieces = blk.pieces, p.row = at.row, p.block = at.block;
+            }
+            sp.place[s] = p;
+            base[s] = workers + before;
+        }
+        workers += in_all;
+    }
+    __syncthreads();
+    for (int w = t; w < min(workers, sp.few_most); w += 1024) {
+        int s = 0, hi = n; // the last slot with base[s] <= w
+        while (hi - s > 1) {
+            const int mid = (s + hi) >> 1;
+            if (base[mid] <= w) s = mid;
+            else hi = mid;
+        }
+        const SlotRows r = slot_rows(kv, s);
+        const int own = tiles_of(r, s), ways = (int)((own + piece - 1) / piece);
+        if (!ways) continue; // (there is none such: the last slot before w has pieces)
+        const int kh = (w - base[s]) / ways, i = (w - base[s]) % ways;
+        sp.few[w] = FewPiece{s,       kh,  (int)((long long)own * i / ways),
+                             (int)((long long)own * (i + 1) / ways),
+                             r.begin, r.n, r.len,
+                             shares(s) << kv.shift, ways, {}};
+    }
+    if (t == 0) *sp.head = SharedHead{Plan{blocks, parts}, min(workers, sp.few_most)};
 }
 
 } // namespace
 
 int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *stream)
 {
-    const SharedPlan sp = shared_plan(plan, kv.seqs, kv.kvh, kv.heads, kv.rows);
+    const SharedPlan sp = shared_plan(plan, kv.seqs, kv.kvh, kv.heads);
     const int few = paged_few_rows(kv.heads / kv.kvh);
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(shared_runs_kernel, dim3(kv.seqs), dim3(256), 0, st, kv, group, few,
                        sp.leader, sp.run);
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(1024), (size_t)kv.seqs * 24, st, kv, few,
-                       sp);
+    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(1024),
+                       (size_t)kv.seqs * 24 + (size_t)sp.cap * 4, st, kv, few, sp);
     return (int)hipGetLastError();
 }
 
