@@ -391,14 +391,15 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 // them from the first slot's table row, a piece a workgroup, and leaves parts that
 // the merge joins with the slots' own. Those are attended by the few-row form, whose
 // pieces, one of a slot and KV head for a worker, the plan lists too.
-constexpr int FEW_PIECES = 3072; // three waves on each SIMD
+constexpr int FEW_PIECES = 2048; // two waves on each SIMD
 // (a slot and KV head has a piece at least)
 inline int few_most(int seqs, int kvh) { return (FEW_PIECES + seqs * kvh + 3) / 4 * 4; }
 struct SharedPlace {
     int begin, n;     // the slot's rows (n = 0: not of the few-row form)
     int part, pieces; // of its block (0 pieces: in no group)
-    int row, block;   // its first row there
+    int row;          // its first row there
     int first, ways;  // its first worker, and its workers for each KV head
+    int unused;
 };
 struct FewPiece {
     int slot, kh, t0, t1;      // tiles of the slot's positions from skip on
@@ -417,12 +418,11 @@ struct SharedPlan {
     SharedPlace *place; // [seqs]
     FewPiece *few;      // [few_most]
     int *list;          // [cap * tq] packed rows, -1 where none
-    Block *blocks;      // [cap]
     Piece *pieces;      // [most]
     int tq, cap, most, few_most;
 };
 struct SharedLayout {
-    size_t ints, place, few, list, blocks, pieces, bytes;
+    size_t ints, place, few, list, pieces, bytes;
     int cap, most;
 };
 inline SharedLayout shared_layout(int seqs, int kvh, int heads)
@@ -437,8 +437,7 @@ inline SharedLayout shared_layout(int seqs, int kvh, int heads)
     l.place = l.ints + up((size_t)seqs * 4) * 3;
     l.few = l.place + up((size_t)seqs * sizeof(SharedPlace));
     l.list = l.few + up((size_t)few_most(seqs, kvh) * sizeof(FewPiece));
-    l.blocks = l.list + up((size_t)l.cap * tq * 4);
-    l.pieces = l.blocks + up((size_t)l.cap * sizeof(Block));
+    l.pieces = l.list + up((size_t)l.cap * tq * 4);
     l.bytes = l.pieces + up((size_t)l.most * sizeof(Piece));
     return l;
 }
@@ -455,7 +454,6 @@ inline SharedPlan shared_plan(const void *plan, int seqs, int kvh, int heads)
     p.place = (SharedPlace *)(base + l.place);
     p.few = (FewPiece *)(base + l.few);
     p.list = (int *)(base + l.list);
-    p.blocks = (Block *)(base + l.blocks);
     p.pieces = (Piece *)(base + l.pieces);
     p.tq = PR_ROWS / (heads / kvh);
     p.cap = l.cap;

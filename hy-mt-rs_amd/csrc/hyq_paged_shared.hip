@@ -2,7 +2,7 @@
 // them once: the plan of hyq_paged_shared_attention_d, made on the device.
 //
 // A launch of one workgroup per slot finds the first slot of its group and counts
-// the entries that both tables have in common. One workgroup then takes of every
+// the entries that both tables have in common. A second launch takes of every
 // group the prefix that saves most, sum over its slots but one of the prefix's
 // pages, gives the slots that have it their places in blocks, and cuts the blocks'
 // steps into pieces that fill the GPU once. Everything is whole numbers, and every
@@ -91,201 +91,264 @@ __device__ __forceinline__ int scan1024(int mine, int &before, int *wsum)
     __syncthreads();
     if (lane == 63) wsum[wave] = v;
     __syncthreads();
-    int base = 0, all = 0;
+    int u = wsum[lane & 15]; // the waves' sums, summed by each 16 lanes
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        if (w < wave) base += wsum[w];
-        all += wsum[w];
+    for (int o = 1; o < 16; o <<= 1) {
+        const int x = __shfl_up(u, o, 16);
+        if ((lane & 15) >= o) u += x;
     }
-    before = base + v - mine;
-    return all;
+    before = v - mine + (wave ? __builtin_amdgcn_readlane(u, wave - 1) : 0);
+    return __builtin_amdgcn_readlane(u, 15);
 }
 
-// One workgroup. A wave takes a slot at a time where others are counted for it.
+// What the i-th of k pieces takes of x tiles or steps: the first x % k one more.
+__device__ __forceinline__ int2 share(int x, int i, int k)
+{
+    const int q = (int)((unsigned)x / (unsigned)k), more = x - q * k, from = i * q + min(i, more);
+    return make_int2(from, from + q + (i < more));
+}
+// The last of n ascending numbers that is at most x (the first is).
+__device__ __forceinline__ int last_of(const int *a, int n, int x)
+{
+    int s = 0;
+    while (n - s > 1) {
+        const int mid = (s + n) >> 1;
+        if (a[mid] <= x) s = mid;
+        else n = mid;
+    }
+    return s;
+}
+__device__ __forceinline__ int pieces_of(int tiles, int piece)
+{
+    return (int)((unsigned)(tiles + piece - 1) / (unsigned)piece);
+}
+
+// What the plan knows of its slots and blocks, in LDS.
+struct PlanLds {
+    unsigned *key; // [seqs], in whole fours: the group's first slot << 20 | pages in common
+    int *ways;     // (where `key` was) a slot's pieces
+    unsigned long long *best; // [seqs] of a group's first slot: saving, pages
+    int *begin, *len;         // (where `best` was) the slot's rows, its positions
+    int *pages;  // the group's slots with as many pages in common; then those it attends
+    int *first;  // of a group's first slot: its slots, its first block; then a slot's first worker
+    int *wide;   // new rows of the group's slots at most
+    unsigned *steps;     // [cap] a block's steps
+    int *part;           // [cap + 1] its first part
+    int *rank;           // the slot's place in its group, then in its block
+    short *block;        // and that
+    short *of;           // [cap] a block's group
+    unsigned char *rows; // new rows of the slot
+    unsigned char *toks; // [cap] a block's tokens
+    static size_t bytes(int n, int cap)
+    {
+        return (size_t)((n + 3) & ~3) * 4 + (size_t)n * 27 + (size_t)cap * 11 + 4;
+    }
+    __device__ PlanLds(void *at, int n, int cap)
+    {
+        key = (unsigned *)at, ways = (int *)at, begin = (int *)(key + ((n + 3) & ~3));
+        best = (unsigned long long *)begin, len = begin + n, pages = len + n, first = pages + n;
+        wide = first + n, rank = wide + n, steps = (unsigned *)(rank + n);
+        part = (int *)(steps + cap), block = (short *)(part + cap + 1), of = block + n;
+        rows = (unsigned char *)(of + cap), toks = rows + n;
+    }
+    // Adds to into[s], for the slots s of 64 lanes and by 16 waves a share of the keys
+    // each, those of [0, end) of the group of `from` that have as many pages in common.
+    __device__ __forceinline__ void count(unsigned from, int end, int *into) const
+    {
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        const unsigned room = 0xfffffu - (from & 0xfffffu);
+        int n = 0;
+#pragma unroll 1
+        for (int b = 4 * (threadIdx.x >> 6); b < end; b += 64) {
+            const u32x4 k = *(const u32x4 *)(key + b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += b + i < end && k[i] - from <= room;
+        }
+        if (n) atomicAdd(into, n);
+    }
+};
+
+// PLAN_GROUPS workgroups, each of which makes the whole plan for itself; the first
+// one writes it, but for the few-row form's pieces, of which each writes some (2048
+// of them by one workgroup: 6 us of 15). Their time is that of their barriers and of
+// their code, which they find in no cache: what they need is read once, numbers are
+// 32 bits, and few loops are unrolled.
+constexpr int PLAN_GROUPS = 8;
 __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few, SharedPlan sp)
 {
-    extern __shared__ unsigned long long best[]; // [seqs] of a group's first slot: saving, pages
-    // [seqs] each; base: the group's slots, its first block, then a slot's first worker
-    int *run = (int *)(best + kv.seqs), *base = run + kv.seqs;
-    short *lead = (short *)(base + kv.seqs);
-    unsigned char *rows = (unsigned char *)(lead + kv.seqs), *wide = rows + kv.seqs;
-    unsigned *steps = (unsigned *)(best + 3 * kv.seqs); // [cap]
+    extern __shared__ __align__(16) unsigned lds[];
     constexpr int TRIES = 16;
     __shared__ int wsum[16], tried[TRIES];
+    __shared__ unsigned sum[3]; // all blocks' steps; all slots' tiles, and those that have some
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = kv.seqs;
-    for (int s = t; s < n; s += 1024) {
-        best[s] = 0;
-        lead[s] = (short)sp.leader[s];
-        run[s] = sp.run[s];
-        rows[s] = (unsigned char)(lead[s] < 0 ? 0 : slot_rows(kv, s).n);
-        base[s] = 0;
+    const PlanLds x(lds, n, sp.cap);
+    const bool writes = blockIdx.x == 0;
+    constexpr unsigned NONE = 0xfff00000u; // (a group has a page in common at least)
+    if (t < 3) sum[t] = 0;
+#pragma unroll 1
+    for (int s = t; s < ((n + 3) & ~3); s += 1024) {
+        const int l = s < n ? sp.leader[s] : -1;
+        x.key[s] = l < 0 ? NONE : (unsigned)l << 20 | (unsigned)sp.run[s];
+        if (s >= n) break;
+        const SlotRows r = slot_rows(kv, s);
+        x.best[s] = 0;
+        x.rows[s] = (unsigned char)(r.n <= few ? r.n : 0);
+        x.first[s] = x.wide[s] = x.pages[s] = x.rank[s] = 0;
     }
     __syncthreads();
     // the saving of a prefix as long as each slot's run, and the largest of a group
-    for (int s = wave; s < n; s += 16) {
-        const int l = lead[s], pages = run[s];
-        if (l < 0 || pages < 1) continue;
-        int others = -1;
-        for (int b = l; b < n; b += 64) {
-            const int x = min(b + lane, n - 1);
-            others += __popcll(__ballot(b + lane < n && lead[x] == l && run[x] >= pages));
-        }
-        if (lane == 0 && others > 0)
-            atomicMax(best + l, (unsigned long long)others * pages << 24 | (unsigned)pages);
+#pragma unroll 1
+    for (int s = lane; s < n; s += 64)
+        if (x.key[s] != NONE) x.count(x.key[s], n, x.pages + s);
+    __syncthreads();
+#pragma unroll 1
+    for (int s = t; s < n; s += 1024) {
+        const unsigned key = x.key[s], run = key & 0xfffffu;
+        const int others = run ? x.pages[s] - 1 : 0;
+        if (others > 0)
+            atomicMax(x.best + (key >> 20), (unsigned long long)others * run << 24 | run);
     }
     __syncthreads();
-    // the pages that a slot's group attends for it
-    auto shares = [&](int s) {
-        const int pages = lead[s] < 0 ? 0 : (int)(best[lead[s]] & 0xffffff);
-        return pages > 0 && run[s] >= pages ? pages : 0;
-    };
     // a slot's place among its group's, the group's slots and its widest one's tokens
-    for (int s = wave; s < n; s += 16) {
-        const int l = lead[s], pages = shares(s);
-        int before = 0, all = 0, most = 0;
-        if (pages)
-            for (int b = l; b < n; b += 64) {
-                const int x = min(b + lane, n - 1);
-                const bool in = b + lane < n && lead[x] == l && run[x] >= pages;
-                before += __popcll(__ballot(in && x < s));
-                all += __popcll(__ballot(in));
-                most = max(most, in ? (int)rows[x] : 0);
-            }
-        if (lane == 0) {
-            sp.skip[s] = pages << kv.shift;
-            sp.place[s].block = before;
-        }
-        if (l != s || !pages) continue;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
-        if (lane == 0) {
-            base[s] = all;
-            wide[s] = (unsigned char)most;
-        }
+    auto pages_of = [&](unsigned key) {
+        const unsigned run = key & 0xfffffu, pages = run ? (unsigned)x.best[key >> 20] & 0xffffffu : 0;
+        return run >= pages ? pages : 0;
+    };
+#pragma unroll 1
+    for (int s = lane; s < n; s += 64) {
+        const unsigned key = x.key[s], pages = pages_of(key);
+        if (pages) x.count((key & NONE) | pages, s, x.rank + s);
+    }
+#pragma unroll 1
+    for (int s = t; s < n; s += 1024) {
+        const unsigned l = x.key[s] >> 20, pages = pages_of(x.key[s]);
+        x.pages[s] = (int)pages;
+        if (writes) sp.skip[s] = (int)(pages << kv.shift);
+        if (!pages) continue;
+        atomicAdd(x.first + l, 1);
+        atomicMax(x.wide + l, (int)x.rows[s]);
     }
     __syncthreads();
     int blocks = 0;
+#pragma unroll 1
     for (int b = 0; b < n; b += 1024) {
-        const int s = b + t, slots = s < n ? base[s] : 0;
-        const int each = slots ? sp.tq / wide[s] : 1, mine = (slots + each - 1) / each;
+        const int s = b + t, slots = s < n ? x.first[s] : 0;
+        const int each = slots ? sp.tq / x.wide[s] : 1, mine = (slots + each - 1) / each;
         int before;
         const int all = scan1024(mine, before, wsum);
         const int first = blocks + before;
+#pragma unroll 1
         for (int i = 0; i < mine && first + i < sp.cap; ++i) {
-            const int pages = shares(s);
-            sp.blocks[first + i] = Block{s, min(each, slots - i * each) * wide[s], 0, 0};
-            steps[first + i] = (((unsigned)pages << kv.shift) + PR_TILE - 1) / PR_TILE;
+            const unsigned steps = ((x.pages[s] << kv.shift) + PR_TILE - 1) / PR_TILE;
+            x.of[first + i] = (short)s;
+            x.steps[first + i] = steps;
+            x.toks[first + i] = (unsigned char)(min(each, slots - i * each) * x.wide[s]);
+            atomicAdd(&sum[0], steps);
         }
-        if (s < n) base[s] = first;
+        if (s < n) x.first[s] = first;
         blocks += all;
     }
     blocks = min(blocks, sp.cap);
     __syncthreads();
+    // the slots' places in the blocks, and what their own positions are
+    const int tile = kv.type == KV_T_Q8 ? 5 : 4; // (the few-row form's step, as a logarithm)
+    auto tiles_of = [&](int s) {
+        const int own = x.len[s] - (x.pages[s] << kv.shift);
+        return x.rows[s] ? max(1, (own + (1 << tile) - 1) >> tile) : 0;
+    };
+#pragma unroll 1
     for (int s = t; s < n; s += 1024) {
-        if (!shares(s)) continue;
-        const int l = lead[s], each = sp.tq / wide[l], rank = sp.place[s].block;
-        const int b = min(base[l] + rank / each, sp.cap - 1), at = rank % each * wide[l];
-        const int begin = slot_rows(kv, s).begin;
-        for (int i = 0; i < wide[l]; ++i)
-            sp.list[b * sp.tq + at + i] = i < rows[s] ? begin + i : -1;
-        sp.place[s].row = at * (kv.heads / kv.kvh);
-        sp.place[s].block = b;
+        const SlotRows r = slot_rows(kv, s);
+        x.begin[s] = r.begin;
+        x.len[s] = r.len;
+        const int tiles = tiles_of(s);
+        if (tiles) {
+            atomicAdd(&sum[1], (unsigned)min(tiles, (1 << 20) - 1));
+            atomicAdd(&sum[2], 1u);
+        }
+        if (!x.pages[s]) continue;
+        const int l = (int)(x.key[s] >> 20), wide = x.wide[l], each = sp.tq / wide;
+        const int up = x.rank[s] / each, at = (x.rank[s] - up * each) * wide;
+        const int b = min(x.first[l] + up, sp.cap - 1);
+#pragma unroll 1
+        for (int i = 0; writes && i < wide; ++i)
+            sp.list[b * sp.tq + at + i] = i < x.rows[s] ? x.begin[s] + i : -1;
+        x.block[s] = (short)b;
+        x.rank[s] = at; // (its first token's place in the block)
     }
     // Pieces of at most `each` steps: the least, of sixteen lengths, with which they
     // number no more than fill the GPU once, or the last one, of which that is sure
     // unless the blocks alone are many.
-    int count = 0;
-    for (int b = t; b < blocks; b += 1024) count += (int)steps[b];
-    int unused;
-    const int total = scan1024(count, unused, wsum);
-    const int fill = fill_pieces(kv.kvh), room = max(fill - blocks, (fill + 1) / 2);
+    const int total = (int)sum[0], fill = fill_pieces(kv.kvh);
+    const int room = max(fill - blocks, (fill + 1) / 2);
     const int least = max(PR_MIN_TILES, (total + fill - 1) / fill);
     const int most = max(least, (total + room - 1) / room);
-    auto length = [&](int i) { return least + (int)((long long)(most - least) * i / (TRIES - 1)); };
+    const int more = (most - least + TRIES - 2) / (TRIES - 1);
     int pieces = 0;
-    for (int b = lane; b < blocks; b += 64) pieces += ((int)steps[b] - 1) / length(wave) + 1;
+#pragma unroll 1
+    for (int b = lane; b < blocks; b += 64)
+        pieces += pieces_of((int)x.steps[b], least + more * wave);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) pieces += __shfl_xor(pieces, o, 64);
     if (lane == 0) tried[wave] = pieces;
     __syncthreads();
-    int each = most;
-    for (int i = TRIES - 1; i >= 0; --i)
-        if (tried[i] <= fill) each = length(i);
+    const unsigned fits = (unsigned)__ballot(tried[lane & (TRIES - 1)] <= fill) & 0xffffu;
+    const int each = least + more * (fits ? __ffs((int)fits) - 1 : TRIES - 1);
     int parts = 0;
+#pragma unroll 1
     for (int b = 0; b < blocks; b += 1024) {
-        Block blk{};
-        int x = 0, k = 0, before;
-        if (b + t < blocks) {
-            blk = sp.blocks[b + t];
-            x = (int)steps[b + t];
-            k = (x - 1) / each + 1;
-        }
-        const int all = scan1024(k, before, wsum);
-        for (int i = 0; i < k; ++i)
-            sp.pieces[parts + before + i] = Piece{
-                blk.row, b + t, (int)((long long)x * i / k), (int)((long long)x * (i + 1) / k),
-                parts + before + i, 0, blk.toks, shares(blk.row) << kv.shift};
-        if (k) sp.blocks[b + t] = Block{blk.row, blk.toks, parts + before, k};
+        const int at = b + t, steps = at < blocks ? (int)x.steps[at] : 0;
+        int before;
+        const int all = scan1024(pieces_of(steps, each), before, wsum);
+        if (at < blocks) x.part[at] = parts + before;
         parts += all;
     }
-    // The slots' own positions, by the few-row form: pieces of at most `length` tiles,
+    if (t == 0) x.part[blocks] = parts;
+    __syncthreads();
+#pragma unroll 1
+    for (int p = t; writes && p < parts; p += 1024) {
+        const int b = last_of(x.part, blocks, p), s = x.of[b];
+        const int2 by = share((int)x.steps[b], p - x.part[b], x.part[b + 1] - x.part[b]);
+        sp.pieces[p] = Piece{s, b, by.x, by.y, p, 0, x.toks[b], x.pages[s] << kv.shift};
+    }
+    // The slots' own positions, by the few-row form: pieces of at most `piece` tiles,
     // so long that they number FEW_PIECES at most (or half as many beside a piece for
     // each slot and head, where those are many).
-    const int tile = kv.type == KV_T_Q8 ? 32 : 16;
-    auto tiles_of = [&](const SlotRows &r, int s) {
-        const int skip = shares(s) << kv.shift;
-        return r.n < 1 || r.n > few ? 0 : max(1, (r.len - skip + tile - 1) / tile);
-    };
-    long long all = 0;
-    int units = 0;
-    for (int b = 0; b < n; b += 1024) {
-        const int own = b + t < n ? tiles_of(slot_rows(kv, b + t), b + t) : 0;
-        int before;
-        all += scan1024(own, before, wsum);
-        units += __syncthreads_count(own > 0);
-    }
-    all *= kv.kvh;
-    units *= kv.kvh;
-    const int spread = max(FEW_PIECES - units, FEW_PIECES / 2);
-    const long long piece = max(1ll, (all + spread - 1) / spread);
+    const int head = FEW_PIECES / kv.kvh; // pieces of a KV head
+    const int spread = max(head - (int)sum[2], head / 2);
+    const int piece = max(1, pieces_of((int)min(sum[1], 0x7fff0000u), spread));
     int workers = 0;
+#pragma unroll 1
     for (int b = 0; b < n; b += 1024) {
-        const int s = b + t;
-        const SlotRows r = s < n ? slot_rows(kv, s) : SlotRows{};
-        const int own = s < n ? tiles_of(r, s) : 0;
-        const int ways = (int)((own + piece - 1) / piece);
+        const int s = b + t, ways = s < n ? pieces_of(tiles_of(s), piece) : 0;
         int before;
-        const int in_all = scan1024(ways * kv.kvh, before, wsum);
+        const int all = scan1024(ways * kv.kvh, before, wsum);
         if (s < n) {
-            SharedPlace p{r.begin, own ? r.n : 0, 0, 0, 0, 0, workers + before, ways};
-            if (shares(s)) {
-                const SharedPlace at = sp.place[s];
-                const Block blk = sp.blocks[at.block];
-                p.part = blk.part, p.pieces = blk.pieces, p.row = at.row, p.block = at.block;
+            SharedPlace p{x.begin[s], x.rows[s], 0, 0, 0, workers + before, ways, 0};
+            if (x.pages[s]) {
+                const int at = x.block[s];
+                p.part = x.part[at];
+                p.pieces = x.part[at + 1] - p.part;
+                p.row = x.rank[s] * (kv.heads / kv.kvh);
             }
-            sp.place[s] = p;
-            base[s] = workers + before;
+            if (writes) sp.place[s] = p;
+            x.first[s] = workers + before;
+            x.ways[s] = ways;
         }
-        workers += in_all;
+        workers += all;
     }
+    workers = min(workers, sp.few_most);
     __syncthreads();
-    for (int w = t; w < min(workers, sp.few_most); w += 1024) {
-        int s = 0, hi = n; // the last slot with base[s] <= w
-        while (hi - s > 1) {
-            const int mid = (s + hi) >> 1;
-            if (base[mid] <= w) s = mid;
-            else hi = mid;
-        }
-        const SlotRows r = slot_rows(kv, s);
-        const int own = tiles_of(r, s), ways = (int)((own + piece - 1) / piece);
-        if (!ways) continue; // (there is none such: the last slot before w has pieces)
-        const int kh = (w - base[s]) / ways, i = (w - base[s]) % ways;
-        sp.few[w] = FewPiece{s,       kh,  (int)((long long)own * i / ways),
-                             (int)((long long)own * (i + 1) / ways),
-                             r.begin, r.n, r.len,
-                             shares(s) << kv.shift, ways, {}};
+#pragma unroll 1
+    for (int w = blockIdx.x * 256 + t; t < 256 && w < workers; w += PLAN_GROUPS * 256) {
+        const int s = last_of(x.first, n, w), ways = max(1, x.ways[s]); // (a slot that has pieces)
+        const int kh = (int)((unsigned)(w - x.first[s]) / (unsigned)ways);
+        const int2 by = share(tiles_of(s), w - x.first[s] - kh * ways, ways);
+        sp.few[w] = FewPiece{s,          kh,        by.x,     by.y,
+                             x.begin[s], x.rows[s], x.len[s], x.pages[s] << kv.shift,
+                             ways,       {}};
     }
-    if (t == 0) *sp.head = SharedHead{Plan{blocks, parts}, min(workers, sp.few_most)};
+    if (writes && t == 0) *sp.head = SharedHead{Plan{blocks, parts}, workers};
 }
 
 } // namespace
@@ -297,8 +360,8 @@ int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *st
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(shared_runs_kernel, dim3(kv.seqs), dim3(256), 0, st, kv, group, few,
                        sp.leader, sp.run);
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(1024),
-                       (size_t)kv.seqs * 24 + (size_t)sp.cap * 4, st, kv, few, sp);
+    hipLaunchKernelGGL(shared_plan_kernel, dim3(PLAN_GROUPS), dim3(1024),
+                       PlanLds::bytes(kv.seqs, sp.cap), st, kv, few, sp);
     return (int)hipGetLastError();
 }
 
