@@ -129,6 +129,7 @@ SIGNATURES = {
     "hyq_paged_attention_d": (I, [P, P, P, I, P, P, P, SZ, SZ, SZ, P, P, SZ, P]),
     "hyq_paged_shared_plan_bytes": (SZ, [P, SZ, SZ]),
     "hyq_paged_shared_plan_d": (I, [P, P, P, P, P, P, SZ, SZ, P, SZ]),
+    "hyq_paged_shared_plan_least_d": (I, [P, P, P, P, P, P, SZ, SZ, SZ, P, SZ]),
     "hyq_paged_shared_attention_scratch_bytes": (SZ, [P, SZ, SZ, SZ]),
     "hyq_paged_shared_attention_d": (I, [P, P, P, I, P, P, P, SZ, SZ, SZ, P, SZ, P, P, SZ, P]),
     "hyq_pages_fork_d": (I, [P, P, P, P, P, P, P, P, P]),
@@ -845,15 +846,20 @@ class PagedCache:
             buffers.append(self.ctx.empty(max(need, 2 * have, 16), np.uint8))
         return buffers[-1]
 
-    def share_d(self, start_d: int, rows: int, heads: int, group_d: int | None = None) -> None:
+    def share_d(self, start_d: int, rows: int, heads: int, group_d: int | None = None,
+                least: int | None = None) -> None:
         """hyq_paged_shared_plan_d: finds the prefixes that slots share, for the
         ``attention_d`` calls with ``shared`` until the next fork, extension or
-        compaction. Its buffer grows as attention_d's."""
+        compaction; with ``least``, hyq_paged_shared_plan_least_d. Its buffer grows as
+        attention_d's."""
         need = lib().hyq_paged_shared_plan_bytes(self._kl, rows, heads)
         plan = self._grown(self._plans, need)
-        check(lib().hyq_paged_shared_plan_d(
-            self.ctx.handle, self._kl, group_d, self.table.ptr, self._rows_len.ptr, start_d, rows,
-            heads, plan.ptr, plan.nbytes))
+        args = [self.ctx.handle, self._kl, group_d, self.table.ptr, self._rows_len.ptr, start_d,
+                rows, heads]
+        if least is None:
+            check(lib().hyq_paged_shared_plan_d(*args, plan.ptr, plan.nbytes))
+        else:
+            check(lib().hyq_paged_shared_plan_least_d(*args, least, plan.ptr, plan.nbytes))
         self._planned = (start_d, rows, heads)
 
     def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,

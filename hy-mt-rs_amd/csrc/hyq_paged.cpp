@@ -143,6 +143,29 @@ int extend(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, const int32_t *a
     return HYQ_OK;
 }
 
+int shared_plan(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
+                const int32_t *table_d, const int32_t *len_d, const int32_t *start_d, size_t rows,
+                size_t heads, long long least, void *plan_d, size_t plan_bytes)
+{
+    int rc = check_layout(ctx, kl, "paged_shared_plan");
+    if (rc) return rc;
+    if (!table_d || !len_d || !start_d || !plan_d)
+        return fail(HYQ_EINVAL, "paged_shared_plan: null argument");
+    if (!heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS)
+        return fail(HYQ_EINVAL, "paged_shared_plan: %zu rows, heads %zu/%d", rows, heads,
+                    kl->kv_heads);
+    if (!aligned(plan_d)) return fail(HYQ_EINVAL, "paged_shared_plan: the plan is not 16-byte aligned");
+    const size_t need = hyq_paged_shared_plan_bytes(kl, rows, heads);
+    if (plan_bytes < need)
+        return fail(HYQ_EINVAL, "paged_shared_plan: a plan of %zu bytes, %zu needed", plan_bytes,
+                    need);
+    DeviceGuard g(ctx->device);
+    HYQ_LAUNCH(launch_shared_plan(view(kl, nullptr, 0, table_d, len_d, start_d, rows, heads),
+                                  group_d, least, plan_d, ctx->stream),
+               "paged_shared_plan");
+    return HYQ_OK;
+}
+
 } // namespace
 
 extern "C" {
@@ -251,23 +274,26 @@ int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t
                             const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
                             size_t rows, size_t heads, void *plan_d, size_t plan_bytes)
 {
-    int rc = check_layout(ctx, kl, "paged_shared_plan");
-    if (rc) return rc;
-    if (!table_d || !len_d || !start_d || !plan_d)
-        return fail(HYQ_EINVAL, "paged_shared_plan: null argument");
-    if (!heads_ok(kl, heads) || rows == 0 || rows > MAX_ROWS)
-        return fail(HYQ_EINVAL, "paged_shared_plan: %zu rows, heads %zu/%d", rows, heads,
-                    kl->kv_heads);
-    if (!aligned(plan_d)) return fail(HYQ_EINVAL, "paged_shared_plan: the plan is not 16-byte aligned");
-    const size_t need = hyq_paged_shared_plan_bytes(kl, rows, heads);
-    if (plan_bytes < need)
-        return fail(HYQ_EINVAL, "paged_shared_plan: a plan of %zu bytes, %zu needed", plan_bytes,
-                    need);
-    DeviceGuard g(ctx->device);
-    HYQ_LAUNCH(launch_shared_plan(view(kl, nullptr, 0, table_d, len_d, start_d, rows, heads),
-                                  group_d, plan_d, ctx->stream),
-               "paged_shared_plan");
-    return HYQ_OK;
+    // What sharing has to save to be worth its launch and its parts, in positions
+    // times KV heads. One group of slots before 1,024 to 16,384 common positions and
+    // some 50 of their own, with and without it, us, at 16 heads over 4 and 32 over 8:
+    // f16 pages 22 and 24 at 115,000, 22 and 24 at 98,000, 22 and 20 at 61,000, 23 and
+    // 20 at 57,000; f32 25 and 29 at 115,000, 26 and 30 at 98,000, 25 and 22 at 49,000;
+    // 8-bit ones, whose reads are cheaper, 23 and 23 at 229,000, 26 and 30 at 491,000,
+    // 23 and 19 at 123,000.
+    const long long least = kl && kl->dtype == HYQ_KV_Q8 ? 230000 : 90000;
+    return shared_plan(ctx, kl, group_d, table_d, len_d, start_d, rows, heads, least, plan_d,
+                       plan_bytes);
+}
+
+int hyq_paged_shared_plan_least_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
+                                  const int32_t *table_d, const int32_t *len_d,
+                                  const int32_t *start_d, size_t rows, size_t heads, size_t least,
+                                  void *plan_d, size_t plan_bytes)
+{
+    if (least > ((size_t)1 << 62)) least = (size_t)1 << 62;
+    return shared_plan(ctx, kl, group_d, table_d, len_d, start_d, rows, heads, (long long)least,
+                       plan_d, plan_bytes);
 }
 
 size_t hyq_paged_shared_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows,

@@ -53,7 +53,9 @@ int launch_paged_attention(const PagedKv &kv, int max_rows, const float *q, void
 // The plan of a step's shared prefixes. group: the slots' groups, or null.
 size_t shared_plan_bytes(int seqs, int kvh, int heads);
 size_t shared_attention_scratch(int type, int seqs, int kvh, int heads, int rows, int max_rows);
-int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *stream);
+// least: positions times KV heads that it is to save.
+int launch_shared_plan(const PagedKv &kv, const int *group, long long least, void *plan,
+                       void *stream);
 
 struct PagesArgs {
     int type, layers, kvh, shift, npages, seqs, stride;

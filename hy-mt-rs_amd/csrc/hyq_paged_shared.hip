@@ -174,17 +174,19 @@ struct PlanLds {
 // their code, which they find in no cache: what they need is read once, numbers are
 // 32 bits, and few loops are unrolled.
 constexpr int PLAN_GROUPS = 8;
-__global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few, SharedPlan sp)
+__global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
+                                                           long long worth, SharedPlan sp)
 {
     extern __shared__ __align__(16) unsigned lds[];
     constexpr int TRIES = 16;
     __shared__ int wsum[16], tried[TRIES];
-    __shared__ unsigned sum[3]; // all blocks' steps; all slots' tiles, and those that have some
+    // all blocks' steps; all slots' tiles, and those that have some; the groups' saving
+    __shared__ unsigned sum[4];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = kv.seqs;
     const PlanLds x(lds, n, sp.cap);
     const bool writes = blockIdx.x == 0;
     constexpr unsigned NONE = 0xfff00000u; // (a group has a page in common at least)
-    if (t < 3) sum[t] = 0;
+    if (t < 4) sum[t] = 0;
 #pragma unroll 1
     for (int s = t; s < ((n + 3) & ~3); s += 1024) {
         const int l = s < n ? sp.leader[s] : -1;
@@ -209,9 +211,16 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few, 
             atomicMax(x.best + (key >> 20), (unsigned long long)others * run << 24 | run);
     }
     __syncthreads();
+    // (a group's at most 2^20, of 2048 at most)
+#pragma unroll 1
+    for (int s = t; s < n; s += 1024)
+        if (x.best[s]) atomicAdd(&sum[3], min((unsigned)(x.best[s] >> 24), 1u << 20));
+    __syncthreads();
+    const bool shares = ((long long)sum[3] << kv.shift) * kv.kvh >= worth;
     // a slot's place among its group's, the group's slots and its widest one's tokens
     auto pages_of = [&](unsigned key) {
-        const unsigned run = key & 0xfffffu, pages = run ? (unsigned)x.best[key >> 20] & 0xffffffu : 0;
+        const unsigned run = key & 0xfffffu;
+        const unsigned pages = run && shares ? (unsigned)x.best[key >> 20] & 0xffffffu : 0;
         return run >= pages ? pages : 0;
     };
 #pragma unroll 1
@@ -353,7 +362,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few, 
 
 } // namespace
 
-int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *stream)
+int launch_shared_plan(const PagedKv &kv, const int *group, long long least, void *plan,
+                       void *stream)
 {
     const SharedPlan sp = shared_plan(plan, kv.seqs, kv.kvh, kv.heads);
     const int few = paged_few_rows(kv.heads / kv.kvh);
@@ -361,7 +371,7 @@ int launch_shared_plan(const PagedKv &kv, const int *group, void *plan, void *st
     hipLaunchKernelGGL(shared_runs_kernel, dim3(kv.seqs), dim3(256), 0, st, kv, group, few,
                        sp.leader, sp.run);
     hipLaunchKernelGGL(shared_plan_kernel, dim3(PLAN_GROUPS), dim3(1024),
-                       PlanLds::bytes(kv.seqs, sp.cap), st, kv, few, sp);
+                       PlanLds::bytes(kv.seqs, sp.cap), st, kv, few, least, sp);
     return (int)hipGetLastError();
 }
 

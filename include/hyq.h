@@ -446,6 +446,9 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
  * at most 16 * kv_heads / heads new rows, and at least a page of positions before
  * them. They are compared with the first of them, and the prefix is as many whole
  * pages as save the most: pages in common, times the slots but one that have them.
+ * Where all groups together save less than sharing costs (about 90,000 positions
+ * times KV heads, 230,000 in an HYQ_KV_Q8 pool) nothing is shared;
+ * hyq_paged_shared_plan_least_d takes that number from the caller (0: whatever it saves).
  * (Ids are compared, not assumed: a wrong group costs time, no result.) The plan
  * goes by the table, lengths and starts as they are, and holds for attention calls
  * with the same ones, layout, rows and heads; with others the results are wrong,
@@ -455,6 +458,10 @@ size_t hyq_paged_shared_plan_bytes(const hyq_kv_layout *kl, size_t rows, size_t 
 int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
                             const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
                             size_t rows, size_t heads, void *plan_d, size_t plan_bytes);
+int hyq_paged_shared_plan_least_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t *group_d,
+                                  const int32_t *table_d, const int32_t *len_d,
+                                  const int32_t *start_d, size_t rows, size_t heads, size_t least,
+                                  void *plan_d, size_t plan_bytes);
 /* hyq_paged_attention_d by a plan; its arguments, limits and refusals. The keys and
  * values of an F32 pool must lie within the f16 range in a shared prefix too.
  * scratch_d: hyq_paged_shared_attention_scratch_bytes bytes. */

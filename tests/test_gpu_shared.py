@@ -47,11 +47,16 @@ class Call:
         self.scratch = ctx.array(np.full(self.ns, 0xFF, np.uint8))
         self.out = ctx.array(np.full((b.rows + 1, b.heads, D), -7, np.float32))
 
-    def make(self):
-        self.hyq.check(self.L.hyq_paged_shared_plan_d(
-            self.ctx.handle, self.k, self.group.ptr if self.group else None, self.d["table"].ptr,
-            self.d["len"].ptr, self.d["start"].ptr, self.b.rows, self.b.heads, self.plan.ptr,
-            self.np))
+    def make(self, least=0):
+        """(least: None for the rule of the call without it)"""
+        args = [self.ctx.handle, self.k, self.group.ptr if self.group else None,
+                self.d["table"].ptr, self.d["len"].ptr, self.d["start"].ptr, self.b.rows,
+                self.b.heads]
+        if least is None:
+            rc = self.L.hyq_paged_shared_plan_d(*args, self.plan.ptr, self.np)
+        else:
+            rc = self.L.hyq_paged_shared_plan_least_d(*args, least, self.plan.ptr, self.np)
+        self.hyq.check(rc)
         return self
 
     def enqueue(self):
@@ -189,6 +194,31 @@ def test_the_prefix_that_saves_most(gpu_ctx, hyq, kind):
     c = Call(hyq, gpu_ctx, b, group=[-1, -1, 1, 1, 9, 9, -3, 4, 3]).make()
     assert np.array_equal(c.skips(), plain_skips(b, [-1, -1, 1, 1, 9, 9, -3, 4, 3]))
     check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind,least", [("F32", 90000), ("F16", 90000), ("Q8", 230000)])
+def test_what_is_worth_sharing(gpu_ctx, hyq, kind, least):
+    """Nothing is shared where all groups together save less than the given number, or
+    the rule's; the results are the same but for rounding."""
+    b = batch(kind, [150] * 8, [1] * 8, (4, 2), 16, seed=19)
+    share(b, [0, 2, 4], 7)
+    share(b, [1, 5, 6, 7], 5)
+    skips = plain_skips(b)
+    saving = (2 * 7 + 3 * 5) * 16 * 2
+    for n, want in ((0, skips), (saving, skips), (saving + 1, 0), (1 << 63, 0), (None, 0)):
+        c = Call(hyq, gpu_ctx, b).make(n)
+        assert np.all(c.skips() == want), n
+        check(b, c.attend())
+    # the rule at its number: one group of 26 slots over 4 heads (the plan reads no pool)
+    pages = -(-least // (25 * 4 * 16))
+    for n, want in ((pages, pages * 16), (pages - 1, 0)):
+        b = batch(kind, [40] * 26, [1] * 26, (4, 4), 16, seed=20)
+        b.width = pages + 3
+        b.table = np.arange(26 * b.width, dtype=np.int32).reshape(26, -1)
+        b.pages = 26 * b.width
+        b.table[:, :n] = b.table[0, :n]
+        b.lens = np.full(26, n * 16 + 5, np.int32)
+        assert np.all(Call(hyq, gpu_ctx, b).make(None).skips() == want)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -343,7 +373,7 @@ def test_cache(gpu_ctx, hyq, kind):
                    qo.ptr)
         with pytest.raises(ValueError, match="share_d"):
             c.attention_d(0, start.ptr, rows, max(news), 4, qo.ptr, out[0].ptr, shared=True)
-        c.share_d(start.ptr, rows, 4)
+        c.share_d(start.ptr, rows, 4, least=0)
         c.attention_d(0, start.ptr, rows, max(news), 4, qo.ptr, out[0].ptr, shared=True)
         c.attention_d(0, start.ptr, rows, max(news), 4, qo.ptr, out[1].ptr)
         a, b = (o.numpy() for o in out)

@@ -22,6 +22,8 @@ def test_refusals(hyq, dtype):
     calls = {
         "plan": (L.hyq_paged_shared_plan_d, [ctx, k, None, p, p, p, 5, 16, p, plan], [3, 4, 5, 8],
                  [8]),
+        "plan_least": (L.hyq_paged_shared_plan_least_d,
+                       [ctx, k, None, p, p, p, 5, 16, 7, p, plan], [3, 4, 5, 9], [9]),
         "attention": (L.hyq_paged_shared_attention_d,
                       [ctx, k, p, 0, p, p, p, 5, 2, 16, p, plan, p, p, need, p + 64],
                       [2, 4, 5, 6, 10, 12, 13, 15], [2, 10, 12, 13, 15]),
@@ -46,14 +48,17 @@ def test_refusals(hyq, dtype):
         refused(name, b"layout", _1=ctypes.byref(bad2))
     for heads in (0, 6, 68):
         refused("plan", b"heads", _7=heads)
+        refused("plan_least", b"heads", _7=heads)
         refused("attention", b"heads", _9=heads)
     for rows in (0, (1 << 20) + 1):
         refused("plan", b"rows", _6=rows)
+        refused("plan_least", b"rows", _6=rows)
         refused("attention", b"rows", _7=rows)
     refused("attention", b"rows", _8=0)
     for layer in (-1, 2):
         refused("attention", b"layer", _3=layer)
     refused("plan", b"needed", _9=plan - 1)
+    refused("plan_least", b"needed", _10=plan - 1)
     refused("attention", b"plan", _11=plan - 1)
     refused("attention", b"scratch", _14=need - 1)
     refused("attention", b"must not be q", _15=p)
