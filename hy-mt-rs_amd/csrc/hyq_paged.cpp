@@ -274,14 +274,13 @@ int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t
                             const int32_t *table_d, const int32_t *len_d, const int32_t *start_d,
                             size_t rows, size_t heads, void *plan_d, size_t plan_bytes)
 {
-    // What sharing has to save to be worth its launch and its parts, in positions
-    // times KV heads. One group of slots before 1,024 to 16,384 common positions and
-    // some 50 of their own, with and without it, us, at 16 heads over 4 and 32 over 8:
-    // f16 pages 22 and 24 at 115,000, 22 and 24 at 98,000, 22 and 20 at 61,000, 23 and
-    // 20 at 57,000; f32 25 and 29 at 115,000, 26 and 30 at 98,000, 25 and 22 at 49,000;
-    // 8-bit ones, whose reads are cheaper, 23 and 23 at 229,000, 26 and 30 at 491,000,
-    // 23 and 19 at 123,000.
-    const long long least = kl && kl->dtype == HYQ_KV_Q8 ? 230000 : 90000;
+    // What sharing has to save to be worth its parts, in positions times KV heads. One
+    // group of slots before 256 to 4096 common positions and some 50 of their own,
+    // shared and not, us, at 16 heads over 4 and 32 over 8: f16 pages 15 and 14 at
+    // 15,000, 17 and 18 at 32,000, 20 and 20 at 57,000, 21 and 24 at 125,000; f32 17 and
+    // 16 at 28,000, 19 and 21 at 63,000, 22 and 30 at 98,000; 8-bit ones, whose reads
+    // are cheaper, 18 and 19 at 63,000, 21 and 20 at 120,000, 22 and 23 at 237,000.
+    const long long least = kl && kl->dtype == HYQ_KV_Q8 ? 120000 : 50000;
     return shared_plan(ctx, kl, group_d, table_d, len_d, start_d, rows, heads, least, plan_d,
                        plan_bytes);
 }

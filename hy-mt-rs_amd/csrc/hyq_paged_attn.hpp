@@ -385,30 +385,46 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 
 // ---- prefixes that several slots share ----
 // A group's slots have their first `skip` positions in common, on the same pages.
-// The tokens of the group's slots stand in blocks of tq in `list` (block b's at b *
-// tq ..), each slot in as many places as the group's widest, so that none lies in
-// two blocks, and their query rows see those positions whole: the tile form attends
-// them from the first slot's table row, a piece a workgroup, and leaves parts that
-// the merge joins with the slots' own. Those are attended by the few-row form, whose
-// pieces, one of a slot and KV head for a worker, the plan lists too.
+// The tokens of the group's slots stand in blocks in `list`, each slot in as many
+// places as the group's widest, so that none lies in two blocks, and their query
+// rows see those positions whole. Blocks of 16 rows are attended by the few-row form
+// beside the slots' own positions (narrow), where they are many blocks of 128 rows by
+// the tile form in a launch of its own, both from the first slot's table row. They
+// leave parts that the merge joins with the slots' own. The plan lists the pieces of
+// both forms, one of a block or a slot and of one KV head for a worker of the few-row
+// form.
 constexpr int FEW_PIECES = 2048; // two waves on each SIMD
 // (a slot and KV head has a piece at least)
-inline int few_most(int seqs, int kvh) { return (FEW_PIECES + seqs * kvh + 3) / 4 * 4; }
+inline int shared_cap(int seqs)
+{
+    // (a group has two slots or more, a block of the tile form eight or more but for
+    // its last one)
+    return seqs / 8 + seqs / 2 + 1;
+}
+inline int few_most(int seqs, int kvh)
+{
+    constexpr int LOT = 256 * FEW_WAVES; // (whole ones: a workgroup on each CU)
+    return (FEW_PIECES + (seqs + shared_cap(seqs)) * kvh + LOT - 1) / LOT * LOT;
+}
 struct SharedPlace {
     int begin, n;     // the slot's rows (n = 0: not of the few-row form)
-    int part, pieces; // of its block (0 pieces: in no group)
-    int row;          // its first row there
+    int part, pieces; // of its block (0 pieces: in no group); narrow: its first worker and
+                      // its workers for each KV head
+    int row;          // the slot's first row there
     int first, ways;  // its first worker, and its workers for each KV head
     int unused;
 };
 struct FewPiece {
     int slot, kh, t0, t1;      // tiles of the slot's positions from skip on
     int begin, n, len, skip;   // the slot's rows and positions
-    int ways, unused[3];
+    int ways;                  // pieces of the slot
+    int narrow;                // a block: n places of the list from begin on, len positions
+    int unused[2];
 };
 struct SharedHead {
     Plan plan;   // blocks, their pieces (as groups)
     int workers; // of the few-row form, a piece each
+    int narrow;  // blocks of 16 rows
 };
 struct SharedPlan {
     SharedHead *head;
@@ -430,8 +446,7 @@ inline SharedLayout shared_layout(int seqs, int kvh, int heads)
     const int tq = PR_ROWS / (heads / kvh);
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     SharedLayout l;
-    // (a group has two slots or more, a block eight or more but for its last one)
-    l.cap = seqs / 8 + seqs / 2 + 1;
+    l.cap = shared_cap(seqs);
     l.most = l.cap + fill_pieces(kvh);
     l.ints = up(sizeof(SharedHead));
     l.place = l.ints + up((size_t)seqs * 4) * 3;
@@ -466,13 +481,17 @@ inline size_t shared_parts_bytes(int seqs, int kvh, int heads)
     return (size_t)shared_layout(seqs, kvh, heads).most * kvh * PR_ROWS * PAGED_PART * 4;
 }
 // A worker's piece, cut to what there is: the plan may be of another batch.
-template <int TILE> __device__ __forceinline__ FewPiece few_piece(const PagedKv &kv, const FewPiece *p)
+template <int TILE>
+__device__ __forceinline__ FewPiece few_piece(const PagedKv &kv, const SharedPlan &sp, int w)
 {
-    FewPiece f = *p;
+    FewPiece f = sp.few[w];
     f.slot = min(max(f.slot, 0), kv.seqs - 1);
     f.kh = min(max(f.kh, 0), kv.kvh - 1);
-    f.begin = min(max(f.begin, 0), kv.rows);
-    f.n = min(max(f.n, 0), kv.rows - f.begin);
+    // (begin: a row there is, read whatever n)
+    const int places = f.narrow ? sp.cap * sp.tq : kv.rows;
+    f.begin = min(max(f.begin, 0), places - 1);
+    f.n = min(max(f.n, 0), places - f.begin);
+    if (f.narrow) f.n = min(f.n, sp.tq / 8);
     f.len = (int)min((long long)max(f.len, 0), (long long)kv.stride << kv.shift);
     f.skip = min(max(f.skip, 0), f.len) & ~15;
     const int tiles = (f.len - f.skip + TILE - 1) / TILE;

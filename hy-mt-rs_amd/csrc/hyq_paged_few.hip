@@ -273,11 +273,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_kern
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     // (uniform over the wave, and known to be; few workers lie on many CUs: two
     // slots of 1100 positions took 1.5 us longer with four to a workgroup)
-    // (SHARED: alike on the SIMDs of a CU, whose workgroups are 256 apart)
-    const int w = __builtin_amdgcn_readfirstlane(
-        blockIdx.x + max_workers / FEW_WAVES *
-                         (((threadIdx.x >> 6) + (SHARED ? blockIdx.x >> 8 : 0)) & 3));
-    if (w >= (SHARED ? sp.head->workers : plan.workers)) return;
+    int workers, w;
+    if constexpr (SHARED) { // whole workgroups, and the last waves alike on a CU's SIMDs
+        workers = min(sp.head->workers, sp.few_most);
+        const int groups = (workers + 256 * FEW_WAVES - 1) / (256 * FEW_WAVES) * 256;
+        w = (int)blockIdx.x < groups
+                ? blockIdx.x + groups * (((threadIdx.x >> 6) + (blockIdx.x >> 8)) & 3)
+                : workers;
+    } else {
+        workers = plan.workers;
+        w = blockIdx.x + max_workers / FEW_WAVES * (threadIdx.x >> 6);
+    }
+    w = __builtin_amdgcn_readfirstlane(w);
+    if (w >= workers) return;
     long long at = SHARED ? 0 : plan.begin(w);
     const long long stop = SHARED ? 1 : plan.begin(w + 1);
     const int rep = kv.heads / kv.kvh;
@@ -298,13 +306,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_kern
     while (at < stop) {
         SlotRows sr;
         int kh, t0, t1, tiles = 0, skip = 0;
+        bool narrow = false; // a block of several slots' rows, which see all positions
         bool whole; // no other worker's part, and no prefix's, is to be joined
         if constexpr (SHARED) {
-            const FewPiece f = few_piece<TILE>(kv, sp.few + w);
-            if (f.n > few_rows) return;
+            const FewPiece f = few_piece<TILE>(kv, sp, w);
+            if (!f.narrow && f.n > few_rows) return;
             s = f.slot, kh = f.kh, t0 = f.t0, t1 = f.t1, skip = f.skip;
             sr = SlotRows{f.begin, f.n, f.len};
-            whole = f.ways == 1 && skip == 0;
+            whole = f.ways == 1 && skip == 0 && !f.narrow;
+            narrow = f.narrow != 0;
             at = stop;
         } else {
             while (before[s + 1] <= at) ++s; // slots without tiles
@@ -320,11 +330,21 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_kern
 
         // this lane's row: token c / rep of the slot's new rows
         const int tok = c / rep;
-        const bool ok = tok < sr.n;
+        bool ok = tok < sr.n;
         const int head = kh * rep + c % rep;
-        const size_t row = (size_t)(sr.begin + (ok ? tok : 0)) * kv.heads + head;
-        const int first = sr.len - sr.n;           // the first new row's position
-        const int sees = ok ? first + tok : -1;    // this row's last visible position
+        int packed = sr.begin + (ok ? tok : 0);
+        int first = sr.len - sr.n;        // the first new row's position
+        int sees = ok ? first + tok : -1; // this row's last visible position
+        if constexpr (SHARED) {
+            if (narrow) {
+                const int listed = ok ? sp.list[packed] : -1;
+                ok = (unsigned)listed < (unsigned)kv.rows;
+                packed = ok ? listed : 0;
+                first = sr.len - 1;
+                sees = ok ? first : -1;
+            }
+        }
+        const size_t row = (size_t)packed * kv.heads + head;
         Ops<T> ops;
         ops.load_q(q + row * KV_D, ok, g);
         f32x4 acc[8];
@@ -371,7 +391,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_kern
                   above = s + 1 < kv.seqs ? entries[at0 + kv.stride] : -1;
         int page = page_of(p_begin);
         const bool alone =
-            __builtin_amdgcn_readfirstlane(mine != below && mine != above) != 0;
+            __builtin_amdgcn_readfirstlane(mine != below && mine != above && !narrow) != 0;
         bool odd = false;
         auto stream = [&](auto once) {
             load_k(once, p_begin, page);
@@ -522,13 +542,18 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     const int rep = kv.heads / kv.kvh;
     SlotRows sr;
     SharedPlace pl{};
+    bool narrow = false;
     int w0, n;
     if constexpr (SHARED) {
         pl = sp.place[s];
         sr.begin = min(max(pl.begin, 0), kv.rows);
         sr.n = min(max(pl.n, 0), kv.rows - sr.begin);
-        pl.part = min(max(pl.part, 0), sp.most - 1);
-        pl.pieces = min(max(pl.pieces, 0), sp.most - pl.part);
+        narrow = sp.head->narrow != 0;
+        const int most = narrow ? sp.few_most : sp.most;
+        pl.part = min(max(pl.part, 0), most - 1);
+        pl.pieces = min(max(pl.pieces, 0), most - pl.part);
+        if (narrow) pl.part = (int)min((long long)pl.part + (long long)kh * pl.pieces,
+                                       (long long)(most - pl.pieces));
         n = min(max(pl.ways, 0), sp.few_most);
         w0 = (int)min((long long)max(pl.first, 0) + (long long)kh * n, (long long)sp.few_most);
         n = min(n, sp.few_most - w0);
@@ -550,9 +575,11 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     j.add({p + (size_t)a * step}, step, b - a, 2 * lane);
     if constexpr (SHARED) { // the prefix's pieces, for this row of its block
         const int c0 = wide ? pl.pieces * g / 4 : 0, c1 = wide ? pl.pieces * (g + 1) / 4 : pl.pieces;
-        const size_t each = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
-        const float *x = prefix + ((size_t)pl.part * kv.kvh + kh) * PR_ROWS * PAGED_PART +
-                         (size_t)min(min(max(pl.row, 0), PR_ROWS) + r, PR_ROWS - 1) * PAGED_PART;
+        const int last = narrow ? part_rows - 1 : PR_ROWS - 1;
+        const size_t each = narrow ? step : (size_t)kv.kvh * PR_ROWS * PAGED_PART;
+        const float *x = narrow ? part + (size_t)pl.part * each
+                                : prefix + ((size_t)pl.part * kv.kvh + kh) * PR_ROWS * PAGED_PART;
+        x += (size_t)min(min(max(pl.row, 0), last) + r, last) * PAGED_PART;
         j.add({x + (size_t)c0 * each}, each, c1 - c0, 2 * lane);
     }
     float *o = out + ((size_t)(sr.begin + r / rep) * kv.heads + kh * rep + r % rep) * KV_D;
@@ -615,7 +642,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_ro
                                                           const float *__restrict__ prefix,
                                                           float *__restrict__ out)
 {
-    const int each = wide ? part_rows : (part_rows + 3) / 4; // workgroups of a slot and KV head
+    const int rows = few_rows * (kv.heads / kv.kvh); // of a slot and KV head, `each` workgroups
+    const int each = wide ? rows : (rows + 3) / 4;
     const int kh = blockIdx.x % kv.kvh, i = blockIdx.x / kv.kvh, n = kv.seqs * each;
     if (i < n)
         merge_few<SHARED>(kv, few_rows, part_rows, part, shared, sp, prefix, out, kh, i / each,
@@ -642,6 +670,9 @@ int paged_few_rows(int rep) { return 16 / rep; }
 
 namespace {
 
+// Rows of a part: those that a slot can have, or a block's.
+int part_rows_of(bool shared, int few, int rep) { return (shared ? paged_few_rows(rep) : few) * rep; }
+
 size_t parts_bytes(int type, bool shared, int seqs, int kvh, int part_rows)
 {
     const size_t n = shared ? (size_t)few_most(seqs, kvh) // (a plan's pieces, one a worker)
@@ -655,14 +686,14 @@ size_t parts_bytes(int type, bool shared, int seqs, int kvh, int part_rows)
 size_t paged_few_scratch(int type, bool shared, int seqs, int kvh, int heads, int few)
 {
     const size_t units = ((size_t)seqs * kvh * 8 + 255) / 256 * 256;
-    return parts_bytes(type, shared, seqs, kvh, few * (heads / kvh)) + units;
+    return parts_bytes(type, shared, seqs, kvh, part_rows_of(shared, few, heads / kvh)) + units;
 }
 
 int launch_paged_few(const PagedKv &kv, int few, const RowsScratch &rs, const SharedPlan *sp,
                      const float *q, float *part, float *out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
-    const int part_rows = few * (kv.heads / kv.kvh);
+    const int part_rows = part_rows_of(sp, few, kv.heads / kv.kvh);
     int2 *shared = (int2 *)((char *)part + parts_bytes(kv.type, sp, kv.seqs, kv.kvh, part_rows));
     const size_t lds = ((size_t)kv.seqs + 1) * 8;
     const int workers = sp ? sp->few_most : few_workers(kv.type);
@@ -681,15 +712,16 @@ int launch_paged_merge(const PagedKv &kv, int few, const RowsScratch &rs, const 
                        const float *part, const float *prefix, float *out, void *stream)
 {
     hipStream_t st = (hipStream_t)stream;
-    const int part_rows = few * (kv.heads / kv.kvh);
+    const int part_rows = part_rows_of(sp, few, kv.heads / kv.kvh);
     const int2 *shared =
         (const int2 *)((const char *)part + parts_bytes(kv.type, sp, kv.seqs, kv.kvh, part_rows));
     // Few rows have many parts each (1024 workers over four slots of four KV
     // heads: 64), which all of a workgroup's waves read; many rows have few, and
     // a wave each. Wide and not: four slots of 60001 positions 124 and 134 us,
     // 64 slots of 8192 173 and 170.
-    const int wide = kv.seqs * kv.kvh * part_rows <= 1024;
-    const int each = wide ? part_rows : (part_rows + 3) / 4;
+    const int rows = few * (kv.heads / kv.kvh);
+    const int wide = kv.seqs * kv.kvh * rows <= 1024;
+    const int each = wide ? rows : (rows + 3) / 4;
     const dim3 grid((unsigned)merge_groups(kv.seqs, kv.kvh, each, rs.cap));
     auto kernel = sp ? paged_merge_kernel<true> : paged_merge_kernel<false>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, kv, few, part_rows, wide, rs, part, shared,

@@ -129,11 +129,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
     FewPlan plan;
     if constexpr (!SHARED) plan = few_plan<TILE>(kv, few_rows, max_workers, before, wsum);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    // (SHARED: alike on the SIMDs of a CU, whose workgroups are 256 apart)
-    const int w = __builtin_amdgcn_readfirstlane(
-        blockIdx.x + max_workers / FEW_WAVES *
-                         (((threadIdx.x >> 6) + (SHARED ? blockIdx.x >> 8 : 0)) & 3));
-    if (w >= (SHARED ? sp.head->workers : plan.workers)) return;
+    int workers, w;
+    if constexpr (SHARED) { // whole workgroups, and the last waves alike on a CU's SIMDs
+        workers = min(sp.head->workers, sp.few_most);
+        const int groups = (workers + 256 * FEW_WAVES - 1) / (256 * FEW_WAVES) * 256;
+        w = (int)blockIdx.x < groups
+                ? blockIdx.x + groups * (((threadIdx.x >> 6) + (blockIdx.x >> 8)) & 3)
+                : workers;
+    } else {
+        workers = plan.workers;
+        w = blockIdx.x + max_workers / FEW_WAVES * (threadIdx.x >> 6);
+    }
+    w = __builtin_amdgcn_readfirstlane(w);
+    if (w >= workers) return;
     long long at = SHARED ? 0 : plan.begin(w);
     const long long stop = SHARED ? 1 : plan.begin(w + 1);
     const int rep = kv.heads / kv.kvh;
@@ -153,13 +161,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
     while (at < stop) {
         SlotRows sr;
         int kh, t0, t1, tiles = 0, skip = 0;
+        bool narrow = false; // a block of several slots' rows, which see all positions
         bool whole; // no other worker's part, and no prefix's, is to be joined
         if constexpr (SHARED) {
-            const FewPiece f = few_piece<TILE>(kv, sp.few + w);
-            if (f.n > few_rows) return;
+            const FewPiece f = few_piece<TILE>(kv, sp, w);
+            if (!f.narrow && f.n > few_rows) return;
             s = f.slot, kh = f.kh, t0 = f.t0, t1 = f.t1, skip = f.skip;
             sr = SlotRows{f.begin, f.n, f.len};
-            whole = f.ways == 1 && skip == 0;
+            whole = f.ways == 1 && skip == 0 && !f.narrow;
+            narrow = f.narrow != 0;
             at = stop;
         } else {
             while (before[s + 1] <= at) ++s; // slots without tiles
@@ -175,10 +185,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
 
         // this lane's row: token c / rep of the slot's new rows
         const int tok = c / rep;
-        const bool ok = tok < sr.n;
+        bool ok = tok < sr.n;
         const int head = kh * rep + c % rep;
-        const size_t row = (size_t)(sr.begin + (ok ? tok : 0)) * kv.heads + head;
-        const int sees = ok ? sr.len - sr.n + tok : -1; // this row's last visible position
+        int packed = sr.begin + (ok ? tok : 0);
+        int sees = ok ? sr.len - sr.n + tok : -1; // this row's last visible position
+        if constexpr (SHARED) {
+            if (narrow) {
+                const int listed = ok ? sp.list[packed] : -1;
+                ok = (unsigned)listed < (unsigned)kv.rows;
+                packed = ok ? listed : 0;
+                sees = ok ? sr.len - 1 : -1;
+            }
+        }
+        const size_t row = (size_t)packed * kv.heads + head;
         f32x4 qrow[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
                   above = s + 1 < kv.seqs ? entries[at0 + kv.stride] : -1;
         Pages pages = pages_of(p_begin);
         const bool alone =
-            __builtin_amdgcn_readfirstlane(mine != below && mine != above) != 0;
+            __builtin_amdgcn_readfirstlane(mine != below && mine != above && !narrow) != 0;
         auto stream = [&](auto once) {
             load_k(once, p_begin, pages);
             load_v(once, p_begin, pages);

@@ -174,19 +174,26 @@ struct PlanLds {
 // their code, which they find in no cache: what they need is read once, numbers are
 // 32 bits, and few loops are unrolled.
 constexpr int PLAN_GROUPS = 8;
+// The tiles of narrow blocks, over all KV heads, up to which they take less time than
+// the tile form, in steps of 16 positions, and of 32 in 8-bit pages. Narrow and wide,
+// us, 16 heads over 4: f16 pages at 2048 tiles 21 and 23, at 4096 27 and 27, at 8192
+// 31 and 27; f32 ones at 2048 23 and 26, 4096 28 and 28, 8192 34 and 29; 8-bit ones at
+// 8192 30 and 33, 16384 38 and 36, 32768 52 and 44.
+constexpr int NARROW_TILES = 4096, NARROW_TILES_Q8 = 12288;
 __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
                                                            long long worth, SharedPlan sp)
 {
     extern __shared__ __align__(16) unsigned lds[];
     constexpr int TRIES = 16;
     __shared__ int wsum[16], tried[TRIES];
-    // all blocks' steps; all slots' tiles, and those that have some; the groups' saving
-    __shared__ unsigned sum[4];
+    // all blocks' steps; the tiles of the few-row form, and its slots and blocks; the
+    // groups' saving; the narrow blocks' tiles, and those blocks
+    __shared__ unsigned sum[6];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = kv.seqs;
     const PlanLds x(lds, n, sp.cap);
     const bool writes = blockIdx.x == 0;
     constexpr unsigned NONE = 0xfff00000u; // (a group has a page in common at least)
-    if (t < 4) sum[t] = 0;
+    if (t < 6) sum[t] = 0;
 #pragma unroll 1
     for (int s = t; s < ((n + 3) & ~3); s += 1024) {
         const int l = s < n ? sp.leader[s] : -1;
@@ -238,17 +245,31 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
         atomicMax(x.wide + l, (int)x.rows[s]);
     }
     __syncthreads();
+    const int tile = kv.type == KV_T_Q8 ? 5 : 4; // (the few-row form's step, as a logarithm)
+    auto tiles = [&](int positions) { return max(1, (positions + (1 << tile) - 1) >> tile); };
+#pragma unroll 1
+    for (int s = t; s < n; s += 1024)
+        if (x.first[s]) {
+            const int each = few / x.wide[s], mine = pieces_of(x.first[s], each);
+            atomicAdd(&sum[4], min((unsigned)mine * (unsigned)tiles(x.pages[s] << kv.shift), 1u << 20));
+            atomicAdd(&sum[5], (unsigned)mine);
+        }
+    __syncthreads();
+    const int most_narrow = kv.type == KV_T_Q8 ? NARROW_TILES_Q8 : NARROW_TILES;
+    const bool narrow = (long long)sum[4] * kv.kvh <= most_narrow && (int)sum[5] <= sp.cap;
+    const int tq = narrow ? few : sp.tq;
     int blocks = 0;
 #pragma unroll 1
     for (int b = 0; b < n; b += 1024) {
         const int s = b + t, slots = s < n ? x.first[s] : 0;
-        const int each = slots ? sp.tq / x.wide[s] : 1, mine = (slots + each - 1) / each;
+        const int each = slots ? tq / x.wide[s] : 1, mine = (slots + each - 1) / each;
         int before;
         const int all = scan1024(mine, before, wsum);
         const int first = blocks + before;
 #pragma unroll 1
         for (int i = 0; i < mine && first + i < sp.cap; ++i) {
-            const unsigned steps = ((x.pages[s] << kv.shift) + PR_TILE - 1) / PR_TILE;
+            const int positions = x.pages[s] << kv.shift;
+            const unsigned steps = narrow ? tiles(positions) : (positions + PR_TILE - 1) / PR_TILE;
             x.of[first + i] = (short)s;
             x.steps[first + i] = steps;
             x.toks[first + i] = (unsigned char)(min(each, slots - i * each) * x.wide[s]);
@@ -260,73 +281,88 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
     blocks = min(blocks, sp.cap);
     __syncthreads();
     // the slots' places in the blocks, and what their own positions are
-    const int tile = kv.type == KV_T_Q8 ? 5 : 4; // (the few-row form's step, as a logarithm)
     auto tiles_of = [&](int s) {
-        const int own = x.len[s] - (x.pages[s] << kv.shift);
-        return x.rows[s] ? max(1, (own + (1 << tile) - 1) >> tile) : 0;
+        return x.rows[s] ? tiles(x.len[s] - (x.pages[s] << kv.shift)) : 0;
     };
 #pragma unroll 1
     for (int s = t; s < n; s += 1024) {
         const SlotRows r = slot_rows(kv, s);
         x.begin[s] = r.begin;
         x.len[s] = r.len;
-        const int tiles = tiles_of(s);
-        if (tiles) {
-            atomicAdd(&sum[1], (unsigned)min(tiles, (1 << 20) - 1));
+        const int own = tiles_of(s);
+        if (own) {
+            atomicAdd(&sum[1], (unsigned)min(own, (1 << 20) - 1));
             atomicAdd(&sum[2], 1u);
         }
         if (!x.pages[s]) continue;
-        const int l = (int)(x.key[s] >> 20), wide = x.wide[l], each = sp.tq / wide;
+        const int l = (int)(x.key[s] >> 20), wide = x.wide[l], each = tq / wide;
         const int up = x.rank[s] / each, at = (x.rank[s] - up * each) * wide;
         const int b = min(x.first[l] + up, sp.cap - 1);
 #pragma unroll 1
         for (int i = 0; writes && i < wide; ++i)
-            sp.list[b * sp.tq + at + i] = i < x.rows[s] ? x.begin[s] + i : -1;
+            sp.list[b * tq + at + i] = i < x.rows[s] ? x.begin[s] + i : -1;
         x.block[s] = (short)b;
         x.rank[s] = at; // (its first token's place in the block)
     }
-    // Pieces of at most `each` steps: the least, of sixteen lengths, with which they
-    // number no more than fill the GPU once, or the last one, of which that is sure
-    // unless the blocks alone are many.
-    const int total = (int)sum[0], fill = fill_pieces(kv.kvh);
-    const int room = max(fill - blocks, (fill + 1) / 2);
-    const int least = max(PR_MIN_TILES, (total + fill - 1) / fill);
-    const int most = max(least, (total + room - 1) / room);
-    const int more = (most - least + TRIES - 2) / (TRIES - 1);
-    int pieces = 0;
-#pragma unroll 1
-    for (int b = lane; b < blocks; b += 64)
-        pieces += pieces_of((int)x.steps[b], least + more * wave);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) pieces += __shfl_xor(pieces, o, 64);
-    if (lane == 0) tried[wave] = pieces;
-    __syncthreads();
-    const unsigned fits = (unsigned)__ballot(tried[lane & (TRIES - 1)] <= fill) & 0xffffu;
-    const int each = least + more * (fits ? __ffs((int)fits) - 1 : TRIES - 1);
     int parts = 0;
+    if (!narrow) {
+        // Pieces of at most `each` steps: the least, of sixteen lengths, with which they
+        // number no more than fill the GPU once, or the last one, of which that is sure
+        // unless the blocks alone are many.
+        const int total = (int)sum[0], fill = fill_pieces(kv.kvh);
+        const int room = max(fill - blocks, (fill + 1) / 2);
+        const int least = max(PR_MIN_TILES, (total + fill - 1) / fill);
+        const int most = max(least, (total + room - 1) / room);
+        const int more = (most - least + TRIES - 2) / (TRIES - 1);
+        int pieces = 0;
 #pragma unroll 1
-    for (int b = 0; b < blocks; b += 1024) {
-        const int at = b + t, steps = at < blocks ? (int)x.steps[at] : 0;
-        int before;
-        const int all = scan1024(pieces_of(steps, each), before, wsum);
-        if (at < blocks) x.part[at] = parts + before;
-        parts += all;
-    }
-    if (t == 0) x.part[blocks] = parts;
-    __syncthreads();
+        for (int b = lane; b < blocks; b += 64)
+            pieces += pieces_of((int)x.steps[b], least + more * wave);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) pieces += __shfl_xor(pieces, o, 64);
+        if (lane == 0) tried[wave] = pieces;
+        __syncthreads();
+        const unsigned fits = (unsigned)__ballot(tried[lane & (TRIES - 1)] <= fill) & 0xffffu;
+        const int each = least + more * (fits ? __ffs((int)fits) - 1 : TRIES - 1);
 #pragma unroll 1
-    for (int p = t; writes && p < parts; p += 1024) {
-        const int b = last_of(x.part, blocks, p), s = x.of[b];
-        const int2 by = share((int)x.steps[b], p - x.part[b], x.part[b + 1] - x.part[b]);
-        sp.pieces[p] = Piece{s, b, by.x, by.y, p, 0, x.toks[b], x.pages[s] << kv.shift};
+        for (int b = 0; b < blocks; b += 1024) {
+            const int at = b + t, steps = at < blocks ? (int)x.steps[at] : 0;
+            int before;
+            const int all = scan1024(pieces_of(steps, each), before, wsum);
+            if (at < blocks) x.part[at] = parts + before;
+            parts += all;
+        }
+        if (t == 0) x.part[blocks] = parts;
+        __syncthreads();
+#pragma unroll 1
+        for (int p = t; writes && p < parts; p += 1024) {
+            const int b = last_of(x.part, blocks, p), s = x.of[b];
+            const int2 by = share((int)x.steps[b], p - x.part[b], x.part[b + 1] - x.part[b]);
+            sp.pieces[p] = Piece{s, b, by.x, by.y, p, 0, x.toks[b], x.pages[s] << kv.shift};
+        }
+    } else {
+        __syncthreads();
     }
     // The slots' own positions, by the few-row form: pieces of at most `piece` tiles,
     // so long that they number FEW_PIECES at most (or half as many beside a piece for
     // each slot and head, where those are many).
     const int head = FEW_PIECES / kv.kvh; // pieces of a KV head
-    const int spread = max(head - (int)sum[2], head / 2);
-    const int piece = max(1, pieces_of((int)min(sum[1], 0x7fff0000u), spread));
+    const unsigned units = sum[2] + (narrow ? sum[5] : 0), all_tiles = sum[1] + (narrow ? sum[4] : 0);
+    const int spread = max(head - (int)units, head / 2);
+    const int piece = max(1, pieces_of((int)min(all_tiles, 0x7fff0000u), spread));
     int workers = 0;
+    if (narrow) {
+#pragma unroll 1
+        for (int b = 0; b < blocks; b += 1024) {
+            const int at = b + t, ways = at < blocks ? pieces_of((int)x.steps[at], piece) : 0;
+            int before;
+            const int all = scan1024(ways * kv.kvh, before, wsum);
+            if (at < blocks) x.part[at] = workers + before;
+            workers += all;
+        }
+        __syncthreads();
+    }
+    const int of_blocks = workers;
 #pragma unroll 1
     for (int b = 0; b < n; b += 1024) {
         const int s = b + t, ways = s < n ? pieces_of(tiles_of(s), piece) : 0;
@@ -337,7 +373,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
             if (x.pages[s]) {
                 const int at = x.block[s];
                 p.part = x.part[at];
-                p.pieces = x.part[at + 1] - p.part;
+                p.pieces = narrow ? pieces_of((int)x.steps[at], piece) : x.part[at + 1] - p.part;
                 p.row = x.rank[s] * (kv.heads / kv.kvh);
             }
             if (writes) sp.place[s] = p;
@@ -350,14 +386,21 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
     __syncthreads();
 #pragma unroll 1
     for (int w = blockIdx.x * 256 + t; t < 256 && w < workers; w += PLAN_GROUPS * 256) {
+        if (w < of_blocks) {
+            const int b = last_of(x.part, blocks, w), s = x.of[b], ways = pieces_of((int)x.steps[b], piece);
+            const int kh = (int)((unsigned)(w - x.part[b]) / (unsigned)ways);
+            const int2 by = share((int)x.steps[b], w - x.part[b] - kh * ways, ways);
+            sp.few[w] = FewPiece{s, kh, by.x, by.y, b * tq, x.toks[b], x.pages[s] << kv.shift, 0, ways, 1, {}};
+            continue;
+        }
         const int s = last_of(x.first, n, w), ways = max(1, x.ways[s]); // (a slot that has pieces)
         const int kh = (int)((unsigned)(w - x.first[s]) / (unsigned)ways);
         const int2 by = share(tiles_of(s), w - x.first[s] - kh * ways, ways);
         sp.few[w] = FewPiece{s,          kh,        by.x,     by.y,
                              x.begin[s], x.rows[s], x.len[s], x.pages[s] << kv.shift,
-                             ways,       {}};
+                             ways,       0,         {}};
     }
-    if (writes && t == 0) *sp.head = SharedHead{Plan{blocks, parts}, workers};
+    if (writes && t == 0) *sp.head = SharedHead{Plan{blocks, parts}, workers, narrow};
 }
 
 } // namespace

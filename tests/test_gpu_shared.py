@@ -174,6 +174,31 @@ def test_more_rows_than_a_block(gpu_ctx, hyq, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pt,heads", [(64, (16, 4)), (32, (6, 2))], ids=str)
+def test_prefixes_of_many_tiles(gpu_ctx, hyq, pt, heads, kind):
+    """Groups whose blocks of 16 rows would have more tiles than the plan gives the
+    few-row form: blocks of 128 rows by the tile form, more than one and partly filled,
+    one of a prefix that is no whole steps, with slots beside them."""
+    r = np.random.default_rng(pt)
+    kvh = heads[1]
+    most = {"Q8": 12288 * 32}.get(kind, 4096 * 16)
+    few = 16 // (heads[0] // heads[1])
+    news = np.where(np.arange(75) % 9 == 8, 0, r.integers(1, 3, 75))
+    blocks = -(-int((news[:60] > 0).sum()) // (few // 2))  # of 16 rows, of the larger group
+    pages = int(1.1 * most / kvh / blocks / pt) + 1
+    lens = news + pages * pt + r.integers(0, 30, 75)
+    lens[60:] = news[60:] + (pages // 2) * pt + r.integers(0, 30, 15)
+    b = batch(kind, lens, news, heads, pt, seed=pt, tail=1)
+    share(b, list(range(60)), pages)
+    share(b, [60, 61, 63, 64], pages // 2 - 1)
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.array_equal(c.skips(), plain_skips(b))
+    head = c.plan.numpy()[:16].view(np.int32)
+    assert head[0] >= 2 and head[1] > head[0] and head[3] == 0  # blocks, their pieces, not narrow
+    check(b, c.attend())
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_the_prefix_that_saves_most(gpu_ctx, hyq, kind):
     """One instruction of a page before several requests' beams: beams that share more
     with the first slot are taken, if they save more; and by groups, each request's."""
@@ -196,7 +221,7 @@ def test_the_prefix_that_saves_most(gpu_ctx, hyq, kind):
     check(b, c.attend())
 
 
-@pytest.mark.parametrize("kind,least", [("F32", 90000), ("F16", 90000), ("Q8", 230000)])
+@pytest.mark.parametrize("kind,least", [("F32", 50000), ("F16", 50000), ("Q8", 120000)])
 def test_what_is_worth_sharing(gpu_ctx, hyq, kind, least):
     """Nothing is shared where all groups together save less than the given number, or
     the rule's; the results are the same but for rounding."""
