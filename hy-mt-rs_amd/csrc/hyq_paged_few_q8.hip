@@ -19,9 +19,9 @@
 // eight positions of a dim in a lane: a lane loads eight dims of each of its
 // positions, and one byte permutation per pair of positions picks a dim's two
 // codes into the low bytes of two halves, u 2^-24 as f16, which an fma makes
-// (u - 128) 2^-9. The weights' two f16 parts keep 22 bits: p lies up to 2^14 and
-// b below the power of two that passes all scales the row has seen, so that a
-// weight's error is at most 2^-39 of the largest.
+// (u - 128) 2^-9. The weights' two f16 parts keep 22 bits: p lies up to 2^14 over
+// the power of two that passes all scales the row has seen, and p b below 2^14, so
+// that its error is at most 2^-39 of the largest.
 //
 // Bound by memory: 264 bytes a position and head.
 #include <hip/hip_runtime.h>
@@ -209,8 +209,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
 #pragma unroll
         for (int x = 0; x < 8; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
         // m: the running maximum less LIFT; top: a power of two above all scales of
-        // values seen (not below 2^-100, that its inverse be one too)
-        float m = -INFINITY, l = 0.f, top = 0x1p-100f;
+        // values seen (not below 2^-88, that sums of weights over it be numbers)
+        float m = -INFINITY, l = 0.f, top = 0x1p-88f, log_top = -88.f;
 
         const int *entries = kv.table + (size_t)s * kv.stride;
         int have = -64, ids = -1; // lane i: the slot's page have + i
@@ -310,23 +310,22 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
                 mx = wave::max_halves(wave::max_rows2(mx));
                 bm = wave::max_halves(wave::max_rows2(bm));
                 const float mn = fmaxf(m, mx - LIFT);
-                // (the power of two above bm)
-                const float up = __builtin_bit_cast(
-                    float, (__builtin_bit_cast(unsigned, bm) & 0x7f800000u) + 0x00800000u);
-                const float tn = bm > top ? up : top;
-                // a row that has seen nothing yet keeps zero weights
-                const float base = mn == -INFINITY ? 0.f : mn;
-                if (__any(mn != m || tn != top)) {
-                    const float corr = __builtin_amdgcn_exp2f(m - base);
-                    const float both = corr * (top / tn);
+                if (__any(mn != m || bm > top)) {
+                    float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                    if (bm > top) { // (the power of two above bm)
+                        const unsigned up =
+                            (__builtin_bit_cast(unsigned, bm) & 0x7f800000u) + 0x00800000u;
+                        corr *= top / __builtin_bit_cast(float, up);
+                        top = __builtin_bit_cast(float, up);
+                        log_top = (float)((int)(up >> 23) - 127);
+                    }
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) acc[x] *= both;
+                    for (int x = 0; x < 8; ++x) acc[x] *= corr;
                     l *= corr;
                     m = mn;
-                    top = tn;
                 }
-                const float inv = __builtin_bit_cast(
-                    float, 0x7f000000u - __builtin_bit_cast(unsigned, top)); // 1 / top
+                // a row that has seen nothing yet keeps zero weights
+                const float base = m == -INFINITY ? 0.f : m + log_top;
                 half8 hi, lo;
                 float sum = 0.f;
 #pragma unroll
@@ -335,7 +334,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
                                 p1 = __builtin_amdgcn_exp2f(sv[i + 1] - base);
                     sum += p0 + p1;
                     half2 x, y;
-                    split2(p0 * (b[i] * inv), p1 * (b[i + 1] * inv), x, y);
+                    split2(p0 * b[i], p1 * b[i + 1], x, y);
                     hi[i] = x[0];
                     hi[i + 1] = x[1];
                     lo[i] = y[0];
@@ -370,13 +369,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
         if (whole) {
             // (a row that saw nothing gives zeros)
             o = out + row * KV_D;
-            f = l > 0.f || l != l ? top * (512.f / l) : 0.f;
+            f = l > 0.f || l != l ? 512.f / l : 0.f;
         } else {
             const long long slot = SHARED ? w : (long long)w + (long long)s * kv.kvh + kh;
             o = part + ((size_t)slot * part_rows + c) * PAGED_PART;
             if (ok && g == 0) { // (the maximum itself, and weights of at most 1)
                 o[0] = m + LIFT;
-                o[1] = l * 0x1p-14f;
+                o[1] = l * (top * 0x1p-14f);
             }
             o += 4;
             f = top * 0x1p-5f;

@@ -21,8 +21,8 @@
 // 8-bit pages hold a code for each number, which f16 holds too, and a scale for
 // each position of a head: codes go through both products, the scores are
 // multiplied with the keys' scales, and the weights with the values' before they
-// are split. Those are kept below 2^15 by a power of two above all scales that the
-// row has seen, which the sums are a multiple of.
+// are split. Those are kept below 2^15 by weights that are smaller by a power of two
+// above all scales that the row has seen.
 //
 // Keys and values go through LDS, two steps of them, rows as they are (values
 // are transposed by ds_read_b64_tr_b16 on their way to the matrix operand).
@@ -205,6 +205,7 @@ template <bool LO> struct RowsLds { // one step
 struct CodesLds {
     _Float16 khi[PR_TILE][PR_KP], vhi[PR_TILE][PR_VP];
     float scale[2][PR_TILE]; // of keys, of values
+    float most[4];           // of the first and the second half's values, at most
 };
 
 // WHOLE: a step lies in one page (of 64 tokens or more), so that it takes one
@@ -357,7 +358,12 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                                                  : g == 1 ? pg.at(1)
                                                  : g == 2 ? pg.at(2)
                                                           : pg.at(3);
-                    l.scale[wave][lane] = lane < seen_end - p0 && e >= 0 ? raw.scale : 0.f;
+                    const float x = lane < seen_end - p0 && e >= 0 ? raw.scale : 0.f;
+                    l.scale[wave][lane] = x;
+                    if (wave) { // (a NaN is none)
+                        const float most = wave::max_rows2(wave::max16(x));
+                        if ((lane & 31) == 0) l.most[lane >> 5] = most;
+                    }
                 }
             } else if (n & 1)
                 R::put(&l.vhi[r][d], &l.vlo[LO ? r : 0][LO ? d : 0], raw.v[n >> 1]);
@@ -441,7 +447,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
         float m_run = -INFINITY, l_run = 0.f;
-        float top = 0x1p-100f; // (codes: above all scales of values seen, see above)
+        float top = 0x1p-88f, log_top = -88.f; // (codes: above all scales of values seen)
 
         // A step that some row sees in part: values of it that are not finite, or
         // would not be as f16 parts, must not reach the rows that do not see them
@@ -525,31 +531,33 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             // resolve 2^-25, which is 2^-32 of the first weight. (Many equal small
             // weights are rounded the same way, and their errors add up.)
             const float m_new = fmaf(wave::max_halves(tmax), qscale, -7.f);
-            float bmax = 0.f;
-            if constexpr (Q8) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) bmax = fmaxf(bmax, bs[e]);
-                bmax = wave::max_halves(bmax);
-            }
-            if (__any(m_new > m_run + 8.f || (Q8 && bmax > top))) {
+            float most = 0.f;
+            if constexpr (Q8) most = l.most[part_of];
+            if (__any(m_new > m_run + 8.f || (Q8 && most > top))) {
                 const float m = fmaxf(m_run, m_new);
                 float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
-                l_run *= corr;
                 if constexpr (Q8) {
+                    float bmax = 0.f; // of the positions that the row sees
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) bmax = fmaxf(bmax, bs[e]);
+                    bmax = wave::max_halves(bmax);
                     if (bmax > top) { // (the power of two above bmax)
-                        const float up = __builtin_bit_cast(
-                            float, (__builtin_bit_cast(unsigned, bmax) & 0x7f800000u) + 0x00800000u);
-                        corr *= top / up;
-                        top = up;
+                        const unsigned up =
+                            (__builtin_bit_cast(unsigned, bmax) & 0x7f800000u) + 0x00800000u;
+                        corr *= top / __builtin_bit_cast(float, up);
+                        top = __builtin_bit_cast(float, up);
+                        log_top = (float)((int)(up >> 23) - 127);
                     }
                 }
+                l_run *= corr;
 #pragma unroll
                 for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[j][e] *= corr;
                 m_run = m;
             }
-            const float base = m_run == -INFINITY ? 0.f : m_run; // (nothing seen yet: zero weights)
+            // (nothing seen yet: zero weights)
+            const float base = m_run == -INFINITY ? 0.f : Q8 ? m_run + log_top : m_run;
             float rs[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -558,10 +566,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             }
             l_run += rs[0] + rs[1];
             if constexpr (Q8) {
-                const float inv = __builtin_bit_cast(
-                    float, 0x7f000000u - __builtin_bit_cast(unsigned, top)); // 1 / top
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sv[e] *= bs[e] * inv;
+                for (int e = 0; e < 16; ++e) sv[e] *= bs[e];
             }
             // operand element 4 x + i of product (kk, j): position 16 kk + 8 x + 4 h + i,
             // which is the lane's weight 8 kk + 4 x + i
@@ -621,7 +627,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[j][e] *= top * 0x1p-15f;
-            l_run *= 0x1p-15f;
+            l_run *= top * 0x1p-15f;
             m_run += 15.f;
         }
         if (__syncthreads_or(odd)) {
