@@ -40,7 +40,14 @@
 // work, which overlap in part: a step takes 3.0 and 1.8 us. 512 new tokens of
 // one slot over 2012 positions, 16 heads over 4, f32 pages: 45 us in all, the
 // plan 6, this launch 37 (eight steps, and 13 us to begin and end: cold code and
-// loads that wait for each other), the merge 5.
+// loads that wait for each other), the merge 5. The same over 8-bit pages: this
+// launch 31. Three prompts of up to 400 beside 27 sessions of up to 4000 positions,
+// 32 heads over 8: 114 us over 8-bit pages, of which MFMAs are 30 % and VALU work
+// 33 % (106 over f16 ones: the codes' conversion and the scales are the difference;
+// scores by products of whole numbers would save the keys' conversion and take as
+// much for the queries' third part). A prefix of 8192 positions for 64 slots of four
+// rows, 32 heads over 8, f16 pages: 29 us; four of 3100 for 24 slots of three tokens
+// each, 8-bit pages: 45.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -106,7 +113,7 @@ __device__ __forceinline__ bool has_parts(float x) { return fabsf(x) < 65520.f; 
 // of 16 bytes a lane.
 template <class T> struct Raw;
 template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
-    static constexpr int N = 4;
+    static constexpr int N = 4, PUTS = 8;
     typedef float4 Vec;
     Vec k[N], v[N];
     static constexpr int STEP = 16;
@@ -139,7 +146,7 @@ template <> struct Raw<float> { // row (t / 32) + 16 i, dims 4 (t % 32) ..
     }
 };
 template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
-    static constexpr int N = 2;
+    static constexpr int N = 2, PUTS = 4;
     typedef half8 Vec;
     Vec k[N], v[N];
     static constexpr int STEP = 32;
@@ -166,7 +173,7 @@ template <> struct Raw<_Float16> { // row (t / 16) + 32 i, dims 8 (t % 16) ..
 };
 
 template <> struct Raw<unsigned char> { // row t / 8, dims 16 (t % 8) ..
-    static constexpr int N = 1;
+    static constexpr int N = 1, PUTS = 4;
     typedef u32x4 Vec;
     Vec k[N], v[N];
     float scale; // waves 0 and 1: of the keys and the values of row t % 64
@@ -177,24 +184,28 @@ template <> struct Raw<unsigned char> { // row t / 8, dims 16 (t % 8) ..
     // (codes are numbers wherever they lie; the scales of rows that nobody sees are
     // put away as zeros)
     __device__ __forceinline__ bool clean(const bool (&)[N]) { return false; }
-    // u + 1024 is a byte u under the exponent of 1024
-    static __device__ __forceinline__ void put(_Float16 *hi, const u32x4 &x, unsigned sign)
+    // Half i of the 16 dims, the other one in every second four lanes, so that eight
+    // lanes write to all banks at once (three prompts beside 27 sessions: 151 us, and
+    // 154 with each lane's halves in order, two lanes to a bank). u + 1024 is a byte u
+    // under the exponent of 1024.
+    static __device__ __forceinline__ void put(_Float16 *hi, const u32x4 &x, int i, int t,
+                                               unsigned sign)
     {
-        half8 y[2];
+        const bool second = (i ^ (t >> 2)) & 1;
+        half8 y;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const unsigned u = x[w] ^ sign;
-            const half2 a = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)),
-                        b = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+        for (int w = 0; w < 2; ++w) {
+            constexpr unsigned UP = 0x64646464u;
+            const unsigned u = (second ? x[w + 2] : x[w]) ^ sign;
             const half2 from = {(_Float16)1152.f, (_Float16)1152.f};
-            const half2 c = a - from, d = b - from;
-            y[w >> 1][4 * (w & 1)] = c[0];
-            y[w >> 1][4 * (w & 1) + 1] = c[1];
-            y[w >> 1][4 * (w & 1) + 2] = d[0];
-            y[w >> 1][4 * (w & 1) + 3] = d[1];
+            const half2 a = __builtin_bit_cast(half2, __builtin_amdgcn_perm(UP, u, 0x04010400u)) - from;
+            const half2 b = __builtin_bit_cast(half2, __builtin_amdgcn_perm(UP, u, 0x04030402u)) - from;
+            y[4 * w] = a[0];
+            y[4 * w + 1] = a[1];
+            y[4 * w + 2] = b[0];
+            y[4 * w + 3] = b[1];
         }
-        *reinterpret_cast<half8 *>(hi) = y[0];
-        *reinterpret_cast<half8 *>(hi + 8) = y[1];
+        *reinterpret_cast<half8 *>(hi + (second ? 8 : 0)) = y;
     }
 };
 
@@ -345,13 +356,13 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                 }
             }
         };
-        // one of the 2 N rows of `raw`, the step from p0 on, converted, to a buffer
+        // one of the PUTS parts of `raw`, the step from p0 on, converted, to a buffer
         auto store = [&](int buf, int n, int p0, const Pages &pg) {
             Lds &l = lds.step[buf];
-            const int d = R::dim(t), r = R::row(t) + R::STEP * (n >> 1);
+            const int d = R::dim(t), r = R::row(t) + (Q8 ? 0 : R::STEP * (n >> 1));
             if constexpr (Q8) {
-                if (n) R::put(&l.vhi[r][d], raw.v[0], 0u);
-                else R::put(&l.khi[r][d], raw.k[0], 0x80808080u);
+                if (n < 2) R::put(&l.khi[r][d], raw.k[0], n, t, 0x80808080u);
+                else R::put(&l.vhi[r][d], raw.v[0], n, t, 0u);
                 if (n == 0 && wave < 2) {
                     const int g = lane >> 4, e = WHOLE    ? pg.e[0]
                                                  : g == 0 ? pg.at(0)
@@ -454,7 +465,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         // (0 * inf), see below.
         bool odd = partial(p_begin, cur) && clean(p_begin, cur);
 #pragma unroll
-        for (int n = 0; n < 2 * R::N; ++n) store(0, n, p_begin, cur);
+        for (int n = 0; n < R::PUTS; ++n) store(0, n, p_begin, cur);
         load(p_begin + PR_TILE, next);
         __syncthreads();
         int buf = 0;
@@ -492,7 +503,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     sv = mfma(ahi[kk & 1], qhi[kk], sv);
                     sv = mfma(ahi[kk & 1], qlo[kk], sv);
                 }
-                if (kk < 2 * R::N) store(buf ^ 1, kk, p0 + PR_TILE, next);
+                if (kk < R::PUTS) store(buf ^ 1, kk, p0 + PR_TILE, next);
                 __builtin_amdgcn_sched_barrier(0);
             }
             load(p0 + 2 * PR_TILE, after);
