@@ -725,10 +725,11 @@ class PagedCache:
     A serving step: ``fork`` (beams, ended requests), ``extend`` (room for the
     new tokens), then for every layer ``append_d`` and ``attention_d`` of the
     packed rows. ``dtype`` KV_Q8 holds a byte for each number and a scale for each
-    128; ``read`` gives them back. ``fork``, ``extend`` and ``compact`` take and return host values
-    and wait for the context's stream. The calls whose names end in _d take device
-    buffers, are only enqueued and can be captured in a graph: ``fork_d``,
-    ``extend_d`` (the statuses stay in ``status``), ``append_d``, ``attention_d``.
+    128; ``read`` gives them back. ``fork``, ``extend`` and ``compact`` take and return
+    host values and wait for the context's stream. The calls whose names end in _d take
+    device buffers, are only enqueued and can be captured in a graph: ``fork_d``,
+    ``extend_d`` (the statuses stay in ``status``), ``append_d``, ``share_d``,
+    ``attention_d``, ``read_d``.
     A fork leaves ``table`` and ``len`` in a second pair of buffers, the extension
     after it (or a second fork) brings them back, and a captured graph keeps the
     buffers of its capture: capture every fork with its extension, and replay after
@@ -756,7 +757,7 @@ class PagedCache:
         self._rows_len = self.len  # the lengths that append and attention go by
         self._live = ctx.empty(1, np.int32)
         self._scratch = ctx.empty(lib().hyq_pages_scratch_bytes(self._kl), np.uint8)
-        self._attention, self._plans, self._planned = [], [], None
+        self._attention, self._plans, self._planned = [], {}, None
 
     def _slots(self, values, into: DeviceArray) -> int:
         a = np.ascontiguousarray(values, np.int32)
@@ -850,10 +851,12 @@ class PagedCache:
                 least: int | None = None) -> None:
         """hyq_paged_shared_plan_d: finds the prefixes that slots share, for the
         ``attention_d`` calls with ``shared`` until the next fork, extension or
-        compaction; with ``least``, hyq_paged_shared_plan_least_d. Its buffer grows as
-        attention_d's."""
+        compaction; with ``least``, hyq_paged_shared_plan_least_d. The plan of a number
+        of heads has one buffer, which a captured graph keeps and the next plan takes,
+        a replayed graph's too: capture attention with its share_d, and after a replay
+        call share_d again before attention outside the graph."""
         need = lib().hyq_paged_shared_plan_bytes(self._kl, rows, heads)
-        plan = self._grown(self._plans, need)
+        plan = self._grown(self._plans.setdefault(heads, []), need)
         args = [self.ctx.handle, self._kl, group_d, self.table.ptr, self._rows_len.ptr, start_d,
                 rows, heads]
         if least is None:
@@ -877,7 +880,7 @@ class PagedCache:
         args = [self.ctx.handle, self._kl, self.pool.ptr, layer, self.table.ptr,
                 self._rows_len.ptr, start_d, rows, max_rows, heads]
         if shared:
-            plan = self._plans[-1]
+            plan = self._plans[heads][-1]
             check(lib().hyq_paged_shared_attention_d(*args, plan.ptr, plan.nbytes, q_d,
                                                      scratch.ptr, scratch.nbytes, out_d))
         else:

@@ -447,3 +447,35 @@ def test_captured(gpu_ctx, hyq):
             ok(hip("hipGraphDestroy")(graph))
     finally:
         other.close()
+
+
+def test_a_captured_attention_keeps_its_plan(gpu_ctx, hyq):
+    """Attention captured without its plan goes by the plan that is made before each
+    replay, also after one of another number of heads, whose buffer is larger."""
+    c = hyq.PagedCache(gpu_ctx, 1, 2, 64, 4, 200, page_tokens=16)
+    c.pool.copy_from(np.random.default_rng(19).integers(0, 40, c.pool.shape).astype(np.uint8))
+    start = gpu_ctx.array(np.arange(5, dtype=np.int32))
+    q = gpu_ctx.array(np.random.default_rng(20).normal(0, 1, (4, 16, D)).astype(np.float32))
+    outs = [gpu_ctx.array(np.full((4, 16, D), -7, np.float32)) for _ in range(3)]
+    assert not c.extend([75, 0, 0, 0]).any()
+    c.fork([0, 0, 0, 0])
+    assert not c.extend([1, 1, 1, 1]).any()
+
+    def attend(out, **kw):
+        c.attention_d(0, start.ptr, 4, 1, 16, q.ptr, out.ptr, **kw)
+
+    c.share_d(start.ptr, 4, 16, least=0)
+    attend(outs[0], shared=True)
+    graph, run = captured(gpu_ctx, lambda: attend(outs[0], shared=True))
+    c.share_d(start.ptr, 4, 2, least=0)
+    for i in range(3):
+        assert not c.extend([1 + 20 * i, 2, 1, 3]).any()
+        c.share_d(start.ptr, 4, 16, least=0)
+        ok(hip("hipGraphLaunch")(run, ctypes.c_void_p(gpu_ctx.stream)))
+        attend(outs[1], shared=True)
+        attend(outs[2])
+        a, b, plain = (o.numpy() for o in outs)
+        assert np.array_equal(a, b)
+        assert np.abs(a - plain).max() <= 2e-5 * np.abs(plain).max()
+    ok(hip("hipGraphExecDestroy")(run))
+    ok(hip("hipGraphDestroy")(graph))
