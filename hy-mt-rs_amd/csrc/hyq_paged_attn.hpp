@@ -393,7 +393,10 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 // leave parts that the merge joins with the slots' own. The plan lists the pieces of
 // both forms, one of a block or a slot and of one KV head for a worker of the few-row
 // form.
-constexpr int FEW_PIECES = 2048; // two waves on each SIMD
+// Two waves on each SIMD. The few-row form's launch beside 64 slots that share 8192
+// positions of f16 pages, and beside four groups of 24 that share 3100 of 8-bit ones, us:
+// 25 and 41 with 1024, 19 and 38 with 1536, 18 and 31 with 2048, 22 and 36 with 3072.
+constexpr int FEW_PIECES = 2048;
 // (a slot and KV head has a piece at least)
 inline int shared_cap(int seqs)
 {
@@ -408,8 +411,8 @@ inline int few_most(int seqs, int kvh)
 }
 struct SharedPlace {
     int begin, n;     // the slot's rows (n = 0: not of the few-row form)
-    int part, pieces; // of its block (0 pieces: in no group); narrow: its first worker and
-                      // its workers for each KV head
+    int part, pieces; // of its block (0 pieces: in no group); narrow: the block's first
+                      // worker and its workers for each KV head
     int row;          // the slot's first row there
     int first, ways;  // its first worker, and its workers for each KV head
     int unused;

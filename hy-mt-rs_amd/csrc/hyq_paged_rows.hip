@@ -43,7 +43,7 @@
 // loads that wait for each other), the merge 5. The same over 8-bit pages: this
 // launch 31. Three prompts of up to 400 beside 27 sessions of up to 4000 positions,
 // 32 heads over 8: 114 us over 8-bit pages, of which MFMAs are 30 % and VALU work
-// 33 % (106 over f16 ones: the codes' conversion and the scales are the difference;
+// 35 % (106 over f16 ones: the codes' conversion and the scales are the difference;
 // scores by products of whole numbers would save the keys' conversion and take as
 // much for the queries' third part). A prefix of 8192 positions for 64 slots of four
 // rows, 32 heads over 8, f16 pages: 29 us; four of 3100 for 24 slots of three tokens

@@ -9,7 +9,10 @@
 // slot's place follows from the slots before it, so the plan does not depend on
 // the order in which threads run.
 //
-// Bound by loads that wait for each other: once a step, not a layer.
+// Bound by loads that wait for each other and by barriers: 14 us for eight slots, 18 for
+// 64, 20 for 105, once a step, not a layer. What a layer then takes, with the plan's share
+// of one of two, and without sharing: 64 slots over 8200 positions in common and 300 of
+// their own, 32 heads over 8, f16 pages, 61 and 146 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -169,10 +172,10 @@ struct PlanLds {
 };
 
 // PLAN_GROUPS workgroups, each of which makes the whole plan for itself; the first
-// one writes it, but for the few-row form's pieces, of which each writes some (2048
-// of them by one workgroup: 6 us of 15). Their time is that of their barriers and of
-// their code, which they find in no cache: what they need is read once, numbers are
-// 32 bits, and few loops are unrolled.
+// one writes it, but for the few-row form's pieces, of which each writes some (64 slots
+// 14.3 us, and 15.4 where one workgroup wrote them all; 105 slots 16.5 and 17.9). Their
+// time is that of their barriers and of their code, which they find in no cache: what
+// they need is read once, numbers are 32 bits, and few loops are unrolled.
 constexpr int PLAN_GROUPS = 8;
 // The tiles of narrow blocks, over all KV heads, up to which they take less time than
 // the tile form, in steps of 16 positions, and of 32 in 8-bit pages. Narrow and wide,
@@ -251,7 +254,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
     for (int s = t; s < n; s += 1024)
         if (x.first[s]) {
             const int each = few / x.wide[s], mine = pieces_of(x.first[s], each);
-            atomicAdd(&sum[4], min((unsigned)mine * (unsigned)tiles(x.pages[s] << kv.shift), 1u << 20));
+            atomicAdd(&sum[4],
+                      min((unsigned)mine * (unsigned)tiles(x.pages[s] << kv.shift), 1u << 20));
             atomicAdd(&sum[5], (unsigned)mine);
         }
     __syncthreads();
@@ -347,7 +351,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
     // so long that they number FEW_PIECES at most (or half as many beside a piece for
     // each slot and head, where those are many).
     const int head = FEW_PIECES / kv.kvh; // pieces of a KV head
-    const unsigned units = sum[2] + (narrow ? sum[5] : 0), all_tiles = sum[1] + (narrow ? sum[4] : 0);
+    const unsigned units = sum[2] + (narrow ? sum[5] : 0);
+    const unsigned all_tiles = sum[1] + (narrow ? sum[4] : 0);
     const int spread = max(head - (int)units, head / 2);
     const int piece = max(1, pieces_of((int)min(all_tiles, 0x7fff0000u), spread));
     int workers = 0;
@@ -387,10 +392,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
 #pragma unroll 1
     for (int w = blockIdx.x * 256 + t; t < 256 && w < workers; w += PLAN_GROUPS * 256) {
         if (w < of_blocks) {
-            const int b = last_of(x.part, blocks, w), s = x.of[b], ways = pieces_of((int)x.steps[b], piece);
+            const int b = last_of(x.part, blocks, w), s = x.of[b];
+            const int ways = pieces_of((int)x.steps[b], piece);
             const int kh = (int)((unsigned)(w - x.part[b]) / (unsigned)ways);
             const int2 by = share((int)x.steps[b], w - x.part[b] - kh * ways, ways);
-            sp.few[w] = FewPiece{s, kh, by.x, by.y, b * tq, x.toks[b], x.pages[s] << kv.shift, 0, ways, 1, {}};
+            sp.few[w] = FewPiece{s,         kh,        by.x, by.y, b * tq, x.toks[b],
+                                 x.pages[s] << kv.shift, 0,    ways, 1,      {}};
             continue;
         }
         const int s = last_of(x.first, n, w), ways = max(1, x.ways[s]); // (a slot that has pieces)

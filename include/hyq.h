@@ -372,8 +372,9 @@ int hyq_argmax_d(hyq_ctx *ctx, const float *x_d, size_t n, float *scratch_d, int
  * the kernels check every id and bound, so a wrong one makes wrong or missing
  * results but no access outside the buffers given. Pools, rows and scratch
  * must be 16-byte aligned. Calls that overlap in time (two contexts, two
- * captured graphs replayed at once) need scratch of their own. Every call can
- * be captured in a HIP graph: none allocates, copies to the host or waits. */
+ * captured graphs replayed at once) need scratch, and plans that are made in
+ * them, of their own. Every call can be captured in a HIP graph: none allocates,
+ * copies to the host or waits. */
 enum { HYQ_KV_Q8 = 1008 }; /* of pools alone: no format of a file or weight */
 typedef struct {
     int dtype;       /* HYQ_F32, HYQ_F16 or HYQ_KV_Q8: element type of the pool */
@@ -396,10 +397,11 @@ size_t hyq_kv_pool_bytes(const hyq_kv_layout *kl);
  * F16 pool holds the values rounded once, to nearest. An HYQ_KV_Q8 pool holds the
  * 128 numbers x of a position and head as scale = max |x| / 127 in f32 and codes
  * rint(x / scale), off by at most half a scale; one that is not finite makes the
- * scale, and with it the head, a NaN. Such keys are formed in 64 bits. The angle position * freq_d[j] is taken in 64
- * bits, where hyq_rope_norm_append_d rounds the product to 32 (the reference's
- * table, src/model.rs:919-925): the two differ by up to position * 2^-24
- * radians times the frequency, and agree where the product is exact. */
+ * scale, and with it the head, a NaN. Such keys are formed in 64 bits. The angle
+ * position * freq_d[j] is taken in 64 bits, where hyq_rope_norm_append_d rounds the
+ * product to 32 (the reference's table, src/model.rs:919-925): the two differ by
+ * up to position * 2^-24 radians times the frequency, and agree where the product
+ * is exact. */
 int hyq_paged_rope_norm_append_d(hyq_ctx *ctx, const hyq_kv_layout *kl, void *pool_d, int layer,
                                  const int32_t *table_d, const int32_t *len_d,
                                  const int32_t *start_d, size_t rows, size_t heads,
@@ -424,10 +426,10 @@ int hyq_paged_read_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, 
  * finite in any form, makes its dim of the rows that see it not finite (such a
  * key the whole of those rows), and changes no other row. An HYQ_KV_Q8 pool has
  * no such limit: its codes enter the products exactly, queries to 22 bits of the
- * row's largest, values to 2^-31 of the largest that the row sees (each). What places hold that
- * no position uses (a page's rest, pages never written) is never part of a
- * result. out_d must not be q_d. scratch_d: hyq_paged_attention_scratch_bytes
- * bytes (0 for arguments that the call refuses). */
+ * row's largest, values to 2^-31 of the largest that the row sees (each) or of
+ * 2^-81, the larger. What places hold that no position uses (a page's rest, pages
+ * never written) is never part of a result. out_d must not be q_d. scratch_d:
+ * hyq_paged_attention_scratch_bytes bytes (0 for arguments that the call refuses). */
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,
                                          size_t heads);
 int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, int layer,
@@ -448,7 +450,8 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
  * pages as save the most: pages in common, times the slots but one that have them.
  * Where all groups together save less than sharing costs (about 50,000 positions
  * times KV heads, 120,000 in an HYQ_KV_Q8 pool) nothing is shared;
- * hyq_paged_shared_plan_least_d takes that number from the caller (0: whatever it saves).
+ * hyq_paged_shared_plan_least_d takes that number from the caller (0: whatever it
+ * saves).
  * (Ids are compared, not assumed: a wrong group costs time, no result.) The plan
  * goes by the table, lengths and starts as they are, and holds for attention calls
  * with the same ones, layout, rows and heads; with others the results are wrong,
