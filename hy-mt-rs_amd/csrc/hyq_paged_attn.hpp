@@ -395,7 +395,7 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 // form.
 // Two waves on each SIMD. The few-row form's launch beside 64 slots that share 8192
 // positions of f16 pages, and beside four groups of 24 that share 3100 of 8-bit ones, us:
-// 25 and 41 with 1024, 19 and 38 with 1536, 18 and 31 with 2048, 22 and 36 with 3072.
+// 25 and 41 with 1024, 19 and 38 with 1536, 18 and 31 with 2048, 22 and 36 with three waves.
 constexpr int FEW_PIECES = 2048;
 // (a slot and KV head has a piece at least)
 inline int shared_cap(int seqs)

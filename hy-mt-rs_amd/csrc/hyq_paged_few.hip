@@ -658,7 +658,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedKv kv, int few_ro
 // f16 pages: 184 us with 1024, 143 with 2048, 149 with 3072; four of up to 60001
 // in f32 pages: 105 with 1024, 113 with 2048). Numbers between leave SIMDs
 // unequal: 165 with 1536 in f16 pages, 146 with 1280 in f32 ones. 8-bit pages as f16
-// ones: 64 sessions 86 with 2048, 100 with 1536, 105 with 2560, 108 with 3072.
+// ones: 64 sessions 86 with 2048, 100 with 1536, 105 with 2560, 108 with three waves.
 int few_workers(int type) { return type == KV_T_F32 ? 1024 : 2048; }
 
 } // namespace
