@@ -473,7 +473,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_kern
     }
 }
 
-// ROWS rows' parts p, p + step, ..., n of each, eight in flight in all: the
+// ROWS rows' parts, part(r, 0 .. n - 1) of each, eight in flight in all: the
 // running maxima m, exp-sums l and a lane's sums x.
 template <class V, int ROWS> struct Joined {
     float m[ROWS], l[ROWS];
@@ -487,7 +487,7 @@ template <class V, int ROWS> struct Joined {
             x[r] = V{};
         }
     }
-    __device__ __forceinline__ void add(const float *const (&p)[ROWS], size_t step, int n, int d)
+    template <class F> __device__ __forceinline__ void add(F part, int n, int d)
     {
         constexpr int DEPTH = 8 / ROWS;
         for (int b = 0; b < n; b += DEPTH) {
@@ -497,7 +497,7 @@ template <class V, int ROWS> struct Joined {
             for (int r = 0; r < ROWS; ++r)
 #pragma unroll
                 for (int k = 0; k < DEPTH; ++k) {
-                    const float *o = p[r] + (size_t)min(b + k, n - 1) * step;
+                    const float *o = part(r, min(b + k, n - 1));
                     ml[r][k] = *reinterpret_cast<const float2v *>(o);
                     v[r][k] = *reinterpret_cast<const V *>(o + 4 + d);
                 }
@@ -572,15 +572,18 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     const float *p = part + ((size_t)slot * part_rows + r) * PAGED_PART;
     const int a = wide ? n * g / 4 : 0, b = wide ? n * (g + 1) / 4 : n;
     Joined<float2v, 1> j;
-    j.add({p + (size_t)a * step}, step, b - a, 2 * lane);
-    if constexpr (SHARED) { // the prefix's pieces, for this row of its block
+    if constexpr (!SHARED) {
+        j.add([&](int, int i) { return p + (size_t)(a + i) * step; }, b - a, 2 * lane);
+    } else { // and the prefix's pieces, for this row of its block, in flight with them
         const int c0 = wide ? pl.pieces * g / 4 : 0, c1 = wide ? pl.pieces * (g + 1) / 4 : pl.pieces;
         const int last = narrow ? part_rows - 1 : PR_ROWS - 1;
         const size_t each = narrow ? step : (size_t)kv.kvh * PR_ROWS * PAGED_PART;
         const float *x = narrow ? part + (size_t)pl.part * each
                                 : prefix + ((size_t)pl.part * kv.kvh + kh) * PR_ROWS * PAGED_PART;
         x += (size_t)min(min(max(pl.row, 0), last) + r, last) * PAGED_PART;
-        j.add({x + (size_t)c0 * each}, each, c1 - c0, 2 * lane);
+        j.add([&](int, int i) {
+            return i < b - a ? p + (size_t)(a + i) * step : x + (size_t)(c0 + i - (b - a)) * each;
+        }, b - a + c1 - c0, 2 * lane);
     }
     float *o = out + ((size_t)(sr.begin + r / rep) * kv.heads + kh * rep + r % rep) * KV_D;
     if (!wide) {
@@ -620,7 +623,8 @@ __device__ __forceinline__ void merge_rows(const PagedKv &kv, const RowsScratch 
     if (r / rep >= blk.toks) return;
     const float *p = rs.parts + (((size_t)blk.part * kv.kvh + kh) * PR_ROWS + r) * PAGED_PART;
     Joined<f32x4, 2> j; // (a row past the block's is not stored)
-    j.add({p, p + 8 * PAGED_PART}, (size_t)kv.kvh * PR_ROWS * PAGED_PART, blk.pieces, d);
+    const size_t step = (size_t)kv.kvh * PR_ROWS * PAGED_PART;
+    j.add([&](int i, int k) { return p + 8 * PAGED_PART * i + k * step; }, blk.pieces, d);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int at = r + 8 * i, tl = at / rep;
