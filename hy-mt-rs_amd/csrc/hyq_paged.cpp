@@ -275,12 +275,11 @@ int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t
                             size_t rows, size_t heads, void *plan_d, size_t plan_bytes)
 {
     // What sharing has to save to be worth its parts, in positions times KV heads. One
-    // group of slots before 256 to 4096 common positions and some 50 of their own,
-    // shared and not, us, at 16 heads over 4 and 32 over 8: f16 pages 15 and 14 at
-    // 15,000, 17 and 18 at 32,000, 20 and 20 at 57,000, 21 and 24 at 125,000; f32 17 and
-    // 16 at 28,000, 19 and 21 at 63,000, 22 and 30 at 98,000; 8-bit ones, whose reads
-    // are cheaper, 18 and 19 at 63,000, 21 and 20 at 120,000, 22 and 23 at 237,000.
-    const long long least = kl && kl->dtype == HYQ_KV_Q8 ? 120000 : 50000;
+    // group of slots before 600 to 6000 common positions and some 60 of their own, 16
+    // heads over 4, us a layer, shared and not: 8-bit pages 12.8 and 12.4 at 16,800, 13.8
+    // and 14.5 at 42,000, 14.9 and 16.2 at 60,000; f16 13.5 and 13.4, 16.9 and 18.4, 17.1
+    // and 19.0; f32 13.3 and 13.9, 17.0 and 17.0, 17.0 and 19.3.
+    constexpr long long least = 25000;
     return shared_plan(ctx, kl, group_d, table_d, len_d, start_d, rows, heads, least, plan_d,
                        plan_bytes);
 }

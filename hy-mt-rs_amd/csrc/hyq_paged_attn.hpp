@@ -393,10 +393,16 @@ __device__ __forceinline__ void rows_plan(const PagedKv &kv, int few_rows, const
 // leave parts that the merge joins with the slots' own. The plan lists the pieces of
 // both forms, one of a block or a slot and of one KV head for a worker of the few-row
 // form.
-// Two waves on each SIMD. The few-row form's launch beside 64 slots that share 8192
-// positions of f16 pages, and beside four groups of 24 that share 3100 of 8-bit ones, us:
-// 25 and 41 with 1024, 19 and 38 with 1536, 18 and 31 with 2048, 22 and 36 with three waves.
+// Two waves on each SIMD, and one for f32 pages. The few-row form's launch beside 64 slots
+// that share 8192 positions of f16 pages, and beside four groups of 24 that share 3100 of
+// 8-bit ones, us: 25 and 41 with 1024, 19 and 38 with 1536, 18 and 31 with 2048, 22 and 36
+// with three waves. Four layers of eight slots over 3000 positions, of f32 pages, 117 us
+// with 2048 and 92 with 1024.
 constexpr int FEW_PIECES = 2048;
+__host__ __device__ inline int few_pieces(int type)
+{
+    return type == KV_T_F32 ? FEW_PIECES / 2 : FEW_PIECES;
+}
 // (a slot and KV head has a piece at least)
 inline int shared_cap(int seqs)
 {

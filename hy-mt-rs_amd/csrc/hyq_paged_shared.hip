@@ -178,11 +178,15 @@ struct PlanLds {
 // they need is read once, numbers are 32 bits, and few loops are unrolled.
 constexpr int PLAN_GROUPS = 8;
 // The tiles of narrow blocks, over all KV heads, up to which they take less time than
-// the tile form, in steps of 16 positions, and of 32 in 8-bit pages. Narrow and wide,
-// us, 16 heads over 4: f16 pages at 2048 tiles 21 and 23, at 4096 27 and 27, at 8192
-// 31 and 27; f32 ones at 2048 23 and 26, 4096 28 and 28, 8192 34 and 29; 8-bit ones at
-// 8192 30 and 33, 16384 38 and 36, 32768 52 and 44.
-constexpr int NARROW_TILES = 4096, NARROW_TILES_Q8 = 12288;
+// the tile form, in steps of 16 positions, and of 32 in 8-bit pages. Narrow and wide, us
+// a layer, 16 heads over 4 and 32 over 8: f16 pages at 3008 tiles 22.0 and 24.9, at 4000
+// 27.7 and 26.3, at 8064 33.2 and 30.9; f32 ones at 4000 24.0 and 28.8, 6016 27.4 and
+// 29.6, 8032 31.5 and 31.6, 16000 55.9 and 38.2; 8-bit ones at 4096 26.7 and 29.1, 8064
+// 32.4 and 32.6, 16000 41.7 and 38.1.
+__device__ __forceinline__ int most_narrow_tiles(int type)
+{
+    return type == KV_T_Q8 ? 8192 : type == KV_T_F16 ? 3500 : 6500;
+}
 __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
                                                            long long worth, SharedPlan sp)
 {
@@ -259,7 +263,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
             atomicAdd(&sum[5], (unsigned)mine);
         }
     __syncthreads();
-    const int most_narrow = kv.type == KV_T_Q8 ? NARROW_TILES_Q8 : NARROW_TILES;
+    const int most_narrow = most_narrow_tiles(kv.type);
     const bool narrow = (long long)sum[4] * kv.kvh <= most_narrow && (int)sum[5] <= sp.cap;
     const int tq = narrow ? few : sp.tq;
     int blocks = 0;
@@ -347,14 +351,32 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
     } else {
         __syncthreads();
     }
-    // The slots' own positions, by the few-row form: pieces of at most `piece` tiles,
-    // so long that they number FEW_PIECES at most (or half as many beside a piece for
-    // each slot and head, where those are many).
-    const int head = FEW_PIECES / kv.kvh; // pieces of a KV head
+    // The slots' own positions, by the few-row form: pieces of at most `piece` tiles, so
+    // long that they number as many as few_pieces says. (Each slot's and block's last one
+    // is shorter; the matrix unit bounds f32 pages, whose pieces are cut as if there were
+    // none. Others, 32 heads over 8, us for two layers in f16 pages of 128 slots over
+    // 2000 positions in common and 500 of their own, and of four groups in 8-bit ones:
+    // 287 and 176 with half the number at least, 272 and 176 with 5/8, 265 and 176 with
+    // 11/16, 264 and 178 with 3/4.)
+    const int head = few_pieces(kv.type) / kv.kvh; // of a KV head
     const unsigned units = sum[2] + (narrow ? sum[5] : 0);
     const unsigned all_tiles = sum[1] + (narrow ? sum[4] : 0);
-    const int spread = max(head - (int)units, head / 2);
-    const int piece = max(1, pieces_of((int)min(all_tiles, 0x7fff0000u), spread));
+    const int spread = kv.type == KV_T_F32 ? head : max(head - (int)units, head * 11 / 16);
+    // (The merge waits for a row's parts: where blocks are narrow, pieces are no shorter
+    // than about the root of a 24th of the longest one's tiles. Eight slots over 600, 1500
+    // and 3000 positions in common, 16 heads over 4, us a layer with pieces of 1, 2, 3, 4
+    // and 6 tiles at least: f16 pages 14.1 13.5 14.7 16.4 18.3, 18.2 16.1 16.9 17.2 18.0,
+    // 27.1 21.0 19.3 19.0 20.5; 32 slots over 1000 23.3 23.1 19.9 19.9 21.8.)
+    int least = 1;
+    if (narrow) {
+        int longest = 0;
+#pragma unroll 1
+        for (int b = lane; b < blocks; b += 64) longest = max(longest, (int)x.steps[b]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+        least = longest <= 16 ? 1 : longest <= 48 ? 2 : longest <= 128 ? 3 : 4;
+    }
+    const int piece = max(least, pieces_of((int)min(all_tiles, 0x7fff0000u), spread));
     int workers = 0;
     if (narrow) {
 #pragma unroll 1

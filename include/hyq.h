@@ -448,10 +448,9 @@ int hyq_paged_attention_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *poo
  * at most 16 * kv_heads / heads new rows, and at least a page of positions before
  * them. They are compared with the first of them, and the prefix is as many whole
  * pages as save the most: pages in common, times the slots but one that have them.
- * Where all groups together save less than sharing costs (about 50,000 positions
- * times KV heads, 120,000 in an HYQ_KV_Q8 pool) nothing is shared;
- * hyq_paged_shared_plan_least_d takes that number from the caller (0: whatever it
- * saves).
+ * Where all groups together save less than sharing costs (about 25,000 positions
+ * times KV heads) nothing is shared; hyq_paged_shared_plan_least_d takes that number
+ * from the caller (0: whatever it saves).
  * (Ids are compared, not assumed: a wrong group costs time, no result.) The plan
  * goes by the table, lengths and starts as they are, and holds for attention calls
  * with the same ones, layout, rows and heads; with others the results are wrong,

@@ -181,7 +181,7 @@ def test_prefixes_of_many_tiles(gpu_ctx, hyq, pt, heads, kind):
     one of a prefix that is no whole steps, with slots beside them."""
     r = np.random.default_rng(pt)
     kvh = heads[1]
-    most = {"Q8": 12288 * 32}.get(kind, 4096 * 16)
+    most = {"Q8": 12288 * 32, "F32": 6500 * 16}.get(kind, 4096 * 16)
     few = 16 // (heads[0] // heads[1])
     news = np.where(np.arange(75) % 9 == 8, 0, r.integers(1, 3, 75))
     blocks = -(-int((news[:60] > 0).sum()) // (few // 2))  # of 16 rows, of the larger group
@@ -221,7 +221,7 @@ def test_the_prefix_that_saves_most(gpu_ctx, hyq, kind):
     check(b, c.attend())
 
 
-@pytest.mark.parametrize("kind,least", [("F32", 50000), ("F16", 50000), ("Q8", 120000)])
+@pytest.mark.parametrize("kind,least", [(k, 25000) for k in KINDS])
 def test_what_is_worth_sharing(gpu_ctx, hyq, kind, least):
     """Nothing is shared where all groups together save less than the given number, or
     the rule's; the results are the same but for rounding."""
