@@ -9,10 +9,9 @@
 // slot's place follows from the slots before it, so the plan does not depend on
 // the order in which threads run.
 //
-// Bound by loads that wait for each other and by barriers: 14 us for eight slots, 18 for
-// 64, 20 for 105, once a step, not a layer. What a layer then takes, with the plan's share
-// of one of two, and without sharing: 64 slots over 8200 positions in common and 300 of
-// their own, 32 heads over 8, f16 pages, 61 and 146 us.
+// Bound by loads that wait for each other and by barriers: 15 us for eight slots, 19 for
+// 64, 20 for 105, once a step, not a layer. A layer of 64 slots over 8200 positions in
+// common and 300 of their own, 32 heads over 8, f16 pages: 51 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
