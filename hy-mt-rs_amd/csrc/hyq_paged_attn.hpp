@@ -72,6 +72,36 @@ __device__ __forceinline__ void split2(float x, float y, half2 &hi, half2 &lo)
     lo = __builtin_convertvector((float2v{a, b}), half2);
 }
 
+// ---- scales of 8-bit values ----
+// A weight p and the scale b of its position become f16 parts of p b, over `top`, a
+// power of two above all scales b that the row has seen. Its logarithm is taken off
+// p's exponent, up to Q8_LOG_MOST: beyond it p would fall below f32's normal numbers,
+// where the exponential is zero (at 2^122 each weight below 2^-18 of the largest). The
+// rest is taken off b.
+constexpr float Q8_LOG_MOST = 32.f, Q8_MOST = 0x1p32f;
+// Partial rows hold weights of at most 2^-24, so that the sum of 2^24 positions'
+// values is not beyond the largest of them.
+constexpr float Q8_DOWN = 24.f;
+__device__ __forceinline__ float q8_rest(float top) { return fminf(Q8_MOST / top, 1.f); }
+// A new `top`, where a scale b passes the old one, and what the sums of weights and of
+// values over it are to be multiplied with.
+struct Q8Top {
+    float weights, sums;
+};
+__device__ __forceinline__ Q8Top q8_top(float b, float &top, float &log_top)
+{
+    Q8Top to{1.f, 1.f};
+    if (b > top) {
+        const unsigned up = (__builtin_bit_cast(unsigned, b) & 0x7f800000u) + 0x00800000u;
+        const float was = fminf(top, Q8_MOST);
+        to.sums = top / __builtin_bit_cast(float, up);
+        top = __builtin_bit_cast(float, up);
+        to.weights = was / fminf(top, Q8_MOST);
+        log_top = fminf((float)((int)(up >> 23) - 127), Q8_LOG_MOST);
+    }
+    return to;
+}
+
 // ---- the few-row form's plan ----
 constexpr int FEW_WAVES = 4;
 

@@ -21,7 +21,9 @@
 // codes into the low bytes of two halves, u 2^-24 as f16, which an fma makes
 // (u - 128) 2^-9. The weights' two f16 parts keep 22 bits: p lies up to 2^14 over
 // the power of two that passes all scales the row has seen, and p b below 2^14, so
-// that its error is at most 2^-39 of the largest.
+// that its error is at most 2^-39 of the largest. (Where the scales pass 2^32, p lies
+// over 2^32 and b is brought down by the rest: an exponential below f32's normal
+// numbers is zero, and so none above 2^-108 of the largest is.)
 //
 // Bound by memory, 264 bytes a position and head, and for few positions by loads that
 // wait for each other and the merge's launch. With the merge: 64 slots of up to 8192
@@ -213,7 +215,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
 #pragma unroll
         for (int x = 0; x < 8; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
         // m: the running maximum less LIFT; top: a power of two above all scales of
-        // values seen (not below 2^-88, that sums of weights over it be numbers)
+        // values seen (not below 2^-88, that sums of weights over it be numbers);
+        // log_top: its logarithm as it enters the weights (not above Q8_LOG_MOST)
         float m = -INFINITY, l = 0.f, top = 0x1p-88f, log_top = -88.f;
 
         const int *entries = kv.table + (size_t)s * kv.stride;
@@ -315,18 +318,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
                 bm = wave::max_halves(wave::max_rows2(bm));
                 const float mn = fmaxf(m, mx - LIFT);
                 if (__any(mn != m || bm > top)) {
-                    float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                    if (bm > top) { // (the power of two above bm)
-                        const unsigned up =
-                            (__builtin_bit_cast(unsigned, bm) & 0x7f800000u) + 0x00800000u;
-                        corr *= top / __builtin_bit_cast(float, up);
-                        top = __builtin_bit_cast(float, up);
-                        log_top = (float)((int)(up >> 23) - 127);
-                    }
+                    const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                    const Q8Top to = q8_top(bm, top, log_top);
+                    l = l * corr * to.weights; // (in turn: their product may be too small)
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) acc[x] *= corr;
-                    l *= corr;
+                    for (int x = 0; x < 8; ++x) acc[x] *= corr * to.sums;
                     m = mn;
+                }
+                if (__any(top > Q8_MOST)) { // (rare)
+                    const float rest = q8_rest(top);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[i] *= rest;
                 }
                 // a row that has seen nothing yet keeps zero weights
                 const float base = m == -INFINITY ? 0.f : m + log_top;
@@ -373,16 +375,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, SHARED ? 3 : 2) void paged_few_q8_k
         if (whole) {
             // (a row that saw nothing gives zeros)
             o = out + row * KV_D;
-            f = l > 0.f || l != l ? 512.f / l : 0.f;
+            f = l > 0.f || l != l ? 512.f / (l * q8_rest(top)) : 0.f;
         } else {
             const long long slot = SHARED ? w : (long long)w + (long long)s * kv.kvh + kh;
             o = part + ((size_t)slot * part_rows + c) * PAGED_PART;
-            if (ok && g == 0) { // (the maximum itself, and weights of at most 1)
-                o[0] = m + LIFT;
-                o[1] = l * (top * 0x1p-14f);
+            if (ok && g == 0) { // (weights of at most 2^-24, see Q8_DOWN)
+                o[0] = m + (LIFT + Q8_DOWN);
+                o[1] = l * (fminf(top, Q8_MOST) * 0x1p-38f);
             }
             o += 4;
-            f = top * 0x1p-5f;
+            f = top * 0x1p-29f;
         }
         if (ok) {
 #pragma unroll

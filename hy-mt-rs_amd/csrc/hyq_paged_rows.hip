@@ -22,7 +22,7 @@
 // each position of a head: codes go through both products, the scores are
 // multiplied with the keys' scales, and the weights with the values' before they
 // are split. Those are kept below 2^15 by weights that are smaller by a power of two
-// above all scales that the row has seen.
+// above all scales that the row has seen (and scales, where those pass 2^32).
 //
 // Keys and values go through LDS, two steps of them, rows as they are (values
 // are transposed by ds_read_b64_tr_b16 on their way to the matrix operand).
@@ -547,20 +547,15 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             if (__any(m_new > m_run + 8.f || (Q8 && most > top))) {
                 const float m = fmaxf(m_run, m_new);
                 float corr = m == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+                l_run *= corr;
                 if constexpr (Q8) {
                     float bmax = 0.f; // of the positions that the row sees
 #pragma unroll
                     for (int e = 0; e < 16; ++e) bmax = fmaxf(bmax, bs[e]);
-                    bmax = wave::max_halves(bmax);
-                    if (bmax > top) { // (the power of two above bmax)
-                        const unsigned up =
-                            (__builtin_bit_cast(unsigned, bmax) & 0x7f800000u) + 0x00800000u;
-                        corr *= top / __builtin_bit_cast(float, up);
-                        top = __builtin_bit_cast(float, up);
-                        log_top = (float)((int)(up >> 23) - 127);
-                    }
+                    const Q8Top to = q8_top(wave::max_halves(bmax), top, log_top);
+                    l_run *= to.weights;
+                    corr *= to.sums;
                 }
-                l_run *= corr;
 #pragma unroll
                 for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
@@ -577,6 +572,11 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             }
             l_run += rs[0] + rs[1];
             if constexpr (Q8) {
+                if (__any(top > Q8_MOST)) { // (rare)
+                    const float rest = q8_rest(top);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) bs[e] *= rest;
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sv[e] *= bs[e];
             }
@@ -633,13 +633,13 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             next = after;
             buf ^= 1;
         }
-        if constexpr (Q8) { // the sums themselves, of weights of at most 1
+        if constexpr (Q8) { // the sums themselves, of weights of at most 2^-24 (Q8_DOWN)
 #pragma unroll
             for (int j = 0; j < KV_D / 32; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[j][e] *= top * 0x1p-15f;
-            l_run *= top * 0x1p-15f;
-            m_run += 15.f;
+                for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * 0x1p-24f * (top * 0x1p-15f);
+            l_run = l_run * 0x1p-24f * (fminf(top, Q8_MOST) * 0x1p-15f);
+            m_run += 15.f + Q8_DOWN;
         }
         if (__syncthreads_or(odd)) {
             // the values left out, for the rows that see them: whatever its weight,

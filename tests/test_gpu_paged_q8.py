@@ -123,6 +123,69 @@ def test_sizes_of_queries_and_values(gpu_ctx, hyq, news, size):
     check(b, attention(hyq, gpu_ctx, b))
 
 
+def far(b, case):
+    """Values up to the ends of f32's range. small: as many weights of 2^-21 of the largest
+    as make 2^-10 of a sum, the largest one's values of the other sign; equal: equal
+    weights of values whose sum is beyond f32; jump: values below 2^-90, then far ones."""
+    b.codes[:, 0, ..., 1:] = 0  # (keys of one number)
+    b.codes[:, 0, ..., 0] = 0
+    b.scales[:, 0] = np.float32(2.0 ** -7)
+    b.codes[:, 1] = np.abs(b.codes[:, 1])
+    b.q[:] = 0
+    with np.errstate(invalid="ignore"):
+        b.scales[:, 1] = np.where(np.isnan(b.scales[:, 1]), np.nan, 2.6e36 if case == "equal" else 8e35)
+    if case == "small":
+        b.q[..., 0] = 21 * np.log(2.0) * np.sqrt(D) * 2.0 ** 7 / 127
+    for s in range(b.seqs):
+        at = np.arange(b.lens[s])
+        page, place = b.table[s, at // b.pt], at % b.pt
+        if case == "small":
+            x = (b.lens[s] - b.news[s]) // 2
+            b.codes[page[x], 0, :, place[x], 0] = 127
+            b.codes[page[x], 1, :, place[x]] *= -1
+        if case == "jump":
+            half = at < len(at) // 2
+            b.scales[page[half], 1, :, place[half]] = np.float32(2.0 ** -100)
+    b.bytes = Q.join(b.codes, b.scales)
+
+
+@pytest.mark.parametrize("case", ["small", "equal", "jump"])
+@pytest.mark.parametrize("news", [1, 40])
+def test_values_at_the_ends_of_the_range(gpu_ctx, hyq, news, case):
+    """Small weights of far values count, sums of many do not leave f32 and weights of
+    values before far ones stay, in slots that one worker takes and in cut ones."""
+    b = Q.BatchQ8([2100, 60 if news > 1 else 30, 700], [news, news, 2], 4, 2, 32, seed=14)
+    far(b, case)
+    check(b, attention(hyq, gpu_ctx, b))
+
+
+@pytest.mark.parametrize("case", ["small", "jump"])
+@pytest.mark.parametrize("news", [1, 40])
+def test_far_values_in_one_piece(gpu_ctx, hyq, news, case):
+    """The same where one wave or workgroup goes through all of a slot: in a batch that
+    gives each worker more tiles than the slot has, and one of more blocks than pieces.
+    (The other slots name the first one's pages, over and over.)"""
+    b = Q.BatchQ8([2100], [news], 4, 2, 32, seed=15)
+    far(b, case)
+    want, tol = b.attention()
+    seqs, pages = (21, 3600) if news == 1 else (200, b.width)
+    row = np.resize(b.table[0, :2100 // 32], pages).astype(np.int32)
+    b.table = np.concatenate([np.resize(b.table[0], (1, b.width))] * seqs) if news > 1 else (
+        np.concatenate([np.full((1, pages), -1, np.int32)] + [row[None]] * (seqs - 1)))
+    if news == 1:
+        b.table[0, :66] = Q.BatchQ8([2100], [news], 4, 2, 32, seed=15).table[0, :66]
+    b.seqs, b.width = seqs, pages
+    b.lens = np.full(seqs, 2100 if news > 1 else pages * 32, np.int32)
+    b.lens[0] = 2100
+    b.news = np.full(seqs, news, np.int32)
+    b.start = (np.arange(seqs + 1) * news).astype(np.int32)
+    b.q, b.rows = np.concatenate([b.q] * seqs), seqs * news
+    got = attention(hyq, gpu_ctx, b)
+    for s in range(seqs if news > 1 else 1):
+        err = np.abs(got[s * news:(s + 1) * news] - want).max(-1)
+        assert np.all(err <= tol), (s, (err / tol).max())
+
+
 @pytest.mark.parametrize("pt", [16, 64])
 @pytest.mark.parametrize("news", [3, 50])
 def test_missing_pages(gpu_ctx, hyq, news, pt):

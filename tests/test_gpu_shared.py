@@ -8,6 +8,7 @@ import pytest
 
 import paged_q8_ref as Q
 import paged_ref as R
+from test_gpu_paged_q8 import far
 from test_gpu_serving import captured, hip, ok
 
 pytestmark = pytest.mark.gpu
@@ -195,6 +196,40 @@ def test_prefixes_of_many_tiles(gpu_ctx, hyq, pt, heads, kind):
     assert np.array_equal(c.skips(), plain_skips(b))
     head = c.plan.numpy()[:16].view(np.int32)
     assert head[0] >= 2 and head[1] > head[0] and head[3] == 0  # blocks, their pieces, not narrow
+    check(b, c.attend())
+
+
+def alike(b, seqs, pages, seed):
+    """A batch of many slots of one new token that name the pages of b's only slot: the
+    first `pages` whole, and one to 30 positions of the next."""
+    r = np.random.default_rng(seed)
+    b.seqs, b.table = seqs, np.repeat(b.table, seqs, 0)
+    b.lens = (pages * b.pt + 1 + np.arange(seqs) % 30).astype(np.int32)
+    b.news = np.ones(seqs, np.int32)
+    b.start = np.arange(seqs + 1, dtype=np.int32)
+    b.new = b.rows = seqs
+    b.q = np.resize(b.q[0], (seqs, b.heads, D)) + r.normal(0, 0.5, (seqs, b.heads, D)).astype(
+        np.float32) * (np.abs(b.q[0]).max() > 0)
+    return b
+
+
+# tiles over all KV heads up to which blocks are narrow, and a tile's positions
+MOST_NARROW = {"F32": (6500, 16), "F16": (3500, 16), "Q8": (8192, 32)}
+
+
+@pytest.mark.parametrize("case", ["equal", "jump"])
+@pytest.mark.parametrize("over", [0, 1], ids=["narrow", "wide"])
+def test_far_values_in_a_prefix(gpu_ctx, hyq, over, case):
+    """8-bit values near the end of f32's range in narrow and in wide blocks, whose parts
+    are joined with the slots' own."""
+    most, tile = MOST_NARROW["Q8"]
+    pages = most // (15 * 2) + over  # 15 blocks of two slots, over two heads
+    b = Q.BatchQ8([pages * tile + 30], [1], 16, 2, tile, seed=21)
+    far(b, case)
+    b = alike(b, 30, pages, seed=22)
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.all(c.skips() == pages * tile)
+    assert c.plan.numpy()[:16].view(np.int32)[3] == 1 - over
     check(b, c.attend())
 
 
