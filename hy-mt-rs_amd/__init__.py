@@ -757,7 +757,7 @@ class PagedCache:
         self._rows_len = self.len  # the lengths that append and attention go by
         self._live = ctx.empty(1, np.int32)
         self._scratch = ctx.empty(lib().hyq_pages_scratch_bytes(self._kl), np.uint8)
-        self._attention, self._plans, self._planned = [], {}, None
+        self._attention, self._plans, self._planned = [], {}, {}  # (plans by heads)
 
     def _slots(self, values, into: DeviceArray) -> int:
         a = np.ascontiguousarray(values, np.int32)
@@ -779,7 +779,7 @@ class PagedCache:
                                      self.len.ptr, table.ptr, length.ptr, self.refs.ptr))
         self._other = (self.table, self.len)
         self.table, self.len = table, length
-        self._rows_len, self._planned = self.len, None
+        self._rows_len, self._planned = self.len, {}
 
     def extend(self, add) -> np.ndarray:
         """Room for add[s] more tokens; the slots' status (0 done, 1 no pages
@@ -798,7 +798,7 @@ class PagedCache:
         if self.table is not table:
             self._other = (self.table, self.len)
             self.table, self.len = table, length
-        self._rows_len, self._planned = self._served, None
+        self._rows_len, self._planned = self._served, {}
 
     def compact(self) -> int:
         """hyq_pages_compact_d: the pages in use become 0 .. live-1; live."""
@@ -806,7 +806,7 @@ class PagedCache:
             self.ctx.handle, self._kl, self.pool.ptr, self.table.ptr, self.refs.ptr,
             self.table.ptr, self.refs.ptr, self._live.ptr, self._scratch.ptr,
             self._scratch.nbytes))
-        self._planned = None
+        self._planned = {}
         return int(self._live.numpy()[0])
 
     def lengths(self) -> np.ndarray:
@@ -863,7 +863,7 @@ class PagedCache:
             check(lib().hyq_paged_shared_plan_d(*args, plan.ptr, plan.nbytes))
         else:
             check(lib().hyq_paged_shared_plan_least_d(*args, least, plan.ptr, plan.nbytes))
-        self._planned = (start_d, rows, heads)
+        self._planned[heads] = (start_d, rows)
 
     def attention_d(self, layer: int, start_d: int, rows: int, max_rows: int, heads: int,
                     q_d: int, out_d: int, shared: bool = False) -> None:
@@ -872,7 +872,7 @@ class PagedCache:
         with the largest call, at least twofold; the smaller ones live as long as the
         cache, since a captured graph may hold them. (A capture allocates
         nothing: run the largest call once before it.)"""
-        if shared and self._planned != (start_d, rows, heads):
+        if shared and self._planned.get(heads) != (start_d, rows):
             raise ValueError("no plan of these rows: share_d comes first, after a step's pages")
         size = (lib().hyq_paged_shared_attention_scratch_bytes if shared else
                 lib().hyq_paged_attention_scratch_bytes)

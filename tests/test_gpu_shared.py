@@ -514,3 +514,34 @@ def test_a_captured_attention_keeps_its_plan(gpu_ctx, hyq):
         assert np.abs(a - plain).max() <= 2e-5 * np.abs(plain).max()
     ok(hip("hipGraphExecDestroy")(run))
     ok(hip("hipGraphDestroy")(graph))
+
+
+def test_plans_of_two_numbers_of_heads(gpu_ctx, hyq):
+    """Each number of heads keeps its plan until the next step's pages, whichever was
+    made last; a plan of other rows takes the place of the one before."""
+    c = hyq.PagedCache(gpu_ctx, 1, 2, 64, 4, 200, page_tokens=16)
+    c.pool.copy_from(np.random.default_rng(23).integers(0, 40, c.pool.shape).astype(np.uint8))
+    start, other = (gpu_ctx.array(np.arange(5, dtype=np.int32)) for _ in range(2))
+    q = gpu_ctx.array(np.random.default_rng(24).normal(0, 1, (4, 16, D)).astype(np.float32))
+    outs = [gpu_ctx.array(np.full((4, 16, D), -7, np.float32)) for _ in range(2)]
+    assert not c.extend([75, 0, 0, 0]).any()
+    c.fork([0, 0, 0, 0])
+    assert not c.extend([1, 1, 1, 1]).any()
+    for heads in (16, 2):
+        c.share_d(start.ptr, 4, heads, least=0)
+    for heads in (16, 2, 16):
+        for out, shared in zip(outs, (True, False)):
+            c.attention_d(0, start.ptr, 4, 1, heads, q.ptr, out.ptr, shared=shared)
+        a, b = (o.numpy().ravel()[:4 * heads * D] for o in outs)
+        assert np.abs(a - b).max() <= 2e-5 * np.abs(b).max()
+    c.share_d(other.ptr, 4, 16, least=0)
+    attend = lambda at, heads: c.attention_d(0, at.ptr, 4, 1, heads, q.ptr, outs[0].ptr,
+                                             shared=True)
+    attend(other, 16)
+    attend(start, 2)
+    with pytest.raises(ValueError, match="share_d"):
+        attend(start, 16)
+    assert not c.extend([1, 1, 1, 1]).any()
+    for at, heads in ((other, 16), (start, 2)):
+        with pytest.raises(ValueError, match="share_d"):
+            attend(at, heads)
