@@ -832,7 +832,7 @@ class PagedCache:
         ``DenseDecoder.load_kv`` takes."""
         start = np.concatenate([[0], np.cumsum(self.lengths(), dtype=np.int64)])
         rows, width = int(start[-1]), self.layout.kv_heads * self.layout.head_dim
-        if rows >= 1 << 20:
+        if rows > 1 << 20:
             raise ValueError("more than 2^20 positions: read them in parts (read_d)")
         at = self.ctx.array(start.astype(np.int32))
         k, v = (self.ctx.empty((max(rows, 1), width), np.float32) for _ in range(2))

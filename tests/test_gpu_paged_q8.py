@@ -364,6 +364,21 @@ def test_read(gpu_ctx, hyq, kvh, pt, dtype):
                                          ld.ptr, sd.ptr, 0, k.ptr, v.ptr))  # no rows: nothing
 
 
+def test_cache_reads_as_many_rows_as_a_call_takes(gpu_ctx, hyq):
+    """2^20 positions at once; one more are to be read in parts."""
+    c = hyq.PagedCache(gpu_ctx, 1, 1, 4097, 2, 1 << 20, page_tokens=256, dtype=hyq.F16)
+    page = np.random.default_rng(25).normal(0, 1, (2, 256, D)).astype(np.float16)
+    c.pool.copy_from(np.resize(page.view(np.uint8), c.pool.shape))
+    assert not c.extend([1 << 20, 0]).any()
+    k, v = c.read(0)[0]
+    for got, want in ((k, page[0]), (v, page[1])):
+        assert got.shape == (1 << 20, D)
+        assert np.array_equal(got[:256], want) and np.array_equal(got[-256:], want)
+    assert not c.extend([0, 1]).any()
+    with pytest.raises(ValueError, match="parts"):
+        c.read(0)
+
+
 # ---- the pages' bookkeeping ----
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layers,kvh,pt", [(2, 1, 16), (1, 3, 64), (3, 2, 256)])
