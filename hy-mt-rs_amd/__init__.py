@@ -904,6 +904,10 @@ def adjust_logits(ctx: "Context", logits: np.ndarray, history=None, prompt_len=N
         keep.append(ctx.array(np.ascontiguousarray(values, dtype)))
         return keep[-1].ptr
 
+    def tokens(values):  # (what 32 bits do not hold is no token either)
+        a = np.asarray(values).astype(np.int64)
+        return np.where(a == a.astype(np.int32), a, -1)
+
     each = lambda v, t: put(np.broadcast_to(np.asarray(v, t), (rows,)), t)
     if history is not None:
         if len(history) != rows:
@@ -911,7 +915,7 @@ def adjust_logits(ctx: "Context", logits: np.ndarray, history=None, prompt_len=N
         held = [len(h) for h in history]
         table = np.zeros((rows, max(held + [1])), np.int32)
         for r, h in enumerate(history):
-            table[r, :held[r]] = h
+            table[r, :held[r]] = tokens(h)
         rules.history, rules.history_stride = put(table, np.int32), table.shape[1]
         rules.history_len = put(held, np.int32)
         rules.prompt_len = None if prompt_len is None else each(prompt_len, np.int32)
@@ -923,7 +927,7 @@ def adjust_logits(ctx: "Context", logits: np.ndarray, history=None, prompt_len=N
         rules.biases = sum(len(t) for t, _ in bias)
         rules.bias_start = put(np.cumsum([0] + [len(t) for t, _ in bias]), np.int32)
         # (one more of each: a list may be empty, an array may not)
-        rules.bias_token = put(np.concatenate([t for t, _ in bias] + [[0]]), np.int32)
+        rules.bias_token = put(tokens(np.concatenate([t for t, _ in bias] + [[0]])), np.int32)
         rules.bias = put(np.concatenate([v for _, v in bias] + [[0]]), np.float32)
     if masks is not None:
         masks = np.asarray(masks, bool)

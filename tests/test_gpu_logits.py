@@ -156,3 +156,14 @@ def test_with_the_sampler(gpu_ctx, hyq):
     for i in range(4):
         want = R.sample(y[i], [0.7, 0.7, 0, 0][i], 0, 1.0, 0.0, 0.5)
         assert (token[i], pytest.approx(prob[i], abs=1e-6)) == want
+
+
+def test_tokens_beyond_32_bits(gpu_ctx, hyq):
+    """Tokens of 64 bits are passed over, not cut to others of the vocabulary."""
+    x = np.arange(1, 17, dtype=np.float32).reshape(2, 8)
+    far = [np.array([(1 << 32) + 5, 2]), [(1 << 40) + 1, -(1 << 32) + 3]]
+    got = hyq.adjust_logits(gpu_ctx, x, history=far, repetition=2.0,
+                            bias=[(far[0], [100.0, 1.0]), (far[1], [100.0, 100.0])])
+    want = x.copy()
+    want[0, 2] = want[0, 2] / 2 + 1
+    assert np.array_equal(got, want)
