@@ -855,6 +855,8 @@ class PagedCache:
         of heads has one buffer, which a captured graph keeps and the next plan takes,
         a replayed graph's too: capture attention with its share_d, and after a replay
         call share_d again before attention outside the graph."""
+        if least is not None and least < 0:
+            raise ValueError("least is a number of positions times KV heads, or None")
         need = lib().hyq_paged_shared_plan_bytes(self._kl, rows, heads)
         plan = self._grown(self._plans.setdefault(heads, []), need)
         args = [self.ctx.handle, self._kl, group_d, self.table.ptr, self._rows_len.ptr, start_d,

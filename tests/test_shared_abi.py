@@ -66,3 +66,10 @@ def test_refusals(hyq, dtype):
         assert L.hyq_paged_shared_plan_bytes(k, rows, heads) == 0
         assert L.hyq_paged_shared_attention_scratch_bytes(k, rows, 1, heads) == 0
     assert L.hyq_paged_shared_attention_scratch_bytes(k, 5, 0, 16) == 0
+
+
+def test_python_refuses_a_negative_least(hyq):
+    """(As a size it would be the largest there is, and nothing be shared.)"""
+    cache = hyq.PagedCache.__new__(hyq.PagedCache)
+    with pytest.raises(ValueError, match="least"):
+        cache.share_d(0, 4, 16, least=-1)
