@@ -21,8 +21,11 @@
 //
 //   s = max |x| / 127 (rounded to 32 bits), codes c = rint(x / s), x ~ s c,
 //
-// off by at most s / 2; one number that is not finite makes s a NaN, and with it
-// the whole head. Keys are formed and divided in 64 bits: a code is the same on
+// off by at most s / 2, and by 127 2^-150 more where max |x| < 127 2^-126, whose scale
+// is no normal number: its codes are cut to 127, and at 127 2^-150 it is zero. (Of
+// numbers at the end of f32's range s is the f32 below, if 127 of it would be
+// infinite.) One number that is not finite makes s a NaN, and with it the whole
+// head. Keys are formed and divided in 64 bits: a code is the same on
 // every run and in every order of summation but where x / s lies within 2^-40 of
 // a half, which f32 would make one in 2^15. 2367 rows of 32 + 2 * 8 heads move 89 MB
 // in 26 us, bound by the norms, rotations and divisions in 64 bits; 48 rows of 16 + 2 *
@@ -238,6 +241,8 @@ __device__ __forceinline__ void store_codes(unsigned char *row, float *scale, co
         fine = __shfl_xor((int)fine, o, 16) && fine;
     }
     float s = (float)(top / 127.);
+    if (top <= 3.4028234663852886e38 && 127.f * s == INFINITY)
+        s = __builtin_bit_cast(float, __builtin_bit_cast(int, s) - 1);
     const double inv = s > 0.f ? 1. / (double)s : 0.;
     if (!fine || !(s < INFINITY)) s = __builtin_nanf("");
     auto word = [&](const double (&x)[4]) {

@@ -396,8 +396,11 @@ size_t hyq_kv_pool_bytes(const hyq_kv_layout *kl);
  * that two slots name, either stays: hyq_pages_extend_d gives each its own). An
  * F16 pool holds the values rounded once, to nearest. An HYQ_KV_Q8 pool holds the
  * 128 numbers x of a position and head as scale = max |x| / 127 in f32 and codes
- * rint(x / scale), off by at most half a scale; one that is not finite makes the
- * scale, and with it the head, a NaN. Such keys are formed in 64 bits. The angle
+ * rint(x / scale), off by at most half a scale, and by 127 * 2^-150 more where
+ * max |x| is below 127 * 2^-126 (its scale is no normal number, its codes are cut to
+ * 127; at 127 * 2^-150 the scale and with it the head is zero). The scale is the f32
+ * below where 127 of it would be infinite. A number that is not finite makes
+ * the scale, and with it the head, a NaN. Such keys are formed in 64 bits. The angle
  * position * freq_d[j] is taken in 64 bits, where hyq_rope_norm_append_d rounds the
  * product to 32 (the reference's table, src/model.rs:919-925): the two differ by
  * up to position * 2^-24 radians times the frequency, and agree where the product

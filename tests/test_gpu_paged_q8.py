@@ -327,6 +327,33 @@ def test_append_of_halves_and_extremes(gpu_ctx, hyq):
     assert list(want[4, :3]) == [127, 0, 2]
 
 
+def test_read_back_at_the_ends_of_the_range(gpu_ctx, hyq):
+    """Half a scale from what was written, and 127 * 2^-150 more where the scale is no
+    normal number; never infinite. (A code's product with the scale is rounded once.)"""
+    top, step = float(np.finfo(np.float32).max), 2.0 ** -149
+    heads = [top, top * (1 - 2.0 ** -24), top * (1 - 2.0 ** -22), 127 * 2.0 ** -126,
+             126 * 2.0 ** -126, 178 * step, 190 * step, 127 * step, 64 * step, 63 * step, step]
+    n = len(heads)
+    b = Q.BatchQ8([n], [n], 2, 1, 16, seed=26)
+    v = np.array(heads)[:, None] * np.linspace(-1, 1, D)
+    v = v.astype(np.float32).reshape(n, 1, D)
+    one, freq = np.ones(D, np.float32), np.zeros(64, np.float32)
+    _, pool = append(hyq, gpu_ctx, b, b.bytes, np.ones((n, 1, D), np.float32), v, one, one, freq,
+                     1e-5, 0)
+    scales = Q.split(pool, 1, 16)[1][b.table[0, 0], 1, 0, :n].astype(np.float64)
+    kl = layout(hyq, b)
+    d = [gpu_ctx.array(x) for x in (pool, b.table, b.lens, b.start)]
+    k, got = (gpu_ctx.array(np.full((n, 1, D), -7, np.float32)) for _ in range(2))
+    hyq.check(hyq.lib().hyq_paged_read_d(gpu_ctx.handle, ctypes.byref(kl), d[0].ptr, 0, d[1].ptr,
+                                         d[2].ptr, d[3].ptr, n, k.ptr, got.ptr))
+    got = got.numpy()[:, 0].astype(np.float64)
+    assert np.isfinite(got).all()
+    most = np.abs(v[:, 0].astype(np.float64)).max(-1)
+    bound = scales / 2 + np.where(most < 127 * 2.0 ** -126, 127 * 2.0 ** -150, 0)
+    err = np.abs(got - v[:, 0])
+    assert np.all(err <= (bound + most * R.U)[:, None]), (err.max(-1) / bound)
+
+
 DTYPES = ["F32", "F16", "Q8"]
 
 
