@@ -217,6 +217,23 @@ def alike(b, seqs, pages, seed):
 MOST_NARROW = {"F32": (6500, 16), "F16": (3500, 16), "Q8": (8192, 32)}
 
 
+@pytest.mark.parametrize("over", [0, 1], ids=["narrow", "wide"])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,seqs", [((16, 4), 32), ((6, 2), 45)], ids=str)
+def test_the_border_of_narrow_blocks(gpu_ctx, hyq, heads, seqs, kind, over):
+    """As many tiles as blocks of 16 rows may have, and a page's more: either form's
+    results."""
+    most, tile = MOST_NARROW[kind]
+    blocks = -(-seqs // (16 // (heads[0] // heads[1])))
+    pages = most // (blocks * heads[1]) + over
+    b = alike(batch(kind, [pages * tile + 30], [1], heads, tile, seed=27), seqs, pages, seed=28)
+    c = Call(hyq, gpu_ctx, b).make()
+    assert np.all(c.skips() == pages * tile)
+    head = c.plan.numpy()[:16].view(np.int32)
+    assert head[3] == 1 - over and (over or head[0] == blocks)
+    check(b, c.attend())
+
+
 @pytest.mark.parametrize("case", ["equal", "jump"])
 @pytest.mark.parametrize("over", [0, 1], ids=["narrow", "wide"])
 def test_far_values_in_a_prefix(gpu_ctx, hyq, over, case):
