@@ -427,7 +427,8 @@ int hyq_paged_read_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, 
  * (those products split them into two f16 parts: 22 bits of numbers from 2^-14
  * up, 2^-36 absolutely below). A value beyond it there, and one that is not
  * finite in any form, makes its dim of the rows that see it not finite (such a
- * key the whole of those rows), and changes no other row. An HYQ_KV_Q8 pool has
+ * key the whole of those rows, but that an infinite one whose score is minus
+ * infinity may also count as nothing), and changes no other row. An HYQ_KV_Q8 pool has
  * no such limit: its codes enter the products exactly, queries to 22 bits of the
  * row's largest, values to 2^-31 of the largest that the row sees (each) or of
  * 2^-81, the larger. What places hold that no position uses (a page's rest, pages
@@ -468,7 +469,11 @@ int hyq_paged_shared_plan_least_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const i
                                   const int32_t *start_d, size_t rows, size_t heads, size_t least,
                                   void *plan_d, size_t plan_bytes);
 /* hyq_paged_attention_d by a plan; its arguments, limits and refusals. The keys and
- * values of an F32 pool must lie within the f16 range in a shared prefix too.
+ * values of an F32 pool must lie within the f16 range in a shared prefix too: where
+ * the plan's prefixes are long for many slots (6,500 steps of 16 positions over all
+ * blocks of 16 rows and KV heads) they go through the two f16 parts, 22 bits, that
+ * slots of many new rows do, and in shorter ones they enter the products as they
+ * are. So the same slot's result may differ by that rounding with the batch.
  * scratch_d: hyq_paged_shared_attention_scratch_bytes bytes. */
 size_t hyq_paged_shared_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows,
                                                 size_t max_rows, size_t heads);

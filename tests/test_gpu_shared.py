@@ -234,6 +234,96 @@ def test_the_border_of_narrow_blocks(gpu_ctx, hyq, heads, seqs, kind, over):
     check(b, c.attend())
 
 
+def not_finite(kind, b, where, value):
+    """Puts `value` into keys or values (where[1]) of a page's place and head: number 7,
+    of an 8-bit page the scale (a NaN, whatever the value)."""
+    page, x, h, place = where
+    if kind == "Q8":
+        b.scales[page, x, h, place] = np.nan
+        b.bytes = Q.join(b.codes, b.scales)
+    else:
+        b.pool[page, x, h, place, 7] = value
+
+
+def without(b, where):
+    """The 64-bit form over all positions but that of a place."""
+    seen = b.kv
+
+    def kv(s, h):
+        k, v, ok = seen(s, h)
+        at = np.flatnonzero(b.table[s] == where[0])
+        for page in at:
+            p = page * b.pt + where[3]
+            if p < len(ok):
+                ok = ok.copy()
+                ok[p] = False
+        return k, v, ok
+
+    b.kv = kv
+    try:
+        return b.attention()
+    finally:
+        del b.kv
+
+
+@pytest.mark.parametrize("form", ["narrow", "wide"])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pt", [16, 64])
+def test_numbers_of_a_prefix_that_are_not_finite(gpu_ctx, hyq, pt, kind, form):
+    """In the common pages of one of two groups, in whole steps and in a last step of
+    which the prefix has a part, in narrow and in wide blocks: keys reach their head's
+    whole rows of that group, values one dim of them, and no other number changes. A
+    value that f32 holds and f16 does not is finite in narrow blocks and no number in
+    wide ones. An infinite key's score may be minus infinity, its weight exp(-inf) = 0:
+    such a row may also be as if the position were not there."""
+    seqs, rep, kvh = 24, 8, 2  # (narrow blocks of two slots)
+    pages = (5 if pt == 16 else 3) if form == "narrow" else (
+        MOST_NARROW[kind][0] // (2 * 6) * MOST_NARROW[kind][1] // pt + 1)
+    pages += pt == 16 and pages % 4 == 0  # (the last step of 64 positions in part)
+    b = batch(kind, [pages * pt + 30] * 2, [1] * 2, (rep * kvh, kvh), pt, seed=29)
+    table, half = b.table.copy(), seqs // 2
+    b = alike(b, seqs, pages, seed=30)
+    b.table = np.concatenate([np.repeat(table[:1], half, 0), np.repeat(table[1:], half, 0)])
+
+    def attend():
+        c = Call(hyq, gpu_ctx, b).make()
+        assert np.all(c.skips() == pages * pt)
+        assert c.plan.numpy()[:16].view(np.int32)[3] == (form == "narrow")
+        return c.attend()
+
+    clean = attend()
+    n = pages * pt
+    values = [np.nan] if kind == "Q8" else [np.inf, np.nan] + [1e5] * (kind == "F32")
+    for value in values:
+        for at in (3, n - 2):
+            for x in (0, 1):
+                where = (table[0, at // pt], x, 1, at % pt)
+                kept = b.scales.copy() if kind == "Q8" else b.pool[where].copy()
+                not_finite(kind, b, where, value)
+                got = attend()
+                if kind == "Q8":
+                    b.scales = kept
+                    b.bytes = Q.join(b.codes, b.scales)
+                else:
+                    b.pool[where] = kept
+                bad = np.zeros(got.shape, bool)
+                bad[:half, rep:] = True
+                if x and kind != "Q8":
+                    bad[..., :7] = bad[..., 8:] = False
+                none = np.zeros(got.shape[:2], bool)
+                if x == 0 and value == np.inf:
+                    none = bad.all(-1) & np.isfinite(got).all(-1)
+                    assert np.all(b.q[..., 7][none] < 0), (value, at)
+                if none.any():
+                    want, tol = without(b, where)
+                    assert np.all(np.abs(got - want).max(-1)[none] <= tol[none]), (value, at)
+                if value == 1e5 and form == "narrow":
+                    assert np.isfinite(got).all()
+                else:
+                    assert not np.isfinite(got[bad & ~none[..., None]]).any(), (value, at, x)
+                assert np.array_equal(got[~bad], clean[~bad]), (value, at, x)
+
+
 @pytest.mark.parametrize("case", ["equal", "jump"])
 @pytest.mark.parametrize("over", [0, 1], ids=["narrow", "wide"])
 def test_far_values_in_a_prefix(gpu_ctx, hyq, over, case):
