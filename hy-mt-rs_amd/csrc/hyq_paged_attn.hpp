@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "hyq_paged.hpp"
+#include "hyq_paged_pieces.hpp"
 #include "hyq_wave.hpp"
 
 namespace hyq {
@@ -193,12 +194,6 @@ constexpr int PR_MIN_TILES = 2;     // the shortest piece worth its partial rows
 struct Block {
     int row, toks;    // its first packed row and its tokens
     int part, pieces; // its first partial block and its pieces
-};
-// A range of steps of a block, with what its workgroup needs to begin.
-struct Piece {
-    int slot, index, t0, t1;
-    int part;            // the partial block it writes, -1 for the output
-    int begin, n, first; // the slot's rows, and the first one's position
 };
 struct Plan {
     int blocks, groups;
@@ -445,21 +440,6 @@ inline int few_most(int seqs, int kvh)
     constexpr int LOT = 256 * FEW_WAVES; // (whole ones: a workgroup on each CU)
     return (FEW_PIECES + (seqs + shared_cap(seqs)) * kvh + LOT - 1) / LOT * LOT;
 }
-struct SharedPlace {
-    int begin, n;     // the slot's rows (n = 0: not of the few-row form)
-    int part, pieces; // of its block (0 pieces: in no group); narrow: the block's first
-                      // worker and its workers for each KV head
-    int row;          // the slot's first row there
-    int first, ways;  // its first worker, and its workers for each KV head
-    int unused;
-};
-struct FewPiece {
-    int slot, kh, t0, t1;      // tiles of the slot's positions from skip on
-    int begin, n, len, skip;   // the slot's rows and positions
-    int ways;                  // pieces of the slot
-    int narrow;                // a block: n places of the list from begin on, len positions
-    int unused[2];
-};
 struct SharedHead {
     Plan plan;   // blocks, their pieces (as groups)
     int workers; // of the few-row form, a piece each
@@ -475,6 +455,10 @@ struct SharedPlan {
     int *list;          // [cap * tq] packed rows, -1 where none
     Piece *pieces;      // [most]
     int tq, cap, most, few_most;
+    __device__ __forceinline__ PlanSizes sizes(const PagedKv &kv) const
+    {
+        return PlanSizes{kv.seqs, kv.kvh, kv.rows, kv.stride, kv.shift, tq, cap, most, few_most};
+    }
 };
 struct SharedLayout {
     size_t ints, place, few, list, pieces, bytes;
@@ -519,24 +503,11 @@ inline size_t shared_parts_bytes(int seqs, int kvh, int heads)
 {
     return (size_t)shared_layout(seqs, kvh, heads).most * kvh * PR_ROWS * PAGED_PART * 4;
 }
-// A worker's piece, cut to what there is: the plan may be of another batch.
+// A worker's piece, cut to what there is.
 template <int TILE>
 __device__ __forceinline__ FewPiece few_piece(const PagedKv &kv, const SharedPlan &sp, int w)
 {
-    FewPiece f = sp.few[w];
-    f.slot = min(max(f.slot, 0), kv.seqs - 1);
-    f.kh = min(max(f.kh, 0), kv.kvh - 1);
-    // (begin: a row there is, read whatever n)
-    const int places = f.narrow ? sp.cap * sp.tq : kv.rows;
-    f.begin = min(max(f.begin, 0), places - 1);
-    f.n = min(max(f.n, 0), places - f.begin);
-    if (f.narrow) f.n = min(f.n, sp.tq / 8);
-    f.len = (int)min((long long)max(f.len, 0), (long long)kv.stride << kv.shift);
-    f.skip = min(max(f.skip, 0), f.len) & ~15;
-    const int tiles = (f.len - f.skip + TILE - 1) / TILE;
-    f.t0 = min(max(f.t0, 0), max(tiles - 1, 0));
-    f.t1 = min(max(f.t1, f.t0 + 1), max(tiles, 1));
-    return f;
+    return cut_few_piece(sp.sizes(kv), TILE, sp.few[w]);
 }
 
 // hyq_paged_few.hip: slots of at most `few` <= paged_few_rows(heads / kv_heads)

@@ -545,18 +545,10 @@ __device__ __forceinline__ void merge_few(const PagedKv &kv, int few_rows, int p
     bool narrow = false;
     int w0, n;
     if constexpr (SHARED) {
-        pl = sp.place[s];
-        sr.begin = min(max(pl.begin, 0), kv.rows);
-        sr.n = min(max(pl.n, 0), kv.rows - sr.begin);
         narrow = sp.head->narrow != 0;
-        const int most = narrow ? sp.few_most : sp.most;
-        pl.part = min(max(pl.part, 0), most - 1);
-        pl.pieces = min(max(pl.pieces, 0), most - pl.part);
-        if (narrow) pl.part = (int)min((long long)pl.part + (long long)kh * pl.pieces,
-                                       (long long)(most - pl.pieces));
-        n = min(max(pl.ways, 0), sp.few_most);
-        w0 = (int)min((long long)max(pl.first, 0) + (long long)kh * n, (long long)sp.few_most);
-        n = min(n, sp.few_most - w0);
+        pl = cut_place(sp.sizes(kv), kh, narrow, sp.place[s]);
+        sr.begin = pl.begin, sr.n = pl.n;
+        w0 = pl.first, n = pl.ways;
     } else {
         const int2 by = shared[(size_t)s * kv.kvh + kh]; // (of a slot without rows: anything)
         sr = slot_rows(kv, s);

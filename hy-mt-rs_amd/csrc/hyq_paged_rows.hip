@@ -250,11 +250,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
         if (at_piece > from) __syncthreads(); // the last piece's readers of LDS are done
         Piece piece = rs.pieces[at_piece];
         if constexpr (PREFIX) {
-            piece.slot = min(max(piece.slot, 0), kv.seqs - 1);
-            piece.index = min(max(piece.index, 0), rs.cap - 1);
-            piece.part = min(max(piece.part, 0), rs.most - 1);
-            piece.first = (int)min((long long)max(piece.first, 0), (long long)kv.stride << kv.shift);
-            piece.t0 = min(max(piece.t0, 0), piece.first / PR_TILE);
+            const PlanSizes z{kv.seqs, kv.kvh, kv.rows, kv.stride, kv.shift, rs.tq, rs.cap, rs.most, 0};
+            piece = cut_piece(z, PR_TILE, piece);
         }
         const int s = piece.slot, tq = rs.tq;
         const int t = threadIdx.x, lane = t & 63, h = lane >> 5, c = lane & 31;

@@ -516,6 +516,57 @@ def test_a_plan_of_another_batch(gpu_ctx, hyq):
         c.attend()
 
 
+class Guarded:
+    """A buffer between two others that are to stay as they are."""
+    ROOM = 1 << 16
+
+    def __init__(self, ctx, nbytes):
+        self.whole = ctx.array(np.full(nbytes + 2 * self.ROOM, 0xA5, np.uint8))
+        self.ptr = self.whole.ptr + self.ROOM
+
+    def intact(self):
+        a = self.whole.numpy()
+        return np.all(a[:self.ROOM] == 0xA5) and np.all(a[-self.ROOM:] == 0xA5)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,pt", [((8, 2), 32), ((6, 2), 64), ((16, 1), 16)], ids=str)
+def test_plans_of_any_bytes(gpu_ctx, hyq, heads, pt, kind):
+    """A batch's plan with some numbers exchanged, and plans of small numbers and of any
+    bytes: nothing beside the scratch and the output is written, and no input."""
+    few = 16 // (heads[0] // heads[1])
+    b = batch(kind, [9 * pt + 3] * 6, [min(2, few)] * 6, heads, pt, seed=31, tail=3)
+    share(b, [0, 1, 2, 4, 5], 8)
+    c = Call(hyq, gpu_ctx, b)
+    out = Guarded(gpu_ctx, b.rows * b.heads * D * 4)
+    c.scratch, c.out, plan = Guarded(gpu_ctx, c.ns), out, Guarded(gpu_ctx, c.np)
+    c.plan = plan
+    c.make()
+    held = {n: a.numpy() for n, a in c.d.items()}
+    true = plan.whole.numpy()[plan.ROOM:-plan.ROOM].copy()
+    r = np.random.default_rng(32)
+    for i in range(24):
+        junk = true.copy()
+        words = junk[:junk.size // 4 * 4].view(np.int32)
+        if i % 3 == 0:  # (an eighth of the numbers another one)
+            at = r.random(words.size) < 0.125
+            words[at] = r.integers(-3, 300, at.sum())
+        elif i % 3 == 1:
+            words[:] = r.integers(-3, 40, words.size)
+        else:
+            junk[:] = r.integers(0, 256, junk.size)
+        words[:2] = r.integers(1, 12, 2)  # blocks, pieces
+        words[2:4] = [r.integers(1, 3000), i // 3 % 2]  # workers, narrow
+        given = np.concatenate([np.full(plan.ROOM, 0xA5, np.uint8), junk,
+                                np.full(plan.ROOM, 0xA5, np.uint8)])
+        plan.whole.copy_from(given)
+        c.enqueue()
+        assert c.scratch.intact() and out.intact(), i
+        assert np.array_equal(plan.whole.numpy(), given), i
+    for n, a in c.d.items():
+        assert np.array_equal(a.numpy().view(np.uint8), held[n].view(np.uint8)), n
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_cache(gpu_ctx, hyq, kind):
     """PagedCache: forked slots attend with and without the plan alike; a plan is
