@@ -278,7 +278,9 @@ int hyq_paged_shared_plan_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const int32_t
     // group of slots before 600 to 6000 common positions and some 60 of their own, 16
     // heads over 4, us a layer, shared and not: 8-bit pages 12.8 and 12.4 at 16,800, 13.8
     // and 14.5 at 42,000, 14.9 and 16.2 at 60,000; f16 13.5 and 13.4, 16.9 and 18.4, 17.1
-    // and 19.0; f32 13.3 and 13.9, 17.0 and 17.0, 17.0 and 19.3.
+    // and 19.0; f32 13.3 and 13.9, 17.0 and 17.0, 17.0 and 19.3. (The plan, 15 us a step,
+    // is spent before it is known, and pays over the layers or not: four layers of the
+    // f32 pages at 42,000 take 76 us with it and 70 without.)
     constexpr long long least = 25000;
     return shared_plan(ctx, kl, group_d, table_d, len_d, start_d, rows, heads, least, plan_d,
                        plan_bytes);

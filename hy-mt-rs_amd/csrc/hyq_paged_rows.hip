@@ -42,7 +42,7 @@
 // plan 6, this launch 37 (eight steps, and 13 us to begin and end: cold code and
 // loads that wait for each other), the merge 5. The same over 8-bit pages: this
 // launch 31. Three prompts of up to 400 beside 27 sessions of up to 4000 positions,
-// 32 heads over 8: 114 us over 8-bit pages, of which MFMAs are 30 % and VALU work
+// 32 heads over 8: 115 us over 8-bit pages, of which MFMAs are 30 % and VALU work
 // 35 % (106 over f16 ones: the codes' conversion and the scales are the difference;
 // scores by products of whole numbers would save the keys' conversion and take as
 // much for the queries' third part). A prefix of 8192 positions for 64 slots of four

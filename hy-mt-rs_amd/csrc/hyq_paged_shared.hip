@@ -9,9 +9,12 @@
 // slot's place follows from the slots before it, so the plan does not depend on
 // the order in which threads run.
 //
-// Bound by loads that wait for each other and by barriers: 15 us for eight slots, 19 for
-// 64, 20 for 105, once a step, not a layer. A layer of 64 slots over 8200 positions in
-// common and 300 of their own, 32 heads over 8, f16 pages: 51 us.
+// Bound by loads that wait for each other and by barriers (the waves of the first launch
+// wait 90 % of their cycles, of the second 71): 14 us for eight slots, 18 for 64, 19 for
+// 105, 24 for 256, once a step, not a layer. Then by the counts, which compare each
+// slot's key with those of all slots, in every workgroup: 37 us for 512, 91 for 1024,
+// 1040 for 4096. A layer of 64 slots over 8200 positions in common and 300 of their own,
+// 32 heads over 8, f16 pages: 51 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -181,7 +184,8 @@ constexpr int PLAN_GROUPS = 8;
 // a layer, 16 heads over 4 and 32 over 8: f16 pages at 3008 tiles 22.0 and 24.9, at 4000
 // 27.7 and 26.3, at 8064 33.2 and 30.9; f32 ones at 4000 24.0 and 28.8, 6016 27.4 and
 // 29.6, 8032 31.5 and 31.6, 16000 55.9 and 38.2; 8-bit ones at 4096 26.7 and 29.1, 8064
-// 32.4 and 32.6, 16000 41.7 and 38.1.
+// 32.4 and 32.6, 16000 41.7 and 38.1. (f32's limit lies before its crossing, at some 8000:
+// between them wide blocks take up to 2 us more.)
 __device__ __forceinline__ int most_narrow_tiles(int type)
 {
     return type == KV_T_Q8 ? 8192 : type == KV_T_F16 ? 3500 : 6500;
@@ -262,6 +266,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
             atomicAdd(&sum[5], (unsigned)mine);
         }
     __syncthreads();
+    // (and where they are no more than there is room for: blocks of one slot each, as with
+    // nine query heads or more to a KV head, may be)
     const int most_narrow = most_narrow_tiles(kv.type);
     const bool narrow = (long long)sum[4] * kv.kvh <= most_narrow && (int)sum[5] <= sp.cap;
     const int tq = narrow ? few : sp.tq;
@@ -361,11 +367,13 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(PagedKv kv, int few,
     const unsigned units = sum[2] + (narrow ? sum[5] : 0);
     const unsigned all_tiles = sum[1] + (narrow ? sum[4] : 0);
     const int spread = kv.type == KV_T_F32 ? head : max(head - (int)units, head * 11 / 16);
-    // (The merge waits for a row's parts: where blocks are narrow, pieces are no shorter
-    // than about the root of a 24th of the longest one's tiles. Eight slots over 600, 1500
-    // and 3000 positions in common, 16 heads over 4, us a layer with pieces of 1, 2, 3, 4
+    // (The merge waits for a row's parts: where blocks are narrow, pieces grow with the
+    // longest block's tiles, up to four. Eight slots over 600, 1500 and 3000 positions in
+    // common, 38, 94 and 188 tiles, 16 heads over 4, us a layer with pieces of 1, 2, 3, 4
     // and 6 tiles at least: f16 pages 14.1 13.5 14.7 16.4 18.3, 18.2 16.1 16.9 17.2 18.0,
-    // 27.1 21.0 19.3 19.0 20.5; 32 slots over 1000 23.3 23.1 19.9 19.9 21.8.)
+    // 27.1 21.0 19.3 19.0 20.5; 32 slots over 1000, 63 tiles, 23.3 23.1 19.9 19.9 21.8. Of
+    // few blocks with 49 to 128 tiles two would be the better: the 94 tiles in f32 pages
+    // take 15.6 with two and 17.0 with three.)
     int least = 1;
     if (narrow) {
         int longest = 0;

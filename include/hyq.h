@@ -470,10 +470,11 @@ int hyq_paged_shared_plan_least_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const i
                                   void *plan_d, size_t plan_bytes);
 /* hyq_paged_attention_d by a plan; its arguments, limits and refusals. The keys and
  * values of an F32 pool must lie within the f16 range in a shared prefix too: where
- * the plan's prefixes are long for many slots (6,500 steps of 16 positions over all
- * blocks of 16 rows and KV heads) they go through the two f16 parts, 22 bits, that
- * slots of many new rows do, and in shorter ones they enter the products as they
- * are. So the same slot's result may differ by that rounding with the batch.
+ * the plan's prefixes are long for many slots (over 6,500 steps of 16 positions over
+ * all blocks of 16 rows and KV heads, or more blocks than 5 / 8 of the table's slots)
+ * they go through the two f16 parts, 22 bits, that slots of many new rows do, and
+ * elsewhere they enter the products as they are. So the same slot's result may differ
+ * by that rounding with the batch.
  * scratch_d: hyq_paged_shared_attention_scratch_bytes bytes. */
 size_t hyq_paged_shared_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows,
                                                 size_t max_rows, size_t heads);
