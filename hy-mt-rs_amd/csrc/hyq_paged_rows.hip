@@ -505,7 +505,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             }
             load(p0 + 2 * PR_TILE, after);
             if constexpr (LO) sv += sx * (1.f / LO_SCALE);
-            // the scales of the lane's positions
+            // the scales of the lane's positions (a key's with the query's, then a score:
+            // a key's with a sum of codes' products may pass f32's range)
             f32x16 bs;
             if constexpr (Q8) {
 #pragma unroll
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
                     const f32x4 y = *reinterpret_cast<const f32x4 *>(&l.scale[1][o + 8 * a + 4 * h]);
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
-                        sv[4 * a + b] *= x[b];
+                        sv[4 * a + b] *= x[b] * qscale;
                         bs[4 * a + b] = y[b];
                     }
                 }
@@ -538,7 +539,8 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             // below the maximum, so that weights go up to 2^15: their f16 parts
             // resolve 2^-25, which is 2^-32 of the first weight. (Many equal small
             // weights are rounded the same way, and their errors add up.)
-            const float m_new = fmaf(wave::max_halves(tmax), qscale, -7.f);
+            const float post = Q8 ? 1.f : qscale;
+            const float m_new = fmaf(wave::max_halves(tmax), post, -7.f);
             float most = 0.f;
             if constexpr (Q8) most = l.most[part_of];
             if (__any(m_new > m_run + 8.f || (Q8 && most > top))) {
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(PR_THREADS, 2) void paged_rows_kernel(
             float rs[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                sv[e] = __builtin_amdgcn_exp2f(fmaf(sv[e], qscale, -base));
+                sv[e] = __builtin_amdgcn_exp2f(fmaf(sv[e], post, -base));
                 rs[e & 1] += sv[e];
             }
             l_run += rs[0] + rs[1];

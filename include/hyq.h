@@ -430,8 +430,8 @@ int hyq_paged_read_d(hyq_ctx *ctx, const hyq_kv_layout *kl, const void *pool_d, 
  * key the whole of those rows, but that an infinite one whose score is minus
  * infinity may also count as nothing), and changes no other row. An HYQ_KV_Q8 pool has
  * no such limit: its codes enter the products exactly, queries to 22 bits of the
- * row's largest, values to 2^-31 of the largest that the row sees (each) or of
- * 2^-81, the larger. What places hold that no position uses (a page's rest, pages
+ * row's largest or of 2^-100, the larger, values to 2^-31 of the largest that the row
+ * sees (each) or of 2^-81, the larger. What places hold that no position uses (a page's rest, pages
  * never written) is never part of a result. out_d must not be q_d. scratch_d:
  * hyq_paged_attention_scratch_bytes bytes (0 for arguments that the call refuses). */
 size_t hyq_paged_attention_scratch_bytes(const hyq_kv_layout *kl, size_t rows, size_t max_rows,

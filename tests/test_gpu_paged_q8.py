@@ -159,6 +159,27 @@ def test_values_at_the_ends_of_the_range(gpu_ctx, hyq, news, case):
     check(b, attention(hyq, gpu_ctx, b))
 
 
+@pytest.mark.parametrize("news", [2, 40])
+def test_far_keys_of_small_queries(gpu_ctx, hyq, news):
+    """Keys of 2^116 and queries of 2^-100: scores of +-5000, so that one position has all
+    the weight (the others' is 2^-14426 of it, zero) and its values are the result, to the
+    roundings of their product with the scale, of the weight's two parts and of the
+    normalisation."""
+    b = Q.BatchQ8([150, 77], [news] * 2, 4, 2, 32, seed=16)
+    b.codes[:, 0, ..., 1:] = 0
+    b.codes[:, 0, ..., 0] = -127
+    with np.errstate(invalid="ignore"):
+        b.scales[:, 0] = np.where(np.isnan(b.scales[:, 0]), np.nan,
+                                  np.float32(5000 * np.sqrt(D) / 127 * 2.0 ** 100))
+    b.q[:], b.q[..., 0] = 0, np.float32(2.0 ** -100)
+    for s, at in enumerate((37, 20)):
+        b.codes[b.table[s, at // 32], 0, :, at % 32, 0] = 127
+    b.bytes = Q.join(b.codes, b.scales)
+    got, (want, _) = attention(hyq, gpu_ctx, b), b.attention()
+    big = np.abs(want).max(-1, keepdims=True)
+    assert np.all(np.abs(got - want) <= big * (8 * R.U + 2.0 ** -22))
+
+
 @pytest.mark.parametrize("case", ["small", "jump"])
 @pytest.mark.parametrize("news", [1, 40])
 def test_far_values_in_one_piece(gpu_ctx, hyq, news, case):
